@@ -599,6 +599,87 @@ int kvca_move_cycle(const kvca_chunk_desc* tokens, const kvca_paged_desc* token_
                     int64_t num_seqs, int64_t spill_rows, int32_t flags, void* d_scratch, int64_t* d_status,
                     kvca_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Attention over the paged cache                                            */
+/* ------------------------------------------------------------------------ */
+
+/* Element types of a query or a cache. */
+#define KVCA_TYPE_F16 0
+#define KVCA_TYPE_BF16 1
+#define KVCA_TYPE_E4M3 2 /* cache only; one factor each for keys and values */
+
+/*
+ * A batch of sequences over one layer's paged K and V.  Token t of sequence s
+ * lives in block b = block_tables[s * table_stride + t / block_size] at
+ *   key + b * key_block_stride + (t % block_size) * key_token_stride
+ *       + head * key_head_stride
+ * (bytes; head_dim elements in a row; V alike), so any order of block, token
+ * and head dims does, K and V of one merged block too.  Addresses and strides
+ * are multiples of 16 bytes, head_dim a multiple of 8 (of 16 with e4m3), at
+ * most 256.  q_heads is a multiple of kv_heads: query head h reads K/V head
+ * h / (q_heads / kv_heads).  An e4m3 value stands for itself times key_scale
+ * (value_scale); both are 1 otherwise.
+ *
+ * A query at position p of its sequence sees the tokens
+ *   j <= p  with  window == 0, or j > p - window, or j < sinks,
+ * and gets  sum_j softmax_j(scale * q . k_j) v_j  over them.  What the cache
+ * holds at tokens that no query of the call sees is never part of a result,
+ * and page table entries of blocks without a seen token are not read (pages
+ * behind the window may have been given back).  seq_lens[s]: the tokens of
+ * sequence s, the new ones among them (their K and V are in the cache);
+ * 0: none; negative: an idle row, whose outputs are left as they were.
+ * A length above table_width * block_size or a block outside [0, num_blocks)
+ * gives KVCA_ERR_BAD_INDEX; that sequence's outputs then hold no defined
+ * values.  table_width * block_size is at most 2^30.
+ */
+typedef struct kvca_attend_desc {
+  uint64_t key;
+  uint64_t value;
+  int64_t key_block_stride;
+  int64_t key_token_stride;
+  int64_t key_head_stride;
+  int64_t value_block_stride;
+  int64_t value_token_stride;
+  int64_t value_head_stride;
+  int64_t num_blocks;
+  int64_t block_size;
+  const int64_t* block_tables;
+  int64_t table_stride;
+  int64_t table_width;
+  const int64_t* seq_lens;
+  int64_t num_seqs;
+  int32_t q_heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t query_type;
+  int32_t cache_type; /* the query's, or KVCA_TYPE_E4M3 */
+  float scale;
+  float key_scale;
+  float value_scale;
+  int64_t window; /* 0: none */
+  int64_t sinks;
+  uint64_t query;           /* row r, head h: query + r * query_row_stride + h * query_head_stride */
+  int64_t query_row_stride; /* bytes, multiples of 16 */
+  int64_t query_head_stride;
+  uint64_t out; /* (rows, q_heads, head_dim) of the query's type, dense */
+  float* lse;   /* (rows, q_heads), dense: log of the sum of exp(scale * q . k), or null */
+} kvca_attend_desc;
+
+/*
+ * Attention of one new token per sequence: row s of query and out is the last
+ * token of sequence s (position seq_lens[s] - 1; the decode step after the
+ * token scatter of adapter.py:1275-1285).  seq_lens[s] == 0 gives zeros (lse
+ * -inf).  Two launches, no host synchronisation; the work is split evenly
+ * over the SMs whatever the lengths.  workspace:
+ * kvca_attend_step_workspace_bytes(desc) bytes (lengths and values do not
+ * matter) of device memory, 16-byte aligned, any contents; calls that may
+ * overlap on the GPU need one each.  No reference counterpart: the reference
+ * places the pages that an engine's attention reads.
+ */
+int64_t kvca_attend_step_workspace_bytes(const kvca_attend_desc* desc);
+int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t workspace_bytes, int64_t* d_status,
+                     kvca_stream_t stream);
+
 /*
  * Measurement aid, not an adapter path: moves `rows` rows of row_bytes (64,
  * 128, 256, 576, 1152 or 2048) between two dense buffers through a uint32

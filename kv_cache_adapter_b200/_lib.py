@@ -30,6 +30,10 @@ KVCA_FLAG_HOST_MEMORY = 2
 KVCA_FLAG_INPUTS_READY = 4
 KVCA_MAX_PLANES = 256
 
+KVCA_TYPE_F16 = 0
+KVCA_TYPE_BF16 = 1
+KVCA_TYPE_E4M3 = 2
+
 c_i64 = ctypes.c_int64
 c_int = ctypes.c_int
 c_ptr = ctypes.c_void_p
@@ -97,6 +101,43 @@ class AdapterSession(ctypes.Structure):
         ("status", c_ptr),
         ("stream", c_ptr),
         ("sequence", c_i64),
+    ]
+
+
+class AttendDesc(ctypes.Structure):
+    """kvca_attend_desc."""
+
+    _fields_ = [
+        ("key", ctypes.c_uint64),
+        ("value", ctypes.c_uint64),
+        ("key_block_stride", c_i64),
+        ("key_token_stride", c_i64),
+        ("key_head_stride", c_i64),
+        ("value_block_stride", c_i64),
+        ("value_token_stride", c_i64),
+        ("value_head_stride", c_i64),
+        ("num_blocks", c_i64),
+        ("block_size", c_i64),
+        ("block_tables", c_ptr),
+        ("table_stride", c_i64),
+        ("table_width", c_i64),
+        ("seq_lens", c_ptr),
+        ("num_seqs", c_i64),
+        ("q_heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("query_type", ctypes.c_int32),
+        ("cache_type", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("key_scale", ctypes.c_float),
+        ("value_scale", ctypes.c_float),
+        ("window", c_i64),
+        ("sinks", c_i64),
+        ("query", ctypes.c_uint64),
+        ("query_row_stride", c_i64),
+        ("query_head_stride", c_i64),
+        ("out", ctypes.c_uint64),
+        ("lse", c_ptr),
     ]
 
 
@@ -205,6 +246,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [ctypes.POINTER(ChunkDesc), ctypes.POINTER(PagedDesc), c_i64, c_i64, c_i64, ctypes.POINTER(PagedDesc),
          ctypes.POINTER(ChunkDesc), c_i64, c_i64, c_i64, ctypes.c_int32, ctypes.c_int32, c_ptr, c_ptr],
     ),
+    "kvca_attend_step_workspace_bytes": (c_i64, [ctypes.POINTER(AttendDesc)]),
+    "kvca_attend_step": (c_int, [ctypes.POINTER(AttendDesc), c_ptr, c_i64, c_ptr, c_ptr]),
     "kvca_copy_paged": (
         c_int,
         [ctypes.POINTER(PagedDesc), ctypes.POINTER(PagedDesc), c_i64, c_i64, c_i64, ctypes.c_int32,

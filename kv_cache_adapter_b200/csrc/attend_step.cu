@@ -1,0 +1,829 @@
+// Attention of one new token per sequence over a paged cache.
+//
+// Bound by HBM: every visible K and V row is read once, for 4 operations per
+// element and query head.  Work is cut into tiles of 16 visible tokens of one
+// (sequence, head group), numbered sequence by sequence; the tiles of all
+// sequences are dealt out evenly, a contiguous run to each warp of one CTA per
+// SM, so ragged batches and single long sequences load every SM alike.  A
+// warp streams its run through a ring of its own in shared memory (cp.async,
+// no barrier with other warps) and keeps the running maximum and sum of the
+// softmax and the output in registers.  A (sequence, head group) that lies
+// inside one run is written directly; one that several warps share leaves a
+// partial result per warp (joined within the CTA first), which a second,
+// programmatically launched kernel joins in run order.
+//
+// Both products run transposed on m16n8k16: S^T = K Q^T has the 16 tokens as
+// rows and up to 8 query heads that share the K/V head as columns, O^T = V^T
+// P^T the head dim as rows, so that 8 heads cost no padding and the transposed
+// probabilities move between the two with one movmatrix per 8 x 8.
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "attend_common.cuh"
+#include "kvca_host.cuh"
+
+namespace kvca {
+namespace {
+
+constexpr int kTile = 16;         // tokens per tile: the rows of one m16n8k16
+constexpr int kScanGroups = 1024; // sequences (or runs of them) in the shared tile counts
+constexpr int kJoinThreads = 256;
+constexpr int kJoinChunk = 64;    // partial results weighted at a time
+
+// Warps of a CTA: 8 with 24 KiB of ring each, 4 with 48 for rows of 512 bytes.
+__host__ __device__ constexpr int step_warps(int row_bytes) { return row_bytes > 256 ? 4 : 8; }
+
+// DP: head dim padded to 64, 128 or 256; NG: tiles of 8 query heads.
+template <typename Cache, int DP, int NG>
+struct StepShape {
+  static constexpr int kRowBytes = DP * Cache::kBytes;
+  static constexpr int kChunks = kRowBytes / 16;       // 16-byte chunks of a row
+  static constexpr int kStageBytes = 2 * kTile * kRowBytes;
+  static constexpr int kWarps = step_warps(kRowBytes);
+  static constexpr int kThreads = 32 * kWarps;
+  // 192 KiB of rings per SM
+  static constexpr int kRingBytes = 192 * 1024 / kWarps;
+  static constexpr int kStages = kRingBytes / kStageBytes < 8 ? kRingBytes / kStageBytes : 8;
+  static constexpr int kHeads = 8 * NG;
+  static constexpr int kAcc = DP * kHeads;  // floats of a partial output
+  static constexpr int kSmem = kWarps * kStages * kStageBytes;
+};
+
+// Shared memory address of 16-byte chunk c of row r: chunks are permuted
+// within 128 bytes so that the 8 rows an ldmatrix reads fall on distinct banks.
+template <int kChunks>
+__device__ __forceinline__ uint32_t chunk_offset(int r, int c) {
+  if constexpr (kChunks >= 8)
+    return static_cast<uint32_t>((r * kChunks + (c ^ (r & 7))) * 16);
+  else
+    return static_cast<uint32_t>((r * kChunks + (c ^ ((r >> 1) & 3))) * 16);
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (kBf16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The workspace: the run bounds, then per warp ("worker") what it left.
+struct StepHeader {
+  int64_t tiles;    // of the whole call
+  int64_t workers;  // that got tiles
+};
+
+struct StepPiece {
+  int32_t tail;   // segment whose continuation this worker's slot 0 holds, or -1
+  int32_t head;   // segment whose beginning slot 1 holds, or -1
+  int32_t last;   // worker with the last tile of `head`
+  int32_t unused;
+};
+
+template <int kHeads, int kAcc>
+struct StepWorkspace {
+  StepHeader* header;
+  StepPiece* pieces;
+  float* ml;   // [worker][slot][2][heads]: maxima, then sums
+  float* acc;  // [worker][slot][dim][heads]
+
+  static __host__ __device__ size_t bytes(int64_t workers) {
+    return 256 + static_cast<size_t>(workers) * (sizeof(StepPiece) + 2 * (2 * kHeads + kAcc) * sizeof(float));
+  }
+  __host__ __device__ StepWorkspace(void* base, int64_t workers) {
+    char* p = static_cast<char*>(base);
+    header = reinterpret_cast<StepHeader*>(p);
+    acc = reinterpret_cast<float*>(p + 256);
+    ml = acc + workers * 2 * kAcc;
+    pieces = reinterpret_cast<StepPiece*>(ml + workers * 2 * 2 * kHeads);
+  }
+  __device__ __forceinline__ float* ml_of(int64_t worker, int slot) const { return ml + (worker * 2 + slot) * 2 * kHeads; }
+  __device__ __forceinline__ float* acc_of(int64_t worker, int slot) const { return acc + (worker * 2 + slot) * kAcc; }
+};
+
+__device__ __forceinline__ int64_t run_begin(int64_t tiles, int64_t workers, int64_t w) {
+  return tiles * w / workers;  // below 2^31 tiles x a few thousand workers
+}
+
+__device__ __forceinline__ int64_t worker_of(int64_t tiles, int64_t workers, int64_t t) {
+  return (workers * (t + 1) - 1) / tiles;
+}
+
+// A position in the numbering of tiles: sequence, head group, tile.
+struct Cursor {
+  int seq;
+  int part;  // kv head * head groups + head group
+  int tile;
+  int tiles;  // of this sequence's visible tokens
+  Visible vis;
+
+  __device__ __forceinline__ void load(const AttendArgs& a) {
+    vis = visible_tokens(max(sequence_length(a, seq), 0), a.window, a.sinks);
+    tiles = (vis.count + kTile - 1) / kTile;
+  }
+  // Called only while tiles remain, so a next sequence with tokens exists.
+  __device__ __forceinline__ void advance(const AttendArgs& a, int parts) {
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++part < parts) return;
+    part = 0;
+    do {
+      ++seq;
+      load(a);
+    } while (tiles == 0);
+  }
+};
+
+template <typename Cache, int DP, int NG>
+__global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
+    attend_step_kernel(const __grid_constant__ AttendArgs a, void* workspace) {
+  using Shape = StepShape<Cache, DP, NG>;
+  constexpr bool kBf16 = Cache::kBf16;
+  constexpr bool kE4m3 = Cache::kBytes == 1;
+  constexpr int kChunks = Shape::kChunks;
+  constexpr int kStages = Shape::kStages;
+  constexpr int kHeads = Shape::kHeads;
+  constexpr int kSteps = DP / 16;
+  constexpr int kWarps = Shape::kWarps;
+  extern __shared__ __align__(128) unsigned char rings[];
+  __shared__ int64_t prefix[kScanGroups + 1];
+  __shared__ int64_t scan[33];
+  __shared__ int held[kWarps];
+  __shared__ float held_ml[kWarps][2 * kHeads];
+
+  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  const int head_groups = (a.group + kHeads - 1) / kHeads;
+  const int parts = a.kv_heads * head_groups;
+  StepWorkspace<kHeads, Shape::kAcc> ws(workspace, static_cast<int64_t>(gridDim.x) * kWarps);
+
+  // Tile counts of the sequences, or of runs of `per` of them.
+  const int per = (a.num_seqs + kScanGroups - 1) / kScanGroups;
+  const int groups = (a.num_seqs + per - 1) / per;
+  int64_t run = 0;
+  for (int base = 0; base < groups; base += Shape::kThreads) {
+    const int g = base + threadIdx.x;
+    int64_t n = 0;
+    if (g < groups) {
+      const int end = min(a.num_seqs, (g + 1) * per);
+      for (int seq = g * per; seq < end; ++seq) {
+        Cursor c;
+        c.seq = seq;
+        c.load(a);
+        n += static_cast<int64_t>(c.tiles) * parts;
+      }
+    }
+    int64_t total;
+    const int64_t before = block_excl_scan(n, &total, scan);
+    if (g < groups) prefix[g] = run + before;
+    run += total;
+  }
+  const int64_t tiles = run;
+  const int64_t all = static_cast<int64_t>(gridDim.x) * kWarps;
+  const int64_t workers = tiles < all ? tiles : all;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *ws.header = StepHeader{tiles, workers};
+  __syncthreads();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // Sequences without tokens: the sum over nothing.
+  for (int seq = blockIdx.x; seq < a.num_seqs; seq += gridDim.x) {
+    if (__ldg(a.lens + seq) != 0) continue;
+    const int64_t row = static_cast<int64_t>(seq) * a.kv_heads * a.group;
+    const int n = a.kv_heads * a.group;
+    for (int i = threadIdx.x; i < n * a.dim; i += Shape::kThreads)
+      static_cast<uint16_t*>(a.out)[row * a.dim + i] = 0;
+    if (a.lse != nullptr)
+      for (int i = threadIdx.x; i < n; i += Shape::kThreads) a.lse[row + i] = -INFINITY;
+  }
+
+  const int64_t worker = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+  int held_segment = -1;
+  bool held_starts = false;
+  StepPiece piece{-1, -1, -1, 0};
+
+  float acc[NG][kSteps][4];
+  float m[NG][2], l[NG][2];  // of the heads 2 * (lane % 4), + 1 of each tile of 8
+
+  if (worker < workers) {
+    const int64_t begin = run_begin(tiles, workers, worker);
+    const int count = static_cast<int>(run_begin(tiles, workers, worker + 1) - begin);
+
+    Cursor at;  // the tile computed next
+    {
+      int lo = 0, hi = groups;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (prefix[mid] <= begin) lo = mid; else hi = mid;
+      }
+      int64_t rest = begin - prefix[lo];
+      at.seq = lo * per;
+      at.load(a);
+      while (rest >= static_cast<int64_t>(at.tiles) * parts) {
+        rest -= static_cast<int64_t>(at.tiles) * parts;
+        ++at.seq;
+        at.load(a);
+      }
+      at.part = static_cast<int>(rest / at.tiles);
+      at.tile = static_cast<int>(rest - static_cast<int64_t>(at.part) * at.tiles);
+    }
+
+    const uint32_t ring = smem_addr(rings) + warp * (kStages * Shape::kStageBytes);
+    const int row_chunks = a.dim * Cache::kBytes / 16;
+    if (row_chunks < kChunks) {  // the padded dims stay zero: no copy writes them
+      for (int i = lane; i < kStages * Shape::kStageBytes / 16; i += 32)
+        *reinterpret_cast<uint4*>(rings + warp * (kStages * Shape::kStageBytes) + i * 16) = make_uint4(0, 0, 0, 0);
+      __syncwarp();
+    }
+
+    // Lane i holds K's row of token i % 16, lane 16 + i V's.  The page of the
+    // next tile is read one iteration before its rows.
+    const int token = lane & 15;
+    const bool value_side = lane >= 16;
+    const char* const plane = value_side ? a.value : a.key;
+    const int64_t block_stride = value_side ? a.value_block : a.key_block;
+    const int64_t token_stride = value_side ? a.value_token : a.key_token;
+    const int64_t head_stride = value_side ? a.value_head : a.key_head;
+    constexpr int64_t kHidden = -1ll << 62;  // no token of this tile
+    Cursor ahead = at;
+    int64_t page = kHidden;
+    int offset = 0, page_head = 0;
+    auto look_up = [&]() {
+      const int v = ahead.tile * kTile + token;
+      page = kHidden;
+      page_head = ahead.part / head_groups;
+      if (v < ahead.vis.count) {
+        const int pos = ahead.vis.position(v);
+        const int block = a.block_shift >= 0 ? pos >> a.block_shift : pos / a.block_size;
+        offset = pos - block * a.block_size;
+        page = __ldg(a.tables + static_cast<int64_t>(ahead.seq) * a.table_stride + block);
+      }
+    };
+    int issued = 0;
+    auto issue = [&]() {
+      if (issued < count) {
+        const char* row = nullptr;
+        if (page >= 0 && page < a.num_blocks)
+          row = plane + page * block_stride + offset * token_stride + page_head * head_stride;
+        else if (page != kHidden)
+          report(a.status, KVCA_ERR_BAD_INDEX, page);  // its rows read as zeros
+        const uint32_t stage = ring + (issued % kStages) * Shape::kStageBytes;
+        constexpr int kPerInstr = 32 / kChunks > 0 ? 32 / kChunks : 1;
+        const int r0 = kChunks >= 32 ? 0 : lane / kChunks;
+        const int c = lane % kChunks;
+#pragma unroll
+        for (int r = 0; r < 2 * kTile; r += kPerInstr) {
+          const char* src = reinterpret_cast<const char*>(
+              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), r + r0));
+          if (c < row_chunks)
+            cp_async16(stage + chunk_offset<kChunks>(r + r0, c), src != nullptr ? src + c * 16 : a.key, src != nullptr);
+        }
+        if (++issued < count) {
+          ahead.advance(a, parts);
+          look_up();
+        }
+      }
+      cp_async_commit();
+    };
+    look_up();
+#pragma unroll 1
+    for (int s = 0; s < kStages - 1; ++s) issue();
+
+    uint32_t q[NG][kSteps][2];
+    float unit[NG][2];  // score factor of the heads 2 * (lane % 4), + 1
+    bool starts = at.tile == 0;
+    bool fresh = true;
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) {
+      if (fresh) {
+        // the segment's queries as the B operand: column (head) lane / 4
+        const int kv_head = at.part / head_groups;
+        const int first = (at.part - kv_head * head_groups) * kHeads;
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          const int h = first + n * 8 + (lane >> 2);
+          const bool live = h < a.group;
+          const uint16_t* row = static_cast<const uint16_t*>(a.query) + static_cast<int64_t>(at.seq) * a.query_row +
+                                static_cast<int64_t>(kv_head * a.group + (live ? h : 0)) * a.query_head;
+          if constexpr (!kE4m3) {
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const int d = k * 16 + j * 8 + 2 * (lane & 3);
+                q[n][k][j] = live && d < a.dim ? *reinterpret_cast<const uint32_t*>(row + d) : 0u;
+              }
+            unit[n][0] = unit[n][1] = a.scale_log2;
+          } else {
+            // fp16 products: each row times a power of two that brings its
+            // largest value into [2^12, 2^13), so a bf16 row keeps its bits
+            // (values 2^-27 of the largest and less fall among fp16's
+            // subnormals); the inverse goes into the score factor.
+            float big = 0.f;
+            const bool bf16 = a.query_type == KVCA_TYPE_BF16;
+            uint2 raw[kSteps];
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+              const int d = k * 16 + 4 * (lane & 3);
+              raw[k] = live && d < a.dim ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0, 0);
+              const float2 x = bf16 ? unpack2<true>(raw[k].x) : unpack2<false>(raw[k].x);
+              const float2 y = bf16 ? unpack2<true>(raw[k].y) : unpack2<false>(raw[k].y);
+              big = fmaxf(big, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(y.x), fabsf(y.y))));
+            }
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            const int e = big > 0.f && big < INFINITY ? min(max(12 - ilogbf(big), -120), 120) : 0;
+            const float up = ldexpf(1.f, e);
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+              const float2 x = bf16 ? unpack2<true>(raw[k].x) : unpack2<false>(raw[k].x);
+              const float2 y = bf16 ? unpack2<true>(raw[k].y) : unpack2<false>(raw[k].y);
+              q[n][k][0] = pack2<false>(x.x * up, x.y * up);
+              q[n][k][1] = pack2<false>(y.x * up, y.y * up);
+            }
+            const float mine = a.scale_log2 * ldexpf(1.f, -e);
+            unit[n][0] = __shfl_sync(0xffffffffu, mine, (2 * (lane & 3)) * 4);
+            unit[n][1] = __shfl_sync(0xffffffffu, mine, (2 * (lane & 3) + 1) * 4);
+          }
+#pragma unroll
+          for (int t = 0; t < kSteps; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[n][t][j] = 0.f;
+          m[n][0] = m[n][1] = -INFINITY;
+          l[n][0] = l[n][1] = 0.f;
+        }
+        fresh = false;
+      }
+
+      cp_async_wait<kStages - 2>();
+      __syncwarp();
+      const uint32_t keys = ring + (i % kStages) * Shape::kStageBytes;
+      issue();  // into the stage that the tile before this one left
+
+      // S^T = K Q^T, even and odd steps apart for two shorter chains
+      float s[NG][2][4];
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][0][j] = s[n][1][j] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kSteps; k += kE4m3 ? 2 : 1) {
+        uint32_t f[4];
+        if constexpr (!kE4m3) {
+          ldmatrix4(f, keys + chunk_offset<kChunks>(lane & 15, 2 * k + (lane >> 4)));
+#pragma unroll
+          for (int n = 0; n < NG; ++n) mma16816<kBf16>(s[n][k & 1], f, q[n][k][0], q[n][k][1]);
+        } else {
+          // a chunk holds the 16 dims of one step; a thread's four bytes of
+          // it are the columns 2t, 2t + 1 and 2t + 8, 2t + 9 of the operand,
+          // as the query's are above
+          ldmatrix4(f, keys + chunk_offset<kChunks>(lane & 15, k + (lane >> 4)));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t w[4] = {e4m3_to_f16x2(f[2 * j]), e4m3_to_f16x2(f[2 * j + 1]),
+                                   e4m3_to_f16x2(f[2 * j] >> 16), e4m3_to_f16x2(f[2 * j + 1] >> 16)};
+#pragma unroll
+            for (int n = 0; n < NG; ++n) mma16816<false>(s[n][j], w, q[n][k + j][0], q[n][k + j][1]);
+          }
+        }
+      }
+
+      // softmax over the tile's tokens (rows lane / 4 and + 8)
+      const int left = at.vis.count - at.tile * kTile;
+      const bool row0 = (lane >> 2) < left, row1 = (lane >> 2) + 8 < left;
+      uint32_t p[NG][2], p_low[NG][2];
+      bool grew = false;
+      float decay[NG][2];
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        float x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          x[j] = (j < 2 ? row0 : row1) ? (s[n][0][j] + s[n][1][j]) * unit[n][j & 1] : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float top = fmaxf(x[j], x[j + 2]);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          const float next = fmaxf(m[n][j], top);
+          const float base = next == -INFINITY ? 0.f : next;
+          decay[n][j] = exp2_approx(m[n][j] - base);
+          grew |= next != m[n][j];
+          m[n][j] = next;
+          x[j] = exp2_approx(x[j] - base);
+          x[j + 2] = exp2_approx(x[j + 2] - base);
+          l[n][j] = l[n][j] * decay[n][j] + (x[j] + x[j + 2]);
+        }
+        const uint32_t top = pack2<kBf16>(x[0], x[1]), bottom = pack2<kBf16>(x[2], x[3]);
+        p[n][0] = transpose8x8(top);
+        p[n][1] = transpose8x8(bottom);
+        if constexpr (kBf16) {
+          // bf16 would leave 8 bits of a probability: the remainder goes in
+          // as a second product (the tensor cores idle here anyway)
+          const float2 t = unpack2<true>(top), b = unpack2<true>(bottom);
+          p_low[n][0] = transpose8x8(pack2<true>(x[0] - t.x, x[1] - t.y));
+          p_low[n][1] = transpose8x8(pack2<true>(x[2] - b.x, x[3] - b.y));
+        }
+      }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+          for (int t = 0; t < kSteps; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[n][t][j] *= decay[n][j & 1];
+      }
+
+      // O^T += V^T P^T
+      const uint32_t values = keys + kTile * Shape::kRowBytes;
+#pragma unroll
+      for (int t = 0; t < kSteps; t += kE4m3 ? 2 : 1) {
+        uint32_t f[4];
+        if constexpr (!kE4m3) {
+          // 8 x 8 pieces: dims 0-7 and 8-15 of tokens 0-7, then of 8-15
+          ldmatrix4_trans(f, values + chunk_offset<kChunks>((lane & 7) + (lane >> 4) * 8, 2 * t + ((lane >> 3) & 1)));
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+            mma16816<kBf16>(acc[n][t], f, p[n][0], p[n][1]);
+            if constexpr (kBf16) mma16816<kBf16>(acc[n][t], f, p_low[n][0], p_low[n][1]);
+          }
+        } else {
+          // pieces: chunk t of tokens 0-7 and 8-15, then chunk t + 1; a
+          // transposed 16-bit element is two dims of one token, so row g of
+          // the operand is dim 2 g of the chunk and row g + 8 dim 2 g + 1
+          ldmatrix4_trans(f, values + chunk_offset<kChunks>(lane & 15, t + (lane >> 4)));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t v = __byte_perm(f[2 * j + half], 0, 0x3120);
+              w[2 * half] = e4m3_to_f16x2(v);
+              w[2 * half + 1] = e4m3_to_f16x2(v >> 16);
+            }
+#pragma unroll
+            for (int n = 0; n < NG; ++n) mma16816<false>(acc[n][t + j], w, p[n][0], p[n][1]);
+          }
+        }
+      }
+
+      const bool ends = at.tile + 1 == at.tiles;
+      if (!ends && i + 1 < count) {
+        ++at.tile;
+        continue;
+      }
+      // the segment, or this worker's share of it, is done
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 4);
+          l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 8);
+          l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
+        }
+      const int segment = at.seq * parts + at.part;
+      if (ends && starts) {
+        const int kv_head = at.part / head_groups;
+        const int first = (at.part - kv_head * head_groups) * kHeads;
+        const int64_t row = (static_cast<int64_t>(at.seq) * a.kv_heads + kv_head) * a.group;
+        const bool bf16 = a.query_type == KVCA_TYPE_BF16;
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          const float r0 = a.value_scale / l[n][0], r1 = a.value_scale / l[n][1];
+          const int h = first + n * 8 + (lane >> 2);
+          uint16_t* const out = static_cast<uint16_t*>(a.out) + (row + h) * a.dim;
+#pragma unroll
+          for (int t = 0; t < kSteps; ++t) {
+            uint32_t top, bottom;
+            if (bf16) {
+              top = pack2<true>(acc[n][t][0] * r0, acc[n][t][1] * r1);
+              bottom = pack2<true>(acc[n][t][2] * r0, acc[n][t][3] * r1);
+            } else {
+              top = pack2<false>(acc[n][t][0] * r0, acc[n][t][1] * r1);
+              bottom = pack2<false>(acc[n][t][2] * r0, acc[n][t][3] * r1);
+            }
+            top = transpose8x8(top);  // now head lane / 4, rows 2 * (lane % 4), + 1
+            bottom = transpose8x8(bottom);
+            if (h >= a.group) continue;
+            if constexpr (!kE4m3) {
+              const int d = t * 16 + 2 * (lane & 3);
+              if (d < a.dim) *reinterpret_cast<uint32_t*>(out + d) = top;
+              if (d + 8 < a.dim) *reinterpret_cast<uint32_t*>(out + d + 8) = bottom;
+            } else {
+              const int d = t * 16 + 4 * (lane & 3);
+              if (d < a.dim)
+                *reinterpret_cast<uint2*>(out + d) =
+                    make_uint2(__byte_perm(top, bottom, 0x5410), __byte_perm(top, bottom, 0x7632));
+            }
+          }
+          if (a.lse != nullptr && lane < 4) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int hh = first + n * 8 + 2 * lane + j;
+              if (hh < a.group) a.lse[row + hh] = m[n][j] * kLn2 + logf(l[n][j]);
+            }
+          }
+        }
+      } else if (ends) {
+        // the end of a segment that an earlier worker began
+        piece.tail = segment;
+        float* const ml = ws.ml_of(worker, 0);
+        float* const part = ws.acc_of(worker, 0);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          const int h = n * 8 + 2 * (lane & 3);
+          if (lane < 4) {
+            *reinterpret_cast<float2*>(ml + h) = make_float2(m[n][0], m[n][1]);
+            *reinterpret_cast<float2*>(ml + kHeads + h) = make_float2(l[n][0], l[n][1]);
+          }
+#pragma unroll
+          for (int t = 0; t < kSteps; ++t) {
+            const int d0 = kE4m3 ? t * 16 + 2 * (lane >> 2) : t * 16 + (lane >> 2);
+            const int d1 = kE4m3 ? d0 + 1 : d0 + 8;
+            *reinterpret_cast<float2*>(part + d0 * kHeads + h) = make_float2(acc[n][t][0], acc[n][t][1]);
+            *reinterpret_cast<float2*>(part + d1 * kHeads + h) = make_float2(acc[n][t][2], acc[n][t][3]);
+          }
+        }
+      } else {
+        held_segment = segment;
+        held_starts = starts;
+        if (starts)
+          piece.last = static_cast<int>(worker_of(
+              tiles, workers, begin + i + (at.tiles - 1 - at.tile)));
+      }
+      if (i + 1 < count) {
+        at.advance(a, parts);
+        starts = true;
+        fresh = true;
+      }
+    }
+    cp_async_wait<0>();
+  }
+
+  // Partial results that the CTA's warps still hold, joined where neighbours
+  // hold the same segment: the rings are free now.
+  if (lane == 0) held[warp] = held_segment;
+  __syncthreads();
+  float* const parked = reinterpret_cast<float*>(rings);
+  if (held_segment >= 0) {
+    float* const mine = parked + warp * Shape::kAcc;
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      const int h = n * 8 + 2 * (lane & 3);
+      if (lane < 4) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          held_ml[warp][h + j] = m[n][j];
+          held_ml[warp][kHeads + h + j] = l[n][j];
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < kSteps; ++t) {
+        const int d0 = kE4m3 ? t * 16 + 2 * (lane >> 2) : t * 16 + (lane >> 2);
+        const int d1 = kE4m3 ? d0 + 1 : d0 + 8;
+        *reinterpret_cast<float2*>(mine + d0 * kHeads + h) = make_float2(acc[n][t][0], acc[n][t][1]);
+        *reinterpret_cast<float2*>(mine + d1 * kHeads + h) = make_float2(acc[n][t][2], acc[n][t][3]);
+      }
+    }
+    const bool leads = warp == 0 || held[warp - 1] != held_segment;
+    if (leads) (held_starts ? piece.head : piece.tail) = held_segment;
+  }
+  if (lane == 0 && worker < workers) ws.pieces[worker] = piece;
+  __syncthreads();
+  for (int w = 0; w < kWarps;) {
+    const int segment = held[w];
+    int end = w + 1;
+    if (segment < 0) {
+      w = end;
+      continue;
+    }
+    while (end < kWarps && held[end] == segment) ++end;
+    // a worker whose only tiles continue a segment leads with slot 0, one
+    // that began it with slot 1
+    const int64_t leader = static_cast<int64_t>(blockIdx.x) * kWarps + w;
+    const bool begins = ws.pieces[leader].head == segment;
+    float* const out = ws.acc_of(leader, begins ? 1 : 0);
+    float* const ml = ws.ml_of(leader, begins ? 1 : 0);
+    for (int i = threadIdx.x; i < Shape::kAcc; i += Shape::kThreads) {
+      const int h = i % kHeads;
+      float top = -INFINITY;
+      for (int k = w; k < end; ++k) top = fmaxf(top, held_ml[k][h]);
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, total = 0.f;
+      for (int k = w; k < end; ++k) {
+        const float weight = exp2_approx(held_ml[k][h] - base);
+        sum += weight * parked[k * Shape::kAcc + i];
+        total += weight * held_ml[k][kHeads + h];
+      }
+      out[i] = sum;
+      if (i < kHeads) {
+        ml[i] = top;
+        ml[kHeads + i] = total;
+      }
+    }
+    w = end;
+  }
+}
+
+// Joins the partial results of the segments that several workers share: one
+// block per worker that began such a segment.
+template <int DP, int NG>
+__global__ void __launch_bounds__(kJoinThreads) attend_step_join_kernel(const __grid_constant__ AttendArgs a,
+                                                                       void* workspace, int64_t max_workers) {
+  constexpr int kHeads = 8 * NG;
+  constexpr int kAcc = DP * kHeads;
+  constexpr int kVecs = (kAcc / 4 + kJoinThreads - 1) / kJoinThreads;  // float4 per thread
+  __shared__ int scan[33];
+  __shared__ int list[kJoinThreads];
+  __shared__ float weight[kJoinChunk][kHeads];
+  __shared__ float top[kHeads], total[kHeads];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  StepWorkspace<kHeads, kAcc> ws(workspace, max_workers);
+  const int64_t worker = blockIdx.x;
+  if (worker >= ws.header->workers) return;
+  const StepPiece own = ws.pieces[worker];
+  if (own.head < 0) return;
+  const int segment = own.head;
+  const int head_groups = (a.group + kHeads - 1) / kHeads;
+  const int parts = a.kv_heads * head_groups;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+
+  if (threadIdx.x < kHeads) {
+    top[threadIdx.x] = -INFINITY;
+    total[threadIdx.x] = 0.f;
+  }
+  float4 sum[kVecs];
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) sum[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+
+  // workers whose results belong here, kJoinThreads candidates at a time
+  for (int64_t base = worker; base <= own.last; base += kJoinThreads) {
+    const int64_t w = base + threadIdx.x;
+    const bool mine = w <= own.last && (w == worker || ws.pieces[w].tail == segment);
+    int found;
+    const int at = block_excl_scan(mine ? 1 : 0, &found, scan);
+    if (mine) list[at] = static_cast<int>(w);
+    __syncthreads();
+    for (int c = 0; c < found; c += kJoinChunk) {
+      const int n = min(kJoinChunk, found - c);
+      // maxima of this chunk against the running ones, a warp per head
+      for (int h = warp; h < kHeads; h += kJoinThreads / 32) {
+        float best = top[h];
+        for (int k = lane; k < n; k += 32) {
+          const int64_t p = list[c + k];
+          weight[k][h] = __ldcg(ws.ml_of(p, p == worker) + h);
+          best = fmaxf(best, weight[k][h]);
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
+        const float floor = best == -INFINITY ? 0.f : best;
+        float part = 0.f;
+        for (int k = lane; k < n; k += 32) {
+          const int64_t p = list[c + k];
+          const float x = exp2_approx(weight[k][h] - floor);
+          weight[k][h] = x;
+          part += x * __ldcg(ws.ml_of(p, p == worker) + kHeads + h);
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+        __syncwarp();
+        if (lane == 0) {
+          const float decay = exp2_approx(top[h] - floor);
+          total[h] = total[h] * decay + part;
+          top[h] = best;
+          scan[h] = __float_as_int(decay);
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        const int i = (threadIdx.x + v * kJoinThreads) * 4;
+        if (i >= kAcc) break;
+        const int h = i % kHeads;
+        float4 x = sum[v];
+        x.x *= __int_as_float(scan[h]);
+        x.y *= __int_as_float(scan[h + 1]);
+        x.z *= __int_as_float(scan[h + 2]);
+        x.w *= __int_as_float(scan[h + 3]);
+#pragma unroll 8
+        for (int k = 0; k < n; ++k) {
+          const int64_t p = list[c + k];
+          const float4 o = __ldcg(reinterpret_cast<const float4*>(ws.acc_of(p, p == worker) + i));
+          x.x += weight[k][h] * o.x;
+          x.y += weight[k][h + 1] * o.y;
+          x.z += weight[k][h + 2] * o.z;
+          x.w += weight[k][h + 3] * o.w;
+        }
+        sum[v] = x;
+      }
+      __syncthreads();
+    }
+  }
+
+  const int seq = segment / parts, part = segment - seq * parts;
+  const int kv_head = part / head_groups;
+  const int first = (part - kv_head * head_groups) * kHeads;
+  const int64_t row = (static_cast<int64_t>(seq) * a.kv_heads + kv_head) * a.group;
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) {
+    const int i = (threadIdx.x + v * kJoinThreads) * 4;
+    if (i >= kAcc) break;
+    const int d = i / kHeads;
+    if (d >= a.dim) break;
+    const float x[4] = {sum[v].x, sum[v].y, sum[v].z, sum[v].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int h = i % kHeads + j;
+      if (first + h >= a.group) continue;
+      const float y = x[j] * (a.value_scale / total[h]);
+      uint16_t* const out = static_cast<uint16_t*>(a.out) + (row + first + h) * a.dim + d;
+      *out = static_cast<uint16_t>(a.query_type == KVCA_TYPE_BF16 ? pack2<true>(y, 0.f) : pack2<false>(y, 0.f));
+    }
+  }
+  if (a.lse != nullptr && threadIdx.x < kHeads && first + threadIdx.x < a.group)
+    a.lse[row + first + threadIdx.x] = top[threadIdx.x] * kLn2 + logf(total[threadIdx.x]);
+}
+
+template <typename Cache, int DP, int NG>
+cudaError_t launch_typed(const AttendArgs& a, void* workspace, int sms, cudaStream_t stream) {
+  using Shape = StepShape<Cache, DP, NG>;
+  auto kernel = attend_step_kernel<Cache, DP, NG>;
+  static DeviceFlags configured;
+  int dev = -1;
+  if (needs_setup(configured, &dev)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
+    if (e != cudaSuccess) return e;
+    mark_setup(configured, dev);
+  }
+  kernel<<<sms, Shape::kThreads, Shape::kSmem, stream>>>(a, workspace);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const int64_t workers = static_cast<int64_t>(sms) * Shape::kWarps;
+  return launch_dependent(attend_step_join_kernel<DP, NG>, dim3(static_cast<unsigned>(workers)), kJoinThreads, 0,
+                          stream, a, workspace, workers);
+}
+
+template <typename Cache, int DP>
+size_t workspace_of(int tiles, int sms) {
+  const int64_t workers = static_cast<int64_t>(sms) * step_warps(DP * Cache::kBytes);
+  return tiles == 1 ? StepWorkspace<8, DP * 8>::bytes(workers) : StepWorkspace<16, DP * 16>::bytes(workers);
+}
+
+// Tiles of 8 query heads that share one pass over the rows: two for groups
+// above 8, except at head dims above 128, whose outputs fill the registers;
+// larger groups pass over the rows once per 16 (8) heads.
+int head_tiles(const AttendArgs& a) { return a.group > 8 && a.dim <= 128 ? 2 : 1; }
+
+}  // namespace
+
+size_t attend_step_workspace(const AttendArgs& a, int sms) {
+  const int n = head_tiles(a);
+  const bool e4m3 = a.cache_type == KVCA_TYPE_E4M3;
+  if (a.dim <= 64) return e4m3 ? workspace_of<CacheE4m3, 64>(n, sms) : workspace_of<CacheF16, 64>(n, sms);
+  if (a.dim <= 128) return e4m3 ? workspace_of<CacheE4m3, 128>(n, sms) : workspace_of<CacheF16, 128>(n, sms);
+  return e4m3 ? workspace_of<CacheE4m3, 256>(n, sms) : workspace_of<CacheF16, 256>(n, sms);
+}
+
+template <typename Cache>
+static cudaError_t launch_cache(const AttendArgs& a, void* workspace, int sms, cudaStream_t stream) {
+  const int n = head_tiles(a);
+  if (a.dim <= 64)
+    return n == 1 ? launch_typed<Cache, 64, 1>(a, workspace, sms, stream)
+                  : launch_typed<Cache, 64, 2>(a, workspace, sms, stream);
+  if (a.dim <= 128)
+    return n == 1 ? launch_typed<Cache, 128, 1>(a, workspace, sms, stream)
+                  : launch_typed<Cache, 128, 2>(a, workspace, sms, stream);
+  return launch_typed<Cache, 256, 1>(a, workspace, sms, stream);
+}
+
+cudaError_t launch_attend_step(const AttendArgs& a, void* workspace, int sms, cudaStream_t stream) {
+  switch (a.cache_type) {
+    case KVCA_TYPE_F16: return launch_cache<CacheF16>(a, workspace, sms, stream);
+    case KVCA_TYPE_BF16: return launch_cache<CacheBf16>(a, workspace, sms, stream);
+    default: return launch_cache<CacheE4m3>(a, workspace, sms, stream);
+  }
+}
+
+}  // namespace kvca

@@ -79,6 +79,74 @@ void to_side(const kvca_chunk_desc* d, kvca::ChunkSide* s) {
   s->plane_stride = d->plane_stride;
 }
 
+bool aligned16(uint64_t x) { return x % 16 == 0; }
+
+// The checked arguments of an attention call as the kernels take them.
+int to_attend(const kvca_attend_desc* d, int64_t* d_status, kvca::AttendArgs* a) {
+  if (d == nullptr || d->num_seqs < 0 || d->num_blocks < 0 || d->block_size < 1 || d->table_width < 0 ||
+      d->table_stride < 0 || d->window < 0 || d->sinks < 0 || d->kv_heads < 1 || d->q_heads < 1 ||
+      d->q_heads % d->kv_heads != 0 || d->head_dim < 8 || d->head_dim > 256)
+    return KVCA_ERR_BAD_ARGUMENT;
+  if (d->query_type != KVCA_TYPE_F16 && d->query_type != KVCA_TYPE_BF16) return KVCA_ERR_BAD_ARGUMENT;
+  const bool e4m3 = d->cache_type == KVCA_TYPE_E4M3;
+  if (!e4m3 && d->cache_type != d->query_type) return KVCA_ERR_BAD_ARGUMENT;
+  if (d->head_dim % (e4m3 ? 16 : 8) != 0) return KVCA_ERR_BAD_ARGUMENT;
+  const uint64_t strides[] = {d->key, d->value, static_cast<uint64_t>(d->key_block_stride),
+                              static_cast<uint64_t>(d->key_token_stride), static_cast<uint64_t>(d->key_head_stride),
+                              static_cast<uint64_t>(d->value_block_stride),
+                              static_cast<uint64_t>(d->value_token_stride),
+                              static_cast<uint64_t>(d->value_head_stride), d->query,
+                              static_cast<uint64_t>(d->query_row_stride),
+                              static_cast<uint64_t>(d->query_head_stride), d->out};
+  for (uint64_t x : strides)
+    if (!aligned16(x)) return KVCA_ERR_BAD_ARGUMENT;
+  const int64_t limit = int64_t{1} << 30;
+  if (d->table_width > limit / d->block_size || d->num_seqs > limit / d->q_heads || d->q_heads > 65536)
+    return KVCA_ERR_SIZE_LIMIT;
+  memset(a, 0, sizeof(*a));
+  a->key = reinterpret_cast<const char*>(d->key);
+  a->value = reinterpret_cast<const char*>(d->value);
+  a->key_block = d->key_block_stride;
+  a->key_token = d->key_token_stride;
+  a->key_head = d->key_head_stride;
+  a->value_block = d->value_block_stride;
+  a->value_token = d->value_token_stride;
+  a->value_head = d->value_head_stride;
+  a->num_blocks = d->num_blocks;
+  a->block_size = static_cast<int>(d->block_size < limit ? d->block_size : limit);
+  a->block_shift = -1;
+  for (int b = 0; b < 31; ++b)
+    if (a->block_size == 1 << b) a->block_shift = b;
+  a->tables = d->block_tables;
+  a->table_stride = d->table_stride;
+  a->capacity = static_cast<int>(d->table_width * d->block_size);
+  a->lens = d->seq_lens;
+  a->num_seqs = static_cast<int>(d->num_seqs);
+  a->kv_heads = d->kv_heads;
+  a->group = d->q_heads / d->kv_heads;
+  a->dim = d->head_dim;
+  a->scale_log2 = static_cast<float>(static_cast<double>(d->scale) * d->key_scale * 1.4426950408889634);
+  a->value_scale = d->value_scale;
+  a->window = static_cast<int>(d->window < limit ? d->window : limit);
+  a->sinks = static_cast<int>(d->sinks < limit ? d->sinks : limit);
+  a->query = reinterpret_cast<const void*>(d->query);
+  a->query_row = d->query_row_stride / 2;
+  a->query_head = d->query_head_stride / 2;
+  a->out = reinterpret_cast<void*>(d->out);
+  a->lse = d->lse;
+  a->query_type = d->query_type;
+  a->cache_type = d->cache_type;
+  a->status = d_status;
+  return KVCA_OK;
+}
+
+// Pointers that a call which has work to do cannot go without.
+bool attend_pointers_ok(const kvca::AttendArgs& a) {
+  return a.lens != nullptr && a.query != nullptr && a.out != nullptr &&
+         (a.capacity == 0 || a.num_blocks == 0 ||
+          (a.key != nullptr && a.value != nullptr && a.tables != nullptr));
+}
+
 bool common_move_args_ok(int64_t num_planes, int64_t num_rows, int64_t row_bytes) {
   return num_planes >= 1 && num_planes <= KVCA_MAX_PLANES && num_rows >= 0 && row_bytes >= 1;
 }
@@ -700,6 +768,27 @@ int kvca_move_cycle(const kvca_chunk_desc* tokens, const kvca_paged_desc* token_
                     num_seqs, spill_rows, token_row_bytes, block_row_bytes, flags,
                     static_cast<unsigned char*>(d_scratch), d_status};
   return status_of(kvca::launch_move_cycle(a, stream));
+}
+
+int64_t kvca_attend_step_workspace_bytes(const kvca_attend_desc* desc) {
+  kvca::AttendArgs a;
+  if (to_attend(desc, nullptr, &a) != KVCA_OK) return -1;
+  return static_cast<int64_t>(kvca::attend_step_workspace(a, kvca_device_sm_count()));
+}
+
+int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t workspace_bytes, int64_t* d_status,
+                     kvca_stream_t stream) {
+  kvca::AttendArgs a;
+  const int rc = to_attend(desc, d_status, &a);
+  if (rc != KVCA_OK) return rc;
+  if (a.num_seqs == 0) return KVCA_OK;
+  if (!attend_pointers_ok(a)) return KVCA_ERR_BAD_ARGUMENT;
+  const int sms = kvca_device_sm_count();
+  if (sms < 1) return KVCA_ERR_CUDA;
+  if (d_workspace == nullptr || !aligned16(reinterpret_cast<uint64_t>(d_workspace)) ||
+      workspace_bytes < static_cast<int64_t>(kvca::attend_step_workspace(a, sms)))
+    return KVCA_ERR_BAD_ARGUMENT;
+  return status_of(kvca::launch_attend_step(a, d_workspace, sms, stream));
 }
 
 int kvca_copy_paged(const kvca_paged_desc* src, const kvca_paged_desc* dst, int64_t num_planes,

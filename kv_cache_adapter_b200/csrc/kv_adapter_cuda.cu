@@ -25,84 +25,12 @@
 #include <atomic>
 #include <utility>
 
+#include "kvca_device.cuh"
+#include "kvca_host.cuh"
 #include "kvca_launch.h"
 
 namespace kvca {
 namespace {
-
-// ---------------------------------------------------------------------------
-// Status reporting
-// ---------------------------------------------------------------------------
-
-__device__ __forceinline__ void report(int64_t* status, int64_t code, int64_t value) {
-  if (status == nullptr) return;
-  const unsigned long long prev = atomicCAS(reinterpret_cast<unsigned long long*>(status), 0ull,
-                                            static_cast<unsigned long long>(code));
-  if (prev == 0ull) status[1] = value;
-}
-
-// ---------------------------------------------------------------------------
-// Packed slot metadata: pin count in the low half of the word, usage count in
-// the high half (adapter.py:1419-1432).
-// ---------------------------------------------------------------------------
-
-template <typename MetaT>
-struct Meta {
-  static constexpr int kFieldBits = static_cast<int>(sizeof(MetaT)) * 4;
-  static constexpr unsigned kFieldMask = (1u << kFieldBits) - 1u;
-  static constexpr int kUsageMax = static_cast<int>(kFieldMask);
-  static constexpr int kSlotsPerVec = 16 / static_cast<int>(sizeof(MetaT));
-
-  __device__ __forceinline__ static unsigned pin(unsigned w) { return w & kFieldMask; }
-  __device__ __forceinline__ static unsigned usage(unsigned w) {
-    return (w >> kFieldBits) & kFieldMask;
-  }
-  // Masks both fields exactly like _pack_slot_meta: pins above the field
-  // maximum and negative pins wrap.
-  __device__ __forceinline__ static MetaT pack(int64_t pin_count, int64_t usage_count) {
-    const uint64_t p = static_cast<uint64_t>(pin_count) & kFieldMask;
-    const uint64_t u = static_cast<uint64_t>(usage_count) & kFieldMask;
-    return static_cast<MetaT>(p | (u << kFieldBits));
-  }
-  __device__ __forceinline__ static unsigned sat_inc(unsigned usage_count) {
-    return usage_count + 1u > kFieldMask ? kFieldMask : usage_count + 1u;
-  }
-};
-
-// ---------------------------------------------------------------------------
-// Block-wide exclusive scan (blockDim.x a multiple of 32, at most 1024).
-// `sm` holds 33 ints.  Contains three __syncthreads.
-// ---------------------------------------------------------------------------
-
-__device__ __forceinline__ int block_excl_scan(int x, int* total, int* sm) {
-  const int lane = threadIdx.x & 31;
-  const int warp = threadIdx.x >> 5;
-  int incl = x;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += y;
-  }
-  if (lane == 31) sm[warp] = incl;
-  __syncthreads();
-  if (warp == 0) {
-    const int nwarps = static_cast<int>(blockDim.x >> 5);
-    const int w = lane < nwarps ? sm[lane] : 0;
-    int wi = w;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, wi, d);
-      if (lane >= d) wi += y;
-    }
-    if (lane < nwarps) sm[lane] = wi - w;
-    if (lane == 31) sm[32] = wi;
-  }
-  __syncthreads();
-  const int result = sm[warp] + incl - x;
-  *total = sm[32];
-  __syncthreads();
-  return result;
-}
 
 // ---------------------------------------------------------------------------
 // Metadata vector access: 16 bytes per thread when the table is 16-byte
@@ -3049,50 +2977,6 @@ __global__ void __launch_bounds__(kMoverThreads, KVCA_PAIR_ALL_MIN_CTAS)
   }
   run_mover_body<kA, false, true, kEarly>(a, blockIdx.x, gridDim.x);
   run_mover_body<kB, true, false, kEarly>(b, blockIdx.x, gridDim.x);
-}
-
-// Launch as a programmatic dependent of the kernel before it on the stream
-// (the kernel must begin with dependent_launch_entry()).
-template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem,
-                             cudaStream_t stream, Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(block);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-  return e != cudaSuccess ? e : cudaGetLastError();
-}
-
-int device_sm_count() {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  int sms = 0;
-  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  return sms;
-}
-
-// Function attributes (the dynamic shared-memory limit, the carve-out)
-// belong to the current device's context, so a launcher sets them once per
-// device: `done` records the ordinals done (devices past the table are set
-// up on every call).
-constexpr int kTrackedDevices = 64;
-using DeviceFlags = std::atomic<bool>[kTrackedDevices];
-
-bool needs_setup(const DeviceFlags& done, int* dev) {
-  *dev = -1;
-  if (cudaGetDevice(dev) != cudaSuccess) return true;
-  return *dev < 0 || *dev >= kTrackedDevices || !done[*dev].load(std::memory_order_acquire);
-}
-
-void mark_setup(DeviceFlags& done, int dev) {
-  if (dev >= 0 && dev < kTrackedDevices) done[dev].store(true, std::memory_order_release);
 }
 
 template <bool kSrcPaged, bool kDstPaged, typename V, bool kHost = false>

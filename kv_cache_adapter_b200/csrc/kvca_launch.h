@@ -117,6 +117,38 @@ struct ExchangeArgs {
 
 cudaError_t launch_exchange(const ExchangeArgs& args, cudaStream_t stream);
 
+// Attention over a paged cache (kvca_attend_step, kvca_attend_chunk).
+// Strides of the cache in bytes, of the query in elements.
+struct AttendArgs {
+  const char* key;
+  const char* value;
+  int64_t key_block, key_token, key_head;
+  int64_t value_block, value_token, value_head;
+  int64_t num_blocks;
+  int block_size;
+  int block_shift;  // log2(block_size), or -1
+  const int64_t* tables;
+  int64_t table_stride;
+  int capacity;  // tokens that a row of the page table holds
+  const int64_t* lens;
+  int num_seqs;
+  int kv_heads, group, dim;
+  float scale_log2;  // scale * key_scale * log2(e)
+  float value_scale;
+  int window;  // 0: none
+  int sinks;
+  const void* query;
+  int64_t query_row, query_head;
+  void* out;   // (rows, heads, dim), dense
+  float* lse;  // (rows, heads), dense, or null
+  int query_type;
+  int cache_type;
+  int64_t* status;
+};
+
+size_t attend_step_workspace(const AttendArgs& args, int sms);
+cudaError_t launch_attend_step(const AttendArgs& args, void* workspace, int sms, cudaStream_t stream);
+
 cudaError_t launch_inspect_load(int meta_bits, const int64_t* l2p, int64_t num_logical,
                                 const void* meta, int64_t num_slots, const int64_t* ids,
                                 int64_t count, int64_t* cur_out, uint8_t* resident_out,

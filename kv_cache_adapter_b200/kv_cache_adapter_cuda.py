@@ -53,6 +53,7 @@ __all__ = [
     "scatter_tokens_gather_layers",
     "move_cycle",
     "exchange_blocks",
+    "attend_step",
     "batched_fused_single_layer_kv_transfer",
     "load_device_store",
     "save_device_store",
@@ -1272,6 +1273,132 @@ def move_cycle(token_caches, slot_mapping: torch.Tensor, token_rows: torch.Tenso
             _ptr(_status(dev)), _stream(dev))
     _host_rc(rc, "move_cycle")
     _maybe_check(dev, check, "move_cycle")
+
+
+# ---------------------------------------------------------------------------
+# attention over the paged cache
+# ---------------------------------------------------------------------------
+
+_ATTEND_TYPES = {torch.float16: _lib.KVCA_TYPE_F16, torch.bfloat16: _lib.KVCA_TYPE_BF16,
+                 torch.float8_e4m3fn: _lib.KVCA_TYPE_E4M3}
+_attend_workspace_bytes: dict[tuple, int] = {}
+
+
+def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                 block_tables: torch.Tensor, seq_lens: torch.Tensor, scale, window, sinks, key_scale, value_scale,
+                 out, lse) -> tuple[_lib.AttendDesc, torch.Tensor]:
+    """The checked arguments of an attention call and its output tensor."""
+    for t, name in ((query, "query"), (key_cache, "key_cache"), (value_cache, "value_cache"),
+                    (block_tables, "block_tables"), (seq_lens, "seq_lens")):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be torch.Tensor")
+    dev = query.device
+    if not query.is_cuda:
+        raise ValueError("query must be a CUDA tensor")
+    for t, name in ((key_cache, "key_cache"), (value_cache, "value_cache"), (block_tables, "block_tables"),
+                    (seq_lens, "seq_lens")):
+        if t.device != dev:
+            raise ValueError(f"{name} must be on {dev}")
+    if query.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"query has incorrect dtype {query.dtype}")
+    if query.dim() != 3 or key_cache.dim() != 4:
+        raise ValueError("query must be (rows, heads, head_dim) and the caches (num_blocks, block_size, kv_heads, "
+                         "head_dim)")
+    ctype = key_cache.dtype
+    if ctype != query.dtype and ctype != torch.float8_e4m3fn:
+        raise TypeError(f"key_cache has incorrect dtype {ctype}")
+    if value_cache.dtype != ctype or value_cache.shape != key_cache.shape:
+        raise ValueError("key_cache and value_cache must share shape and dtype")
+    rows, heads, dim = query.shape
+    num_blocks, block_size, kv_heads, cache_dim = key_cache.shape
+    if cache_dim != dim:
+        raise ValueError(f"the caches' head_dim {cache_dim} is not the query's {dim}")
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError(f"the query heads ({heads}) must be a positive multiple of the K/V heads ({kv_heads})")
+    if block_size < 1:
+        raise ValueError("block_size must be positive")
+    step = 16 if ctype == torch.float8_e4m3fn else 8
+    if dim < step or dim > 256 or dim % step:
+        raise ValueError(f"head_dim must be a multiple of {step} up to 256, got {dim}")
+    if block_tables.dtype != torch.int64 or seq_lens.dtype != torch.int64:
+        raise TypeError("block_tables and seq_lens must be int64")
+    if seq_lens.dim() != 1 or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be 1D and contiguous")
+    if block_tables.dim() != 2 or block_tables.shape[0] != seq_lens.shape[0] or (
+            block_tables.numel() and block_tables.stride(1) != 1):
+        raise ValueError("block_tables must be (num_seqs, max_blocks) with contiguous rows")
+    window = 0 if window is None else int(window)
+    sinks = int(sinks)
+    if window < 0 or sinks < 0 or (window == 0 and sinks > 0):
+        raise ValueError("window must be positive (or None) and sinks need a window")
+    if ctype != torch.float8_e4m3fn and (key_scale != 1.0 or value_scale != 1.0):
+        raise ValueError("key_scale and value_scale belong to an e4m3 cache")
+    esz = key_cache.element_size()
+    ks, vs, qs = key_cache.stride(), value_cache.stride(), query.stride()
+    for st, t, name in ((ks, key_cache, "key_cache"), (vs, value_cache, "value_cache"), (qs, query, "query")):
+        size = t.element_size()
+        if t.numel() and (st[-1] != 1 or t.data_ptr() % 16 or any(
+                n > 1 and x * size % 16 for n, x in zip(t.shape[:-1], st[:-1]))):
+            raise ValueError(f"{name}: rows of head_dim must be contiguous and 16-byte aligned")
+    # a dim of size 1 may carry any stride
+    ks, vs, qs = ([x if n > 1 else 0 for n, x in zip(t.shape[:-1], t.stride())] for t in (key_cache, value_cache, query))
+    if out is None:
+        out = torch.empty((rows, heads, dim), dtype=query.dtype, device=dev)
+    elif (tuple(out.shape) != (rows, heads, dim) or out.dtype != query.dtype or out.device != dev
+          or not out.is_contiguous() or out.data_ptr() % 16):
+        raise ValueError(f"out must be a contiguous, 16-byte aligned {(rows, heads, dim)} {query.dtype} tensor on {dev}")
+    if lse is not None and (tuple(lse.shape) != (rows, heads) or lse.dtype != torch.float32 or lse.device != dev
+                            or not lse.is_contiguous()):
+        raise ValueError(f"lse must be a contiguous {(rows, heads)} float32 tensor on {dev}")
+    desc = _lib.AttendDesc(
+        key_cache.data_ptr(), value_cache.data_ptr(), ks[0] * esz, ks[1] * esz, ks[2] * esz, vs[0] * esz, vs[1] * esz,
+        vs[2] * esz, num_blocks, block_size, block_tables.data_ptr() or None, block_tables.stride(0),
+        block_tables.shape[1], seq_lens.data_ptr() or None, seq_lens.shape[0], heads, kv_heads, dim,
+        _ATTEND_TYPES[query.dtype], _ATTEND_TYPES[ctype], dim ** -0.5 if scale is None else scale, key_scale,
+        value_scale, window, sinks, query.data_ptr(), qs[0] * 2, qs[1] * 2, out.data_ptr(),
+        None if lse is None else lse.data_ptr())
+    return desc, out
+
+
+def attend_step(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_tables: torch.Tensor,
+                seq_lens: torch.Tensor, *, scale: float | None = None, window: int | None = None, sinks: int = 0,
+                key_scale: float = 1.0, value_scale: float = 1.0, out: torch.Tensor | None = None,
+                lse: torch.Tensor | None = None, check: bool | None = None) -> torch.Tensor:
+    """Attention of one new token per sequence over the paged cache
+    (kvca_attend_step): the step after ``scatter_tokens`` wrote the token's
+    K and V.  ``query`` ``(num_seqs, heads, head_dim)`` fp16 or bf16;
+    ``key_cache`` / ``value_cache`` ``(num_blocks, block_size, kv_heads,
+    head_dim)`` of the same dtype or e4m3 (values times ``key_scale`` /
+    ``value_scale``), any order of the leading dims in memory, K and V planes
+    of a merged cache too; ``block_tables`` int64 ``(num_seqs, max_blocks)``;
+    ``seq_lens`` int64, the new token included.  The token at the end of a
+    sequence sees all of it, or with ``window`` its last ``window`` tokens and
+    the first ``sinks`` ones.  ``scale`` defaults to ``head_dim ** -0.5``.
+    Returns ``out`` ``(num_seqs, heads, head_dim)``; ``lse`` (float32
+    ``(num_seqs, heads)``) also gets the log of each softmax's sum.  A
+    sequence of length 0 gives zeros (``lse`` -inf); rows of negative length
+    are left as they were."""
+    desc, out = _attend_desc(query, key_cache, value_cache, block_tables, seq_lens, scale, window, sinks, key_scale,
+                             value_scale, out, lse)
+    if query.shape[0] != seq_lens.shape[0]:
+        raise ValueError("query needs one row per sequence")
+    if query.shape[0] == 0:
+        return out
+    dev = query.device
+    with _on(dev):
+        shape = ("step", _index(dev), desc.q_heads // desc.kv_heads, desc.head_dim, desc.cache_type)
+        need = _attend_workspace_bytes.get(shape)
+        if need is None:
+            need = _lib_handle.kvca_attend_step_workspace_bytes(ctypes.byref(desc))
+            if need < 0:
+                _raise_for(_lib.KVCA_ERR_BAD_ARGUMENT, 0, "attend_step")
+            _attend_workspace_bytes[shape] = need
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        rc = _lib_handle.kvca_attend_step(ctypes.byref(desc), workspace.data_ptr(), need, _ptr(_status(dev)),
+                                          _stream(dev))
+    _host_rc(rc, "attend_step")
+    _maybe_check(dev, check, "attend_step")
+    return out
 
 
 def copy_tokens(src_caches, src_mapping: torch.Tensor, dst_caches, dst_mapping: torch.Tensor, *,
