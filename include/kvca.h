@@ -681,6 +681,26 @@ int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t wo
                      kvca_stream_t stream);
 
 /*
+ * Attention of a ragged chunk of new tokens per sequence (a prompt, the next
+ * piece of one, drafted tokens to verify): rows query_offsets[s] ..
+ * query_offsets[s + 1] of query and out (of num_rows in all) are the last
+ * tokens of sequence s, so row i of n is at position seq_lens[s] - n + i and
+ * its K and V, and those of the rows before it, are in the cache.  Offsets
+ * (num_seqs + 1, device memory) do not decrease; rows outside them, and those
+ * of a sequence of negative length, are left as they were.  Offsets out of
+ * order or outside [0, num_rows], and a sequence shorter than its chunk, give
+ * KVCA_ERR_BAD_INDEX (that sequence's rows then hold no defined values).
+ * head_dim is at most 128.  Three launches, no host synchronisation; the work
+ * is split evenly over the SMs whatever the lengths.  workspace:
+ * kvca_attend_chunk_workspace_bytes(desc, num_rows) bytes, as for
+ * kvca_attend_step.  A bounded wait that runs out gives
+ * KVCA_ERR_DEVICE_TIMEOUT.  No reference counterpart.
+ */
+int64_t kvca_attend_chunk_workspace_bytes(const kvca_attend_desc* desc, int64_t num_rows);
+int kvca_attend_chunk(const kvca_attend_desc* desc, const int64_t* d_query_offsets, int64_t num_rows,
+                      void* d_workspace, int64_t workspace_bytes, int64_t* d_status, kvca_stream_t stream);
+
+/*
  * Measurement aid, not an adapter path: moves `rows` rows of row_bytes (64,
  * 128, 256, 576, 1152 or 2048) between two dense buffers through a uint32
  * permutation, scatter (dst row d_perm[r] = src row r) or gather (dst row r

@@ -1,0 +1,1037 @@
+// Attention of a ragged chunk of new tokens per sequence over a paged cache.
+//
+// For one K/V head, the chunk's rows are its (token, query head of the group)
+// pairs, token by token; a block of up to 256 of them (two tiles of 128, one
+// per softmax warpgroup) shares a pass over the keys that any of them sees.
+// Those keys, numbered without the gap between sinks and window, are cut into
+// tiles of 128.  The tiles of all blocks and heads are dealt out evenly, a
+// contiguous run to each SM, so causal triangles, ragged chunks and a few rows
+// over a long cache all load the SMs alike; a block that several SMs share
+// leaves one partial result per SM, which a last kernel joins.
+//
+// One persistent CTA per SM, 16 warps:
+//   warps 0-3, 4-7  softmax of row tile 0 and 1, a thread per row: scores from
+//                   tensor memory, running maximum and sum in registers,
+//                   probabilities back to tensor memory, output at the end
+//   warps 8-11      rows of the pages to shared memory (cp.async per 16 bytes,
+//                   so that any block size and stride does; e4m3 is widened on
+//                   the way), 128-byte swizzled as the tensor cores read them
+//   warp 12         issues tcgen05.mma: S = Q K^T, O += P V
+// The two tiles alternate: while one's softmax runs, the tensor cores work on
+// the other's products.  The output is rescaled only when a row's maximum grew
+// by more than 2^8, so that most tiles leave it alone; a probability is then at
+// most 2^8.
+//
+// Bound by the tensor cores and the exponentials (16 per SM and clock) for
+// long chunks, by HBM for a few tokens.
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include <string.h>
+
+#include "attend_common.cuh"
+#include "kvca_host.cuh"
+
+namespace kvca {
+namespace {
+
+constexpr int kRows = 256;      // rows of a block
+constexpr int kKeys = 128;      // keys of a tile
+constexpr int kThreads = 512;
+constexpr int kPlanThreads = 1024;
+constexpr int kJoinThreads = 256;
+constexpr int kJoinRows = 16;   // rows per block of the join
+constexpr float kGrowth = 8.f;  // log2 of how far a maximum may lag
+constexpr uint32_t kWaitTries = 1u << 22;
+
+template <int DP>
+struct ChunkShape {
+  static constexpr int kHalves = DP / 64;                 // 64 dims (128 bytes) each
+  static constexpr int kTileBytes = kHalves * kKeys * 128;  // 128 rows of DP 16-bit values
+  static constexpr int kStages = 128 * 1024 / kTileBytes;
+  static constexpr int kSmem = 1024 + 2 * kTileBytes + kStages * kTileBytes;
+};
+
+// ---------------------------------------------------------------------------
+// Plan: the blocks of all chunks and their tiles
+// ---------------------------------------------------------------------------
+
+struct ChunkHeader {
+  int64_t tiles;  // of all blocks and heads
+  int64_t ctas;   // that get tiles
+  int32_t blocks;
+  int32_t unused;
+};
+
+struct ChunkBlock {
+  int32_t seq;
+  int32_t row;    // first (token, head) row within the chunk
+  int32_t rows;
+  int32_t tiles;  // per head
+};
+
+struct ChunkPiece {
+  int32_t tail;  // segment (block * heads + head) whose continuation slot 0 holds, or -1
+  int32_t head;  // segment whose beginning slot 1 holds, or -1
+  int32_t last;  // CTA with the last tile of `head`
+  int32_t unused;
+};
+
+struct ChunkWorkspace {
+  ChunkHeader* header;
+  float* acc;        // [cta][slot][row][dim]
+  float* ml;         // [cta][slot][2][row]
+  ChunkPiece* pieces;
+  int64_t* first;    // tiles before each block
+  ChunkBlock* blocks;
+
+  static __host__ __device__ size_t bytes(int dp, int64_t ctas, int64_t max_blocks) {
+    return 256 + static_cast<size_t>(ctas) * (sizeof(ChunkPiece) + 2 * kRows * (dp + 2) * sizeof(float)) +
+           static_cast<size_t>(max_blocks + 1) * (sizeof(int64_t) + sizeof(ChunkBlock));
+  }
+  __host__ __device__ ChunkWorkspace(void* base, int dp, int64_t ctas, int64_t max_blocks) {
+    char* p = static_cast<char*>(base);
+    header = reinterpret_cast<ChunkHeader*>(p);
+    acc = reinterpret_cast<float*>(p + 256);
+    ml = acc + ctas * 2 * kRows * dp;
+    pieces = reinterpret_cast<ChunkPiece*>(ml + ctas * 2 * 2 * kRows);
+    blocks = reinterpret_cast<ChunkBlock*>(pieces + ctas);
+    first = reinterpret_cast<int64_t*>(blocks + max_blocks + 1);
+  }
+};
+
+// What a block's rows see.  v numbers the keys without the gap: v < sinks is
+// key v, any other key v + skip.
+struct BlockView {
+  int seq, row, rows;
+  int context;  // position of the chunk's first token
+  int skip, sinks, count;
+
+  __device__ __forceinline__ int key(int v) const { return v < sinks ? v : v + skip; }
+};
+
+__device__ __forceinline__ BlockView view_of(const AttendArgs& a, int seq, int row, int rows, int tokens, int len) {
+  BlockView b;
+  b.seq = seq;
+  b.row = row;
+  b.rows = rows;
+  b.context = len - tokens;
+  const int first = b.context + row / a.group, last = b.context + (row + rows - 1) / a.group;
+  const int low = a.window > 0 ? max(0, first - a.window + 1) : 0;
+  b.sinks = min(a.sinks, low);
+  b.skip = low - b.sinks;
+  b.count = last + 1 - b.skip;
+  return b;
+}
+
+// Tokens of sequence `seq`'s chunk (0: none, or an idle or bad sequence).
+__device__ __forceinline__ int chunk_tokens(const AttendArgs& a, const ChunkArgs& c, int seq, int* len) {
+  const int64_t begin = __ldg(c.offsets + seq), end = __ldg(c.offsets + seq + 1);
+  *len = sequence_length(a, seq);
+  if (end == begin || *len < 0) return 0;
+  if (begin < 0 || end < begin || end > c.rows) {
+    report(a.status, KVCA_ERR_BAD_INDEX, end);
+    return 0;
+  }
+  if (end - begin > *len) {
+    report(a.status, KVCA_ERR_BAD_INDEX, __ldg(a.lens + seq));
+    return 0;
+  }
+  return static_cast<int>(end - begin);
+}
+
+__global__ void __launch_bounds__(kPlanThreads) attend_chunk_plan_kernel(const __grid_constant__ AttendArgs a,
+                                                                        const __grid_constant__ ChunkArgs c,
+                                                                        void* workspace, int dp, int64_t ctas) {
+  __shared__ int64_t scan[33];
+  ChunkWorkspace ws(workspace, dp, ctas, c.max_blocks);
+  int64_t run = 0;
+  for (int base = 0; base < a.num_seqs; base += kPlanThreads) {
+    const int seq = base + threadIdx.x;
+    int rows = 0;
+    if (seq < a.num_seqs) {
+      int len;
+      rows = chunk_tokens(a, c, seq, &len) * a.group;
+    }
+    const int n = (rows + kRows - 1) / kRows;
+    int64_t total;
+    const int64_t at = run + block_excl_scan<int64_t>(n, &total, scan);
+    // offsets that go back and forth may name more rows than there are
+    if (at + n > c.max_blocks) {
+      if (n > 0) report(a.status, KVCA_ERR_BAD_INDEX, __ldg(c.offsets + seq));
+    } else {
+      for (int b = 0; b < n; ++b)
+        ws.blocks[at + b] = ChunkBlock{seq, b * kRows, min(kRows, rows - b * kRows), 0};
+    }
+    run += total;
+  }
+  const int blocks = static_cast<int>(min(run, static_cast<int64_t>(c.max_blocks)));
+  const bool whole = run <= c.max_blocks;
+  __syncthreads();
+  run = 0;
+  for (int base = 0; base < blocks; base += kPlanThreads) {
+    const int i = base + threadIdx.x;
+    int tiles = 0;
+    if (i < blocks && whole) {
+      const ChunkBlock b = ws.blocks[i];
+      int len;
+      const int tokens = chunk_tokens(a, c, b.seq, &len);
+      tiles = (view_of(a, b.seq, b.row, b.rows, tokens, len).count + kKeys - 1) / kKeys;
+      ws.blocks[i].tiles = tiles;
+    }
+    int64_t total;
+    const int64_t before = run + block_excl_scan<int64_t>(static_cast<int64_t>(tiles) * a.kv_heads, &total, scan);
+    if (i < blocks) ws.first[i] = before;
+    run += total;
+  }
+  if (threadIdx.x == 0) {
+    ws.first[blocks] = run;
+    *ws.header = ChunkHeader{run, run < ctas ? run : ctas, blocks, 0};
+  }
+}
+
+__device__ __forceinline__ int64_t share_begin(int64_t tiles, int64_t ctas, int64_t c) { return tiles * c / ctas; }
+
+// ---------------------------------------------------------------------------
+// Barriers and tensor memory
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ void barrier_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void barrier_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+
+// Waits for a phase; gives up, as every other warp of the CTA then does, after
+// kWaitTries tries (a try suspends the thread for a while) or once another
+// warp gave up.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* abort, int64_t* status) {
+  for (uint32_t i = 0; i < kWaitTries; ++i) {
+    if (barrier_try(bar, parity)) return true;
+    if ((i & 255u) == 255u && *abort) return false;
+  }
+  *abort = 1;
+  report(status, KVCA_ERR_DEVICE_TIMEOUT, blockIdx.x);
+  return false;
+}
+
+// The same for a whole warp: every lane waits, and all go on or none.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort, int64_t* status) {
+  return __all_sync(0xffffffffu, barrier_wait(bar, parity, abort, status));
+}
+
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Arrives on `bar` when the tensor core work issued so far is done.
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u) : "memory");
+}
+
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u) : "memory");
+}
+
+// Shared memory operand with 128-byte swizzle; 8 rows of 128 bytes are 1 KiB.
+// K-major (queries, keys): groups of 8 rows 1 KiB apart.  MN-major (values:
+// tokens are the reduced dim): groups of 8 tokens 1 KiB apart, 64 dims
+// `leading` bytes apart.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t leading) {
+  return static_cast<uint64_t>((addr >> 4) & 0x3fffu) | (static_cast<uint64_t>(leading >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// fp32 accumulators; both operands fp16 or both bf16; m x n.
+__device__ __forceinline__ constexpr uint32_t mma_shape(bool bf16, int m, int n, bool values) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (values ? 1u << 16 : 0u) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// 32 columns of this warp's 32 lanes: a thread gets its lane's.
+__device__ __forceinline__ void tmem_load32(float (&r)[32], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+        "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(addr));
+}
+
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const float (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+      "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]), "f"(r[8]), "f"(r[9]),
+      "f"(r[10]), "f"(r[11]), "f"(r[12]), "f"(r[13]), "f"(r[14]), "f"(r[15]), "f"(r[16]), "f"(r[17]), "f"(r[18]),
+      "f"(r[19]), "f"(r[20]), "f"(r[21]), "f"(r[22]), "f"(r[23]), "f"(r[24]), "f"(r[25]), "f"(r[26]), "f"(r[27]),
+      "f"(r[28]), "f"(r[29]), "f"(r[30]), "f"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// Keeps the uses of loaded values behind the wait before this.
+__device__ __forceinline__ void tmem_landed(float (&r)[32]) {
+  asm volatile(""
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+                 "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
+                 "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]),
+                 "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]),
+                 "+f"(r[30]), "+f"(r[31]));
+}
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---------------------------------------------------------------------------
+// The CTA's share of the tiles, segment by segment
+// ---------------------------------------------------------------------------
+
+struct Share {
+  int64_t left;    // tiles of the share from here on
+  int block, head;
+  int tile;        // first tile of the segment that is this CTA's
+  int tiles;       // of the segment
+  int end;         // past the last tile that is this CTA's
+  BlockView view;
+  int64_t out_row;  // the chunk's first row of query and out
+
+  __device__ __forceinline__ void load(const AttendArgs& a, const ChunkArgs& c, const ChunkWorkspace& ws) {
+    const ChunkBlock b = ws.blocks[block];
+    out_row = __ldg(c.offsets + b.seq);
+    const int tokens = static_cast<int>(__ldg(c.offsets + b.seq + 1) - out_row);
+    view = view_of(a, b.seq, b.row, b.rows, tokens, sequence_length(a, b.seq));
+    tiles = b.tiles;
+    end = static_cast<int>(min(static_cast<int64_t>(tiles), tile + left));
+  }
+  // To the next segment; false when the share is done.
+  __device__ __forceinline__ bool next(const AttendArgs& a, const ChunkArgs& c, const ChunkWorkspace& ws) {
+    left -= end - tile;
+    if (left <= 0) return false;
+    tile = 0;
+    if (++head == a.kv_heads) {
+      head = 0;
+      do {
+        ++block;
+      } while (ws.blocks[block].tiles == 0);
+      load(a, c, ws);
+    }
+    end = static_cast<int>(min(static_cast<int64_t>(tiles), left));
+    return true;
+  }
+  __device__ __forceinline__ int row_tiles() const { return view.rows > 128 ? 2 : 1; }
+};
+
+// A row whose output is not finite although its sum is: the tensor cores
+// multiplied a key that another row of the block sees, with an infinity or NaN
+// among its values, by this row's zero.  The warp sums the row again over the
+// keys that it sees alone.
+template <typename Cache>
+__device__ __forceinline__ void row_again(const AttendArgs& a, const ChunkArgs& c, const Share& s, int row, float base,
+                                       float unit, float* sum) {
+  const int lane = threadIdx.x & 31;
+  const int token = row / a.group, head = s.head * a.group + row % a.group;
+  const int p = s.view.context + token;
+  const uint16_t* q = static_cast<const uint16_t*>(a.query) + (s.out_row + token) * a.query_row + head * a.query_head;
+  const int v_last = p - s.view.skip;
+  const int v_low = a.window > 0 ? p - a.window - s.view.skip : -1;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  const bool bf16 = a.query_type == KVCA_TYPE_BF16;
+  const int v_end = min(s.view.count, s.end * kKeys);
+  for (int v = s.tile * kKeys; v < v_end; ++v) {
+    if (v > v_last || (v >= a.sinks && v <= v_low)) continue;
+    const int key = s.view.key(v);
+    const int block = key / a.block_size;
+    const int64_t page = __ldg(a.tables + static_cast<int64_t>(s.view.seq) * a.table_stride + block);
+    if (page < 0 || page >= a.num_blocks) continue;
+    const int offset = key - block * a.block_size;
+    const char* k = a.key + page * a.key_block + offset * a.key_token + s.head * a.key_head;
+    const char* x = a.value + page * a.value_block + offset * a.value_token + s.head * a.value_head;
+    auto element = [&](const char* base_ptr, int d) {
+      if constexpr (Cache::kBytes == 1) {
+        return unpack2<false>(e4m3_to_f16x2(reinterpret_cast<const uint8_t*>(base_ptr)[d])).x;
+      } else {
+        return unpack2<Cache::kBf16>(reinterpret_cast<const uint16_t*>(base_ptr)[d]).x;
+      }
+    };
+    float dot = 0.f;
+    for (int d = lane; d < a.dim; d += 32)
+      dot += (bf16 ? unpack2<true>(q[d]).x : unpack2<false>(q[d]).x) * element(k, d);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    const float w = exp2_approx(dot * unit - base);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (lane + 32 * j < a.dim) acc[j] += w * element(x, lane + 32 * j);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sum[j] = acc[j];
+}
+
+template <typename Cache, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+    attend_chunk_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ ChunkArgs c, void* workspace) {
+  using Shape = ChunkShape<DP>;
+  constexpr bool kBf16 = Cache::kBf16;
+  constexpr bool kE4m3 = Cache::kBytes == 1;
+  constexpr int kStages = Shape::kStages;
+  constexpr int kTileBytes = Shape::kTileBytes;
+  extern __shared__ unsigned char dynamic[];
+  __shared__ uint64_t bars[2 * kStages + 9];
+  __shared__ float row_unit[kRows];
+  __shared__ uint32_t tmem_base;
+  __shared__ int start_block;
+  __shared__ int abort_flag;
+
+  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  const uint32_t smem = (smem_addr(dynamic) + 1023u) & ~1023u;
+  unsigned char* const smem_ptr = dynamic + (smem - smem_addr(dynamic));
+  const uint32_t kv_smem = smem + 2 * kTileBytes;
+  const uint32_t full = smem_addr(bars), empty = full + 8 * kStages;
+  const uint32_t q_full = empty + 8 * kStages, q_empty = q_full + 8;
+  const uint32_t s_full = q_full + 16, p_ready = q_full + 32, o_full = q_full + 48;
+  const uint32_t drained = q_full + 64;
+  volatile int* const abort = &abort_flag;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      barrier_init(full + 8 * i, 128);
+      barrier_init(empty + 8 * i, 1);
+    }
+    barrier_init(q_full, 128);
+    barrier_init(q_empty, 1 + kRows);
+    for (int i = 0; i < 2; ++i) {
+      barrier_init(s_full + 8 * i, 1);
+      barrier_init(p_ready + 8 * i, 128);
+      barrier_init(o_full + 8 * i, 1);
+    }
+    barrier_init(drained, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    abort_flag = 0;
+    start_block = 0;
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_base))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // Padded dims stay zero: no copy writes them.
+  const int row_chunks = a.dim / 8;  // 16-byte chunks of 16-bit values
+  if (row_chunks < DP / 8)
+    for (int i = threadIdx.x; i < (kStages + 2) * kTileBytes / 16; i += kThreads)
+      reinterpret_cast<uint4*>(smem_ptr)[i] = make_uint4(0, 0, 0, 0);
+  fence_async_proxy();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  ChunkWorkspace ws(workspace, DP, gridDim.x, c.max_blocks);
+  const ChunkHeader plan = *ws.header;
+  const bool working = blockIdx.x < plan.ctas;
+  const int64_t begin = working ? share_begin(plan.tiles, plan.ctas, blockIdx.x) : 0;
+  const int64_t share = working ? share_begin(plan.tiles, plan.ctas, blockIdx.x + 1) - begin : 0;
+  __syncthreads();
+  if (working)
+    for (int i = threadIdx.x; i < plan.blocks; i += kThreads)
+      if (ws.first[i] <= begin && begin < ws.first[i + 1]) start_block = i;
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = tmem_base;
+
+  Share s;
+  if (working) {
+    s.left = share;
+    s.block = start_block;
+    const int64_t rest = begin - ws.first[s.block];
+    const int tiles = ws.blocks[s.block].tiles;
+    s.head = static_cast<int>(rest / tiles);
+    s.tile = static_cast<int>(rest - static_cast<int64_t>(s.head) * tiles);
+    s.load(a, c, ws);
+  }
+
+  if (warp >= 12) {
+    // ------------------------------------------------------------------ MMA
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 12 && lane == 0 && working) {
+      constexpr uint32_t kScores = mma_shape(kBf16, 128, kKeys, false);
+      constexpr uint32_t kOutput = mma_shape(kBf16, 128, DP, true);
+      uint32_t used = 0;      // ring entries consumed
+      uint32_t segment = 0;
+      uint32_t p_phase[2] = {0, 0};
+      bool ok = true;
+      auto stage_of = [&](uint32_t n) { return n % kStages; };
+      auto wait_full = [&](uint32_t n) {
+        ok = ok && barrier_wait(full + 8 * stage_of(n), (n / kStages) & 1, abort, a.status);
+        fence_after_sync();
+      };
+      auto scores = [&](int q, uint32_t n) {  // S_q = Q_q K^T, K in ring entry n
+        const uint32_t keys = kv_smem + stage_of(n) * kTileBytes;
+        const uint32_t queries = smem + q * kTileBytes;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint32_t at = (k >> 2) * (kKeys * 128) + (k & 3) * 32;
+          mma_ss(tmem + q * 128, operand(queries + at, 16), operand(keys + at, 16), kScores, k > 0);
+        }
+        mma_commit(s_full + 8 * q);
+      };
+      do {
+        const int n = s.end - s.tile;
+        const int row_tiles = s.row_tiles();
+        ok = ok && barrier_wait(q_full, segment & 1, abort, a.status);
+        wait_full(used);
+        if (!ok) break;
+        for (int q = 0; q < row_tiles; ++q) scores(q, used);
+        mma_commit(empty + 8 * stage_of(used));
+        ++used;
+        for (int i = 0; i < n && ok; ++i) {
+          const uint32_t values_at = used, keys_at = used + 1;
+          const bool more = i + 1 < n;
+          wait_full(values_at);
+          for (int q = 0; q < row_tiles; ++q) {
+            ok = ok && barrier_wait(p_ready + 8 * q, p_phase[q] & 1, abort, a.status);
+            ++p_phase[q];
+            if (more && q == 0) wait_full(keys_at);
+            if (!ok) break;
+            fence_after_sync();
+            const uint32_t values = kv_smem + stage_of(values_at) * kTileBytes;
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k)
+              mma_ts(tmem + 256 + q * 128, tmem + q * 128 + k * 8, operand(values + k * 2048, kKeys * 128), kOutput,
+                     i > 0 || k > 0);
+            if (more)
+              scores(q, keys_at);
+            else
+              mma_commit(o_full + 8 * q);
+          }
+          if (!ok) break;
+          mma_commit(empty + 8 * stage_of(values_at));
+          if (more) mma_commit(empty + 8 * stage_of(keys_at));
+          used += more ? 2 : 1;
+        }
+        if (ok) mma_commit(q_empty);
+        ++segment;
+      } while (ok && s.next(a, c, ws));
+      if (!ok) {
+        // what was issued may still run: let it end before the memory goes
+        mma_commit(drained);
+        for (uint32_t i = 0; i < 4096 && !barrier_try(drained, 0); ++i) {
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 8) {
+    // ---------------------------------------------------------------- loads
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (working) {
+      const int w = warp - 8;
+      constexpr int kRowChunks = DP / 8;             // of a row in shared memory
+      constexpr int kPerInstr = 32 / kRowChunks;     // rows per instruction (16-bit rows)
+      const int chunk = lane % kRowChunks, sub = lane / kRowChunks;
+      // Where 16-byte chunk `ch` of row r of a tile lies.
+      auto place = [](int r, int ch) {
+        return static_cast<uint32_t>((ch >> 3) * (kKeys * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+      };
+      bool ok = true;
+      uint32_t issued = 0, arrived = 0;
+      uint32_t segment = 0;
+      constexpr uint32_t kAhead = 2;  // tiles in flight behind the one being issued
+      auto complete = [&]() {
+        fence_async_proxy();
+        barrier_arrive(full + 8 * (arrived % kStages));
+        ++arrived;
+      };
+      auto drain = [&]() {
+        while (arrived < issued) {
+          if (issued - arrived == kAhead)
+            cp_async_wait<kAhead - 1>();
+          else
+            cp_async_wait<0>();
+          complete();
+        }
+      };
+      // The ring entry of the next tile.  Before it waits for one, a warp
+      // hands over what it has in flight.
+      auto claim = [&]() {
+        if (issued < kStages || !ok) return;
+        const uint32_t bar = empty + 8 * (issued % kStages), parity = ((issued / kStages) - 1) & 1;
+        if (__all_sync(0xffffffffu, barrier_try(bar, parity))) return;
+        if constexpr (!kE4m3) drain();
+        ok = warp_wait(bar, parity, abort, a.status);
+      };
+      constexpr int64_t kHidden = -1ll << 62;
+      do {
+        // queries, through registers: the sign of a negative scale, the
+        // zeros of a zero one, or (e4m3) a power of two per row goes into them
+        if (segment > 0) ok = ok && warp_wait(q_empty, (segment - 1) & 1, abort, a.status);
+        if (!ok) break;
+        for (int r0 = w * 64; r0 < w * 64 + 64; r0 += kPerInstr) {
+          const int r = r0 + sub;
+          const int row = s.view.row + r;
+          const bool live = r < s.view.rows && chunk < row_chunks;
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (live) {
+            const int token = row / a.group;
+            const uint16_t* src = static_cast<const uint16_t*>(a.query) + (s.out_row + token) * a.query_row +
+                                  static_cast<int64_t>(s.head * a.group + row - token * a.group) * a.query_head;
+            x = __ldg(reinterpret_cast<const uint4*>(src) + chunk);
+          }
+          uint32_t* const word = reinterpret_cast<uint32_t*>(&x);
+          if constexpr (kE4m3) {
+            const bool bf16 = a.query_type == KVCA_TYPE_BF16;
+            float2 f[4];
+            float big = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              f[j] = bf16 ? unpack2<true>(word[j]) : unpack2<false>(word[j]);
+              big = fmaxf(big, fmaxf(fabsf(f[j].x), fabsf(f[j].y)));
+            }
+#pragma unroll
+            for (int o = kRowChunks / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+            const int e = big > 0.f && big < INFINITY ? min(max(12 - ilogbf(big), -120), 120) : 0;
+            const float up = ldexpf(1.f, e);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) word[j] = pack2<false>(f[j].x * up, f[j].y * up);
+            if (chunk == 0) row_unit[r] = c.scale_log2 * ldexpf(1.f, -e);
+          } else {
+            if (chunk == 0) row_unit[r] = c.scale_log2;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) word[j] = (word[j] & c.query_and) ^ c.query_xor;
+          if (chunk < row_chunks)
+            *reinterpret_cast<uint4*>(smem_ptr + (r >> 7) * kTileBytes + place(r & 127, chunk)) = x;
+        }
+        fence_async_proxy();
+        barrier_arrive(q_full);
+
+        // keys and values, tile by tile; a lane looks up the page of one token
+        int64_t page;
+        int offset = 0;
+        auto look_up = [&](int tile) {
+          const int v = tile * kKeys + w * 32 + lane;
+          page = kHidden;
+          if (v < s.view.count) {
+            const int key = s.view.key(v);
+            const int block = a.block_shift >= 0 ? key >> a.block_shift : key / a.block_size;
+            offset = key - block * a.block_size;
+            page = __ldg(a.tables + static_cast<int64_t>(s.view.seq) * a.table_stride + block);
+          }
+        };
+        look_up(s.tile);
+        for (int tile = s.tile; tile < s.end && ok; ++tile) {
+          const char* rows[2] = {nullptr, nullptr};
+          if (page >= 0 && page < a.num_blocks) {
+            rows[0] = a.key + page * a.key_block + offset * a.key_token + s.head * a.key_head;
+            rows[1] = a.value + page * a.value_block + offset * a.value_token + s.head * a.value_head;
+          } else if (page != kHidden) {
+            report(a.status, KVCA_ERR_BAD_INDEX, page);  // its rows read as zeros
+          }
+          if (tile + 1 < s.end) look_up(tile + 1);
+#pragma unroll
+          for (int side = 0; side < 2; ++side) {
+            const unsigned long long row = reinterpret_cast<unsigned long long>(rows[side]);
+            if constexpr (!kE4m3) {
+              claim();
+              if (!ok) break;
+              const uint32_t dst = kv_smem + (issued % kStages) * kTileBytes;
+#pragma unroll
+              for (int r = 0; r < 32; r += kPerInstr) {
+                const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, r + sub));
+                if (chunk < row_chunks)
+                  cp_async16(dst + place(w * 32 + r + sub, chunk), src != nullptr ? src + chunk * 16 : a.key,
+                             src != nullptr);
+              }
+              cp_async_commit();
+              ++issued;
+              if (issued - arrived > kAhead) {
+                cp_async_wait<kAhead>();
+                complete();
+              }
+            } else {
+              // 16 e4m3 values per load become two chunks
+              constexpr int kLoads = kRowChunks / 2;       // per row
+              constexpr int kRowsPer = 32 / kLoads;
+              const int part = lane % kLoads, which = lane / kLoads;
+              uint4 x[32 / kRowsPer];
+#pragma unroll
+              for (int i = 0; i < 32 / kRowsPer; ++i) {
+                const char* src =
+                    reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, i * kRowsPer + which));
+                x[i] = src != nullptr && part * 16 < a.dim ? __ldg(reinterpret_cast<const uint4*>(src) + part)
+                                                           : make_uint4(0, 0, 0, 0);
+              }
+              claim();
+              if (!ok) break;
+              unsigned char* const dst = smem_ptr + 2 * kTileBytes + (issued % kStages) * kTileBytes;
+#pragma unroll
+              for (int i = 0; i < 32 / kRowsPer; ++i) {
+                const int r = w * 32 + i * kRowsPer + which;
+                const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                uint32_t wide[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  wide[2 * j] = e4m3_to_f16x2(in[j]);
+                  wide[2 * j + 1] = e4m3_to_f16x2(in[j] >> 16);
+                }
+                *reinterpret_cast<uint4*>(dst + place(r, 2 * part)) = make_uint4(wide[0], wide[1], wide[2], wide[3]);
+                *reinterpret_cast<uint4*>(dst + place(r, 2 * part + 1)) =
+                    make_uint4(wide[4], wide[5], wide[6], wide[7]);
+              }
+              ++issued;
+              complete();
+            }
+          }
+        }
+        // what is still in flight: its readers may have to finish before this
+        // segment's queries leave
+        if constexpr (!kE4m3) {
+          drain();
+        }
+        ++segment;
+      } while (ok && s.next(a, c, ws));
+      cp_async_wait<0>();
+    }
+  } else {
+    // -------------------------------------------------------------- softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    const int q = warp >> 2;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t scores = tmem + lanes + q * 128, output = tmem + lanes + 256 + q * 128;
+    const int r = q * 128 + (warp & 3) * 32 + lane;  // this thread's row of the block
+    ChunkPiece piece{-1, -1, -1, 0};
+    if (working) {
+      bool ok = true;
+      uint32_t segment = 0, phase = 0, o_phase = 0;
+      int64_t done = 0;  // tiles of the share before this segment
+      do {
+        ok = ok && warp_wait(q_full, segment & 1, abort, a.status);
+        if (!ok) break;
+        const float unit = row_unit[r];
+        barrier_arrive(q_empty);
+        const int n = s.end - s.tile;
+        const bool starts = s.tile == 0, ends = s.end == s.tiles;
+        if (q < s.row_tiles()) {
+          // what this row sees, in numbers of the block's keys
+          const int own = min(s.view.row + r, s.view.row + s.view.rows - 1);
+          const int p = s.view.context + own / a.group;
+          const int v_last = p - s.view.skip;
+          const int v_low = a.window > 0 ? p - a.window - s.view.skip : -1;
+          // the same for the tile's first and last row
+          const int row_first = s.view.row + q * 128, row_last = min(row_first + 127, s.view.row + s.view.rows - 1);
+          const int all_last = s.view.context + row_first / a.group - s.view.skip;
+          const int all_low = a.window > 0 ? s.view.context + row_last / a.group - a.window - s.view.skip : -1;
+
+          float m = -INFINITY, l = 0.f;  // m in units of the raw scores
+          for (int i = 0; i < n; ++i) {
+            ok = ok && warp_wait(s_full + 8 * q, phase & 1, abort, a.status);
+            if (!ok) break;
+            ++phase;
+            fence_after_sync();
+            float x[4][32];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) tmem_load32(x[j], scores + j * 32);
+            tmem_wait_load();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) tmem_landed(x[j]);
+            const int v0 = (s.tile + i) * kKeys;
+            if (v0 + kKeys - 1 > all_last || (v0 + kKeys > a.sinks && max(v0, a.sinks) <= all_low)) {
+              const int last = v_last - v0, low = v_low - v0, sinks = a.sinks - v0;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                  const int v = j * 32 + k;
+                  if (v > last || (v <= low && v >= sinks)) x[j][k] = -INFINITY;
+                }
+            }
+            float top[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              top[j] = x[j][0];
+#pragma unroll
+              for (int k = 1; k < 32; ++k) top[j] = fmaxf(top[j], x[j][k]);
+            }
+            const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            const float old = m;
+            // (-inf) - (-inf) is no growth
+            if ((best - m) * unit > kGrowth) m = best;
+            const float base = m == -INFINITY ? 0.f : m * unit;
+            const float decay = m != old ? exp2_approx(old * unit - base) : 1.f;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t packed[16];
+#pragma unroll
+              for (int k = 0; k < 32; k += 2) {
+                const float e0 = exp2_approx(fmaf(x[j][k], unit, -base));
+                const float e1 = exp2_approx(fmaf(x[j][k + 1], unit, -base));
+                sum[j] += e0 + e1;
+                packed[k >> 1] = pack2<kBf16>(e0, e1);
+              }
+              tmem_store16(scores + j * 16, packed);
+            }
+            l = l * decay + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+            if (i > 0 && __any_sync(0xffffffffu, m != old)) {
+#pragma unroll
+              for (int j = 0; j < DP / 32; ++j) {
+                float o[32];
+                tmem_load32(o, output + j * 32);
+                tmem_wait_load();
+                tmem_landed(o);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] *= decay;
+                tmem_store32(output + j * 32, o);
+              }
+            }
+            tmem_wait_store();
+            fence_before_sync();
+            barrier_arrive(p_ready + 8 * q);
+          }
+          ok = ok && warp_wait(o_full + 8 * q, o_phase & 1, abort, a.status);
+          if (!ok) break;
+          ++o_phase;
+          fence_after_sync();
+
+          const float base = m == -INFINITY ? 0.f : m * unit;
+          const bool live = r < s.view.rows;
+          const bool whole = starts && ends;
+          const float factor = whole ? a.value_scale / l : 1.f;
+          const int token = own / a.group;
+          const int64_t row = s.out_row + token;
+          const int head = s.head * a.group + own - token * a.group;
+          const int64_t out_row = row * (static_cast<int64_t>(a.kv_heads) * a.group) + head;
+          const int64_t slot = static_cast<int64_t>(blockIdx.x) * 2 + (starts ? 1 : 0);
+          float* const part = ws.acc + (slot * kRows + r) * DP;
+          uint16_t* const out = static_cast<uint16_t*>(a.out) + out_row * a.dim;
+          bool finite = true;
+#pragma unroll
+          for (int j = 0; j < DP / 32; ++j) {
+            float o[32];
+            __syncwarp();
+            tmem_load32(o, output + j * 32);
+            tmem_wait_load();
+            tmem_landed(o);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) finite &= fabsf(o[k]) < INFINITY;
+            if (live && whole) {
+              const bool bf16 = a.query_type == KVCA_TYPE_BF16;
+#pragma unroll
+              for (int k = 0; k < 32; k += 8) {
+                if (j * 32 + k >= a.dim) break;
+                uint4 w;
+                uint32_t* const word = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                  const float x0 = o[k + 2 * h] * factor, x1 = o[k + 2 * h + 1] * factor;
+                  word[h] = bf16 ? pack2<true>(x0, x1) : pack2<false>(x0, x1);
+                }
+                *reinterpret_cast<uint4*>(out + j * 32 + k) = w;
+              }
+            } else if (live) {
+#pragma unroll
+              for (int k = 0; k < 32; k += 4)
+                *reinterpret_cast<float4*>(part + j * 32 + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+            }
+          }
+          if (live) {
+            if (whole) {
+              if (a.lse != nullptr) a.lse[out_row] = base * kLn2 + logf(l);
+            } else {
+              float* const ml = ws.ml + slot * 2 * kRows;
+              ml[r] = m == -INFINITY ? -INFINITY : base;
+              ml[kRows + r] = l;
+            }
+          }
+          unsigned again = __ballot_sync(0xffffffffu, live && !finite && l < INFINITY);
+          while (again) {
+            const int who = __ffs(again) - 1;
+            again &= again - 1;
+            float sum[4];
+            const float w_base = __shfl_sync(0xffffffffu, base, who);
+            const float w_factor = __shfl_sync(0xffffffffu, factor, who);
+            const int w_row = __shfl_sync(0xffffffffu, own, who);
+            const int64_t w_out = __shfl_sync(0xffffffffu, out_row, who);
+            row_again<Cache>(a, c, s, w_row, w_base, a.scale_log2, sum);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int d = lane + 32 * j;
+              if (d >= a.dim) break;
+              if (whole) {
+                const uint32_t y = a.query_type == KVCA_TYPE_BF16 ? pack2<true>(sum[j] * w_factor, 0.f)
+                                                                  : pack2<false>(sum[j] * w_factor, 0.f);
+                static_cast<uint16_t*>(a.out)[w_out * a.dim + d] = static_cast<uint16_t>(y);
+              } else {
+                ws.acc[(slot * kRows + q * 128 + (warp & 3) * 32 + who) * DP + d] = sum[j];
+              }
+            }
+          }
+          fence_before_sync();
+        }
+        if (!(starts && ends)) {
+          const int id = s.block * a.kv_heads + s.head;
+          if (starts) {
+            piece.head = id;
+            const int64_t last = begin + done + s.tiles - 1;
+            piece.last = static_cast<int>((plan.ctas * (last + 1) - 1) / plan.tiles);
+          } else {
+            piece.tail = id;
+          }
+        }
+        done += n;
+        ++segment;
+      } while (s.next(a, c, ws));
+    }
+    if (threadIdx.x == 0 && working) ws.pieces[blockIdx.x] = piece;
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 12) {
+    fence_after_sync();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// Joins the partial results of the blocks that several CTAs share: a column
+// of blocks of the grid per CTA that began one, kJoinRows rows each.
+template <int DP>
+__global__ void __launch_bounds__(kJoinThreads) attend_chunk_join_kernel(const __grid_constant__ AttendArgs a,
+                                                                        const __grid_constant__ ChunkArgs c,
+                                                                        void* workspace, int64_t ctas) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  ChunkWorkspace ws(workspace, DP, ctas, c.max_blocks);
+  const int64_t owner = blockIdx.x;
+  if (owner >= ws.header->ctas) return;
+  const ChunkPiece own = ws.pieces[owner];
+  if (own.head < 0) return;
+  const int block = own.head / a.kv_heads, kv_head = own.head - block * a.kv_heads;
+  const ChunkBlock b = ws.blocks[block];
+  constexpr int kPerRow = kJoinThreads / kJoinRows;  // threads per row
+  const int r = blockIdx.y * kJoinRows + threadIdx.x / kPerRow;
+  if (r >= b.rows) return;
+  const int t = threadIdx.x % kPerRow;
+  float top = -INFINITY;
+  for (int64_t p = owner; p <= own.last; ++p)
+    top = fmaxf(top, __ldcg(ws.ml + (p * 2 + (p == owner)) * 2 * kRows + r));
+  const float base = top == -INFINITY ? 0.f : top;
+  constexpr int kVecs = DP / 4 / kPerRow;
+  float4 sum[kVecs];
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) sum[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float total = 0.f;
+#pragma unroll 4
+  for (int64_t p = owner; p <= own.last; ++p) {
+    const int64_t slot = p * 2 + (p == owner);
+    const float* const ml = ws.ml + slot * 2 * kRows;
+    const float w = exp2_approx(__ldcg(ml + r) - base);
+    total += w * __ldcg(ml + kRows + r);
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      const float4 o = __ldcg(reinterpret_cast<const float4*>(ws.acc + (slot * kRows + r) * DP) + t + v * kPerRow);
+      sum[v].x += w * o.x;
+      sum[v].y += w * o.y;
+      sum[v].z += w * o.z;
+      sum[v].w += w * o.w;
+    }
+  }
+  const int flat = b.row + r;
+  const int token = flat / a.group;
+  const int64_t out_row = (__ldg(c.offsets + b.seq) + token) * (static_cast<int64_t>(a.kv_heads) * a.group) +
+                          kv_head * a.group + flat - token * a.group;
+  const float factor = a.value_scale / total;
+  const bool bf16 = a.query_type == KVCA_TYPE_BF16;
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) {
+    const int d = (t + v * kPerRow) * 4;
+    if (d >= a.dim) continue;
+    uint2 w;
+    w.x = bf16 ? pack2<true>(sum[v].x * factor, sum[v].y * factor) : pack2<false>(sum[v].x * factor, sum[v].y * factor);
+    w.y = bf16 ? pack2<true>(sum[v].z * factor, sum[v].w * factor) : pack2<false>(sum[v].z * factor, sum[v].w * factor);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + out_row * a.dim + d) = w;
+  }
+  if (a.lse != nullptr && t == 0) a.lse[out_row] = base * kLn2 + logf(total);
+}
+
+template <typename Cache, int DP>
+cudaError_t launch_typed(const AttendArgs& a, const ChunkArgs& c, void* workspace, int sms, cudaStream_t stream) {
+  auto kernel = attend_chunk_kernel<Cache, DP>;
+  static DeviceFlags configured;
+  int dev = -1;
+  if (needs_setup(configured, &dev)) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkShape<DP>::kSmem);
+    if (e != cudaSuccess) return e;
+    mark_setup(configured, dev);
+  }
+  const int64_t ctas = sms;
+  attend_chunk_plan_kernel<<<1, kPlanThreads, 0, stream>>>(a, c, workspace, DP, ctas);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  e = launch_dependent(kernel, dim3(sms), kThreads, ChunkShape<DP>::kSmem, stream, a, c, workspace);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(attend_chunk_join_kernel<DP>, dim3(sms, kRows / kJoinRows), kJoinThreads, 0, stream, a, c,
+                          workspace, ctas);
+}
+
+template <typename Cache>
+cudaError_t launch_cache(const AttendArgs& a, const ChunkArgs& c, void* workspace, int sms, cudaStream_t stream) {
+  return a.dim <= 64 ? launch_typed<Cache, 64>(a, c, workspace, sms, stream)
+                     : launch_typed<Cache, 128>(a, c, workspace, sms, stream);
+}
+
+}  // namespace
+
+int64_t attend_chunk_max_blocks(const AttendArgs& a, int64_t rows) {
+  return rows * a.group / kRows + a.num_seqs;  // each sequence's last block may be short
+}
+
+size_t attend_chunk_workspace(const AttendArgs& a, int64_t rows, int sms) {
+  return ChunkWorkspace::bytes(a.dim <= 64 ? 64 : 128, sms, attend_chunk_max_blocks(a, rows));
+}
+
+cudaError_t launch_attend_chunk(const AttendArgs& args, const int64_t* offsets, int64_t rows, void* workspace, int sms,
+                                cudaStream_t stream) {
+  AttendArgs a = args;
+  ChunkArgs c;
+  c.offsets = offsets;
+  c.rows = rows;
+  c.max_blocks = static_cast<int>(attend_chunk_max_blocks(a, rows));
+  // the softmax takes the maximum of the raw scores, so their factor is positive
+  c.scale_log2 = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
+  c.query_and = a.scale_log2 == 0.f ? 0u : 0xffffffffu;
+  c.query_xor = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+  switch (a.cache_type) {
+    case KVCA_TYPE_F16: return launch_cache<CacheF16>(a, c, workspace, sms, stream);
+    case KVCA_TYPE_BF16: return launch_cache<CacheBf16>(a, c, workspace, sms, stream);
+    default: return launch_cache<CacheE4m3>(a, c, workspace, sms, stream);
+  }
+}
+
+}  // namespace kvca

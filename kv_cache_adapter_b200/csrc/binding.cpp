@@ -791,6 +791,39 @@ int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t wo
   return status_of(kvca::launch_attend_step(a, d_workspace, sms, stream));
 }
 
+namespace {
+
+int to_chunk(const kvca_attend_desc* desc, int64_t num_rows, int64_t* d_status, kvca::AttendArgs* a) {
+  const int rc = to_attend(desc, d_status, a);
+  if (rc != KVCA_OK) return rc;
+  if (num_rows < 0 || a->dim > kvca::kChunkMaxDim) return KVCA_ERR_BAD_ARGUMENT;
+  if (num_rows > (int64_t{1} << 30) / desc->q_heads) return KVCA_ERR_SIZE_LIMIT;
+  return KVCA_OK;
+}
+
+}  // namespace
+
+int64_t kvca_attend_chunk_workspace_bytes(const kvca_attend_desc* desc, int64_t num_rows) {
+  kvca::AttendArgs a;
+  if (to_chunk(desc, num_rows, nullptr, &a) != KVCA_OK) return -1;
+  return static_cast<int64_t>(kvca::attend_chunk_workspace(a, num_rows, kvca_device_sm_count()));
+}
+
+int kvca_attend_chunk(const kvca_attend_desc* desc, const int64_t* d_query_offsets, int64_t num_rows,
+                      void* d_workspace, int64_t workspace_bytes, int64_t* d_status, kvca_stream_t stream) {
+  kvca::AttendArgs a;
+  const int rc = to_chunk(desc, num_rows, d_status, &a);
+  if (rc != KVCA_OK) return rc;
+  if (a.num_seqs == 0 || num_rows == 0) return KVCA_OK;
+  if (!attend_pointers_ok(a) || d_query_offsets == nullptr) return KVCA_ERR_BAD_ARGUMENT;
+  const int sms = kvca_device_sm_count();
+  if (sms < 1) return KVCA_ERR_CUDA;
+  if (d_workspace == nullptr || !aligned16(reinterpret_cast<uint64_t>(d_workspace)) ||
+      workspace_bytes < static_cast<int64_t>(kvca::attend_chunk_workspace(a, num_rows, sms)))
+    return KVCA_ERR_BAD_ARGUMENT;
+  return status_of(kvca::launch_attend_chunk(a, d_query_offsets, num_rows, d_workspace, sms, stream));
+}
+
 int kvca_copy_paged(const kvca_paged_desc* src, const kvca_paged_desc* dst, int64_t num_planes,
                     int64_t num_rows, int64_t row_bytes, int32_t flags, int64_t* d_status,
                     kvca_stream_t stream) {

@@ -146,8 +146,23 @@ struct AttendArgs {
   int64_t* status;
 };
 
+// What a chunk call adds; the scores' factor without its sign, which goes
+// into the queries (query bits & query_and, ^ query_xor).
+struct ChunkArgs {
+  const int64_t* offsets;  // num_seqs + 1
+  int64_t rows;            // of query
+  int max_blocks;          // blocks that the offsets can make of them
+  float scale_log2;
+  uint32_t query_and, query_xor;
+};
+
 size_t attend_step_workspace(const AttendArgs& args, int sms);
 cudaError_t launch_attend_step(const AttendArgs& args, void* workspace, int sms, cudaStream_t stream);
+
+constexpr int kChunkMaxDim = 128;  // two output tiles fill the tensor memory
+size_t attend_chunk_workspace(const AttendArgs& args, int64_t rows, int sms);
+cudaError_t launch_attend_chunk(const AttendArgs& args, const int64_t* offsets, int64_t rows, void* workspace, int sms,
+                                cudaStream_t stream);
 
 cudaError_t launch_inspect_load(int meta_bits, const int64_t* l2p, int64_t num_logical,
                                 const void* meta, int64_t num_slots, const int64_t* ids,

@@ -54,6 +54,7 @@ __all__ = [
     "move_cycle",
     "exchange_blocks",
     "attend_step",
+    "attend_chunk",
     "batched_fused_single_layer_kv_transfer",
     "load_device_store",
     "save_device_store",
@@ -1398,6 +1399,44 @@ def attend_step(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
                                           _stream(dev))
     _host_rc(rc, "attend_step")
     _maybe_check(dev, check, "attend_step")
+    return out
+
+
+def attend_chunk(query: torch.Tensor, query_offsets: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                 block_tables: torch.Tensor, seq_lens: torch.Tensor, *, scale: float | None = None,
+                 window: int | None = None, sinks: int = 0, key_scale: float = 1.0, value_scale: float = 1.0,
+                 out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                 check: bool | None = None) -> torch.Tensor:
+    """Attention of a ragged chunk of new tokens per sequence over the paged
+    cache (kvca_attend_chunk): prompts, pieces of them, drafted tokens.
+    ``query`` ``(rows, heads, head_dim)``, head_dim at most 128; rows
+    ``query_offsets[s]:query_offsets[s + 1]`` (int64, ``num_seqs + 1``) are
+    the last tokens of sequence s, whose K and V the cache holds already
+    (``seq_lens`` counts them).  Each row sees the tokens up to its own, with
+    ``window`` only the last ``window`` of them and the first ``sinks`` of the
+    sequence.  The other arguments and ``lse`` are ``attend_step``'s.  Rows
+    outside the offsets, and those of a sequence of negative length, are left
+    as they were."""
+    desc, out = _attend_desc(query, key_cache, value_cache, block_tables, seq_lens, scale, window, sinks, key_scale,
+                             value_scale, out, lse)
+    if query.shape[2] > 128:
+        raise ValueError(f"head_dim must be at most 128, got {query.shape[2]}")
+    dev = query.device
+    _require_index(query_offsets, dev, "query_offsets")
+    if query_offsets.numel() != seq_lens.shape[0] + 1:
+        raise ValueError("query_offsets must have num_seqs + 1 entries")
+    rows = query.shape[0]
+    if rows == 0 or seq_lens.shape[0] == 0:
+        return out
+    with _on(dev):
+        need = _lib_handle.kvca_attend_chunk_workspace_bytes(ctypes.byref(desc), rows)
+        if need < 0:
+            _raise_for(_lib.KVCA_ERR_BAD_ARGUMENT, 0, "attend_chunk")
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        rc = _lib_handle.kvca_attend_chunk(ctypes.byref(desc), query_offsets.data_ptr(), rows, workspace.data_ptr(),
+                                           need, _ptr(_status(dev)), _stream(dev))
+    _host_rc(rc, "attend_chunk")
+    _maybe_check(dev, check, "attend_chunk")
     return out
 
 
