@@ -600,6 +600,99 @@ int kvca_move_cycle(const kvca_chunk_desc* tokens, const kvca_paged_desc* token_
                     kvca_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* Pages of sequences                                                        */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Sequences that own pages of the cache: row s of block_tables (int64,
+ * table_stride apart, table_width wide) names the slots of the pages of
+ * sequence s in order, ceil(seq_lens[s] / block_size) of them; a negative
+ * entry is a page given back (behind a window).  A sequence of length 0 or
+ * less owns none.  The slot pool is the one of the metadata operators above;
+ * a slot's pin count is the number of its holders, so every page of a
+ * sequence is pinned, once per sequence that shares it.
+ */
+typedef struct kvca_page_pool {
+  int32_t meta_bits;
+  int32_t reserved;
+  void* slot_meta;
+  int64_t num_slots;
+  int64_t* l2p;
+  int64_t num_logical;
+  int64_t* p2l;
+  int64_t* block_tables;
+  int64_t table_stride;
+  int64_t table_width;
+  int64_t* seq_lens;
+  int64_t num_seqs;
+  int64_t block_size;
+} kvca_page_pool;
+
+/*
+ * Sequence children[j] becomes a copy of sequence parents[j] (count pairs, a
+ * parent may repeat).  The parent's full pages are shared: the child's table
+ * names the same slots and their pin counts rise by one.  A partly filled
+ * last page is not shared: its filled token rows are copied, in every plane
+ * of `cache`, to slot fresh_slots[j] (unpinned, as kvca_pop_reusable_slots
+ * hands them out), which is committed as kvca_commit_save_metadata does: its
+ * old logical id unmapped, logical id fresh_ids[j] mapped to it, pin 1, usage
+ * 1.  Without such a page fresh_slots[j] and fresh_ids[j] are not used.  The
+ * child gets the parent's length.
+ * Everything is checked before anything changes.  KVCA_ERR_BAD_INDEX: a
+ * sequence, slot or id outside its table, a length that the table cannot
+ * hold.  KVCA_ERR_BAD_ARGUMENT (value: the sequence, slot or id): a child
+ * that is not empty, is listed twice or is a parent; a parent of negative
+ * length; a used fresh slot that is pinned or listed twice; a fresh id that is
+ * mapped or listed twice; a page that is not pinned or whose pin count is at
+ * its maximum.  Either leaves all as it was (d_status must be given).
+ * cache: the token view (block_size tokens per block, num_blocks = num_slots,
+ * index unused).  count <= 64,512, table_width <= 2^25.  workspace:
+ * kvca_fork_workspace_bytes(count, table_width) bytes of device memory, 16-byte
+ * aligned, any contents; one for each call that may overlap another.  No
+ * reference counterpart as one call.
+ */
+size_t kvca_fork_workspace_bytes(int64_t count, int64_t table_width);
+int kvca_fork_sequences(const kvca_page_pool* pool, const int64_t* d_parents, const int64_t* d_children,
+                        const int64_t* d_fresh_slots, const int64_t* d_fresh_ids, int64_t count,
+                        const kvca_paged_desc* cache, int64_t num_planes, int64_t row_bytes, void* d_workspace,
+                        int64_t workspace_bytes, int64_t* d_status, kvca_stream_t stream);
+
+/*
+ * The sequences d_sequences[count] (distinct) give their pages back: each
+ * page's pin count falls by one per sequence that held it, the table entries
+ * become -1 and the lengths 0.  A page that nobody holds any more stays
+ * resident for kvca_pop_reusable_slots to evict, or, with `discard`, is
+ * unmapped (its logical id, the slot's id and its word cleared).  Sequences
+ * that own no pages are left as they are.  Everything is checked before
+ * anything changes: KVCA_ERR_BAD_INDEX (a sequence or slot outside its table,
+ * a length that the table cannot hold), KVCA_ERR_BAD_ARGUMENT (a sequence
+ * listed twice, a page that is not pinned as often as the call's sequences
+ * name it).  Limits and workspace as for the fork.  No reference counterpart
+ * as one call (kvca_release_metadata per sequence).
+ */
+size_t kvca_free_workspace_bytes(int64_t count, int64_t table_width);
+int kvca_free_sequences(const kvca_page_pool* pool, const int64_t* d_sequences, int64_t count, int32_t discard,
+                        void* d_workspace, int64_t workspace_bytes, int64_t* d_status, kvca_stream_t stream);
+
+/*
+ * The live slots (p2l >= 0 or pinned; K of them) move into the first K slots:
+ * the live slots from K on go, in order, to the dead slots below K, in order.
+ * Their bytes move in every plane of `cache`, slot_meta, p2l and l2p with
+ * them, and the entries of every sequence's pages in block_tables are
+ * renamed.  The slots they leave are empty (p2l -1, word 0), so a pool can
+ * give its tail back.  d_remap[slot] is each live slot's new place (its own
+ * when it stays), -1 for dead ones; *d_live = K.  search_start needs no
+ * change.  A table entry outside the pool gives KVCA_ERR_BAD_INDEX and is left
+ * as it is; so is a logical id outside its table.  num_slots < 2^31.
+ * workspace: kvca_compact_workspace_bytes(num_slots), as for the fork.  No
+ * reference counterpart.
+ */
+size_t kvca_compact_workspace_bytes(int64_t num_slots);
+int kvca_compact_pages(const kvca_page_pool* pool, const kvca_paged_desc* cache, int64_t num_planes,
+                       int64_t row_bytes, int64_t* d_remap, int64_t* d_live, void* d_workspace,
+                       int64_t workspace_bytes, int64_t* d_status, kvca_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* Attention over the paged cache                                            */
 /* ------------------------------------------------------------------------ */
 

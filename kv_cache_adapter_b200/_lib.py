@@ -104,6 +104,26 @@ class AdapterSession(ctypes.Structure):
     ]
 
 
+class PagePool(ctypes.Structure):
+    """kvca_page_pool."""
+
+    _fields_ = [
+        ("meta_bits", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("slot_meta", c_ptr),
+        ("num_slots", c_i64),
+        ("l2p", c_ptr),
+        ("num_logical", c_i64),
+        ("p2l", c_ptr),
+        ("block_tables", c_ptr),
+        ("table_stride", c_i64),
+        ("table_width", c_i64),
+        ("seq_lens", c_ptr),
+        ("num_seqs", c_i64),
+        ("block_size", c_i64),
+    ]
+
+
 class AttendDesc(ctypes.Structure):
     """kvca_attend_desc."""
 
@@ -245,6 +265,21 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [ctypes.POINTER(ChunkDesc), ctypes.POINTER(PagedDesc), c_i64, c_i64, c_i64, ctypes.POINTER(PagedDesc),
          ctypes.POINTER(ChunkDesc), c_i64, c_i64, c_i64, ctypes.c_int32, ctypes.c_int32, c_ptr, c_ptr],
+    ),
+    "kvca_fork_workspace_bytes": (ctypes.c_size_t, [c_i64, c_i64]),
+    "kvca_fork_sequences": (
+        c_int,
+        [ctypes.POINTER(PagePool), c_ptr, c_ptr, c_ptr, c_ptr, c_i64, ctypes.POINTER(PagedDesc), c_i64, c_i64, c_ptr,
+         c_i64, c_ptr, c_ptr],
+    ),
+    "kvca_free_workspace_bytes": (ctypes.c_size_t, [c_i64, c_i64]),
+    "kvca_free_sequences": (
+        c_int, [ctypes.POINTER(PagePool), c_ptr, c_i64, ctypes.c_int32, c_ptr, c_i64, c_ptr, c_ptr],
+    ),
+    "kvca_compact_workspace_bytes": (ctypes.c_size_t, [c_i64]),
+    "kvca_compact_pages": (
+        c_int,
+        [ctypes.POINTER(PagePool), ctypes.POINTER(PagedDesc), c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_ptr],
     ),
     "kvca_attend_step_workspace_bytes": (c_i64, [ctypes.POINTER(AttendDesc)]),
     "kvca_attend_step": (c_int, [ctypes.POINTER(AttendDesc), c_ptr, c_i64, c_ptr, c_ptr]),

@@ -21,8 +21,8 @@ PKG = pathlib.Path(__file__).resolve().parent
 REPO = PKG.parent
 CSRC = PKG / "csrc"
 INCLUDE = REPO / "include"
-SOURCES = [CSRC / "kv_adapter_cuda.cu", CSRC / "attend_step.cu", CSRC / "attend_chunk.cu", CSRC / "row_ceiling.cu",
-           CSRC / "binding.cpp"]
+SOURCES = [CSRC / "kv_adapter_cuda.cu", CSRC / "attend_step.cu", CSRC / "attend_chunk.cu", CSRC / "page_ops.cu",
+           CSRC / "row_ceiling.cu", CSRC / "binding.cpp"]
 HEADERS = [CSRC / "kvca_launch.h", CSRC / "kvca_device.cuh", CSRC / "kvca_host.cuh", CSRC / "attend_common.cuh",
            INCLUDE / "kvca.h"]
 TARGET = PKG / "libkvca_b200.so"

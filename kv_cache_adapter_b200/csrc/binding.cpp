@@ -770,6 +770,115 @@ int kvca_move_cycle(const kvca_chunk_desc* tokens, const kvca_paged_desc* token_
   return status_of(kvca::launch_move_cycle(a, stream));
 }
 
+namespace {
+
+int to_pages(const kvca_page_pool* p, int64_t* d_status, kvca::PagePool* pool, kvca::PageTable* table) {
+  if (p == nullptr || !valid_meta_bits(p->meta_bits) || p->num_slots < 0 || p->num_logical < 0 || p->table_width < 0 ||
+      p->table_stride < 0 || p->num_seqs < 0 || p->block_size < 1 ||
+      (p->num_seqs > 1 && p->table_stride < p->table_width))
+    return KVCA_ERR_BAD_ARGUMENT;
+  if (p->num_slots >= (int64_t{1} << 31) || p->table_width > (int64_t{1} << 25) || p->block_size > (int64_t{1} << 30) ||
+      p->num_seqs >= (int64_t{1} << 31))
+    return KVCA_ERR_SIZE_LIMIT;
+  *pool = kvca::PagePool{p->slot_meta, p->num_slots, p->l2p, p->num_logical, p->p2l, d_status};
+  *table = kvca::PageTable{p->block_tables, p->table_stride, p->table_width, p->seq_lens, p->num_seqs, p->block_size};
+  return KVCA_OK;
+}
+
+bool page_pointers_ok(const kvca::PagePool& pool, const kvca::PageTable& t) {
+  return (pool.num_slots == 0 || (pool.slot_meta != nullptr && pool.p2l != nullptr)) &&
+         (pool.num_logical == 0 || pool.l2p != nullptr) &&
+         (t.num_seqs == 0 || (t.lens != nullptr && (t.width == 0 || t.tables != nullptr)));
+}
+
+// The cache side of a page operator: whole blocks of block_size token rows.
+bool check_pages(const kvca_paged_desc* d, const kvca_page_pool* p, int64_t num_planes, int64_t row_bytes, int* vec) {
+  if (num_planes < 1 || num_planes > KVCA_MAX_PLANES || row_bytes < 1) return false;
+  *vec = align_of(static_cast<uint64_t>(row_bytes));
+  return check_paged(d, num_planes, row_bytes, vec) && d->num_blocks == p->num_slots &&
+         d->block_size == p->block_size && (d->block_size == 1 || d->row_stride >= row_bytes) &&
+         (d->num_blocks <= 1 || d->block_stride >= (d->block_size - 1) * d->row_stride + row_bytes);
+}
+
+}  // namespace
+
+size_t kvca_fork_workspace_bytes(int64_t count, int64_t table_width) {
+  return count < 0 || table_width < 0 ? 0 : kvca::fork_workspace(count, table_width);
+}
+
+size_t kvca_free_workspace_bytes(int64_t count, int64_t table_width) {
+  return count < 0 || table_width < 0 ? 0 : kvca::free_workspace(count, table_width);
+}
+
+size_t kvca_compact_workspace_bytes(int64_t num_slots) { return num_slots < 0 ? 0 : kvca::compact_workspace(num_slots); }
+
+int kvca_fork_sequences(const kvca_page_pool* pool, const int64_t* d_parents, const int64_t* d_children,
+                        const int64_t* d_fresh_slots, const int64_t* d_fresh_ids, int64_t count,
+                        const kvca_paged_desc* cache, int64_t num_planes, int64_t row_bytes, void* d_workspace,
+                        int64_t workspace_bytes, int64_t* d_status, kvca_stream_t stream) {
+  kvca::ForkArgs f;
+  const int rc = to_pages(pool, d_status, &f.pool, &f.table);
+  if (rc != KVCA_OK) return rc;
+  int vec = 16;
+  if (count < 0 || !check_pages(cache, pool, num_planes, row_bytes, &vec)) return KVCA_ERR_BAD_ARGUMENT;
+  if (count == 0) return KVCA_OK;
+  if (count > kvca::kPageOpMaxSequences || count * pool->table_width > (int64_t{1} << 38)) return KVCA_ERR_SIZE_LIMIT;
+  if (!page_pointers_ok(f.pool, f.table) || !d_parents || !d_children || !d_fresh_slots || !d_fresh_ids || !d_status ||
+      !d_workspace || !aligned16(reinterpret_cast<uint64_t>(d_workspace)) ||
+      workspace_bytes < static_cast<int64_t>(kvca::fork_workspace(count, pool->table_width)))
+    return KVCA_ERR_BAD_ARGUMENT;
+  f.parents = d_parents;
+  f.children = d_children;
+  f.fresh_slots = d_fresh_slots;
+  f.fresh_ids = d_fresh_ids;
+  f.count = count;
+  kvca::PagedSide side;
+  to_side(cache, num_planes, &side);
+  return status_of(kvca::launch_fork(pool->meta_bits, f, side, static_cast<int>(num_planes), row_bytes, vec,
+                                     d_workspace, stream));
+}
+
+int kvca_free_sequences(const kvca_page_pool* pool, const int64_t* d_sequences, int64_t count, int32_t discard,
+                        void* d_workspace, int64_t workspace_bytes, int64_t* d_status, kvca_stream_t stream) {
+  kvca::FreeArgs f;
+  const int rc = to_pages(pool, d_status, &f.pool, &f.table);
+  if (rc != KVCA_OK) return rc;
+  if (count < 0) return KVCA_ERR_BAD_ARGUMENT;
+  if (count == 0) return KVCA_OK;
+  if (count > kvca::kPageOpMaxSequences || count * pool->table_width > (int64_t{1} << 38)) return KVCA_ERR_SIZE_LIMIT;
+  if (!page_pointers_ok(f.pool, f.table) || !d_sequences || !d_status || !d_workspace ||
+      !aligned16(reinterpret_cast<uint64_t>(d_workspace)) ||
+      workspace_bytes < static_cast<int64_t>(kvca::free_workspace(count, pool->table_width)))
+    return KVCA_ERR_BAD_ARGUMENT;
+  f.sequences = d_sequences;
+  f.count = count;
+  f.discard = discard != 0;
+  f.lens_before = nullptr;
+  return status_of(kvca::launch_free(pool->meta_bits, f, d_workspace, stream));
+}
+
+int kvca_compact_pages(const kvca_page_pool* pool, const kvca_paged_desc* cache, int64_t num_planes,
+                       int64_t row_bytes, int64_t* d_remap, int64_t* d_live, void* d_workspace,
+                       int64_t workspace_bytes, int64_t* d_status, kvca_stream_t stream) {
+  kvca::CompactArgs c;
+  const int rc = to_pages(pool, d_status, &c.pool, &c.table);
+  if (rc != KVCA_OK) return rc;
+  int vec = 16;
+  if (!check_pages(cache, pool, num_planes, row_bytes, &vec)) return KVCA_ERR_BAD_ARGUMENT;
+  if (pool->num_slots == 0) return KVCA_OK;
+  if (pool->num_seqs * ((pool->table_width + 1023) / 1024) > (int64_t{1} << 30)) return KVCA_ERR_SIZE_LIMIT;
+  if (!page_pointers_ok(c.pool, c.table) || !d_remap || !d_live || !d_status || !d_workspace ||
+      !aligned16(reinterpret_cast<uint64_t>(d_workspace)) ||
+      workspace_bytes < static_cast<int64_t>(kvca::compact_workspace(pool->num_slots)))
+    return KVCA_ERR_BAD_ARGUMENT;
+  c.remap = d_remap;
+  c.live = d_live;
+  kvca::PagedSide side;
+  to_side(cache, num_planes, &side);
+  return status_of(kvca::launch_compact(pool->meta_bits, c, side, static_cast<int>(num_planes), row_bytes, vec,
+                                        d_workspace, stream));
+}
+
 int64_t kvca_attend_step_workspace_bytes(const kvca_attend_desc* desc) {
   kvca::AttendArgs a;
   if (to_attend(desc, nullptr, &a) != KVCA_OK) return -1;

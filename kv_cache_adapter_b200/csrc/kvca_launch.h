@@ -164,6 +164,62 @@ size_t attend_chunk_workspace(const AttendArgs& args, int64_t rows, int sms);
 cudaError_t launch_attend_chunk(const AttendArgs& args, const int64_t* offsets, int64_t rows, void* workspace, int sms,
                                 cudaStream_t stream);
 
+// The slot pool and the page tables of the operators on sequences' pages.
+struct PagePool {
+  void* slot_meta;
+  int64_t num_slots;
+  int64_t* l2p;
+  int64_t num_logical;
+  int64_t* p2l;
+  int64_t* status;
+};
+
+struct PageTable {
+  int64_t* tables;
+  int64_t stride;
+  int64_t width;
+  int64_t* lens;
+  int64_t num_seqs;
+  int64_t block_size;
+};
+
+struct ForkArgs {
+  PagePool pool;
+  PageTable table;
+  const int64_t* parents;
+  const int64_t* children;
+  const int64_t* fresh_slots;
+  const int64_t* fresh_ids;
+  int64_t count;
+};
+
+struct FreeArgs {
+  PagePool pool;
+  PageTable table;
+  const int64_t* sequences;
+  int64_t count;
+  bool discard;
+  int64_t* lens_before;  // in the workspace
+};
+
+struct CompactArgs {
+  PagePool pool;
+  PageTable table;
+  int64_t* remap;
+  int64_t* live;
+};
+
+constexpr int64_t kPageOpMaxSequences = 63 * 1024;
+
+size_t fork_workspace(int64_t count, int64_t table_width);
+size_t free_workspace(int64_t count, int64_t table_width);
+size_t compact_workspace(int64_t num_slots);
+cudaError_t launch_fork(int meta_bits, const ForkArgs& args, const PagedSide& cache, int num_planes,
+                        int64_t row_bytes, int vec_bytes, void* workspace, cudaStream_t stream);
+cudaError_t launch_free(int meta_bits, const FreeArgs& args, void* workspace, cudaStream_t stream);
+cudaError_t launch_compact(int meta_bits, const CompactArgs& args, const PagedSide& cache, int num_planes,
+                           int64_t row_bytes, int vec_bytes, void* workspace, cudaStream_t stream);
+
 cudaError_t launch_inspect_load(int meta_bits, const int64_t* l2p, int64_t num_logical,
                                 const void* meta, int64_t num_slots, const int64_t* ids,
                                 int64_t count, int64_t* cur_out, uint8_t* resident_out,

@@ -53,6 +53,9 @@ __all__ = [
     "scatter_tokens_gather_layers",
     "move_cycle",
     "exchange_blocks",
+    "fork_sequences",
+    "free_sequences",
+    "compact_pages",
     "attend_step",
     "attend_chunk",
     "batched_fused_single_layer_kv_transfer",
@@ -1274,6 +1277,141 @@ def move_cycle(token_caches, slot_mapping: torch.Tensor, token_rows: torch.Tenso
             _ptr(_status(dev)), _stream(dev))
     _host_rc(rc, "move_cycle")
     _maybe_check(dev, check, "move_cycle")
+
+
+# ---------------------------------------------------------------------------
+# pages of sequences
+# ---------------------------------------------------------------------------
+
+
+def _page_pool(slot_meta, logical_to_physical, physical_to_logical, block_tables, seq_lens,
+               block_size: int) -> _lib.PagePool:
+    """The checked slot pool and page tables of an operator on sequences' pages."""
+    _require(slot_meta, _META_DTYPES, "slot_meta")
+    dev = slot_meta.device
+    for t, name in ((logical_to_physical, "logical_to_physical"), (physical_to_logical, "physical_to_logical"),
+                    (seq_lens, "seq_lens")):
+        _require_index(t, dev, name)
+    if physical_to_logical.numel() != slot_meta.numel():
+        raise ValueError("physical_to_logical needs one entry per slot")
+    if not isinstance(block_tables, torch.Tensor):
+        raise TypeError("block_tables must be torch.Tensor")
+    if block_tables.dtype != torch.int64:
+        raise TypeError(f"block_tables has incorrect dtype {block_tables.dtype}")
+    if block_tables.device != dev:
+        raise ValueError(f"block_tables must be on {dev}")
+    if block_tables.dim() != 2 or block_tables.shape[0] != seq_lens.numel():
+        raise ValueError("block_tables must be (num_seqs, max_blocks)")
+    rows, width = block_tables.shape
+    if block_tables.numel() and (block_tables.stride(1) != 1 and width > 1
+                                 or block_tables.stride(0) < width and rows > 1):
+        raise ValueError("block_tables: rows must be contiguous and must not overlap")
+    if block_size < 1:
+        raise ValueError("block_size must be positive")
+    return _lib.PagePool(_meta_bits(slot_meta), 0, slot_meta.data_ptr() or None, slot_meta.numel(),
+                         logical_to_physical.data_ptr() or None, logical_to_physical.numel(),
+                         physical_to_logical.data_ptr() or None, block_tables.data_ptr() or None,
+                         block_tables.stride(0) if rows > 1 else width, width, seq_lens.data_ptr() or None, rows,
+                         block_size)
+
+
+def _page_caches(caches, slot_meta: torch.Tensor) -> PlaneTable:
+    pl = _planes(caches, 2, "caches")
+    if pl.device != slot_meta.device:
+        raise ValueError(f"caches must be on {slot_meta.device}")
+    if pl.num_blocks != slot_meta.numel():
+        raise ValueError(f"caches hold {pl.num_blocks} blocks, slot_meta {slot_meta.numel()} slots")
+    return pl
+
+
+def fork_sequences(slot_meta: torch.Tensor, logical_to_physical: torch.Tensor, physical_to_logical: torch.Tensor,
+                   block_tables: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor, children: torch.Tensor,
+                   fresh_slots: torch.Tensor, fresh_ids: torch.Tensor, caches, *, check: bool | None = None) -> None:
+    """Sequence ``children[j]`` becomes a copy of sequence ``parents[j]``
+    (kvca_fork_sequences): the parent's full pages are shared, one pin more
+    each; a partly filled last page is copied in every plane of ``caches``
+    (token planes ``(num_blocks, block_size, *row)`` or a
+    ``PlaneTable(planes, 2)``) to slot ``fresh_slots[j]`` (as
+    ``pop_reusable_slots`` hands them out), which becomes logical block
+    ``fresh_ids[j]``, pinned.  ``block_tables`` int64 ``(num_seqs,
+    max_blocks)`` names each sequence's slots, ``seq_lens`` its tokens; the
+    children must be empty.  Everything is checked first: an error leaves all
+    as it was."""
+    pl = _page_caches(caches, slot_meta)
+    pool = _page_pool(slot_meta, logical_to_physical, physical_to_logical, block_tables, seq_lens, pl.block_size)
+    dev = slot_meta.device
+    count = parents.numel()
+    for t, name in ((parents, "parents"), (children, "children"), (fresh_slots, "fresh_slots"),
+                    (fresh_ids, "fresh_ids")):
+        _require_index(t, dev, name)
+        if t.numel() != count:
+            raise ValueError("parents, children, fresh_slots and fresh_ids must have the same length")
+    if count == 0:
+        return
+    need = int(_lib_handle.kvca_fork_workspace_bytes(count, pool.table_width))
+    with _on(dev):
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        rc = _lib_handle.kvca_fork_sequences(
+            ctypes.byref(pool), parents.data_ptr(), children.data_ptr(), fresh_slots.data_ptr(), fresh_ids.data_ptr(),
+            count, ctypes.byref(pl.desc(None)), len(pl.planes), pl.row_bytes, workspace.data_ptr(), need,
+            _ptr(_status(dev)), _stream(dev))
+    _host_rc(rc, "fork_sequences")
+    _maybe_check(dev, check, "fork_sequences")
+
+
+def free_sequences(slot_meta: torch.Tensor, logical_to_physical: torch.Tensor, physical_to_logical: torch.Tensor,
+                   block_tables: torch.Tensor, seq_lens: torch.Tensor, sequences: torch.Tensor, block_size: int, *,
+                   discard: bool = False, check: bool | None = None) -> None:
+    """The ``sequences`` (distinct) give their pages back
+    (kvca_free_sequences): one pin less per page, table entries -1, length 0.
+    Pages that nobody holds any more stay resident, to be evicted by
+    ``pop_reusable_slots``, or are unmapped with ``discard``.  Everything is
+    checked first: an error leaves all as it was."""
+    pool = _page_pool(slot_meta, logical_to_physical, physical_to_logical, block_tables, seq_lens, int(block_size))
+    dev = slot_meta.device
+    _require_index(sequences, dev, "sequences")
+    count = sequences.numel()
+    if count == 0:
+        return
+    need = int(_lib_handle.kvca_free_workspace_bytes(count, pool.table_width))
+    with _on(dev):
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        rc = _lib_handle.kvca_free_sequences(ctypes.byref(pool), sequences.data_ptr(), count, int(bool(discard)),
+                                             workspace.data_ptr(), need, _ptr(_status(dev)), _stream(dev))
+    _host_rc(rc, "free_sequences")
+    _maybe_check(dev, check, "free_sequences")
+
+
+def compact_pages(slot_meta: torch.Tensor, logical_to_physical: torch.Tensor, physical_to_logical: torch.Tensor,
+                  block_tables: torch.Tensor, seq_lens: torch.Tensor, caches, *, remap: torch.Tensor | None = None,
+                  check: bool | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The live slots (mapped or pinned, K of them) move into the first K
+    (kvca_compact_pages): their blocks in every plane of ``caches`` (as for
+    ``fork_sequences``), their metadata, and their names in the sequences'
+    page tables.  Returns ``(remap, live)``: each live slot's new place (-1
+    for dead ones; ``remap`` if given) and K, both int64 on the device."""
+    pl = _page_caches(caches, slot_meta)
+    pool = _page_pool(slot_meta, logical_to_physical, physical_to_logical, block_tables, seq_lens, pl.block_size)
+    dev = slot_meta.device
+    n = slot_meta.numel()
+    if remap is None:
+        remap = torch.empty(n, dtype=torch.int64, device=dev)
+    else:
+        _require_index(remap, dev, "remap")
+        if remap.numel() != n:
+            raise ValueError("remap needs one entry per slot")
+    live = torch.empty(1, dtype=torch.int64, device=dev)
+    if n == 0:
+        return remap, live.zero_()
+    need = int(_lib_handle.kvca_compact_workspace_bytes(n))
+    with _on(dev):
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        rc = _lib_handle.kvca_compact_pages(ctypes.byref(pool), ctypes.byref(pl.desc(None)), len(pl.planes),
+                                            pl.row_bytes, remap.data_ptr(), live.data_ptr(), workspace.data_ptr(), need,
+                                            _ptr(_status(dev)), _stream(dev))
+    _host_rc(rc, "compact_pages")
+    _maybe_check(dev, check, "compact_pages")
+    return remap, live
 
 
 # ---------------------------------------------------------------------------
