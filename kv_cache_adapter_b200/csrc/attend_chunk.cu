@@ -212,6 +212,15 @@ __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 
+// Whether a phase is over, without the suspension of a try.
+__device__ __forceinline__ bool barrier_test(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+
 // Waits for a phase; gives up, as every other warp of the CTA then does, after
 // kWaitTries tries (a try suspends the thread for a while) or once another
 // warp gave up.
@@ -511,6 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         for (int q = 0; q < row_tiles; ++q) scores(q, used);
         mma_commit(empty + 8 * stage_of(used));
+        if (n == 1) mma_commit(q_empty);
         ++used;
         for (int i = 0; i < n && ok; ++i) {
           const uint32_t values_at = used, keys_at = used + 1;
@@ -535,9 +545,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!ok) break;
           mma_commit(empty + 8 * stage_of(values_at));
           if (more) mma_commit(empty + 8 * stage_of(keys_at));
+          if (i + 2 == n) mma_commit(q_empty);  // the last scores of the segment were just issued
           used += more ? 2 : 1;
         }
-        if (ok) mma_commit(q_empty);
         ++segment;
       } while (ok && s.next(a, c, ws));
       if (!ok) {
@@ -564,15 +574,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t issued = 0, arrived = 0;
       uint32_t segment = 0;
       constexpr uint32_t kAhead = 2;  // tiles in flight behind the one being issued
+      bool queries = false;           // in flight, before any tile
+      // Hands over the oldest of what is in flight.
       auto complete = [&]() {
         fence_async_proxy();
-        barrier_arrive(full + 8 * (arrived % kStages));
-        ++arrived;
+        if (queries) {
+          barrier_arrive(q_full);
+          queries = false;
+        } else {
+          barrier_arrive(full + 8 * (arrived % kStages));
+          ++arrived;
+        }
       };
       auto drain = [&]() {
-        while (arrived < issued) {
-          if (issued - arrived == kAhead)
-            cp_async_wait<kAhead - 1>();
+        for (uint32_t left = issued - arrived + (queries ? 1 : 0); left > 0; --left) {
+          if (left == 3)
+            cp_async_wait<2>();
+          else if (left == 2)
+            cp_async_wait<1>();
           else
             cp_async_wait<0>();
           complete();
@@ -583,54 +602,78 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto claim = [&]() {
         if (issued < kStages || !ok) return;
         const uint32_t bar = empty + 8 * (issued % kStages), parity = ((issued / kStages) - 1) & 1;
-        if (__all_sync(0xffffffffu, barrier_try(bar, parity))) return;
+        if (__all_sync(0xffffffffu, barrier_test(bar, parity))) return;
         if constexpr (!kE4m3) drain();
         ok = warp_wait(bar, parity, abort, a.status);
       };
       constexpr int64_t kHidden = -1ll << 62;
       do {
-        // queries, through registers: the sign of a negative scale, the
-        // zeros of a zero one, or (e4m3) a power of two per row goes into them
+        // Queries.  With e4m3 they go through registers, times a power of two
+        // per row (see attend_step.cu); so they do when the sign of a negative
+        // scale or the zeros of a zero one go into them.
         if (segment > 0) ok = ok && warp_wait(q_empty, (segment - 1) & 1, abort, a.status);
         if (!ok) break;
-        for (int r0 = w * 64; r0 < w * 64 + 64; r0 += kPerInstr) {
-          const int r = r0 + sub;
-          const int row = s.view.row + r;
-          const bool live = r < s.view.rows && chunk < row_chunks;
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (live) {
-            const int token = row / a.group;
-            const uint16_t* src = static_cast<const uint16_t*>(a.query) + (s.out_row + token) * a.query_row +
-                                  static_cast<int64_t>(s.head * a.group + row - token * a.group) * a.query_head;
-            x = __ldg(reinterpret_cast<const uint4*>(src) + chunk);
-          }
-          uint32_t* const word = reinterpret_cast<uint32_t*>(&x);
-          if constexpr (kE4m3) {
-            const bool bf16 = a.query_type == KVCA_TYPE_BF16;
-            float2 f[4];
-            float big = 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              f[j] = bf16 ? unpack2<true>(word[j]) : unpack2<false>(word[j]);
-              big = fmaxf(big, fmaxf(fabsf(f[j].x), fabsf(f[j].y)));
-            }
-#pragma unroll
-            for (int o = kRowChunks / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-            const int e = big > 0.f && big < INFINITY ? min(max(12 - ilogbf(big), -120), 120) : 0;
-            const float up = ldexpf(1.f, e);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) word[j] = pack2<false>(f[j].x * up, f[j].y * up);
-            if (chunk == 0) row_unit[r] = c.scale_log2 * ldexpf(1.f, -e);
-          } else {
+        auto query_row = [&](int r) -> const uint4* {
+          if (r >= s.view.rows || chunk >= row_chunks) return nullptr;
+          const int row = s.view.row + r, token = row / a.group;
+          const uint16_t* src = static_cast<const uint16_t*>(a.query) + (s.out_row + token) * a.query_row +
+                                static_cast<int64_t>(s.head * a.group + row - token * a.group) * a.query_head;
+          return reinterpret_cast<const uint4*>(src) + chunk;
+        };
+        if (!kE4m3 && c.query_and == 0xffffffffu && c.query_xor == 0u) {
+#pragma unroll 4
+          for (int r = w * 64 + sub; r < w * 64 + 64; r += kPerInstr) {
+            const uint4* src = query_row(r);
+            if (chunk < row_chunks)
+              cp_async16(smem + (r >> 7) * kTileBytes + place(r & 127, chunk), src != nullptr ? src : a.query,
+                         src != nullptr);
             if (chunk == 0) row_unit[r] = c.scale_log2;
           }
+          cp_async_commit();
+          queries = true;
+        } else {
+          constexpr int kBatch = 8;
+#pragma unroll 1
+          for (int r0 = w * 64 + sub; r0 < w * 64 + 64; r0 += kBatch * kPerInstr) {
+            uint4 x[kBatch];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) word[j] = (word[j] & c.query_and) ^ c.query_xor;
-          if (chunk < row_chunks)
-            *reinterpret_cast<uint4*>(smem_ptr + (r >> 7) * kTileBytes + place(r & 127, chunk)) = x;
+            for (int i = 0; i < kBatch; ++i) {
+              const uint4* src = query_row(r0 + i * kPerInstr);
+              x[i] = src != nullptr ? __ldg(src) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+              const int r = r0 + i * kPerInstr;
+              uint32_t word[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+              float unit = c.scale_log2;
+              if constexpr (kE4m3) {
+                const bool bf16 = a.query_type == KVCA_TYPE_BF16;
+                float2 f[4];
+                float big = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  f[j] = bf16 ? unpack2<true>(word[j]) : unpack2<false>(word[j]);
+                  big = fmaxf(big, fmaxf(fabsf(f[j].x), fabsf(f[j].y)));
+                }
+#pragma unroll
+                for (int o = kRowChunks / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                const int e = big > 0.f && big < INFINITY ? min(max(12 - ilogbf(big), -120), 120) : 0;
+                const float up = ldexpf(1.f, e);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) word[j] = pack2<false>(f[j].x * up, f[j].y * up);
+                unit *= ldexpf(1.f, -e);
+              }
+              if (chunk == 0) row_unit[r] = unit;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) word[j] = (word[j] & c.query_and) ^ c.query_xor;
+              if (chunk < row_chunks)
+                *reinterpret_cast<uint4*>(smem_ptr + (r >> 7) * kTileBytes + place(r & 127, chunk)) =
+                    make_uint4(word[0], word[1], word[2], word[3]);
+            }
+          }
+          fence_async_proxy();
+          barrier_arrive(q_full);
         }
-        fence_async_proxy();
-        barrier_arrive(q_full);
 
         // keys and values, tile by tile; a lane looks up the page of one token
         int64_t page;
@@ -662,16 +705,19 @@ __global__ void __launch_bounds__(kThreads, 1)
               claim();
               if (!ok) break;
               const uint32_t dst = kv_smem + (issued % kStages) * kTileBytes;
+              const char* src[32 / kPerInstr];
 #pragma unroll
-              for (int r = 0; r < 32; r += kPerInstr) {
-                const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, r + sub));
-                if (chunk < row_chunks)
-                  cp_async16(dst + place(w * 32 + r + sub, chunk), src != nullptr ? src + chunk * 16 : a.key,
-                             src != nullptr);
+              for (int i = 0; i < 32 / kPerInstr; ++i)
+                src[i] = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, i * kPerInstr + sub));
+              if (chunk < row_chunks) {
+#pragma unroll
+                for (int i = 0; i < 32 / kPerInstr; ++i)
+                  cp_async16(dst + place(w * 32 + i * kPerInstr + sub, chunk),
+                             src[i] != nullptr ? src[i] + chunk * 16 : a.key, src[i] != nullptr);
               }
               cp_async_commit();
               ++issued;
-              if (issued - arrived > kAhead) {
+              if (issued - arrived + (queries ? 1 : 0) > kAhead) {
                 cp_async_wait<kAhead>();
                 complete();
               }
