@@ -248,25 +248,30 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u) : "memory");
+// One 128 x n x 16 product; operands given by the low words of their
+// descriptors (kOperandHigh above them).
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile("{\n.reg .pred p;\n.reg .b64 a, b;\nmov.b64 a, {%1, %3};\nmov.b64 b, {%2, %3};\n"
+               "setp.ne.u32 p, %5, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}"
+               ::"r"(d), "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u) : "memory");
+// The same with `a` in tensor memory.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t high, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile("{\n.reg .pred p;\n.reg .b64 b;\nmov.b64 b, {%2, %3};\n"
+               "setp.ne.u32 p, %5, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}"
+               ::"r"(d), "r"(a), "r"(b), "r"(high), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-// Shared memory operand with 128-byte swizzle; 8 rows of 128 bytes are 1 KiB.
+// Shared memory operands with 128-byte swizzle; 8 rows of 128 bytes are 1 KiB.
 // K-major (queries, keys): groups of 8 rows 1 KiB apart.  MN-major (values:
 // tokens are the reduced dim): groups of 8 tokens 1 KiB apart, 64 dims
 // `leading` bytes apart.
-__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t leading) {
-  return static_cast<uint64_t>((addr >> 4) & 0x3fffu) | (static_cast<uint64_t>(leading >> 4) << 16) |
-         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+constexpr uint32_t kOperandHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ constexpr uint32_t operand_low(uint32_t addr, uint32_t leading) {
+  return (addr >> 4) | ((leading >> 4) << 16);  // shared memory ends below 2^18
 }
 
 // fp32 accumulators; both operands fp16 or both bf16; m x n.
@@ -490,67 +495,84 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= 12) {
     // ------------------------------------------------------------------ MMA
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 12 && lane == 0 && working) {
+    if (warp == 12 && working) {
+      // the whole warp keeps step, one lane issues
       constexpr uint32_t kScores = mma_shape(kBf16, 128, kKeys, false);
       constexpr uint32_t kOutput = mma_shape(kBf16, 128, DP, true);
-      uint32_t used = 0;      // ring entries consumed
+      constexpr uint32_t kHalf = kKeys * 128 >> 4;  // between 64 dims, in descriptor units
+      const uint32_t q_low = operand_low(smem, 16), k_low = operand_low(kv_smem, 16);
+      const uint32_t v_low = operand_low(kv_smem, kKeys * 128);
+      const bool issues = lane == 0;
+      uint32_t stage = 0, round = 0;  // of the next ring entry
       uint32_t segment = 0;
       uint32_t p_phase[2] = {0, 0};
       bool ok = true;
-      auto stage_of = [&](uint32_t n) { return n % kStages; };
-      auto wait_full = [&](uint32_t n) {
-        ok = ok && barrier_wait(full + 8 * stage_of(n), (n / kStages) & 1, abort, a.status);
-        fence_after_sync();
+      auto step = [&]() {
+        if (++stage == kStages) {
+          stage = 0;
+          round ^= 1;
+        }
       };
-      auto scores = [&](int q, uint32_t n) {  // S_q = Q_q K^T, K in ring entry n
-        const uint32_t keys = kv_smem + stage_of(n) * kTileBytes;
-        const uint32_t queries = smem + q * kTileBytes;
+      auto scores = [&](int q, uint32_t at) {  // S_q = Q_q K^T, K in ring entry `at`
+        const uint32_t keys = k_low + at * (kTileBytes >> 4), queries = q_low + q * (kTileBytes >> 4);
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t at = (k >> 2) * (kKeys * 128) + (k & 3) * 32;
-          mma_ss(tmem + q * 128, operand(queries + at, 16), operand(keys + at, 16), kScores, k > 0);
+          const uint32_t off = (k >> 2) * kHalf + (k & 3) * 2;
+          mma_ss(tmem + q * 128, queries + off, keys + off, kOperandHigh, kScores, k > 0);
         }
         mma_commit(s_full + 8 * q);
       };
       do {
         const int n = s.end - s.tile;
         const int row_tiles = s.row_tiles();
-        ok = ok && barrier_wait(q_full, segment & 1, abort, a.status);
-        wait_full(used);
+        ok = ok && warp_wait(q_full, segment & 1, abort, a.status) &&
+             warp_wait(full + 8 * stage, round, abort, a.status);
         if (!ok) break;
-        for (int q = 0; q < row_tiles; ++q) scores(q, used);
-        mma_commit(empty + 8 * stage_of(used));
-        if (n == 1) mma_commit(q_empty);
-        ++used;
-        for (int i = 0; i < n && ok; ++i) {
-          const uint32_t values_at = used, keys_at = used + 1;
+        fence_after_sync();
+        if (issues) {
+          scores(0, stage);
+          if (row_tiles > 1) scores(1, stage);
+          mma_commit(empty + 8 * stage);
+          if (n == 1) mma_commit(q_empty);
+        }
+        step();
+        for (int i = 0; i < n; ++i) {
+          const uint32_t values_at = stage;
           const bool more = i + 1 < n;
-          wait_full(values_at);
-          for (int q = 0; q < row_tiles; ++q) {
-            ok = ok && barrier_wait(p_ready + 8 * q, p_phase[q] & 1, abort, a.status);
+          ok = ok && warp_wait(full + 8 * stage, round, abort, a.status);
+          step();
+          const uint32_t keys_at = stage;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            if (q >= row_tiles) break;
+            ok = ok && warp_wait(p_ready + 8 * q, p_phase[q] & 1, abort, a.status);
             ++p_phase[q];
-            if (more && q == 0) wait_full(keys_at);
+            if (more && q == 0) ok = ok && warp_wait(full + 8 * stage, round, abort, a.status);
             if (!ok) break;
             fence_after_sync();
-            const uint32_t values = kv_smem + stage_of(values_at) * kTileBytes;
+            if (issues) {
+              const uint32_t values = v_low + values_at * (kTileBytes >> 4);
 #pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k)
-              mma_ts(tmem + 256 + q * 128, tmem + q * 128 + k * 8, operand(values + k * 2048, kKeys * 128), kOutput,
-                     i > 0 || k > 0);
-            if (more)
-              scores(q, keys_at);
-            else
-              mma_commit(o_full + 8 * q);
+              for (int k = 0; k < kKeys / 16; ++k)
+                mma_ts(tmem + 256 + q * 128, tmem + q * 128 + k * 8, values + k * 128, kOperandHigh, kOutput,
+                       k > 0 ? 1u : static_cast<uint32_t>(i));
+              if (more)
+                scores(q, keys_at);
+              else
+                mma_commit(o_full + 8 * q);
+            }
           }
           if (!ok) break;
-          mma_commit(empty + 8 * stage_of(values_at));
-          if (more) mma_commit(empty + 8 * stage_of(keys_at));
-          if (i + 2 == n) mma_commit(q_empty);  // the last scores of the segment were just issued
-          used += more ? 2 : 1;
+          if (issues) {
+            mma_commit(empty + 8 * values_at);
+            if (more) mma_commit(empty + 8 * keys_at);
+            if (i + 2 == n) mma_commit(q_empty);  // the last scores of the segment were just issued
+          }
+          if (more) step();
         }
         ++segment;
       } while (ok && s.next(a, c, ws));
-      if (!ok) {
+      if (!ok && issues) {
         // what was issued may still run: let it end before the memory goes
         mma_commit(drained);
         for (uint32_t i = 0; i < 4096 && !barrier_try(drained, 0); ++i) {
@@ -690,14 +712,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         look_up(s.tile);
         for (int tile = s.tile; tile < s.end && ok; ++tile) {
-          const char* rows[2] = {nullptr, nullptr};
-          if (page >= 0 && page < a.num_blocks) {
-            rows[0] = a.key + page * a.key_block + offset * a.key_token + s.head * a.key_head;
-            rows[1] = a.value + page * a.value_block + offset * a.value_token + s.head * a.value_head;
-          } else if (page != kHidden) {
-            report(a.status, KVCA_ERR_BAD_INDEX, page);  // its rows read as zeros
-          }
+          // rows of hidden tokens, and of a page outside the cache, read as zeros
+          const bool good = page >= 0 && page < a.num_blocks;
+          if (!good && page != kHidden) report(a.status, KVCA_ERR_BAD_INDEX, page);
+          const int64_t block = good ? page : 0;
+          const unsigned seen = __ballot_sync(0xffffffffu, good);
+          const char* rows[2];
+          rows[0] = a.key + block * a.key_block + offset * a.key_token + s.head * a.key_head;
+          rows[1] = a.value + block * a.value_block + offset * a.value_token + s.head * a.value_head;
           if (tile + 1 < s.end) look_up(tile + 1);
+          const char* src[32 / kPerInstr];
 #pragma unroll
           for (int side = 0; side < 2; ++side) {
             const unsigned long long row = reinterpret_cast<unsigned long long>(rows[side]);
@@ -705,15 +729,25 @@ __global__ void __launch_bounds__(kThreads, 1)
               claim();
               if (!ok) break;
               const uint32_t dst = kv_smem + (issued % kStages) * kTileBytes;
-              const char* src[32 / kPerInstr];
-#pragma unroll
-              for (int i = 0; i < 32 / kPerInstr; ++i)
-                src[i] = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, i * kPerInstr + sub));
-              if (chunk < row_chunks) {
+              if (side == 0 || !c.same_layout) {
 #pragma unroll
                 for (int i = 0; i < 32 / kPerInstr; ++i)
-                  cp_async16(dst + place(w * 32 + i * kPerInstr + sub, chunk),
-                             src[i] != nullptr ? src[i] + chunk * 16 : a.key, src[i] != nullptr);
+                  src[i] = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, i * kPerInstr + sub)) + chunk * 16;
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32 / kPerInstr; ++i) src[i] += a.value - a.key;
+              }
+              if (chunk < row_chunks) {
+                if (seen == 0xffffffffu) {
+#pragma unroll
+                  for (int i = 0; i < 32 / kPerInstr; ++i)
+                    cp_async16(dst + place(w * 32 + i * kPerInstr + sub, chunk), src[i]);
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 32 / kPerInstr; ++i)
+                    cp_async16(dst + place(w * 32 + i * kPerInstr + sub, chunk), src[i],
+                               (seen >> (i * kPerInstr + sub)) & 1u);
+                }
               }
               cp_async_commit();
               ++issued;
@@ -729,10 +763,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               uint4 x[32 / kRowsPer];
 #pragma unroll
               for (int i = 0; i < 32 / kRowsPer; ++i) {
-                const char* src =
-                    reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, i * kRowsPer + which));
-                x[i] = src != nullptr && part * 16 < a.dim ? __ldg(reinterpret_cast<const uint4*>(src) + part)
-                                                           : make_uint4(0, 0, 0, 0);
+                const int r = i * kRowsPer + which;
+                const uint4* from = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, row, r)) + part;
+                x[i] = ((seen >> r) & 1u) && part * 16 < a.dim ? __ldg(from) : make_uint4(0, 0, 0, 0);
               }
               claim();
               if (!ok) break;
@@ -1071,6 +1104,7 @@ cudaError_t launch_attend_chunk(const AttendArgs& args, const int64_t* offsets, 
   c.max_blocks = static_cast<int>(attend_chunk_max_blocks(a, rows));
   // the softmax takes the maximum of the raw scores, so their factor is positive
   c.scale_log2 = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
+  c.same_layout = a.key_block == a.value_block && a.key_token == a.value_token && a.key_head == a.value_head;
   c.query_and = a.scale_log2 == 0.f ? 0u : 0xffffffffu;
   c.query_xor = a.scale_log2 < 0.f ? 0x80008000u : 0u;
   switch (a.cache_type) {
