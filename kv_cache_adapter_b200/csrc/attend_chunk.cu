@@ -312,6 +312,29 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[
       : "memory");
 }
 
+// Two floats at once.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\n"
+      "fma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 d, a, b;\n"
+      "mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Keeps the uses of loaded values behind the wait before this.
@@ -423,6 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ float row_unit[kRows];
   __shared__ uint32_t tmem_base;
   __shared__ int start_block;
+  __shared__ Share shares[kThreads / 32];
   __shared__ int abort_flag;
 
   const int lane = threadIdx.x & 31;
@@ -481,8 +505,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after_sync();
   const uint32_t tmem = tmem_base;
 
-  Share s;
-  if (working) {
+  Share& s = shares[warp];
+  if (working && lane == 0) {
     s.left = share;
     s.block = start_block;
     const int64_t rest = begin - ws.first[s.block];
@@ -491,6 +515,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     s.tile = static_cast<int>(rest - static_cast<int64_t>(s.head) * tiles);
     s.load(a, c, ws);
   }
+  __syncwarp();
+  // The warp's copy of the share to its next segment.
+  auto next_segment = [&]() {
+    __syncwarp();
+    int more = 0;
+    if (lane == 0) more = s.next(a, c, ws);
+    __syncwarp();
+    return __shfl_sync(0xffffffffu, more, 0) != 0;
+  };
 
   if (warp >= 12) {
     // ------------------------------------------------------------------ MMA
@@ -571,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (more) step();
         }
         ++segment;
-      } while (ok && s.next(a, c, ws));
+      } while (ok && next_segment());
       if (!ok && issues) {
         // what was issued may still run: let it end before the memory goes
         mma_commit(drained);
@@ -795,7 +828,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           drain();
         }
         ++segment;
-      } while (ok && s.next(a, c, ws));
+      } while (ok && next_segment());
       cp_async_wait<0>();
     }
   } else {
@@ -829,7 +862,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int all_low = a.window > 0 ? s.view.context + row_last / a.group - a.window - s.view.skip : -1;
 
           float m = -INFINITY, l = 0.f;  // m in units of the raw scores
-          for (int i = 0; i < n; ++i) {
+          int v0 = s.tile * kKeys;
+#pragma unroll 1
+          for (int i = 0; i < n; ++i, v0 += kKeys) {
             ok = ok && warp_wait(s_full + 8 * q, phase & 1, abort, a.status);
             if (!ok) break;
             ++phase;
@@ -840,7 +875,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_wait_load();
 #pragma unroll
             for (int j = 0; j < 4; ++j) tmem_landed(x[j]);
-            const int v0 = (s.tile + i) * kKeys;
             if (v0 + kKeys - 1 > all_last || (v0 + kKeys > a.sinks && max(v0, a.sinks) <= all_low)) {
               const int last = v_last - v0, low = v_low - v0, sinks = a.sinks - v0;
 #pragma unroll
@@ -853,31 +887,32 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             float top[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              top[j] = x[j][0];
+            for (int j = 0; j < 4; ++j) top[j] = fmaxf(x[j][0], x[j][1]);
 #pragma unroll
-              for (int k = 1; k < 32; ++k) top[j] = fmaxf(top[j], x[j][k]);
-            }
-            const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            for (int k = 2; k < 32; k += 2)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) top[j] = max3(top[j], x[j][k], x[j][k + 1]);
+            const float best = fmaxf(max3(top[0], top[1], top[2]), top[3]);
             const float old = m;
             // (-inf) - (-inf) is no growth
             if ((best - m) * unit > kGrowth) m = best;
             const float base = m == -INFINITY ? 0.f : m * unit;
             const float decay = m != old ? exp2_approx(old * unit - base) : 1.f;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            const float2 units = make_float2(unit, unit), bases = make_float2(-base, -base);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               uint32_t packed[16];
 #pragma unroll
               for (int k = 0; k < 32; k += 2) {
-                const float e0 = exp2_approx(fmaf(x[j][k], unit, -base));
-                const float e1 = exp2_approx(fmaf(x[j][k + 1], unit, -base));
-                sum[j] += e0 + e1;
-                packed[k >> 1] = pack2<kBf16>(e0, e1);
+                float2 e = fma2(make_float2(x[j][k], x[j][k + 1]), units, bases);
+                e = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+                sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], e);
+                packed[k >> 1] = pack2<kBf16>(e.x, e.y);
               }
               tmem_store16(scores + j * 16, packed);
             }
-            l = l * decay + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+            l = l * decay + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
             if (i > 0 && __any_sync(0xffffffffu, m != old)) {
 #pragma unroll
               for (int j = 0; j < DP / 32; ++j) {
@@ -986,7 +1021,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         done += n;
         ++segment;
-      } while (s.next(a, c, ws));
+      } while (next_segment());
     }
     if (threadIdx.x == 0 && working) ws.pieces[blockIdx.x] = piece;
   }
