@@ -17,6 +17,8 @@
 //                   so that any block size and stride does; e4m3 is widened on
 //                   the way), 128-byte swizzled as the tensor cores read them
 //   warp 12         issues tcgen05.mma: S = Q K^T, O += P V
+//   warp 13         finds the CTA's next segments (block, head, tiles)
+//   warps 14, 15    queries to shared memory
 // The two tiles alternate: while one's softmax runs, the tensor cores work on
 // the other's products.  The output is rescaled only when a row's maximum grew
 // by more than 2^8, so that most tiles leave it alone; a probability is then at
@@ -41,6 +43,11 @@ constexpr int kThreads = 512;
 constexpr int kPlanThreads = 1024;
 constexpr int kJoinThreads = 256;
 constexpr int kJoinRows = 16;   // rows per block of the join
+constexpr int kSlots = 4;       // segments announced ahead
+constexpr int kReaders = 15;    // warps that read them
+// What a segment costs beside its tiles, in tiles: queries, first loads, the
+// output.  It counts when the tiles are dealt out, as tiles before the first.
+constexpr int kSegmentCost = 1;
 constexpr float kGrowth = 8.f;  // log2 of how far a maximum may lag
 constexpr uint32_t kWaitTries = 1u << 22;
 
@@ -57,7 +64,7 @@ struct ChunkShape {
 // ---------------------------------------------------------------------------
 
 struct ChunkHeader {
-  int64_t tiles;  // of all blocks and heads
+  int64_t tiles;  // of all blocks and heads, segment costs included
   int64_t ctas;   // that get tiles
   int32_t blocks;
   int32_t unused;
@@ -155,7 +162,7 @@ __global__ void __launch_bounds__(kPlanThreads) attend_chunk_plan_kernel(const _
     }
     const int n = (rows + kRows - 1) / kRows;
     int64_t total;
-    const int64_t at = run + block_excl_scan<int64_t>(n, &total, scan);
+    const int64_t at = run + block_excl_scan(static_cast<int64_t>(n), &total, scan);
     // offsets that go back and forth may name more rows than there are
     if (at + n > c.max_blocks) {
       if (n > 0) report(a.status, KVCA_ERR_BAD_INDEX, __ldg(c.offsets + seq));
@@ -180,7 +187,8 @@ __global__ void __launch_bounds__(kPlanThreads) attend_chunk_plan_kernel(const _
       ws.blocks[i].tiles = tiles;
     }
     int64_t total;
-    const int64_t before = run + block_excl_scan<int64_t>(static_cast<int64_t>(tiles) * a.kv_heads, &total, scan);
+    const int64_t cost = tiles > 0 ? static_cast<int64_t>(tiles + kSegmentCost) * a.kv_heads : 0;
+    const int64_t before = run + block_excl_scan(cost, &total, scan);
     if (i < blocks) ws.first[i] = before;
     run += total;
   }
@@ -353,38 +361,50 @@ __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::
 // ---------------------------------------------------------------------------
 
 struct Share {
-  int64_t left;    // tiles of the share from here on
+  int64_t left;    // of the share from this segment's first cost or tile on
   int block, head;
+  int from;        // where in the segment (costs, then tiles) the share begins
   int tile;        // first tile of the segment that is this CTA's
+  int end;         // past the last one; `tile` when the share is done
   int tiles;       // of the segment
-  int end;         // past the last tile that is this CTA's
+  int last_cta;    // that has the segment's last tile
   BlockView view;
   int64_t out_row;  // the chunk's first row of query and out
 
+  __device__ __forceinline__ int row_tiles() const { return view.rows > 128 ? 2 : 1; }
+
+  // The tiles of (block, head) that are this CTA's, none perhaps.
+  __device__ __forceinline__ void place() {
+    const int64_t stop = min(static_cast<int64_t>(tiles) + kSegmentCost, from + left);
+    tile = max(0, from - kSegmentCost);
+    end = max(tile, static_cast<int>(stop) - kSegmentCost);
+  }
   __device__ __forceinline__ void load(const AttendArgs& a, const ChunkArgs& c, const ChunkWorkspace& ws) {
     const ChunkBlock b = ws.blocks[block];
     out_row = __ldg(c.offsets + b.seq);
     const int tokens = static_cast<int>(__ldg(c.offsets + b.seq + 1) - out_row);
     view = view_of(a, b.seq, b.row, b.rows, tokens, sequence_length(a, b.seq));
     tiles = b.tiles;
-    end = static_cast<int>(min(static_cast<int64_t>(tiles), tile + left));
   }
-  // To the next segment; false when the share is done.
-  __device__ __forceinline__ bool next(const AttendArgs& a, const ChunkArgs& c, const ChunkWorkspace& ws) {
-    left -= end - tile;
-    if (left <= 0) return false;
-    tile = 0;
-    if (++head == a.kv_heads) {
-      head = 0;
-      do {
-        ++block;
-      } while (ws.blocks[block].tiles == 0);
-      load(a, c, ws);
-    }
-    end = static_cast<int>(min(static_cast<int64_t>(tiles), left));
-    return true;
+  // To the next segment with tiles of this CTA; without one, end == tile.
+  __device__ __forceinline__ void next(const AttendArgs& a, const ChunkArgs& c, const ChunkWorkspace& ws) {
+    do {
+      left -= tiles + kSegmentCost - from;
+      from = 0;
+      if (left <= kSegmentCost) {
+        end = tile;
+        return;
+      }
+      if (++head == a.kv_heads) {
+        head = 0;
+        do {
+          ++block;
+        } while (ws.blocks[block].tiles == 0);
+        load(a, c, ws);
+      }
+      place();
+    } while (end == tile);
   }
-  __device__ __forceinline__ int row_tiles() const { return view.rows > 128 ? 2 : 1; }
 };
 
 // A row whose output is not finite although its sum is: the tensor cores
@@ -442,11 +462,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kStages = Shape::kStages;
   constexpr int kTileBytes = Shape::kTileBytes;
   extern __shared__ unsigned char dynamic[];
-  __shared__ uint64_t bars[2 * kStages + 9];
+  __shared__ uint64_t bars[2 * kStages + 2 * kSlots + 9];
   __shared__ float row_unit[kRows];
   __shared__ uint32_t tmem_base;
   __shared__ int start_block;
-  __shared__ Share shares[kThreads / 32];
+  __shared__ Share shares[kSlots];
   __shared__ int abort_flag;
 
   const int lane = threadIdx.x & 31;
@@ -457,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t full = smem_addr(bars), empty = full + 8 * kStages;
   const uint32_t q_full = empty + 8 * kStages, q_empty = q_full + 8;
   const uint32_t s_full = q_full + 16, p_ready = q_full + 32, o_full = q_full + 48;
-  const uint32_t drained = q_full + 64;
+  const uint32_t drained = q_full + 64, announced = q_full + 72, released = announced + 8 * kSlots;
   volatile int* const abort = &abort_flag;
 
   if (threadIdx.x == 0) {
@@ -465,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       barrier_init(full + 8 * i, 128);
       barrier_init(empty + 8 * i, 1);
     }
-    barrier_init(q_full, 128);
+    barrier_init(q_full, 64);
     barrier_init(q_empty, 1 + kRows);
     for (int i = 0; i < 2; ++i) {
       barrier_init(s_full + 8 * i, 1);
@@ -473,6 +493,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       barrier_init(o_full + 8 * i, 1);
     }
     barrier_init(drained, 1);
+    for (int i = 0; i < kSlots; ++i) {
+      barrier_init(announced + 8 * i, 1);
+      barrier_init(released + 8 * i, kReaders);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     abort_flag = 0;
     start_block = 0;
@@ -505,24 +529,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after_sync();
   const uint32_t tmem = tmem_base;
 
-  Share& s = shares[warp];
-  if (working && lane == 0) {
-    s.left = share;
-    s.block = start_block;
-    const int64_t rest = begin - ws.first[s.block];
-    const int tiles = ws.blocks[s.block].tiles;
-    s.head = static_cast<int>(rest / tiles);
-    s.tile = static_cast<int>(rest - static_cast<int64_t>(s.head) * tiles);
-    s.load(a, c, ws);
-  }
-  __syncwarp();
-  // The warp's copy of the share to its next segment.
-  auto next_segment = [&]() {
+  // Where 16-byte chunk `ch` of row r of a tile lies.
+  auto place = [](int r, int ch) {
+    return static_cast<uint32_t>((ch >> 3) * (kKeys * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+  };
+  // The segment that a warp turns to, and the end of its use of one.
+  auto announced_segment = [&](uint32_t n) {
+    return warp_wait(announced + 8 * (n % kSlots), (n / kSlots) & 1, abort, a.status);
+  };
+  auto release_segment = [&](uint32_t n) {
     __syncwarp();
-    int more = 0;
-    if (lane == 0) more = s.next(a, c, ws);
-    __syncwarp();
-    return __shfl_sync(0xffffffffu, more, 0) != 0;
+    if (lane == 0) barrier_arrive(released + 8 * (n % kSlots));
   };
 
   if (warp >= 12) {
@@ -555,11 +572,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mma_commit(s_full + 8 * q);
       };
-      do {
+      for (;; ++segment) {
+        ok = announced_segment(segment);
+        if (!ok) break;
+        const Share& s = shares[segment % kSlots];
         const int n = s.end - s.tile;
         const int row_tiles = s.row_tiles();
-        ok = ok && warp_wait(q_full, segment & 1, abort, a.status) &&
-             warp_wait(full + 8 * stage, round, abort, a.status);
+        release_segment(segment);
+        if (n == 0) break;
+        ok = warp_wait(q_full, segment & 1, abort, a.status) && warp_wait(full + 8 * stage, round, abort, a.status);
         if (!ok) break;
         fence_after_sync();
         if (issues) {
@@ -603,8 +624,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (more) step();
         }
-        ++segment;
-      } while (ok && next_segment());
+        if (!ok) break;
+      }
       if (!ok && issues) {
         // what was issued may still run: let it end before the memory goes
         mma_commit(drained);
@@ -613,92 +634,94 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
-  } else if (warp >= 8) {
-    // ---------------------------------------------------------------- loads
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (working) {
-      const int w = warp - 8;
-      constexpr int kRowChunks = DP / 8;             // of a row in shared memory
-      constexpr int kPerInstr = 32 / kRowChunks;     // rows per instruction (16-bit rows)
+    if (warp == 13 && lane == 0 && working) {
+      // -------------------------------------------------------- next segments
+      Share s;
+      s.left = share;
+      s.block = start_block;
+      const int64_t rest = begin - ws.first[s.block];
+      const int span = ws.blocks[s.block].tiles + kSegmentCost;
+      s.head = static_cast<int>(rest / span);
+      s.from = static_cast<int>(rest - static_cast<int64_t>(s.head) * span);
+      s.load(a, c, ws);
+      s.place();
+      if (s.end == s.tile) s.next(a, c, ws);
+      for (uint32_t n = 0;; ++n) {
+        if (n >= kSlots && !barrier_wait(released + 8 * (n % kSlots), (n / kSlots - 1) & 1, abort, a.status)) break;
+        // the CTA of the segment's last tile
+        const int64_t last = ws.first[s.block] + static_cast<int64_t>(s.head + 1) * (s.tiles + kSegmentCost) - 1;
+        s.last_cta = static_cast<int>((plan.ctas * (last + 1) - 1) / plan.tiles);
+        shares[n % kSlots] = s;
+        barrier_arrive(announced + 8 * (n % kSlots));
+        if (s.end == s.tile) break;
+        s.next(a, c, ws);
+      }
+    }
+    __syncwarp();
+    if (warp >= 14 && working) {
+      // -------------------------------------------------------------- queries
+      const int w = warp - 14;
+      constexpr int kRowChunks = DP / 8;
+      constexpr int kPerInstr = 32 / kRowChunks;
       const int chunk = lane % kRowChunks, sub = lane / kRowChunks;
-      // Where 16-byte chunk `ch` of row r of a tile lies.
-      auto place = [](int r, int ch) {
-        return static_cast<uint32_t>((ch >> 3) * (kKeys * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
-      };
+      constexpr int kBatch = 8;  // rows of a lane in flight through registers; 8 * kPerInstr divides 32
       bool ok = true;
-      uint32_t issued = 0, arrived = 0;
-      uint32_t segment = 0;
-      constexpr uint32_t kAhead = 2;  // tiles in flight behind the one being issued
-      bool queries = false;           // in flight, before any tile
-      // Hands over the oldest of what is in flight.
-      auto complete = [&]() {
-        fence_async_proxy();
-        if (queries) {
-          barrier_arrive(q_full);
-          queries = false;
-        } else {
-          barrier_arrive(full + 8 * (arrived % kStages));
-          ++arrived;
-        }
-      };
-      auto drain = [&]() {
-        for (uint32_t left = issued - arrived + (queries ? 1 : 0); left > 0; --left) {
-          if (left == 3)
-            cp_async_wait<2>();
-          else if (left == 2)
-            cp_async_wait<1>();
-          else
-            cp_async_wait<0>();
-          complete();
-        }
-      };
-      // The ring entry of the next tile.  Before it waits for one, a warp
-      // hands over what it has in flight.
-      auto claim = [&]() {
-        if (issued < kStages || !ok) return;
-        const uint32_t bar = empty + 8 * (issued % kStages), parity = ((issued / kStages) - 1) & 1;
-        if (__all_sync(0xffffffffu, barrier_test(bar, parity))) return;
-        if constexpr (!kE4m3) drain();
-        ok = warp_wait(bar, parity, abort, a.status);
-      };
-      constexpr int64_t kHidden = -1ll << 62;
-      do {
+      for (uint32_t segment = 0;; ++segment) {
+        ok = announced_segment(segment);
+        if (!ok) break;
+        const Share& s = shares[segment % kSlots];
+        if (s.end == s.tile) break;
         // Queries.  With e4m3 they go through registers, times a power of two
         // per row (see attend_step.cu); so they do when the sign of a negative
         // scale or the zeros of a zero one go into them.
-        if (segment > 0) ok = ok && warp_wait(q_empty, (segment - 1) & 1, abort, a.status);
+        if (segment > 0) ok = warp_wait(q_empty, (segment - 1) & 1, abort, a.status);
         if (!ok) break;
-        auto query_row = [&](int r) -> const uint4* {
-          if (r >= s.view.rows || chunk >= row_chunks) return nullptr;
+        // a lane finds four of the warp's 128 rows
+        unsigned long long row_at[4];
+        unsigned live[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const int r = w * 128 + h * 32 + lane;
           const int row = s.view.row + r, token = row / a.group;
           const uint16_t* src = static_cast<const uint16_t*>(a.query) + (s.out_row + token) * a.query_row +
                                 static_cast<int64_t>(s.head * a.group + row - token * a.group) * a.query_head;
-          return reinterpret_cast<const uint4*>(src) + chunk;
-        };
+          live[h] = __ballot_sync(0xffffffffu, r < s.view.rows);
+          row_at[h] = reinterpret_cast<unsigned long long>(r < s.view.rows ? src : a.query);
+          if (!kE4m3) row_unit[r] = c.scale_log2;
+        }
+        const uint32_t queries = smem + w * kTileBytes;
         if (!kE4m3 && c.query_and == 0xffffffffu && c.query_xor == 0u) {
-#pragma unroll 4
-          for (int r = w * 64 + sub; r < w * 64 + 64; r += kPerInstr) {
-            const uint4* src = query_row(r);
-            if (chunk < row_chunks)
-              cp_async16(smem + (r >> 7) * kTileBytes + place(r & 127, chunk), src != nullptr ? src : a.query,
-                         src != nullptr);
-            if (chunk == 0) row_unit[r] = c.scale_log2;
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const char* src[32 / kPerInstr];
+#pragma unroll
+            for (int i = 0; i < 32 / kPerInstr; ++i)
+              src[i] = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row_at[h], i * kPerInstr + sub)) + chunk * 16;
+            if (chunk < row_chunks) {
+#pragma unroll
+              for (int i = 0; i < 32 / kPerInstr; ++i)
+                cp_async16(queries + place(h * 32 + i * kPerInstr + sub, chunk), src[i],
+                           (live[h] >> (i * kPerInstr + sub)) & 1u);
+            }
           }
           cp_async_commit();
-          queries = true;
+          cp_async_wait<0>();
         } else {
-          constexpr int kBatch = 8;
 #pragma unroll 1
-          for (int r0 = w * 64 + sub; r0 < w * 64 + 64; r0 += kBatch * kPerInstr) {
+          for (int r0 = 0; r0 < 128; r0 += kBatch * kPerInstr) {
+            const int h = r0 >> 5;
+            const unsigned long long mine = h == 0 ? row_at[0] : h == 1 ? row_at[1] : h == 2 ? row_at[2] : row_at[3];
+            const unsigned mask = h == 0 ? live[0] : h == 1 ? live[1] : h == 2 ? live[2] : live[3];
             uint4 x[kBatch];
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-              const uint4* src = query_row(r0 + i * kPerInstr);
-              x[i] = src != nullptr ? __ldg(src) : make_uint4(0, 0, 0, 0);
+              const int from = (r0 & 31) + i * kPerInstr + sub;
+              const uint4* src = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, mine, from)) + chunk;
+              x[i] = ((mask >> from) & 1u) && chunk < row_chunks ? __ldg(src) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-              const int r = r0 + i * kPerInstr;
+              const int r = r0 + i * kPerInstr + sub;
               uint32_t word[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
               float unit = c.scale_log2;
               if constexpr (kE4m3) {
@@ -718,18 +741,68 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int j = 0; j < 4; ++j) word[j] = pack2<false>(f[j].x * up, f[j].y * up);
                 unit *= ldexpf(1.f, -e);
               }
-              if (chunk == 0) row_unit[r] = unit;
+              if (kE4m3 && chunk == 0) row_unit[w * 128 + r] = unit;
 #pragma unroll
               for (int j = 0; j < 4; ++j) word[j] = (word[j] & c.query_and) ^ c.query_xor;
               if (chunk < row_chunks)
-                *reinterpret_cast<uint4*>(smem_ptr + (r >> 7) * kTileBytes + place(r & 127, chunk)) =
+                *reinterpret_cast<uint4*>(smem_ptr + w * kTileBytes + place(r, chunk)) =
                     make_uint4(word[0], word[1], word[2], word[3]);
             }
           }
-          fence_async_proxy();
-          barrier_arrive(q_full);
         }
-
+        fence_async_proxy();
+        barrier_arrive(q_full);
+        release_segment(segment);
+      }
+    }
+  } else if (warp >= 8) {
+    // ---------------------------------------------------------------- loads
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (working) {
+      const int w = warp - 8;
+      constexpr int kRowChunks = DP / 8;             // of a row in shared memory
+      constexpr int kPerInstr = 32 / kRowChunks;     // rows per instruction (16-bit rows)
+      const int chunk = lane % kRowChunks, sub = lane / kRowChunks;
+      bool ok = true;
+      uint32_t issued = 0, arrived = 0;
+      uint32_t segment = 0;
+      constexpr uint32_t kAhead = 2;  // tiles in flight behind the one being issued
+      // Hands over the oldest of the tiles in flight.
+      auto complete = [&]() {
+        fence_async_proxy();
+        barrier_arrive(full + 8 * (arrived % kStages));
+        ++arrived;
+      };
+      auto drain = [&]() {
+        while (arrived < issued) {
+          if (issued - arrived == kAhead)
+            cp_async_wait<kAhead - 1>();
+          else
+            cp_async_wait<0>();
+          complete();
+        }
+      };
+      // The ring entry of the next tile.  Before it waits for one, a warp
+      // hands over what it has in flight.
+      auto claim = [&]() {
+        if (issued < kStages || !ok) return;
+        const uint32_t bar = empty + 8 * (issued % kStages), parity = ((issued / kStages) - 1) & 1;
+        if (__all_sync(0xffffffffu, barrier_test(bar, parity))) return;
+        if constexpr (!kE4m3) drain();
+        ok = warp_wait(bar, parity, abort, a.status);
+      };
+      constexpr int64_t kHidden = -1ll << 62;
+      for (; ok; ++segment) {
+        if constexpr (!kE4m3) {
+          // nothing in flight is held back while the next segment is awaited
+          if (arrived < issued &&
+              !__all_sync(0xffffffffu, barrier_test(announced + 8 * (segment % kSlots), (segment / kSlots) & 1)))
+            drain();
+        }
+        ok = announced_segment(segment);
+        if (!ok) break;
+        const Share& s = shares[segment % kSlots];
+        if (s.end == s.tile) break;
         // keys and values, tile by tile; a lane looks up the page of one token
         int64_t page;
         int offset = 0;
@@ -784,7 +857,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               cp_async_commit();
               ++issued;
-              if (issued - arrived + (queries ? 1 : 0) > kAhead) {
+              if (issued - arrived > kAhead) {
                 cp_async_wait<kAhead>();
                 complete();
               }
@@ -822,13 +895,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        // what is still in flight: its readers may have to finish before this
-        // segment's queries leave
-        if constexpr (!kE4m3) {
-          drain();
-        }
-        ++segment;
-      } while (ok && next_segment());
+        release_segment(segment);
+      }
+      if constexpr (!kE4m3) drain();
       cp_async_wait<0>();
     }
   } else {
@@ -842,9 +911,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (working) {
       bool ok = true;
       uint32_t segment = 0, phase = 0, o_phase = 0;
-      int64_t done = 0;  // tiles of the share before this segment
-      do {
-        ok = ok && warp_wait(q_full, segment & 1, abort, a.status);
+      for (;; ++segment) {
+        ok = announced_segment(segment);
+        if (!ok) break;
+        const Share& s = shares[segment % kSlots];
+        if (s.end == s.tile) break;
+        ok = warp_wait(q_full, segment & 1, abort, a.status);
         if (!ok) break;
         const float unit = row_unit[r];
         barrier_arrive(q_empty);
@@ -875,15 +947,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_wait_load();
 #pragma unroll
             for (int j = 0; j < 4; ++j) tmem_landed(x[j]);
-            if (v0 + kKeys - 1 > all_last || (v0 + kKeys > a.sinks && max(v0, a.sinks) <= all_low)) {
-              const int last = v_last - v0, low = v_low - v0, sinks = a.sinks - v0;
+            // Hidden keys: behind the row's own token, which only the block's
+            // last tiles have, or between the sinks and the window.
+            if (v0 + kKeys - 1 > all_last) {
+              const int last = v_last - v0;
 #pragma unroll
               for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                  const int v = j * 32 + k;
-                  if (v > last || (v <= low && v >= sinks)) x[j][k] = -INFINITY;
-                }
+                for (int k = 0; k < 32; ++k) x[j][k] = j * 32 + k > last ? -INFINITY : x[j][k];
+            }
+            if (v0 + kKeys > a.sinks && max(v0, a.sinks) <= all_low) {
+              const int first = a.sinks - v0;
+              const unsigned gap = max(v_low - v0 + 1 - first, 0);
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                  x[j][k] = static_cast<unsigned>(j * 32 + k - first) < gap ? -INFINITY : x[j][k];
             }
             float top[4];
 #pragma unroll
@@ -914,7 +994,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             l = l * decay + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
             if (i > 0 && __any_sync(0xffffffffu, m != old)) {
-#pragma unroll
+#pragma unroll 1
               for (int j = 0; j < DP / 32; ++j) {
                 float o[32];
                 tmem_load32(o, output + j * 32);
@@ -946,7 +1026,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float* const part = ws.acc + (slot * kRows + r) * DP;
           uint16_t* const out = static_cast<uint16_t*>(a.out) + out_row * a.dim;
           bool finite = true;
-#pragma unroll
+#pragma unroll 1
           for (int j = 0; j < DP / 32; ++j) {
             float o[32];
             __syncwarp();
@@ -1013,15 +1093,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int id = s.block * a.kv_heads + s.head;
           if (starts) {
             piece.head = id;
-            const int64_t last = begin + done + s.tiles - 1;
-            piece.last = static_cast<int>((plan.ctas * (last + 1) - 1) / plan.tiles);
+            piece.last = s.last_cta;
           } else {
             piece.tail = id;
           }
         }
-        done += n;
-        ++segment;
-      } while (next_segment());
+        release_segment(segment);
+      }
     }
     if (threadIdx.x == 0 && working) ws.pieces[blockIdx.x] = piece;
   }
