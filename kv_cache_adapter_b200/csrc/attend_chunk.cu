@@ -232,19 +232,18 @@ __device__ __forceinline__ bool barrier_test(uint32_t bar, uint32_t parity) {
 // Waits for a phase; gives up, as every other warp of the CTA then does, after
 // kWaitTries tries (a try suspends the thread for a while) or once another
 // warp gave up.
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* abort, int64_t* status) {
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
   for (uint32_t i = 0; i < kWaitTries; ++i) {
     if (barrier_try(bar, parity)) return true;
     if ((i & 255u) == 255u && *abort) return false;
   }
   *abort = 1;
-  report(status, KVCA_ERR_DEVICE_TIMEOUT, blockIdx.x);
   return false;
 }
 
 // The same for a whole warp: every lane waits, and all go on or none.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort, int64_t* status) {
-  return __all_sync(0xffffffffu, barrier_wait(bar, parity, abort, status));
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, barrier_wait(bar, parity, abort));
 }
 
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -423,6 +422,7 @@ __device__ __forceinline__ void row_again(const AttendArgs& a, const ChunkArgs& 
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   const bool bf16 = a.query_type == KVCA_TYPE_BF16;
   const int v_end = min(s.view.count, s.end * kKeys);
+#pragma unroll 1
   for (int v = s.tile * kKeys; v < v_end; ++v) {
     if (v > v_last || (v >= a.sinks && v <= v_low)) continue;
     const int key = s.view.key(v);
@@ -440,6 +440,7 @@ __device__ __forceinline__ void row_again(const AttendArgs& a, const ChunkArgs& 
       }
     };
     float dot = 0.f;
+#pragma unroll 1
     for (int d = lane; d < a.dim; d += 32)
       dot += (bf16 ? unpack2<true>(q[d]).x : unpack2<false>(q[d]).x) * element(k, d);
 #pragma unroll
@@ -535,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   // The segment that a warp turns to, and the end of its use of one.
   auto announced_segment = [&](uint32_t n) {
-    return warp_wait(announced + 8 * (n % kSlots), (n / kSlots) & 1, abort, a.status);
+    return warp_wait(announced + 8 * (n % kSlots), (n / kSlots) & 1, abort);
   };
   auto release_segment = [&](uint32_t n) {
     __syncwarp();
@@ -555,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool issues = lane == 0;
       uint32_t stage = 0, round = 0;  // of the next ring entry
       uint32_t segment = 0;
-      uint32_t p_phase[2] = {0, 0};
+      uint32_t p_phase = 0;  // a bit per row tile
       bool ok = true;
       auto step = [&]() {
         if (++stage == kStages) {
@@ -580,12 +581,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int row_tiles = s.row_tiles();
         release_segment(segment);
         if (n == 0) break;
-        ok = warp_wait(q_full, segment & 1, abort, a.status) && warp_wait(full + 8 * stage, round, abort, a.status);
+        ok = warp_wait(q_full, segment & 1, abort) && warp_wait(full + 8 * stage, round, abort);
         if (!ok) break;
         fence_after_sync();
         if (issues) {
-          scores(0, stage);
-          if (row_tiles > 1) scores(1, stage);
+#pragma unroll 1
+          for (int q = 0; q < row_tiles; ++q) scores(q, stage);
           mma_commit(empty + 8 * stage);
           if (n == 1) mma_commit(q_empty);
         }
@@ -593,15 +594,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < n; ++i) {
           const uint32_t values_at = stage;
           const bool more = i + 1 < n;
-          ok = ok && warp_wait(full + 8 * stage, round, abort, a.status);
+          ok = ok && warp_wait(full + 8 * stage, round, abort);
           step();
           const uint32_t keys_at = stage;
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            if (q >= row_tiles) break;
-            ok = ok && warp_wait(p_ready + 8 * q, p_phase[q] & 1, abort, a.status);
-            ++p_phase[q];
-            if (more && q == 0) ok = ok && warp_wait(full + 8 * stage, round, abort, a.status);
+#pragma unroll 1
+          for (int q = 0; q < row_tiles; ++q) {
+            ok = ok && warp_wait(p_ready + 8 * q, (p_phase >> q) & 1, abort);
+            p_phase ^= 1u << q;
+            if (more && q == 0) ok = ok && warp_wait(full + 8 * stage, round, abort);
             if (!ok) break;
             fence_after_sync();
             if (issues) {
@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       s.place();
       if (s.end == s.tile) s.next(a, c, ws);
       for (uint32_t n = 0;; ++n) {
-        if (n >= kSlots && !barrier_wait(released + 8 * (n % kSlots), (n / kSlots - 1) & 1, abort, a.status)) break;
+        if (n >= kSlots && !barrier_wait(released + 8 * (n % kSlots), (n / kSlots - 1) & 1, abort)) break;
         // the CTA of the segment's last tile
         const int64_t last = ws.first[s.block] + static_cast<int64_t>(s.head + 1) * (s.tiles + kSegmentCost) - 1;
         s.last_cta = static_cast<int>((plan.ctas * (last + 1) - 1) / plan.tiles);
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr int kRowChunks = DP / 8;
       constexpr int kPerInstr = 32 / kRowChunks;
       const int chunk = lane % kRowChunks, sub = lane / kRowChunks;
-      constexpr int kBatch = 8;  // rows of a lane in flight through registers; 8 * kPerInstr divides 32
+      constexpr int kBatch = 8;  // rows of a lane in flight through registers; kBatch * kPerInstr divides 32
       bool ok = true;
       for (uint32_t segment = 0;; ++segment) {
         ok = announced_segment(segment);
@@ -674,54 +674,45 @@ __global__ void __launch_bounds__(kThreads, 1)
         // Queries.  With e4m3 they go through registers, times a power of two
         // per row (see attend_step.cu); so they do when the sign of a negative
         // scale or the zeros of a zero one go into them.
-        if (segment > 0) ok = warp_wait(q_empty, (segment - 1) & 1, abort, a.status);
+        if (segment > 0) ok = warp_wait(q_empty, (segment - 1) & 1, abort);
         if (!ok) break;
-        // a lane finds four of the warp's 128 rows
-        unsigned long long row_at[4];
-        unsigned live[4];
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const int r = w * 128 + h * 32 + lane;
-          const int row = s.view.row + r, token = row / a.group;
-          const uint16_t* src = static_cast<const uint16_t*>(a.query) + (s.out_row + token) * a.query_row +
-                                static_cast<int64_t>(s.head * a.group + row - token * a.group) * a.query_head;
-          live[h] = __ballot_sync(0xffffffffu, r < s.view.rows);
-          row_at[h] = reinterpret_cast<unsigned long long>(r < s.view.rows ? src : a.query);
-          if (!kE4m3) row_unit[r] = c.scale_log2;
-        }
         const uint32_t queries = smem + w * kTileBytes;
-        if (!kE4m3 && c.query_and == 0xffffffffu && c.query_xor == 0u) {
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
+        const bool as_is = !kE4m3 && c.query_and == 0xffffffffu && c.query_xor == 0u;
+#pragma unroll 1
+        for (int r0 = 0; r0 < 128 && w < s.row_tiles(); r0 += 32) {  // a lane finds one of 32 rows
+          const int r = w * 128 + r0 + lane;
+          const int row = s.view.row + r, token = row / a.group;
+          const uint16_t* own = static_cast<const uint16_t*>(a.query) + (s.out_row + token) * a.query_row +
+                                static_cast<int64_t>(s.head * a.group + row - token * a.group) * a.query_head;
+          const bool live = r < s.view.rows;
+          const unsigned lives = __ballot_sync(0xffffffffu, live);
+          const unsigned long long row_at = reinterpret_cast<unsigned long long>(live ? own : a.query);
+          if (!kE4m3) row_unit[r] = c.scale_log2;
+          if (as_is) {
             const char* src[32 / kPerInstr];
 #pragma unroll
             for (int i = 0; i < 32 / kPerInstr; ++i)
-              src[i] = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row_at[h], i * kPerInstr + sub)) + chunk * 16;
+              src[i] = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row_at, i * kPerInstr + sub)) + chunk * 16;
             if (chunk < row_chunks) {
 #pragma unroll
               for (int i = 0; i < 32 / kPerInstr; ++i)
-                cp_async16(queries + place(h * 32 + i * kPerInstr + sub, chunk), src[i],
-                           (live[h] >> (i * kPerInstr + sub)) & 1u);
+                cp_async16(queries + place(r0 + i * kPerInstr + sub, chunk), src[i],
+                           (lives >> (i * kPerInstr + sub)) & 1u);
             }
+            continue;
           }
-          cp_async_commit();
-          cp_async_wait<0>();
-        } else {
 #pragma unroll 1
-          for (int r0 = 0; r0 < 128; r0 += kBatch * kPerInstr) {
-            const int h = r0 >> 5;
-            const unsigned long long mine = h == 0 ? row_at[0] : h == 1 ? row_at[1] : h == 2 ? row_at[2] : row_at[3];
-            const unsigned mask = h == 0 ? live[0] : h == 1 ? live[1] : h == 2 ? live[2] : live[3];
+          for (int r1 = 0; r1 < 32; r1 += kBatch * kPerInstr) {
             uint4 x[kBatch];
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-              const int from = (r0 & 31) + i * kPerInstr + sub;
-              const uint4* src = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, mine, from)) + chunk;
-              x[i] = ((mask >> from) & 1u) && chunk < row_chunks ? __ldg(src) : make_uint4(0, 0, 0, 0);
+              const int from = r1 + i * kPerInstr + sub;
+              const uint4* src = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, row_at, from)) + chunk;
+              x[i] = ((lives >> from) & 1u) && chunk < row_chunks ? __ldg(src) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-              const int r = r0 + i * kPerInstr + sub;
+              const int at = r0 + r1 + i * kPerInstr + sub;
               uint32_t word[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
               float unit = c.scale_log2;
               if constexpr (kE4m3) {
@@ -741,15 +732,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int j = 0; j < 4; ++j) word[j] = pack2<false>(f[j].x * up, f[j].y * up);
                 unit *= ldexpf(1.f, -e);
               }
-              if (kE4m3 && chunk == 0) row_unit[w * 128 + r] = unit;
+              if (kE4m3 && chunk == 0) row_unit[w * 128 + at] = unit;
 #pragma unroll
               for (int j = 0; j < 4; ++j) word[j] = (word[j] & c.query_and) ^ c.query_xor;
               if (chunk < row_chunks)
-                *reinterpret_cast<uint4*>(smem_ptr + w * kTileBytes + place(r, chunk)) =
+                *reinterpret_cast<uint4*>(smem_ptr + w * kTileBytes + place(at, chunk)) =
                     make_uint4(word[0], word[1], word[2], word[3]);
             }
           }
         }
+        cp_async_wait_all();
         fence_async_proxy();
         barrier_arrive(q_full);
         release_segment(segment);
@@ -789,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t bar = empty + 8 * (issued % kStages), parity = ((issued / kStages) - 1) & 1;
         if (__all_sync(0xffffffffu, barrier_test(bar, parity))) return;
         if constexpr (!kE4m3) drain();
-        ok = warp_wait(bar, parity, abort, a.status);
+        ok = warp_wait(bar, parity, abort);
       };
       constexpr int64_t kHidden = -1ll << 62;
       for (; ok; ++segment) {
@@ -823,26 +815,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!good && page != kHidden) report(a.status, KVCA_ERR_BAD_INDEX, page);
           const int64_t block = good ? page : 0;
           const unsigned seen = __ballot_sync(0xffffffffu, good);
-          const char* rows[2];
-          rows[0] = a.key + block * a.key_block + offset * a.key_token + s.head * a.key_head;
-          rows[1] = a.value + block * a.value_block + offset * a.value_token + s.head * a.value_head;
+          const char* const key_row = a.key + block * a.key_block + offset * a.key_token + s.head * a.key_head;
+          const char* const value_row = a.value + block * a.value_block + offset * a.value_token + s.head * a.value_head;
           if (tile + 1 < s.end) look_up(tile + 1);
-          const char* src[32 / kPerInstr];
-#pragma unroll
+#pragma unroll 1
           for (int side = 0; side < 2; ++side) {
-            const unsigned long long row = reinterpret_cast<unsigned long long>(rows[side]);
+            const unsigned long long row = reinterpret_cast<unsigned long long>(side == 0 ? key_row : value_row);
             if constexpr (!kE4m3) {
               claim();
               if (!ok) break;
               const uint32_t dst = kv_smem + (issued % kStages) * kTileBytes;
-              if (side == 0 || !c.same_layout) {
+              const char* src[32 / kPerInstr];
 #pragma unroll
-                for (int i = 0; i < 32 / kPerInstr; ++i)
-                  src[i] = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, i * kPerInstr + sub)) + chunk * 16;
-              } else {
-#pragma unroll
-                for (int i = 0; i < 32 / kPerInstr; ++i) src[i] += a.value - a.key;
-              }
+              for (int i = 0; i < 32 / kPerInstr; ++i)
+                src[i] = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, i * kPerInstr + sub)) + chunk * 16;
               if (chunk < row_chunks) {
                 if (seen == 0xffffffffu) {
 #pragma unroll
@@ -916,7 +902,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         const Share& s = shares[segment % kSlots];
         if (s.end == s.tile) break;
-        ok = warp_wait(q_full, segment & 1, abort, a.status);
+        ok = warp_wait(q_full, segment & 1, abort);
         if (!ok) break;
         const float unit = row_unit[r];
         barrier_arrive(q_empty);
@@ -937,7 +923,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           int v0 = s.tile * kKeys;
 #pragma unroll 1
           for (int i = 0; i < n; ++i, v0 += kKeys) {
-            ok = ok && warp_wait(s_full + 8 * q, phase & 1, abort, a.status);
+            ok = ok && warp_wait(s_full + 8 * q, phase & 1, abort);
             if (!ok) break;
             ++phase;
             fence_after_sync();
@@ -1009,7 +995,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             fence_before_sync();
             barrier_arrive(p_ready + 8 * q);
           }
-          ok = ok && warp_wait(o_full + 8 * q, o_phase & 1, abort, a.status);
+          ok = ok && warp_wait(o_full + 8 * q, o_phase & 1, abort);
           if (!ok) break;
           ++o_phase;
           fence_after_sync();
@@ -1105,6 +1091,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   fence_before_sync();
   __syncthreads();
+  if (threadIdx.x == 0 && abort_flag != 0) report(a.status, KVCA_ERR_DEVICE_TIMEOUT, blockIdx.x);
   if (warp == 12) {
     fence_after_sync();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
@@ -1217,7 +1204,6 @@ cudaError_t launch_attend_chunk(const AttendArgs& args, const int64_t* offsets, 
   c.max_blocks = static_cast<int>(attend_chunk_max_blocks(a, rows));
   // the softmax takes the maximum of the raw scores, so their factor is positive
   c.scale_log2 = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
-  c.same_layout = a.key_block == a.value_block && a.key_token == a.value_token && a.key_head == a.value_head;
   c.query_and = a.scale_log2 == 0.f ? 0u : 0xffffffffu;
   c.query_xor = a.scale_log2 < 0.f ? 0x80008000u : 0u;
   switch (a.cache_type) {

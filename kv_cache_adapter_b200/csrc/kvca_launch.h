@@ -154,7 +154,6 @@ struct ChunkArgs {
   int max_blocks;          // blocks that the offsets can make of them
   float scale_log2;
   uint32_t query_and, query_xor;
-  bool same_layout;        // K and V have the same strides
 };
 
 size_t attend_step_workspace(const AttendArgs& args, int sms);
