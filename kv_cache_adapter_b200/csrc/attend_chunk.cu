@@ -47,7 +47,7 @@ constexpr int kSlots = 4;       // segments announced ahead
 constexpr int kReaders = 15;    // warps that read them
 // What a segment costs beside its tiles, in tiles: queries, first loads, the
 // output.  It counts when the tiles are dealt out, as tiles before the first.
-constexpr int kSegmentCost = 1;
+constexpr int kSegmentCost = 3;
 constexpr float kGrowth = 8.f;  // log2 of how far a maximum may lag
 constexpr uint32_t kWaitTries = 1u << 22;
 
@@ -56,7 +56,8 @@ struct ChunkShape {
   static constexpr int kHalves = DP / 64;                 // 64 dims (128 bytes) each
   static constexpr int kTileBytes = kHalves * kKeys * 128;  // 128 rows of DP 16-bit values
   static constexpr int kStages = 128 * 1024 / kTileBytes;
-  static constexpr int kSmem = 1024 + 2 * kTileBytes + kStages * kTileBytes;
+  static constexpr int kQueries = DP == 64 ? 2 : 1;        // segments whose queries are there at once
+  static constexpr int kSmem = 1024 + (2 * kQueries + kStages) * kTileBytes;
 };
 
 // ---------------------------------------------------------------------------
@@ -462,9 +463,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr bool kE4m3 = Cache::kBytes == 1;
   constexpr int kStages = Shape::kStages;
   constexpr int kTileBytes = Shape::kTileBytes;
+  constexpr int kQueries = Shape::kQueries;
   extern __shared__ unsigned char dynamic[];
-  __shared__ uint64_t bars[2 * kStages + 2 * kSlots + 9];
-  __shared__ float row_unit[kRows];
+  __shared__ uint64_t bars[2 * kStages + 2 * kSlots + 2 * kQueries + 7];
+  __shared__ float row_unit[kQueries][kRows];
   __shared__ uint32_t tmem_base;
   __shared__ int start_block;
   __shared__ Share shares[kSlots];
@@ -474,11 +476,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5;
   const uint32_t smem = (smem_addr(dynamic) + 1023u) & ~1023u;
   unsigned char* const smem_ptr = dynamic + (smem - smem_addr(dynamic));
-  const uint32_t kv_smem = smem + 2 * kTileBytes;
+  const uint32_t kv_smem = smem + 2 * kQueries * kTileBytes;
   const uint32_t full = smem_addr(bars), empty = full + 8 * kStages;
-  const uint32_t q_full = empty + 8 * kStages, q_empty = q_full + 8;
-  const uint32_t s_full = q_full + 16, p_ready = q_full + 32, o_full = q_full + 48;
-  const uint32_t drained = q_full + 64, announced = q_full + 72, released = announced + 8 * kSlots;
+  const uint32_t q_full = empty + 8 * kStages, q_empty = q_full + 8 * kQueries;
+  const uint32_t s_full = q_empty + 8 * kQueries, p_ready = s_full + 16, o_full = s_full + 32;  // per row tile
+  const uint32_t drained = s_full + 48, announced = s_full + 56, released = announced + 8 * kSlots;
   volatile int* const abort = &abort_flag;
 
   if (threadIdx.x == 0) {
@@ -486,8 +488,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       barrier_init(full + 8 * i, 128);
       barrier_init(empty + 8 * i, 1);
     }
-    barrier_init(q_full, 64);
-    barrier_init(q_empty, 1 + kRows);
+    for (int i = 0; i < kQueries; ++i) {
+      barrier_init(q_full + 8 * i, 64);
+      barrier_init(q_empty + 8 * i, 1 + kRows);
+    }
     for (int i = 0; i < 2; ++i) {
       barrier_init(s_full + 8 * i, 1);
       barrier_init(p_ready + 8 * i, 128);
@@ -510,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Padded dims stay zero: no copy writes them.
   const int row_chunks = a.dim / 8;  // 16-byte chunks of 16-bit values
   if (row_chunks < DP / 8)
-    for (int i = threadIdx.x; i < (kStages + 2) * kTileBytes / 16; i += kThreads)
+    for (int i = threadIdx.x; i < (kStages + 2 * kQueries) * kTileBytes / 16; i += kThreads)
       reinterpret_cast<uint4*>(smem_ptr)[i] = make_uint4(0, 0, 0, 0);
   fence_async_proxy();
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -534,6 +538,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto place = [](int r, int ch) {
     return static_cast<uint32_t>((ch >> 3) * (kKeys * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
   };
+  auto queries_barrier = [&](uint32_t bar, uint32_t n) { return bar + 8 * (n % kQueries); };
+  auto queries_parity = [&](uint32_t n) { return (n / kQueries) & 1u; };
   // The segment that a warp turns to, and the end of its use of one.
   auto announced_segment = [&](uint32_t n) {
     return warp_wait(announced + 8 * (n % kSlots), (n / kSlots) & 1, abort);
@@ -551,7 +557,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t kScores = mma_shape(kBf16, 128, kKeys, false);
       constexpr uint32_t kOutput = mma_shape(kBf16, 128, DP, true);
       constexpr uint32_t kHalf = kKeys * 128 >> 4;  // between 64 dims, in descriptor units
-      const uint32_t q_low = operand_low(smem, 16), k_low = operand_low(kv_smem, 16);
+      uint32_t q_low = 0;  // this segment's queries
+      const uint32_t k_low = operand_low(kv_smem, 16);
       const uint32_t v_low = operand_low(kv_smem, kKeys * 128);
       const bool issues = lane == 0;
       uint32_t stage = 0, round = 0;  // of the next ring entry
@@ -581,14 +588,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int row_tiles = s.row_tiles();
         release_segment(segment);
         if (n == 0) break;
-        ok = warp_wait(q_full, segment & 1, abort) && warp_wait(full + 8 * stage, round, abort);
+        q_low = operand_low(smem, 16) + 2 * (segment % kQueries) * (kTileBytes >> 4);
+        ok = warp_wait(queries_barrier(q_full, segment), queries_parity(segment), abort) && warp_wait(full + 8 * stage, round, abort);
         if (!ok) break;
         fence_after_sync();
         if (issues) {
 #pragma unroll 1
           for (int q = 0; q < row_tiles; ++q) scores(q, stage);
           mma_commit(empty + 8 * stage);
-          if (n == 1) mma_commit(q_empty);
+          if (n == 1) mma_commit(queries_barrier(q_empty, segment));
         }
         step();
         for (int i = 0; i < n; ++i) {
@@ -620,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (issues) {
             mma_commit(empty + 8 * values_at);
             if (more) mma_commit(empty + 8 * keys_at);
-            if (i + 2 == n) mma_commit(q_empty);  // the last scores of the segment were just issued
+            if (i + 2 == n) mma_commit(queries_barrier(q_empty, segment));  // the last scores of the segment were just issued
           }
           if (more) step();
         }
@@ -672,11 +680,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const Share& s = shares[segment % kSlots];
         if (s.end == s.tile) break;
         // Queries.  With e4m3 they go through registers, times a power of two
-        // per row (see attend_step.cu); so they do when the sign of a negative
+        // per row (power_up); so they do when the sign of a negative
         // scale or the zeros of a zero one go into them.
-        if (segment > 0) ok = warp_wait(q_empty, (segment - 1) & 1, abort);
+        if (segment >= kQueries)
+          ok = warp_wait(queries_barrier(q_empty, segment), queries_parity(segment - kQueries), abort);
         if (!ok) break;
-        const uint32_t queries = smem + w * kTileBytes;
+        const uint32_t tile = (2 * (segment % kQueries) + w) * kTileBytes;  // of this warp's 128 rows
+        float* const unit_of = row_unit[segment % kQueries] + w * 128;
         const bool as_is = !kE4m3 && c.query_and == 0xffffffffu && c.query_xor == 0u;
 #pragma unroll 1
         for (int r0 = 0; r0 < 128 && w < s.row_tiles(); r0 += 32) {  // a lane finds one of 32 rows
@@ -687,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool live = r < s.view.rows;
           const unsigned lives = __ballot_sync(0xffffffffu, live);
           const unsigned long long row_at = reinterpret_cast<unsigned long long>(live ? own : a.query);
-          if (!kE4m3) row_unit[r] = c.scale_log2;
+          if (!kE4m3) unit_of[r0 + lane] = c.scale_log2;
           if (as_is) {
             const char* src[32 / kPerInstr];
 #pragma unroll
@@ -696,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (chunk < row_chunks) {
 #pragma unroll
               for (int i = 0; i < 32 / kPerInstr; ++i)
-                cp_async16(queries + place(r0 + i * kPerInstr + sub, chunk), src[i],
+                cp_async16(smem + tile + place(r0 + i * kPerInstr + sub, chunk), src[i],
                            (lives >> (i * kPerInstr + sub)) & 1u);
             }
             continue;
@@ -726,24 +736,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
 #pragma unroll
                 for (int o = kRowChunks / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-                const int e = big > 0.f && big < INFINITY ? min(max(12 - ilogbf(big), -120), 120) : 0;
-                const float up = ldexpf(1.f, e);
+                const int e = power_up(big);
+                const float up = power_of_two(e);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) word[j] = pack2<false>(f[j].x * up, f[j].y * up);
-                unit *= ldexpf(1.f, -e);
+                unit *= power_of_two(-e);
               }
-              if (kE4m3 && chunk == 0) row_unit[w * 128 + at] = unit;
+              if (kE4m3 && chunk == 0) unit_of[at] = unit;
 #pragma unroll
               for (int j = 0; j < 4; ++j) word[j] = (word[j] & c.query_and) ^ c.query_xor;
               if (chunk < row_chunks)
-                *reinterpret_cast<uint4*>(smem_ptr + w * kTileBytes + place(at, chunk)) =
+                *reinterpret_cast<uint4*>(smem_ptr + tile + place(at, chunk)) =
                     make_uint4(word[0], word[1], word[2], word[3]);
             }
           }
         }
         cp_async_wait_all();
         fence_async_proxy();
-        barrier_arrive(q_full);
+        barrier_arrive(queries_barrier(q_full, segment));
         release_segment(segment);
       }
     }
@@ -830,16 +840,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int i = 0; i < 32 / kPerInstr; ++i)
                 src[i] = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, i * kPerInstr + sub)) + chunk * 16;
               if (chunk < row_chunks) {
-                if (seen == 0xffffffffu) {
 #pragma unroll
-                  for (int i = 0; i < 32 / kPerInstr; ++i)
-                    cp_async16(dst + place(w * 32 + i * kPerInstr + sub, chunk), src[i]);
-                } else {
-#pragma unroll
-                  for (int i = 0; i < 32 / kPerInstr; ++i)
-                    cp_async16(dst + place(w * 32 + i * kPerInstr + sub, chunk), src[i],
-                               (seen >> (i * kPerInstr + sub)) & 1u);
-                }
+                for (int i = 0; i < 32 / kPerInstr; ++i)
+                  cp_async16(dst + place(w * 32 + i * kPerInstr + sub, chunk), src[i],
+                             (seen >> (i * kPerInstr + sub)) & 1u);
               }
               cp_async_commit();
               ++issued;
@@ -861,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               claim();
               if (!ok) break;
-              unsigned char* const dst = smem_ptr + 2 * kTileBytes + (issued % kStages) * kTileBytes;
+              unsigned char* const dst = smem_ptr + 2 * kQueries * kTileBytes + (issued % kStages) * kTileBytes;
 #pragma unroll
               for (int i = 0; i < 32 / kRowsPer; ++i) {
                 const int r = w * 32 + i * kRowsPer + which;
@@ -902,10 +906,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         const Share& s = shares[segment % kSlots];
         if (s.end == s.tile) break;
-        ok = warp_wait(q_full, segment & 1, abort);
+        ok = warp_wait(queries_barrier(q_full, segment), queries_parity(segment), abort);
         if (!ok) break;
-        const float unit = row_unit[r];
-        barrier_arrive(q_empty);
+        const float unit = row_unit[segment % kQueries][r];
+        barrier_arrive(queries_barrier(q_empty, segment));
         const int n = s.end - s.tile;
         const bool starts = s.tile == 0, ends = s.end == s.tiles;
         if (q < s.row_tiles()) {

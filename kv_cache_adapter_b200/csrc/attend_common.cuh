@@ -94,6 +94,18 @@ __device__ __forceinline__ uint32_t e4m3_to_f16x2(uint32_t v) {
   return r;
 }
 
+// Powers of two that bring a row of queries, whose largest magnitude is
+// `big`, into fp16 for the products with e4m3 keys: the largest value falls
+// into [2^12, 2^13), so a bf16 row keeps its bits (values 2^-27 of the largest
+// and less fall among fp16's subnormals).  The inverse goes into the factor of
+// the scores.
+__device__ __forceinline__ int power_up(float big) {
+  const int exponent = static_cast<int>(__float_as_uint(big) >> 23);  // 0: zero or subnormal, 255: not finite
+  return exponent == 0 || exponent == 255 ? 0 : min(max(12 + 127 - exponent, -120), 120);
+}
+
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+
 // The tokens that the query at the end of a sequence of `len` tokens sees,
 // numbered 0 .. count - 1: the first `sinks` ones, then those of the window.
 struct Visible {

@@ -336,10 +336,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
               }
             unit[n][0] = unit[n][1] = a.scale_log2;
           } else {
-            // fp16 products: each row times a power of two that brings its
-            // largest value into [2^12, 2^13), so a bf16 row keeps its bits
-            // (values 2^-27 of the largest and less fall among fp16's
-            // subnormals); the inverse goes into the score factor.
+            // fp16 products, each row times a power of two (power_up)
             float big = 0.f;
             const bool bf16 = a.query_type == KVCA_TYPE_BF16;
             uint2 raw[kSteps];
@@ -353,8 +350,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
             }
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-            const int e = big > 0.f && big < INFINITY ? min(max(12 - ilogbf(big), -120), 120) : 0;
-            const float up = ldexpf(1.f, e);
+            const int e = power_up(big);
+            const float up = power_of_two(e);
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
               const float2 x = bf16 ? unpack2<true>(raw[k].x) : unpack2<false>(raw[k].x);
@@ -362,7 +359,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
               q[n][k][0] = pack2<false>(x.x * up, x.y * up);
               q[n][k][1] = pack2<false>(y.x * up, y.y * up);
             }
-            const float mine = a.scale_log2 * ldexpf(1.f, -e);
+            const float mine = a.scale_log2 * power_of_two(-e);
             unit[n][0] = __shfl_sync(0xffffffffu, mine, (2 * (lane & 3)) * 4);
             unit[n][1] = __shfl_sync(0xffffffffu, mine, (2 * (lane & 3) + 1) * 4);
           }
