@@ -31,9 +31,21 @@ constexpr int kTile = 16;         // tokens per tile: the rows of one m16n8k16
 constexpr int kScanGroups = 1024; // sequences (or runs of them) in the shared tile counts
 constexpr int kJoinThreads = 256;
 constexpr int kJoinChunk = 64;    // partial results weighted at a time
+// What a segment costs a warp beside its tiles (queries, the output), in
+// tiles.  It counts when the tiles are dealt out, as tiles before the first.
+#ifndef KVCA_STEP_COST
+#define KVCA_STEP_COST 2
+#endif
+constexpr int kSegmentCost = KVCA_STEP_COST;
+#ifndef KVCA_STEP_WARPS
+#define KVCA_STEP_WARPS 8
+#endif
 
-// Warps of a CTA: 8 with 24 KiB of ring each, 4 with 48 for rows of 512 bytes.
-__host__ __device__ constexpr int step_warps(int row_bytes) { return row_bytes > 256 ? 4 : 8; }
+// Warps of a CTA, which share 192 KiB of rings: stages of 32 rows, three of
+// them or more in a ring (two at 256-byte rows).
+__host__ __device__ constexpr int step_warps(int row_bytes, int head_tiles) {
+  return row_bytes > 256 ? 4 : row_bytes > 128 ? KVCA_STEP_WARPS : head_tiles > 1 && row_bytes > 64 ? 8 : 16;
+}
 
 // DP: head dim padded to 64, 128 or 256; NG: tiles of 8 query heads.
 template <typename Cache, int DP, int NG>
@@ -41,7 +53,7 @@ struct StepShape {
   static constexpr int kRowBytes = DP * Cache::kBytes;
   static constexpr int kChunks = kRowBytes / 16;       // 16-byte chunks of a row
   static constexpr int kStageBytes = 2 * kTile * kRowBytes;
-  static constexpr int kWarps = step_warps(kRowBytes);
+  static constexpr int kWarps = step_warps(kRowBytes, NG);
   static constexpr int kThreads = 32 * kWarps;
   // 192 KiB of rings per SM
   static constexpr int kRingBytes = 192 * 1024 / kWarps;
@@ -91,7 +103,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 
 // The workspace: the run bounds, then per warp ("worker") what it left.
 struct StepHeader {
-  int64_t tiles;    // of the whole call
+  int64_t tiles;    // of the whole call, segment costs included
   int64_t workers;  // that got tiles
 };
 
@@ -137,16 +149,21 @@ struct Cursor {
   int part;  // kv head * head groups + head group
   int tile;
   int tiles;  // of this sequence's visible tokens
+  int left;   // of the worker's share, this tile included; none when <= 0
   Visible vis;
 
   __device__ __forceinline__ void load(const AttendArgs& a) {
     vis = visible_tokens(max(sequence_length(a, seq), 0), a.window, a.sinks);
     tiles = (vis.count + kTile - 1) / kTile;
   }
-  // Called only while tiles remain, so a next sequence with tokens exists.
+  __device__ __forceinline__ bool ends() const { return tile + 1 == tiles; }
+  __device__ __forceinline__ bool last() const { return left <= (ends() ? 1 + kSegmentCost : 1); }
+  // To the next tile; only when this one is not the last.
   __device__ __forceinline__ void advance(const AttendArgs& a, int parts) {
+    --left;
     if (++tile < tiles) return;
     tile = 0;
+    left -= kSegmentCost;
     if (++part < parts) return;
     part = 0;
     do {
@@ -155,6 +172,11 @@ struct Cursor {
     } while (tiles == 0);
   }
 };
+
+// The shares a sequence's segments take of the numbering.
+__device__ __forceinline__ int64_t sequence_share(int tiles, int parts) {
+  return tiles > 0 ? static_cast<int64_t>(tiles + kSegmentCost) * parts : 0;
+}
 
 template <typename Cache, int DP, int NG>
 __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
@@ -192,7 +214,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
         Cursor c;
         c.seq = seq;
         c.load(a);
-        n += static_cast<int64_t>(c.tiles) * parts;
+        n += sequence_share(c.tiles, parts);
       }
     }
     int64_t total;
@@ -227,8 +249,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
   float m[NG][2], l[NG][2];  // of the heads 2 * (lane % 4), + 1 of each tile of 8
 
   if (worker < workers) {
-    const int64_t begin = run_begin(tiles, workers, worker);
-    const int count = static_cast<int>(run_begin(tiles, workers, worker + 1) - begin);
+    const int64_t begin = run_begin(tiles, workers, worker), finish = run_begin(tiles, workers, worker + 1);
 
     Cursor at;  // the tile computed next
     {
@@ -240,13 +261,19 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       int64_t rest = begin - prefix[lo];
       at.seq = lo * per;
       at.load(a);
-      while (rest >= static_cast<int64_t>(at.tiles) * parts) {
-        rest -= static_cast<int64_t>(at.tiles) * parts;
+      while (rest >= sequence_share(at.tiles, parts)) {
+        rest -= sequence_share(at.tiles, parts);
         ++at.seq;
         at.load(a);
       }
-      at.part = static_cast<int>(rest / at.tiles);
-      at.tile = static_cast<int>(rest - static_cast<int64_t>(at.part) * at.tiles);
+      const int span = at.tiles + kSegmentCost;
+      at.part = static_cast<int>(rest / span);
+      at.tile = static_cast<int>(rest - static_cast<int64_t>(at.part) * span) - kSegmentCost;
+      at.left = static_cast<int>(finish - begin);
+      if (at.tile < 0) {  // the costs of the first segment
+        at.left += at.tile;
+        at.tile = 0;
+      }
     }
 
     const uint32_t ring = smem_addr(rings) + warp * (kStages * Shape::kStageBytes);
@@ -267,10 +294,16 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
     const int64_t head_stride = value_side ? a.value_head : a.key_head;
     constexpr int64_t kHidden = -1ll << 62;  // no token of this tile
     Cursor ahead = at;
+    bool more = at.left > 0;  // tiles to issue
     int64_t page = kHidden;
     int offset = 0, page_head = 0;
+    bool in_page = false;  // all 16 tokens of the tile, one after the other in one page
     auto look_up = [&]() {
-      const int v = ahead.tile * kTile + token;
+      const int v0 = ahead.tile * kTile, v = v0 + token;
+      const int first = ahead.vis.position(v0);
+      const int first_offset = a.block_shift >= 0 ? first & (a.block_size - 1) : first % a.block_size;
+      in_page = v0 + kTile <= ahead.vis.count && first_offset + kTile <= a.block_size &&
+                ahead.vis.position(v0 + kTile - 1) == first + kTile - 1;
       page = kHidden;
       page_head = ahead.part / head_groups;
       if (v < ahead.vis.count) {
@@ -279,43 +312,70 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
         offset = pos - block * a.block_size;
         page = __ldg(a.tables + static_cast<int64_t>(ahead.seq) * a.table_stride + block);
       }
+      if (ahead.tile == 0) {
+        // the segment's queries, on their way to the first-level cache
+        const int kv_head = page_head, h = (ahead.part - kv_head * head_groups) * kHeads + (lane >> 1);
+        if (lane < 2 * kHeads && h < a.group)
+          asm volatile("prefetch.global.L1 [%0];" ::"l"(
+              static_cast<const uint16_t*>(a.query) + static_cast<int64_t>(ahead.seq) * a.query_row +
+              static_cast<int64_t>(kv_head * a.group + h) * a.query_head + (lane & 1) * min(64, a.dim - 1)));
+      }
     };
-    int issued = 0;
+    int stage_of = 0;  // ring entry of the next tile issued
     auto issue = [&]() {
-      if (issued < count) {
-        const char* row = nullptr;
-        if (page >= 0 && page < a.num_blocks)
-          row = plane + page * block_stride + offset * token_stride + page_head * head_stride;
-        else if (page != kHidden)
-          report(a.status, KVCA_ERR_BAD_INDEX, page);  // its rows read as zeros
-        const uint32_t stage = ring + (issued % kStages) * Shape::kStageBytes;
+      if (more) {
+        const bool good = page >= 0 && page < a.num_blocks;
+        if (!good && page != kHidden) report(a.status, KVCA_ERR_BAD_INDEX, page);  // its rows read as zeros
+        const unsigned long long row = reinterpret_cast<unsigned long long>(
+            plane + (good ? page : 0) * block_stride + offset * token_stride + page_head * head_stride);
+        const unsigned seen = __ballot_sync(0xffffffffu, good);
+        const uint32_t stage = ring + stage_of * Shape::kStageBytes;
         constexpr int kPerInstr = 32 / kChunks > 0 ? 32 / kChunks : 1;
         const int r0 = kChunks >= 32 ? 0 : lane / kChunks;
         const int c = lane % kChunks;
+        if (in_page && seen == 0xffffffffu) {
+          // one page: rows at a fixed distance
 #pragma unroll
-        for (int r = 0; r < 2 * kTile; r += kPerInstr) {
-          const char* src = reinterpret_cast<const char*>(
-              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), r + r0));
-          if (c < row_chunks)
-            cp_async16(stage + chunk_offset<kChunks>(r + r0, c), src != nullptr ? src + c * 16 : a.key, src != nullptr);
+          for (int side = 0; side < 2; ++side) {
+            const int64_t stride = side == 0 ? a.key_token : a.value_token;
+            const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, side * kTile)) + r0 * stride + c * 16;
+            if (c < row_chunks) {
+#pragma unroll
+              for (int r = 0; r < kTile; r += kPerInstr) {
+                cp_async16(stage + chunk_offset<kChunks>(side * kTile + r + r0, c), src);
+                src += kPerInstr * stride;
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 2 * kTile; r += kPerInstr) {
+            const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, r + r0)) + c * 16;
+            if (c < row_chunks) cp_async16(stage + chunk_offset<kChunks>(r + r0, c), src, (seen >> (r + r0)) & 1u);
+          }
         }
-        if (++issued < count) {
+        if (++stage_of == kStages) stage_of = 0;
+        more = !ahead.last();
+        if (more) {
           ahead.advance(a, parts);
           look_up();
         }
       }
       cp_async_commit();
     };
-    look_up();
+    if (more) {
+      look_up();
 #pragma unroll 1
-    for (int s = 0; s < kStages - 1; ++s) issue();
+      for (int s = 0; s < kStages - 1; ++s) issue();
+    }
 
     uint32_t q[NG][kSteps][2];
     float unit[NG][2];  // score factor of the heads 2 * (lane % 4), + 1
     bool starts = at.tile == 0;
     bool fresh = true;
+    int stage_at = 0;  // ring entry of the tile computed
 #pragma unroll 1
-    for (int i = 0; i < count; ++i) {
+    for (bool go = at.left > 0; go;) {
       if (fresh) {
         // the segment's queries as the B operand: column (head) lane / 4
         const int kv_head = at.part / head_groups;
@@ -375,7 +435,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
 
       cp_async_wait<kStages - 2>();
       __syncwarp();
-      const uint32_t keys = ring + (i % kStages) * Shape::kStageBytes;
+      const uint32_t keys = ring + stage_at * Shape::kStageBytes;
+      if (++stage_at == kStages) stage_at = 0;
       issue();  // into the stage that the tile before this one left
 
       // S^T = K Q^T, even and odd steps apart for two shorter chains
@@ -486,9 +547,11 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
         }
       }
 
-      const bool ends = at.tile + 1 == at.tiles;
-      if (!ends && i + 1 < count) {
+      const bool ends = at.ends();
+      go = !at.last();
+      if (!ends && go) {
         ++at.tile;
+        --at.left;
         continue;
       }
       // the segment, or this worker's share of it, is done
@@ -567,10 +630,9 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
         held_segment = segment;
         held_starts = starts;
         if (starts)
-          piece.last = static_cast<int>(worker_of(
-              tiles, workers, begin + i + (at.tiles - 1 - at.tile)));
+          piece.last = static_cast<int>(worker_of(tiles, workers, finish - at.left + (at.tiles - 1 - at.tile)));
       }
-      if (i + 1 < count) {
+      if (go) {
         at.advance(a, parts);
         starts = true;
         fresh = true;
@@ -784,7 +846,7 @@ cudaError_t launch_typed(const AttendArgs& a, void* workspace, int sms, cudaStre
 
 template <typename Cache, int DP>
 size_t workspace_of(int tiles, int sms) {
-  const int64_t workers = static_cast<int64_t>(sms) * step_warps(DP * Cache::kBytes);
+  const int64_t workers = static_cast<int64_t>(sms) * step_warps(DP * Cache::kBytes, tiles);
   return tiles == 1 ? StepWorkspace<8, DP * 8>::bytes(workers) : StepWorkspace<16, DP * 16>::bytes(workers);
 }
 
