@@ -4,13 +4,15 @@
 // element and query head.  Work is cut into tiles of 16 visible tokens of one
 // (sequence, head group), numbered sequence by sequence; the tiles of all
 // sequences are dealt out evenly, a contiguous run to each warp of one CTA per
-// SM, so ragged batches and single long sequences load every SM alike.  A
-// warp streams its run through a ring of its own in shared memory (cp.async,
-// no barrier with other warps) and keeps the running maximum and sum of the
-// softmax and the output in registers.  A (sequence, head group) that lies
-// inside one run is written directly; one that several warps share leaves a
-// partial result per warp (joined within the CTA first), which a second,
-// programmatically launched kernel joins in run order.
+// SM, so ragged batches and single long sequences load every SM alike.  Warps
+// side by side take the same run for different heads, whose rows lie side by
+// side in memory (96 ragged sequences with 8 K/V heads: KVCA_A us, one run per
+// warp and head 95).  A warp streams its run through a ring of its own in
+// shared memory (cp.async, no barrier with other warps) and keeps the running
+// maximum and sum of the softmax and the output in registers.  A (sequence,
+// head group) that lies inside one run is written directly; one that several
+// runs share leaves a partial result per warp (joined within the CTA first),
+// which a second, programmatically launched kernel joins in run order.
 //
 // Both products run transposed on m16n8k16: S^T = K Q^T has the 16 tokens as
 // rows and up to 8 query heads that share the K/V head as columns, O^T = V^T
@@ -101,16 +103,42 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// The workspace: the run bounds, then per warp ("worker") what it left.
+// How a call's work lies on the warps: `span` warps side by side share a run,
+// each for a head group of its own.
+struct StepLayout {
+  int parts;   // head groups of a sequence: K/V heads x tiles of query heads
+  int span;    // of them in a run
+  int chunks;  // runs' worth of them, one after the other in the numbering
+  int groups;  // runs of a CTA at a time
+
+  __host__ __device__ StepLayout(int kv_heads, int group, int heads, int warps) {
+    parts = kv_heads * ((group + heads - 1) / heads);
+    int a = parts, b = warps;
+    while (b != 0) {
+      const int r = a % b;
+      a = b;
+      b = r;
+    }
+    span = a;  // the greatest common divisor: no warp is left out
+    chunks = parts / span;
+    groups = warps / span;
+  }
+  // The warp (of the grid) that has run r for the j-th of a run's heads.
+  __device__ __forceinline__ int64_t warp_of(int64_t r, int j, int warps) const {
+    return r / groups * warps + r % groups * span + j;
+  }
+};
+
+// The workspace: the run bounds, then what each warp left.
 struct StepHeader {
-  int64_t tiles;    // of the whole call, segment costs included
-  int64_t workers;  // that got tiles
+  int64_t tiles;  // of the whole call, segment costs included
+  int64_t runs;   // that got tiles
 };
 
 struct StepPiece {
-  int32_t tail;   // segment whose continuation this worker's slot 0 holds, or -1
+  int32_t tail;   // segment whose continuation this warp's slot 0 holds, or -1
   int32_t head;   // segment whose beginning slot 1 holds, or -1
-  int32_t last;   // worker with the last tile of `head`
+  int32_t last;   // run with the last tile of `head`
   int32_t unused;
 };
 
@@ -118,38 +146,38 @@ template <int kHeads, int kAcc>
 struct StepWorkspace {
   StepHeader* header;
   StepPiece* pieces;
-  float* ml;   // [worker][slot][2][heads]: maxima, then sums
-  float* acc;  // [worker][slot][dim][heads]
+  float* ml;   // [warp][slot][2][heads]: maxima, then sums
+  float* acc;  // [warp][slot][dim][heads]
 
-  static __host__ __device__ size_t bytes(int64_t workers) {
-    return 256 + static_cast<size_t>(workers) * (sizeof(StepPiece) + 2 * (2 * kHeads + kAcc) * sizeof(float));
+  static __host__ __device__ size_t bytes(int64_t warps) {
+    return 256 + static_cast<size_t>(warps) * (sizeof(StepPiece) + 2 * (2 * kHeads + kAcc) * sizeof(float));
   }
-  __host__ __device__ StepWorkspace(void* base, int64_t workers) {
+  __host__ __device__ StepWorkspace(void* base, int64_t warps) {
     char* p = static_cast<char*>(base);
     header = reinterpret_cast<StepHeader*>(p);
     acc = reinterpret_cast<float*>(p + 256);
-    ml = acc + workers * 2 * kAcc;
-    pieces = reinterpret_cast<StepPiece*>(ml + workers * 2 * 2 * kHeads);
+    ml = acc + warps * 2 * kAcc;
+    pieces = reinterpret_cast<StepPiece*>(ml + warps * 2 * 2 * kHeads);
   }
-  __device__ __forceinline__ float* ml_of(int64_t worker, int slot) const { return ml + (worker * 2 + slot) * 2 * kHeads; }
-  __device__ __forceinline__ float* acc_of(int64_t worker, int slot) const { return acc + (worker * 2 + slot) * kAcc; }
+  __device__ __forceinline__ float* ml_of(int64_t warp, int slot) const { return ml + (warp * 2 + slot) * 2 * kHeads; }
+  __device__ __forceinline__ float* acc_of(int64_t warp, int slot) const { return acc + (warp * 2 + slot) * kAcc; }
 };
 
-__device__ __forceinline__ int64_t run_begin(int64_t tiles, int64_t workers, int64_t w) {
-  return tiles * w / workers;  // below 2^31 tiles x a few thousand workers
+__device__ __forceinline__ int64_t run_begin(int64_t tiles, int64_t runs, int64_t r) {
+  return tiles * r / runs;  // below 2^31 tiles x a few thousand runs
 }
 
-__device__ __forceinline__ int64_t worker_of(int64_t tiles, int64_t workers, int64_t t) {
-  return (workers * (t + 1) - 1) / tiles;
+__device__ __forceinline__ int64_t run_of(int64_t tiles, int64_t runs, int64_t t) {
+  return (runs * (t + 1) - 1) / tiles;
 }
 
-// A position in the numbering of tiles: sequence, head group, tile.
+// A position in the numbering of tiles: sequence, chunk of head groups, tile.
 struct Cursor {
   int seq;
-  int part;  // kv head * head groups + head group
+  int chunk;
   int tile;
   int tiles;  // of this sequence's visible tokens
-  int left;   // of the worker's share, this tile included; none when <= 0
+  int left;   // of the run, this tile included; none when <= 0
   Visible vis;
 
   __device__ __forceinline__ void load(const AttendArgs& a) {
@@ -159,13 +187,13 @@ struct Cursor {
   __device__ __forceinline__ bool ends() const { return tile + 1 == tiles; }
   __device__ __forceinline__ bool last() const { return left <= (ends() ? 1 + kSegmentCost : 1); }
   // To the next tile; only when this one is not the last.
-  __device__ __forceinline__ void advance(const AttendArgs& a, int parts) {
+  __device__ __forceinline__ void advance(const AttendArgs& a, int chunks) {
     --left;
     if (++tile < tiles) return;
     tile = 0;
     left -= kSegmentCost;
-    if (++part < parts) return;
-    part = 0;
+    if (++chunk < chunks) return;
+    chunk = 0;
     do {
       ++seq;
       load(a);
@@ -174,8 +202,8 @@ struct Cursor {
 };
 
 // The shares a sequence's segments take of the numbering.
-__device__ __forceinline__ int64_t sequence_share(int tiles, int parts) {
-  return tiles > 0 ? static_cast<int64_t>(tiles + kSegmentCost) * parts : 0;
+__device__ __forceinline__ int64_t sequence_share(int tiles, int chunks) {
+  return tiles > 0 ? static_cast<int64_t>(tiles + kSegmentCost) * chunks : 0;
 }
 
 template <typename Cache, int DP, int NG>
@@ -198,7 +226,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
   const int head_groups = (a.group + kHeads - 1) / kHeads;
-  const int parts = a.kv_heads * head_groups;
+  const StepLayout layout(a.kv_heads, a.group, kHeads, kWarps);
+  const int chunks = layout.chunks, span = layout.span;
   StepWorkspace<kHeads, Shape::kAcc> ws(workspace, static_cast<int64_t>(gridDim.x) * kWarps);
 
   // Tile counts of the sequences, or of runs of `per` of them.
@@ -214,7 +243,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
         Cursor c;
         c.seq = seq;
         c.load(a);
-        n += sequence_share(c.tiles, parts);
+        n += sequence_share(c.tiles, chunks);
       }
     }
     int64_t total;
@@ -223,9 +252,9 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
     run += total;
   }
   const int64_t tiles = run;
-  const int64_t all = static_cast<int64_t>(gridDim.x) * kWarps;
-  const int64_t workers = tiles < all ? tiles : all;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *ws.header = StepHeader{tiles, workers};
+  const int64_t all = static_cast<int64_t>(gridDim.x) * layout.groups;
+  const int64_t runs = tiles < all ? tiles : all;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *ws.header = StepHeader{tiles, runs};
   __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -240,7 +269,9 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       for (int i = threadIdx.x; i < n; i += Shape::kThreads) a.lse[row + i] = -INFINITY;
   }
 
-  const int64_t worker = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+  const int64_t own = static_cast<int64_t>(blockIdx.x) * kWarps + warp;  // where this warp leaves results
+  const int64_t my_run = static_cast<int64_t>(blockIdx.x) * layout.groups + warp / span;
+  const int lane_of_heads = warp % span;
   int held_segment = -1;
   bool held_starts = false;
   StepPiece piece{-1, -1, -1, 0};
@@ -248,8 +279,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
   float acc[NG][kSteps][4];
   float m[NG][2], l[NG][2];  // of the heads 2 * (lane % 4), + 1 of each tile of 8
 
-  if (worker < workers) {
-    const int64_t begin = run_begin(tiles, workers, worker), finish = run_begin(tiles, workers, worker + 1);
+  if (my_run < runs) {
+    const int64_t begin = run_begin(tiles, runs, my_run), finish = run_begin(tiles, runs, my_run + 1);
 
     Cursor at;  // the tile computed next
     {
@@ -261,14 +292,14 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       int64_t rest = begin - prefix[lo];
       at.seq = lo * per;
       at.load(a);
-      while (rest >= sequence_share(at.tiles, parts)) {
-        rest -= sequence_share(at.tiles, parts);
+      while (rest >= sequence_share(at.tiles, chunks)) {
+        rest -= sequence_share(at.tiles, chunks);
         ++at.seq;
         at.load(a);
       }
-      const int span = at.tiles + kSegmentCost;
-      at.part = static_cast<int>(rest / span);
-      at.tile = static_cast<int>(rest - static_cast<int64_t>(at.part) * span) - kSegmentCost;
+      const int segment = at.tiles + kSegmentCost;
+      at.chunk = static_cast<int>(rest / segment);
+      at.tile = static_cast<int>(rest - static_cast<int64_t>(at.chunk) * segment) - kSegmentCost;
       at.left = static_cast<int>(finish - begin);
       if (at.tile < 0) {  // the costs of the first segment
         at.left += at.tile;
@@ -305,7 +336,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       in_page = v0 + kTile <= ahead.vis.count && first_offset + kTile <= a.block_size &&
                 ahead.vis.position(v0 + kTile - 1) == first + kTile - 1;
       page = kHidden;
-      page_head = ahead.part / head_groups;
+      const int part = ahead.chunk * span + lane_of_heads;
+      page_head = part / head_groups;
       if (v < ahead.vis.count) {
         const int pos = ahead.vis.position(v);
         const int block = a.block_shift >= 0 ? pos >> a.block_shift : pos / a.block_size;
@@ -314,7 +346,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       }
       if (ahead.tile == 0) {
         // the segment's queries, on their way to the first-level cache
-        const int kv_head = page_head, h = (ahead.part - kv_head * head_groups) * kHeads + (lane >> 1);
+        const int kv_head = page_head, h = (part - kv_head * head_groups) * kHeads + (lane >> 1);
         if (lane < 2 * kHeads && h < a.group)
           asm volatile("prefetch.global.L1 [%0];" ::"l"(
               static_cast<const uint16_t*>(a.query) + static_cast<int64_t>(ahead.seq) * a.query_row +
@@ -357,7 +389,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
         if (++stage_of == kStages) stage_of = 0;
         more = !ahead.last();
         if (more) {
-          ahead.advance(a, parts);
+          ahead.advance(a, chunks);
           look_up();
         }
       }
@@ -378,8 +410,9 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
     for (bool go = at.left > 0; go;) {
       if (fresh) {
         // the segment's queries as the B operand: column (head) lane / 4
-        const int kv_head = at.part / head_groups;
-        const int first = (at.part - kv_head * head_groups) * kHeads;
+        const int part = at.chunk * span + lane_of_heads;
+        const int kv_head = part / head_groups;
+        const int first = (part - kv_head * head_groups) * kHeads;
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
           const int h = first + n * 8 + (lane >> 2);
@@ -554,7 +587,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
         --at.left;
         continue;
       }
-      // the segment, or this worker's share of it, is done
+      // the segment, or this run's share of it, is done
 #pragma unroll
       for (int n = 0; n < NG; ++n)
 #pragma unroll
@@ -563,10 +596,11 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
           l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 8);
           l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
         }
-      const int segment = at.seq * parts + at.part;
+      const int segment = at.seq * layout.parts + at.chunk * span + lane_of_heads;
       if (ends && starts) {
-        const int kv_head = at.part / head_groups;
-        const int first = (at.part - kv_head * head_groups) * kHeads;
+        const int part = at.chunk * span + lane_of_heads;
+        const int kv_head = part / head_groups;
+        const int first = (part - kv_head * head_groups) * kHeads;
         const int64_t row = (static_cast<int64_t>(at.seq) * a.kv_heads + kv_head) * a.group;
         const bool bf16 = a.query_type == KVCA_TYPE_BF16;
 #pragma unroll
@@ -607,10 +641,10 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
           }
         }
       } else if (ends) {
-        // the end of a segment that an earlier worker began
+        // the end of a segment that an earlier run began
         piece.tail = segment;
-        float* const ml = ws.ml_of(worker, 0);
-        float* const part = ws.acc_of(worker, 0);
+        float* const ml = ws.ml_of(own, 0);
+        float* const part = ws.acc_of(own, 0);
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
           const int h = n * 8 + 2 * (lane & 3);
@@ -630,10 +664,10 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
         held_segment = segment;
         held_starts = starts;
         if (starts)
-          piece.last = static_cast<int>(worker_of(tiles, workers, finish - at.left + (at.tiles - 1 - at.tile)));
+          piece.last = static_cast<int>(run_of(tiles, runs, finish - at.left + (at.tiles - 1 - at.tile)));
       }
       if (go) {
-        at.advance(a, parts);
+        at.advance(a, chunks);
         starts = true;
         fresh = true;
       }
@@ -641,8 +675,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
     cp_async_wait<0>();
   }
 
-  // Partial results that the CTA's warps still hold, joined where neighbours
-  // hold the same segment: the rings are free now.
+  // Partial results that the CTA's warps still hold, joined where runs that
+  // follow each other hold the same segment: the rings are free now.
   if (lane == 0) held[warp] = held_segment;
   __syncthreads();
   float* const parked = reinterpret_cast<float*>(rings);
@@ -666,21 +700,18 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
         *reinterpret_cast<float2*>(mine + d1 * kHeads + h) = make_float2(acc[n][t][2], acc[n][t][3]);
       }
     }
-    const bool leads = warp == 0 || held[warp - 1] != held_segment;
+    const bool leads = warp < span || held[warp - span] != held_segment;
     if (leads) (held_starts ? piece.head : piece.tail) = held_segment;
   }
-  if (lane == 0 && worker < workers) ws.pieces[worker] = piece;
+  if (lane == 0 && my_run < runs) ws.pieces[own] = piece;
   __syncthreads();
-  for (int w = 0; w < kWarps;) {
+  for (int w = 0; w < kWarps; ++w) {
     const int segment = held[w];
-    int end = w + 1;
-    if (segment < 0) {
-      w = end;
-      continue;
-    }
-    while (end < kWarps && held[end] == segment) ++end;
-    // a worker whose only tiles continue a segment leads with slot 0, one
-    // that began it with slot 1
+    if (segment < 0 || (w >= span && held[w - span] == segment)) continue;
+    int end = w + span;
+    while (end < kWarps && held[end] == segment) end += span;
+    // a run whose only tiles continue a segment leads with slot 0, one that
+    // began it with slot 1
     const int64_t leader = static_cast<int64_t>(blockIdx.x) * kWarps + w;
     const bool begins = ws.pieces[leader].head == segment;
     float* const out = ws.acc_of(leader, begins ? 1 : 0);
@@ -688,10 +719,10 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
     for (int i = threadIdx.x; i < Shape::kAcc; i += Shape::kThreads) {
       const int h = i % kHeads;
       float top = -INFINITY;
-      for (int k = w; k < end; ++k) top = fmaxf(top, held_ml[k][h]);
+      for (int k = w; k < end; k += span) top = fmaxf(top, held_ml[k][h]);
       const float base = top == -INFINITY ? 0.f : top;
       float sum = 0.f, total = 0.f;
-      for (int k = w; k < end; ++k) {
+      for (int k = w; k < end; k += span) {
         const float weight = exp2_approx(held_ml[k][h] - base);
         sum += weight * parked[k * Shape::kAcc + i];
         total += weight * held_ml[k][kHeads + h];
@@ -702,15 +733,14 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
         ml[kHeads + i] = total;
       }
     }
-    w = end;
   }
 }
 
-// Joins the partial results of the segments that several workers share: one
-// block per worker that began such a segment.
+// Joins the partial results of the segments that several runs share: one block
+// per warp that began such a segment.
 template <int DP, int NG>
 __global__ void __launch_bounds__(kJoinThreads) attend_step_join_kernel(const __grid_constant__ AttendArgs a,
-                                                                       void* workspace, int64_t max_workers) {
+                                                                       void* workspace, int64_t all_warps, int warps) {
   constexpr int kHeads = 8 * NG;
   constexpr int kAcc = DP * kHeads;
   constexpr int kVecs = (kAcc / 4 + kJoinThreads - 1) / kJoinThreads;  // float4 per thread
@@ -719,14 +749,17 @@ __global__ void __launch_bounds__(kJoinThreads) attend_step_join_kernel(const __
   __shared__ float weight[kJoinChunk][kHeads];
   __shared__ float top[kHeads], total[kHeads];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  StepWorkspace<kHeads, kAcc> ws(workspace, max_workers);
-  const int64_t worker = blockIdx.x;
-  if (worker >= ws.header->workers) return;
-  const StepPiece own = ws.pieces[worker];
+  StepWorkspace<kHeads, kAcc> ws(workspace, all_warps);
+  const StepLayout layout(a.kv_heads, a.group, kHeads, warps);
+  const int lane_of_heads = static_cast<int>(blockIdx.x) % warps % layout.span;
+  const int64_t first_run = static_cast<int64_t>(blockIdx.x) / warps * layout.groups + blockIdx.x % warps / layout.span;
+  if (first_run >= ws.header->runs) return;
+  const int64_t owner = blockIdx.x;
+  const StepPiece own = ws.pieces[owner];
   if (own.head < 0) return;
   const int segment = own.head;
   const int head_groups = (a.group + kHeads - 1) / kHeads;
-  const int parts = a.kv_heads * head_groups;
+  const int parts = layout.parts;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
   if (threadIdx.x < kHeads) {
@@ -737,10 +770,10 @@ __global__ void __launch_bounds__(kJoinThreads) attend_step_join_kernel(const __
 #pragma unroll
   for (int v = 0; v < kVecs; ++v) sum[v] = make_float4(0.f, 0.f, 0.f, 0.f);
 
-  // workers whose results belong here, kJoinThreads candidates at a time
-  for (int64_t base = worker; base <= own.last; base += kJoinThreads) {
-    const int64_t w = base + threadIdx.x;
-    const bool mine = w <= own.last && (w == worker || ws.pieces[w].tail == segment);
+  // runs whose results belong here, kJoinThreads candidates at a time
+  for (int64_t base = first_run; base <= own.last; base += kJoinThreads) {
+    const int64_t w = layout.warp_of(base + threadIdx.x, lane_of_heads, warps);
+    const bool mine = base + threadIdx.x <= own.last && (w == owner || ws.pieces[w].tail == segment);
     int found;
     const int at = block_excl_scan(mine ? 1 : 0, &found, scan);
     if (mine) list[at] = static_cast<int>(w);
@@ -752,7 +785,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_step_join_kernel(const __
         float best = top[h];
         for (int k = lane; k < n; k += 32) {
           const int64_t p = list[c + k];
-          weight[k][h] = __ldcg(ws.ml_of(p, p == worker) + h);
+          weight[k][h] = __ldcg(ws.ml_of(p, p == owner) + h);
           best = fmaxf(best, weight[k][h]);
         }
 #pragma unroll
@@ -763,7 +796,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_step_join_kernel(const __
           const int64_t p = list[c + k];
           const float x = exp2_approx(weight[k][h] - floor);
           weight[k][h] = x;
-          part += x * __ldcg(ws.ml_of(p, p == worker) + kHeads + h);
+          part += x * __ldcg(ws.ml_of(p, p == owner) + kHeads + h);
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
@@ -789,7 +822,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_step_join_kernel(const __
 #pragma unroll 8
         for (int k = 0; k < n; ++k) {
           const int64_t p = list[c + k];
-          const float4 o = __ldcg(reinterpret_cast<const float4*>(ws.acc_of(p, p == worker) + i));
+          const float4 o = __ldcg(reinterpret_cast<const float4*>(ws.acc_of(p, p == owner) + i));
           x.x += weight[k][h] * o.x;
           x.y += weight[k][h + 1] * o.y;
           x.z += weight[k][h + 2] * o.z;
@@ -839,15 +872,15 @@ cudaError_t launch_typed(const AttendArgs& a, void* workspace, int sms, cudaStre
   kernel<<<sms, Shape::kThreads, Shape::kSmem, stream>>>(a, workspace);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  const int64_t workers = static_cast<int64_t>(sms) * Shape::kWarps;
-  return launch_dependent(attend_step_join_kernel<DP, NG>, dim3(static_cast<unsigned>(workers)), kJoinThreads, 0,
-                          stream, a, workspace, workers);
+  const int64_t warps = static_cast<int64_t>(sms) * Shape::kWarps;
+  return launch_dependent(attend_step_join_kernel<DP, NG>, dim3(static_cast<unsigned>(warps)), kJoinThreads, 0, stream,
+                          a, workspace, warps, Shape::kWarps);
 }
 
 template <typename Cache, int DP>
 size_t workspace_of(int tiles, int sms) {
-  const int64_t workers = static_cast<int64_t>(sms) * step_warps(DP * Cache::kBytes, tiles);
-  return tiles == 1 ? StepWorkspace<8, DP * 8>::bytes(workers) : StepWorkspace<16, DP * 16>::bytes(workers);
+  const int64_t warps = static_cast<int64_t>(sms) * step_warps(DP * Cache::kBytes, tiles);
+  return tiles == 1 ? StepWorkspace<8, DP * 8>::bytes(warps) : StepWorkspace<16, DP * 16>::bytes(warps);
 }
 
 // Tiles of 8 query heads that share one pass over the rows: two for groups
