@@ -6,8 +6,8 @@
 // sequences are dealt out evenly, a contiguous run to each warp of one CTA per
 // SM, so ragged batches and single long sequences load every SM alike.  Warps
 // side by side take the same run for different heads, whose rows lie side by
-// side in memory (96 ragged sequences with 8 K/V heads: KVCA_A us, one run per
-// warp and head 95).  A warp streams its run through a ring of its own in
+// side in memory (256 windowed sequences with 8 e4m3 K/V heads: 243 us, a run
+// per warp and head 288).  A warp streams its run through a ring of its own in
 // shared memory (cp.async, no barrier with other warps) and keeps the running
 // maximum and sum of the softmax and the output in registers.  A (sequence,
 // head group) that lies inside one run is written directly; one that several
@@ -31,22 +31,15 @@ namespace {
 
 constexpr int kTile = 16;         // tokens per tile: the rows of one m16n8k16
 constexpr int kScanGroups = 1024; // sequences (or runs of them) in the shared tile counts
-constexpr int kJoinThreads = 256;
-constexpr int kJoinChunk = 64;    // partial results weighted at a time
 // What a segment costs a warp beside its tiles (queries, the output), in
 // tiles.  It counts when the tiles are dealt out, as tiles before the first.
-#ifndef KVCA_STEP_COST
-#define KVCA_STEP_COST 2
-#endif
-constexpr int kSegmentCost = KVCA_STEP_COST;
-#ifndef KVCA_STEP_WARPS
-#define KVCA_STEP_WARPS 8
-#endif
+constexpr int kSegmentCost = 2;
 
 // Warps of a CTA, which share 192 KiB of rings: stages of 32 rows, three of
-// them or more in a ring (two at 256-byte rows).
+// them or more in a ring, two at 256-byte rows (96 ragged sequences: 8 warps
+// with three stages 94.5 us, 12 with two 92).
 __host__ __device__ constexpr int step_warps(int row_bytes, int head_tiles) {
-  return row_bytes > 256 ? 4 : row_bytes > 128 ? KVCA_STEP_WARPS : head_tiles > 1 && row_bytes > 64 ? 8 : 16;
+  return row_bytes > 256 ? 4 : row_bytes > 128 ? 12 : head_tiles > 1 && row_bytes > 64 ? 8 : 16;
 }
 
 // DP: head dim padded to 64, 128 or 256; NG: tiles of 8 query heads.
@@ -57,6 +50,9 @@ struct StepShape {
   static constexpr int kStageBytes = 2 * kTile * kRowBytes;
   static constexpr int kWarps = step_warps(kRowBytes, NG);
   static constexpr int kThreads = 32 * kWarps;
+  // Registers of two more warps stay free with 8 warps, so that a block of
+  // the joining kernel fits beside the CTA and waits there.
+  static constexpr int kBound = kWarps == 8 ? 320 : kThreads;
   // 192 KiB of rings per SM
   static constexpr int kRingBytes = 192 * 1024 / kWarps;
   static constexpr int kStages = kRingBytes / kStageBytes < 8 ? kRingBytes / kStageBytes : 8;
@@ -207,7 +203,7 @@ __device__ __forceinline__ int64_t sequence_share(int tiles, int chunks) {
 }
 
 template <typename Cache, int DP, int NG>
-__global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
+__global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kBound, 1)
     attend_step_kernel(const __grid_constant__ AttendArgs a, void* workspace) {
   using Shape = StepShape<Cache, DP, NG>;
   constexpr bool kBf16 = Cache::kBf16;
@@ -253,7 +249,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
   }
   const int64_t tiles = run;
   const int64_t all = static_cast<int64_t>(gridDim.x) * layout.groups;
-  const int64_t runs = tiles < all ? tiles : all;
+  const int64_t runs = min(all, tiles);
   if (blockIdx.x == 0 && threadIdx.x == 0) *ws.header = StepHeader{tiles, runs};
   __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -346,11 +342,11 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       }
       if (ahead.tile == 0) {
         // the segment's queries, on their way to the first-level cache
-        const int kv_head = page_head, h = (part - kv_head * head_groups) * kHeads + (lane >> 1);
+        const int h = (part - page_head * head_groups) * kHeads + (lane >> 1);
         if (lane < 2 * kHeads && h < a.group)
           asm volatile("prefetch.global.L1 [%0];" ::"l"(
               static_cast<const uint16_t*>(a.query) + static_cast<int64_t>(ahead.seq) * a.query_row +
-              static_cast<int64_t>(kv_head * a.group + h) * a.query_head + (lane & 1) * min(64, a.dim - 1)));
+              static_cast<int64_t>(page_head * a.group + h) * a.query_head + (lane & 1) * min(64, a.dim - 1)));
       }
     };
     int stage_of = 0;  // ring entry of the next tile issued
@@ -737,125 +733,113 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
 }
 
 // Joins the partial results of the segments that several runs share: one block
-// per warp that began such a segment.
+// per warp that began such a segment.  Its warps take the runs in turn, a lane
+// for the same elements of each, and meet in shared memory; a chain of three
+// dependent reads (what the owner left, the runs' results, no more) bounds it.
 template <int DP, int NG>
-__global__ void __launch_bounds__(kJoinThreads) attend_step_join_kernel(const __grid_constant__ AttendArgs a,
-                                                                       void* workspace, int64_t all_warps, int warps) {
-  constexpr int kHeads = 8 * NG;
-  constexpr int kAcc = DP * kHeads;
-  constexpr int kVecs = (kAcc / 4 + kJoinThreads - 1) / kJoinThreads;  // float4 per thread
-  __shared__ int scan[33];
-  __shared__ int list[kJoinThreads];
-  __shared__ float weight[kJoinChunk][kHeads];
-  __shared__ float top[kHeads], total[kHeads];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  StepWorkspace<kHeads, kAcc> ws(workspace, all_warps);
+struct JoinShape {
+  static constexpr int kHeads = 8 * NG;
+  static constexpr int kAcc = DP * kHeads;
+  static constexpr int kWarps = 4096 / kAcc < 8 ? 4096 / kAcc : 8;  // 16 KiB of results: a block fits beside a CTA
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kVecs = kAcc / 128;  // float4 per lane
+};
+
+template <int DP, int NG>
+__global__ void __launch_bounds__(JoinShape<DP, NG>::kThreads)
+    attend_step_join_kernel(const __grid_constant__ AttendArgs a, void* workspace, int64_t all_warps, int warps) {
+  using Shape = JoinShape<DP, NG>;
+  constexpr int kHeads = Shape::kHeads;
+  constexpr int kAcc = Shape::kAcc;
+  __shared__ __align__(16) float parked[Shape::kWarps][kAcc];
+  __shared__ __align__(16) float parked_ml[Shape::kWarps][2][kHeads];
   const StepLayout layout(a.kv_heads, a.group, kHeads, warps);
+  const int64_t owner = blockIdx.x;
   const int lane_of_heads = static_cast<int>(blockIdx.x) % warps % layout.span;
   const int64_t first_run = static_cast<int64_t>(blockIdx.x) / warps * layout.groups + blockIdx.x % warps / layout.span;
-  if (first_run >= ws.header->runs) return;
-  const int64_t owner = blockIdx.x;
-  const StepPiece own = ws.pieces[owner];
-  if (own.head < 0) return;
-  const int segment = own.head;
-  const int head_groups = (a.group + kHeads - 1) / kHeads;
-  const int parts = layout.parts;
+  StepWorkspace<kHeads, kAcc> ws(workspace, all_warps);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const StepPiece own = ws.pieces[owner];
+  if (first_run >= ws.header->runs || own.head < 0) return;
+  const int segment = own.head;
 
-  if (threadIdx.x < kHeads) {
-    top[threadIdx.x] = -INFINITY;
-    total[threadIdx.x] = 0.f;
-  }
-  float4 sum[kVecs];
+  const int h4 = lane * 4 % kHeads;  // this lane's four heads
+  float4 top = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), total = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 sum[Shape::kVecs];
 #pragma unroll
-  for (int v = 0; v < kVecs; ++v) sum[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-
-  // runs whose results belong here, kJoinThreads candidates at a time
-  for (int64_t base = first_run; base <= own.last; base += kJoinThreads) {
-    const int64_t w = layout.warp_of(base + threadIdx.x, lane_of_heads, warps);
-    const bool mine = base + threadIdx.x <= own.last && (w == owner || ws.pieces[w].tail == segment);
-    int found;
-    const int at = block_excl_scan(mine ? 1 : 0, &found, scan);
-    if (mine) list[at] = static_cast<int>(w);
-    __syncthreads();
-    for (int c = 0; c < found; c += kJoinChunk) {
-      const int n = min(kJoinChunk, found - c);
-      // maxima of this chunk against the running ones, a warp per head
-      for (int h = warp; h < kHeads; h += kJoinThreads / 32) {
-        float best = top[h];
-        for (int k = lane; k < n; k += 32) {
-          const int64_t p = list[c + k];
-          weight[k][h] = __ldcg(ws.ml_of(p, p == owner) + h);
-          best = fmaxf(best, weight[k][h]);
-        }
+  for (int v = 0; v < Shape::kVecs; ++v) sum[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto fold = [](float& m, float next, float& keep, float& weight) {
+    const float best = fmaxf(m, next), base = best == -INFINITY ? 0.f : best;
+    keep = exp2_approx(m - base);
+    weight = exp2_approx(next - base);
+    m = best;
+  };
+  // Behind the owner: the first run of each later CTA (which leads what the
+  // CTA's runs still held) and the run with the segment's end.
+  const int64_t cta = first_run / layout.groups, last_cta = own.last / layout.groups;
+  const int64_t pieces = last_cta - cta + 1 + (cta == last_cta || own.last % layout.groups != 0 ? 1 : 0);
+  for (int64_t k = warp; k < pieces; k += Shape::kWarps) {
+    const int64_t r = k == 0 ? first_run : k <= last_cta - cta ? (cta + k) * layout.groups : own.last;
+    const int64_t w = layout.warp_of(r, lane_of_heads, warps);
+    const int slot = w == owner ? 1 : 0;
+    const int tail = __ldcg(&ws.pieces[w].tail);
+    const float4 m = __ldcg(reinterpret_cast<const float4*>(ws.ml_of(w, slot) + h4));
+    const float4 l = __ldcg(reinterpret_cast<const float4*>(ws.ml_of(w, slot) + kHeads + h4));
+    const float4* const from = reinterpret_cast<const float4*>(ws.acc_of(w, slot)) + lane;
+    float4 o[Shape::kVecs];
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
-        const float floor = best == -INFINITY ? 0.f : best;
-        float part = 0.f;
-        for (int k = lane; k < n; k += 32) {
-          const int64_t p = list[c + k];
-          const float x = exp2_approx(weight[k][h] - floor);
-          weight[k][h] = x;
-          part += x * __ldcg(ws.ml_of(p, p == owner) + kHeads + h);
-        }
+    for (int v = 0; v < Shape::kVecs; ++v) o[v] = __ldcg(from + 32 * v);
+    if (slot == 0 && tail != segment) continue;  // joined within its CTA, or another segment's
+    float4 keep, weight;
+    fold(top.x, m.x, keep.x, weight.x);
+    fold(top.y, m.y, keep.y, weight.y);
+    fold(top.z, m.z, keep.z, weight.z);
+    fold(top.w, m.w, keep.w, weight.w);
+    total.x = total.x * keep.x + l.x * weight.x;
+    total.y = total.y * keep.y + l.y * weight.y;
+    total.z = total.z * keep.z + l.z * weight.z;
+    total.w = total.w * keep.w + l.w * weight.w;
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
-        __syncwarp();
-        if (lane == 0) {
-          const float decay = exp2_approx(top[h] - floor);
-          total[h] = total[h] * decay + part;
-          top[h] = best;
-          scan[h] = __float_as_int(decay);
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int v = 0; v < kVecs; ++v) {
-        const int i = (threadIdx.x + v * kJoinThreads) * 4;
-        if (i >= kAcc) break;
-        const int h = i % kHeads;
-        float4 x = sum[v];
-        x.x *= __int_as_float(scan[h]);
-        x.y *= __int_as_float(scan[h + 1]);
-        x.z *= __int_as_float(scan[h + 2]);
-        x.w *= __int_as_float(scan[h + 3]);
-#pragma unroll 8
-        for (int k = 0; k < n; ++k) {
-          const int64_t p = list[c + k];
-          const float4 o = __ldcg(reinterpret_cast<const float4*>(ws.acc_of(p, p == owner) + i));
-          x.x += weight[k][h] * o.x;
-          x.y += weight[k][h + 1] * o.y;
-          x.z += weight[k][h + 2] * o.z;
-          x.w += weight[k][h + 3] * o.w;
-        }
-        sum[v] = x;
-      }
-      __syncthreads();
+    for (int v = 0; v < Shape::kVecs; ++v) {
+      sum[v].x = sum[v].x * keep.x + o[v].x * weight.x;
+      sum[v].y = sum[v].y * keep.y + o[v].y * weight.y;
+      sum[v].z = sum[v].z * keep.z + o[v].z * weight.z;
+      sum[v].w = sum[v].w * keep.w + o[v].w * weight.w;
     }
   }
+#pragma unroll
+  for (int v = 0; v < Shape::kVecs; ++v) *reinterpret_cast<float4*>(&parked[warp][(lane + 32 * v) * 4]) = sum[v];
+  if (lane * 4 < kHeads) {
+    *reinterpret_cast<float4*>(&parked_ml[warp][0][h4]) = top;
+    *reinterpret_cast<float4*>(&parked_ml[warp][1][h4]) = total;
+  }
+  __syncthreads();
 
-  const int seq = segment / parts, part = segment - seq * parts;
+  const int head_groups = (a.group + kHeads - 1) / kHeads;
+  const int seq = segment / layout.parts, part = segment - seq * layout.parts;
   const int kv_head = part / head_groups;
   const int first = (part - kv_head * head_groups) * kHeads;
   const int64_t row = (static_cast<int64_t>(seq) * a.kv_heads + kv_head) * a.group;
+  for (int i = threadIdx.x; i < kAcc; i += Shape::kThreads) {
+    const int h = i / DP, d = i % DP;
+    if (first + h >= a.group || d >= a.dim) continue;
+    float best = -INFINITY;
 #pragma unroll
-  for (int v = 0; v < kVecs; ++v) {
-    const int i = (threadIdx.x + v * kJoinThreads) * 4;
-    if (i >= kAcc) break;
-    const int d = i / kHeads;
-    if (d >= a.dim) break;
-    const float x[4] = {sum[v].x, sum[v].y, sum[v].z, sum[v].w};
+    for (int w = 0; w < Shape::kWarps; ++w) best = fmaxf(best, parked_ml[w][0][h]);
+    const float base = best == -INFINITY ? 0.f : best;
+    float x = 0.f, l = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int h = i % kHeads + j;
-      if (first + h >= a.group) continue;
-      const float y = x[j] * (a.value_scale / total[h]);
-      uint16_t* const out = static_cast<uint16_t*>(a.out) + (row + first + h) * a.dim + d;
-      *out = static_cast<uint16_t>(a.query_type == KVCA_TYPE_BF16 ? pack2<true>(y, 0.f) : pack2<false>(y, 0.f));
+    for (int w = 0; w < Shape::kWarps; ++w) {
+      const float weight = exp2_approx(parked_ml[w][0][h] - base);
+      x += weight * parked[w][d * kHeads + h];
+      l += weight * parked_ml[w][1][h];
     }
+    const float y = x * (a.value_scale / l);
+    static_cast<uint16_t*>(a.out)[(row + first + h) * a.dim + d] =
+        static_cast<uint16_t>(a.query_type == KVCA_TYPE_BF16 ? pack2<true>(y, 0.f) : pack2<false>(y, 0.f));
+    if (a.lse != nullptr && d == 0) a.lse[row + first + h] = base * kLn2 + logf(l);
   }
-  if (a.lse != nullptr && threadIdx.x < kHeads && first + threadIdx.x < a.group)
-    a.lse[row + first + threadIdx.x] = top[threadIdx.x] * kLn2 + logf(total[threadIdx.x]);
 }
 
 template <typename Cache, int DP, int NG>
@@ -873,8 +857,8 @@ cudaError_t launch_typed(const AttendArgs& a, void* workspace, int sms, cudaStre
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const int64_t warps = static_cast<int64_t>(sms) * Shape::kWarps;
-  return launch_dependent(attend_step_join_kernel<DP, NG>, dim3(static_cast<unsigned>(warps)), kJoinThreads, 0, stream,
-                          a, workspace, warps, Shape::kWarps);
+  return launch_dependent(attend_step_join_kernel<DP, NG>, dim3(static_cast<unsigned>(warps)),
+                          JoinShape<DP, NG>::kThreads, 0, stream, a, workspace, warps, Shape::kWarps);
 }
 
 template <typename Cache, int DP>

@@ -5,6 +5,7 @@
 // and stride allows, and hands off to the sm_100a launchers.  It allocates
 // nothing and never synchronises the stream.
 
+#include <atomic>
 #include <chrono>
 
 #include <cuda_runtime.h>
@@ -170,10 +171,15 @@ extern "C" {
 int kvca_abi_version(void) { return kAbiVersion; }
 
 int kvca_device_sm_count(void) {
+  // looked up once per device: launchers ask on every call
+  static std::atomic<int> known[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  int sms = 0;
+  const bool tracked = dev >= 0 && dev < 64;
+  int sms = tracked ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (sms > 0) return sms;
   if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (tracked) known[dev].store(sms, std::memory_order_relaxed);
   return sms;
 }
 

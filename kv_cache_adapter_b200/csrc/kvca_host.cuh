@@ -6,6 +6,8 @@
 #include <atomic>
 #include <utility>
 
+#include "kvca.h"
+
 namespace kvca {
 namespace {
 
@@ -28,13 +30,7 @@ cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, unsigned bloc
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-int device_sm_count() {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  int sms = 0;
-  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  return sms;
-}
+int device_sm_count() { return kvca_device_sm_count(); }
 
 // Function attributes (the dynamic shared-memory limit, the carve-out)
 // belong to the current device's context, so a launcher sets them once per

@@ -1423,6 +1423,16 @@ _ATTEND_TYPES = {torch.float16: _lib.KVCA_TYPE_F16, torch.bfloat16: _lib.KVCA_TY
 _attend_workspace_bytes: dict[tuple, int] = {}
 
 
+def _attend_rows(t: torch.Tensor, shape, name: str) -> list[int]:
+    """Strides in bytes of the leading dims of rows of head_dim (0 for a dim of size 1)."""
+    size = t.element_size()
+    stride = t.stride()
+    out = [x * size if n > 1 else 0 for n, x in zip(shape[:-1], stride)]
+    if t.data_ptr() % 16 or sum(x % 16 for x in out) or (stride[-1] != 1 and t.numel()):
+        raise ValueError(f"{name}: rows of head_dim must be contiguous and 16-byte aligned")
+    return out
+
+
 def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
                  block_tables: torch.Tensor, seq_lens: torch.Tensor, scale, window, sinks, key_scale, value_scale,
                  out, lse) -> tuple[_lib.AttendDesc, torch.Tensor]:
@@ -1432,70 +1442,70 @@ def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torc
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be torch.Tensor")
     dev = query.device
-    if not query.is_cuda:
+    if dev.type != "cuda":
         raise ValueError("query must be a CUDA tensor")
-    for t, name in ((key_cache, "key_cache"), (value_cache, "value_cache"), (block_tables, "block_tables"),
-                    (seq_lens, "seq_lens")):
-        if t.device != dev:
-            raise ValueError(f"{name} must be on {dev}")
-    if query.dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"query has incorrect dtype {query.dtype}")
-    if query.dim() != 3 or key_cache.dim() != 4:
+    if (key_cache.device != dev or value_cache.device != dev or block_tables.device != dev
+            or seq_lens.device != dev):
+        raise ValueError(f"key_cache, value_cache, block_tables and seq_lens must be on {dev}")
+    qtype, ctype = query.dtype, key_cache.dtype
+    if qtype is not torch.float16 and qtype is not torch.bfloat16:
+        raise TypeError(f"query has incorrect dtype {qtype}")
+    e4m3 = ctype is torch.float8_e4m3fn
+    if not e4m3 and ctype is not qtype:
+        raise TypeError(f"key_cache has incorrect dtype {ctype}")
+    qshape, kshape = query.shape, key_cache.shape
+    if len(qshape) != 3 or len(kshape) != 4:
         raise ValueError("query must be (rows, heads, head_dim) and the caches (num_blocks, block_size, kv_heads, "
                          "head_dim)")
-    ctype = key_cache.dtype
-    if ctype != query.dtype and ctype != torch.float8_e4m3fn:
-        raise TypeError(f"key_cache has incorrect dtype {ctype}")
-    if value_cache.dtype != ctype or value_cache.shape != key_cache.shape:
+    if value_cache.dtype is not ctype or value_cache.shape != kshape:
         raise ValueError("key_cache and value_cache must share shape and dtype")
-    rows, heads, dim = query.shape
-    num_blocks, block_size, kv_heads, cache_dim = key_cache.shape
+    rows, heads, dim = qshape
+    num_blocks, block_size, kv_heads, cache_dim = kshape
     if cache_dim != dim:
         raise ValueError(f"the caches' head_dim {cache_dim} is not the query's {dim}")
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError(f"the query heads ({heads}) must be a positive multiple of the K/V heads ({kv_heads})")
     if block_size < 1:
         raise ValueError("block_size must be positive")
-    step = 16 if ctype == torch.float8_e4m3fn else 8
+    step = 16 if e4m3 else 8
     if dim < step or dim > 256 or dim % step:
         raise ValueError(f"head_dim must be a multiple of {step} up to 256, got {dim}")
-    if block_tables.dtype != torch.int64 or seq_lens.dtype != torch.int64:
+    if block_tables.dtype is not torch.int64 or seq_lens.dtype is not torch.int64:
         raise TypeError("block_tables and seq_lens must be int64")
+    tshape = block_tables.shape
     if seq_lens.dim() != 1 or not seq_lens.is_contiguous():
         raise ValueError("seq_lens must be 1D and contiguous")
-    if block_tables.dim() != 2 or block_tables.shape[0] != seq_lens.shape[0] or (
-            block_tables.numel() and block_tables.stride(1) != 1):
+    seqs = seq_lens.shape[0]
+    if len(tshape) != 2 or tshape[0] != seqs:
+        raise ValueError("block_tables must be (num_seqs, max_blocks) with contiguous rows")
+    tstride = block_tables.stride()
+    if tstride[1] != 1 and tshape[1] > 1 and seqs:
         raise ValueError("block_tables must be (num_seqs, max_blocks) with contiguous rows")
     window = 0 if window is None else int(window)
     sinks = int(sinks)
     if window < 0 or sinks < 0 or (window == 0 and sinks > 0):
         raise ValueError("window must be positive (or None) and sinks need a window")
-    if ctype != torch.float8_e4m3fn and (key_scale != 1.0 or value_scale != 1.0):
+    if not e4m3 and (key_scale != 1.0 or value_scale != 1.0):
         raise ValueError("key_scale and value_scale belong to an e4m3 cache")
-    esz = key_cache.element_size()
-    ks, vs, qs = key_cache.stride(), value_cache.stride(), query.stride()
-    for st, t, name in ((ks, key_cache, "key_cache"), (vs, value_cache, "value_cache"), (qs, query, "query")):
-        size = t.element_size()
-        if t.numel() and (st[-1] != 1 or t.data_ptr() % 16 or any(
-                n > 1 and x * size % 16 for n, x in zip(t.shape[:-1], st[:-1]))):
-            raise ValueError(f"{name}: rows of head_dim must be contiguous and 16-byte aligned")
-    # a dim of size 1 may carry any stride
-    ks, vs, qs = ([x if n > 1 else 0 for n, x in zip(t.shape[:-1], t.stride())] for t in (key_cache, value_cache, query))
+    ks = _attend_rows(key_cache, kshape, "key_cache")
+    vs = _attend_rows(value_cache, kshape, "value_cache")
+    qs = _attend_rows(query, qshape, "query")
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=query.dtype, device=dev)
-    elif (tuple(out.shape) != (rows, heads, dim) or out.dtype != query.dtype or out.device != dev
-          or not out.is_contiguous() or out.data_ptr() % 16):
-        raise ValueError(f"out must be a contiguous, 16-byte aligned {(rows, heads, dim)} {query.dtype} tensor on {dev}")
-    if lse is not None and (tuple(lse.shape) != (rows, heads) or lse.dtype != torch.float32 or lse.device != dev
-                            or not lse.is_contiguous()):
-        raise ValueError(f"lse must be a contiguous {(rows, heads)} float32 tensor on {dev}")
+        out = torch.empty(qshape, dtype=qtype, device=dev)
+    elif (out.shape != qshape or out.dtype is not qtype or out.device != dev or not out.is_contiguous()
+          or out.data_ptr() % 16):
+        raise ValueError(f"out must be a contiguous, 16-byte aligned {tuple(qshape)} {qtype} tensor on {dev}")
+    if lse is None:
+        lse_ptr = None
+    elif lse.shape != qshape[:2] or lse.dtype is not torch.float32 or lse.device != dev or not lse.is_contiguous():
+        raise ValueError(f"lse must be a contiguous {tuple(qshape[:2])} float32 tensor on {dev}")
+    else:
+        lse_ptr = lse.data_ptr()
     desc = _lib.AttendDesc(
-        key_cache.data_ptr(), value_cache.data_ptr(), ks[0] * esz, ks[1] * esz, ks[2] * esz, vs[0] * esz, vs[1] * esz,
-        vs[2] * esz, num_blocks, block_size, block_tables.data_ptr() or None, block_tables.stride(0),
-        block_tables.shape[1], seq_lens.data_ptr() or None, seq_lens.shape[0], heads, kv_heads, dim,
-        _ATTEND_TYPES[query.dtype], _ATTEND_TYPES[ctype], dim ** -0.5 if scale is None else scale, key_scale,
-        value_scale, window, sinks, query.data_ptr(), qs[0] * 2, qs[1] * 2, out.data_ptr(),
-        None if lse is None else lse.data_ptr())
+        key_cache.data_ptr(), value_cache.data_ptr(), *ks, *vs, num_blocks, block_size,
+        block_tables.data_ptr() or None, tstride[0], tshape[1], seq_lens.data_ptr() or None, seqs, heads, kv_heads, dim,
+        _ATTEND_TYPES[qtype], _ATTEND_TYPES[ctype], dim ** -0.5 if scale is None else scale, key_scale, value_scale,
+        window, sinks, query.data_ptr(), *qs, out.data_ptr(), lse_ptr)
     return desc, out
 
 
