@@ -94,12 +94,20 @@ __device__ __forceinline__ int64_t pages_of(int64_t len, int64_t block_size) {
   return (len + block_size - 1) / block_size;
 }
 
-// Everything about the call that does not concern single pages.
+constexpr int kCheckThreads = 1024;
+
+// What the pairs of a fork are compared with, a block's worth at a time.
+struct ForkTile {
+  int64_t parent[kCheckThreads], child[kCheckThreads], fresh[kCheckThreads], id[kCheckThreads];
+  bool partial[kCheckThreads];
+};
+
+// Everything about pair j that does not concern single pages; the block's
+// threads take pairs side by side (those past the last one help with the
+// tiles).  True when the pair is refused (and reported).
 template <typename MetaT>
-__global__ void __launch_bounds__(1024) fork_check_kernel(const __grid_constant__ ForkArgs f, PageHeader* header) {
-  dependent_trigger();
+__device__ bool fork_refused(const ForkArgs& f, int64_t j, ForkTile& tile) {
   const PageTable& t = f.table;
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x;
   int64_t code = 0, value = 0;
   auto refuse = [&](int64_t c, int64_t v) {
     if (code == 0) {
@@ -107,8 +115,11 @@ __global__ void __launch_bounds__(1024) fork_check_kernel(const __grid_constant_
       value = v;
     }
   };
+  int64_t child = -1, fresh = -1, id = -1;
+  bool partial = false;
   if (j < f.count) {
-    const int64_t parent = f.parents[j], child = f.children[j];
+    const int64_t parent = f.parents[j];
+    child = f.children[j];
     if (parent < 0 || parent >= t.num_seqs)
       refuse(KVCA_ERR_BAD_INDEX, parent);
     else if (child < 0 || child >= t.num_seqs)
@@ -117,8 +128,7 @@ __global__ void __launch_bounds__(1024) fork_check_kernel(const __grid_constant_
       const int64_t len = t.lens[parent];
       if (len < 0 || t.lens[child] > 0) refuse(KVCA_ERR_BAD_ARGUMENT, len < 0 ? parent : child);
       if (len > t.width * t.block_size) refuse(KVCA_ERR_BAD_INDEX, len);
-      const bool partial = code == 0 && len % t.block_size != 0;
-      int64_t fresh = -1, id = -1;
+      partial = code == 0 && len % t.block_size != 0;
       if (partial) {
         fresh = f.fresh_slots[j];
         id = f.fresh_ids[j];
@@ -138,22 +148,125 @@ __global__ void __launch_bounds__(1024) fork_check_kernel(const __grid_constant_
         else if (f.pool.p2l[fresh] >= f.pool.num_logical)
           refuse(KVCA_ERR_BAD_INDEX, f.pool.p2l[fresh]);
       }
-      for (int64_t k = 0; k < f.count && code == 0; ++k) {
-        if (f.parents[k] == child || (k != j && f.children[k] == child)) refuse(KVCA_ERR_BAD_ARGUMENT, child);
-        if (k == j || !partial) continue;
-        if (f.fresh_slots[k] != fresh && f.fresh_ids[k] != id) continue;
-        // the other one counts if it needs its slot, too
-        const int64_t other = f.parents[k];
-        if (other >= 0 && other < t.num_seqs && t.lens[other] > 0 && t.lens[other] % t.block_size != 0)
-          refuse(KVCA_ERR_BAD_ARGUMENT, f.fresh_slots[k] == fresh ? fresh : id);
-      }
     }
   }
+  // against every other pair
+  for (int64_t base = 0; base < f.count; base += kCheckThreads) {
+    const int64_t k = base + threadIdx.x;
+    __syncthreads();
+    if (k < f.count) {
+      const int64_t other = f.parents[k];
+      tile.parent[threadIdx.x] = other;
+      tile.child[threadIdx.x] = f.children[k];
+      tile.fresh[threadIdx.x] = f.fresh_slots[k];
+      tile.id[threadIdx.x] = f.fresh_ids[k];
+      // it counts if it needs its slot, too
+      const bool known = other >= 0 && other < t.num_seqs;
+      tile.partial[threadIdx.x] = known && t.lens[other] > 0 && t.lens[other] % t.block_size != 0;
+    }
+    __syncthreads();
+    if (j >= f.count) continue;
+    const int n = static_cast<int>(min(static_cast<int64_t>(kCheckThreads), f.count - base));
+    const int self = static_cast<int>(min(max(j - base, int64_t{-1}), int64_t{kCheckThreads}));
+    bool same_child = false, same_slot = false, same_id = false;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const bool other = i != self, copies = other & tile.partial[i];
+      same_child |= (tile.parent[i] == child) | (other & (tile.child[i] == child));
+      same_slot |= copies & (tile.fresh[i] == fresh);
+      same_id |= copies & (tile.id[i] == id);
+    }
+    if (same_child) refuse(KVCA_ERR_BAD_ARGUMENT, child);
+    if (partial && same_slot) refuse(KVCA_ERR_BAD_ARGUMENT, fresh);
+    if (partial && same_id) refuse(KVCA_ERR_BAD_ARGUMENT, id);
+  }
   if (code != 0) report(f.pool.status, code, value);
-  const int bad = __syncthreads_or(code != 0);
+  return code != 0;
+}
+
+template <typename MetaT>
+__global__ void __launch_bounds__(kCheckThreads) fork_check_kernel(const __grid_constant__ ForkArgs f,
+                                                                  PageHeader* header) {
+  __shared__ ForkTile tile;
+  dependent_trigger();
+  const int bad = __syncthreads_or(fork_refused<MetaT>(f, static_cast<int64_t>(blockIdx.x) * kCheckThreads + threadIdx.x, tile));
   if (threadIdx.x == 0) {
     header->verdicts[blockIdx.x] = bad;
     if (blockIdx.x == 0) header->refused = 0;
+  }
+}
+
+// Pins page i of pair j's parent; false (and reported) when it cannot.
+template <typename MetaT>
+__device__ __forceinline__ bool fork_pin(const ForkArgs& f, int64_t j, int64_t i, int64_t parent, uint8_t* pinned) {
+  const int64_t slot = f.table.tables[parent * f.table.stride + i];
+  bool done = false, fine = true;
+  if (slot >= f.pool.num_slots) {
+    report(f.pool.status, KVCA_ERR_BAD_INDEX, slot);
+    fine = false;
+  } else if (slot >= 0) {
+    done = fine = add_pin(static_cast<MetaT*>(f.pool.slot_meta), slot, 1, true);
+    if (!done) report(f.pool.status, KVCA_ERR_BAD_ARGUMENT, slot);  // held by nobody, or as often as its field counts
+  }
+  pinned[j * f.table.width + i] = done;
+  return fine;
+}
+
+// Page i of pair j's child, or the pin back.
+template <typename MetaT>
+__device__ __forceinline__ void fork_page(const ForkArgs& f, int64_t j, int64_t i, int64_t parent, int64_t child,
+                                          bool refused, const uint8_t* pinned) {
+  const PageTable& t = f.table;
+  const int64_t slot = t.tables[parent * t.stride + i];
+  if (!refused)
+    t.tables[child * t.stride + i] = slot;
+  else if (pinned[j * t.width + i])
+    add_pin(static_cast<MetaT*>(f.pool.slot_meta), slot, -1, true);
+}
+
+// The rest of pair j's child: its last page's metadata and its length.
+template <typename MetaT>
+__device__ __forceinline__ void fork_child(const ForkArgs& f, int64_t j, int64_t len, int64_t child) {
+  const PageTable& t = f.table;
+  if (len % t.block_size != 0) {
+    const int64_t fresh = f.fresh_slots[j], id = f.fresh_ids[j];
+    t.tables[child * t.stride + len / t.block_size] = fresh;
+    const int64_t old = f.pool.p2l[fresh];
+    if (old >= 0) f.pool.l2p[old] = -1;
+    f.pool.l2p[id] = fresh;
+    f.pool.p2l[fresh] = id;
+    static_cast<MetaT*>(f.pool.slot_meta)[fresh] = Meta<MetaT>::pack(1, 1);
+  }
+  t.lens[child] = len;
+}
+
+// A small fork's checks, pins and tables by one block (the bytes follow).
+template <typename MetaT>
+__global__ void __launch_bounds__(kCheckThreads) fork_small_kernel(const __grid_constant__ ForkArgs f,
+                                                                  PageHeader* header, uint8_t* pinned) {
+  __shared__ ForkTile tile;
+  dependent_trigger();
+  const int bad = __syncthreads_or(fork_refused<MetaT>(f, threadIdx.x, tile));
+  if (threadIdx.x == 0) {
+    header->verdicts[0] = bad;
+    header->refused = 0;
+  }
+  if (bad) return;
+  const PageTable& t = f.table;
+  const int lanes = 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  bool fine = true;
+  for (int64_t j = warp; j < f.count; j += kCheckThreads / lanes) {
+    const int64_t parent = f.parents[j];
+    const int64_t full = t.lens[parent] / t.block_size;
+    for (int64_t i = lane; i < full; i += lanes) fine &= fork_pin<MetaT>(f, j, i, parent, pinned);
+  }
+  const bool refused = __syncthreads_or(!fine) != 0;
+  if (threadIdx.x == 0) header->refused = refused;
+  for (int64_t j = warp; j < f.count; j += kCheckThreads / lanes) {
+    const int64_t parent = f.parents[j], child = f.children[j];
+    const int64_t len = t.lens[parent];
+    for (int64_t i = lane; i < len / t.block_size; i += lanes) fork_page<MetaT>(f, j, i, parent, child, refused, pinned);
+    if (!refused && lane == 0) fork_child<MetaT>(f, j, len, child);
   }
 }
 
@@ -169,21 +282,8 @@ __global__ void __launch_bounds__(kPageThreads) fork_pin_kernel(const __grid_con
   const int64_t parent = f.parents[j];
   const int64_t full = t.lens[parent] / t.block_size;
   const int64_t base = static_cast<int64_t>(blockIdx.y) * kEntriesPerBlock;
-  for (int64_t i = base + threadIdx.x; i < full && i < base + kEntriesPerBlock; i += kPageThreads) {
-    const int64_t slot = t.tables[parent * t.stride + i];
-    bool done = false;
-    if (slot >= f.pool.num_slots) {
-      report(f.pool.status, KVCA_ERR_BAD_INDEX, slot);
-      header->refused = 1;
-    } else if (slot >= 0) {
-      done = add_pin(static_cast<MetaT*>(f.pool.slot_meta), slot, 1, true);
-      if (!done) {
-        report(f.pool.status, KVCA_ERR_BAD_ARGUMENT, slot);  // held by nobody, or as often as its field counts
-        header->refused = 1;
-      }
-    }
-    pinned[j * t.width + i] = done;
-  }
+  for (int64_t i = base + threadIdx.x; i < full && i < base + kEntriesPerBlock; i += kPageThreads)
+    if (!fork_pin<MetaT>(f, j, i, parent, pinned)) header->refused = 1;
 }
 
 // The children's tables, their last pages' metadata and bytes; or, when a
@@ -198,7 +298,6 @@ __global__ void __launch_bounds__(kPageThreads) fork_commit_kernel(const __grid_
   if (!checks_passed(header, checks)) return;
   const bool refused = header->refused != 0;
   const PageTable& t = f.table;
-  MetaT* const meta = static_cast<MetaT*>(f.pool.slot_meta);
   if (static_cast<int>(blockIdx.x) < copy_blocks) {
     if (refused) return;
     const int64_t block_bytes = t.block_size * row_bytes;
@@ -228,56 +327,120 @@ __global__ void __launch_bounds__(kPageThreads) fork_commit_kernel(const __grid_
   const int64_t len = t.lens[parent];
   const int64_t full = len / t.block_size;
   const int64_t base = chunk * kEntriesPerBlock;
-  for (int64_t i = base + threadIdx.x; i < full && i < base + kEntriesPerBlock; i += kPageThreads) {
-    const int64_t slot = t.tables[parent * t.stride + i];
-    if (!refused)
-      t.tables[child * t.stride + i] = slot;
-    else if (pinned[j * t.width + i])
-      add_pin(meta, slot, -1, true);
-  }
-  if (refused || chunk != 0 || threadIdx.x != 0) return;
-  if (len % t.block_size != 0) {
-    const int64_t fresh = f.fresh_slots[j], id = f.fresh_ids[j];
-    t.tables[child * t.stride + full] = fresh;
-    const int64_t old = f.pool.p2l[fresh];
-    if (old >= 0) f.pool.l2p[old] = -1;
-    f.pool.l2p[id] = fresh;
-    f.pool.p2l[fresh] = id;
-    meta[fresh] = Meta<MetaT>::pack(1, 1);
-  }
-  t.lens[child] = len;
+  for (int64_t i = base + threadIdx.x; i < full && i < base + kEntriesPerBlock; i += kPageThreads)
+    fork_page<MetaT>(f, j, i, parent, child, refused, pinned);
+  if (!refused && chunk == 0 && threadIdx.x == 0) fork_child<MetaT>(f, j, len, child);
 }
 
 // ---------------------------------------------------------------------------
 // Free
 // ---------------------------------------------------------------------------
 
-__global__ void __launch_bounds__(1024) free_check_kernel(const __grid_constant__ FreeArgs f, PageHeader* header) {
-  dependent_trigger();
+// Everything about sequence j of the call that does not concern single pages;
+// keeps its length.  True when it is refused (and reported).
+__device__ bool free_refused(const FreeArgs& f, int64_t j, int64_t (&tile)[kCheckThreads]) {
   const PageTable& t = f.table;
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * 1024 + threadIdx.x;
-  int64_t code = 0, value = 0;
+  int64_t code = 0, value = 0, seq = -1;
   if (j < f.count) {
-    const int64_t seq = f.sequences[j];
-    value = seq;
+    value = seq = f.sequences[j];
     if (seq < 0 || seq >= t.num_seqs) {
       code = KVCA_ERR_BAD_INDEX;
-    } else if (t.lens[seq] > t.width * t.block_size) {
-      code = KVCA_ERR_BAD_INDEX;
-      value = t.lens[seq];
     } else {
-      for (int64_t k = 0; k < j && code == 0; ++k)
-        if (f.sequences[k] == seq) code = KVCA_ERR_BAD_ARGUMENT;
+      const int64_t len = t.lens[seq];
+      f.lens_before[j] = len;
+      if (len > t.width * t.block_size) {
+        code = KVCA_ERR_BAD_INDEX;
+        value = len;
+      }
     }
   }
-  if (code != 0)
-    report(f.pool.status, code, value);
-  else if (j < f.count)
-    f.lens_before[j] = t.lens[f.sequences[j]];
-  const int bad = __syncthreads_or(code != 0);
+  for (int64_t base = 0; base < f.count; base += kCheckThreads) {  // twice in the list
+    __syncthreads();
+    if (base + threadIdx.x < f.count) tile[threadIdx.x] = f.sequences[base + threadIdx.x];
+    __syncthreads();
+    if (j >= f.count || code != 0) continue;
+    const int n = static_cast<int>(min(static_cast<int64_t>(kCheckThreads), f.count - base));
+    bool twice = false;
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) twice |= (tile[k] == seq) & (base + k != j);
+    if (twice) code = KVCA_ERR_BAD_ARGUMENT;
+  }
+  if (code != 0) report(f.pool.status, code, value);
+  return code != 0;
+}
+
+__global__ void __launch_bounds__(kCheckThreads) free_check_kernel(const __grid_constant__ FreeArgs f,
+                                                                  PageHeader* header) {
+  __shared__ int64_t tile[kCheckThreads];
+  dependent_trigger();
+  const int bad = __syncthreads_or(free_refused(f, static_cast<int64_t>(blockIdx.x) * kCheckThreads + threadIdx.x, tile));
   if (threadIdx.x == 0) {
     header->verdicts[blockIdx.x] = bad;
     if (blockIdx.x == 0) header->refused = 0;
+  }
+}
+
+// One holder less of page i of sequence j; false (and reported) when it cannot.
+template <typename MetaT>
+__device__ __forceinline__ bool free_unpin(const FreeArgs& f, int64_t j, int64_t i, int64_t seq, uint8_t* unpinned) {
+  const int64_t slot = f.table.tables[seq * f.table.stride + i];
+  bool done = false, fine = true;
+  if (slot >= f.pool.num_slots) {
+    report(f.pool.status, KVCA_ERR_BAD_INDEX, slot);
+    fine = false;
+  } else if (slot >= 0) {
+    done = fine = add_pin(static_cast<MetaT*>(f.pool.slot_meta), slot, -1, true);
+    if (!done) report(f.pool.status, KVCA_ERR_BAD_ARGUMENT, slot);  // held by fewer sequences than name it
+  }
+  unpinned[j * f.table.width + i] = done;
+  return fine;
+}
+
+// Entry i of sequence j cleared, and with `discard` its page unmapped if
+// nobody holds it any more (every sequence that held it writes the same
+// words); or the pin back.
+template <typename MetaT>
+__device__ __forceinline__ void free_page(const FreeArgs& f, int64_t j, int64_t i, int64_t seq, bool refused,
+                                          const uint8_t* unpinned) {
+  const PageTable& t = f.table;
+  MetaT* const meta = static_cast<MetaT*>(f.pool.slot_meta);
+  const int64_t slot = t.tables[seq * t.stride + i];
+  if (refused) {
+    if (unpinned[j * t.width + i]) add_pin(meta, slot, 1, false);
+    return;
+  }
+  t.tables[seq * t.stride + i] = -1;
+  if (slot < 0 || !f.discard) return;
+  if (Meta<MetaT>::pin(*reinterpret_cast<volatile MetaT*>(meta + slot)) != 0) return;
+  const int64_t id = *reinterpret_cast<volatile int64_t*>(f.pool.p2l + slot);
+  if (id >= 0 && id < f.pool.num_logical) f.pool.l2p[id] = -1;
+  f.pool.p2l[slot] = -1;
+  meta[slot] = 0;
+}
+
+// A small call by one block.
+template <typename MetaT>
+__global__ void __launch_bounds__(kCheckThreads) free_small_kernel(const __grid_constant__ FreeArgs f,
+                                                                  uint8_t* unpinned) {
+  __shared__ int64_t tile[kCheckThreads];
+  if (__syncthreads_or(free_refused(f, threadIdx.x, tile))) return;
+  const PageTable& t = f.table;
+  // a sequence's pages to as many warps as there are for it
+  const int warps = kCheckThreads / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int team = f.count >= warps ? 1 : warps / static_cast<int>(f.count);
+  const int teams = warps / team;
+  const bool plays = warp < team * teams;
+  const int64_t first = warp % team * 32 + lane;
+  bool fine = true;
+  for (int64_t j = warp / team; plays && j < f.count; j += teams) {
+    const int64_t pages = f.lens_before[j] > 0 ? pages_of(f.lens_before[j], t.block_size) : 0;
+    for (int64_t i = first; i < pages; i += team * 32) fine &= free_unpin<MetaT>(f, j, i, f.sequences[j], unpinned);
+  }
+  const bool refused = __syncthreads_or(!fine) != 0;
+  for (int64_t j = warp / team; plays && j < f.count; j += teams) {
+    const int64_t len = f.lens_before[j], pages = len > 0 ? pages_of(len, t.block_size) : 0;
+    for (int64_t i = first; i < pages; i += team * 32) free_page<MetaT>(f, j, i, f.sequences[j], refused, unpinned);
+    if (!refused && first == 0 && len > 0) t.lens[f.sequences[j]] = 0;
   }
 }
 
@@ -289,30 +452,13 @@ __global__ void __launch_bounds__(kPageThreads) free_unpin_kernel(const __grid_c
   if (!checks_passed(header, checks)) return;
   const PageTable& t = f.table;
   const int64_t j = blockIdx.x;
-  const int64_t seq = f.sequences[j];
-  const int64_t len = t.lens[seq];
+  const int64_t seq = f.sequences[j], len = f.lens_before[j];
   const int64_t pages = len > 0 ? pages_of(len, t.block_size) : 0;
   const int64_t base = static_cast<int64_t>(blockIdx.y) * kEntriesPerBlock;
-  for (int64_t i = base + threadIdx.x; i < pages && i < base + kEntriesPerBlock; i += kPageThreads) {
-    const int64_t slot = t.tables[seq * t.stride + i];
-    bool done = false;
-    if (slot >= f.pool.num_slots) {
-      report(f.pool.status, KVCA_ERR_BAD_INDEX, slot);
-      header->refused = 1;
-    } else if (slot >= 0) {
-      done = add_pin(static_cast<MetaT*>(f.pool.slot_meta), slot, -1, true);
-      if (!done) {
-        report(f.pool.status, KVCA_ERR_BAD_ARGUMENT, slot);  // held by fewer sequences than name it
-        header->refused = 1;
-      }
-    }
-    unpinned[j * t.width + i] = done;
-  }
+  for (int64_t i = base + threadIdx.x; i < pages && i < base + kEntriesPerBlock; i += kPageThreads)
+    if (!free_unpin<MetaT>(f, j, i, seq, unpinned)) header->refused = 1;
 }
 
-// Entries and lengths cleared, and with `discard` the pages that nobody holds
-// any more unmapped (by every sequence that held one: the same words); or the
-// pins back.
 template <typename MetaT>
 __global__ void __launch_bounds__(kPageThreads) free_commit_kernel(const __grid_constant__ FreeArgs f,
                                                                    const PageHeader* header, const uint8_t* unpinned,
@@ -321,26 +467,12 @@ __global__ void __launch_bounds__(kPageThreads) free_commit_kernel(const __grid_
   if (!checks_passed(header, checks)) return;
   const bool refused = header->refused != 0;
   const PageTable& t = f.table;
-  MetaT* const meta = static_cast<MetaT*>(f.pool.slot_meta);
   const int64_t j = blockIdx.x;
-  const int64_t seq = f.sequences[j];
-  const int64_t len = f.lens_before[j];
+  const int64_t seq = f.sequences[j], len = f.lens_before[j];
   const int64_t pages = len > 0 ? pages_of(len, t.block_size) : 0;
   const int64_t base = static_cast<int64_t>(blockIdx.y) * kEntriesPerBlock;
-  for (int64_t i = base + threadIdx.x; i < pages && i < base + kEntriesPerBlock; i += kPageThreads) {
-    const int64_t slot = t.tables[seq * t.stride + i];
-    if (refused) {
-      if (unpinned[j * t.width + i]) add_pin(meta, slot, 1, false);
-      continue;
-    }
-    t.tables[seq * t.stride + i] = -1;
-    if (slot < 0 || !f.discard) continue;
-    if (Meta<MetaT>::pin(*reinterpret_cast<volatile MetaT*>(meta + slot)) != 0) continue;
-    const int64_t id = *reinterpret_cast<volatile int64_t*>(f.pool.p2l + slot);
-    if (id >= 0 && id < f.pool.num_logical) f.pool.l2p[id] = -1;
-    f.pool.p2l[slot] = -1;
-    meta[slot] = 0;
-  }
+  for (int64_t i = base + threadIdx.x; i < pages && i < base + kEntriesPerBlock; i += kPageThreads)
+    free_page<MetaT>(f, j, i, seq, refused, unpinned);
   if (!refused && blockIdx.y == 0 && threadIdx.x == 0 && len > 0) t.lens[seq] = 0;
 }
 
@@ -383,9 +515,13 @@ __global__ void __launch_bounds__(1024) compact_rank_kernel(const __grid_constan
   dependent_wait();
   dependent_trigger();
   int64_t before = 0, all = 0;
-  for (int i = threadIdx.x; i < runs; i += 1024) {
-    all += counts[i];
-    if (i < static_cast<int>(blockIdx.x)) before += counts[i];
+  if (runs == 1) {  // counted here
+    for (int64_t slot = threadIdx.x; slot < c.pool.num_slots; slot += 1024) all += slot_live<MetaT>(c.pool, slot) ? 1 : 0;
+  } else {
+    for (int i = threadIdx.x; i < runs; i += 1024) {
+      all += counts[i];
+      if (i < static_cast<int>(blockIdx.x)) before += counts[i];
+    }
   }
   int64_t rank, live;
   block_excl_scan(before, &rank, scan);
@@ -490,25 +626,35 @@ int copy_grid(int64_t items, int sms) {
   return static_cast<int>(blocks < most ? blocks : most);
 }
 
+// Calls whose checks, pins and tables one block does in one launch, against
+// three (two with a fork's bytes): each launch costs 4-5 us of the host's time
+// and 2-3 of the GPU's, a block 1,024 entries each few us.
+bool is_small(int64_t count, int64_t width) { return count <= kCheckThreads && count * width <= 8 * 1024; }
+
 template <typename MetaT>
 cudaError_t launch_fork_typed(const ForkArgs& f, const PagedSide& cache, int num_planes, int64_t row_bytes, int vec,
                               void* workspace, cudaStream_t stream) {
   PageHeader* const header = static_cast<PageHeader*>(workspace);
   uint8_t* const pinned = static_cast<uint8_t*>(workspace) + sizeof(PageHeader);
-  const int checks = static_cast<int>((f.count + 1023) / 1024);
-  fork_check_kernel<MetaT><<<checks, 1024, 0, stream>>>(f, header);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+  const int checks = static_cast<int>((f.count + kCheckThreads - 1) / kCheckThreads);
   const int chunks = page_chunks(f.table.width);
   const unsigned count = static_cast<unsigned>(f.count);
-  if (chunks > 0) {
+  const bool small = is_small(f.count, f.table.width);
+  if (small)
+    fork_small_kernel<MetaT><<<1, kCheckThreads, 0, stream>>>(f, header, pinned);
+  else
+    fork_check_kernel<MetaT><<<checks, kCheckThreads, 0, stream>>>(f, header);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  if (!small && chunks > 0) {
     e = launch_dependent(fork_pin_kernel<MetaT>, dim3(count, chunks), kPageThreads, 0, stream, f, header, pinned,
                          checks);
     if (e != cudaSuccess) return e;
   }
   const int64_t parts = (f.table.block_size * row_bytes + kCopyBytes - 1) / kCopyBytes;
   const int copies = copy_grid(f.count * num_planes * parts, device_sm_count());
-  const unsigned grid = static_cast<unsigned>(copies) + count * static_cast<unsigned>(chunks > 0 ? chunks : 1);
+  const unsigned grid =
+      static_cast<unsigned>(copies) + (small ? 0u : count * static_cast<unsigned>(chunks > 0 ? chunks : 1));
   auto go = [&](auto kernel) {
     return launch_dependent(kernel, dim3(grid), kPageThreads, 0, stream, f, cache, num_planes, row_bytes,
                             static_cast<const PageHeader*>(header), static_cast<const uint8_t*>(pinned), checks,
@@ -531,11 +677,14 @@ cudaError_t launch_compact_typed(const CompactArgs& c, const PagedSide& cache, i
   int32_t* const counts = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + 256);
   int32_t* const holes = counts + runs;
   int32_t* const movers = holes + c.pool.num_slots;
-  compact_count_kernel<MetaT><<<runs, 1024, 0, stream>>>(c, counts);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  e = launch_dependent(compact_rank_kernel<MetaT>, dim3(runs), 1024, 0, stream, c, header,
-                       static_cast<const int32_t*>(counts), runs, holes, movers);
+  if (runs > 1) {
+    compact_count_kernel<MetaT><<<runs, 1024, 0, stream>>>(c, counts);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  // (alone, the ranks wait for the work before this call)
+  const cudaError_t e = launch_dependent(compact_rank_kernel<MetaT>, dim3(runs), 1024, 0, stream, c, header,
+                                         static_cast<const int32_t*>(counts), runs, holes, movers);
   if (e != cudaSuccess) return e;
   const int sms = device_sm_count();
   const int64_t parts = (c.table.block_size * row_bytes + kCopyBytes - 1) / kCopyBytes;
@@ -565,8 +714,12 @@ cudaError_t launch_free_typed(const FreeArgs& args, void* workspace, cudaStream_
   PageHeader* const header = static_cast<PageHeader*>(workspace);
   f.lens_before = reinterpret_cast<int64_t*>(header + 1);
   uint8_t* const unpinned = reinterpret_cast<uint8_t*>(f.lens_before + f.count);
-  const int checks = static_cast<int>((f.count + 1023) / 1024);
-  free_check_kernel<<<checks, 1024, 0, stream>>>(f, header);
+  if (is_small(f.count, f.table.width)) {
+    free_small_kernel<MetaT><<<1, kCheckThreads, 0, stream>>>(f, unpinned);
+    return cudaGetLastError();
+  }
+  const int checks = static_cast<int>((f.count + kCheckThreads - 1) / kCheckThreads);
+  free_check_kernel<<<checks, kCheckThreads, 0, stream>>>(f, header);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const int chunks = page_chunks(f.table.width);
