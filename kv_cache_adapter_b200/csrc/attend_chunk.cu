@@ -551,7 +551,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp >= 12) {
     // ------------------------------------------------------------------ MMA
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 12 && working) {
       // the whole warp keeps step, one lane issues
       constexpr uint32_t kScores = mma_shape(kBf16, 128, kKeys, false);
@@ -759,7 +758,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= 8) {
     // ---------------------------------------------------------------- loads
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (working) {
       const int w = warp - 8;
       constexpr int kRowChunks = DP / 8;             // of a row in shared memory
@@ -892,7 +890,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // -------------------------------------------------------------- softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const int q = warp >> 2;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t scores = tmem + lanes + q * 128, output = tmem + lanes + 256 + q * 128;
@@ -931,38 +928,49 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             ++phase;
             fence_after_sync();
-            float x[4][32];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) tmem_load32(x[j], scores + j * 32);
-            tmem_wait_load();
-#pragma unroll
-            for (int j = 0; j < 4; ++j) tmem_landed(x[j]);
-            // Hidden keys: behind the row's own token, which only the block's
-            // last tiles have, or between the sinks and the window.
-            if (v0 + kKeys - 1 > all_last) {
-              const int last = v_last - v0;
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int k = 0; k < 32; ++k) x[j][k] = j * 32 + k > last ? -INFINITY : x[j][k];
-            }
-            if (v0 + kKeys > a.sinks && max(v0, a.sinks) <= all_low) {
-              const int first = a.sinks - v0;
-              const unsigned gap = max(v_low - v0 + 1 - first, 0);
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
+            // Hidden keys, behind the row's own token (only the block's last
+            // tiles have any) or between the sinks and the window, are
+            // overwritten before anything reads them.
+            if (v0 + kKeys - 1 > all_last || (v0 + kKeys > a.sinks && max(v0, a.sinks) <= all_low)) {
+#pragma unroll 1
+              for (int j = 0; j < 4; ++j) {
+                float x[32];
+                tmem_load32(x, scores + j * 32);
+                tmem_wait_load();
+                tmem_landed(x);
+                const int last = v_last - v0 - j * 32, first = a.sinks - v0 - j * 32;
+                const unsigned gap = max(v_low - v0 - j * 32 + 1 - first, 0);
 #pragma unroll
                 for (int k = 0; k < 32; ++k)
-                  x[j][k] = static_cast<unsigned>(j * 32 + k - first) < gap ? -INFINITY : x[j][k];
+                  x[k] = (k > last) | (static_cast<unsigned>(k - first) < gap) ? -INFINITY : x[k];
+                tmem_store32(scores + j * 32, x);
+              }
+              tmem_wait_store();
             }
-            float top[4];
+            float xa[32], xb[32];
+            float best = -INFINITY;
+            auto largest = [&](const float (&x)[32]) {
+              float top[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) top[j] = fmaxf(x[j][0], x[j][1]);
+              for (int k = 0; k < 4; ++k) top[k] = fmaxf(x[2 * k], x[2 * k + 1]);
 #pragma unroll
-            for (int k = 2; k < 32; k += 2)
+              for (int k = 8; k < 32; k += 8)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) top[j] = max3(top[j], x[j][k], x[j][k + 1]);
-            const float best = fmaxf(max3(top[0], top[1], top[2]), top[3]);
+                for (int i = 0; i < 4; ++i) top[i] = max3(top[i], x[k + 2 * i], x[k + 2 * i + 1]);
+              best = fmaxf(best, fmaxf(max3(top[0], top[1], top[2]), top[3]));
+            };
+            tmem_load32(xa, scores);
+#pragma unroll 1
+            for (int j = 0; j < 4; j += 2) {
+              tmem_wait_load();
+              tmem_landed(xa);
+              tmem_load32(xb, scores + j * 32 + 32);
+              largest(xa);
+              tmem_wait_load();
+              tmem_landed(xb);
+              tmem_load32(xa, scores + ((j * 32 + 64) & 127));  // around to the first for the second pass
+              largest(xb);
+            }
             const float old = m;
             // (-inf) - (-inf) is no growth
             if ((best - m) * unit > kGrowth) m = best;
@@ -970,17 +978,27 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float decay = m != old ? exp2_approx(old * unit - base) : 1.f;
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             const float2 units = make_float2(unit, unit), bases = make_float2(-base, -base);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            auto weigh = [&](const float (&x)[32], int j) {
               uint32_t packed[16];
 #pragma unroll
               for (int k = 0; k < 32; k += 2) {
-                float2 e = fma2(make_float2(x[j][k], x[j][k + 1]), units, bases);
+                float2 e = fma2(make_float2(x[k], x[k + 1]), units, bases);
                 e = make_float2(exp2_approx(e.x), exp2_approx(e.y));
                 sum[(k >> 1) & 1] = add2(sum[(k >> 1) & 1], e);
                 packed[k >> 1] = pack2<kBf16>(e.x, e.y);
               }
               tmem_store16(scores + j * 16, packed);
+            };
+#pragma unroll 1
+            for (int j = 0; j < 4; j += 2) {
+              tmem_wait_load();
+              tmem_landed(xa);
+              tmem_load32(xb, scores + j * 32 + 32);
+              weigh(xa, j);
+              tmem_wait_load();
+              tmem_landed(xb);
+              if (j == 0) tmem_load32(xa, scores + 64);
+              weigh(xb, j + 1);
             }
             l = l * decay + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
             if (i > 0 && __any_sync(0xffffffffu, m != old)) {
