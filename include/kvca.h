@@ -762,16 +762,19 @@ typedef struct kvca_attend_desc {
  * Attention of one new token per sequence: row s of query and out is the last
  * token of sequence s (position seq_lens[s] - 1; the decode step after the
  * token scatter of adapter.py:1275-1285).  seq_lens[s] == 0 gives zeros (lse
- * -inf).  Two launches, no host synchronisation; the work is split evenly
- * over the SMs whatever the lengths.  workspace:
+ * -inf).  One launch, no host synchronisation; the work is split evenly over
+ * the SMs whatever the lengths.  workspace:
  * kvca_attend_step_workspace_bytes(desc) bytes (lengths and values do not
- * matter) of device memory, 16-byte aligned, any contents; calls that may
- * overlap on the GPU need one each.  No reference counterpart: the reference
+ * matter) of device memory, 16-byte aligned, any contents.  d_counters:
+ * kvca_attend_step_counters() words, zero on entry and zero again on exit.
+ * Calls that may overlap on the GPU (other streams, graphs replayed side by
+ * side) need both of their own.  No reference counterpart: the reference
  * places the pages that an engine's attention reads.
  */
+int64_t kvca_attend_step_counters(void);
 int64_t kvca_attend_step_workspace_bytes(const kvca_attend_desc* desc);
-int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t workspace_bytes, int64_t* d_status,
-                     kvca_stream_t stream);
+int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t workspace_bytes, uint32_t* d_counters,
+                     int64_t* d_status, kvca_stream_t stream);
 
 /*
  * Attention of a ragged chunk of new tokens per sequence (a prompt, the next
@@ -785,8 +788,8 @@ int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t wo
  * KVCA_ERR_BAD_INDEX (that sequence's rows then hold no defined values).
  * head_dim is at most 128.  Three launches, no host synchronisation; the work
  * is split evenly over the SMs whatever the lengths.  workspace:
- * kvca_attend_chunk_workspace_bytes(desc, num_rows) bytes, as for
- * kvca_attend_step.  A bounded wait that runs out gives
+ * kvca_attend_chunk_workspace_bytes(desc, num_rows) bytes, 16-byte aligned, any
+ * contents, one for each call that may overlap another.  A bounded wait that runs out gives
  * KVCA_ERR_DEVICE_TIMEOUT.  No reference counterpart.
  */
 int64_t kvca_attend_chunk_workspace_bytes(const kvca_attend_desc* desc, int64_t num_rows);

@@ -11,8 +11,9 @@
 // shared memory (cp.async, no barrier with other warps) and keeps the running
 // maximum and sum of the softmax and the output in registers.  A (sequence,
 // head group) that lies inside one run is written directly; one that several
-// runs share leaves a partial result per warp (joined within the CTA first),
-// which a second, programmatically launched kernel joins in run order.
+// runs share leaves a partial result per CTA; the CTA that leaves the last of a
+// segment's results joins them, in run order (a second kernel for that cost 6
+// us of 94 with 96 ragged sequences, and a launch).
 //
 // Both products run transposed on m16n8k16: S^T = K Q^T has the 16 tokens as
 // rows and up to 8 query heads that share the K/V head as columns, O^T = V^T
@@ -50,9 +51,6 @@ struct StepShape {
   static constexpr int kStageBytes = 2 * kTile * kRowBytes;
   static constexpr int kWarps = step_warps(kRowBytes, NG);
   static constexpr int kThreads = 32 * kWarps;
-  // Registers of two more warps stay free with 8 warps, so that a block of
-  // the joining kernel fits beside the CTA and waits there.
-  static constexpr int kBound = kWarps == 8 ? 320 : kThreads;
   // 192 KiB of rings per SM
   static constexpr int kRingBytes = 192 * 1024 / kWarps;
   static constexpr int kStages = kRingBytes / kStageBytes < 8 ? kRingBytes / kStageBytes : 8;
@@ -120,51 +118,54 @@ struct StepLayout {
     groups = warps / span;
   }
   // The warp (of the grid) that has run r for the j-th of a run's heads.
-  __device__ __forceinline__ int64_t warp_of(int64_t r, int j, int warps) const {
-    return r / groups * warps + r % groups * span + j;
+  __device__ __forceinline__ int warp_of(int r, int j, int warps) const {
+    const int cta = r / groups;
+    return cta * warps + (r - cta * groups) * span + j;
   }
 };
 
-// The workspace: the run bounds, then what each warp left.
-struct StepHeader {
-  int64_t tiles;  // of the whole call, segment costs included
-  int64_t runs;   // that got tiles
-};
+// A segment that several runs share leaves one result per CTA (its first run's
+// place) and one from the run that ends it, unless that is a CTA's first.
+__device__ __forceinline__ int result_count(int first_run, int last_run, int groups) {
+  const int cta = first_run / groups, last_cta = last_run / groups;
+  return last_cta - cta + 1 + (cta == last_cta || last_run != last_cta * groups ? 1 : 0);
+}
 
-struct StepPiece {
-  int32_t tail;   // segment whose continuation this warp's slot 0 holds, or -1
-  int32_t head;   // segment whose beginning slot 1 holds, or -1
-  int32_t last;   // run with the last tile of `head`
-  int32_t unused;
-};
+__device__ __forceinline__ int result_run(int k, int first_run, int last_run, int groups) {
+  const int cta = first_run / groups, last_cta = last_run / groups;
+  return k == 0 ? first_run : k <= last_cta - cta ? (cta + k) * groups : last_run;
+}
 
+// The workspace: two partial results per warp, slot 0 for a segment that an
+// earlier run began, slot 1 for one that this warp's run began.
 template <int kHeads, int kAcc>
 struct StepWorkspace {
-  StepHeader* header;
-  StepPiece* pieces;
   float* ml;   // [warp][slot][2][heads]: maxima, then sums
   float* acc;  // [warp][slot][dim][heads]
 
   static __host__ __device__ size_t bytes(int64_t warps) {
-    return 256 + static_cast<size_t>(warps) * (sizeof(StepPiece) + 2 * (2 * kHeads + kAcc) * sizeof(float));
+    return static_cast<size_t>(warps) * 2 * (2 * kHeads + kAcc) * sizeof(float);
   }
   __host__ __device__ StepWorkspace(void* base, int64_t warps) {
-    char* p = static_cast<char*>(base);
-    header = reinterpret_cast<StepHeader*>(p);
-    acc = reinterpret_cast<float*>(p + 256);
+    acc = static_cast<float*>(base);
     ml = acc + warps * 2 * kAcc;
-    pieces = reinterpret_cast<StepPiece*>(ml + warps * 2 * 2 * kHeads);
   }
   __device__ __forceinline__ float* ml_of(int64_t warp, int slot) const { return ml + (warp * 2 + slot) * 2 * kHeads; }
   __device__ __forceinline__ float* acc_of(int64_t warp, int slot) const { return acc + (warp * 2 + slot) * kAcc; }
+};
+
+// A segment to join.
+struct StepJoin {
+  int segment;
+  int first_run, last_run;
 };
 
 __device__ __forceinline__ int64_t run_begin(int64_t tiles, int64_t runs, int64_t r) {
   return tiles * r / runs;  // below 2^31 tiles x a few thousand runs
 }
 
-__device__ __forceinline__ int64_t run_of(int64_t tiles, int64_t runs, int64_t t) {
-  return (runs * (t + 1) - 1) / tiles;
+__device__ __forceinline__ int run_of(int64_t tiles, int64_t runs, int64_t t) {
+  return static_cast<int>((runs * (t + 1) - 1) / tiles);
 }
 
 // A position in the numbering of tiles: sequence, chunk of head groups, tile.
@@ -203,8 +204,8 @@ __device__ __forceinline__ int64_t sequence_share(int tiles, int chunks) {
 }
 
 template <typename Cache, int DP, int NG>
-__global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kBound, 1)
-    attend_step_kernel(const __grid_constant__ AttendArgs a, void* workspace) {
+__global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
+    attend_step_kernel(const __grid_constant__ AttendArgs a, void* workspace, uint32_t* arrived) {
   using Shape = StepShape<Cache, DP, NG>;
   constexpr bool kBf16 = Cache::kBf16;
   constexpr bool kE4m3 = Cache::kBytes == 1;
@@ -217,7 +218,10 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kBound, 1)
   __shared__ int64_t prefix[kScanGroups + 1];
   __shared__ int64_t scan[33];
   __shared__ int held[kWarps];
-  __shared__ float held_ml[kWarps][2 * kHeads];
+  __shared__ bool held_begins[kWarps];
+  __shared__ __align__(16) float held_ml[kWarps][2 * kHeads];
+  __shared__ StepJoin joins[2 * kWarps];
+  __shared__ int join_count;
 
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
@@ -250,9 +254,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kBound, 1)
   const int64_t tiles = run;
   const int64_t all = static_cast<int64_t>(gridDim.x) * layout.groups;
   const int64_t runs = min(all, tiles);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *ws.header = StepHeader{tiles, runs};
+  if (threadIdx.x == 0) join_count = 0;
   __syncthreads();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // Sequences without tokens: the sum over nothing.
   for (int seq = blockIdx.x; seq < a.num_seqs; seq += gridDim.x) {
@@ -270,7 +273,10 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kBound, 1)
   const int lane_of_heads = warp % span;
   int held_segment = -1;
   bool held_starts = false;
-  StepPiece piece{-1, -1, -1, 0};
+  StepJoin held_runs{-1, 0, 0};
+  // what this warp leaves, and the runs of its segment: of a segment that an
+  // earlier run began (slot 0), and of one that this run began (slot 1)
+  StepJoin leaves[2] = {{-1, 0, 0}, {-1, 0, 0}};
 
   float acc[NG][kSteps][4];
   float m[NG][2], l[NG][2];  // of the heads 2 * (lane % 4), + 1 of each tile of 8
@@ -593,6 +599,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kBound, 1)
           l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], 16);
         }
       const int segment = at.seq * layout.parts + at.chunk * span + lane_of_heads;
+      const int64_t here = finish - at.left - at.tile;  // the segment's first tile in the numbering
+      const int this_run = static_cast<int>(my_run);
       if (ends && starts) {
         const int part = at.chunk * span + lane_of_heads;
         const int kv_head = part / head_groups;
@@ -638,7 +646,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kBound, 1)
         }
       } else if (ends) {
         // the end of a segment that an earlier run began
-        piece.tail = segment;
+        leaves[0] = StepJoin{segment, run_of(tiles, runs, here), this_run};
         float* const ml = ws.ml_of(own, 0);
         float* const part = ws.acc_of(own, 0);
 #pragma unroll
@@ -659,8 +667,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kBound, 1)
       } else {
         held_segment = segment;
         held_starts = starts;
-        if (starts)
-          piece.last = static_cast<int>(run_of(tiles, runs, finish - at.left + (at.tiles - 1 - at.tile)));
+        held_runs = StepJoin{segment, starts ? this_run : run_of(tiles, runs, here),
+                             run_of(tiles, runs, here + at.tiles - 1)};
       }
       if (go) {
         at.advance(a, chunks);
@@ -673,7 +681,10 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kBound, 1)
 
   // Partial results that the CTA's warps still hold, joined where runs that
   // follow each other hold the same segment: the rings are free now.
-  if (lane == 0) held[warp] = held_segment;
+  if (lane == 0) {
+    held[warp] = held_segment;
+    held_begins[warp] = held_starts;
+  }
   __syncthreads();
   float* const parked = reinterpret_cast<float*>(rings);
   if (held_segment >= 0) {
@@ -697,9 +708,9 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kBound, 1)
       }
     }
     const bool leads = warp < span || held[warp - span] != held_segment;
-    if (leads) (held_starts ? piece.head : piece.tail) = held_segment;
+    if (leads && held_starts) leaves[1] = held_runs;
+    if (leads && !held_starts) leaves[0] = held_runs;
   }
-  if (lane == 0 && my_run < runs) ws.pieces[own] = piece;
   __syncthreads();
   for (int w = 0; w < kWarps; ++w) {
     const int segment = held[w];
@@ -709,7 +720,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kBound, 1)
     // a run whose only tiles continue a segment leads with slot 0, one that
     // began it with slot 1
     const int64_t leader = static_cast<int64_t>(blockIdx.x) * kWarps + w;
-    const bool begins = ws.pieces[leader].head == segment;
+    const bool begins = held_begins[w];
     float* const out = ws.acc_of(leader, begins ? 1 : 0);
     float* const ml = ws.ml_of(leader, begins ? 1 : 0);
     for (int i = threadIdx.x; i < Shape::kAcc; i += Shape::kThreads) {
@@ -730,120 +741,141 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kBound, 1)
       }
     }
   }
-}
 
-// Joins the partial results of the segments that several runs share: one block
-// per warp that began such a segment.  Its warps take the runs in turn, a lane
-// for the same elements of each, and meet in shared memory; a chain of three
-// dependent reads (what the owner left, the runs' results, no more) bounds it.
-template <int DP, int NG>
-struct JoinShape {
-  static constexpr int kHeads = 8 * NG;
-  static constexpr int kAcc = DP * kHeads;
-  static constexpr int kWarps = 4096 / kAcc < 8 ? 4096 / kAcc : 8;  // 16 KiB of results: a block fits beside a CTA
-  static constexpr int kThreads = 32 * kWarps;
-  static constexpr int kVecs = kAcc / 128;  // float4 per lane
-};
-
-template <int DP, int NG>
-__global__ void __launch_bounds__(JoinShape<DP, NG>::kThreads)
-    attend_step_join_kernel(const __grid_constant__ AttendArgs a, void* workspace, int64_t all_warps, int warps) {
-  using Shape = JoinShape<DP, NG>;
-  constexpr int kHeads = Shape::kHeads;
-  constexpr int kAcc = Shape::kAcc;
-  __shared__ __align__(16) float parked[Shape::kWarps][kAcc];
-  __shared__ __align__(16) float parked_ml[Shape::kWarps][2][kHeads];
-  const StepLayout layout(a.kv_heads, a.group, kHeads, warps);
-  const int64_t owner = blockIdx.x;
-  const int lane_of_heads = static_cast<int>(blockIdx.x) % warps % layout.span;
-  const int64_t first_run = static_cast<int64_t>(blockIdx.x) / warps * layout.groups + blockIdx.x % warps / layout.span;
-  StepWorkspace<kHeads, kAcc> ws(workspace, all_warps);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const StepPiece own = ws.pieces[owner];
-  if (first_run >= ws.header->runs || own.head < 0) return;
-  const int segment = own.head;
-
-  const int h4 = lane * 4 % kHeads;  // this lane's four heads
-  float4 top = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY), total = make_float4(0.f, 0.f, 0.f, 0.f);
-  float4 sum[Shape::kVecs];
-#pragma unroll
-  for (int v = 0; v < Shape::kVecs; ++v) sum[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto fold = [](float& m, float next, float& keep, float& weight) {
-    const float best = fmaxf(m, next), base = best == -INFINITY ? 0.f : best;
-    keep = exp2_approx(m - base);
+  // Whoever leaves the last result of a segment joins them: a warp alone while
+  // they are few, the CTA when they are many (a long sequence over all SMs).
+  // The count of a segment's results is kept at its first run's warp, and is
+  // zero again then.
+  constexpr int kVecs = Shape::kAcc / 128;  // float4 per lane
+  constexpr int kWarpResults = 8;
+  const int h4 = lane * 4 % kHeads;         // a lane's four heads
+  float4 top, total, sum[kVecs];
+  auto fold = [](float& old, float next, float& keep, float& weight) {
+    const float best = fmaxf(old, next), base = best == -INFINITY ? 0.f : best;
+    keep = exp2_approx(old - base);
     weight = exp2_approx(next - base);
-    m = best;
+    old = best;
   };
-  // Behind the owner: the first run of each later CTA (which leads what the
-  // CTA's runs still held) and the run with the segment's end.
-  const int64_t cta = first_run / layout.groups, last_cta = own.last / layout.groups;
-  const int64_t pieces = last_cta - cta + 1 + (cta == last_cta || own.last % layout.groups != 0 ? 1 : 0);
-  for (int64_t k = warp; k < pieces; k += Shape::kWarps) {
-    const int64_t r = k == 0 ? first_run : k <= last_cta - cta ? (cta + k) * layout.groups : own.last;
-    const int64_t w = layout.warp_of(r, lane_of_heads, warps);
-    const int slot = w == owner ? 1 : 0;
-    const int tail = __ldcg(&ws.pieces[w].tail);
-    const float4 m = __ldcg(reinterpret_cast<const float4*>(ws.ml_of(w, slot) + h4));
-    const float4 l = __ldcg(reinterpret_cast<const float4*>(ws.ml_of(w, slot) + kHeads + h4));
-    const float4* const from = reinterpret_cast<const float4*>(ws.acc_of(w, slot)) + lane;
-    float4 o[Shape::kVecs];
+  const int groups_of = layout.groups;
+  auto gather = [&](const StepJoin& join, int results, int first_result, int stride) {
+    top = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    total = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int v = 0; v < Shape::kVecs; ++v) o[v] = __ldcg(from + 32 * v);
-    if (slot == 0 && tail != segment) continue;  // joined within its CTA, or another segment's
-    float4 keep, weight;
-    fold(top.x, m.x, keep.x, weight.x);
-    fold(top.y, m.y, keep.y, weight.y);
-    fold(top.z, m.z, keep.z, weight.z);
-    fold(top.w, m.w, keep.w, weight.w);
-    total.x = total.x * keep.x + l.x * weight.x;
-    total.y = total.y * keep.y + l.y * weight.y;
-    total.z = total.z * keep.z + l.z * weight.z;
-    total.w = total.w * keep.w + l.w * weight.w;
+    for (int v = 0; v < kVecs; ++v) sum[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int k = first_result; k < results; k += stride) {
+      const int r = result_run(k, join.first_run, join.last_run, groups_of);
+      const int w = layout.warp_of(r, join.segment % layout.parts % span, kWarps);
+      const int slot = k == 0 ? 1 : 0;
+      const float4 mk = __ldcg(reinterpret_cast<const float4*>(ws.ml_of(w, slot) + h4));
+      const float4 lk = __ldcg(reinterpret_cast<const float4*>(ws.ml_of(w, slot) + kHeads + h4));
+      const float4* const from = reinterpret_cast<const float4*>(ws.acc_of(w, slot)) + lane;
+      float4 o[kVecs];
 #pragma unroll
-    for (int v = 0; v < Shape::kVecs; ++v) {
-      sum[v].x = sum[v].x * keep.x + o[v].x * weight.x;
-      sum[v].y = sum[v].y * keep.y + o[v].y * weight.y;
-      sum[v].z = sum[v].z * keep.z + o[v].z * weight.z;
-      sum[v].w = sum[v].w * keep.w + o[v].w * weight.w;
+      for (int v = 0; v < kVecs; ++v) o[v] = __ldcg(from + 32 * v);
+      float4 keep, weight;
+      fold(top.x, mk.x, keep.x, weight.x);
+      fold(top.y, mk.y, keep.y, weight.y);
+      fold(top.z, mk.z, keep.z, weight.z);
+      fold(top.w, mk.w, keep.w, weight.w);
+      total.x = total.x * keep.x + lk.x * weight.x;
+      total.y = total.y * keep.y + lk.y * weight.y;
+      total.z = total.z * keep.z + lk.z * weight.z;
+      total.w = total.w * keep.w + lk.w * weight.w;
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        sum[v].x = sum[v].x * keep.x + o[v].x * weight.x;
+        sum[v].y = sum[v].y * keep.y + o[v].y * weight.y;
+        sum[v].z = sum[v].z * keep.z + o[v].z * weight.z;
+        sum[v].w = sum[v].w * keep.w + o[v].w * weight.w;
+      }
+    }
+  };
+  // The joined output from the results of warps [from, to) in shared memory, by
+  // `threads` threads, two dims each at a time.
+  auto put = [&](const StepJoin& join, int from, int to, int thread, int threads) {
+    const int part = join.segment % layout.parts;
+    const int kv_head = part / head_groups;
+    const int first = (part - kv_head * head_groups) * kHeads;
+    const int heads = min(kHeads, a.group - first);
+    const int64_t row =
+        (static_cast<int64_t>(join.segment / layout.parts) * a.kv_heads + kv_head) * a.group + first;
+#pragma unroll 1
+    for (int i = thread; i < kHeads * (DP / 2); i += threads) {
+      const int h = i / (DP / 2), d = i % (DP / 2) * 2;
+      if (h >= heads || d >= a.dim) continue;
+      float best = -INFINITY;
+#pragma unroll 1
+      for (int w = from; w < to; ++w) best = fmaxf(best, held_ml[w][h]);
+      const float base = best == -INFINITY ? 0.f : best;
+      float x = 0.f, y = 0.f, l2 = 0.f;
+#pragma unroll 1
+      for (int w = from; w < to; ++w) {
+        const float weight = exp2_approx(held_ml[w][h] - base);
+        x += weight * parked[w * Shape::kAcc + d * kHeads + h];
+        y += weight * parked[w * Shape::kAcc + (d + 1) * kHeads + h];
+        l2 += weight * held_ml[w][kHeads + h];
+      }
+      const float factor = a.value_scale / l2;
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (row + h) * a.dim + d) =
+          a.query_type == KVCA_TYPE_BF16 ? pack2<true>(x * factor, y * factor) : pack2<false>(x * factor, y * factor);
+      if (a.lse != nullptr && d == 0) a.lse[row + h] = base * kLn2 + logf(l2);
+    }
+  };
+  auto park = [&]() {
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v)
+      *reinterpret_cast<float4*>(parked + warp * Shape::kAcc + (lane + 32 * v) * 4) = sum[v];
+    if (lane * 4 < kHeads) {
+      *reinterpret_cast<float4*>(&held_ml[warp][h4]) = top;
+      *reinterpret_cast<float4*>(&held_ml[warp][kHeads + h4]) = total;
+    }
+  };
+
+  __threadfence();
+  __syncthreads();
+  bool mine_last = false;
+  if (lane < 2) {
+    const StepJoin mine = lane == 0 ? leaves[0] : leaves[1];
+    if (mine.segment >= 0) {
+      uint32_t* const count = arrived + layout.warp_of(mine.first_run, lane_of_heads, kWarps);
+      const int results = result_count(mine.first_run, mine.last_run, layout.groups);
+      if (atomicAdd(count, 1u) == static_cast<uint32_t>(results) - 1) {
+        *count = 0;
+        if (results <= kWarpResults)
+          mine_last = true;
+        else
+          joins[atomicAdd(&join_count, 1)] = mine;
+      }
     }
   }
-#pragma unroll
-  for (int v = 0; v < Shape::kVecs; ++v) *reinterpret_cast<float4*>(&parked[warp][(lane + 32 * v) * 4]) = sum[v];
-  if (lane * 4 < kHeads) {
-    *reinterpret_cast<float4*>(&parked_ml[warp][0][h4]) = top;
-    *reinterpret_cast<float4*>(&parked_ml[warp][1][h4]) = total;
+  __threadfence();
+  const unsigned alone = __ballot_sync(0xffffffffu, mine_last);
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    if (!((alone >> which) & 1u)) continue;
+    const StepJoin join = which == 0 ? leaves[0] : leaves[1];
+    gather(join, result_count(join.first_run, join.last_run, layout.groups), 0, 1);
+    park();
+    __syncwarp();
+    put(join, warp, warp + 1, lane, 32);
+    __syncwarp();
   }
   __syncthreads();
-
-  const int head_groups = (a.group + kHeads - 1) / kHeads;
-  const int seq = segment / layout.parts, part = segment - seq * layout.parts;
-  const int kv_head = part / head_groups;
-  const int first = (part - kv_head * head_groups) * kHeads;
-  const int64_t row = (static_cast<int64_t>(seq) * a.kv_heads + kv_head) * a.group;
-  for (int i = threadIdx.x; i < kAcc; i += Shape::kThreads) {
-    const int h = i / DP, d = i % DP;
-    if (first + h >= a.group || d >= a.dim) continue;
-    float best = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < Shape::kWarps; ++w) best = fmaxf(best, parked_ml[w][0][h]);
-    const float base = best == -INFINITY ? 0.f : best;
-    float x = 0.f, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < Shape::kWarps; ++w) {
-      const float weight = exp2_approx(parked_ml[w][0][h] - base);
-      x += weight * parked[w][d * kHeads + h];
-      l += weight * parked_ml[w][1][h];
-    }
-    const float y = x * (a.value_scale / l);
-    static_cast<uint16_t*>(a.out)[(row + first + h) * a.dim + d] =
-        static_cast<uint16_t>(a.query_type == KVCA_TYPE_BF16 ? pack2<true>(y, 0.f) : pack2<false>(y, 0.f));
-    if (a.lse != nullptr && d == 0) a.lse[row + first + h] = base * kLn2 + logf(l);
+  const int join_total = join_count;
+#pragma unroll 1
+  for (int j = 0; j < join_total; ++j) {
+    const StepJoin join = joins[j];
+    gather(join, result_count(join.first_run, join.last_run, layout.groups), warp, kWarps);
+    park();
+    __syncthreads();
+    put(join, 0, kWarps, threadIdx.x, Shape::kThreads);
+    __syncthreads();
   }
 }
 
 template <typename Cache, int DP, int NG>
-cudaError_t launch_typed(const AttendArgs& a, void* workspace, int sms, cudaStream_t stream) {
+cudaError_t launch_typed(const AttendArgs& a, void* workspace, uint32_t* arrived, int sms, cudaStream_t stream) {
   using Shape = StepShape<Cache, DP, NG>;
   auto kernel = attend_step_kernel<Cache, DP, NG>;
   static DeviceFlags configured;
@@ -853,12 +885,8 @@ cudaError_t launch_typed(const AttendArgs& a, void* workspace, int sms, cudaStre
     if (e != cudaSuccess) return e;
     mark_setup(configured, dev);
   }
-  kernel<<<sms, Shape::kThreads, Shape::kSmem, stream>>>(a, workspace);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  const int64_t warps = static_cast<int64_t>(sms) * Shape::kWarps;
-  return launch_dependent(attend_step_join_kernel<DP, NG>, dim3(static_cast<unsigned>(warps)),
-                          JoinShape<DP, NG>::kThreads, 0, stream, a, workspace, warps, Shape::kWarps);
+  kernel<<<sms, Shape::kThreads, Shape::kSmem, stream>>>(a, workspace, arrived);
+  return cudaGetLastError();
 }
 
 template <typename Cache, int DP>
@@ -883,22 +911,24 @@ size_t attend_step_workspace(const AttendArgs& a, int sms) {
 }
 
 template <typename Cache>
-static cudaError_t launch_cache(const AttendArgs& a, void* workspace, int sms, cudaStream_t stream) {
+static cudaError_t launch_cache(const AttendArgs& a, void* workspace, uint32_t* arrived, int sms,
+                                cudaStream_t stream) {
   const int n = head_tiles(a);
   if (a.dim <= 64)
-    return n == 1 ? launch_typed<Cache, 64, 1>(a, workspace, sms, stream)
-                  : launch_typed<Cache, 64, 2>(a, workspace, sms, stream);
+    return n == 1 ? launch_typed<Cache, 64, 1>(a, workspace, arrived, sms, stream)
+                  : launch_typed<Cache, 64, 2>(a, workspace, arrived, sms, stream);
   if (a.dim <= 128)
-    return n == 1 ? launch_typed<Cache, 128, 1>(a, workspace, sms, stream)
-                  : launch_typed<Cache, 128, 2>(a, workspace, sms, stream);
-  return launch_typed<Cache, 256, 1>(a, workspace, sms, stream);
+    return n == 1 ? launch_typed<Cache, 128, 1>(a, workspace, arrived, sms, stream)
+                  : launch_typed<Cache, 128, 2>(a, workspace, arrived, sms, stream);
+  return launch_typed<Cache, 256, 1>(a, workspace, arrived, sms, stream);
 }
 
-cudaError_t launch_attend_step(const AttendArgs& a, void* workspace, int sms, cudaStream_t stream) {
+cudaError_t launch_attend_step(const AttendArgs& a, void* workspace, uint32_t* arrived, int sms,
+                               cudaStream_t stream) {
   switch (a.cache_type) {
-    case KVCA_TYPE_F16: return launch_cache<CacheF16>(a, workspace, sms, stream);
-    case KVCA_TYPE_BF16: return launch_cache<CacheBf16>(a, workspace, sms, stream);
-    default: return launch_cache<CacheE4m3>(a, workspace, sms, stream);
+    case KVCA_TYPE_F16: return launch_cache<CacheF16>(a, workspace, arrived, sms, stream);
+    case KVCA_TYPE_BF16: return launch_cache<CacheBf16>(a, workspace, arrived, sms, stream);
+    default: return launch_cache<CacheE4m3>(a, workspace, arrived, sms, stream);
   }
 }
 

@@ -891,8 +891,12 @@ int64_t kvca_attend_step_workspace_bytes(const kvca_attend_desc* desc) {
   return static_cast<int64_t>(kvca::attend_step_workspace(a, kvca_device_sm_count()));
 }
 
-int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t workspace_bytes, int64_t* d_status,
-                     kvca_stream_t stream) {
+int64_t kvca_attend_step_counters(void) {
+  return static_cast<int64_t>(kvca_device_sm_count()) * kvca::kStepMaxWarps;
+}
+
+int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t workspace_bytes, uint32_t* d_counters,
+                     int64_t* d_status, kvca_stream_t stream) {
   kvca::AttendArgs a;
   const int rc = to_attend(desc, d_status, &a);
   if (rc != KVCA_OK) return rc;
@@ -900,10 +904,10 @@ int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t wo
   if (!attend_pointers_ok(a)) return KVCA_ERR_BAD_ARGUMENT;
   const int sms = kvca_device_sm_count();
   if (sms < 1) return KVCA_ERR_CUDA;
-  if (d_workspace == nullptr || !aligned16(reinterpret_cast<uint64_t>(d_workspace)) ||
+  if (d_workspace == nullptr || !aligned16(reinterpret_cast<uint64_t>(d_workspace)) || d_counters == nullptr ||
       workspace_bytes < static_cast<int64_t>(kvca::attend_step_workspace(a, sms)))
     return KVCA_ERR_BAD_ARGUMENT;
-  return status_of(kvca::launch_attend_step(a, d_workspace, sms, stream));
+  return status_of(kvca::launch_attend_step(a, d_workspace, d_counters, sms, stream));
 }
 
 namespace {

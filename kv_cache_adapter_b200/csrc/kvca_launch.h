@@ -157,7 +157,9 @@ struct ChunkArgs {
 };
 
 size_t attend_step_workspace(const AttendArgs& args, int sms);
-cudaError_t launch_attend_step(const AttendArgs& args, void* workspace, int sms, cudaStream_t stream);
+constexpr int kStepMaxWarps = 16;  // of a CTA: results are counted per warp
+cudaError_t launch_attend_step(const AttendArgs& args, void* workspace, uint32_t* arrived, int sms,
+                               cudaStream_t stream);
 
 constexpr int kChunkMaxDim = 128;  // two output tiles fill the tensor memory
 size_t attend_chunk_workspace(const AttendArgs& args, int64_t rows, int sms);

@@ -1423,6 +1423,23 @@ _ATTEND_TYPES = {torch.float16: _lib.KVCA_TYPE_F16, torch.bfloat16: _lib.KVCA_TY
 _attend_workspace_bytes: dict[tuple, int] = {}
 
 
+_attend_counters: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def _step_counters(dev: torch.device) -> torch.Tensor:
+    """kvca_attend_step's counters of this (device, stream), zero between
+    calls.  A call that is captured gets counters of its own, cleared by the
+    graph, so that graphs captured on one stream may replay side by side."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(int(_lib_handle.kvca_attend_step_counters()), dtype=torch.int32, device=dev)
+    key = (_index(dev), _stream(dev).value or 0)
+    buf = _attend_counters.get(key)
+    if buf is None:
+        buf = torch.zeros(int(_lib_handle.kvca_attend_step_counters()), dtype=torch.int32, device=dev)
+        _attend_counters[key] = buf
+    return buf
+
+
 def _attend_rows(t: torch.Tensor, shape, name: str) -> list[int]:
     """Strides in bytes of the leading dims of rows of head_dim (0 for a dim of size 1)."""
     size = t.element_size()
@@ -1543,8 +1560,9 @@ def attend_step(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
                 _raise_for(_lib.KVCA_ERR_BAD_ARGUMENT, 0, "attend_step")
             _attend_workspace_bytes[shape] = need
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        rc = _lib_handle.kvca_attend_step(ctypes.byref(desc), workspace.data_ptr(), need, _ptr(_status(dev)),
-                                          _stream(dev))
+        counters = _step_counters(dev)
+        rc = _lib_handle.kvca_attend_step(ctypes.byref(desc), workspace.data_ptr(), need, counters.data_ptr(),
+                                          _ptr(_status(dev)), _stream(dev))
     _host_rc(rc, "attend_step")
     _maybe_check(dev, check, "attend_step")
     return out

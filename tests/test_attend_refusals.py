@@ -33,7 +33,7 @@ BAD = [dict(num_seqs=-1), dict(num_blocks=-1), dict(block_size=0), dict(table_wi
 def test_c_abi_refuses(bad):
     lib = _lib.load()
     d = desc(**bad)
-    assert lib.kvca_attend_step(ctypes.byref(d), 4096, 1 << 40, None, None) == _lib.KVCA_ERR_BAD_ARGUMENT
+    assert lib.kvca_attend_step(ctypes.byref(d), 4096, 1 << 40, 4096, None, None) == _lib.KVCA_ERR_BAD_ARGUMENT
     assert lib.kvca_attend_step_workspace_bytes(ctypes.byref(d)) == -1
 
 
@@ -41,17 +41,17 @@ def test_c_abi_refuses(bad):
                          ids=lambda b: ",".join(b))
 def test_c_abi_size_limits(big):
     lib = _lib.load()
-    assert lib.kvca_attend_step(ctypes.byref(desc(**big)), 4096, 1 << 40, None, None) == _lib.KVCA_ERR_SIZE_LIMIT
+    assert lib.kvca_attend_step(ctypes.byref(desc(**big)), 4096, 1 << 40, 4096, None, None) == _lib.KVCA_ERR_SIZE_LIMIT
 
 
 def test_c_abi_needs_its_pointers():
     lib = _lib.load()
     for missing in ("query", "out", "seq_lens", "key", "value", "block_tables"):
         d = desc(**{missing: 0 if missing in ("query", "out", "key", "value") else None})
-        assert lib.kvca_attend_step(ctypes.byref(d), 4096, 1 << 40, None, None) == _lib.KVCA_ERR_BAD_ARGUMENT
-    assert lib.kvca_attend_step(None, 4096, 1 << 40, None, None) == _lib.KVCA_ERR_BAD_ARGUMENT
+        assert lib.kvca_attend_step(ctypes.byref(d), 4096, 1 << 40, 4096, None, None) == _lib.KVCA_ERR_BAD_ARGUMENT
+    assert lib.kvca_attend_step(None, 4096, 1 << 40, 4096, None, None) == _lib.KVCA_ERR_BAD_ARGUMENT
     # nothing to do: succeeds without a device
-    assert lib.kvca_attend_step(ctypes.byref(desc(num_seqs=0)), None, 0, None, None) == _lib.KVCA_OK
+    assert lib.kvca_attend_step(ctypes.byref(desc(num_seqs=0)), None, 0, None, None, None) == _lib.KVCA_OK
 
 
 def test_python_refuses_cpu_tensors():
