@@ -107,10 +107,15 @@ def _stream(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+_no_switch = contextlib.nullcontext()
+
+
 def _on(device: torch.device):
     """The device's context for a launch (no switch when it is current)."""
-    if _index(device) == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if _index(device) == _current_device():
+        return _no_switch
     return torch.cuda.device(device)
 
 
@@ -1426,13 +1431,13 @@ _attend_workspace_bytes: dict[tuple, int] = {}
 _attend_counters: dict[tuple[int, int], torch.Tensor] = {}
 
 
-def _step_counters(dev: torch.device) -> torch.Tensor:
+def _step_counters(dev: torch.device, stream: int) -> torch.Tensor:
     """kvca_attend_step's counters of this (device, stream), zero between
     calls.  A call that is captured gets counters of its own, cleared by the
     graph, so that graphs captured on one stream may replay side by side."""
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         return torch.zeros(int(_lib_handle.kvca_attend_step_counters()), dtype=torch.int32, device=dev)
-    key = (_index(dev), _stream(dev).value or 0)
+    key = (_index(dev), stream)
     buf = _attend_counters.get(key)
     if buf is None:
         buf = torch.zeros(int(_lib_handle.kvca_attend_step_counters()), dtype=torch.int32, device=dev)
@@ -1445,7 +1450,10 @@ def _attend_rows(t: torch.Tensor, shape, name: str) -> list[int]:
     size = t.element_size()
     stride = t.stride()
     out = [x * size if n > 1 else 0 for n, x in zip(shape[:-1], stride)]
-    if t.data_ptr() % 16 or sum(x % 16 for x in out) or (stride[-1] != 1 and t.numel()):
+    bits = t.data_ptr()
+    for x in out:
+        bits |= x
+    if bits & 15 or (stride[-1] != 1 and t.numel()):
         raise ValueError(f"{name}: rows of head_dim must be contiguous and 16-byte aligned")
     return out
 
@@ -1454,10 +1462,10 @@ def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torc
                  block_tables: torch.Tensor, seq_lens: torch.Tensor, scale, window, sinks, key_scale, value_scale,
                  out, lse) -> tuple[_lib.AttendDesc, torch.Tensor]:
     """The checked arguments of an attention call and its output tensor."""
-    for t, name in ((query, "query"), (key_cache, "key_cache"), (value_cache, "value_cache"),
-                    (block_tables, "block_tables"), (seq_lens, "seq_lens")):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be torch.Tensor")
+    tensor = torch.Tensor
+    if not (isinstance(query, tensor) and isinstance(key_cache, tensor) and isinstance(value_cache, tensor)
+            and isinstance(block_tables, tensor) and isinstance(seq_lens, tensor)):
+        raise TypeError("query, key_cache, value_cache, block_tables and seq_lens must be torch.Tensor")
     dev = query.device
     if dev.type != "cuda":
         raise ValueError("query must be a CUDA tensor")
@@ -1560,9 +1568,9 @@ def attend_step(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
                 _raise_for(_lib.KVCA_ERR_BAD_ARGUMENT, 0, "attend_step")
             _attend_workspace_bytes[shape] = need
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        counters = _step_counters(dev)
-        rc = _lib_handle.kvca_attend_step(ctypes.byref(desc), workspace.data_ptr(), need, counters.data_ptr(),
-                                          _ptr(_status(dev)), _stream(dev))
+        stream = _stream(dev).value or 0
+        rc = _lib_handle.kvca_attend_step(ctypes.byref(desc), workspace.data_ptr(), need,
+                                          _step_counters(dev, stream).data_ptr(), _status(dev).data_ptr(), stream)
     _host_rc(rc, "attend_step")
     _maybe_check(dev, check, "attend_step")
     return out
