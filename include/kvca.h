@@ -1,7 +1,7 @@
 /*
  * kvca.h - C ABI of the B200 (sm_100a) paged-KV adapter hot path.
  *
- * Two families of entry points live behind this header:
+ * Four families of entry points live behind this header:
  *
  *   1. Slot metadata and the clock sweep over a packed slot_meta array.
  *      Each slot has one unsigned word holding a pin count (low half) and a
@@ -17,6 +17,11 @@
  *      (adapter.py:543, adapter.py:653-656, adapter.py:779-787) and the
  *      slot_mapping-driven single-layer KV transfer (adapter.py:1200-1243,
  *      adapter.py:1275-1285).
+ *
+ *   3. Pages of sequences (fork, free, compaction) over page tables and the
+ *      slot metadata.
+ *   4. Attention over the paged cache, one new token or a chunk of them per
+ *      sequence.  3 and 4 have no counterpart in the reference.
  *
  * Conventions
  *   - Every pointer named d_* is a device pointer on the current device.

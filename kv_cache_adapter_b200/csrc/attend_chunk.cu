@@ -24,8 +24,18 @@
 // by more than 2^8, so that most tiles leave it alone; a probability is then at
 // most 2^8.
 //
-// Bound by the tensor cores and the exponentials (16 per SM and clock) for
-// long chunks, by HBM for a few tokens.
+// Long chunks are bound by the chain scores, softmax, probabilities, product of
+// each row tile, with two tiles to overlap: 10,494 new tokens in 5 sequences
+// (32 query heads of 128, bf16) 940 us, 0.87 PFLOP/s, tensor cores 46 % active.
+// At head dim 64 by the softmax's instructions and exponentials (16 per SM and
+// clock): 16,167 tokens, window 1,024, e4m3, 270 us.  A few tokens by latency:
+// 24 sequences with 1-8 tokens over 27,000 keys 50 us (2.1 TB/s).
+//
+// The softmax reads its scores twice from tensor memory, in loops of 32
+// columns: held in registers in one pass (128 of them, unrolled) the prompts
+// took 929 us and the window 303.  Scores in halves of 64 keys, so that the
+// next half comes while a softmax runs, cost the tensor cores more than it
+// gave (1,108 us), as did an issuing warp per row tile (1,183).
 
 #include <cuda_runtime.h>
 #include <stdint.h>

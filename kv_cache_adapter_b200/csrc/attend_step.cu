@@ -15,6 +15,10 @@
 // segment's results joins them, in run order (a second kernel for that cost 6
 // us of 94 with 96 ragged sequences, and a launch).
 //
+// 96 ragged sequences of 37-8,191 tokens, 8 K/V heads of 128 in fp16 (495 MB):
+// 94 us, 5.3 TB/s, 80 % of the measured copy bandwidth; 256 sequences with a
+// window of 4,096 tokens in e4m3 (1.34 GB): 245 us, 5.5 TB/s.
+//
 // Both products run transposed on m16n8k16: S^T = K Q^T has the 16 tokens as
 // rows and up to 8 query heads that share the K/V head as columns, O^T = V^T
 // P^T the head dim as rows, so that 8 heads cost no padding and the transposed

@@ -6,7 +6,9 @@ packed-slot-meta extension API that adapter.py calls on its native branch
 adapter.py:316-330, :397-415, :437-454, :477-491, :557-593, :615-645).  The
 row movers replace the torch indexing the reference uses to move KV bytes
 (adapter.py:543, :653-656, :779-787) and its slot_mapping transfer
-(adapter.py:1200-1243, :1275-1285).
+(adapter.py:1200-1243, :1275-1285).  Beyond the reference: attention over the
+paged cache (``attend_step``, ``attend_chunk``) and the pages of sequences
+(``fork_sequences``, ``free_sequences``, ``compact_pages``).
 
 Every op launches on the current CUDA stream of its tensors' device.  Errors
 found on the device land in a per-device status word.  ``pop_reusable_slots``
