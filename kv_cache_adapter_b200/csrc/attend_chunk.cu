@@ -59,7 +59,7 @@ constexpr int kReaders = 15;    // warps that read them
 // output.  It counts when the tiles are dealt out, as tiles before the first.
 constexpr int kSegmentCost = 3;
 constexpr float kGrowth = 8.f;  // log2 of how far a maximum may lag
-constexpr uint32_t kWaitTries = 1u << 22;
+constexpr uint32_t kWaitTries = 1u << 24;  // a third of a second at least
 
 template <int DP>
 struct ChunkShape {

@@ -196,7 +196,11 @@ struct Cursor {
     if (++chunk < chunks) return;
     chunk = 0;
     do {
-      ++seq;
+      if (++seq >= a.num_seqs) {  // not while the lengths stay as they were counted
+        left = 0;
+        --seq;
+        return;
+      }
       load(a);
     } while (tiles == 0);
   }
@@ -298,7 +302,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       int64_t rest = begin - prefix[lo];
       at.seq = lo * per;
       at.load(a);
-      while (rest >= sequence_share(at.tiles, chunks)) {
+      while (rest >= sequence_share(at.tiles, chunks) && at.seq + 1 < a.num_seqs) {
         rest -= sequence_share(at.tiles, chunks);
         ++at.seq;
         at.load(a);
@@ -396,6 +400,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
         more = !ahead.last();
         if (more) {
           ahead.advance(a, chunks);
+          more = ahead.left > 0;
           look_up();
         }
       }
@@ -676,6 +681,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       }
       if (go) {
         at.advance(a, chunks);
+        go = at.left > 0;
         starts = true;
         fresh = true;
       }

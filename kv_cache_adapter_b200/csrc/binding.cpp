@@ -138,6 +138,8 @@ int to_attend(const kvca_attend_desc* d, int64_t* d_status, kvca::AttendArgs* a)
   a->query_type = d->query_type;
   a->cache_type = d->cache_type;
   a->status = d_status;
+  // without blocks no row is read, but rows that are not read get an address
+  if (d->num_blocks == 0) a->key = a->value = static_cast<const char*>(a->query);
   return KVCA_OK;
 }
 

@@ -184,6 +184,44 @@ def test_calls_on_two_streams():
         assert ((c.cpu().double() - cwant).abs() <= cbound).all()
 
 
+def test_pages_past_four_gigabytes():
+    """Attention, a fork and a compaction over pages whose byte offsets need more than 32 bits."""
+    from kv_cache_adapter_b200 import kv_cache_adapter_cuda as ops
+
+    dev = torch.device("cuda", 0)
+    slots = 1_100_000  # 4.5 GB per plane
+    kv = torch.zeros((2, slots, 16, 1, 128), dtype=torch.float16, device=dev)
+    pages = [slots - 1, 5, slots - 3, 1_060_000]
+    g = torch.Generator(device=dev).manual_seed(4)
+    for p in range(2):
+        kv[p, pages] = torch.randn((4, 16, 1, 128), generator=g, device=dev).half()
+    tables = torch.full((2, 4), -1, dtype=torch.int64, device=dev)
+    tables[0] = torch.tensor(pages, device=dev)
+    lens = torch.tensor([60, 0], device=dev)
+    q = torch.randn((2, 2, 128), generator=g, device=dev).half()
+    rows = kv[:, tables[0]].flatten(1, 2)[:, :60, 0].double()
+    weight = torch.softmax(q[0].double() @ rows[0].T / 128 ** 0.5, -1)
+    want, share = weight @ rows[1], weight @ rows[1].abs()
+    bound = 2.0 ** -10 * share + 2.0 ** -11 * want.abs()  # probabilities and score sums, the result's rounding
+    step = ops.attend_step(q, kv[0], kv[1], tables, lens, check=True)
+    assert ((step[0].double() - want).abs() <= bound).all() and (step[1] == 0).all()
+    chunk = ops.attend_chunk(q[:1].contiguous(), torch.tensor([0, 1, 1], device=dev), kv[0], kv[1], tables, lens,
+                             check=True)
+    assert ((chunk[0].double() - want).abs() <= bound).all()
+    meta = torch.zeros(slots, dtype=torch.uint8, device=dev)
+    l2p, p2l = (torch.full((n,), -1, dtype=torch.int64, device=dev) for n in (100, slots))
+    held = torch.tensor(pages, device=dev)
+    meta[held], p2l[held], l2p[:4] = 0x11, torch.arange(4, device=dev), held
+    pool, one = (meta, l2p, p2l, tables, lens), torch.zeros(1, dtype=torch.int64, device=dev)
+    ops.fork_sequences(*pool, one, one + 1, one + slots - 2, one + 50, [kv[0], kv[1]], check=True)
+    both = ops.attend_step(q[:1].repeat(2, 1, 1), kv[0], kv[1], tables, lens, check=True)
+    assert torch.equal(both[0], step[0]) and torch.equal(both[1], step[0])
+    _, live = ops.compact_pages(*pool, [kv[0], kv[1]], check=True)
+    assert live.item() == 5 and int(tables.max()) == 4
+    both = ops.attend_step(q[:1].repeat(2, 1, 1), kv[0], kv[1], tables, lens, check=True)
+    assert torch.equal(both[0], step[0]) and torch.equal(both[1], step[0])
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_on_a_device_that_is_not_current():
     from kv_cache_adapter_b200 import kv_cache_adapter_cuda as ops
