@@ -1291,14 +1291,21 @@ def move_cycle(token_caches, slot_mapping: torch.Tensor, token_rows: torch.Tenso
 # ---------------------------------------------------------------------------
 
 
+def _ids(t: torch.Tensor, dev: torch.device, name: str) -> None:
+    """_require_index with one test where all is well: a call on pages checks seven of these."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.int64 and t.dim() == 1 and t.device == dev
+            and t.is_contiguous()):
+        _require_index(t, dev, name)
+
+
 def _page_pool(slot_meta, logical_to_physical, physical_to_logical, block_tables, seq_lens,
                block_size: int) -> _lib.PagePool:
     """The checked slot pool and page tables of an operator on sequences' pages."""
     _require(slot_meta, _META_DTYPES, "slot_meta")
     dev = slot_meta.device
-    for t, name in ((logical_to_physical, "logical_to_physical"), (physical_to_logical, "physical_to_logical"),
-                    (seq_lens, "seq_lens")):
-        _require_index(t, dev, name)
+    _ids(logical_to_physical, dev, "logical_to_physical")
+    _ids(physical_to_logical, dev, "physical_to_logical")
+    _ids(seq_lens, dev, "seq_lens")
     if physical_to_logical.numel() != slot_meta.numel():
         raise ValueError("physical_to_logical needs one entry per slot")
     if not isinstance(block_tables, torch.Tensor):
@@ -1347,11 +1354,11 @@ def fork_sequences(slot_meta: torch.Tensor, logical_to_physical: torch.Tensor, p
     pl = _page_caches(caches, slot_meta)
     pool = _page_pool(slot_meta, logical_to_physical, physical_to_logical, block_tables, seq_lens, pl.block_size)
     dev = slot_meta.device
-    count = parents.numel()
+    count = parents.numel() if isinstance(parents, torch.Tensor) else 0
     for t, name in ((parents, "parents"), (children, "children"), (fresh_slots, "fresh_slots"),
                     (fresh_ids, "fresh_ids")):
-        _require_index(t, dev, name)
-        if t.numel() != count:
+        _ids(t, dev, name)
+        if t.shape[0] != count:
             raise ValueError("parents, children, fresh_slots and fresh_ids must have the same length")
     if count == 0:
         return
@@ -1376,7 +1383,7 @@ def free_sequences(slot_meta: torch.Tensor, logical_to_physical: torch.Tensor, p
     checked first: an error leaves all as it was."""
     pool = _page_pool(slot_meta, logical_to_physical, physical_to_logical, block_tables, seq_lens, int(block_size))
     dev = slot_meta.device
-    _require_index(sequences, dev, "sequences")
+    _ids(sequences, dev, "sequences")
     count = sequences.numel()
     if count == 0:
         return
