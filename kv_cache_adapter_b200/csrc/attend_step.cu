@@ -61,6 +61,11 @@ struct StepShape {
   static constexpr int kHeads = 8 * NG;
   static constexpr int kAcc = DP * kHeads;  // floats of a partial output
   static constexpr int kSmem = kWarps * kStages * kStageBytes;
+  // Weights of the values and their sum are held times 2^kShift of the running
+  // maximum's own: fp16 ones then keep 11 bits to 2^-29 of the largest and some
+  // to 2^-39 (to 2^-14 and 2^-24 without, where 2,000 tokens at 2^-26 of a
+  // first one were lost); the largest, 2^15, is within fp16's range.
+  static constexpr float kShift = Cache::kBf16 ? 0.f : 15.f;
 };
 
 // Shared memory address of 16-byte chunk c of row r: chunks are permuted
@@ -534,8 +539,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
           decay[n][j] = exp2_approx(m[n][j] - base);
           grew |= next != m[n][j];
           m[n][j] = next;
-          x[j] = exp2_approx(x[j] - base);
-          x[j + 2] = exp2_approx(x[j + 2] - base);
+          x[j] = exp2_approx(x[j] - (base - Shape::kShift));
+          x[j + 2] = exp2_approx(x[j + 2] - (base - Shape::kShift));
           l[n][j] = l[n][j] * decay[n][j] + (x[j] + x[j + 2]);
         }
         const uint32_t top = pack2<kBf16>(x[0], x[1]), bottom = pack2<kBf16>(x[2], x[3]);
@@ -649,7 +654,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const int hh = first + n * 8 + 2 * lane + j;
-              if (hh < a.group) a.lse[row + hh] = m[n][j] * kLn2 + logf(l[n][j]);
+              if (hh < a.group) a.lse[row + hh] = (m[n][j] - Shape::kShift) * kLn2 + logf(l[n][j]);
             }
           }
         }
@@ -829,7 +834,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       const float factor = a.value_scale / l2;
       *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (row + h) * a.dim + d) =
           a.query_type == KVCA_TYPE_BF16 ? pack2<true>(x * factor, y * factor) : pack2<false>(x * factor, y * factor);
-      if (a.lse != nullptr && d == 0) a.lse[row + h] = base * kLn2 + logf(l2);
+      if (a.lse != nullptr && d == 0) a.lse[row + h] = (base - Shape::kShift) * kLn2 + logf(l2);
     }
   };
   auto park = [&]() {

@@ -1,0 +1,82 @@
+"""attend_step and attend_chunk where single values decide: weights far
+below the largest."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import attend_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16, E4M3 = torch.float16, torch.bfloat16, torch.float8_e4m3fn
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from kv_cache_adapter_b200 import kv_cache_adapter_cuda
+
+    return kv_cache_adapter_cuda
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return torch.device("cuda", 0)
+
+
+def place(b, s, t):
+    """Page and offset of token t of sequence s."""
+    block = b.key.shape[1]
+    return b.tables[s, t // block], t % block
+
+
+def offsets_of(b, dev):
+    return torch.tensor([0] + b.new, device=dev).cumsum(0)
+
+
+def attend(ops, dev, b, which, **kw):
+    key, value = b.on(dev)
+    query, tables, lens = b.query.to(dev), b.tables.to(dev), torch.tensor(b.lens, device=dev)
+    lse = torch.empty(query.shape[:2], device=dev)
+    kw = dict(window=b.window, sinks=b.sinks, lse=lse, check=True, **b.scales, **kw)
+    if which == "step":
+        out = ops.attend_step(query, key, value, tables, lens, **kw)
+    else:
+        out = ops.attend_chunk(query, offsets_of(b, dev), key, value, tables, lens, **kw)
+    return out.cpu().double(), lse.cpu().double()
+
+
+def weak_batch(dtype, cache, sequences, tokens, new, heads, log2_gap):
+    """Per sequence one strong token (the first; its values are 0) and weak ones 2^-log2_gap of its weight (values 1).
+    Returns the batch, the scale and the exact result."""
+    dim, block = 64, 16
+    b = oracle.Batch(lens=[tokens] * sequences, new=[new] * sequences, heads=heads, group=1, dim=dim, block=block,
+                     dtype=dtype, cache=cache, seed=2)
+    b.scales = {}
+    zero = torch.zeros((), dtype=b.key.dtype)
+    b.key[:] = zero
+    b.value[:] = torch.ones((), dtype=torch.float32).to(b.key.dtype)
+    for s in range(sequences):
+        page, off = place(b, s, 0)
+        b.key[page, off, :, 0] = torch.tensor(16.0).to(b.key.dtype)
+        b.value[page, off] = zero
+    b.query = torch.zeros_like(b.query)
+    b.query[:, :, 0] = 1.0
+    return b, log2_gap * math.log(2.0) / 16.0
+
+
+@pytest.mark.parametrize("dtype,cache", [(F16, F16), (BF16, BF16), (F16, E4M3), (BF16, E4M3)])
+def test_step_keeps_weights_far_below_the_largest(ops, dev, dtype, cache):
+    """2,000 tokens at 2^-26.3 of the first one's weight are all of the result."""
+    b, scale = weak_batch(dtype, cache, sequences=40, tokens=2000, new=1, heads=8, log2_gap=26.3)
+    out, lse = attend(ops, dev, b, "step", scale=scale)
+    w = 2.0 ** -26.3
+    want = 1999 * w / (1 + 1999 * w)
+    # a weight to 2^-11 and the exponent's argument (26.3 in fp32, 2^-20), the result to its type's half step (fp16: of
+    # a subnormal, 2^-25)
+    eps = torch.finfo(dtype).eps / 2
+    tol = want * (2.0 ** -11 + 2.0 ** -18 + eps) + (2.0 ** -25 if dtype == F16 else 0)
+    assert ((out - want).abs() <= tol).all(), (out.min(), out.max(), want)
+    assert ((lse - (26.3 * math.log(2.0) + math.log1p(1999 * w))).abs() <= 2.0 ** -17).all()
