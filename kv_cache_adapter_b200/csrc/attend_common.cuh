@@ -42,6 +42,18 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// The larger of two; NaN when either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// Two floats cut off to bf16, in one register, the first in the low half.
+__device__ __forceinline__ uint32_t high_halves(float lo, float hi) {
+  return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+}
+
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }

@@ -66,6 +66,12 @@ struct StepShape {
   // to 2^-39 (to 2^-14 and 2^-24 without, where 2,000 tokens at 2^-26 of a
   // first one were lost); the largest, 2^15, is within fp16's range.
   static constexpr float kShift = Cache::kBf16 ? 0.f : 15.f;
+  // An infinite value at a token that the query sees is the result, however
+  // small its weight: a visible token's weight is never 0 (0 x inf is NaN),
+  // nor is that of a partial result.  The least of fp16 (2^-39 of the largest)
+  // and of bf16 move no sum.  e4m3 has no infinities.
+  static constexpr bool kInfinities = Cache::kBytes == 2;
+  static constexpr float kLeast = Cache::kBf16 ? 0x1p-126f : 0x1p-24f;
 };
 
 // Shared memory address of 16-byte chunk c of row r: chunks are permuted
@@ -293,6 +299,17 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
 
   float acc[NG][kSteps][4];
   float m[NG][2], l[NG][2];  // of the heads 2 * (lane % 4), + 1 of each tile of 8
+  // Weight of a token of score s, and of sums whose maximum is `behind` (<= 0) the whole's.
+  auto token_weight = [](float s, float base) {
+    const float w = exp2_approx(s - (base - Shape::kShift));
+    if constexpr (!Shape::kInfinities) return w;
+    return s == -INFINITY ? 0.f : max_nan(w, Shape::kLeast);
+  };
+  auto partial_weight = [](float behind) {
+    const float w = exp2_approx(behind);
+    if constexpr (!Shape::kInfinities) return w;
+    return max_nan(w, 0x1p-126f);
+  };
 
   if (my_run < runs) {
     const int64_t begin = run_begin(tiles, runs, my_run), finish = run_begin(tiles, runs, my_run + 1);
@@ -536,22 +553,28 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
           const float next = fmaxf(m[n][j], top);
           const float base = next == -INFINITY ? 0.f : next;
-          decay[n][j] = exp2_approx(m[n][j] - base);
+          decay[n][j] = partial_weight(m[n][j] - base);
           grew |= next != m[n][j];
           m[n][j] = next;
-          x[j] = exp2_approx(x[j] - (base - Shape::kShift));
-          x[j + 2] = exp2_approx(x[j + 2] - (base - Shape::kShift));
+          x[j] = token_weight(x[j], base);
+          x[j + 2] = token_weight(x[j + 2], base);
           l[n][j] = l[n][j] * decay[n][j] + (x[j] + x[j + 2]);
         }
-        const uint32_t top = pack2<kBf16>(x[0], x[1]), bottom = pack2<kBf16>(x[2], x[3]);
-        p[n][0] = transpose8x8(top);
-        p[n][1] = transpose8x8(bottom);
         if constexpr (kBf16) {
           // bf16 would leave 8 bits of a probability: the remainder goes in
-          // as a second product (the tensor cores idle here anyway)
+          // as a second product (the tensor cores idle here anyway), to 2^-15
+          // in all.  The first term is cut off, so that the remainder is not
+          // negative, and like it never 0 (inf - inf, 0 x inf).
+          const uint32_t top = high_halves(x[0], x[1]), bottom = high_halves(x[2], x[3]);
           const float2 t = unpack2<true>(top), b = unpack2<true>(bottom);
-          p_low[n][0] = transpose8x8(pack2<true>(x[0] - t.x, x[1] - t.y));
-          p_low[n][1] = transpose8x8(pack2<true>(x[2] - b.x, x[3] - b.y));
+          p[n][0] = transpose8x8(top);
+          p[n][1] = transpose8x8(bottom);
+          p_low[n][0] = transpose8x8(pack2<true>(max_nan(x[0] - t.x, Shape::kLeast), max_nan(x[1] - t.y, Shape::kLeast)));
+          p_low[n][1] = transpose8x8(pack2<true>(max_nan(x[2] - b.x, Shape::kLeast), max_nan(x[3] - b.y, Shape::kLeast)));
+        } else {
+          // fp16: 2^-11, no more than the result's own rounding
+          p[n][0] = transpose8x8(pack2<false>(x[0], x[1]));
+          p[n][1] = transpose8x8(pack2<false>(x[2], x[3]));
         }
       }
       if (__any_sync(0xffffffffu, grew)) {
@@ -745,7 +768,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       const float base = top == -INFINITY ? 0.f : top;
       float sum = 0.f, total = 0.f;
       for (int k = w; k < end; k += span) {
-        const float weight = exp2_approx(held_ml[k][h] - base);
+        const float weight = partial_weight(held_ml[k][h] - base);
         sum += weight * parked[k * Shape::kAcc + i];
         total += weight * held_ml[k][kHeads + h];
       }
@@ -765,10 +788,10 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
   constexpr int kWarpResults = 8;
   const int h4 = lane * 4 % kHeads;         // a lane's four heads
   float4 top, total, sum[kVecs];
-  auto fold = [](float& old, float next, float& keep, float& weight) {
+  auto fold = [&](float& old, float next, float& keep, float& weight) {
     const float best = fmaxf(old, next), base = best == -INFINITY ? 0.f : best;
-    keep = exp2_approx(old - base);
-    weight = exp2_approx(next - base);
+    keep = partial_weight(old - base);
+    weight = partial_weight(next - base);
     old = best;
   };
   const int groups_of = layout.groups;
@@ -826,7 +849,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       float x = 0.f, y = 0.f, l2 = 0.f;
 #pragma unroll 1
       for (int w = from; w < to; ++w) {
-        const float weight = exp2_approx(held_ml[w][h] - base);
+        const float weight = partial_weight(held_ml[w][h] - base);
         x += weight * parked[w * Shape::kAcc + d * kHeads + h];
         y += weight * parked[w * Shape::kAcc + (d + 1) * kHeads + h];
         l2 += weight * held_ml[w][kHeads + h];

@@ -1,5 +1,5 @@
-"""attend_step and attend_chunk where single values decide: weights far
-below the largest."""
+"""attend_step and attend_chunk where single values decide: infinities and NaN
+at visible tokens, weights far below the largest."""
 from __future__ import annotations
 
 import math
@@ -48,9 +48,60 @@ def attend(ops, dev, b, which, **kw):
     return out.cpu().double(), lse.cpu().double()
 
 
+def agree(got, want, bound):
+    """The same infinities and NaN, and every finite value within its bound."""
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.isinf(got), torch.isinf(want))
+    inf = torch.isinf(want)
+    assert torch.equal(got[inf], want[inf])
+    finite = torch.isfinite(want)
+    err = (got - want).abs()[finite]
+    assert (err <= bound[finite]).all(), (err / bound[finite]).max()
+
+
+def plant(b, dims):
+    """dims: (sequence, token, K/V head, dim, value) each."""
+    for s, t, head, d, x in dims:
+        page, off = place(b, s, t)
+        b.value[page, off, head, d] = x
+
+
+INF, NAN = math.inf, math.nan
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_step_of_one_infinite_token(ops, dev, dtype):
+    b = oracle.Batch(lens=[1, 1], heads=1, group=2, dim=64, block=16, dtype=dtype, seed=1)
+    plant(b, [(0, 0, 0, d, INF if d % 2 else -INF) for d in range(64)])
+    out, _ = attend(ops, dev, b, "step")
+    assert (out[0, :, 1::2] == INF).all() and (out[0, :, ::2] == -INF).all() and torch.isfinite(out[1]).all()
+
+
+# magnitude 1: weights of one size; 12: weights to 2^-100 of the largest and less
+@pytest.mark.parametrize("magnitude", [1.0, 12.0])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_step_with_infinite_values_at_visible_tokens(ops, dev, dtype, dim, magnitude):
+    # one sequence over many runs of warps, and short ones within one
+    b = oracle.Batch(lens=[3000, 40, 17, 500], heads=2, group=3, dim=dim, block=16, dtype=dtype, seed=dim,
+                     magnitude=magnitude)
+    marks = []
+    for s, n in enumerate(b.lens):
+        for i in range(0, dim, 5):
+            marks.append((s, (i * 37) % n, i % 2, i, INF))
+            marks.append((s, (i * 53 + 1) % n, i % 2, (i + 1) % dim, -INF))
+        marks += [(s, 3, 0, 2, INF), (s, n - 1, 0, 2, -INF)]  # both: NaN
+        marks += [(s, n // 2, 1, 3, NAN)]
+    plant(b, marks)
+    out, lse = attend(ops, dev, b, "step")
+    _, (want, want_lse, bound, lse_bound) = b.expect(2.0 ** -11)
+    agree(out, want, bound)
+    assert ((lse - want_lse).abs() <= lse_bound).all()
+
+
 def weak_batch(dtype, cache, sequences, tokens, new, heads, log2_gap):
     """Per sequence one strong token (the first; its values are 0) and weak ones 2^-log2_gap of its weight (values 1).
-    Returns the batch, the scale and the exact result."""
+    Returns the batch and the scale."""
     dim, block = 64, 16
     b = oracle.Batch(lens=[tokens] * sequences, new=[new] * sequences, heads=heads, group=1, dim=dim, block=block,
                      dtype=dtype, cache=cache, seed=2)
