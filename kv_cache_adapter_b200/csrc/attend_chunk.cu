@@ -59,6 +59,12 @@ constexpr int kReaders = 15;    // warps that read them
 // output.  It counts when the tiles are dealt out, as tiles before the first.
 constexpr int kSegmentCost = 3;
 constexpr float kGrowth = 8.f;  // log2 of how far a maximum may lag
+// Probabilities, and their sum, are held times 2^7 where they are fp16 (the
+// largest, 2^15, is within its range): those of 2^-21 of the maximum keep 11
+// bits, those of 2^-31 some (2^-14 and 2^-24 without: 2,000 tokens at 2^-26 of a
+// first one were lost).  bf16 has fp32's exponents.
+template <typename Cache>
+constexpr float kShift = Cache::kBf16 ? 0.f : 7.f;
 constexpr uint32_t kWaitTries = 1u << 24;  // a third of a second at least
 
 template <int DP>
@@ -456,7 +462,7 @@ __device__ __forceinline__ void row_again(const AttendArgs& a, const ChunkArgs& 
       dot += (bf16 ? unpack2<true>(q[d]).x : unpack2<false>(q[d]).x) * element(k, d);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    const float w = exp2_approx(dot * unit - base);
+    const float w = exp2_approx(dot * unit - base + kShift<Cache>);
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (lane + 32 * j < a.dim) acc[j] += w * element(x, lane + 32 * j);
@@ -987,7 +993,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float base = m == -INFINITY ? 0.f : m * unit;
             const float decay = m != old ? exp2_approx(old * unit - base) : 1.f;
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-            const float2 units = make_float2(unit, unit), bases = make_float2(-base, -base);
+            const float low = kShift<Cache> - base;
+            const float2 units = make_float2(unit, unit), bases = make_float2(low, low);
             auto weigh = [&](const float (&x)[32], int j) {
               uint32_t packed[16];
 #pragma unroll
@@ -1075,7 +1082,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (live) {
             if (whole) {
-              if (a.lse != nullptr) a.lse[out_row] = base * kLn2 + logf(l);
+              if (a.lse != nullptr) a.lse[out_row] = (base - kShift<Cache>) * kLn2 + logf(l);
             } else {
               float* const ml = ws.ml + slot * 2 * kRows;
               ml[r] = m == -INFINITY ? -INFINITY : base;
@@ -1187,7 +1194,7 @@ __global__ void __launch_bounds__(kJoinThreads) attend_chunk_join_kernel(const _
     w.y = bf16 ? pack2<true>(sum[v].z * factor, sum[v].w * factor) : pack2<false>(sum[v].z * factor, sum[v].w * factor);
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + out_row * a.dim + d) = w;
   }
-  if (a.lse != nullptr && t == 0) a.lse[out_row] = base * kLn2 + logf(total);
+  if (a.lse != nullptr && t == 0) a.lse[out_row] = (base - c.shift) * kLn2 + logf(total);
 }
 
 template <typename Cache, int DP>
@@ -1238,6 +1245,7 @@ cudaError_t launch_attend_chunk(const AttendArgs& args, const int64_t* offsets, 
   c.scale_log2 = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
   c.query_and = a.scale_log2 == 0.f ? 0u : 0xffffffffu;
   c.query_xor = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+  c.shift = a.cache_type == KVCA_TYPE_BF16 ? kShift<CacheBf16> : kShift<CacheF16>;
   switch (a.cache_type) {
     case KVCA_TYPE_F16: return launch_cache<CacheF16>(a, c, workspace, sms, stream);
     case KVCA_TYPE_BF16: return launch_cache<CacheBf16>(a, c, workspace, sms, stream);

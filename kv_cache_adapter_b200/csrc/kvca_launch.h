@@ -154,6 +154,7 @@ struct ChunkArgs {
   int max_blocks;          // blocks that the offsets can make of them
   float scale_log2;
   uint32_t query_and, query_xor;
+  float shift;  // log2 of the factor in partial sums
 };
 
 size_t attend_step_workspace(const AttendArgs& args, int sms);

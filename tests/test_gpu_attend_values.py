@@ -99,10 +99,10 @@ def test_step_with_infinite_values_at_visible_tokens(ops, dev, dtype, dim, magni
     assert ((lse - want_lse).abs() <= lse_bound).all()
 
 
-def weak_batch(dtype, cache, sequences, tokens, new, heads, log2_gap):
+def weak_batch(dtype, cache, sequences, tokens, new, heads, log2_gap, dim=64):
     """Per sequence one strong token (the first; its values are 0) and weak ones 2^-log2_gap of its weight (values 1).
     Returns the batch and the scale."""
-    dim, block = 64, 16
+    block = 16
     b = oracle.Batch(lens=[tokens] * sequences, new=[new] * sequences, heads=heads, group=1, dim=dim, block=block,
                      dtype=dtype, cache=cache, seed=2)
     b.scales = {}
@@ -131,3 +131,21 @@ def test_step_keeps_weights_far_below_the_largest(ops, dev, dtype, cache):
     tol = want * (2.0 ** -11 + 2.0 ** -18 + eps) + (2.0 ** -25 if dtype == F16 else 0)
     assert ((out - want).abs() <= tol).all(), (out.min(), out.max(), want)
     assert ((lse - (26.3 * math.log(2.0) + math.log1p(1999 * w))).abs() <= 2.0 ** -17).all()
+
+
+@pytest.mark.parametrize("dtype,cache", [(F16, F16), (BF16, BF16), (F16, E4M3), (BF16, E4M3)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_chunk_keeps_weights_far_below_the_largest(ops, dev, dtype, cache, dim):
+    b, scale = weak_batch(dtype, cache, sequences=24, tokens=2000, new=8, heads=8, log2_gap=26.3, dim=dim)
+    out, lse = attend(ops, dev, b, "chunk", scale=scale)
+    w = 2.0 ** -26.3
+    weak = torch.arange(1992, 2000, dtype=torch.float64).repeat(24).view(-1, 1)  # a row sees the first token and these
+    want = (weak * w / (1 + weak * w)).unsqueeze(-1)
+    # a weight to 2^-11 (bf16 2^-8) or, as an fp16 subnormal, to 2^-32 of the largest; the rest as for one token
+    p_eps = 2.0 ** -8 if cache == BF16 else 2.0 ** -11
+    steps = 0 if cache == BF16 else 2.0 ** -32
+    tol = want * (p_eps + 2.0 ** -18 + torch.finfo(dtype).eps / 2) + weak.unsqueeze(-1) * steps
+    if dtype == F16:
+        tol = tol + 2.0 ** -25
+    assert ((out - want).abs() <= tol).all(), (out.min(), out.max(), want)
+    assert ((lse - (26.3 * math.log(2.0) + torch.log1p(weak * w))).abs() <= 2.0 ** -17).all()
