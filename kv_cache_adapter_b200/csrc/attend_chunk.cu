@@ -55,6 +55,7 @@ constexpr int kJoinThreads = 256;
 constexpr int kJoinRows = 16;   // rows per block of the join
 constexpr int kSlots = 4;       // segments announced ahead
 constexpr int kReaders = 15;    // warps that read them
+static_assert(kSlots == 4, "marks of tiles in flight hold a slot in two bits");
 // What a segment costs beside its tiles, in tiles: queries, first loads, the
 // output.  It counts when the tiles are dealt out, as tiles before the first.
 constexpr int kSegmentCost = 3;
@@ -385,8 +386,14 @@ struct Share {
   int tiles;       // of the segment
   int last_cta;    // that has the segment's last tile
   BlockView view;
+  int seen_last;   // keys up to here, and
+  int seen_low;    // those behind here or among the sinks, are seen by every row
   int64_t out_row;  // the chunk's first row of query and out
 
+  // Whether a row of the block does not see a key of the tile at v0.
+  __device__ __forceinline__ bool cut(int v0, int sinks) const {
+    return v0 + kKeys - 1 > seen_last || (v0 + kKeys > sinks && max(v0, sinks) <= seen_low);
+  }
   __device__ __forceinline__ int row_tiles() const { return view.rows > 128 ? 2 : 1; }
 
   // The tiles of (block, head) that are this CTA's, none perhaps.
@@ -401,6 +408,8 @@ struct Share {
     const int tokens = static_cast<int>(__ldg(c.offsets + b.seq + 1) - out_row);
     view = view_of(a, b.seq, b.row, b.rows, tokens, sequence_length(a, b.seq));
     tiles = b.tiles;
+    seen_last = view.context + view.row / a.group - view.skip;
+    seen_low = a.window > 0 ? view.context + (view.row + view.rows - 1) / a.group - a.window - view.skip : -1;
   }
   // To the next segment with tiles of this CTA; without one, end == tile.
   __device__ __forceinline__ void next(const AttendArgs& a, const ChunkArgs& c, const ChunkWorkspace& ws) {
@@ -423,52 +432,187 @@ struct Share {
   }
 };
 
-// A row whose output is not finite although its sum is: the tensor cores
-// multiplied a key that another row of the block sees, with an infinity or NaN
-// among its values, by this row's zero.  The warp sums the row again over the
-// keys that it sees alone.
-template <typename Cache>
-__device__ __forceinline__ void row_again(const AttendArgs& a, const ChunkArgs& c, const Share& s, int row, float base,
-                                       float unit, float* sum) {
-  const int lane = threadIdx.x & 31;
-  const int token = row / a.group, head = s.head * a.group + row % a.group;
-  const int p = s.view.context + token;
-  const uint16_t* q = static_cast<const uint16_t*>(a.query) + (s.out_row + token) * a.query_row + head * a.query_head;
-  const int v_last = p - s.view.skip;
-  const int v_low = a.window > 0 ? p - a.window - s.view.skip : -1;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  const bool bf16 = a.query_type == KVCA_TYPE_BF16;
-  const int v_end = min(s.view.count, s.end * kKeys);
-#pragma unroll 1
-  for (int v = s.tile * kKeys; v < v_end; ++v) {
-    if (v > v_last || (v >= a.sinks && v <= v_low)) continue;
-    const int key = s.view.key(v);
-    const int block = key / a.block_size;
-    const int64_t page = __ldg(a.tables + static_cast<int64_t>(s.view.seq) * a.table_stride + block);
-    if (page < 0 || page >= a.num_blocks) continue;
-    const int offset = key - block * a.block_size;
-    const char* k = a.key + page * a.key_block + offset * a.key_token + s.head * a.key_head;
-    const char* x = a.value + page * a.value_block + offset * a.value_token + s.head * a.value_head;
-    auto element = [&](const char* base_ptr, int d) {
-      if constexpr (Cache::kBytes == 1) {
-        return unpack2<false>(e4m3_to_f16x2(reinterpret_cast<const uint8_t*>(base_ptr)[d])).x;
-      } else {
-        return unpack2<Cache::kBf16>(reinterpret_cast<const uint16_t*>(base_ptr)[d]).x;
-      }
-    };
-    float dot = 0.f;
-#pragma unroll 1
-    for (int d = lane; d < a.dim; d += 32)
-      dot += (bf16 ? unpack2<true>(q[d]).x : unpack2<false>(q[d]).x) * element(k, d);
+// ---------------------------------------------------------------------------
+// Infinite and NaN values
+// ---------------------------------------------------------------------------
+//
+// The tensor cores multiply every value of a tile by every row's probability,
+// and 0 times an infinity or a NaN is NaN.  So the values of a tile that is cut
+// (a row of the block does not see one of its keys) go in with 0 in their
+// places, noted per segment, and are added to the rows that see them at the
+// end.  Any other tile is seen by all rows alike: there a row's output shows
+// them, and what they make of it is found from the values alone.  Neither takes
+// a second product; a segment without such values pays one look at the values
+// of its cut tiles.
+
+template <bool kBf16>
+__device__ __forceinline__ bool is_finite16(uint32_t half) {
+  constexpr uint32_t kExponent = kBf16 ? 0x7f80u : 0x7c00u;
+  return (half & kExponent) != kExponent;
+}
+
+// Where 16-byte chunk `ch` of row r of a tile lies.
+__device__ __forceinline__ uint32_t place(int r, int ch) {
+  return static_cast<uint32_t>((ch >> 3) * (kKeys * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+}
+
+// Zeros for the infinite and NaN values among the chunks of 32 rows of a tile
+// that this lane copied (chunk lane % kRowChunks of every kPerInstr-th row);
+// whether this lane found one.
+template <bool kBf16, int DP>
+__device__ __noinline__ bool drop_non_finite(unsigned char* tile, int first_row, int row_chunks) {
+  constexpr int kRowChunks = DP / 8, kPerInstr = 32 / kRowChunks;
+  const int lane = threadIdx.x & 31, chunk = lane % kRowChunks, sub = lane / kRowChunks;
+  if (chunk >= row_chunks) return false;
+  uint32_t sum = 0;  // of the values times 0: NaN with one that is not finite
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    const float w = exp2_approx(dot * unit - base + kShift<Cache>);
+  for (int i = 0; i < 32 / kPerInstr; ++i) {
+    const uint4 x = *reinterpret_cast<const uint4*>(tile + place(first_row + i * kPerInstr + sub, chunk));
+    const uint32_t word[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (kBf16)
+        asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(word[j]), "r"(0u));
+      else
+        asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(sum) : "r"(word[j]), "r"(0u));
+    }
+  }
+  if ((sum & 0x7fff7fffu) == 0) return false;
+#pragma unroll 1
+  for (int i = 0; i < 32 / kPerInstr; ++i) {
+    uint32_t* const word = reinterpret_cast<uint32_t*>(tile + place(first_row + i * kPerInstr + sub, chunk));
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (lane + 32 * j < a.dim) acc[j] += w * element(x, lane + 32 * j);
+      word[j] &= (is_finite16<kBf16>(word[j]) ? 0xffffu : 0u) | (is_finite16<kBf16>(word[j] >> 16) ? 0xffff0000u : 0u);
   }
+  return true;
+}
+
+// The same for four e4m3 values, which have NaN only (all bits but the sign).
+__device__ __forceinline__ uint32_t drop_nan4(uint32_t word, uint32_t* found) {
+  const uint32_t tops = ((word & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+  *found |= tops;
+  return word & ~((tops >> 7) * 255u);
+}
+
+// Puts the infinite and NaN values of a segment's tiles into the outputs of a
+// softmax warp's rows, one per lane: `out` (16 bits, a whole segment) or `part`
+// (fp32, a share of one).  Of uncut tiles (`uncut`) they take an output's
+// place, of cut ones (`cut`) they are added for rows that see the key (`mine`:
+// the lane has a row, and its sum is a number).  A key that is not finite
+// itself has a score of NaN or an infinity: then the row is NaN already, or the
+// value's weight is 0 and its product NaN.
+template <typename Cache, int DP>
+__device__ __noinline__ void put_non_finite(const AttendArgs& a, const Share& s, bool uncut, bool cut, bool mine,
+                                            int v_last, int v_low, uint16_t* out, float* part) {
+  constexpr int kOwn = DP / 32;  // a lane's values of a row
+  constexpr int kBatch = 8;
+  const int lane = threadIdx.x & 31;
+  const bool has = lane * kOwn < a.dim;
+  const bool bf16 = a.query_type == KVCA_TYPE_BF16;
+  auto own_of = [&](unsigned long long row, float (&x)[kOwn]) {
+    const char* const p = reinterpret_cast<const char*>(row) + lane * kOwn * Cache::kBytes;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) sum[j] = acc[j];
+    for (int e = 0; e < kOwn; ++e) {
+      if constexpr (Cache::kBytes == 1)
+        x[e] = unpack2<false>(e4m3_to_f16x2(reinterpret_cast<const uint8_t*>(p)[e])).x;
+      else
+        x[e] = unpack2<Cache::kBf16>(reinterpret_cast<const uint16_t*>(p)[e]).x;
+    }
+  };
+  auto any_non_finite = [&](const float (&x)[kOwn]) {
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < kOwn; ++e) bad |= !(fabsf(x[e]) < INFINITY);
+    return __ballot_sync(0xffffffffu, has && bad);
+  };
+  // y into place d of this lane's row
+  auto put = [&](int d, float y, bool add) {
+    if (out != nullptr) {
+      y *= a.value_scale;
+      if (add) y += bf16 ? unpack2<true>(out[d]).x : unpack2<false>(out[d]).x;
+      out[d] = static_cast<uint16_t>(bf16 ? pack2<true>(y, 0.f) : pack2<false>(y, 0.f));
+    } else {
+      part[d] = add ? part[d] + y : y;
+    }
+  };
+#pragma unroll 1
+  for (int pass = uncut ? 0 : 1; pass < (cut ? 2 : 1); ++pass) {
+    float special[kOwn];  // their sum
+#pragma unroll
+    for (int e = 0; e < kOwn; ++e) special[e] = 0.f;
+#pragma unroll 1
+    for (int tile = s.tile; tile < s.end; ++tile) {
+      if (s.cut(tile * kKeys, a.sinks) != (pass == 1)) continue;
+#pragma unroll 1
+      for (int v0 = tile * kKeys; v0 < min(s.view.count, (tile + 1) * kKeys); v0 += 32) {
+        // a lane finds the rows of one key
+        unsigned long long key_row = 0, value_row = 0;
+        if (v0 + lane < s.view.count) {
+          const int key = s.view.key(v0 + lane), block = key / a.block_size, offset = key - block * a.block_size;
+          const int64_t page = __ldg(a.tables + static_cast<int64_t>(s.view.seq) * a.table_stride + block);
+          if (page >= 0 && page < a.num_blocks) {
+            key_row = reinterpret_cast<unsigned long long>(a.key + page * a.key_block + offset * a.key_token +
+                                                           s.head * a.key_head);
+            value_row = reinterpret_cast<unsigned long long>(a.value + page * a.value_block + offset * a.value_token +
+                                                             s.head * a.value_head);
+          }
+        }
+#pragma unroll 1
+        for (int k0 = 0; k0 < 32; k0 += kBatch) {
+          float x[kBatch][kOwn];
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) {
+            const unsigned long long row = __shfl_sync(0xffffffffu, value_row, k0 + k);
+#pragma unroll
+            for (int e = 0; e < kOwn; ++e) x[k][e] = 0.f;
+            if (row != 0 && has) own_of(row, x[k]);
+          }
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) {
+            unsigned lanes = any_non_finite(x[k]);
+            if (lanes == 0) continue;
+            float of_key[kOwn];
+#pragma unroll
+            for (int e = 0; e < kOwn; ++e) of_key[e] = 0.f;
+            const unsigned long long row = __shfl_sync(0xffffffffu, key_row, k0 + k);
+            if (has) own_of(row, of_key);
+            const bool bad_key = any_non_finite(of_key) != 0;
+#pragma unroll
+            for (int e = 0; e < kOwn; ++e)
+              x[k][e] = fabsf(x[k][e]) < INFINITY ? 0.f : bad_key ? NAN : x[k][e];
+            if (pass == 0) {
+#pragma unroll
+              for (int e = 0; e < kOwn; ++e) special[e] += x[k][e];
+              continue;
+            }
+            const int v = v0 + k0 + k;
+            const bool sees = mine && v <= v_last && !(v >= a.sinks && v <= v_low);
+#pragma unroll 1
+            for (; lanes != 0; lanes &= lanes - 1) {
+              const int from = __ffs(lanes) - 1;
+#pragma unroll
+              for (int e = 0; e < kOwn; ++e) {
+                const float y = __shfl_sync(0xffffffffu, x[k][e], from);
+                if (sees && y != 0.f) put(from * kOwn + e, y, true);
+              }
+            }
+          }
+        }
+      }
+    }
+    if (pass == 0) {
+#pragma unroll 1
+      for (unsigned lanes = any_non_finite(special); lanes != 0; lanes &= lanes - 1) {
+        const int from = __ffs(lanes) - 1;
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e) {
+          const float y = __shfl_sync(0xffffffffu, special[e], from);
+          if (mine && y != 0.f) put(from * kOwn + e, y, false);
+        }
+      }
+    }
+  }
 }
 
 template <typename Cache, int DP>
@@ -487,6 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int start_block;
   __shared__ Share shares[kSlots];
   __shared__ int abort_flag;
+  __shared__ int dropped[kSlots];  // values left out of a segment's cut tiles
 
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
@@ -550,10 +695,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after_sync();
   const uint32_t tmem = tmem_base;
 
-  // Where 16-byte chunk `ch` of row r of a tile lies.
-  auto place = [](int r, int ch) {
-    return static_cast<uint32_t>((ch >> 3) * (kKeys * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
-  };
   auto queries_barrier = [&](uint32_t bar, uint32_t n) { return bar + 8 * (n % kQueries); };
   auto queries_parity = [&](uint32_t n) { return (n / kQueries) & 1u; };
   // The segment that a warp turns to, and the end of its use of one.
@@ -675,6 +816,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int64_t last = ws.first[s.block] + static_cast<int64_t>(s.head + 1) * (s.tiles + kSegmentCost) - 1;
         s.last_cta = static_cast<int>((plan.ctas * (last + 1) - 1) / plan.tiles);
         shares[n % kSlots] = s;
+        dropped[n % kSlots] = 0;
         barrier_arrive(announced + 8 * (n % kSlots));
         if (s.end == s.tile) break;
         s.next(a, c, ws);
@@ -783,8 +925,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t issued = 0, arrived = 0;
       uint32_t segment = 0;
       constexpr uint32_t kAhead = 2;  // tiles in flight behind the one being issued
+      // Of each tile in flight four bits: values of a cut tile, and the
+      // segment's slot (nobody reuses it before its softmax, thus these, is done).
+      uint32_t marks = 0;
       // Hands over the oldest of the tiles in flight.
       auto complete = [&]() {
+        if constexpr (!kE4m3) {
+          const uint32_t mark = marks >> (4 * (arrived & 7u));
+          if (mark & 1u) {
+            unsigned char* const tile = smem_ptr + 2 * kQueries * kTileBytes + (arrived % kStages) * kTileBytes;
+            if (drop_non_finite<kBf16, DP>(tile, w * 32, row_chunks)) *const_cast<volatile int*>(&dropped[(mark >> 1) & 3u]) = 1;
+            __syncwarp();
+          }
+        }
         fence_async_proxy();
         barrier_arrive(full + 8 * (arrived % kStages));
         ++arrived;
@@ -842,6 +995,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const char* const key_row = a.key + block * a.key_block + offset * a.key_token + s.head * a.key_head;
           const char* const value_row = a.value + block * a.value_block + offset * a.value_token + s.head * a.value_head;
           if (tile + 1 < s.end) look_up(tile + 1);
+          const bool cut = s.cut(tile * kKeys, a.sinks);
 #pragma unroll 1
           for (int side = 0; side < 2; ++side) {
             const unsigned long long row = reinterpret_cast<unsigned long long>(side == 0 ? key_row : value_row);
@@ -860,6 +1014,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                              (seen >> (i * kPerInstr + sub)) & 1u);
               }
               cp_async_commit();
+              const uint32_t mark = (side == 1 && cut ? 1u : 0u) | (segment % kSlots) << 1;
+              marks = (marks & ~(15u << (4 * (issued & 7u)))) | mark << (4 * (issued & 7u));
               ++issued;
               if (issued - arrived > kAhead) {
                 cp_async_wait<kAhead>();
@@ -876,6 +1032,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int r = i * kRowsPer + which;
                 const uint4* from = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, row, r)) + part;
                 x[i] = ((seen >> r) & 1u) && part * 16 < a.dim ? __ldg(from) : make_uint4(0, 0, 0, 0);
+              }
+              if (side == 1 && cut) {
+                uint32_t found = 0;
+#pragma unroll
+                for (int i = 0; i < 32 / kRowsPer; ++i)
+                  x[i] = make_uint4(drop_nan4(x[i].x, &found), drop_nan4(x[i].y, &found), drop_nan4(x[i].z, &found),
+                                    drop_nan4(x[i].w, &found));
+                if (found != 0) *const_cast<volatile int*>(&dropped[segment % kSlots]) = 1;
+                __syncwarp();
               }
               claim();
               if (!ok) break;
@@ -1089,29 +1254,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               ml[kRows + r] = l;
             }
           }
-          unsigned again = __ballot_sync(0xffffffffu, live && !finite && l < INFINITY);
-          while (again) {
-            const int who = __ffs(again) - 1;
-            again &= again - 1;
-            float sum[4];
-            const float w_base = __shfl_sync(0xffffffffu, base, who);
-            const float w_factor = __shfl_sync(0xffffffffu, factor, who);
-            const int w_row = __shfl_sync(0xffffffffu, own, who);
-            const int64_t w_out = __shfl_sync(0xffffffffu, out_row, who);
-            row_again<Cache>(a, c, s, w_row, w_base, a.scale_log2, sum);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int d = lane + 32 * j;
-              if (d >= a.dim) break;
-              if (whole) {
-                const uint32_t y = a.query_type == KVCA_TYPE_BF16 ? pack2<true>(sum[j] * w_factor, 0.f)
-                                                                  : pack2<false>(sum[j] * w_factor, 0.f);
-                static_cast<uint16_t*>(a.out)[w_out * a.dim + d] = static_cast<uint16_t>(y);
-              } else {
-                ws.acc[(slot * kRows + q * 128 + (warp & 3) * 32 + who) * DP + d] = sum[j];
-              }
-            }
-          }
+          // the outputs of rows whose sum is a number show values that are not
+          const bool mine = live && l < INFINITY;
+          const bool uncut = __any_sync(0xffffffffu, mine && !finite);
+          const bool cut = *const_cast<volatile int*>(&dropped[segment % kSlots]) != 0;
+          if (uncut || cut)
+            put_non_finite<Cache, DP>(a, s, uncut, cut, mine, v_last, v_low, whole ? out : nullptr, part);
           fence_before_sync();
         }
         if (!(starts && ends)) {
@@ -1168,7 +1316,8 @@ __global__ void __launch_bounds__(kJoinThreads) attend_chunk_join_kernel(const _
   for (int64_t p = owner; p <= own.last; ++p) {
     const int64_t slot = p * 2 + (p == owner);
     const float* const ml = ws.ml + slot * 2 * kRows;
-    const float w = exp2_approx(__ldcg(ml + r) - base);
+    // never 0: an infinite value is the result, however small its weight
+    const float w = max_nan(exp2_approx(__ldcg(ml + r) - base), 0x1p-126f);
     total += w * __ldcg(ml + kRows + r);
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {

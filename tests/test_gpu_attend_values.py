@@ -149,3 +149,84 @@ def test_chunk_keeps_weights_far_below_the_largest(ops, dev, dtype, cache, dim):
         tol = tol + 2.0 ** -25
     assert ((out - want).abs() <= tol).all(), (out.min(), out.max(), want)
     assert ((lse - (26.3 * math.log(2.0) + torch.log1p(weak * w))).abs() <= 2.0 ** -17).all()
+
+
+def expect_chunk(b):
+    return oracle.attention(b.query, b.key, b.value, b.tables.clamp(min=0), b.lens, b.new, window=b.window,
+                            sinks=b.sinks, p_eps=2.0 ** -8 if b.key.dtype == BF16 else 2.0 ** -11, **b.scales)
+
+
+@pytest.mark.parametrize("magnitude", [1.0, 12.0])
+@pytest.mark.parametrize("dtype,cache", [(F16, F16), (BF16, BF16), (F16, E4M3), (BF16, E4M3)])
+@pytest.mark.parametrize("dim", [48, 64, 128])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (150, 20)])
+def test_chunk_with_infinite_values(ops, dev, dtype, cache, dim, magnitude, window, sinks):
+    """At tokens that all rows of a block see, some, or none; and every finite result as without them."""
+    kw = dict(lens=[1700, 300, 300, 40], new=[3, 300, 130, 17], heads=2, group=3, dim=dim, block=16, dtype=dtype,
+              cache=cache, seed=dim, magnitude=magnitude, window=window, sinks=sinks)
+    b, clean = oracle.Batch(**kw), oracle.Batch(**kw)
+    marks = []
+    inf = NAN if cache == E4M3 else INF
+    for s, (n, new) in enumerate(zip(b.lens, b.new)):
+        low = max(0, n - new - window + 1) if window else 0  # no row sees what is before, but for the sinks
+        span = n - low
+        for i in range(0, dim, 7):
+            marks.append((s, low + (i * 37) % span, i % 2, i, inf))
+            marks.append((s, low + (i * 53 + 1) % span, i % 2, (i + 1) % dim, -inf))
+        marks += [(s, low + 3, 0, 2, inf), (s, n - 1, 0, 2, -inf), (s, low + span // 2, 1, 3, NAN)]
+        if window:
+            marks += [(s, 0, 0, 5, inf), (s, sinks - 1, 1, 4, -inf)]
+    plant(b, marks)
+    out, lse = attend(ops, dev, b, "chunk")
+    want, want_lse, bound, lse_bound = expect_chunk(b)
+    agree(out, want, bound)
+    agree(lse, want_lse, lse_bound)  # NaN where e4m3 keys of magnitude 12 x 16 are (above 448)
+    same = attend(ops, dev, clean, "chunk")
+    finite = torch.isfinite(out)
+    assert torch.equal(out[finite], same[0][finite])
+    assert torch.equal(lse.nan_to_num(nan=99.0), same[1].nan_to_num(nan=99.0))
+
+
+@pytest.mark.parametrize("which", ["step", "chunk"])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_infinite_value_of_weight_zero(ops, dev, which, dtype):
+    """A key of -inf: the token's weight is 0, and 0 times an infinite value is NaN."""
+    new = [1, 1] if which == "step" else [90, 3]
+    b = oracle.Batch(lens=[90, 500], new=new, heads=1, group=2, dim=64, block=16, dtype=dtype, seed=4)
+    b.query[:, :, 0] = b.query[:, :, 0].abs() + 0.5
+    for s, t in ((0, 40), (1, 200), (1, 499)):
+        page, off = place(b, s, t)
+        b.key[page, off, 0, 0] = -INF
+        b.value[page, off, 0, 7] = INF
+    out, lse = attend(ops, dev, b, which)
+    sees = torch.tensor([which == "step" or row >= 40 for row in range(b.query.shape[0])])
+    assert torch.isnan(out[sees][:, :, 7]).all()
+    out[:, :, 7] = torch.where(sees.view(-1, 1), 0.0, out[:, :, 7])
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("dtype,cache", [(BF16, BF16), (F16, F16), (BF16, E4M3)])
+def test_long_context_with_an_infinite_value(ops, dev, dtype, cache):
+    """One value of an early token: 60,000 keys, 1,024 new tokens and a few of a second sequence."""
+    n, block, heads, group, dim = 60_000, 16, 2, 4, 128
+    g = torch.Generator(device=dev).manual_seed(3)
+    pages = n // block
+    key = torch.randn((2 * pages, block, heads, dim), generator=g, device=dev).to(cache)
+    value = torch.randn((2 * pages, block, heads, dim), generator=g, device=dev).to(cache)
+    query = torch.randn((1024 + 5, heads * group, dim), generator=g, device=dev).to(dtype)
+    tables = torch.randperm(2 * pages, generator=g, device=dev).view(2, -1)
+    offsets = torch.tensor([0, 1024, 1029], device=dev)
+    lens = torch.tensor([n, n], device=dev)
+    args = (query, offsets, key, value, tables, lens)
+    clean = ops.attend_chunk(*args, check=True)
+    bad = NAN if cache == E4M3 else INF
+    value[tables[0, 100], 3, 1, 17] = bad    # all rows of the first sequence
+    value[tables[0, -1], 8, 0, 20] = -bad    # the last eight tokens' rows
+    value[tables[1, -1], 13, 1, 21] = bad    # the last three rows
+    got = ops.attend_chunk(*args, check=True)
+    want = clean.clone()
+    want[:1024, group:, 17] = bad
+    want[1016:1024, :group, 20] = -bad
+    want[1026:, group:, 21] = bad
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got.nan_to_num(nan=5.0), want.nan_to_num(nan=5.0))
