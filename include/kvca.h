@@ -794,12 +794,22 @@ int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t wo
  * head_dim is at most 128.  Three launches, no host synchronisation; the work
  * is split evenly over the SMs whatever the lengths.  workspace:
  * kvca_attend_chunk_workspace_bytes(desc, num_rows) bytes, 16-byte aligned, any
- * contents, one for each call that may overlap another.  A bounded wait that runs out gives
- * KVCA_ERR_DEVICE_TIMEOUT.  No reference counterpart.
+ * contents, one for each call that may overlap another.  A wait within the
+ * kernel that takes longer than the limit (below) gives
+ * KVCA_ERR_DEVICE_TIMEOUT; the call's outputs then hold no defined values.  No
+ * reference counterpart.
  */
 int64_t kvca_attend_chunk_workspace_bytes(const kvca_attend_desc* desc, int64_t num_rows);
 int kvca_attend_chunk(const kvca_attend_desc* desc, const int64_t* d_query_offsets, int64_t num_rows,
                       void* d_workspace, int64_t workspace_bytes, int64_t* d_status, kvca_stream_t stream);
+
+/*
+ * Sets how long a wait within the kernels of later kvca_attend_chunk calls of
+ * this process may take, in nanoseconds (2 s at first; 0: a wait whose event
+ * has not come yet gives up), and returns the limit before; only returns it
+ * when negative.  A graph keeps the limit of its capture.
+ */
+int64_t kvca_attend_wait_limit(int64_t nanoseconds);
 
 /*
  * Measurement aid, not an adapter path: moves `rows` rows of row_bytes (64,

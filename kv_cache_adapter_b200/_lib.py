@@ -285,6 +285,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kvca_attend_step_counters": (c_i64, []),
     "kvca_attend_step": (c_int, [ctypes.POINTER(AttendDesc), c_ptr, c_i64, c_ptr, c_ptr, c_ptr]),
     "kvca_attend_chunk_workspace_bytes": (c_i64, [ctypes.POINTER(AttendDesc), c_i64]),
+    "kvca_attend_wait_limit": (c_i64, [c_i64]),
     "kvca_attend_chunk": (c_int, [ctypes.POINTER(AttendDesc), c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr]),
     "kvca_copy_paged": (
         c_int,

@@ -66,7 +66,8 @@ constexpr float kGrowth = 8.f;  // log2 of how far a maximum may lag
 // first one were lost).  bf16 has fp32's exponents.
 template <typename Cache>
 constexpr float kShift = Cache::kBf16 ? 0.f : 7.f;
-constexpr uint32_t kWaitTries = 1u << 24;  // a third of a second at least
+constexpr uint32_t kTryTime = 20000;       // ns that a try of a wait may suspend its thread, after the first
+constexpr uint32_t kWaitTries = 1u << 24;  // the second bound of a wait, beside its time
 
 template <int DP>
 struct ChunkShape {
@@ -230,12 +231,28 @@ __device__ __forceinline__ void barrier_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// Whether a phase is over; suspends the thread for a short while if not (the
+// hardware's choice; `time` nanoseconds or so in the second form).
 __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
       "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
       : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   return done != 0;
+}
+
+__device__ __forceinline__ bool barrier_try_for(uint32_t bar, uint32_t parity, uint32_t time) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done) : "r"(bar), "r"(parity), "r"(time) : "memory");
+  return done != 0;
+}
+
+__device__ __forceinline__ uint64_t now_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
 }
 
 // Whether a phase is over, without the suspension of a try.
@@ -247,21 +264,34 @@ __device__ __forceinline__ bool barrier_test(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 
-// Waits for a phase; gives up, as every other warp of the CTA then does, after
-// kWaitTries tries (a try suspends the thread for a while) or once another
-// warp gave up.
-__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+// How long the CTA's waits may take, and whether one of them gave up.
+struct Patience {
+  volatile int* gave_up;
+  int64_t limit;  // ns
+};
+
+// The wait for a phase whose first try was in vain (with the time and the
+// tries bounded here, not in line, drafted tokens took 51.3 us, not 55.5).
+__device__ __noinline__ bool barrier_wait_on(uint32_t bar, uint32_t parity, volatile int* gave_up, int64_t limit) {
+  const uint64_t start = now_ns();
   for (uint32_t i = 0; i < kWaitTries; ++i) {
-    if (barrier_try(bar, parity)) return true;
-    if ((i & 255u) == 255u && *abort) return false;
+    if (*gave_up) return false;
+    if (static_cast<int64_t>(now_ns() - start) >= limit) break;
+    if (barrier_try_for(bar, parity, kTryTime)) return true;
   }
-  *abort = 1;
+  *gave_up = 1;
   return false;
 }
 
+// Waits for a phase; gives up, as every other warp of the CTA then does within
+// kTryTime, after the limit or once another warp gave up.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, const Patience& patience) {
+  return barrier_try(bar, parity) || barrier_wait_on(bar, parity, patience.gave_up, patience.limit);
+}
+
 // The same for a whole warp: every lane waits, and all go on or none.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
-  return __all_sync(0xffffffffu, barrier_wait(bar, parity, abort));
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const Patience& patience) {
+  return __all_sync(0xffffffffu, barrier_wait(bar, parity, patience));
 }
 
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -630,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint32_t tmem_base;
   __shared__ int start_block;
   __shared__ Share shares[kSlots];
-  __shared__ int abort_flag;
+  __shared__ int gave_up;
   __shared__ int dropped[kSlots];  // values left out of a segment's cut tiles
 
   const int lane = threadIdx.x & 31;
@@ -642,7 +672,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t q_full = empty + 8 * kStages, q_empty = q_full + 8 * kQueries;
   const uint32_t s_full = q_empty + 8 * kQueries, p_ready = s_full + 16, o_full = s_full + 32;  // per row tile
   const uint32_t drained = s_full + 48, announced = s_full + 56, released = announced + 8 * kSlots;
-  volatile int* const abort = &abort_flag;
+  const Patience patience{&gave_up, c.wait_limit};
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -664,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       barrier_init(released + 8 * i, kReaders);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    abort_flag = 0;
+    gave_up = 0;
     start_block = 0;
   }
   if (warp == 12) {
@@ -699,7 +729,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto queries_parity = [&](uint32_t n) { return (n / kQueries) & 1u; };
   // The segment that a warp turns to, and the end of its use of one.
   auto announced_segment = [&](uint32_t n) {
-    return warp_wait(announced + 8 * (n % kSlots), (n / kSlots) & 1, abort);
+    return warp_wait(announced + 8 * (n % kSlots), (n / kSlots) & 1, patience);
   };
   auto release_segment = [&](uint32_t n) {
     __syncwarp();
@@ -745,7 +775,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         release_segment(segment);
         if (n == 0) break;
         q_low = operand_low(smem, 16) + 2 * (segment % kQueries) * (kTileBytes >> 4);
-        ok = warp_wait(queries_barrier(q_full, segment), queries_parity(segment), abort) && warp_wait(full + 8 * stage, round, abort);
+        ok = warp_wait(queries_barrier(q_full, segment), queries_parity(segment), patience) && warp_wait(full + 8 * stage, round, patience);
         if (!ok) break;
         fence_after_sync();
         if (issues) {
@@ -758,14 +788,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < n; ++i) {
           const uint32_t values_at = stage;
           const bool more = i + 1 < n;
-          ok = ok && warp_wait(full + 8 * stage, round, abort);
+          ok = ok && warp_wait(full + 8 * stage, round, patience);
           step();
           const uint32_t keys_at = stage;
 #pragma unroll 1
           for (int q = 0; q < row_tiles; ++q) {
-            ok = ok && warp_wait(p_ready + 8 * q, (p_phase >> q) & 1, abort);
+            ok = ok && warp_wait(p_ready + 8 * q, (p_phase >> q) & 1, patience);
             p_phase ^= 1u << q;
-            if (more && q == 0) ok = ok && warp_wait(full + 8 * stage, round, abort);
+            if (more && q == 0) ok = ok && warp_wait(full + 8 * stage, round, patience);
             if (!ok) break;
             fence_after_sync();
             if (issues) {
@@ -790,12 +820,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!ok) break;
       }
-      if (!ok && issues) {
-        // what was issued may still run: let it end before the memory goes
-        mma_commit(drained);
-        for (uint32_t i = 0; i < 4096 && !barrier_try(drained, 0); ++i) {
-        }
-      }
     }
     __syncwarp();
     if (warp == 13 && lane == 0 && working) {
@@ -811,7 +835,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       s.place();
       if (s.end == s.tile) s.next(a, c, ws);
       for (uint32_t n = 0;; ++n) {
-        if (n >= kSlots && !barrier_wait(released + 8 * (n % kSlots), (n / kSlots - 1) & 1, abort)) break;
+        if (n >= kSlots && !barrier_wait(released + 8 * (n % kSlots), (n / kSlots - 1) & 1, patience)) break;
         // the CTA of the segment's last tile
         const int64_t last = ws.first[s.block] + static_cast<int64_t>(s.head + 1) * (s.tiles + kSegmentCost) - 1;
         s.last_cta = static_cast<int>((plan.ctas * (last + 1) - 1) / plan.tiles);
@@ -840,7 +864,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // per row (power_up); so they do when the sign of a negative
         // scale or the zeros of a zero one go into them.
         if (segment >= kQueries)
-          ok = warp_wait(queries_barrier(q_empty, segment), queries_parity(segment - kQueries), abort);
+          ok = warp_wait(queries_barrier(q_empty, segment), queries_parity(segment - kQueries), patience);
         if (!ok) break;
         const uint32_t tile = (2 * (segment % kQueries) + w) * kTileBytes;  // of this warp's 128 rows
         float* const unit_of = row_unit[segment % kQueries] + w * 128;
@@ -958,7 +982,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t bar = empty + 8 * (issued % kStages), parity = ((issued / kStages) - 1) & 1;
         if (__all_sync(0xffffffffu, barrier_test(bar, parity))) return;
         if constexpr (!kE4m3) drain();
-        ok = warp_wait(bar, parity, abort);
+        ok = warp_wait(bar, parity, patience);
       };
       constexpr int64_t kHidden = -1ll << 62;
       for (; ok; ++segment) {
@@ -1084,7 +1108,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         const Share& s = shares[segment % kSlots];
         if (s.end == s.tile) break;
-        ok = warp_wait(queries_barrier(q_full, segment), queries_parity(segment), abort);
+        ok = warp_wait(queries_barrier(q_full, segment), queries_parity(segment), patience);
         if (!ok) break;
         const float unit = row_unit[segment % kQueries][r];
         barrier_arrive(queries_barrier(q_empty, segment));
@@ -1105,7 +1129,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           int v0 = s.tile * kKeys;
 #pragma unroll 1
           for (int i = 0; i < n; ++i, v0 += kKeys) {
-            ok = ok && warp_wait(s_full + 8 * q, phase & 1, abort);
+            ok = ok && warp_wait(s_full + 8 * q, phase & 1, patience);
             if (!ok) break;
             ++phase;
             fence_after_sync();
@@ -1199,7 +1223,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             fence_before_sync();
             barrier_arrive(p_ready + 8 * q);
           }
-          ok = ok && warp_wait(o_full + 8 * q, o_phase & 1, abort);
+          ok = ok && warp_wait(o_full + 8 * q, o_phase & 1, patience);
           if (!ok) break;
           ++o_phase;
           fence_after_sync();
@@ -1278,9 +1302,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   fence_before_sync();
   __syncthreads();
-  if (threadIdx.x == 0 && abort_flag != 0) report(a.status, KVCA_ERR_DEVICE_TIMEOUT, blockIdx.x);
+  if (threadIdx.x == 0 && gave_up != 0) report(a.status, KVCA_ERR_DEVICE_TIMEOUT, blockIdx.x);
   if (warp == 12) {
     fence_after_sync();
+    if (gave_up != 0) {
+      // products that nobody waited for may still run: they end before their
+      // memory goes (bounded, 80 ms)
+      if (lane == 0) mma_commit(drained);
+      for (int i = 0; i < 4096 && !barrier_try_for(drained, 0, kTryTime); ++i) {
+      }
+      __syncwarp();
+    }
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
 }
@@ -1383,12 +1415,13 @@ size_t attend_chunk_workspace(const AttendArgs& a, int64_t rows, int sms) {
   return ChunkWorkspace::bytes(a.dim <= 64 ? 64 : 128, sms, attend_chunk_max_blocks(a, rows));
 }
 
-cudaError_t launch_attend_chunk(const AttendArgs& args, const int64_t* offsets, int64_t rows, void* workspace, int sms,
-                                cudaStream_t stream) {
+cudaError_t launch_attend_chunk(const AttendArgs& args, const int64_t* offsets, int64_t rows, int64_t wait_limit,
+                                void* workspace, int sms, cudaStream_t stream) {
   AttendArgs a = args;
   ChunkArgs c;
   c.offsets = offsets;
   c.rows = rows;
+  c.wait_limit = wait_limit;
   c.max_blocks = static_cast<int>(attend_chunk_max_blocks(a, rows));
   // the softmax takes the maximum of the raw scores, so their factor is positive
   c.scale_log2 = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);

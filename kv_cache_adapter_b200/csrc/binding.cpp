@@ -914,6 +914,8 @@ int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t wo
 
 namespace {
 
+std::atomic<int64_t> attend_wait_limit{2000000000};
+
 int to_chunk(const kvca_attend_desc* desc, int64_t num_rows, int64_t* d_status, kvca::AttendArgs* a) {
   const int rc = to_attend(desc, d_status, a);
   if (rc != KVCA_OK) return rc;
@@ -923,6 +925,10 @@ int to_chunk(const kvca_attend_desc* desc, int64_t num_rows, int64_t* d_status, 
 }
 
 }  // namespace
+
+int64_t kvca_attend_wait_limit(int64_t nanoseconds) {
+  return nanoseconds < 0 ? attend_wait_limit.load() : attend_wait_limit.exchange(nanoseconds);
+}
 
 int64_t kvca_attend_chunk_workspace_bytes(const kvca_attend_desc* desc, int64_t num_rows) {
   kvca::AttendArgs a;
@@ -942,7 +948,8 @@ int kvca_attend_chunk(const kvca_attend_desc* desc, const int64_t* d_query_offse
   if (d_workspace == nullptr || !aligned16(reinterpret_cast<uint64_t>(d_workspace)) ||
       workspace_bytes < static_cast<int64_t>(kvca::attend_chunk_workspace(a, num_rows, sms)))
     return KVCA_ERR_BAD_ARGUMENT;
-  return status_of(kvca::launch_attend_chunk(a, d_query_offsets, num_rows, d_workspace, sms, stream));
+  return status_of(kvca::launch_attend_chunk(a, d_query_offsets, num_rows, attend_wait_limit.load(), d_workspace, sms,
+                                             stream));
 }
 
 int kvca_copy_paged(const kvca_paged_desc* src, const kvca_paged_desc* dst, int64_t num_planes,

@@ -155,6 +155,7 @@ struct ChunkArgs {
   float scale_log2;
   uint32_t query_and, query_xor;
   float shift;  // log2 of the factor in partial sums
+  int64_t wait_limit;  // ns that a wait of the kernel may take
 };
 
 size_t attend_step_workspace(const AttendArgs& args, int sms);
@@ -164,8 +165,8 @@ cudaError_t launch_attend_step(const AttendArgs& args, void* workspace, uint32_t
 
 constexpr int kChunkMaxDim = 128;  // two output tiles fill the tensor memory
 size_t attend_chunk_workspace(const AttendArgs& args, int64_t rows, int sms);
-cudaError_t launch_attend_chunk(const AttendArgs& args, const int64_t* offsets, int64_t rows, void* workspace, int sms,
-                                cudaStream_t stream);
+cudaError_t launch_attend_chunk(const AttendArgs& args, const int64_t* offsets, int64_t rows, int64_t wait_limit,
+                                void* workspace, int sms, cudaStream_t stream);
 
 // The slot pool and the page tables of the operators on sequences' pages.
 struct PagePool {
