@@ -771,11 +771,15 @@ typedef struct kvca_attend_desc {
  * the SMs whatever the lengths.  workspace:
  * kvca_attend_step_workspace_bytes(desc) bytes (lengths and values do not
  * matter) of device memory, 16-byte aligned, any contents.  d_counters:
- * kvca_attend_step_counters() words, zero on entry and zero again on exit.
- * Calls that may overlap on the GPU (other streams, graphs replayed side by
- * side) need both of their own.  No reference counterpart: the reference
- * places the pages that an engine's attention reads.
+ * kvca_attend_step_counters() words, zero on entry and zero again on exit
+ * (unless seq_lens changed while the call ran: zero them then).  Calls that
+ * may overlap on the GPU (other streams, graphs replayed side by side) need
+ * both of their own; kvca_stream_id names a stream for the life of the process,
+ * which its handle does not (all ones if CUDA refuses the handle).  No
+ * reference counterpart: the reference places the pages that an engine's
+ * attention reads.
  */
+uint64_t kvca_stream_id(kvca_stream_t stream);
 int64_t kvca_attend_step_counters(void);
 int64_t kvca_attend_step_workspace_bytes(const kvca_attend_desc* desc);
 int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t workspace_bytes, uint32_t* d_counters,

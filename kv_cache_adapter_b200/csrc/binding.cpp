@@ -893,6 +893,11 @@ int64_t kvca_attend_step_workspace_bytes(const kvca_attend_desc* desc) {
   return static_cast<int64_t>(kvca::attend_step_workspace(a, kvca_device_sm_count()));
 }
 
+uint64_t kvca_stream_id(kvca_stream_t stream) {
+  unsigned long long id = 0;
+  return cudaStreamGetId(stream, &id) == cudaSuccess ? id : ~uint64_t{0};
+}
+
 int64_t kvca_attend_step_counters(void) {
   return static_cast<int64_t>(kvca_device_sm_count()) * kvca::kStepMaxWarps;
 }

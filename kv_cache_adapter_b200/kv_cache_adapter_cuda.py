@@ -109,6 +109,19 @@ def _stream(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+_PER_THREAD_STREAM = 2  # cudaStreamPerThread
+
+
+def _scratch_stream(device: torch.device) -> int:
+    """The current stream, for a call with scratch memory from torch's
+    allocator, which knows streams by their handles: the per-thread default
+    streams of all host threads have one and the same."""
+    stream = _stream(device).value or 0
+    if stream == _PER_THREAD_STREAM:
+        raise ValueError("the per-thread default stream cannot be told from another thread's; use a stream of its own")
+    return stream
+
+
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 _no_switch = contextlib.nullcontext()
@@ -1364,11 +1377,12 @@ def fork_sequences(slot_meta: torch.Tensor, logical_to_physical: torch.Tensor, p
         return
     need = int(_lib_handle.kvca_fork_workspace_bytes(count, pool.table_width))
     with _on(dev):
+        stream = _scratch_stream(dev)
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         rc = _lib_handle.kvca_fork_sequences(
             ctypes.byref(pool), parents.data_ptr(), children.data_ptr(), fresh_slots.data_ptr(), fresh_ids.data_ptr(),
             count, ctypes.byref(pl.desc(None)), len(pl.planes), pl.row_bytes, workspace.data_ptr(), need,
-            _ptr(_status(dev)), _stream(dev))
+            _ptr(_status(dev)), stream)
     _host_rc(rc, "fork_sequences")
     _maybe_check(dev, check, "fork_sequences")
 
@@ -1389,9 +1403,10 @@ def free_sequences(slot_meta: torch.Tensor, logical_to_physical: torch.Tensor, p
         return
     need = int(_lib_handle.kvca_free_workspace_bytes(count, pool.table_width))
     with _on(dev):
+        stream = _scratch_stream(dev)
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         rc = _lib_handle.kvca_free_sequences(ctypes.byref(pool), sequences.data_ptr(), count, int(bool(discard)),
-                                             workspace.data_ptr(), need, _ptr(_status(dev)), _stream(dev))
+                                             workspace.data_ptr(), need, _ptr(_status(dev)), stream)
     _host_rc(rc, "free_sequences")
     _maybe_check(dev, check, "free_sequences")
 
@@ -1419,10 +1434,11 @@ def compact_pages(slot_meta: torch.Tensor, logical_to_physical: torch.Tensor, ph
         return remap, live.zero_()
     need = int(_lib_handle.kvca_compact_workspace_bytes(n))
     with _on(dev):
+        stream = _scratch_stream(dev)
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         rc = _lib_handle.kvca_compact_pages(ctypes.byref(pool), ctypes.byref(pl.desc(None)), len(pl.planes),
                                             pl.row_bytes, remap.data_ptr(), live.data_ptr(), workspace.data_ptr(), need,
-                                            _ptr(_status(dev)), _stream(dev))
+                                            _ptr(_status(dev)), stream)
     _host_rc(rc, "compact_pages")
     _maybe_check(dev, check, "compact_pages")
     return remap, live
@@ -1437,20 +1453,25 @@ _ATTEND_TYPES = {torch.float16: _lib.KVCA_TYPE_F16, torch.bfloat16: _lib.KVCA_TY
 _attend_workspace_bytes: dict[tuple, int] = {}
 
 
-_attend_counters: dict[tuple[int, int], torch.Tensor] = {}
+_attend_counters: dict[tuple[int, int], torch.Tensor] = {}  # by device and stream id, oldest first
+_MOST_COUNTERS = 64
 
 
 def _step_counters(dev: torch.device, stream: int) -> torch.Tensor:
-    """kvca_attend_step's counters of this (device, stream), zero between
-    calls.  A call that is captured gets counters of its own, cleared by the
-    graph, so that graphs captured on one stream may replay side by side."""
+    """kvca_attend_step's counters of this stream, zero between calls.  A
+    handle may come back for another stream while the first one's work still
+    runs; its id does not.  A call that is captured gets counters of its own,
+    cleared by the graph, so that graphs captured on one stream may replay side
+    by side."""
     if _capturing():
         return torch.zeros(int(_lib_handle.kvca_attend_step_counters()), dtype=torch.int32, device=dev)
-    key = (_index(dev), stream)
+    key = (_index(dev), _lib_handle.kvca_stream_id(stream))
     buf = _attend_counters.get(key)
     if buf is None:
         buf = torch.zeros(int(_lib_handle.kvca_attend_step_counters()), dtype=torch.int32, device=dev)
         _attend_counters[key] = buf
+        while len(_attend_counters) > _MOST_COUNTERS:  # freed in the order of the stream that used them
+            _attend_counters.pop(list(_attend_counters)[0], None)
     return buf
 
 
@@ -1569,6 +1590,7 @@ def attend_step(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
         return out
     dev = query.device
     with _on(dev):
+        stream = _scratch_stream(dev)
         shape = ("step", _index(dev), desc.q_heads // desc.kv_heads, desc.head_dim, desc.cache_type)
         need = _attend_workspace_bytes.get(shape)
         if need is None:
@@ -1577,7 +1599,6 @@ def attend_step(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
                 _raise_for(_lib.KVCA_ERR_BAD_ARGUMENT, 0, "attend_step")
             _attend_workspace_bytes[shape] = need
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        stream = _stream(dev).value or 0
         rc = _lib_handle.kvca_attend_step(ctypes.byref(desc), workspace.data_ptr(), need,
                                           _step_counters(dev, stream).data_ptr(), _status(dev).data_ptr(), stream)
     _host_rc(rc, "attend_step")
@@ -1612,12 +1633,13 @@ def attend_chunk(query: torch.Tensor, query_offsets: torch.Tensor, key_cache: to
     if rows == 0 or seq_lens.shape[0] == 0:
         return out
     with _on(dev):
+        stream = _scratch_stream(dev)
         need = _lib_handle.kvca_attend_chunk_workspace_bytes(ctypes.byref(desc), rows)
         if need < 0:
             _raise_for(_lib.KVCA_ERR_BAD_ARGUMENT, 0, "attend_chunk")
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         rc = _lib_handle.kvca_attend_chunk(ctypes.byref(desc), query_offsets.data_ptr(), rows, workspace.data_ptr(),
-                                           need, _ptr(_status(dev)), _stream(dev))
+                                           need, _ptr(_status(dev)), stream)
     _host_rc(rc, "attend_chunk")
     _maybe_check(dev, check, "attend_chunk")
     return out
