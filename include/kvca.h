@@ -792,9 +792,10 @@ int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t wo
  * tokens of sequence s, so row i of n is at position seq_lens[s] - n + i and
  * its K and V, and those of the rows before it, are in the cache.  Offsets
  * (num_seqs + 1, device memory) do not decrease; rows outside them, and those
- * of a sequence of negative length, are left as they were.  Offsets out of
- * order or outside [0, num_rows], and a sequence shorter than its chunk, give
- * KVCA_ERR_BAD_INDEX (that sequence's rows then hold no defined values).
+ * of a sequence of negative length, are left as they were.  KVCA_ERR_BAD_INDEX:
+ * a sequence whose offsets decrease, leave [0, num_rows] or begin before an
+ * earlier one of them, or that is shorter than its chunk; it is left out, and
+ * rows that no other sequence names are left as they were.
  * head_dim is at most 128.  Three launches, no host synchronisation; the work
  * is split evenly over the SMs whatever the lengths.  workspace:
  * kvca_attend_chunk_workspace_bytes(desc, num_rows) bytes, 16-byte aligned, any

@@ -166,39 +166,68 @@ __device__ __forceinline__ int chunk_tokens(const AttendArgs& a, const ChunkArgs
   return static_cast<int>(end - begin);
 }
 
+// The largest x of this and the threads before it; `sm` holds kPlanThreads.
+__device__ __noinline__ int64_t block_incl_max(int64_t x, int64_t* sm) {
+#pragma unroll 1
+  for (int d = 1; d < kPlanThreads; d <<= 1) {
+    sm[threadIdx.x] = x;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) >= d) x = max(x, sm[threadIdx.x - d]);
+    __syncthreads();
+  }
+  return x;
+}
+
 __global__ void __launch_bounds__(kPlanThreads) attend_chunk_plan_kernel(const __grid_constant__ AttendArgs a,
                                                                         const __grid_constant__ ChunkArgs c,
                                                                         void* workspace, int dp, int64_t ctas) {
   __shared__ int64_t scan[33];
+  __shared__ int64_t highest[kPlanThreads];
   ChunkWorkspace ws(workspace, dp, ctas, c.max_blocks);
   int64_t run = 0;
+  auto rows_of = [&](int seq) {
+    int len;
+    return seq < a.num_seqs ? chunk_tokens(a, c, seq, &len) * a.group : 0;
+  };
+  int next_rows = rows_of(threadIdx.x);
+  // Offsets that go back somewhere: a sequence that begins before one of the
+  // offsets ahead of it is bad, so that the others keep their rows to themselves.
+  bool back = false;
+  for (int seq = threadIdx.x; seq < a.num_seqs; seq += kPlanThreads)
+    back |= __ldg(c.offsets + seq + 1) < __ldg(c.offsets + seq);
+  back = __syncthreads_or(back) != 0;
+  int64_t ahead = 0;  // the largest offset within the rows so far
   for (int base = 0; base < a.num_seqs; base += kPlanThreads) {
     const int seq = base + threadIdx.x;
-    int rows = 0;
-    if (seq < a.num_seqs) {
-      int len;
-      rows = chunk_tokens(a, c, seq, &len) * a.group;
+    int rows = next_rows;
+    next_rows = rows_of(seq + kPlanThreads);
+    if (back) {
+      const int64_t begin = seq < a.num_seqs ? __ldg(c.offsets + seq) : 0;
+      const int64_t high = max(ahead, block_incl_max(begin <= c.rows ? begin : 0, highest));
+      if (rows > 0 && begin < high) {
+        report(a.status, KVCA_ERR_BAD_INDEX, begin);
+        rows = 0;
+      }
+      highest[threadIdx.x] = high;
+      __syncthreads();
+      ahead = highest[kPlanThreads - 1];
+      __syncthreads();
     }
     const int n = (rows + kRows - 1) / kRows;
     int64_t total;
     const int64_t at = run + block_excl_scan(static_cast<int64_t>(n), &total, scan);
-    // offsets that go back and forth may name more rows than there are
-    if (at + n > c.max_blocks) {
-      if (n > 0) report(a.status, KVCA_ERR_BAD_INDEX, __ldg(c.offsets + seq));
-    } else {
-      for (int b = 0; b < n; ++b)
-        ws.blocks[at + b] = ChunkBlock{seq, b * kRows, min(kRows, rows - b * kRows), 0};
-    }
+    // (the good sequences' rows do not overlap, so their blocks fit)
+    for (int b = 0; b < n && at + b < c.max_blocks; ++b)
+      ws.blocks[at + b] = ChunkBlock{seq, b * kRows, min(kRows, rows - b * kRows), 0};
     run += total;
   }
   const int blocks = static_cast<int>(min(run, static_cast<int64_t>(c.max_blocks)));
-  const bool whole = run <= c.max_blocks;
   __syncthreads();
   run = 0;
   for (int base = 0; base < blocks; base += kPlanThreads) {
     const int i = base + threadIdx.x;
     int tiles = 0;
-    if (i < blocks && whole) {
+    if (i < blocks) {
       const ChunkBlock b = ws.blocks[i];
       int len;
       const int tokens = chunk_tokens(a, c, b.seq, &len);
