@@ -1536,10 +1536,10 @@ def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torc
     tstride = block_tables.stride()
     if tstride[1] != 1 and tshape[1] > 1 and seqs:
         raise ValueError("block_tables must be (num_seqs, max_blocks) with contiguous rows")
-    window = 0 if window is None else int(window)
     sinks = int(sinks)
-    if window < 0 or sinks < 0 or (window == 0 and sinks > 0):
+    if sinks < 0 or (sinks > 0 if window is None else window < 1):
         raise ValueError("window must be positive (or None) and sinks need a window")
+    window = 0 if window is None else int(window)
     if not e4m3 and (key_scale != 1.0 or value_scale != 1.0):
         raise ValueError("key_scale and value_scale belong to an e4m3 cache")
     ks = _attend_rows(key_cache, kshape, "key_cache")
