@@ -759,7 +759,7 @@ typedef struct kvca_attend_desc {
   uint64_t query;           /* row r, head h: query + r * query_row_stride + h * query_head_stride */
   int64_t query_row_stride; /* bytes, multiples of 16 */
   int64_t query_head_stride;
-  uint64_t out; /* (rows, q_heads, head_dim) of the query's type, dense */
+  uint64_t out; /* (rows, q_heads, head_dim) of the query's type, dense; a dense query's own place, or over nothing else */
   float* lse;   /* (rows, q_heads), dense: log of the sum of exp(scale * q . k), or null */
 } kvca_attend_desc;
 

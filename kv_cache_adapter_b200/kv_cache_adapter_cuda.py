@@ -1488,6 +1488,21 @@ def _attend_rows(t: torch.Tensor, shape, name: str) -> list[int]:
     return out
 
 
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """First byte of a tensor that is not empty, and the byte behind its last."""
+    begin = t.data_ptr()
+    return begin, begin + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _apart(t: torch.Tensor, others, name: str) -> None:
+    """Refuses a result that lies over another tensor of the call."""
+    begin, end = _span(t)
+    for other, what in others:
+        first, last = _span(other)
+        if first < end and begin < last:
+            raise ValueError(f"{name} must not overlap {what}")
+
+
 def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
                  block_tables: torch.Tensor, seq_lens: torch.Tensor, scale, window, sinks, key_scale, value_scale,
                  out, lse) -> tuple[_lib.AttendDesc, torch.Tensor]:
@@ -1547,14 +1562,22 @@ def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torc
     qs = _attend_rows(query, qshape, "query")
     if out is None:
         out = torch.empty(qshape, dtype=qtype, device=dev)
+    elif not isinstance(out, tensor):
+        raise TypeError("out must be torch.Tensor")
     elif (out.shape != qshape or out.dtype is not qtype or out.device != dev or not out.is_contiguous()
           or out.data_ptr() % 16):
         raise ValueError(f"out must be a contiguous, 16-byte aligned {tuple(qshape)} {qtype} tensor on {dev}")
+    elif rows and not (out.data_ptr() == query.data_ptr() and query.is_contiguous()):
+        _apart(out, ((query, "query (unless it is the query)"),), "out")
     if lse is None:
         lse_ptr = None
+    elif not isinstance(lse, tensor):
+        raise TypeError("lse must be torch.Tensor")
     elif lse.shape != qshape[:2] or lse.dtype is not torch.float32 or lse.device != dev or not lse.is_contiguous():
         raise ValueError(f"lse must be a contiguous {tuple(qshape[:2])} float32 tensor on {dev}")
     else:
+        if rows:
+            _apart(lse, ((query, "query"), (out, "out")), "lse")
         lse_ptr = lse.data_ptr()
     desc = _lib.AttendDesc(
         key_cache.data_ptr(), value_cache.data_ptr(), *ks, *vs, num_blocks, block_size,
@@ -1578,10 +1601,11 @@ def attend_step(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
     ``seq_lens`` int64, the new token included.  The token at the end of a
     sequence sees all of it, or with ``window`` its last ``window`` tokens and
     the first ``sinks`` ones.  ``scale`` defaults to ``head_dim ** -0.5``.
-    Returns ``out`` ``(num_seqs, heads, head_dim)``; ``lse`` (float32
-    ``(num_seqs, heads)``) also gets the log of each softmax's sum.  A
-    sequence of length 0 gives zeros (``lse`` -inf); rows of negative length
-    are left as they were."""
+    Returns ``out`` ``(num_seqs, heads, head_dim)``, which may be the query
+    itself; ``lse`` (float32 ``(num_seqs, heads)``) also gets the log of each
+    softmax's sum.  A sequence of length 0 gives zeros (``lse`` -inf); rows of
+    negative length are left as they were.  No gradients: the cache holds no
+    graph."""
     desc, out = _attend_desc(query, key_cache, value_cache, block_tables, seq_lens, scale, window, sinks, key_scale,
                              value_scale, out, lse)
     if query.shape[0] != seq_lens.shape[0]:
