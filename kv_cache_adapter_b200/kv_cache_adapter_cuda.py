@@ -1488,21 +1488,6 @@ def _attend_rows(t: torch.Tensor, shape, name: str) -> list[int]:
     return out
 
 
-def _span(t: torch.Tensor) -> tuple[int, int]:
-    """First byte of a tensor that is not empty, and the byte behind its last."""
-    begin = t.data_ptr()
-    return begin, begin + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-
-
-def _apart(t: torch.Tensor, others, name: str) -> None:
-    """Refuses a result that lies over another tensor of the call."""
-    begin, end = _span(t)
-    for other, what in others:
-        first, last = _span(other)
-        if first < end and begin < last:
-            raise ValueError(f"{name} must not overlap {what}")
-
-
 def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
                  block_tables: torch.Tensor, seq_lens: torch.Tensor, scale, window, sinks, key_scale, value_scale,
                  out, lse) -> tuple[_lib.AttendDesc, torch.Tensor]:
@@ -1560,15 +1545,21 @@ def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torc
     ks = _attend_rows(key_cache, kshape, "key_cache")
     vs = _attend_rows(value_cache, kshape, "value_cache")
     qs = _attend_rows(query, qshape, "query")
+    q_ptr = query.data_ptr()
+    q_end = q_ptr + (rows - 1) * qs[0] + (heads - 1) * qs[1] + 2 * dim  # (without rows nothing is written)
+    size = 2 * rows * heads * dim
     if out is None:
         out = torch.empty(qshape, dtype=qtype, device=dev)
+        out_ptr = out.data_ptr()
     elif not isinstance(out, tensor):
         raise TypeError("out must be torch.Tensor")
-    elif (out.shape != qshape or out.dtype is not qtype or out.device != dev or not out.is_contiguous()
-          or out.data_ptr() % 16):
-        raise ValueError(f"out must be a contiguous, 16-byte aligned {tuple(qshape)} {qtype} tensor on {dev}")
-    elif rows and not (out.data_ptr() == query.data_ptr() and query.is_contiguous()):
-        _apart(out, ((query, "query (unless it is the query)"),), "out")
+    else:
+        out_ptr = out.data_ptr()
+        if (out.shape != qshape or out.dtype is not qtype or out.device != dev or not out.is_contiguous()
+                or out_ptr % 16):
+            raise ValueError(f"out must be a contiguous, 16-byte aligned {tuple(qshape)} {qtype} tensor on {dev}")
+        if out_ptr < q_end and q_ptr < out_ptr + size and not (out_ptr == q_ptr and query.is_contiguous()):
+            raise ValueError("out must not overlap query (unless it is the query)")
     if lse is None:
         lse_ptr = None
     elif not isinstance(lse, tensor):
@@ -1576,14 +1567,15 @@ def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torc
     elif lse.shape != qshape[:2] or lse.dtype is not torch.float32 or lse.device != dev or not lse.is_contiguous():
         raise ValueError(f"lse must be a contiguous {tuple(qshape[:2])} float32 tensor on {dev}")
     else:
-        if rows:
-            _apart(lse, ((query, "query"), (out, "out")), "lse")
         lse_ptr = lse.data_ptr()
+        lse_end = lse_ptr + 4 * rows * heads
+        if lse_ptr < q_end and q_ptr < lse_end or lse_ptr < out_ptr + size and out_ptr < lse_end:
+            raise ValueError("lse must not overlap query or out")
     desc = _lib.AttendDesc(
         key_cache.data_ptr(), value_cache.data_ptr(), *ks, *vs, num_blocks, block_size,
         block_tables.data_ptr() or None, tstride[0], tshape[1], seq_lens.data_ptr() or None, seqs, heads, kv_heads, dim,
         _ATTEND_TYPES[qtype], _ATTEND_TYPES[ctype], dim ** -0.5 if scale is None else scale, key_scale, value_scale,
-        window, sinks, query.data_ptr(), *qs, out.data_ptr(), lse_ptr)
+        window, sinks, q_ptr, *qs, out_ptr, lse_ptr)
     return desc, out
 
 

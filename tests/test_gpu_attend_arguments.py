@@ -68,9 +68,9 @@ def test_results_over_other_tensors_refused(ops, dev, which):
     with pytest.raises(ValueError, match="out must not overlap query"):
         call(wide[:, ::2], *rest, out=wide.view(-1)[:n].view(query.shape))
     sums = both[:2 * query.shape[0] * query.shape[1]].view(torch.float32).view(query.shape[:2])
-    with pytest.raises(ValueError, match="lse must not overlap out"):
+    with pytest.raises(ValueError, match="lse must not overlap"):
         call(query, *rest, out=both[:n].view(query.shape), lse=sums)
-    with pytest.raises(ValueError, match="lse must not overlap query"):
+    with pytest.raises(ValueError, match="lse must not overlap"):
         call(both[:n].view(query.shape), *rest, lse=sums)
     # side by side is fine
     out = both[n:].view(query.shape)
