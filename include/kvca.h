@@ -722,7 +722,8 @@ int kvca_compact_pages(const kvca_page_pool* pool, const kvca_paged_desc* cache,
  *   j <= p  with  window == 0, or j > p - window, or j < sinks,
  * and gets  sum_j softmax_j(scale * q . k_j) v_j  over them.  What the cache
  * holds at tokens that no query of the call sees is never part of a result,
- * and page table entries of blocks without a seen token are not read (pages
+ * and an infinite value that a query sees is its result, however small the
+ * weight.  Page table entries of blocks without a seen token are not read (pages
  * behind the window may have been given back).  seq_lens[s]: the tokens of
  * sequence s, the new ones among them (their K and V are in the cache);
  * 0: none; negative: an idle row, whose outputs are left as they were.

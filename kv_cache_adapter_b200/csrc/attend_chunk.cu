@@ -24,18 +24,27 @@
 // by more than 2^8, so that most tiles leave it alone; a probability is then at
 // most 2^8.
 //
-// Long chunks are bound by the chain scores, softmax, probabilities, product of
-// each row tile, with two tiles to overlap: 10,494 new tokens in 5 sequences
-// (32 query heads of 128, bf16) 940 us, 0.87 PFLOP/s, tensor cores 46 % active.
-// At head dim 64 by the softmax's instructions and exponentials (16 per SM and
-// clock): 16,167 tokens, window 1,024, e4m3, 270 us.  A few tokens by latency:
-// 24 sequences with 1-8 tokens over 27,000 keys 50 us (2.1 TB/s).
+// All are bound by the latency of the chain scores, softmax, probabilities,
+// product of each row tile, with two tiles to overlap; no unit is busy half of
+// the time.  10,494 new tokens in 5 sequences (32 query heads of 128, bf16)
+// 970-1,030 us by the GPU's clock, 0.80-0.85 PFLOP/s: tensor cores 46 % active,
+// exponentials 48 %, issue slots 45 %.  16,167 tokens, window 1,024, head dim
+// 64, e4m3, 275-279 us: 19, 41 and 46 %.  24 sequences with 1-8 tokens over
+// 27,000 keys 51-53 us (2.1 TB/s): at most 32 rows of a block's 256.
+//
+// Probabilities go into the second product as the 16-bit type that the tensor
+// cores multiply values in, rounded to half a step: 2^-11 of each as fp16 (fp16
+// and e4m3 caches), 2^-8 as bf16, as much as the result's own rounding and
+// averaged over the keys (error against 64 bits 1.35 times that of fp32
+// probabilities on the bf16 prompts, 1.33 times on the fp16 drafts).  A second
+// term would double the second product, half of the tensor cores' work.  The
+// sums of the softmax take the fp32 ones.
 //
 // The softmax reads its scores twice from tensor memory, in loops of 32
 // columns: held in registers in one pass (128 of them, unrolled) the prompts
-// took 929 us and the window 303.  Scores in halves of 64 keys, so that the
+// took 2 % less and the window 11 % more.  Scores in halves of 64 keys, so that the
 // next half comes while a softmax runs, cost the tensor cores more than it
-// gave (1,108 us), as did an issuing warp per row tile (1,183).
+// gave (19 % more time), as did an issuing warp per row tile (27 %).
 
 #include <cuda_runtime.h>
 #include <stdint.h>

@@ -6,8 +6,8 @@
 // sequences are dealt out evenly, a contiguous run to each warp of one CTA per
 // SM, so ragged batches and single long sequences load every SM alike.  Warps
 // side by side take the same run for different heads, whose rows lie side by
-// side in memory (256 windowed sequences with 8 e4m3 K/V heads: 243 us, a run
-// per warp and head 288).  A warp streams its run through a ring of its own in
+// side in memory (256 windowed sequences with 8 e4m3 K/V heads: a run per warp
+// and head takes 18 % more).  A warp streams its run through a ring of its own in
 // shared memory (cp.async, no barrier with other warps) and keeps the running
 // maximum and sum of the softmax and the output in registers.  A (sequence,
 // head group) that lies inside one run is written directly; one that several
@@ -16,8 +16,9 @@
 // us of 94 with 96 ragged sequences, and a launch).
 //
 // 96 ragged sequences of 37-8,191 tokens, 8 K/V heads of 128 in fp16 (495 MB):
-// 94 us, 5.3 TB/s, 80 % of the measured copy bandwidth; 256 sequences with a
-// window of 4,096 tokens in e4m3 (1.34 GB): 245 us, 5.5 TB/s.
+// 95 us, 5.2 TB/s, 79 % of the measured copy bandwidth; 256 sequences with a
+// window of 4,096 tokens in e4m3 (1.34 GB): 270-277 us, 4.8-4.95 TB/s, issue
+// slots 65 % (as many instructions per token as fp16, and the conversions).
 //
 // Both products run transposed on m16n8k16: S^T = K Q^T has the 16 tokens as
 // rows and up to 8 query heads that share the K/V head as columns, O^T = V^T
@@ -572,7 +573,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
           p_low[n][0] = transpose8x8(pack2<true>(max_nan(x[0] - t.x, Shape::kLeast), max_nan(x[1] - t.y, Shape::kLeast)));
           p_low[n][1] = transpose8x8(pack2<true>(max_nan(x[2] - b.x, Shape::kLeast), max_nan(x[3] - b.y, Shape::kLeast)));
         } else {
-          // fp16: 2^-11, no more than the result's own rounding
+          // fp16: 2^-11, no more than the result's own rounding (error against
+          // 64 bits of the ragged batch 1.24 times that of fp32 ones)
           p[n][0] = transpose8x8(pack2<false>(x[0], x[1]));
           p[n][1] = transpose8x8(pack2<false>(x[2], x[3]));
         }

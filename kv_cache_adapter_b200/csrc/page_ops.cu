@@ -6,9 +6,9 @@
 // word) until many pages' bytes move, and then by HBM.  Each is a chain of
 // small launches, the later ones programmatic dependents, instead of one
 // kernel with grid barriers, because the work of each part is spread over the
-// whole GPU differently.  240 children of 48 sequences (64 planes, 60 MB): 48 us;
-// 128 sequences with 75,000 pages freed: 36 us; 1.85 GB of pages compacted: 301
-// us, 94 % of the measured copy bandwidth.
+// whole GPU differently.  240 children of 48 sequences (64 planes, 60 MB): 54 us;
+// 128 sequences with 75,000 pages freed: 40 us; 1.85 GB of pages compacted: 310
+// us, 91 % of the measured copy bandwidth.
 
 #include <cuda_runtime.h>
 #include <stdint.h>
