@@ -72,9 +72,11 @@ constexpr float kGrowth = 8.f;  // log2 of how far a maximum may lag
 // Probabilities, and their sum, are held times 2^7 where they are fp16 (the
 // largest, 2^15, is within its range): those of 2^-21 of the maximum keep 11
 // bits, those of 2^-31 some (2^-14 and 2^-24 without: 2,000 tokens at 2^-26 of a
-// first one were lost).  bf16 has fp32's exponents.
+// first one were lost).  bf16 has fp32's exponents: there they are 2^24 times
+// smaller, 2^-16 at most, so that sums of 65,536 of the type's largest values
+// do not overflow.
 template <typename Cache>
-constexpr float kShift = Cache::kBf16 ? 0.f : 7.f;
+constexpr float kShift = Cache::kBf16 ? -24.f : 7.f;
 constexpr uint32_t kTryTime = 20000;       // ns that a try of a wait may suspend its thread, after the first
 constexpr uint32_t kWaitTries = 1u << 24;  // the second bound of a wait, beside its time
 

@@ -65,12 +65,14 @@ struct StepShape {
   // Weights of the values and their sum are held times 2^kShift of the running
   // maximum's own: fp16 ones then keep 11 bits to 2^-29 of the largest and some
   // to 2^-39 (to 2^-14 and 2^-24 without, where 2,000 tokens at 2^-26 of a
-  // first one were lost); the largest, 2^15, is within fp16's range.
-  static constexpr float kShift = Cache::kBf16 ? 0.f : 15.f;
+  // first one were lost); the largest, 2^15, is within fp16's range.  bf16 ones
+  // are held 2^16 times smaller, so that sums of 65,536 of the type's largest
+  // values do not overflow.
+  static constexpr float kShift = Cache::kBf16 ? -16.f : 15.f;
   // An infinite value at a token that the query sees is the result, however
   // small its weight: a visible token's weight is never 0 (0 x inf is NaN),
-  // nor is that of a partial result.  The least of fp16 (2^-39 of the largest)
-  // and of bf16 move no sum.  e4m3 has no infinities.
+  // nor is that of a partial result.  What the least ones add is below a value's
+  // 2^-39 (fp16) or 2^-110 (bf16).  e4m3 has no infinities.
   static constexpr bool kInfinities = Cache::kBytes == 2;
   static constexpr float kLeast = Cache::kBf16 ? 0x1p-126f : 0x1p-24f;
 };

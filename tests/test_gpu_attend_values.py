@@ -230,3 +230,20 @@ def test_long_context_with_an_infinite_value(ops, dev, dtype, cache):
     want[1026:, group:, 21] = bad
     assert torch.equal(torch.isnan(got), torch.isnan(want))
     assert torch.equal(got.nan_to_num(nan=5.0), want.nan_to_num(nan=5.0))
+
+
+@pytest.mark.parametrize("which", ["step", "chunk"])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_large_values(ops, dev, which, dtype):
+    """Averages of half the type's largest value are that value: sums of it do not overflow."""
+    new = [1, 1, 1] if which == "step" else [400, 3, 5]
+    b = oracle.Batch(lens=[400, 3000, 70], new=new, heads=2, group=2, dim=64, block=16, dtype=dtype, seed=6)
+    most = torch.finfo(dtype).max / 2
+    for s, n in enumerate(b.lens):
+        for t in range(n):
+            page, off = place(b, s, t)
+            b.value[page, off, 0], b.value[page, off, 1] = most, -most
+    out, _ = attend(ops, dev, b, which)
+    # a weight's rounding (half a step at most), sums and the exponential (2^-20), the result's rounding
+    tol = most * (torch.finfo(dtype).eps * 1.01 + 2.0 ** -20)
+    assert ((out[:, :2] - most).abs() <= tol).all() and ((out[:, 2:] + most).abs() <= tol).all()
