@@ -49,9 +49,14 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return y;
 }
 
-// Two floats cut off to bf16, in one register, the first in the low half.
-__device__ __forceinline__ uint32_t high_halves(float lo, float hi) {
-  return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+// Two floats cut off to 16 bits (towards 0), in one register, the first in the
+// low half.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t cut2(float lo, float hi) {
+  if constexpr (kBf16) return __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+  uint32_t r;
+  asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {

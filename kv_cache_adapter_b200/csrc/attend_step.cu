@@ -17,7 +17,7 @@
 //
 // 96 ragged sequences of 37-8,191 tokens, 8 K/V heads of 128 in fp16 (495 MB):
 // 95 us, 5.2 TB/s, 79 % of the measured copy bandwidth; 256 sequences with a
-// window of 4,096 tokens in e4m3 (1.34 GB): 270-277 us, 4.8-4.95 TB/s, issue
+// window of 4,096 tokens in e4m3 (1.34 GB): 260-277 us, 4.8-5.1 TB/s, issue
 // slots 65 % (as many instructions per token as fp16, and the conversions).
 //
 // Both products run transposed on m16n8k16: S^T = K Q^T has the 16 tokens as
@@ -231,6 +231,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
   using Shape = StepShape<Cache, DP, NG>;
   constexpr bool kBf16 = Cache::kBf16;
   constexpr bool kE4m3 = Cache::kBytes == 1;
+  constexpr bool kTwoTerms = !kE4m3;  // of a probability
   constexpr int kChunks = Shape::kChunks;
   constexpr int kStages = Shape::kStages;
   constexpr int kHeads = Shape::kHeads;
@@ -563,20 +564,21 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
           x[j + 2] = token_weight(x[j + 2], base);
           l[n][j] = l[n][j] * decay[n][j] + (x[j] + x[j + 2]);
         }
-        if constexpr (kBf16) {
-          // bf16 would leave 8 bits of a probability: the remainder goes in
-          // as a second product (the tensor cores idle here anyway), to 2^-15
-          // in all.  The first term is cut off, so that the remainder is not
-          // negative, and like it never 0 (inf - inf, 0 x inf).
-          const uint32_t top = high_halves(x[0], x[1]), bottom = high_halves(x[2], x[3]);
-          const float2 t = unpack2<true>(top), b = unpack2<true>(bottom);
+        if constexpr (kTwoTerms) {
+          // 16 bits would leave 8 (bf16) or 11 (fp16) of a probability: the
+          // remainder goes in as a second product (the tensor cores idle here
+          // anyway), to 2^-15 (2^-21) in all.  The first term is cut off, so that
+          // the remainder is not negative, and like it never 0 (inf - inf, 0 x
+          // inf).
+          const uint32_t top = cut2<kBf16>(x[0], x[1]), bottom = cut2<kBf16>(x[2], x[3]);
+          const float2 t = unpack2<kBf16>(top), b = unpack2<kBf16>(bottom);
           p[n][0] = transpose8x8(top);
           p[n][1] = transpose8x8(bottom);
-          p_low[n][0] = transpose8x8(pack2<true>(max_nan(x[0] - t.x, Shape::kLeast), max_nan(x[1] - t.y, Shape::kLeast)));
-          p_low[n][1] = transpose8x8(pack2<true>(max_nan(x[2] - b.x, Shape::kLeast), max_nan(x[3] - b.y, Shape::kLeast)));
+          p_low[n][0] = transpose8x8(pack2<kBf16>(max_nan(x[0] - t.x, Shape::kLeast), max_nan(x[1] - t.y, Shape::kLeast)));
+          p_low[n][1] = transpose8x8(pack2<kBf16>(max_nan(x[2] - b.x, Shape::kLeast), max_nan(x[3] - b.y, Shape::kLeast)));
         } else {
-          // fp16: 2^-11, no more than the result's own rounding (error against
-          // 64 bits of the ragged batch 1.24 times that of fp32 ones)
+          // one term, to 2^-11: an e4m3 cache is bound by instructions, and its
+          // values have 4 bits
           p[n][0] = transpose8x8(pack2<false>(x[0], x[1]));
           p[n][1] = transpose8x8(pack2<false>(x[2], x[3]));
         }
@@ -601,7 +603,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
 #pragma unroll
           for (int n = 0; n < NG; ++n) {
             mma16816<kBf16>(acc[n][t], f, p[n][0], p[n][1]);
-            if constexpr (kBf16) mma16816<kBf16>(acc[n][t], f, p_low[n][0], p_low[n][1]);
+            if constexpr (kTwoTerms) mma16816<kBf16>(acc[n][t], f, p_low[n][0], p_low[n][1]);
           }
         } else {
           // pieces: chunk t of tokens 0-7 and 8-15, then chunk t + 1; a

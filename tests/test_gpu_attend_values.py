@@ -247,3 +247,21 @@ def test_large_values(ops, dev, which, dtype):
     # a weight's rounding (half a step at most), sums and the exponential (2^-20), the result's rounding
     tol = most * (torch.finfo(dtype).eps * 1.01 + 2.0 ** -20)
     assert ((out[:, :2] - most).abs() <= tol).all() and ((out[:, 2:] + most).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype,p_eps", [(F16, 2.0 ** -21), (BF16, 2.0 ** -15)])
+def test_step_weights_keep_more_than_their_type(ops, dev, dtype, p_eps):
+    """Two values that nearly cancel: what is left shows the weights' last bits."""
+    n = 64
+    b = oracle.Batch(lens=[2] * n, heads=1, group=1, dim=64, block=16, dtype=dtype, seed=8)
+    b.key.zero_()
+    for s in range(n):
+        page, _ = place(b, s, 0)
+        b.key[page, 0, 0, 0] = 0.01 * (s + 1)
+        b.value[page, 0], b.value[page, 1] = 1000.0, -1000.0
+    b.query.zero_()
+    b.query[:, :, 0] = 1.0
+    out, _ = attend(ops, dev, b, "step", scale=1.0)
+    want, _, bound, _ = oracle.attention(b.query, b.key, b.value, b.tables.clamp(min=0), b.lens, [1] * n, scale=1.0,
+                                         p_eps=p_eps)
+    agree(out, want, bound)
