@@ -379,7 +379,8 @@ def _rotated(x, positions, table, interleaved, transpose):
 def _to_e2m1(x, factor):
     """Codes and scales of rows x (rows, heads, dim): bytes of (rows, heads * dim * 9 / 16)."""
     g = x.unflatten(-1, (-1, 16))
-    scale = (g.abs().amax(-1) / (6 * factor)).clamp(max=448).to(torch.float8_e4m3fn)
+    six = torch.full((), 6 * factor, device=x.device)  # (a quotient by a number of the host is a product in torch)
+    scale = (g.abs().amax(-1) / six).clamp(max=448).to(torch.float8_e4m3fn)
     unit = (scale.float() * factor)[..., None]
     y = torch.where(unit > 0, g / unit, 0.0)
     a = y.abs()
@@ -412,7 +413,7 @@ def _plain_append(st):
         if case["cache"] == "e2m1":
             cache.view(-1, cache.shape[2])[at, :case["heads"] * case["dim"] * 9 // 16] = _to_e2m1(x, 1.0)
         elif case["cache"] == "e4m3":
-            x8 = (x / st["factor"]).clamp(-448, 448).to(torch.float8_e4m3fn)
+            x8 = (x / torch.full((), st["factor"], device=x.device)).clamp(-448, 448).to(torch.float8_e4m3fn)
             cache.view(torch.uint8).flatten(0, 1)[at] = x8.view(torch.uint8)
         else:
             cache.flatten(0, 1)[at] = x.to(cache.dtype)
