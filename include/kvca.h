@@ -705,6 +705,8 @@ int kvca_compact_pages(const kvca_page_pool* pool, const kvca_paged_desc* cache,
 #define KVCA_TYPE_F16 0
 #define KVCA_TYPE_BF16 1
 #define KVCA_TYPE_E4M3 2 /* cache only; one factor each for keys and values */
+#define KVCA_TYPE_E2M1 3 /* cache only; rows as described at kvca_append_tokens */
+#define KVCA_TYPE_F32 4  /* kvca_rotate_tokens, kvca_read_tokens */
 
 /*
  * A batch of sequences over one layer's paged K and V.  Token t of sequence s
@@ -816,6 +818,139 @@ int kvca_attend_chunk(const kvca_attend_desc* desc, const int64_t* d_query_offse
  * when negative.  A graph keeps the limit of its capture.
  */
 int64_t kvca_attend_wait_limit(int64_t nanoseconds);
+
+/* ------------------------------------------------------------------------ */
+/* Rows of new tokens                                                        */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Rotary positions.  A table row of rotary_dim floats per position holds the
+ * cosines c_i, then the sines s_i of the position's angles.  The first
+ * rotary_dim dims of a head (even, at most head_dim) turn in pairs,
+ * (i, i + rotary_dim / 2) or, interleaved, (2 i, 2 i + 1):
+ *   y1 = x1 c_i - x2 s_i,  y2 = x2 c_i + x1 s_i
+ * in fp32, each product and sum rounded by itself; transposed, with -s_i (the
+ * gradient of the former; its inverse where c_i^2 + s_i^2 is 1).  The other
+ * dims stay as they are.
+ *
+ * kvca_rotate_tokens: (num_rows, heads, head_dim) of fp16, bf16 or fp32 into
+ * out, which may be x itself (the same strides) and otherwise overlaps nothing.
+ * Row r turns by positions[r]; a row of negative position is left as it was,
+ * one outside the table too (KVCA_ERR_BAD_INDEX).  Addresses and strides are
+ * multiples of 16 bytes, head_dim a multiple of 8, at most 256.  One launch.
+ * No reference counterpart.
+ */
+typedef struct kvca_rotate_desc {
+  int64_t num_rows;
+  uint64_t x; /* row r, head h: x + r * row_stride + h * head_stride (bytes) */
+  int64_t row_stride;
+  int64_t head_stride;
+  uint64_t out;
+  int64_t out_row_stride;
+  int64_t out_head_stride;
+  const int64_t* positions;
+  const float* table; /* (table_rows, rotary_dim), dense, 16-byte aligned */
+  int64_t table_rows;
+  int32_t heads;
+  int32_t head_dim;
+  int32_t rotary_dim;
+  int32_t type; /* KVCA_TYPE_F16, _BF16 or _F32 */
+  int32_t interleaved;
+  int32_t transpose;
+} kvca_rotate_desc;
+
+int kvca_rotate_tokens(const kvca_rotate_desc* desc, int64_t* d_status, kvca_stream_t stream);
+
+/*
+ * Keys and values of new tokens into a paged cache (the reshape-and-cache step
+ * that adapter.py:1275-1285 names slots for), keys rotated on the way, and the
+ * tokens' queries rotated into query_out.  Row r goes to token slot
+ * slot_mapping[r] = block * block_size + offset (distinct ones); a row of
+ * negative slot is padding: neither stored nor, its query, written.  A slot or
+ * a position out of range leaves its row out (KVCA_ERR_BAD_INDEX).  Without a
+ * table (and positions) keys are stored as they are and there are no queries.
+ * The cache is of the rows' type, or
+ *   KVCA_TYPE_E4M3  x / key_scale (value_scale), to the nearest, at most 448;
+ *   KVCA_TYPE_E2M1  4-bit values with an e4m3 scale for each 16 neighbouring
+ *     dims: scale = e4m3(max |x| / (6 key_scale)), to the nearest, at most 448,
+ *     code = e2m1(x / (scale * key_scale)), to the nearest, at most 6; the value
+ *     code * scale * key_scale.  A token's row: the codes of all heads (two per
+ *     byte, the first in the low half; head_dim / 2 bytes a head), then the
+ *     scales of all heads (head_dim / 16 bytes a head), and unused bytes up to a
+ *     multiple of 16 (kvca_e2m1_row_bytes).  head_dim is a multiple of 32; the
+ *     heads have no stride.  A NaN makes its 16 values NaN, an infinity becomes
+ *     the largest value.
+ * Ties go to even.  Addresses and strides are multiples of 16 bytes, head_dim a
+ * multiple of 8 (16 with e4m3), at most 256.  query_out may be the query (the
+ * same strides); nothing else overlaps.  One launch, no host synchronisation.
+ */
+typedef struct kvca_append_desc {
+  int64_t num_rows;
+  uint64_t query; /* or 0; strides in bytes, as in kvca_rotate_desc */
+  int64_t query_row_stride;
+  int64_t query_head_stride;
+  uint64_t query_out;
+  int64_t query_out_row_stride;
+  int64_t query_out_head_stride;
+  uint64_t key;
+  int64_t key_row_stride;
+  int64_t key_head_stride;
+  uint64_t value;
+  int64_t value_row_stride;
+  int64_t value_head_stride;
+  uint64_t key_cache; /* strides as in kvca_attend_desc */
+  int64_t key_block_stride;
+  int64_t key_token_stride;
+  int64_t key_cache_head_stride;
+  uint64_t value_cache;
+  int64_t value_block_stride;
+  int64_t value_token_stride;
+  int64_t value_cache_head_stride;
+  int64_t num_blocks;
+  int64_t block_size;
+  const int64_t* slot_mapping;
+  const int64_t* positions; /* null without a table */
+  const float* table;       /* (table_rows, rotary_dim), dense, 16-byte aligned, or null */
+  int64_t table_rows;
+  int32_t q_heads; /* 0 without queries */
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t rotary_dim;
+  int32_t type; /* of the rows: KVCA_TYPE_F16 or _BF16 */
+  int32_t cache_type;
+  int32_t interleaved;
+  float key_scale; /* 1 with a cache of the rows' type */
+  float value_scale;
+} kvca_append_desc;
+
+int64_t kvca_e2m1_row_bytes(int64_t kv_heads, int64_t head_dim);
+int kvca_append_tokens(const kvca_append_desc* desc, int64_t* d_status, kvca_stream_t stream);
+
+/*
+ * Token rows slot_mapping[r] of a cache of 8 or 4 bits as fp16, bf16 or fp32
+ * values times scale: out (num_rows, kv_heads, head_dim), dense, 16-byte
+ * aligned.  Rows of negative slot are left as they were, those of a slot
+ * outside the cache too (KVCA_ERR_BAD_INDEX).  One launch.
+ */
+typedef struct kvca_read_desc {
+  uint64_t cache;
+  int64_t block_stride;
+  int64_t token_stride;
+  int64_t head_stride; /* e4m3 only */
+  int64_t num_blocks;
+  int64_t block_size;
+  const int64_t* slot_mapping;
+  int64_t num_rows;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t cache_type; /* KVCA_TYPE_E4M3 or _E2M1 */
+  int32_t type;       /* of out */
+  float scale;
+  int32_t reserved;
+  uint64_t out;
+} kvca_read_desc;
+
+int kvca_read_tokens(const kvca_read_desc* desc, int64_t* d_status, kvca_stream_t stream);
 
 /*
  * Measurement aid, not an adapter path: moves `rows` rows of row_bytes (64,

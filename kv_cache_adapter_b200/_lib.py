@@ -33,6 +33,8 @@ KVCA_MAX_PLANES = 256
 KVCA_TYPE_F16 = 0
 KVCA_TYPE_BF16 = 1
 KVCA_TYPE_E4M3 = 2
+KVCA_TYPE_E2M1 = 3
+KVCA_TYPE_F32 = 4
 
 c_i64 = ctypes.c_int64
 c_int = ctypes.c_int
@@ -158,6 +160,94 @@ class AttendDesc(ctypes.Structure):
         ("query_head_stride", c_i64),
         ("out", ctypes.c_uint64),
         ("lse", c_ptr),
+    ]
+
+
+class RotateDesc(ctypes.Structure):
+    """kvca_rotate_desc."""
+
+    _fields_ = [
+        ("num_rows", c_i64),
+        ("x", ctypes.c_uint64),
+        ("row_stride", c_i64),
+        ("head_stride", c_i64),
+        ("out", ctypes.c_uint64),
+        ("out_row_stride", c_i64),
+        ("out_head_stride", c_i64),
+        ("positions", c_ptr),
+        ("table", c_ptr),
+        ("table_rows", c_i64),
+        ("heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("type", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("transpose", ctypes.c_int32),
+    ]
+
+
+class AppendDesc(ctypes.Structure):
+    """kvca_append_desc."""
+
+    _fields_ = [
+        ("num_rows", c_i64),
+        ("query", ctypes.c_uint64),
+        ("query_row_stride", c_i64),
+        ("query_head_stride", c_i64),
+        ("query_out", ctypes.c_uint64),
+        ("query_out_row_stride", c_i64),
+        ("query_out_head_stride", c_i64),
+        ("key", ctypes.c_uint64),
+        ("key_row_stride", c_i64),
+        ("key_head_stride", c_i64),
+        ("value", ctypes.c_uint64),
+        ("value_row_stride", c_i64),
+        ("value_head_stride", c_i64),
+        ("key_cache", ctypes.c_uint64),
+        ("key_block_stride", c_i64),
+        ("key_token_stride", c_i64),
+        ("key_cache_head_stride", c_i64),
+        ("value_cache", ctypes.c_uint64),
+        ("value_block_stride", c_i64),
+        ("value_token_stride", c_i64),
+        ("value_cache_head_stride", c_i64),
+        ("num_blocks", c_i64),
+        ("block_size", c_i64),
+        ("slot_mapping", c_ptr),
+        ("positions", c_ptr),
+        ("table", c_ptr),
+        ("table_rows", c_i64),
+        ("q_heads", ctypes.c_int32),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("type", ctypes.c_int32),
+        ("cache_type", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("key_scale", ctypes.c_float),
+        ("value_scale", ctypes.c_float),
+    ]
+
+
+class ReadDesc(ctypes.Structure):
+    """kvca_read_desc."""
+
+    _fields_ = [
+        ("cache", ctypes.c_uint64),
+        ("block_stride", c_i64),
+        ("token_stride", c_i64),
+        ("head_stride", c_i64),
+        ("num_blocks", c_i64),
+        ("block_size", c_i64),
+        ("slot_mapping", c_ptr),
+        ("num_rows", c_i64),
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("cache_type", ctypes.c_int32),
+        ("type", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+        ("out", ctypes.c_uint64),
     ]
 
 
@@ -288,6 +378,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kvca_attend_chunk_workspace_bytes": (c_i64, [ctypes.POINTER(AttendDesc), c_i64]),
     "kvca_attend_wait_limit": (c_i64, [c_i64]),
     "kvca_attend_chunk": (c_int, [ctypes.POINTER(AttendDesc), c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr]),
+    "kvca_rotate_tokens": (c_int, [ctypes.POINTER(RotateDesc), c_ptr, c_ptr]),
+    "kvca_e2m1_row_bytes": (c_i64, [c_i64, c_i64]),
+    "kvca_append_tokens": (c_int, [ctypes.POINTER(AppendDesc), c_ptr, c_ptr]),
+    "kvca_read_tokens": (c_int, [ctypes.POINTER(ReadDesc), c_ptr, c_ptr]),
     "kvca_copy_paged": (
         c_int,
         [ctypes.POINTER(PagedDesc), ctypes.POINTER(PagedDesc), c_i64, c_i64, c_i64, ctypes.c_int32,

@@ -111,6 +111,13 @@ __device__ __forceinline__ uint32_t e4m3_to_f16x2(uint32_t v) {
   return r;
 }
 
+// Two e2m1 values (low 8 bits, the first in the lower half) to two fp16 values.
+__device__ __forceinline__ uint32_t e2m1_to_f16x2(uint32_t v) {
+  uint32_t r;
+  asm("{\n.reg .b8 b;\ncvt.u8.u32 b, %1;\ncvt.rn.f16x2.e2m1x2 %0, b;\n}" : "=r"(r) : "r"(v));
+  return r;
+}
+
 // Powers of two that bring a row of queries, whose largest magnitude is
 // `big`, into fp16 for the products with e4m3 keys: the largest value falls
 // into [2^12, 2^13), so a bf16 row keeps its bits (values 2^-27 of the largest

@@ -7,6 +7,7 @@
 
 #include <atomic>
 #include <chrono>
+#include <initializer_list>
 
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -955,6 +956,180 @@ int kvca_attend_chunk(const kvca_attend_desc* desc, const int64_t* d_query_offse
     return KVCA_ERR_BAD_ARGUMENT;
   return status_of(kvca::launch_attend_chunk(a, d_query_offsets, num_rows, attend_wait_limit.load(), d_workspace, sms,
                                              stream));
+}
+
+int64_t kvca_e2m1_row_bytes(int64_t kv_heads, int64_t head_dim) {
+  if (kv_heads < 1 || head_dim < 32 || head_dim > 256 || head_dim % 32 != 0 || kv_heads > 65536) return -1;
+  return (kv_heads * head_dim * 9 / 16 + 15) / 16 * 16;
+}
+
+namespace {
+
+constexpr int64_t kMostTokenRows = int64_t{1} << 24;  // x at most 65,536 heads: a grid's blocks
+
+int log2_or_minus(int64_t x) {
+  for (int b = 0; b < 31; ++b)
+    if (x == int64_t{1} << b) return b;
+  return -1;
+}
+
+// The side of a call's paged cache: tokens that it holds, false if that is too many.
+bool cache_slots(int64_t num_blocks, int64_t block_size, int64_t* slots, int* size, int* shift) {
+  if (block_size > (int64_t{1} << 30) || num_blocks > (int64_t{1} << 62) / block_size) return false;
+  *slots = num_blocks * block_size;
+  *size = static_cast<int>(block_size);
+  *shift = log2_or_minus(block_size);
+  return true;
+}
+
+bool all_aligned16(std::initializer_list<uint64_t> words) {
+  uint64_t bits = 0;
+  for (uint64_t x : words) bits |= x;
+  return aligned16(bits);
+}
+
+bool rotation_ok(int32_t rotary_dim, int32_t head_dim, int64_t table_rows) {
+  return rotary_dim >= 2 && rotary_dim % 2 == 0 && rotary_dim <= head_dim && table_rows >= 0;
+}
+
+}  // namespace
+
+int kvca_rotate_tokens(const kvca_rotate_desc* d, int64_t* d_status, kvca_stream_t stream) {
+  if (d == nullptr || d->num_rows < 0 || d->heads < 1 || d->head_dim < 8 || d->head_dim > 256 || d->head_dim % 8 != 0 ||
+      !rotation_ok(d->rotary_dim, d->head_dim, d->table_rows) ||
+      (d->type != KVCA_TYPE_F16 && d->type != KVCA_TYPE_BF16 && d->type != KVCA_TYPE_F32))
+    return KVCA_ERR_BAD_ARGUMENT;
+  const std::initializer_list<uint64_t> words = {d->x, d->out, static_cast<uint64_t>(d->row_stride), static_cast<uint64_t>(d->head_stride),
+                            static_cast<uint64_t>(d->out_row_stride), static_cast<uint64_t>(d->out_head_stride),
+                            reinterpret_cast<uint64_t>(d->table)};
+  if (!all_aligned16(words)) return KVCA_ERR_BAD_ARGUMENT;
+  if (d->num_rows > kMostTokenRows || d->heads > 65536) return KVCA_ERR_SIZE_LIMIT;
+  if (d->num_rows == 0) return KVCA_OK;
+  if (d->x == 0 || d->out == 0 || d->positions == nullptr || d->table == nullptr) return KVCA_ERR_BAD_ARGUMENT;
+  kvca::TokenArgs a;
+  memset(&a, 0, sizeof(a));
+  a.rows = d->num_rows;
+  a.query = reinterpret_cast<const char*>(d->x);
+  a.query_row = d->row_stride;
+  a.query_head = d->head_stride;
+  a.query_out = reinterpret_cast<char*>(d->out);
+  a.query_out_row = d->out_row_stride;
+  a.query_out_head = d->out_head_stride;
+  a.positions = d->positions;
+  a.table = d->table;
+  a.table_rows = d->table_rows;
+  a.q_heads = d->heads;
+  a.dim = d->head_dim;
+  a.rotary = d->rotary_dim;
+  a.interleaved = d->interleaved != 0;
+  a.transpose = d->transpose != 0;
+  a.status = d_status;
+  return status_of(kvca::launch_rotate_tokens(a, d->type, stream));
+}
+
+int kvca_append_tokens(const kvca_append_desc* d, int64_t* d_status, kvca_stream_t stream) {
+  if (d == nullptr || d->num_rows < 0 || d->kv_heads < 1 || d->q_heads < 0 || d->head_dim < 8 || d->head_dim > 256 ||
+      d->head_dim % 8 != 0 || d->num_blocks < 0 || d->block_size < 1 ||
+      (d->type != KVCA_TYPE_F16 && d->type != KVCA_TYPE_BF16))
+    return KVCA_ERR_BAD_ARGUMENT;
+  const bool e4m3 = d->cache_type == KVCA_TYPE_E4M3, e2m1 = d->cache_type == KVCA_TYPE_E2M1;
+  if (!e4m3 && !e2m1 && d->cache_type != d->type) return KVCA_ERR_BAD_ARGUMENT;
+  if ((e4m3 && d->head_dim % 16 != 0) || (e2m1 && d->head_dim % 32 != 0)) return KVCA_ERR_BAD_ARGUMENT;
+  const bool turns = d->table_rows != 0 || d->table != nullptr || d->rotary_dim != 0;
+  if (turns && !rotation_ok(d->rotary_dim, d->head_dim, d->table_rows)) return KVCA_ERR_BAD_ARGUMENT;
+  if (d->q_heads > 0 && !turns) return KVCA_ERR_BAD_ARGUMENT;
+  for (float f : {d->key_scale, d->value_scale})
+    if (!(f >= 0x1p-60f && f <= 0x1p60f) || (!e4m3 && !e2m1 && f != 1.f)) return KVCA_ERR_BAD_ARGUMENT;
+  const std::initializer_list<uint64_t> words = {d->query, static_cast<uint64_t>(d->query_row_stride),
+                            static_cast<uint64_t>(d->query_head_stride), d->query_out,
+                            static_cast<uint64_t>(d->query_out_row_stride),
+                            static_cast<uint64_t>(d->query_out_head_stride), d->key,
+                            static_cast<uint64_t>(d->key_row_stride), static_cast<uint64_t>(d->key_head_stride),
+                            d->value, static_cast<uint64_t>(d->value_row_stride),
+                            static_cast<uint64_t>(d->value_head_stride), d->key_cache,
+                            static_cast<uint64_t>(d->key_block_stride), static_cast<uint64_t>(d->key_token_stride),
+                            e2m1 ? 0 : static_cast<uint64_t>(d->key_cache_head_stride), d->value_cache,
+                            static_cast<uint64_t>(d->value_block_stride), static_cast<uint64_t>(d->value_token_stride),
+                            e2m1 ? 0 : static_cast<uint64_t>(d->value_cache_head_stride),
+                            reinterpret_cast<uint64_t>(d->table)};
+  if (!all_aligned16(words)) return KVCA_ERR_BAD_ARGUMENT;
+  kvca::TokenArgs a;
+  memset(&a, 0, sizeof(a));
+  if (d->num_rows > kMostTokenRows || d->q_heads > 65536 || d->kv_heads > 65536 ||
+      !cache_slots(d->num_blocks, d->block_size, &a.num_slots, &a.block_size, &a.block_shift))
+    return KVCA_ERR_SIZE_LIMIT;
+  if (d->num_rows == 0) return KVCA_OK;
+  if (d->key == 0 || d->value == 0 || d->slot_mapping == nullptr || (turns && (d->table == nullptr || d->positions == nullptr)) ||
+      (d->q_heads > 0 && (d->query == 0 || d->query_out == 0)) ||
+      (a.num_slots > 0 && (d->key_cache == 0 || d->value_cache == 0)))
+    return KVCA_ERR_BAD_ARGUMENT;
+  a.rows = d->num_rows;
+  a.query = reinterpret_cast<const char*>(d->query);
+  a.query_row = d->query_row_stride;
+  a.query_head = d->query_head_stride;
+  a.query_out = reinterpret_cast<char*>(d->query_out);
+  a.query_out_row = d->query_out_row_stride;
+  a.query_out_head = d->query_out_head_stride;
+  a.key = reinterpret_cast<const char*>(d->key);
+  a.value = reinterpret_cast<const char*>(d->value);
+  a.key_row = d->key_row_stride;
+  a.key_head = d->key_head_stride;
+  a.value_row = d->value_row_stride;
+  a.value_head = d->value_head_stride;
+  a.key_cache = reinterpret_cast<char*>(d->key_cache);
+  a.value_cache = reinterpret_cast<char*>(d->value_cache);
+  a.key_cache_block = d->key_block_stride;
+  a.key_cache_token = d->key_token_stride;
+  a.key_cache_head = d->key_cache_head_stride;
+  a.value_cache_block = d->value_block_stride;
+  a.value_cache_token = d->value_token_stride;
+  a.value_cache_head = d->value_cache_head_stride;
+  a.slots = d->slot_mapping;
+  a.positions = d->positions;
+  a.table = turns ? d->table : nullptr;
+  a.table_rows = d->table_rows;
+  a.q_heads = d->q_heads;
+  a.kv_heads = d->kv_heads;
+  a.dim = d->head_dim;
+  a.rotary = d->rotary_dim;
+  a.interleaved = d->interleaved != 0;
+  a.key_scale = d->key_scale;
+  a.value_scale = d->value_scale;
+  a.status = d_status;
+  return status_of(kvca::launch_append_tokens(a, d->type, d->cache_type, stream));
+}
+
+int kvca_read_tokens(const kvca_read_desc* d, int64_t* d_status, kvca_stream_t stream) {
+  if (d == nullptr || d->num_rows < 0 || d->kv_heads < 1 || d->head_dim < 16 || d->head_dim > 256 ||
+      d->num_blocks < 0 || d->block_size < 1 ||
+      (d->type != KVCA_TYPE_F16 && d->type != KVCA_TYPE_BF16 && d->type != KVCA_TYPE_F32) ||
+      (d->cache_type != KVCA_TYPE_E4M3 && d->cache_type != KVCA_TYPE_E2M1))
+    return KVCA_ERR_BAD_ARGUMENT;
+  const bool e2m1 = d->cache_type == KVCA_TYPE_E2M1;
+  if (d->head_dim % (e2m1 ? 32 : 16) != 0) return KVCA_ERR_BAD_ARGUMENT;
+  const std::initializer_list<uint64_t> words = {d->cache, static_cast<uint64_t>(d->block_stride), static_cast<uint64_t>(d->token_stride),
+                            e2m1 ? 0 : static_cast<uint64_t>(d->head_stride), d->out};
+  if (!all_aligned16(words)) return KVCA_ERR_BAD_ARGUMENT;
+  kvca::ReadArgs a;
+  memset(&a, 0, sizeof(a));
+  if (d->num_rows > kMostTokenRows || d->kv_heads > 1024 ||
+      !cache_slots(d->num_blocks, d->block_size, &a.num_slots, &a.block_size, &a.block_shift))
+    return KVCA_ERR_SIZE_LIMIT;
+  if (d->num_rows == 0) return KVCA_OK;
+  if (d->slot_mapping == nullptr || d->out == 0 || (a.num_slots > 0 && d->cache == 0)) return KVCA_ERR_BAD_ARGUMENT;
+  a.cache = reinterpret_cast<const char*>(d->cache);
+  a.cache_block = d->block_stride;
+  a.cache_token = d->token_stride;
+  a.cache_head = d->head_stride;
+  a.slots = d->slot_mapping;
+  a.rows = d->num_rows;
+  a.heads = d->kv_heads;
+  a.dim = d->head_dim;
+  a.cache_type = d->cache_type;
+  a.scale = d->scale;
+  a.out = reinterpret_cast<char*>(d->out);
+  a.status = d_status;
+  return status_of(kvca::launch_read_tokens(a, d->type, stream));
 }
 
 int kvca_copy_paged(const kvca_paged_desc* src, const kvca_paged_desc* dst, int64_t num_planes,

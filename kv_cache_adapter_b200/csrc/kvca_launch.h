@@ -168,6 +168,55 @@ size_t attend_chunk_workspace(const AttendArgs& args, int64_t rows, int sms);
 cudaError_t launch_attend_chunk(const AttendArgs& args, const int64_t* offsets, int64_t rows, int64_t wait_limit,
                                 void* workspace, int sms, cudaStream_t stream);
 
+// Rows of tokens to rotate, and to store in a paged cache.
+struct TokenArgs {
+  int64_t rows;
+  const char* query;  // (row, head) at bytes row * query_row + head * query_head
+  int64_t query_row, query_head;
+  char* query_out;
+  int64_t query_out_row, query_out_head;
+  const char* key;
+  const char* value;
+  int64_t key_row, key_head, value_row, value_head;
+  char* key_cache;
+  char* value_cache;
+  int64_t key_cache_block, key_cache_token, key_cache_head;
+  int64_t value_cache_block, value_cache_token, value_cache_head;
+  int64_t num_slots;  // tokens that the cache holds
+  int block_size;
+  int block_shift;  // log2(block_size), or -1
+  const int64_t* slots;
+  const int64_t* positions;
+  const float* table;  // null: no rotation
+  int64_t table_rows;
+  int q_heads, kv_heads, dim, rotary;
+  bool interleaved, transpose;
+  float key_scale, value_scale;
+  int token_warps;  // that share a token (the launchers set it)
+  int64_t* status;
+};
+
+cudaError_t launch_append_tokens(const TokenArgs& args, int type, int cache_type, cudaStream_t stream);
+cudaError_t launch_rotate_tokens(const TokenArgs& args, int type, cudaStream_t stream);
+
+// Rows of a cache of 8 or 4 bits to read as wider values (out: dense).
+struct ReadArgs {
+  const char* cache;
+  int64_t cache_block, cache_token, cache_head;
+  int64_t num_slots;
+  int block_size;
+  int block_shift;
+  const int64_t* slots;
+  int64_t rows;
+  int heads, dim;
+  int cache_type;
+  float scale;
+  char* out;
+  int64_t* status;
+};
+
+cudaError_t launch_read_tokens(const ReadArgs& args, int type, cudaStream_t stream);
+
 // The slot pool and the page tables of the operators on sequences' pages.
 struct PagePool {
   void* slot_meta;

@@ -60,6 +60,11 @@ __all__ = [
     "compact_pages",
     "attend_step",
     "attend_chunk",
+    "rotary_table",
+    "rotate_tokens",
+    "append_tokens",
+    "read_tokens",
+    "e2m1_row_bytes",
     "batched_fused_single_layer_kv_transfer",
     "load_device_store",
     "save_device_store",
@@ -1658,6 +1663,350 @@ def attend_chunk(query: torch.Tensor, query_offsets: torch.Tensor, key_cache: to
                                            need, _ptr(_status(dev)), stream)
     _host_rc(rc, "attend_chunk")
     _maybe_check(dev, check, "attend_chunk")
+    return out
+
+
+# ---------------------------------------------------------------------------
+# rows of new tokens
+# ---------------------------------------------------------------------------
+
+_ROW_TYPES = {torch.float16: _lib.KVCA_TYPE_F16, torch.bfloat16: _lib.KVCA_TYPE_BF16,
+              torch.float32: _lib.KVCA_TYPE_F32}
+
+
+def rotary_table(num_positions: int, rotary_dim: int, *, base: float = 10000.0, scaling: str | None = None,
+                 factor: float = 1.0, original_positions: int | None = None, beta_fast: float = 32.0,
+                 beta_slow: float = 1.0, magnitude: float | None = None,
+                 device: torch.device | str | None = None) -> torch.Tensor:
+    """The table of ``rotate_tokens`` and ``append_tokens``: float32
+    ``(num_positions, rotary_dim)``, the cosines and then the sines of position
+    times ``base ** (-2 i / rotary_dim)``, computed in 64 bits.  ``scaling``
+    stretches it to contexts ``factor`` times as long: ``"linear"`` divides the
+    positions by ``factor``; ``"ntk"`` raises the base, so that the slowest angle
+    is divided by ``factor`` and the fastest not; ``"yarn"`` divides the angles
+    that turn less than ``beta_slow`` times within ``original_positions``, leaves
+    those that turn more than ``beta_fast`` times, blends between them, and
+    multiplies cosines and sines by ``magnitude`` (default ``0.1 ln(factor) + 1``;
+    1 for the other scalings)."""
+    if num_positions < 0 or rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("num_positions must not be negative, rotary_dim must be positive and even")
+    if scaling not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"unknown scaling {scaling!r}")
+    if not (base > 1.0 and math.isfinite(base)) or not (factor >= 1.0 and math.isfinite(factor)):
+        raise ValueError("base must be above 1 and factor at least 1")
+    if scaling is None and factor != 1.0:
+        raise ValueError("factor needs a scaling")
+    steps = torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device)
+    if scaling == "ntk" and rotary_dim > 2:
+        base *= factor ** (rotary_dim / (rotary_dim - 2))
+    rate = base ** (-steps / rotary_dim)
+    if scaling == "linear":
+        rate = rate / factor
+    elif scaling == "yarn":
+        if original_positions is None or original_positions < 1:
+            raise ValueError("the yarn scaling needs original_positions")
+        if not 0.0 < beta_slow < beta_fast:
+            raise ValueError("beta_slow must be positive and below beta_fast")
+
+        def dim_of(turns: float) -> float:
+            return rotary_dim * math.log(original_positions / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+        low = max(math.floor(dim_of(beta_fast)), 0)
+        high = min(math.ceil(dim_of(beta_slow)), rotary_dim - 1)
+        keep = 1.0 - ((steps / 2 - low) / max(high - low, 0.001)).clamp(0.0, 1.0)
+        rate = rate * (keep + (1.0 - keep) / factor)
+        if magnitude is None:
+            magnitude = 0.1 * math.log(factor) + 1.0
+    angle = torch.arange(num_positions, dtype=torch.float64, device=device).unsqueeze(1) * rate
+    return torch.cat([angle.cos(), angle.sin()], 1).mul_(1.0 if magnitude is None else magnitude).float()
+
+
+def e2m1_row_bytes(kv_heads: int, head_dim: int) -> int:
+    """Bytes of a token's row in a 4-bit cache plane, uint8 ``(num_blocks,
+    block_size, e2m1_row_bytes(kv_heads, head_dim))``: the e2m1 codes of all
+    heads, two to a byte, an e4m3 scale per 16 dims, and up to 15 unused bytes
+    (kvca_append_tokens).  ``head_dim`` is a multiple of 32 up to 256."""
+    size = int(_lib_handle.kvca_e2m1_row_bytes(kv_heads, head_dim))
+    if size < 0:
+        raise ValueError(f"a 4-bit cache takes positive kv_heads and a head_dim in multiples of 32 up to 256, got "
+                         f"{kv_heads} and {head_dim}")
+    return size
+
+
+def _e2m1_heads(cache: torch.Tensor, dim: int, name: str) -> int:
+    """K/V heads of a 4-bit cache plane."""
+    if cache.dim() != 3:
+        raise ValueError(f"{name}: a 4-bit cache is uint8 (num_blocks, block_size, row bytes)")
+    size = cache.shape[2]
+    if dim < 32 or dim > 256 or dim % 32:
+        raise ValueError(f"head_dim must be a multiple of 32 up to 256 with a 4-bit cache, got {dim}")
+    heads = size * 16 // (dim * 9)
+    if heads < 1 or -(-heads * dim * 9 // 256) * 16 != size:
+        raise ValueError(f"{name}: rows of {size} bytes are no heads of {dim} 4-bit values (e2m1_row_bytes)")
+    return heads
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """First and last address (past it) of a tensor's elements."""
+    at = t.data_ptr()
+    return at, at + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else at
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _distinct(t: torch.Tensor, name: str) -> None:
+    """No two elements of a tensor that is written share a place."""
+    if t.is_contiguous():
+        return
+    end = 1
+    for stride, size in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
+        if stride < end:
+            raise ValueError(f"{name}: elements must not share memory")
+        end = stride * (size - 1) + end
+
+
+def _token_rows(t: torch.Tensor, dev: torch.device, name: str) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be torch.Tensor")
+    if t.device != dev:
+        raise ValueError(f"{name} must be on {dev}")
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be (rows, heads, head_dim)")
+
+
+def _rotation(table: torch.Tensor, positions: torch.Tensor, rows: int, dim: int, dev: torch.device) -> None:
+    if not isinstance(table, torch.Tensor):
+        raise TypeError("table must be torch.Tensor")
+    if table.dtype is not torch.float32:
+        raise TypeError(f"table has incorrect dtype {table.dtype}")
+    if table.device != dev or table.dim() != 2 or not table.is_contiguous() or table.data_ptr() % 16:
+        raise ValueError(f"table must be a contiguous, 16-byte aligned (positions, rotary_dim) tensor on {dev}")
+    positions_held, rotary = table.shape
+    if positions_held < 1:
+        raise ValueError("table holds no positions")
+    if rotary < 2 or rotary % 2 or rotary > dim:
+        raise ValueError(f"the table's rotary_dim must be even and at most head_dim {dim}, got {rotary}")
+    _ids(positions, dev, "positions")
+    if positions.shape[0] != rows:
+        raise ValueError("positions needs one entry per row")
+
+
+def _result_rows(out: torch.Tensor | None, x: torch.Tensor, name: str) -> torch.Tensor:
+    """The result of rows x: x itself, or a tensor that nothing of x lies in."""
+    if out is None:
+        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if out is not x:
+        _token_rows(out, x.device, name)
+    _distinct(out, name)
+    if out.shape != x.shape or out.dtype is not x.dtype:
+        raise ValueError(f"{name} must be {tuple(x.shape)} {x.dtype}")
+    same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
+    if not same and _overlap(out, x):
+        raise ValueError(f"{name} must not overlap what it is computed from (unless it is the same rows)")
+    return out
+
+
+def rotate_tokens(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, *, interleaved: bool = False,
+                  transpose: bool = False, out: torch.Tensor | None = None,
+                  check: bool | None = None) -> torch.Tensor:
+    """Rotary positions (kvca_rotate_tokens): ``x`` ``(rows, heads, head_dim)``
+    fp16, bf16 or fp32, row r turned by ``positions[r]`` (int64), the angles from
+    ``table`` (``rotary_table``), whose width says how many dims of a head turn:
+    pairs ``(i, i + rotary_dim / 2)``, or ``(2 i, 2 i + 1)`` with ``interleaved``.
+    ``transpose`` multiplies by the transposed rotation: the gradient of the
+    former, and the way back to position 0.  Returns ``out``, which may be ``x``
+    itself; rows of negative position are left as they were in it."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be torch.Tensor")
+    if not x.is_cuda:
+        raise ValueError("x must be a CUDA tensor")
+    if x.dtype not in _ROW_TYPES:
+        raise TypeError(f"x has incorrect dtype {x.dtype}")
+    dev = x.device
+    _token_rows(x, dev, "x")
+    rows, heads, dim = x.shape
+    if heads < 1 or dim < 8 or dim > 256 or dim % 8:
+        raise ValueError(f"x must have heads, and a head_dim in multiples of 8 up to 256, got {heads} and {dim}")
+    _rotation(table, positions, rows, dim, dev)
+    strides = _attend_rows(x, x.shape, "x")
+    out = _result_rows(out, x, "out")
+    if _overlap(out, table) or _overlap(out, positions):
+        raise ValueError("out must not overlap table or positions")
+    if rows == 0:
+        return out
+    desc = _lib.RotateDesc(rows, x.data_ptr(), *strides, out.data_ptr(), *_attend_rows(out, out.shape, "out"),
+                           positions.data_ptr(), table.data_ptr() or None, table.shape[0], heads, dim, table.shape[1],
+                           _ROW_TYPES[x.dtype], bool(interleaved), bool(transpose))
+    with _on(dev):
+        rc = _lib_handle.kvca_rotate_tokens(ctypes.byref(desc), _status(dev).data_ptr(), _stream(dev))
+    _host_rc(rc, "rotate_tokens")
+    _maybe_check(dev, check, "rotate_tokens")
+    return out
+
+
+def _cache_side(cache: torch.Tensor, heads: int, dim: int, name: str) -> list[int]:
+    """Strides in bytes of a cache plane's blocks, tokens and heads."""
+    if cache.dtype is not torch.uint8:
+        return _attend_rows(cache, cache.shape, name)
+    return [*_attend_rows(cache, cache.shape, name), dim // 2]
+
+
+def append_tokens(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                  slot_mapping: torch.Tensor, *, positions: torch.Tensor | None = None,
+                  table: torch.Tensor | None = None, interleaved: bool = False, query: torch.Tensor | None = None,
+                  query_out: torch.Tensor | None = None, key_scale: float = 1.0, value_scale: float = 1.0,
+                  check: bool | None = None) -> torch.Tensor | None:
+    """Keys and values of new tokens into the paged cache, keys rotated on the
+    way, and the tokens' queries rotated (kvca_append_tokens): the step before
+    ``attend_step`` or ``attend_chunk``, in one launch.  ``key`` and ``value``
+    ``(rows, kv_heads, head_dim)`` and ``query`` ``(rows, heads, head_dim)`` are
+    fp16 or bf16, in any order of rows and heads (slices of one projection too).
+    Row r goes to slot ``slot_mapping[r]`` (int64, block * block_size + offset,
+    distinct); rows of negative slot are padding: nothing of them is written.
+    The caches are those of ``attend_step``: of the rows' dtype, e4m3 (which
+    holds ``x / key_scale``, ``x / value_scale``), or uint8 rows of 4-bit values
+    (``e2m1_row_bytes``; scales chosen per 16 dims, times ``key_scale``,
+    ``value_scale``).  ``positions`` and ``table`` are ``rotate_tokens``'s;
+    without them keys are stored as they are.  Returns ``query_out`` (the query
+    itself if given as such), None without a query."""
+    tensor = torch.Tensor
+    for t, name in ((key, "key"), (value, "value"), (key_cache, "key_cache"), (value_cache, "value_cache"),
+                    (slot_mapping, "slot_mapping")):
+        if not isinstance(t, tensor):
+            raise TypeError(f"{name} must be torch.Tensor")
+    if not key.is_cuda:
+        raise ValueError("key must be a CUDA tensor")
+    dev, dtype, ctype = key.device, key.dtype, key_cache.dtype
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+        raise TypeError(f"key has incorrect dtype {dtype}")
+    _token_rows(key, dev, "key")
+    _token_rows(value, dev, "value")
+    rows, heads, dim = key.shape
+    if value.shape != key.shape or value.dtype is not dtype:
+        raise ValueError("key and value must share shape and dtype")
+    four = ctype is torch.uint8
+    if not four and ctype is not torch.float8_e4m3fn and ctype is not dtype:
+        raise TypeError(f"key_cache has incorrect dtype {ctype}")
+    if value_cache.dtype is not ctype or value_cache.shape != key_cache.shape:
+        raise ValueError("key_cache and value_cache must share shape and dtype")
+    if key_cache.device != dev or value_cache.device != dev:
+        raise ValueError(f"key_cache and value_cache must be on {dev}")
+    if heads < 1 or dim < 8 or dim > 256 or dim % (32 if four else 16 if ctype is not dtype else 8):
+        raise ValueError(f"heads or head_dim out of range: {heads} and {dim}")
+    if four:
+        if _e2m1_heads(key_cache, dim, "key_cache") != heads:
+            raise ValueError(f"the caches do not hold {heads} heads of {dim}")
+    elif key_cache.dim() != 4 or key_cache.shape[2:] != (heads, dim):
+        raise ValueError(f"the caches must be (num_blocks, block_size, {heads}, {dim})")
+    num_blocks, block_size = key_cache.shape[:2]
+    if block_size < 1:
+        raise ValueError("block_size must be positive")
+    if ctype is dtype and (key_scale != 1.0 or value_scale != 1.0):
+        raise ValueError("key_scale and value_scale belong to a cache of 8 or 4 bits")
+    if not (2.0 ** -60 <= key_scale <= 2.0 ** 60 and 2.0 ** -60 <= value_scale <= 2.0 ** 60):
+        raise ValueError("key_scale and value_scale must be positive (2^-60 to 2^60)")
+    _ids(slot_mapping, dev, "slot_mapping")
+    if slot_mapping.shape[0] != rows:
+        raise ValueError("slot_mapping needs one entry per row")
+    if (positions is None) != (table is None):
+        raise ValueError("positions and table go together")
+    if table is not None:
+        _rotation(table, positions, rows, dim, dev)
+    q = (0, 0, 0, 0, 0, 0)
+    q_heads = 0
+    if query is not None:
+        _token_rows(query, dev, "query")
+        if table is None:
+            raise ValueError("query needs positions and table")
+        q_heads = query.shape[1]
+        if query.shape[0] != rows or query.shape[2] != dim or query.dtype is not dtype or q_heads < 1:
+            raise ValueError(f"query must be ({rows}, heads, {dim}) {dtype}")
+        query_out = _result_rows(query_out, query, "query_out")
+        if query_out.data_ptr() != query.data_ptr() and (_overlap(query_out, key) or _overlap(query_out, value)):
+            raise ValueError("query_out must not overlap key or value")
+        q = (query.data_ptr(), *_attend_rows(query, query.shape, "query"), query_out.data_ptr(),
+             *_attend_rows(query_out, query_out.shape, "query_out"))
+    elif query_out is not None:
+        raise ValueError("query_out needs a query")
+    for cache in (key_cache, value_cache):
+        _distinct(cache, "caches")
+        if any(t is not None and _overlap(cache, t) for t in (key, value, query, query_out)):
+            raise ValueError("the caches must not overlap the rows")
+    if key_cache.data_ptr() == value_cache.data_ptr() and key_cache.numel():
+        raise ValueError("key_cache and value_cache must be two caches")
+    desc = _lib.AppendDesc(
+        rows, *q, key.data_ptr(), *_attend_rows(key, key.shape, "key"), value.data_ptr(),
+        *_attend_rows(value, value.shape, "value"), key_cache.data_ptr(), *_cache_side(key_cache, heads, dim, "key_cache"),
+        value_cache.data_ptr(), *_cache_side(value_cache, heads, dim, "value_cache"), num_blocks, block_size,
+        slot_mapping.data_ptr() or None, None if positions is None else positions.data_ptr() or None,
+        None if table is None else table.data_ptr() or None, 0 if table is None else table.shape[0], q_heads, heads, dim,
+        0 if table is None else table.shape[1], _ROW_TYPES[dtype],
+        _lib.KVCA_TYPE_E2M1 if four else _ATTEND_TYPES[ctype], bool(interleaved), key_scale, value_scale)
+    if rows:
+        with _on(dev):
+            rc = _lib_handle.kvca_append_tokens(ctypes.byref(desc), _status(dev).data_ptr(), _stream(dev))
+        _host_rc(rc, "append_tokens")
+        _maybe_check(dev, check, "append_tokens")
+    return query_out
+
+
+def read_tokens(cache: torch.Tensor, slot_mapping: torch.Tensor, *, head_dim: int | None = None, scale: float = 1.0,
+                dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
+                check: bool | None = None) -> torch.Tensor:
+    """Token rows of an 8- or 4-bit cache plane as wider values
+    (kvca_read_tokens): row ``slot_mapping[r]`` of ``cache`` (e4m3 ``(num_blocks,
+    block_size, kv_heads, head_dim)`` or uint8 rows of 4-bit values, whose
+    ``head_dim`` has to be given) times ``scale`` in ``out`` ``(rows, kv_heads,
+    head_dim)`` fp16, bf16 or fp32 (``dtype`` where it is not given).  Rows of
+    negative slot are left as they were in ``out``."""
+    if not isinstance(cache, torch.Tensor):
+        raise TypeError("cache must be torch.Tensor")
+    if not cache.is_cuda:
+        raise ValueError("cache must be a CUDA tensor")
+    dev = cache.device
+    four = cache.dtype is torch.uint8
+    if four:
+        if head_dim is None:
+            raise ValueError("a 4-bit cache needs head_dim")
+        heads, dim = _e2m1_heads(cache, int(head_dim), "cache"), int(head_dim)
+    elif cache.dtype is torch.float8_e4m3fn:
+        if cache.dim() != 4:
+            raise ValueError("cache must be (num_blocks, block_size, kv_heads, head_dim)")
+        heads, dim = cache.shape[2:]
+        if head_dim is not None and head_dim != dim:
+            raise ValueError(f"the cache's head_dim is {dim}, not {head_dim}")
+        if heads < 1 or dim < 16 or dim > 256 or dim % 16:
+            raise ValueError(f"heads or head_dim out of range: {heads} and {dim}")
+    else:
+        raise TypeError(f"cache has incorrect dtype {cache.dtype}")
+    if cache.shape[1] < 1:
+        raise ValueError("block_size must be positive")
+    _ids(slot_mapping, dev, "slot_mapping")
+    rows = slot_mapping.shape[0]
+    if out is None:
+        if dtype not in _ROW_TYPES:
+            raise TypeError(f"incorrect dtype {dtype}")
+        out = torch.empty((rows, heads, dim), dtype=dtype, device=dev)
+    else:
+        _token_rows(out, dev, "out")
+        if out.dtype not in _ROW_TYPES:
+            raise TypeError(f"out has incorrect dtype {out.dtype}")
+        if out.shape != (rows, heads, dim) or not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError(f"out must be a contiguous, 16-byte aligned ({rows}, {heads}, {dim}) tensor on {dev}")
+        if _overlap(out, cache) or _overlap(out, slot_mapping):
+            raise ValueError("out must not overlap cache or slot_mapping")
+    strides = _cache_side(cache, heads, dim, "cache")
+    if rows:
+        desc = _lib.ReadDesc(cache.data_ptr(), *strides, cache.shape[0], cache.shape[1], slot_mapping.data_ptr(), rows,
+                             heads, dim, _lib.KVCA_TYPE_E2M1 if four else _lib.KVCA_TYPE_E4M3, _ROW_TYPES[out.dtype],
+                             scale, 0, out.data_ptr())
+        with _on(dev):
+            rc = _lib_handle.kvca_read_tokens(ctypes.byref(desc), _status(dev).data_ptr(), _stream(dev))
+        _host_rc(rc, "read_tokens")
+        _maybe_check(dev, check, "read_tokens")
     return out
 
 
