@@ -22,18 +22,29 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Storage types of the cache, and what its matrix products run in: e4m3
-// widens to fp16, which holds every e4m3 value.
+// widens to fp16, which holds every e4m3 value, and e2m1 times its scale, which
+// fp16 holds too (2 bits times 4, from 2^-10 to 2,688).
 struct CacheF16 {
   static constexpr int kBytes = 2;
   static constexpr bool kBf16 = false;
+  static constexpr bool kOdd = false;
 };
 struct CacheBf16 {
   static constexpr int kBytes = 2;
   static constexpr bool kBf16 = true;
+  static constexpr bool kOdd = false;
 };
 struct CacheE4m3 {
   static constexpr int kBytes = 1;
   static constexpr bool kBf16 = false;
+  static constexpr bool kOdd = false;
+};
+// Odd: a head's scales do not fill 4, 8 or 16 bytes of their own.
+template <bool Odd>
+struct CacheE2m1 {
+  static constexpr int kBytes = 0;  // half of one
+  static constexpr bool kBf16 = false;
+  static constexpr bool kOdd = Odd;
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -71,6 +82,13 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool r
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// The same for 4 or 8 bytes.
+template <int kSize>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, bool read) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kSize), "r"(read ? kSize : 0)
+               : "memory");
 }
 
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }

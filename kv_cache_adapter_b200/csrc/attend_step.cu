@@ -51,10 +51,12 @@ __host__ __device__ constexpr int step_warps(int row_bytes, int head_tiles) {
 // DP: head dim padded to 64, 128 or 256; NG: tiles of 8 query heads.
 template <typename Cache, int DP, int NG>
 struct StepShape {
-  static constexpr int kRowBytes = DP * Cache::kBytes;
+  static constexpr bool kFour = Cache::kBytes == 0;
+  static constexpr int kRowBytes = kFour ? DP / 2 : DP * Cache::kBytes;
   static constexpr int kChunks = kRowBytes / 16;       // 16-byte chunks of a row
-  static constexpr int kStageBytes = 2 * kTile * kRowBytes;
-  static constexpr int kWarps = step_warps(kRowBytes, NG);
+  static constexpr int kScaleBytes = !kFour ? 0 : Cache::kOdd ? 32 : DP / 16;  // of a row, after those of all rows
+  static constexpr int kStageBytes = 2 * kTile * (kRowBytes + kScaleBytes);
+  static constexpr int kWarps = step_warps(kFour ? DP : kRowBytes, NG);
   static constexpr int kThreads = 32 * kWarps;
   // 192 KiB of rings per SM
   static constexpr int kRingBytes = 192 * 1024 / kWarps;
@@ -85,6 +87,73 @@ __device__ __forceinline__ uint32_t chunk_offset(int r, int c) {
     return static_cast<uint32_t>((r * kChunks + (c ^ (r & 7))) * 16);
   else
     return static_cast<uint32_t>((r * kChunks + (c ^ ((r >> 1) & 3))) * 16);
+}
+
+// The same for rows of 4-bit values, whose lanes read as described at their
+// products: keys a quarter row of token (i / 2) + 4 (i % 2), i = lane / 4;
+// values an eighth of a row of token lane % 4 (+ 4, 8, 12).
+template <int kChunks, bool kValues>
+__device__ __forceinline__ uint32_t chunk_offset_four(int r, int c) {
+  if constexpr (kChunks == 2)  // 32-byte rows: keys with bits 1 and 2 of the row exchanged
+    return static_cast<uint32_t>((kValues ? r : (r & 9) | (r & 2) << 1 | (r & 4) >> 1) * 32 + c * 16);
+  else if constexpr (kChunks == 4)  // 64-byte rows: keys with bit 2 in front, values with halves exchanged
+    return kValues ? static_cast<uint32_t>(r * 64 + (c ^ (r & 2)) * 16)
+                   : static_cast<uint32_t>(((r & 8) | (r & 3) << 1 | (r & 4) >> 2) * 64 + c * 16);
+  else
+    return static_cast<uint32_t>(r * 128 + (c ^ (kValues ? (r & 3) << 1 : (r & 4) >> 2)) * 16);
+}
+
+// N = 1, 2, 4 or 8 words of shared memory.
+template <int N>
+__device__ __forceinline__ void load_shared(uint32_t (&w)[N], uint32_t addr) {
+  if constexpr (N == 1)
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr) : "memory");
+  else if constexpr (N == 2)
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
+  else
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ uint32_t load_shared16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ uint32_t load_shared8(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// The scales of kGroups groups of a row, each twice in a register: those from
+// `first` on of the row's `groups`, which begin `at` bytes into its place (0
+// unless they are odd); groups beyond have none.
+template <typename Cache, int kGroups>
+__device__ __forceinline__ void read_scales(uint32_t (&unit)[kGroups], uint32_t addr, int first, int at, int groups) {
+  if constexpr (kGroups == 1) {
+    const uint32_t v = load_shared8(addr + at + first);
+    unit[0] = e4m3_to_f16x2(__byte_perm(v, 0, 0x4400));
+  } else {
+#pragma unroll
+    for (int j = 0; j < kGroups; j += 2) {
+      const uint32_t v = e4m3_to_f16x2(load_shared16(addr + at + first + j));
+      unit[j] = __byte_perm(v, 0, 0x1010);
+      unit[j + 1] = __byte_perm(v, 0, 0x3232);
+    }
+  }
+  if constexpr (Cache::kOdd) {
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j)
+      if (first + j >= groups) unit[j] = 0;
+  }
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -230,8 +299,10 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
     attend_step_kernel(const __grid_constant__ AttendArgs a, void* workspace, uint32_t* arrived) {
   using Shape = StepShape<Cache, DP, NG>;
   constexpr bool kBf16 = Cache::kBf16;
+  constexpr bool kFour = Shape::kFour;
   constexpr bool kE4m3 = Cache::kBytes == 1;
-  constexpr bool kTwoTerms = !kE4m3;  // of a probability
+  constexpr bool kNarrow = Cache::kBytes < 2;  // widened to fp16
+  constexpr bool kTwoTerms = !kNarrow;         // of a probability
   constexpr int kChunks = Shape::kChunks;
   constexpr int kStages = Shape::kStages;
   constexpr int kHeads = Shape::kHeads;
@@ -301,6 +372,15 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
   // earlier run began (slot 0), and of one that this run began (slot 1)
   StepJoin leaves[2] = {{-1, 0, 0}, {-1, 0, 0}};
 
+  // Rows of tile (MMA row lane / 4) and dims of acc[][t]: the first two values
+  // are of dim first_dim(t), the others of the one kSecondDim after it.
+  const int my_token = kFour ? (lane >> 3) + (lane & 4) : lane >> 2;
+  constexpr int kSecondDim = kFour ? 2 : kE4m3 ? 1 : 8;
+  auto first_dim = [lane](int t) {
+    if constexpr (kFour) return (lane >> 2) * (DP / 8) + 4 * (t >> 1) + (t & 1);
+    return t * 16 + (kE4m3 ? 2 * (lane >> 2) : lane >> 2);
+  };
+  int scale_at = 0;  // (4 bits, odd) where the head's scales begin in a row's 32 bytes
   float acc[NG][kSteps][4];
   float m[NG][2], l[NG][2];  // of the heads 2 * (lane % 4), + 1 of each tile of 8
   // Weight of a token of score s, and of sums whose maximum is `behind` (<= 0) the whole's.
@@ -344,7 +424,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
     }
 
     const uint32_t ring = smem_addr(rings) + warp * (kStages * Shape::kStageBytes);
-    const int row_chunks = a.dim * Cache::kBytes / 16;
+    const int row_chunks = kFour ? a.dim / 32 : a.dim * Cache::kBytes / 16;
     if (row_chunks < kChunks) {  // the padded dims stay zero: no copy writes them
       for (int i = lane; i < kStages * Shape::kStageBytes / 16; i += 32)
         *reinterpret_cast<uint4*>(rings + warp * (kStages * Shape::kStageBytes) + i * 16) = make_uint4(0, 0, 0, 0);
@@ -398,6 +478,29 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
             plane + (good ? page : 0) * block_stride + offset * token_stride + page_head * head_stride);
         const unsigned seen = __ballot_sync(0xffffffffu, good);
         const uint32_t stage = ring + stage_of * Shape::kStageBytes;
+        if constexpr (kFour) {
+          // a lane copies its row's scales; where they do not start and end on
+          // a power of two, the 16 bytes that they lie in, or 32
+          const int head_scales = a.dim / 16;
+          const int in_row = a.kv_heads * (a.dim / 2) + page_head * head_scales;
+          const char* const from = plane + (good ? page : 0) * block_stride + offset * token_stride + in_row;
+          const uint32_t to = stage + 2 * kTile * Shape::kRowBytes + lane * Shape::kScaleBytes;
+          if constexpr (Cache::kOdd) {
+            cp_async16(to, from - (in_row & 15), good);
+            if ((in_row & 15) + head_scales > 16) cp_async16(to + 16, from - (in_row & 15) + 16, good);
+          } else if constexpr (Shape::kScaleBytes == 16) {
+            cp_async16(to, from, good);
+          } else {
+            cp_async_small<Shape::kScaleBytes>(to, from, good);
+          }
+        }
+        auto spot = [&](int r, int c) {
+          if constexpr (kFour)
+            return r < kTile ? chunk_offset_four<kChunks, false>(r, c)
+                             : kTile * Shape::kRowBytes + chunk_offset_four<kChunks, true>(r - kTile, c);
+          else
+            return chunk_offset<kChunks>(r, c);
+        };
         constexpr int kPerInstr = 32 / kChunks > 0 ? 32 / kChunks : 1;
         const int r0 = kChunks >= 32 ? 0 : lane / kChunks;
         const int c = lane % kChunks;
@@ -410,7 +513,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
             if (c < row_chunks) {
 #pragma unroll
               for (int r = 0; r < kTile; r += kPerInstr) {
-                cp_async16(stage + chunk_offset<kChunks>(side * kTile + r + r0, c), src);
+                cp_async16(stage + spot(side * kTile + r + r0, c), src);
                 src += kPerInstr * stride;
               }
             }
@@ -419,7 +522,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
 #pragma unroll
           for (int r = 0; r < 2 * kTile; r += kPerInstr) {
             const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, r + r0)) + c * 16;
-            if (c < row_chunks) cp_async16(stage + chunk_offset<kChunks>(r + r0, c), src, (seen >> (r + r0)) & 1u);
+            if (c < row_chunks) cp_async16(stage + spot(r + r0, c), src, (seen >> (r + r0)) & 1u);
           }
         }
         if (++stage_of == kStages) stage_of = 0;
@@ -450,13 +553,14 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
         const int part = at.chunk * span + lane_of_heads;
         const int kv_head = part / head_groups;
         const int first = (part - kv_head * head_groups) * kHeads;
+        if constexpr (kFour && Cache::kOdd) scale_at = (a.kv_heads * (a.dim / 2) + kv_head * (a.dim / 16)) & 15;
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
           const int h = first + n * 8 + (lane >> 2);
           const bool live = h < a.group;
           const uint16_t* row = static_cast<const uint16_t*>(a.query) + static_cast<int64_t>(at.seq) * a.query_row +
                                 static_cast<int64_t>(kv_head * a.group + (live ? h : 0)) * a.query_head;
-          if constexpr (!kE4m3) {
+          if constexpr (!kNarrow) {
 #pragma unroll
             for (int k = 0; k < kSteps; ++k)
 #pragma unroll
@@ -472,7 +576,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
             uint2 raw[kSteps];
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
-              const int d = k * 16 + 4 * (lane & 3);
+              const int d = kFour ? (lane & 3) * (DP / 4) + 4 * k : k * 16 + 4 * (lane & 3);
               raw[k] = live && d < a.dim ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0, 0);
               const float2 x = bf16 ? unpack2<true>(raw[k].x) : unpack2<false>(raw[k].x);
               const float2 y = bf16 ? unpack2<true>(raw[k].y) : unpack2<false>(raw[k].y);
@@ -515,8 +619,38 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       for (int n = 0; n < NG; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[n][0][j] = s[n][1][j] = 0.f;
+      if constexpr (kFour) {
+        // lane 4 i + t: dims t DP / 4 and on of the rows' tokens, four dims per
+        // step, as the query's are above; each value times its scale is exact
+        constexpr int kWords = DP / 32, kRead = kWords > 4 ? 4 : kWords;
+        constexpr int kGroups = DP / 64;  // of 16 dims, of a lane
+        uint32_t w[2][kWords], unit16[2][kGroups];
 #pragma unroll
-      for (int k = 0; k < kSteps; k += kE4m3 ? 2 : 1) {
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int part = 0; part < kWords / kRead; ++part) {
+            uint32_t x[kRead];
+            const int byte = (lane & 3) * (DP / 8) + part * 16;
+            load_shared(x, keys + chunk_offset_four<kChunks, false>(my_token + 8 * i, byte / 16) + byte % 16);
+#pragma unroll
+            for (int j = 0; j < kRead; ++j) w[i][part * kRead + j] = x[j];
+          }
+          read_scales<Cache, kGroups>(unit16[i], keys + 2 * kTile * Shape::kRowBytes + (my_token + 8 * i) * Shape::kScaleBytes,
+                               (lane & 3) * kGroups, scale_at, Cache::kOdd ? a.dim / 16 : DP / 16);
+        }
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+          const uint32_t x = w[0][k / 2] >> (16 * (k & 1)), y = w[1][k / 2] >> (16 * (k & 1));
+          const uint32_t f[4] = {mul_f16x2(e2m1_to_f16x2(x), unit16[0][k / 4]),
+                                 mul_f16x2(e2m1_to_f16x2(y), unit16[1][k / 4]),
+                                 mul_f16x2(e2m1_to_f16x2(x >> 8), unit16[0][k / 4]),
+                                 mul_f16x2(e2m1_to_f16x2(y >> 8), unit16[1][k / 4])};
+#pragma unroll
+          for (int n = 0; n < NG; ++n) mma16816<false>(s[n][k & 1], f, q[n][k][0], q[n][k][1]);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < (kFour ? 0 : kSteps); k += kE4m3 ? 2 : 1) {
         uint32_t f[4];
         if constexpr (!kE4m3) {
           ldmatrix4(f, keys + chunk_offset<kChunks>(lane & 15, 2 * k + (lane >> 4)));
@@ -537,9 +671,9 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
         }
       }
 
-      // softmax over the tile's tokens (rows lane / 4 and + 8)
+      // softmax over the tile's tokens (rows lane / 4 and + 8: tokens my_token and + 8)
       const int left = at.vis.count - at.tile * kTile;
-      const bool row0 = (lane >> 2) < left, row1 = (lane >> 2) + 8 < left;
+      const bool row0 = my_token < left, row1 = my_token + 8 < left;
       uint32_t p[NG][2], p_low[NG][2];
       bool grew = false;
       float decay[NG][2];
@@ -577,8 +711,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
           p_low[n][0] = transpose8x8(pack2<kBf16>(max_nan(x[0] - t.x, Shape::kLeast), max_nan(x[1] - t.y, Shape::kLeast)));
           p_low[n][1] = transpose8x8(pack2<kBf16>(max_nan(x[2] - b.x, Shape::kLeast), max_nan(x[3] - b.y, Shape::kLeast)));
         } else {
-          // one term, to 2^-11: an e4m3 cache is bound by instructions, and its
-          // values have 4 bits
+          // one term, to 2^-11: a cache of 8 or 4 bits is bound by instructions,
+          // and its values have 4 bits or 2
           p[n][0] = transpose8x8(pack2<false>(x[0], x[1]));
           p[n][1] = transpose8x8(pack2<false>(x[2], x[3]));
         }
@@ -594,8 +728,50 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
 
       // O^T += V^T P^T
       const uint32_t values = keys + kTile * Shape::kRowBytes;
+      if constexpr (kFour) {
+        // A lane's byte is two dims of one token, where the operand wants one
+        // dim of two tokens in a register.  So the reduced index goes over pairs
+        // (token, which of the two dims), and the other operand holds the
+        // token's weight beside a 0: two products per step, one for the even
+        // dims and one for the odd ones, on tensor cores that wait anyway, rather
+        // than a byte permutation per register.  Lane 4 i + t: dims i DP / 8 and
+        // on of tokens t, t + 4 and then t + 8, t + 12.
+        constexpr int kWords = DP / 64;  // of a lane's dims of a token
+        constexpr int kGroups = DP > 128 ? 2 : 1;
 #pragma unroll
-      for (int t = 0; t < kSteps; t += kE4m3 ? 2 : 1) {
+        for (int half = 0; half < 2; ++half) {
+          uint32_t w[2][kWords], unit16[2][kGroups];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int tok = (lane & 3) + 4 * i + 8 * half, byte = (lane >> 2) * (DP / 16);
+            load_shared(w[i], values + chunk_offset_four<kChunks, true>(tok, byte / 16) + byte % 16);
+            read_scales<Cache, kGroups>(unit16[i], values + kTile * Shape::kRowBytes + (kTile + tok) * Shape::kScaleBytes,
+                                 DP == 64 ? lane >> 3 : (lane >> 2) * kGroups, scale_at,
+                                 Cache::kOdd ? a.dim / 16 : DP / 16);
+          }
+          uint32_t even[NG][2], odd[NG][2];
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+            even[n][0] = p[n][half] & 0xffffu, even[n][1] = p[n][half] >> 16;
+            odd[n][0] = p[n][half] << 16, odd[n][1] = p[n][half] & 0xffff0000u;
+          }
+#pragma unroll
+          for (int r = 0; r < DP / 32; ++r) {
+            const uint32_t x = w[0][r / 2] >> (16 * (r & 1)), y = w[1][r / 2] >> (16 * (r & 1));
+            const uint32_t f[4] = {mul_f16x2(e2m1_to_f16x2(x), unit16[0][r / 4]),
+                                   mul_f16x2(e2m1_to_f16x2(x >> 8), unit16[0][r / 4]),
+                                   mul_f16x2(e2m1_to_f16x2(y), unit16[1][r / 4]),
+                                   mul_f16x2(e2m1_to_f16x2(y >> 8), unit16[1][r / 4])};
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+              mma16816<false>(acc[n][2 * r], f, even[n][0], even[n][1]);
+              mma16816<false>(acc[n][2 * r + 1], f, odd[n][0], odd[n][1]);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < (kFour ? 0 : kSteps); t += kE4m3 ? 2 : 1) {
         uint32_t f[4];
         if constexpr (!kE4m3) {
           // 8 x 8 pieces: dims 0-7 and 8-15 of tokens 0-7, then of 8-15
@@ -655,6 +831,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
           const float r0 = a.value_scale / l[n][0], r1 = a.value_scale / l[n][1];
           const int h = first + n * 8 + (lane >> 2);
           uint16_t* const out = static_cast<uint16_t*>(a.out) + (row + h) * a.dim;
+          uint32_t even_top = 0, even_bottom = 0;  // (4 bits) of the step before
 #pragma unroll
           for (int t = 0; t < kSteps; ++t) {
             uint32_t top, bottom;
@@ -667,8 +844,23 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
             }
             top = transpose8x8(top);  // now head lane / 4, rows 2 * (lane % 4), + 1
             bottom = transpose8x8(bottom);
+            if constexpr (kFour) {
+              // even dims, then odd ones, of 4 dims in each of two lanes' rows
+              if (t % 2 == 0) {
+                even_top = top, even_bottom = bottom;
+                continue;
+              }
+            }
             if (h >= a.group) continue;
-            if constexpr (!kE4m3) {
+            if constexpr (kFour) {
+              const int d = (lane & 3) * (DP / 4) + 2 * (t - 1);
+              if (d < a.dim)
+                *reinterpret_cast<uint2*>(out + d) =
+                    make_uint2(__byte_perm(even_top, top, 0x5410), __byte_perm(even_bottom, bottom, 0x5410));
+              if (d + DP / 8 < a.dim)
+                *reinterpret_cast<uint2*>(out + d + DP / 8) =
+                    make_uint2(__byte_perm(even_top, top, 0x7632), __byte_perm(even_bottom, bottom, 0x7632));
+            } else if constexpr (!kE4m3) {
               const int d = t * 16 + 2 * (lane & 3);
               if (d < a.dim) *reinterpret_cast<uint32_t*>(out + d) = top;
               if (d + 8 < a.dim) *reinterpret_cast<uint32_t*>(out + d + 8) = bottom;
@@ -701,8 +893,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
           }
 #pragma unroll
           for (int t = 0; t < kSteps; ++t) {
-            const int d0 = kE4m3 ? t * 16 + 2 * (lane >> 2) : t * 16 + (lane >> 2);
-            const int d1 = kE4m3 ? d0 + 1 : d0 + 8;
+            const int d0 = first_dim(t), d1 = d0 + kSecondDim;
             *reinterpret_cast<float2*>(part + d0 * kHeads + h) = make_float2(acc[n][t][0], acc[n][t][1]);
             *reinterpret_cast<float2*>(part + d1 * kHeads + h) = make_float2(acc[n][t][2], acc[n][t][3]);
           }
@@ -745,8 +936,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       }
 #pragma unroll
       for (int t = 0; t < kSteps; ++t) {
-        const int d0 = kE4m3 ? t * 16 + 2 * (lane >> 2) : t * 16 + (lane >> 2);
-        const int d1 = kE4m3 ? d0 + 1 : d0 + 8;
+        const int d0 = first_dim(t), d1 = d0 + kSecondDim;
         *reinterpret_cast<float2*>(mine + d0 * kHeads + h) = make_float2(acc[n][t][0], acc[n][t][1]);
         *reinterpret_cast<float2*>(mine + d1 * kHeads + h) = make_float2(acc[n][t][2], acc[n][t][3]);
       }
@@ -935,7 +1125,8 @@ cudaError_t launch_typed(const AttendArgs& a, void* workspace, uint32_t* arrived
 
 template <typename Cache, int DP>
 size_t workspace_of(int tiles, int sms) {
-  const int64_t warps = static_cast<int64_t>(sms) * step_warps(DP * Cache::kBytes, tiles);
+  const int64_t warps =
+      static_cast<int64_t>(sms) * (tiles == 1 ? StepShape<Cache, DP, 1>::kWarps : StepShape<Cache, DP, 2>::kWarps);
   return tiles == 1 ? StepWorkspace<8, DP * 8>::bytes(warps) : StepWorkspace<16, DP * 16>::bytes(warps);
 }
 
@@ -946,12 +1137,20 @@ int head_tiles(const AttendArgs& a) { return a.group > 8 && a.dim <= 128 ? 2 : 1
 
 }  // namespace
 
-size_t attend_step_workspace(const AttendArgs& a, int sms) {
+template <typename Cache>
+static size_t workspace_cache(const AttendArgs& a, int sms) {
   const int n = head_tiles(a);
-  const bool e4m3 = a.cache_type == KVCA_TYPE_E4M3;
-  if (a.dim <= 64) return e4m3 ? workspace_of<CacheE4m3, 64>(n, sms) : workspace_of<CacheF16, 64>(n, sms);
-  if (a.dim <= 128) return e4m3 ? workspace_of<CacheE4m3, 128>(n, sms) : workspace_of<CacheF16, 128>(n, sms);
-  return e4m3 ? workspace_of<CacheE4m3, 256>(n, sms) : workspace_of<CacheF16, 256>(n, sms);
+  return a.dim <= 64    ? workspace_of<Cache, 64>(n, sms)
+         : a.dim <= 128 ? workspace_of<Cache, 128>(n, sms)
+                        : workspace_of<Cache, 256>(n, sms);
+}
+
+size_t attend_step_workspace(const AttendArgs& a, int sms) {
+  switch (a.cache_type) {
+    case KVCA_TYPE_E4M3: return workspace_cache<CacheE4m3>(a, sms);
+    case KVCA_TYPE_E2M1: return workspace_cache<CacheE2m1<false>>(a, sms);
+    default: return workspace_cache<CacheF16>(a, sms);
+  }
 }
 
 template <typename Cache>
@@ -972,6 +1171,10 @@ cudaError_t launch_attend_step(const AttendArgs& a, void* workspace, uint32_t* a
   switch (a.cache_type) {
     case KVCA_TYPE_F16: return launch_cache<CacheF16>(a, workspace, arrived, sms, stream);
     case KVCA_TYPE_BF16: return launch_cache<CacheBf16>(a, workspace, arrived, sms, stream);
+    case KVCA_TYPE_E2M1:
+      if (a.dim == 64 || a.dim == 128 || a.dim == 256)
+        return launch_cache<CacheE2m1<false>>(a, workspace, arrived, sms, stream);
+      return launch_cache<CacheE2m1<true>>(a, workspace, arrived, sms, stream);
     default: return launch_cache<CacheE4m3>(a, workspace, arrived, sms, stream);
   }
 }

@@ -90,9 +90,9 @@ int to_attend(const kvca_attend_desc* d, int64_t* d_status, kvca::AttendArgs* a)
       d->q_heads % d->kv_heads != 0 || d->head_dim < 8 || d->head_dim > 256)
     return KVCA_ERR_BAD_ARGUMENT;
   if (d->query_type != KVCA_TYPE_F16 && d->query_type != KVCA_TYPE_BF16) return KVCA_ERR_BAD_ARGUMENT;
-  const bool e4m3 = d->cache_type == KVCA_TYPE_E4M3;
-  if (!e4m3 && d->cache_type != d->query_type) return KVCA_ERR_BAD_ARGUMENT;
-  if (d->head_dim % (e4m3 ? 16 : 8) != 0) return KVCA_ERR_BAD_ARGUMENT;
+  const bool e4m3 = d->cache_type == KVCA_TYPE_E4M3, e2m1 = d->cache_type == KVCA_TYPE_E2M1;
+  if (!e4m3 && !e2m1 && d->cache_type != d->query_type) return KVCA_ERR_BAD_ARGUMENT;
+  if (d->head_dim % (e2m1 ? 32 : e4m3 ? 16 : 8) != 0) return KVCA_ERR_BAD_ARGUMENT;
   const uint64_t strides[] = {d->key, d->value, static_cast<uint64_t>(d->key_block_stride),
                               static_cast<uint64_t>(d->key_token_stride), static_cast<uint64_t>(d->key_head_stride),
                               static_cast<uint64_t>(d->value_block_stride),
@@ -110,10 +110,10 @@ int to_attend(const kvca_attend_desc* d, int64_t* d_status, kvca::AttendArgs* a)
   a->value = reinterpret_cast<const char*>(d->value);
   a->key_block = d->key_block_stride;
   a->key_token = d->key_token_stride;
-  a->key_head = d->key_head_stride;
+  a->key_head = e2m1 ? d->head_dim / 2 : d->key_head_stride;
   a->value_block = d->value_block_stride;
   a->value_token = d->value_token_stride;
-  a->value_head = d->value_head_stride;
+  a->value_head = e2m1 ? d->head_dim / 2 : d->value_head_stride;
   a->num_blocks = d->num_blocks;
   a->block_size = static_cast<int>(d->block_size < limit ? d->block_size : limit);
   a->block_shift = -1;
@@ -925,7 +925,7 @@ std::atomic<int64_t> attend_wait_limit{2000000000};
 int to_chunk(const kvca_attend_desc* desc, int64_t num_rows, int64_t* d_status, kvca::AttendArgs* a) {
   const int rc = to_attend(desc, d_status, a);
   if (rc != KVCA_OK) return rc;
-  if (num_rows < 0 || a->dim > kvca::kChunkMaxDim) return KVCA_ERR_BAD_ARGUMENT;
+  if (num_rows < 0 || a->dim > kvca::kChunkMaxDim || a->cache_type == KVCA_TYPE_E2M1) return KVCA_ERR_BAD_ARGUMENT;
   if (num_rows > (int64_t{1} << 30) / desc->q_heads) return KVCA_ERR_SIZE_LIMIT;
   return KVCA_OK;
 }

@@ -1454,7 +1454,7 @@ def compact_pages(slot_meta: torch.Tensor, logical_to_physical: torch.Tensor, ph
 # ---------------------------------------------------------------------------
 
 _ATTEND_TYPES = {torch.float16: _lib.KVCA_TYPE_F16, torch.bfloat16: _lib.KVCA_TYPE_BF16,
-                 torch.float8_e4m3fn: _lib.KVCA_TYPE_E4M3}
+                 torch.float8_e4m3fn: _lib.KVCA_TYPE_E4M3, torch.uint8: _lib.KVCA_TYPE_E2M1}
 _attend_workspace_bytes: dict[tuple, int] = {}
 
 
@@ -1510,24 +1510,28 @@ def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torc
     qtype, ctype = query.dtype, key_cache.dtype
     if qtype is not torch.float16 and qtype is not torch.bfloat16:
         raise TypeError(f"query has incorrect dtype {qtype}")
-    e4m3 = ctype is torch.float8_e4m3fn
-    if not e4m3 and ctype is not qtype:
+    e4m3, four = ctype is torch.float8_e4m3fn, ctype is torch.uint8
+    if not e4m3 and not four and ctype is not qtype:
         raise TypeError(f"key_cache has incorrect dtype {ctype}")
     qshape, kshape = query.shape, key_cache.shape
-    if len(qshape) != 3 or len(kshape) != 4:
+    if len(qshape) != 3 or len(kshape) != 4 and not four:
         raise ValueError("query must be (rows, heads, head_dim) and the caches (num_blocks, block_size, kv_heads, "
                          "head_dim)")
     if value_cache.dtype is not ctype or value_cache.shape != kshape:
         raise ValueError("key_cache and value_cache must share shape and dtype")
     rows, heads, dim = qshape
-    num_blocks, block_size, kv_heads, cache_dim = kshape
-    if cache_dim != dim:
-        raise ValueError(f"the caches' head_dim {cache_dim} is not the query's {dim}")
+    if four:
+        kv_heads = _e2m1_heads(key_cache, dim, "key_cache")
+        num_blocks, block_size = kshape[:2]
+    else:
+        num_blocks, block_size, kv_heads, cache_dim = kshape
+        if cache_dim != dim:
+            raise ValueError(f"the caches' head_dim {cache_dim} is not the query's {dim}")
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError(f"the query heads ({heads}) must be a positive multiple of the K/V heads ({kv_heads})")
     if block_size < 1:
         raise ValueError("block_size must be positive")
-    step = 16 if e4m3 else 8
+    step = 32 if four else 16 if e4m3 else 8
     if dim < step or dim > 256 or dim % step:
         raise ValueError(f"head_dim must be a multiple of {step} up to 256, got {dim}")
     if block_tables.dtype is not torch.int64 or seq_lens.dtype is not torch.int64:
@@ -1545,10 +1549,13 @@ def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torc
     if sinks < 0 or (sinks > 0 if window is None else window < 1):
         raise ValueError("window must be positive (or None) and sinks need a window")
     window = 0 if window is None else int(window)
-    if not e4m3 and (key_scale != 1.0 or value_scale != 1.0):
-        raise ValueError("key_scale and value_scale belong to an e4m3 cache")
+    if not e4m3 and not four and (key_scale != 1.0 or value_scale != 1.0):
+        raise ValueError("key_scale and value_scale belong to a cache of 8 or 4 bits")
     ks = _attend_rows(key_cache, kshape, "key_cache")
     vs = _attend_rows(value_cache, kshape, "value_cache")
+    if four:
+        ks.append(dim // 2)
+        vs.append(dim // 2)
     qs = _attend_rows(query, qshape, "query")
     q_ptr = query.data_ptr()
     q_end = q_ptr + (rows - 1) * qs[0] + (heads - 1) * qs[1] + 2 * dim  # (without rows nothing is written)
