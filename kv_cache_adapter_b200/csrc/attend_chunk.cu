@@ -14,8 +14,8 @@
 //                   tensor memory, running maximum and sum in registers,
 //                   probabilities back to tensor memory, output at the end
 //   warps 8-11      rows of the pages to shared memory (cp.async per 16 bytes,
-//                   so that any block size and stride does; e4m3 is widened on
-//                   the way), 128-byte swizzled as the tensor cores read them
+//                   so that any block size and stride does; e4m3 and e2m1 are widened
+//                   on the way), 128-byte swizzled as the tensor cores read them
 //   warp 12         issues tcgen05.mma: S = Q K^T, O += P V
 //   warp 13         finds the CTA's next segments (block, head, tiles)
 //   warps 14, 15    queries to shared memory
@@ -565,6 +565,11 @@ __device__ __forceinline__ uint32_t drop_nan4(uint32_t word, uint32_t* found) {
   return word & ~((tops >> 7) * 255u);
 }
 
+// Bytes from a head's 4-bit values in a token's row to its scales.
+__device__ __forceinline__ int scales_after(const AttendArgs& a, int head) {
+  return (a.kv_heads - head) * (a.dim / 2) + head * (a.dim / 16);
+}
+
 // Puts the infinite and NaN values of a segment's tiles into the outputs of a
 // softmax warp's rows, one per lane: `out` (16 bits, a whole segment) or `part`
 // (fp32, a share of one).  Of uncut tiles (`uncut`) they take an output's
@@ -581,10 +586,20 @@ __device__ __noinline__ void put_non_finite(const AttendArgs& a, const Share& s,
   const bool has = lane * kOwn < a.dim;
   const bool bf16 = a.query_type == KVCA_TYPE_BF16;
   auto own_of = [&](unsigned long long row, float (&x)[kOwn]) {
+    if constexpr (Cache::kBytes == 0) {
+      const uint8_t* const p = reinterpret_cast<const uint8_t*>(row);
+      const float unit = unpack2<false>(e4m3_to_f16x2(p[scales_after(a, s.head) + lane * kOwn / 16])).x;
+#pragma unroll
+      for (int e = 0; e < kOwn; e += 2) {
+        const float2 f = unpack2<false>(e2m1_to_f16x2(p[(lane * kOwn + e) / 2]));
+        x[e] = f.x * unit, x[e + 1] = f.y * unit;
+      }
+      return;
+    }
     const char* const p = reinterpret_cast<const char*>(row) + lane * kOwn * Cache::kBytes;
 #pragma unroll
     for (int e = 0; e < kOwn; ++e) {
-      if constexpr (Cache::kBytes == 1)
+      if constexpr (Cache::kBytes < 2)
         x[e] = unpack2<false>(e4m3_to_f16x2(reinterpret_cast<const uint8_t*>(p)[e])).x;
       else
         x[e] = unpack2<Cache::kBf16>(reinterpret_cast<const uint16_t*>(p)[e]).x;
@@ -690,7 +705,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     attend_chunk_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ ChunkArgs c, void* workspace) {
   using Shape = ChunkShape<DP>;
   constexpr bool kBf16 = Cache::kBf16;
-  constexpr bool kE4m3 = Cache::kBytes == 1;
+  constexpr bool kFour = Cache::kBytes == 0;
+  constexpr bool kNarrow = Cache::kBytes < 2;  // widened to fp16
   constexpr int kStages = Shape::kStages;
   constexpr int kTileBytes = Shape::kTileBytes;
   constexpr int kQueries = Shape::kQueries;
@@ -900,7 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         const Share& s = shares[segment % kSlots];
         if (s.end == s.tile) break;
-        // Queries.  With e4m3 they go through registers, times a power of two
+        // Queries.  With e4m3 and e2m1 they go through registers, times a power of two
         // per row (power_up); so they do when the sign of a negative
         // scale or the zeros of a zero one go into them.
         if (segment >= kQueries)
@@ -908,7 +924,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         const uint32_t tile = (2 * (segment % kQueries) + w) * kTileBytes;  // of this warp's 128 rows
         float* const unit_of = row_unit[segment % kQueries] + w * 128;
-        const bool as_is = !kE4m3 && c.query_and == 0xffffffffu && c.query_xor == 0u;
+        const bool as_is = !kNarrow && c.query_and == 0xffffffffu && c.query_xor == 0u;
 #pragma unroll 1
         for (int r0 = 0; r0 < 128 && w < s.row_tiles(); r0 += 32) {  // a lane finds one of 32 rows
           const int r = w * 128 + r0 + lane;
@@ -918,7 +934,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool live = r < s.view.rows;
           const unsigned lives = __ballot_sync(0xffffffffu, live);
           const unsigned long long row_at = reinterpret_cast<unsigned long long>(live ? own : a.query);
-          if (!kE4m3) unit_of[r0 + lane] = c.scale_log2;
+          if (!kNarrow) unit_of[r0 + lane] = c.scale_log2;
           if (as_is) {
             const char* src[32 / kPerInstr];
 #pragma unroll
@@ -946,7 +962,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int at = r0 + r1 + i * kPerInstr + sub;
               uint32_t word[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
               float unit = c.scale_log2;
-              if constexpr (kE4m3) {
+              if constexpr (kNarrow) {
                 const bool bf16 = a.query_type == KVCA_TYPE_BF16;
                 float2 f[4];
                 float big = 0.f;
@@ -963,7 +979,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int j = 0; j < 4; ++j) word[j] = pack2<false>(f[j].x * up, f[j].y * up);
                 unit *= power_of_two(-e);
               }
-              if (kE4m3 && chunk == 0) unit_of[at] = unit;
+              if (kNarrow && chunk == 0) unit_of[at] = unit;
 #pragma unroll
               for (int j = 0; j < 4; ++j) word[j] = (word[j] & c.query_and) ^ c.query_xor;
               if (chunk < row_chunks)
@@ -994,7 +1010,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t marks = 0;
       // Hands over the oldest of the tiles in flight.
       auto complete = [&]() {
-        if constexpr (!kE4m3) {
+        if constexpr (!kNarrow) {
           const uint32_t mark = marks >> (4 * (arrived & 7u));
           if (mark & 1u) {
             unsigned char* const tile = smem_ptr + 2 * kQueries * kTileBytes + (arrived % kStages) * kTileBytes;
@@ -1021,12 +1037,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (issued < kStages || !ok) return;
         const uint32_t bar = empty + 8 * (issued % kStages), parity = ((issued / kStages) - 1) & 1;
         if (__all_sync(0xffffffffu, barrier_test(bar, parity))) return;
-        if constexpr (!kE4m3) drain();
+        if constexpr (!kNarrow) drain();
         ok = warp_wait(bar, parity, patience);
       };
       constexpr int64_t kHidden = -1ll << 62;
       for (; ok; ++segment) {
-        if constexpr (!kE4m3) {
+        if constexpr (!kNarrow) {
           // nothing in flight is held back while the next segment is awaited
           if (arrived < issued &&
               !__all_sync(0xffffffffu, barrier_test(announced + 8 * (segment % kSlots), (segment / kSlots) & 1)))
@@ -1063,7 +1079,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (int side = 0; side < 2; ++side) {
             const unsigned long long row = reinterpret_cast<unsigned long long>(side == 0 ? key_row : value_row);
-            if constexpr (!kE4m3) {
+            if constexpr (!kNarrow) {
               claim();
               if (!ok) break;
               const uint32_t dst = kv_smem + (issued % kStages) * kTileBytes;
@@ -1085,6 +1101,48 @@ __global__ void __launch_bounds__(kThreads, 1)
                 cp_async_wait<kAhead>();
                 complete();
               }
+            } else if constexpr (kFour) {
+              // 32 e2m1 values per load, with two scales, become four chunks
+              constexpr int kLoads = kRowChunks / 4;       // per row
+              constexpr int kRowsPer = 32 / kLoads;
+              const int part = lane % kLoads, which = lane / kLoads;
+              const int scales = scales_after(a, s.head) + 2 * part;
+              uint4 x[32 / kRowsPer];
+              uint32_t unit[32 / kRowsPer];
+#pragma unroll
+              for (int i = 0; i < 32 / kRowsPer; ++i) {
+                const int r = i * kRowsPer + which;
+                const char* const from = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, r));
+                const bool read = ((seen >> r) & 1u) && part * 32 < a.dim;
+                x[i] = read ? __ldg(reinterpret_cast<const uint4*>(from) + part) : make_uint4(0, 0, 0, 0);
+                unit[i] = read ? __ldg(reinterpret_cast<const uint16_t*>(from + scales)) : 0;
+              }
+              if (side == 1 && cut) {
+                uint32_t found = 0;
+#pragma unroll
+                for (int i = 0; i < 32 / kRowsPer; ++i) unit[i] = drop_nan4(unit[i], &found);
+                if (found != 0) *const_cast<volatile int*>(&dropped[segment % kSlots]) = 1;
+                __syncwarp();
+              }
+              claim();
+              if (!ok) break;
+              unsigned char* const dst = smem_ptr + 2 * kQueries * kTileBytes + (issued % kStages) * kTileBytes;
+#pragma unroll
+              for (int i = 0; i < 32 / kRowsPer; ++i) {
+                const int r = w * 32 + i * kRowsPer + which;
+                const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                const uint32_t both = e4m3_to_f16x2(unit[i]);
+                const uint32_t factor[2] = {__byte_perm(both, 0, 0x1010), __byte_perm(both, 0, 0x3232)};
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  *reinterpret_cast<uint4*>(dst + place(r, 4 * part + j)) =
+                      make_uint4(mul_f16x2(e2m1_to_f16x2(in[j]), factor[j / 2]),
+                                 mul_f16x2(e2m1_to_f16x2(in[j] >> 8), factor[j / 2]),
+                                 mul_f16x2(e2m1_to_f16x2(in[j] >> 16), factor[j / 2]),
+                                 mul_f16x2(e2m1_to_f16x2(in[j] >> 24), factor[j / 2]));
+              }
+              ++issued;
+              complete();
             } else {
               // 16 e4m3 values per load become two chunks
               constexpr int kLoads = kRowChunks / 2;       // per row
@@ -1130,7 +1188,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         release_segment(segment);
       }
-      if constexpr (!kE4m3) drain();
+      if constexpr (!kNarrow) drain();
       cp_async_wait<0>();
     }
   } else {
@@ -1471,6 +1529,7 @@ cudaError_t launch_attend_chunk(const AttendArgs& args, const int64_t* offsets, 
   switch (a.cache_type) {
     case KVCA_TYPE_F16: return launch_cache<CacheF16>(a, c, workspace, sms, stream);
     case KVCA_TYPE_BF16: return launch_cache<CacheBf16>(a, c, workspace, sms, stream);
+    case KVCA_TYPE_E2M1: return launch_cache<CacheE2m1<false>>(a, c, workspace, sms, stream);
     default: return launch_cache<CacheE4m3>(a, c, workspace, sms, stream);
   }
 }

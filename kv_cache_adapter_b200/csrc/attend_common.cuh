@@ -136,6 +136,12 @@ __device__ __forceinline__ uint32_t e2m1_to_f16x2(uint32_t v) {
   return r;
 }
 
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // Powers of two that bring a row of queries, whose largest magnitude is
 // `big`, into fp16 for the products with e4m3 keys: the largest value falls
 // into [2^12, 2^13), so a bf16 row keeps its bits (values 2^-27 of the largest

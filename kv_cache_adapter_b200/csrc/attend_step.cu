@@ -127,12 +127,6 @@ __device__ __forceinline__ uint32_t load_shared8(uint32_t addr) {
   return v;
 }
 
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-
 // The scales of kGroups groups of a row, each twice in a register: those from
 // `first` on of the row's `groups`, which begin `at` bytes into its place (0
 // unless they are odd); groups beyond have none.

@@ -925,7 +925,7 @@ std::atomic<int64_t> attend_wait_limit{2000000000};
 int to_chunk(const kvca_attend_desc* desc, int64_t num_rows, int64_t* d_status, kvca::AttendArgs* a) {
   const int rc = to_attend(desc, d_status, a);
   if (rc != KVCA_OK) return rc;
-  if (num_rows < 0 || a->dim > kvca::kChunkMaxDim || a->cache_type == KVCA_TYPE_E2M1) return KVCA_ERR_BAD_ARGUMENT;
+  if (num_rows < 0 || a->dim > kvca::kChunkMaxDim) return KVCA_ERR_BAD_ARGUMENT;
   if (num_rows > (int64_t{1} << 30) / desc->q_heads) return KVCA_ERR_SIZE_LIMIT;
   return KVCA_OK;
 }
