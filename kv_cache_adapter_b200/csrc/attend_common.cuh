@@ -136,6 +136,13 @@ __device__ __forceinline__ uint32_t e2m1_to_f16x2(uint32_t v) {
   return r;
 }
 
+// Eight e2m1 values to four times two fp16 values.
+__device__ __forceinline__ void e2m1x8_to_f16x2(uint32_t (&r)[4], uint32_t v) {
+  asm("{\n.reg .b8 a, b, c, d;\nmov.b32 {a, b, c, d}, %4;\ncvt.rn.f16x2.e2m1x2 %0, a;\ncvt.rn.f16x2.e2m1x2 %1, b;\n"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\ncvt.rn.f16x2.e2m1x2 %3, d;\n}"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(v));
+}
+
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));

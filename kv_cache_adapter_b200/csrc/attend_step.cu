@@ -35,7 +35,7 @@
 namespace kvca {
 namespace {
 
-constexpr int kTile = 16;         // tokens per tile: the rows of one m16n8k16
+constexpr int kRows = 16;         // tokens of one m16n8k16
 constexpr int kScanGroups = 1024; // sequences (or runs of them) in the shared tile counts
 // What a segment costs a warp beside its tiles (queries, the output), in
 // tiles.  It counts when the tiles are dealt out, as tiles before the first.
@@ -52,14 +52,17 @@ __host__ __device__ constexpr int step_warps(int row_bytes, int head_tiles) {
 template <typename Cache, int DP, int NG>
 struct StepShape {
   static constexpr bool kFour = Cache::kBytes == 0;
+  // Tokens of a tile: two m16n8k16 of 4-bit values, whose pages are looked up at
+  // once, a token per lane.
+  static constexpr int kTile = kFour ? 2 * kRows : kRows;
   static constexpr int kRowBytes = kFour ? DP / 2 : DP * Cache::kBytes;
   static constexpr int kChunks = kRowBytes / 16;       // 16-byte chunks of a row
   static constexpr int kScaleBytes = !kFour ? 0 : Cache::kOdd ? 32 : DP / 16;  // of a row, after those of all rows
   static constexpr int kStageBytes = 2 * kTile * (kRowBytes + kScaleBytes);
-  static constexpr int kWarps = step_warps(kFour ? DP : kRowBytes, NG);
+  static constexpr int kWarps = kFour ? (DP > 128 || (NG > 1 && DP > 64) ? 8 : 16) : step_warps(kRowBytes, NG);
   static constexpr int kThreads = 32 * kWarps;
-  // 192 KiB of rings per SM
-  static constexpr int kRingBytes = 192 * 1024 / kWarps;
+  // 192 KiB of rings per SM (4 bits: 216, three stages at head dim 128)
+  static constexpr int kRingBytes = (kFour ? 216 : 192) * 1024 / kWarps;
   static constexpr int kStages = kRingBytes / kStageBytes < 8 ? kRingBytes / kStageBytes : 8;
   static constexpr int kHeads = 8 * NG;
   static constexpr int kAcc = DP * kHeads;  // floats of a partial output
@@ -70,7 +73,9 @@ struct StepShape {
   // first one were lost); the largest, 2^15, is within fp16's range.  bf16 ones
   // are held 2^16 times smaller, so that sums of 65,536 of the type's largest
   // values do not overflow.
-  static constexpr float kShift = Cache::kBf16 ? -16.f : 15.f;
+  // 4-bit ones are held times 2^7: their maximum may lag by up to 2^kGrowth.
+  static constexpr float kShift = kFour ? 7.f : Cache::kBf16 ? -16.f : 15.f;
+  static constexpr float kGrowth = 8.f;
   // An infinite value at a token that the query sees is the result, however
   // small its weight: a visible token's weight is never 0 (0 x inf is NaN),
   // nor is that of a partial result.  What the least ones add is below a value's
@@ -95,15 +100,15 @@ __device__ __forceinline__ uint32_t chunk_offset(int r, int c) {
 template <int kChunks, bool kValues>
 __device__ __forceinline__ uint32_t chunk_offset_four(int r, int c) {
   if constexpr (kChunks == 2)  // 32-byte rows: keys with bits 1 and 2 of the row exchanged
-    return static_cast<uint32_t>((kValues ? r : (r & 9) | (r & 2) << 1 | (r & 4) >> 1) * 32 + c * 16);
+    return static_cast<uint32_t>((kValues ? r : (r & ~6) | (r & 2) << 1 | (r & 4) >> 1) * 32 + c * 16);
   else if constexpr (kChunks == 4)  // 64-byte rows: keys with bit 2 in front, values with halves exchanged
     return kValues ? static_cast<uint32_t>(r * 64 + (c ^ (r & 2)) * 16)
-                   : static_cast<uint32_t>(((r & 8) | (r & 3) << 1 | (r & 4) >> 2) * 64 + c * 16);
+                   : static_cast<uint32_t>(((r & ~7) | (r & 3) << 1 | (r & 4) >> 2) * 64 + c * 16);
   else
     return static_cast<uint32_t>(r * 128 + (c ^ (kValues ? (r & 3) << 1 : (r & 4) >> 2)) * 16);
 }
 
-// N = 1, 2, 4 or 8 words of shared memory.
+// N = 1, 2 or 4 words of shared memory.
 template <int N>
 __device__ __forceinline__ void load_shared(uint32_t (&w)[N], uint32_t addr) {
   if constexpr (N == 1)
@@ -134,7 +139,7 @@ template <typename Cache, int kGroups>
 __device__ __forceinline__ void read_scales(uint32_t (&unit)[kGroups], uint32_t addr, int first, int at, int groups) {
   if constexpr (kGroups == 1) {
     const uint32_t v = load_shared8(addr + at + first);
-    unit[0] = e4m3_to_f16x2(__byte_perm(v, 0, 0x4400));
+    unit[0] = e4m3_to_f16x2(v * 0x101u);
   } else {
 #pragma unroll
     for (int j = 0; j < kGroups; j += 2) {
@@ -250,6 +255,7 @@ __device__ __forceinline__ int run_of(int64_t tiles, int64_t runs, int64_t t) {
 }
 
 // A position in the numbering of tiles: sequence, chunk of head groups, tile.
+template <int kTile>
 struct Cursor {
   int seq;
   int chunk;
@@ -297,6 +303,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
   constexpr bool kE4m3 = Cache::kBytes == 1;
   constexpr bool kNarrow = Cache::kBytes < 2;  // widened to fp16
   constexpr bool kTwoTerms = !kNarrow;         // of a probability
+  constexpr int kTile = Shape::kTile;
   constexpr int kChunks = Shape::kChunks;
   constexpr int kStages = Shape::kStages;
   constexpr int kHeads = Shape::kHeads;
@@ -328,7 +335,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
     if (g < groups) {
       const int end = min(a.num_seqs, (g + 1) * per);
       for (int seq = g * per; seq < end; ++seq) {
-        Cursor c;
+        Cursor<Shape::kTile> c;
         c.seq = seq;
         c.load(a);
         n += sequence_share(c.tiles, chunks);
@@ -366,15 +373,17 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
   // earlier run began (slot 0), and of one that this run began (slot 1)
   StepJoin leaves[2] = {{-1, 0, 0}, {-1, 0, 0}};
 
-  // Rows of tile (MMA row lane / 4) and dims of acc[][t]: the first two values
-  // are of dim first_dim(t), the others of the one kSecondDim after it.
-  const int my_token = kFour ? (lane >> 3) + (lane & 4) : lane >> 2;
+  // (4 bits) The token of row lane / 4, and where the head's scales begin in a
+  // row's 32 bytes, if odd.
+  const int my_token = (lane >> 3) + (lane & 4);
+  int scale_at = 0;
+  // The first two values of acc[][t] are of dim first_dim(t), the others of the
+  // one kSecondDim after it.
   constexpr int kSecondDim = kFour ? 2 : kE4m3 ? 1 : 8;
   auto first_dim = [lane](int t) {
     if constexpr (kFour) return (lane >> 2) * (DP / 8) + 4 * (t >> 1) + (t & 1);
     return t * 16 + (kE4m3 ? 2 * (lane >> 2) : lane >> 2);
   };
-  int scale_at = 0;  // (4 bits, odd) where the head's scales begin in a row's 32 bytes
   float acc[NG][kSteps][4];
   float m[NG][2], l[NG][2];  // of the heads 2 * (lane % 4), + 1 of each tile of 8
   // Weight of a token of score s, and of sums whose maximum is `behind` (<= 0) the whole's.
@@ -392,7 +401,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
   if (my_run < runs) {
     const int64_t begin = run_begin(tiles, runs, my_run), finish = run_begin(tiles, runs, my_run + 1);
 
-    Cursor at;  // the tile computed next
+    Cursor<kTile> at;  // the tile computed next
     {
       int lo = 0, hi = groups;
       while (hi - lo > 1) {
@@ -425,16 +434,16 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       __syncwarp();
     }
 
-    // Lane i holds K's row of token i % 16, lane 16 + i V's.  The page of the
-    // next tile is read one iteration before its rows.
-    const int token = lane & 15;
+    // Lane i holds K's row of token i % 16, lane 16 + i V's (4 bits: both of token
+    // i).  The page of the next tile is read one iteration before its rows.
+    const int token = kFour ? lane : lane & 15;
     const bool value_side = lane >= 16;
     const char* const plane = value_side ? a.value : a.key;
     const int64_t block_stride = value_side ? a.value_block : a.key_block;
     const int64_t token_stride = value_side ? a.value_token : a.key_token;
     const int64_t head_stride = value_side ? a.value_head : a.key_head;
     constexpr int64_t kHidden = -1ll << 62;  // no token of this tile
-    Cursor ahead = at;
+    Cursor<kTile> ahead = at;
     bool more = at.left > 0;  // tiles to issue
     int64_t page = kHidden;
     int offset = 0, page_head = 0;
@@ -443,7 +452,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       const int v0 = ahead.tile * kTile, v = v0 + token;
       const int first = ahead.vis.position(v0);
       const int first_offset = a.block_shift >= 0 ? first & (a.block_size - 1) : first % a.block_size;
-      in_page = v0 + kTile <= ahead.vis.count && first_offset + kTile <= a.block_size &&
+      in_page = !kFour && v0 + kTile <= ahead.vis.count && first_offset + kTile <= a.block_size &&
                 ahead.vis.position(v0 + kTile - 1) == first + kTile - 1;
       page = kHidden;
       const int part = ahead.chunk * span + lane_of_heads;
@@ -464,61 +473,108 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       }
     };
     int stage_of = 0;  // ring entry of the next tile issued
-    auto issue = [&]() {
-      if (more) {
-        const bool good = page >= 0 && page < a.num_blocks;
-        if (!good && page != kHidden) report(a.status, KVCA_ERR_BAD_INDEX, page);  // its rows read as zeros
-        const unsigned long long row = reinterpret_cast<unsigned long long>(
-            plane + (good ? page : 0) * block_stride + offset * token_stride + page_head * head_stride);
-        const unsigned seen = __ballot_sync(0xffffffffu, good);
-        const uint32_t stage = ring + stage_of * Shape::kStageBytes;
-        if constexpr (kFour) {
-          // a lane copies its row's scales; where they do not start and end on
-          // a power of two, the 16 bytes that they lie in, or 32
-          const int head_scales = a.dim / 16;
-          const int in_row = a.kv_heads * (a.dim / 2) + page_head * head_scales;
-          const char* const from = plane + (good ? page : 0) * block_stride + offset * token_stride + in_row;
-          const uint32_t to = stage + 2 * kTile * Shape::kRowBytes + lane * Shape::kScaleBytes;
-          if constexpr (Cache::kOdd) {
-            cp_async16(to, from - (in_row & 15), good);
-            if ((in_row & 15) + head_scales > 16) cp_async16(to + 16, from - (in_row & 15) + 16, good);
-          } else if constexpr (Shape::kScaleBytes == 16) {
-            cp_async16(to, from, good);
-          } else {
-            cp_async_small<Shape::kScaleBytes>(to, from, good);
-          }
-        }
-        auto spot = [&](int r, int c) {
-          if constexpr (kFour)
-            return r < kTile ? chunk_offset_four<kChunks, false>(r, c)
-                             : kTile * Shape::kRowBytes + chunk_offset_four<kChunks, true>(r - kTile, c);
-          else
-            return chunk_offset<kChunks>(r, c);
-        };
-        constexpr int kPerInstr = 32 / kChunks > 0 ? 32 / kChunks : 1;
-        const int r0 = kChunks >= 32 ? 0 : lane / kChunks;
-        const int c = lane % kChunks;
-        if (in_page && seen == 0xffffffffu) {
-          // one page: rows at a fixed distance
+    // The rows of 16 tokens, 16 or 8 bits.
+    auto issue_rows = [&]() {
+      const bool good = page >= 0 && page < a.num_blocks;
+      if (!good && page != kHidden) report(a.status, KVCA_ERR_BAD_INDEX, page);  // its rows read as zeros
+      const unsigned long long row = reinterpret_cast<unsigned long long>(
+          plane + (good ? page : 0) * block_stride + offset * token_stride + page_head * head_stride);
+      const unsigned seen = __ballot_sync(0xffffffffu, good);
+      const uint32_t stage = ring + stage_of * Shape::kStageBytes;
+      constexpr int kPerInstr = 32 / kChunks > 0 ? 32 / kChunks : 1;
+      const int r0 = kChunks >= 32 ? 0 : lane / kChunks;
+      const int c = lane % kChunks;
+      if (in_page && seen == 0xffffffffu) {
+        // one page: rows at a fixed distance
 #pragma unroll
-          for (int side = 0; side < 2; ++side) {
-            const int64_t stride = side == 0 ? a.key_token : a.value_token;
-            const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, side * kTile)) + r0 * stride + c * 16;
-            if (c < row_chunks) {
+        for (int side = 0; side < 2; ++side) {
+          const int64_t stride = side == 0 ? a.key_token : a.value_token;
+          const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, side * kTile)) + r0 * stride + c * 16;
+          if (c < row_chunks) {
 #pragma unroll
-              for (int r = 0; r < kTile; r += kPerInstr) {
-                cp_async16(stage + spot(side * kTile + r + r0, c), src);
-                src += kPerInstr * stride;
-              }
+            for (int r = 0; r < kTile; r += kPerInstr) {
+              cp_async16(stage + chunk_offset<kChunks>(side * kTile + r + r0, c), src);
+              src += kPerInstr * stride;
             }
           }
-        } else {
+        }
+      } else {
 #pragma unroll
-          for (int r = 0; r < 2 * kTile; r += kPerInstr) {
-            const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, r + r0)) + c * 16;
-            if (c < row_chunks) cp_async16(stage + spot(r + r0, c), src, (seen >> (r + r0)) & 1u);
+        for (int r = 0; r < 2 * kTile; r += kPerInstr) {
+          const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, r + r0)) + c * 16;
+          if (c < row_chunks) cp_async16(stage + chunk_offset<kChunks>(r + r0, c), src, (seen >> (r + r0)) & 1u);
+        }
+      }
+    };
+    // The rows of 32 tokens, 4 bits, and their scales.
+    auto issue_four = [&]() {
+      const bool good = page >= 0 && page < a.num_blocks;
+      if (!good && page != kHidden) report(a.status, KVCA_ERR_BAD_INDEX, page);  // its rows read as zeros
+      constexpr int kPerInstr = 32 / kChunks;  // rows
+      const int r0 = lane / kChunks, c = lane % kChunks;
+      const uint32_t stage = ring + stage_of * Shape::kStageBytes;
+      const uint32_t values = stage + kTile * Shape::kRowBytes;
+      const int64_t head = page_head * a.key_head;
+      // a lane copies its token's scales; where they do not fill a power of two of
+      // bytes, the 16 bytes that they lie in, or 32
+      const int in_row = a.kv_heads * (a.dim / 2) + page_head * (a.dim / 16);
+      const uint32_t scales = stage + 2 * kTile * Shape::kRowBytes + lane * Shape::kScaleBytes;
+      auto copy_scales = [&](uint32_t to, const char* row) {
+        if constexpr (Cache::kOdd) {
+          const char* const from = row + (in_row & ~15);
+          cp_async16(to, from, good);
+          if ((in_row & 15) + a.dim / 16 > 16) cp_async16(to + 16, from + 16, good);
+        } else if constexpr (Shape::kScaleBytes == 16) {
+          cp_async16(to, row + in_row, good);
+        } else {
+          cp_async_small<Shape::kScaleBytes>(to, row + in_row, good);
+        }
+      };
+      if (a.by_slot) {
+        const int slot = good ? static_cast<int>(page) * a.block_size + offset : -1;
+        const char* const key0 = a.key + head + c * 16;
+        const char* const value0 = a.value + head + c * 16;
+        const int key_token = static_cast<int>(a.key_token), value_token = static_cast<int>(a.value_token);
+#pragma unroll
+        for (int r = 0; r < kTile; r += kPerInstr) {
+          const int from = __shfl_sync(0xffffffffu, slot, r + r0);
+          const int at = max(from, 0);
+          if (c < row_chunks) {
+            cp_async16(stage + chunk_offset_four<kChunks, false>(r + r0, c), key0 + static_cast<int64_t>(at) * key_token, from >= 0);
+            cp_async16(values + chunk_offset_four<kChunks, true>(r + r0, c), value0 + static_cast<int64_t>(at) * value_token,
+                       from >= 0);
           }
         }
+        const int at = max(slot, 0);
+        copy_scales(scales, a.key + static_cast<int64_t>(at) * key_token);
+        copy_scales(scales + kTile * Shape::kScaleBytes, a.value + static_cast<int64_t>(at) * value_token);
+      } else {
+        const int64_t block = good ? page : 0;
+        const char* const key_row = a.key + block * a.key_block + offset * a.key_token;
+        const char* const value_row = a.value + block * a.value_block + offset * a.value_token;
+        const unsigned seen = __ballot_sync(0xffffffffu, good);
+#pragma unroll
+        for (int r = 0; r < kTile; r += kPerInstr) {
+          const unsigned long long k_row = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(key_row), r + r0);
+          const unsigned long long v_row =
+              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(value_row), r + r0);
+          const bool read = (seen >> (r + r0)) & 1u;
+          if (c < row_chunks) {
+            cp_async16(stage + chunk_offset_four<kChunks, false>(r + r0, c), reinterpret_cast<const char*>(k_row) + head + c * 16, read);
+            cp_async16(values + chunk_offset_four<kChunks, true>(r + r0, c), reinterpret_cast<const char*>(v_row) + head + c * 16,
+                       read);
+          }
+        }
+        copy_scales(scales, key_row);
+        copy_scales(scales + kTile * Shape::kScaleBytes, value_row);
+      }
+    };
+    auto issue = [&]() {
+      if (more) {
+        if constexpr (kFour)
+          issue_four();
+        else
+          issue_rows();
         if (++stage_of == kStages) stage_of = 0;
         more = !ahead.last();
         if (more) {
@@ -607,44 +663,16 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       if (++stage_at == kStages) stage_at = 0;
       issue();  // into the stage that the tile before this one left
 
+      // 16 or 8 bits: the 16 tokens of a tile.
+      auto compute_rows = [&]() {
       // S^T = K Q^T, even and odd steps apart for two shorter chains
       float s[NG][2][4];
 #pragma unroll
       for (int n = 0; n < NG; ++n)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[n][0][j] = s[n][1][j] = 0.f;
-      if constexpr (kFour) {
-        // lane 4 i + t: dims t DP / 4 and on of the rows' tokens, four dims per
-        // step, as the query's are above; each value times its scale is exact
-        constexpr int kWords = DP / 32, kRead = kWords > 4 ? 4 : kWords;
-        constexpr int kGroups = DP / 64;  // of 16 dims, of a lane
-        uint32_t w[2][kWords], unit16[2][kGroups];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-          for (int part = 0; part < kWords / kRead; ++part) {
-            uint32_t x[kRead];
-            const int byte = (lane & 3) * (DP / 8) + part * 16;
-            load_shared(x, keys + chunk_offset_four<kChunks, false>(my_token + 8 * i, byte / 16) + byte % 16);
-#pragma unroll
-            for (int j = 0; j < kRead; ++j) w[i][part * kRead + j] = x[j];
-          }
-          read_scales<Cache, kGroups>(unit16[i], keys + 2 * kTile * Shape::kRowBytes + (my_token + 8 * i) * Shape::kScaleBytes,
-                               (lane & 3) * kGroups, scale_at, Cache::kOdd ? a.dim / 16 : DP / 16);
-        }
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-          const uint32_t x = w[0][k / 2] >> (16 * (k & 1)), y = w[1][k / 2] >> (16 * (k & 1));
-          const uint32_t f[4] = {mul_f16x2(e2m1_to_f16x2(x), unit16[0][k / 4]),
-                                 mul_f16x2(e2m1_to_f16x2(y), unit16[1][k / 4]),
-                                 mul_f16x2(e2m1_to_f16x2(x >> 8), unit16[0][k / 4]),
-                                 mul_f16x2(e2m1_to_f16x2(y >> 8), unit16[1][k / 4])};
-#pragma unroll
-          for (int n = 0; n < NG; ++n) mma16816<false>(s[n][k & 1], f, q[n][k][0], q[n][k][1]);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < (kFour ? 0 : kSteps); k += kE4m3 ? 2 : 1) {
+      for (int k = 0; k < kSteps; k += kE4m3 ? 2 : 1) {
         uint32_t f[4];
         if constexpr (!kE4m3) {
           ldmatrix4(f, keys + chunk_offset<kChunks>(lane & 15, 2 * k + (lane >> 4)));
@@ -665,9 +693,9 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
         }
       }
 
-      // softmax over the tile's tokens (rows lane / 4 and + 8: tokens my_token and + 8)
-      const int left = at.vis.count - at.tile * kTile;
-      const bool row0 = my_token < left, row1 = my_token + 8 < left;
+      // softmax over the tile's tokens (rows lane / 4 and + 8)
+      const int left = at.vis.count - at.tile * kRows;
+      const bool row0 = (lane >> 2) < left, row1 = (lane >> 2) + 8 < left;
       uint32_t p[NG][2], p_low[NG][2];
       bool grew = false;
       float decay[NG][2];
@@ -705,8 +733,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
           p_low[n][0] = transpose8x8(pack2<kBf16>(max_nan(x[0] - t.x, Shape::kLeast), max_nan(x[1] - t.y, Shape::kLeast)));
           p_low[n][1] = transpose8x8(pack2<kBf16>(max_nan(x[2] - b.x, Shape::kLeast), max_nan(x[3] - b.y, Shape::kLeast)));
         } else {
-          // one term, to 2^-11: a cache of 8 or 4 bits is bound by instructions,
-          // and its values have 4 bits or 2
+          // one term, to 2^-11: an e4m3 cache is bound by instructions, and its
+          // values have 4 bits
           p[n][0] = transpose8x8(pack2<false>(x[0], x[1]));
           p[n][1] = transpose8x8(pack2<false>(x[2], x[3]));
         }
@@ -721,51 +749,9 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       }
 
       // O^T += V^T P^T
-      const uint32_t values = keys + kTile * Shape::kRowBytes;
-      if constexpr (kFour) {
-        // A lane's byte is two dims of one token, where the operand wants one
-        // dim of two tokens in a register.  So the reduced index goes over pairs
-        // (token, which of the two dims), and the other operand holds the
-        // token's weight beside a 0: two products per step, one for the even
-        // dims and one for the odd ones, on tensor cores that wait anyway, rather
-        // than a byte permutation per register.  Lane 4 i + t: dims i DP / 8 and
-        // on of tokens t, t + 4 and then t + 8, t + 12.
-        constexpr int kWords = DP / 64;  // of a lane's dims of a token
-        constexpr int kGroups = DP > 128 ? 2 : 1;
+      const uint32_t values = keys + kRows * Shape::kRowBytes;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t w[2][kWords], unit16[2][kGroups];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int tok = (lane & 3) + 4 * i + 8 * half, byte = (lane >> 2) * (DP / 16);
-            load_shared(w[i], values + chunk_offset_four<kChunks, true>(tok, byte / 16) + byte % 16);
-            read_scales<Cache, kGroups>(unit16[i], values + kTile * Shape::kRowBytes + (kTile + tok) * Shape::kScaleBytes,
-                                 DP == 64 ? lane >> 3 : (lane >> 2) * kGroups, scale_at,
-                                 Cache::kOdd ? a.dim / 16 : DP / 16);
-          }
-          uint32_t even[NG][2], odd[NG][2];
-#pragma unroll
-          for (int n = 0; n < NG; ++n) {
-            even[n][0] = p[n][half] & 0xffffu, even[n][1] = p[n][half] >> 16;
-            odd[n][0] = p[n][half] << 16, odd[n][1] = p[n][half] & 0xffff0000u;
-          }
-#pragma unroll
-          for (int r = 0; r < DP / 32; ++r) {
-            const uint32_t x = w[0][r / 2] >> (16 * (r & 1)), y = w[1][r / 2] >> (16 * (r & 1));
-            const uint32_t f[4] = {mul_f16x2(e2m1_to_f16x2(x), unit16[0][r / 4]),
-                                   mul_f16x2(e2m1_to_f16x2(x >> 8), unit16[0][r / 4]),
-                                   mul_f16x2(e2m1_to_f16x2(y), unit16[1][r / 4]),
-                                   mul_f16x2(e2m1_to_f16x2(y >> 8), unit16[1][r / 4])};
-#pragma unroll
-            for (int n = 0; n < NG; ++n) {
-              mma16816<false>(acc[n][2 * r], f, even[n][0], even[n][1]);
-              mma16816<false>(acc[n][2 * r + 1], f, odd[n][0], odd[n][1]);
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < (kFour ? 0 : kSteps); t += kE4m3 ? 2 : 1) {
+      for (int t = 0; t < kSteps; t += kE4m3 ? 2 : 1) {
         uint32_t f[4];
         if constexpr (!kE4m3) {
           // 8 x 8 pieces: dims 0-7 and 8-15 of tokens 0-7, then of 8-15
@@ -793,6 +779,164 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
             for (int n = 0; n < NG; ++n) mma16816<false>(acc[n][t + j], w, p[n][0], p[n][1]);
           }
         }
+      }
+      };
+      // 4 bits: 16 of a tile's 32 tokens, from token `sub` on.
+      auto compute_four = [&](int sub) {
+        // S^T = K Q^T.  Lane 4 i + t: dims t DP / 4 and on of the rows' tokens (row i
+        // is token my_token), four dims per step, as the query's are above; a value
+        // times its scale is exact.
+        const uint32_t values = keys + kTile * Shape::kRowBytes;
+        const uint32_t scales = keys + (2 * kTile * Shape::kRowBytes + sub * Shape::kScaleBytes);
+        const int groups = Cache::kOdd ? a.dim / 16 : DP / 16;
+        float s[NG][2][4];
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[n][0][j] = s[n][1][j] = 0.f;
+        {
+          constexpr int kWords = DP / 32, kRead = kWords > 4 ? 4 : kWords;
+          constexpr int kGroups = DP / 64;  // of 16 dims, of a lane
+          uint32_t w[2][kWords], unit16[2][kGroups];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int part = 0; part < kWords / kRead; ++part) {
+              uint32_t x[kRead];
+              const int byte = (lane & 3) * (DP / 8) + part * 16;
+              load_shared(x, keys + sub * Shape::kRowBytes + 8 * i * Shape::kRowBytes +
+                                 chunk_offset_four<kChunks, false>(my_token, byte / 16) + byte % 16);
+#pragma unroll
+              for (int j = 0; j < kRead; ++j) w[i][part * kRead + j] = x[j];
+            }
+            read_scales<Cache, kGroups>(unit16[i], scales + (my_token + 8 * i) * Shape::kScaleBytes,
+                                        (lane & 3) * kGroups, scale_at, groups);
+          }
+#pragma unroll
+          for (int k = 0; k < kSteps; k += 2) {
+            uint32_t x[4], y[4];
+            e2m1x8_to_f16x2(x, w[0][k / 2]);
+            e2m1x8_to_f16x2(y, w[1][k / 2]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              x[j] = mul_f16x2(x[j], unit16[0][k / 4]);
+              y[j] = mul_f16x2(y[j], unit16[1][k / 4]);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t f[4] = {x[2 * j], y[2 * j], x[2 * j + 1], y[2 * j + 1]};
+#pragma unroll
+              for (int n = 0; n < NG; ++n) mma16816<false>(s[n][j], f, q[n][k + j][0], q[n][k + j][1]);
+            }
+          }
+        }
+
+        // Softmax.  The maximum is raised only when a score is past it by more than
+        // kGrowth, so that most tiles need no look across the lanes.
+        const int left = at.vis.count - at.tile * kTile - sub;
+        uint32_t p[NG][2];
+        bool grew = false;
+        float x[NG][4];
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[n][j] = (s[n][0][j] + s[n][1][j]) * unit[n][j & 1];
+          if (left < kRows) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (my_token + (j < 2 ? 0 : 8) >= left) x[n][j] = -INFINITY;
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) grew |= fmaxf(x[n][j], x[n][j + 2]) > m[n][j] + Shape::kGrowth;
+        }
+        if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+            float decay[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float top = fmaxf(x[n][j], x[n][j + 2]);
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+              const float next = fmaxf(m[n][j], top);
+              decay[j] = exp2_approx(m[n][j] - (next == -INFINITY ? 0.f : next));
+              m[n][j] = next;
+              l[n][j] *= decay[j];
+            }
+#pragma unroll
+            for (int t = 0; t < kSteps; ++t)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[n][t][j] *= decay[j & 1];
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float base = (m[n][j] == -INFINITY ? 0.f : m[n][j]) - Shape::kShift;
+            x[n][j] = exp2_approx(x[n][j] - base);
+            x[n][j + 2] = exp2_approx(x[n][j + 2] - base);
+            l[n][j] += x[n][j] + x[n][j + 2];
+          }
+          // one term, to 2^-11: this cache is bound by instructions, and its values
+          // have 2 bits
+          p[n][0] = transpose8x8(pack2<false>(x[n][0], x[n][1]));
+          p[n][1] = transpose8x8(pack2<false>(x[n][2], x[n][3]));
+        }
+
+        // O^T += V^T P^T.  A lane's byte is two dims of one token, where the operand
+        // wants one dim of two tokens in a register.  So the reduced index goes over
+        // pairs (token, which of the two dims), and the other operand holds the
+        // token's weight beside a 0: two products per step, one for the even dims and
+        // one for the odd ones, on tensor cores that wait anyway, rather than a byte
+        // permutation per register.  Lane 4 i + t: dims i DP / 8 and on of tokens t,
+        // t + 4 and then t + 8, t + 12.
+        constexpr int kWords = DP / 64;  // of a lane's dims of a token
+        constexpr int kGroups = DP > 128 ? 2 : 1;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t w[2][kWords], unit16[2][kGroups];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int tok = (lane & 3) + 4 * i + 8 * half, byte = (lane >> 2) * (DP / 16);
+            load_shared(w[i], values + sub * Shape::kRowBytes + chunk_offset_four<kChunks, true>(tok, byte / 16) + byte % 16);
+            read_scales<Cache, kGroups>(unit16[i], scales + (kTile + tok) * Shape::kScaleBytes,
+                                        DP == 64 ? lane >> 3 : (lane >> 2) * kGroups, scale_at, groups);
+          }
+          uint32_t even[NG][2], odd[NG][2];
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+            even[n][0] = p[n][half] & 0xffffu, even[n][1] = p[n][half] >> 16;
+            odd[n][0] = p[n][half] << 16, odd[n][1] = p[n][half] & 0xffff0000u;
+          }
+#pragma unroll
+          for (int r = 0; r < DP / 32; r += 2) {
+            uint32_t x2[4], y2[4];
+            e2m1x8_to_f16x2(x2, w[0][r / 2]);
+            e2m1x8_to_f16x2(y2, w[1][r / 2]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              x2[j] = mul_f16x2(x2[j], unit16[0][r / 4]);
+              y2[j] = mul_f16x2(y2[j], unit16[1][r / 4]);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t f[4] = {x2[2 * j], x2[2 * j + 1], y2[2 * j], y2[2 * j + 1]};
+#pragma unroll
+              for (int n = 0; n < NG; ++n) {
+                mma16816<false>(acc[n][2 * (r + j)], f, even[n][0], even[n][1]);
+                mma16816<false>(acc[n][2 * (r + j) + 1], f, odd[n][0], odd[n][1]);
+              }
+            }
+          }
+        }
+      };
+      if constexpr (kFour) {
+        compute_four(0);
+        if (at.vis.count - at.tile * kTile > kRows) compute_four(kRows);
+      } else {
+        compute_rows();
       }
 
       const bool ends = at.ends();

@@ -138,6 +138,14 @@ int to_attend(const kvca_attend_desc* d, int64_t* d_status, kvca::AttendArgs* a)
   a->lse = d->lse;
   a->query_type = d->query_type;
   a->cache_type = d->cache_type;
+  if (d->block_size == 1) {  // every offset is 0
+    a->key_token = a->key_block;
+    a->value_token = a->value_block;
+  }
+  const int64_t most = int64_t{1} << 31;
+  a->by_slot = e2m1 && d->block_size < most && d->num_blocks < most / d->block_size && a->key_token < most &&
+               a->value_token < most && a->key_token >= 0 && a->value_token >= 0 &&
+               a->key_block == d->block_size * a->key_token && a->value_block == d->block_size * a->value_token;
   a->status = d_status;
   // without blocks no row is read, but rows that are not read get an address
   if (d->num_blocks == 0) a->key = a->value = static_cast<const char*>(a->query);
@@ -1024,7 +1032,9 @@ int kvca_rotate_tokens(const kvca_rotate_desc* d, int64_t* d_status, kvca_stream
   a.interleaved = d->interleaved != 0;
   a.transpose = d->transpose != 0;
   a.status = d_status;
-  return status_of(kvca::launch_rotate_tokens(a, d->type, stream));
+  const int sms = kvca_device_sm_count();
+  if (sms < 1) return KVCA_ERR_CUDA;
+  return status_of(kvca::launch_rotate_tokens(a, d->type, sms, stream));
 }
 
 int kvca_append_tokens(const kvca_append_desc* d, int64_t* d_status, kvca_stream_t stream) {
@@ -1096,7 +1106,9 @@ int kvca_append_tokens(const kvca_append_desc* d, int64_t* d_status, kvca_stream
   a.key_scale = d->key_scale;
   a.value_scale = d->value_scale;
   a.status = d_status;
-  return status_of(kvca::launch_append_tokens(a, d->type, d->cache_type, stream));
+  const int sms = kvca_device_sm_count();
+  if (sms < 1) return KVCA_ERR_CUDA;
+  return status_of(kvca::launch_append_tokens(a, d->type, d->cache_type, sms, stream));
 }
 
 int kvca_read_tokens(const kvca_read_desc* d, int64_t* d_status, kvca_stream_t stream) {

@@ -143,6 +143,9 @@ struct AttendArgs {
   float* lse;  // (rows, heads), dense, or null
   int query_type;
   int cache_type;
+  // (4 bits) Token rows of both sides at slot * token stride, slots and strides
+  // below 2^31.
+  bool by_slot;
   int64_t* status;
 };
 
@@ -192,12 +195,13 @@ struct TokenArgs {
   int q_heads, kv_heads, dim, rotary;
   bool interleaved, transpose;
   float key_scale, value_scale;
-  int token_warps;  // that share a token (the launchers set it)
+  int token_warps;  // that share a token, and those of them that take its queries
+  int query_warps;  // alone (the launchers set both)
   int64_t* status;
 };
 
-cudaError_t launch_append_tokens(const TokenArgs& args, int type, int cache_type, cudaStream_t stream);
-cudaError_t launch_rotate_tokens(const TokenArgs& args, int type, cudaStream_t stream);
+cudaError_t launch_append_tokens(const TokenArgs& args, int type, int cache_type, int sms, cudaStream_t stream);
+cudaError_t launch_rotate_tokens(const TokenArgs& args, int type, int sms, cudaStream_t stream);
 
 // Rows of a cache of 8 or 4 bits to read as wider values (out: dense).
 struct ReadArgs {

@@ -9,12 +9,11 @@
 // (no fused multiply-add), so that the values to be stored in few bits do not
 // depend on how an expression was compiled.
 //
-// A warp takes some rows (heads) of one token at a time, a lane 8 neighbouring
-// dims (16 where they are stored in 4 bits: one group with a scale) and keeps
-// its angles for the next rows of the token.  Each output is computed from its
-// own value and its pair's, both loaded (the second comes from the first-level
-// cache), so that one form does for every layout; a row never leaves its warp,
-// so its place may be its result's.
+// A warp takes some rows (heads) of one token at a time and keeps the angles for
+// its next rows.  Where pairs are half the rotary dims apart, a lane holds both
+// sides of 8 of them, so each value is loaded once and its place may be its
+// result's; neighbouring pairs (and pairs at odd distances) lie 8 dims to a lane,
+// 16 where they are stored in 4 bits: a group with its scale.
 
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -31,23 +30,44 @@ struct InF32 {
   static constexpr int kBytes = 4;
 };
 
-// 8 neighbouring values, 16-byte aligned.
+// 8 values as they lie in memory, and as floats.
 template <typename In>
-__device__ __forceinline__ void load8(const char* p, float (&x)[8]) {
-  if constexpr (In::kBytes == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 16);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-    x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+struct Raw8 {
+  uint4 w[In::kBytes / 2 > 0 ? In::kBytes / 2 : 1];
+
+  __device__ __forceinline__ void load(const char* p) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = unpack2<In::kBf16>(w[j]);
-      x[2 * j] = f.x, x[2 * j + 1] = f.y;
+    for (int j = 0; j < In::kBytes / 2; ++j) w[j] = *reinterpret_cast<const uint4*>(p + 16 * j);
+  }
+  __device__ __forceinline__ void store(char* p) const {
+#pragma unroll
+    for (int j = 0; j < In::kBytes / 2; ++j) *reinterpret_cast<uint4*>(p + 16 * j) = w[j];
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    if constexpr (In::kBytes == 4) {
+      x[0] = __uint_as_float(w[0].x), x[1] = __uint_as_float(w[0].y);
+      x[2] = __uint_as_float(w[0].z), x[3] = __uint_as_float(w[0].w);
+      x[4] = __uint_as_float(w[1].x), x[5] = __uint_as_float(w[1].y);
+      x[6] = __uint_as_float(w[1].z), x[7] = __uint_as_float(w[1].w);
+    } else {
+      const uint32_t v[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = unpack2<In::kBf16>(v[j]);
+        x[2 * j] = f.x, x[2 * j + 1] = f.y;
+      }
     }
   }
-}
+  __device__ __forceinline__ void set(const float (&x)[8]) {
+    if constexpr (In::kBytes == 4) {
+      w[0] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+      w[1] = make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
+    } else {
+      w[0] = make_uint4(pack2<In::kBf16>(x[0], x[1]), pack2<In::kBf16>(x[2], x[3]), pack2<In::kBf16>(x[4], x[5]),
+                        pack2<In::kBf16>(x[6], x[7]));
+    }
+  }
+};
 
 template <typename In>
 __device__ __forceinline__ float load1(const char* p) {
@@ -57,110 +77,127 @@ __device__ __forceinline__ float load1(const char* p) {
     return unpack2<In::kBf16>(*reinterpret_cast<const uint16_t*>(p)).x;
 }
 
-template <typename Out>
-__device__ __forceinline__ void store8(char* p, const float (&x)[8]) {
-  if constexpr (Out::kBytes == 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-    *reinterpret_cast<float4*>(p + 16) = make_float4(x[4], x[5], x[6], x[7]);
-  } else {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack2<Out::kBf16>(x[0], x[1]), pack2<Out::kBf16>(x[2], x[3]),
-                                              pack2<Out::kBf16>(x[4], x[5]), pack2<Out::kBf16>(x[6], x[7]));
-  }
-}
-
 // ---------------------------------------------------------------------------
 // Rotation
 // ---------------------------------------------------------------------------
 
 enum TurnMode {
-  kTurnNone,
-  kTurnHalves,       // pairs (i, i + rotary / 2), rotary / 2 a multiple of 8
-  kTurnHalvesLoose,  // the same, any rotary / 2
-  kTurnPairs,        // pairs (2 i, 2 i + 1)
-};
-
-// The angles of dims d0 .. d0 + 7 and where their pairs are.
-template <int kMode>
-struct Turn8 {
-  static constexpr int kAngles = kMode == kTurnPairs ? 4 : 8;
-  float c[kAngles], s[kAngles];  // s with the sign that an output's pair takes
-  int other[kMode == kTurnHalvesLoose ? 8 : 1];  // dims to the pair's value
-  unsigned on;                                   // a bit per angle: rotated
-
-  __device__ __forceinline__ void load(const TokenArgs& a, const float* angles, int d0) {
-    const int half = a.rotary / 2;
-    const float sign = a.transpose ? -1.f : 1.f;
-    on = 0;
-    if constexpr (kMode == kTurnHalves) {
-      const bool second = d0 >= half;
-      other[0] = second ? -half : half;
-      if (d0 >= a.rotary) return;
-      on = 0xffu;
-      const int i = second ? d0 - half : d0;
-#pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        const float4 cc = __ldg(reinterpret_cast<const float4*>(angles + i + e));
-        const float4 ss = __ldg(reinterpret_cast<const float4*>(angles + half + i + e));
-        c[e] = cc.x, c[e + 1] = cc.y, c[e + 2] = cc.z, c[e + 3] = cc.w;
-        const float side = second ? sign : -sign;
-        s[e] = ss.x * side, s[e + 1] = ss.y * side, s[e + 2] = ss.z * side, s[e + 3] = ss.w * side;
-      }
-    } else if constexpr (kMode == kTurnHalvesLoose) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = d0 + e;
-        const bool second = d >= half;
-        const int i = second ? d - half : d;
-        other[e] = second ? -half : half;
-        c[e] = 1.f, s[e] = 0.f;
-        if (d >= a.rotary) continue;
-        on |= 1u << e;
-        c[e] = __ldg(angles + i);
-        s[e] = __ldg(angles + half + i) * (second ? sign : -sign);
-      }
-    } else if constexpr (kMode == kTurnPairs) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = d0 / 2 + e;
-        c[e] = 1.f, s[e] = 0.f;
-        if (i >= half) continue;
-        on |= 1u << e;
-        c[e] = __ldg(angles + i);
-        s[e] = __ldg(angles + half + i) * sign;
-      }
-    }
-  }
+  kTurnHalves,  // pairs (i, i + rotary / 2) with rotary / 2 a multiple of 8 (4 bits: of 16): a lane has both sides
+  kTurnLoose,   // the same at any distance, or no rotation
+  kTurnPairs,   // pairs (2 i, 2 i + 1)
 };
 
 __device__ __forceinline__ float turned(float own, float c, float pair, float s) {
   return __fadd_rn(__fmul_rn(own, c), __fmul_rn(pair, s));
 }
 
-// x: dims d0 .. d0 + 7 of the row at p, rotated.
-template <typename In, int kMode>
-__device__ __forceinline__ void load_turned(const char* row, int d0, const Turn8<kMode>& t, float (&x)[8]) {
-  load8<In>(row + d0 * In::kBytes, x);
-  if constexpr (kMode == kTurnHalves) {
-    if (t.on == 0) return;
-    float y[8];
-    load8<In>(row + (d0 + t.other[0]) * In::kBytes, y);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = turned(x[e], t.c[e], y[e], t.s[e]);
-  } else if constexpr (kMode == kTurnHalvesLoose) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if ((t.on >> e) & 1u) x[e] = turned(x[e], t.c[e], load1<In>(row + (d0 + e + t.other[e]) * In::kBytes), t.s[e]);
-  } else if constexpr (kMode == kTurnPairs) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float y = turned(x[2 * e], t.c[e], x[2 * e + 1], -t.s[e]);
-      const float z = turned(x[2 * e + 1], t.c[e], x[2 * e], t.s[e]);
-      const bool on = (t.on >> e) & 1u;
-      x[2 * e] = on ? y : x[2 * e];
-      x[2 * e + 1] = on ? z : x[2 * e + 1];
+// A lane's share of a row: 8 dims from `first` on, and in kTurnHalves the 8 that
+// they turn with (4 bits, other modes: the 8 after them).
+template <int kMode, bool kWide>
+struct Lane8 {
+  static constexpr int kParts = kMode == kTurnHalves || kWide ? 2 : 1;  // of 8 dims
+  static constexpr int kAngles = kMode == kTurnPairs ? 4 * kParts : 8;
+  int lanes;    // per row
+  int first;
+  int second;   // dims of the other part, or -1
+  bool turns;   // (kTurnHalves) both parts by the angles
+  float c[kAngles], s[kAngles];
+  unsigned on;  // (other modes) a bit per angle or dim: rotated
+
+  __device__ __forceinline__ void place(const TokenArgs& a, int lane) {
+    const int half = a.rotary / 2;
+    if constexpr (kMode == kTurnHalves) {
+      const int pairs = half / 8;
+      lanes = pairs + (a.dim - a.rotary) / 8;
+      const int at = lane % lanes;
+      turns = at < pairs;
+      first = turns ? at * 8 : a.rotary + (at - pairs) * 8;
+      second = turns ? first + half : -1;
+    } else {
+      lanes = a.dim / (8 * kParts);
+      first = lane % lanes * 8 * kParts;
+      second = kParts == 2 ? first + 8 : -1;
     }
   }
-}
+  __device__ __forceinline__ void load(const TokenArgs& a, const float* angles) {
+    const int half = a.rotary / 2;
+    on = 0;
+    if constexpr (kMode == kTurnHalves) {
+      if (!turns) return;
+      const float sign = a.transpose ? -1.f : 1.f;
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const float4 cc = __ldg(reinterpret_cast<const float4*>(angles + first + e));
+        const float4 ss = __ldg(reinterpret_cast<const float4*>(angles + half + first + e));
+        c[e] = cc.x, c[e + 1] = cc.y, c[e + 2] = cc.z, c[e + 3] = cc.w;
+        s[e] = ss.x * sign, s[e + 1] = ss.y * sign, s[e + 2] = ss.z * sign, s[e + 3] = ss.w * sign;
+      }
+    } else if constexpr (kMode == kTurnPairs) {
+#pragma unroll
+      for (int e = 0; e < kAngles; ++e) {
+        const int i = first / 2 + e;
+        c[e] = 1.f, s[e] = 0.f;
+        if (i >= half) continue;
+        on |= 1u << e;
+        c[e] = __ldg(angles + i);
+        s[e] = a.transpose ? -__ldg(angles + half + i) : __ldg(angles + half + i);
+      }
+    }
+  }
+
+  // The parts of the row at p, rotated; those that stay, as they were.
+  template <typename In>
+  __device__ __forceinline__ void rotate(const TokenArgs& a, const char* p, const float* angles,
+                                         Raw8<In> (&raw)[kParts], float (&x)[kParts][8], bool keep_floats) {
+#pragma unroll
+    for (int j = 0; j < kParts; ++j) raw[j].get(x[j]);
+    if constexpr (kMode == kTurnHalves) {
+      if (!turns) return;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = turned(x[0][e], c[e], x[1][e], -s[e]);
+        x[1][e] = turned(x[1][e], c[e], x[0][e], s[e]);
+        x[0][e] = y;
+      }
+      if (keep_floats) return;
+      raw[0].set(x[0]);
+      raw[1].set(x[1]);
+    } else if constexpr (kMode == kTurnPairs) {
+#pragma unroll
+      for (int j = 0; j < kParts; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = j * 4 + e;
+          const float y = turned(x[j][2 * e], c[k], x[j][2 * e + 1], -s[k]);
+          const float z = turned(x[j][2 * e + 1], c[k], x[j][2 * e], s[k]);
+          const bool turn = (on >> k) & 1u;
+          x[j][2 * e] = turn ? y : x[j][2 * e];
+          x[j][2 * e + 1] = turn ? z : x[j][2 * e + 1];
+        }
+      if (keep_floats) return;
+#pragma unroll
+      for (int j = 0; j < kParts; ++j)
+        if ((on >> (4 * j)) & 15u) raw[j].set(x[j]);
+    } else {
+      if (angles == nullptr) return;
+      const int half = a.rotary / 2;
+#pragma unroll
+      for (int j = 0; j < kParts; ++j) {
+        if (first + 8 * j >= a.rotary) continue;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int d = first + 8 * j + e;
+          if (d >= a.rotary) continue;
+          const bool back = d >= half;
+          const float sine = __ldg(angles + (back ? d : d + half));
+          x[j][e] = turned(x[j][e], __ldg(angles + (back ? d - half : d)),
+                           load1<In>(p + (back ? d - half : d + half) * In::kBytes), back != a.transpose ? sine : -sine);
+        }
+        if (!keep_floats) raw[j].set(x[j]);
+      }
+    }
+  }
+};
 
 // ---------------------------------------------------------------------------
 // 8 and 4 bits
@@ -183,26 +220,47 @@ __device__ __forceinline__ uint32_t to_e2m1x2(float lo, float hi) {
 
 __device__ __forceinline__ float e4m3_to_float(uint32_t byte) { return unpack2<false>(e4m3_to_f16x2(byte)).x; }
 
-// 16 values as codes with one scale, which is chosen so that the largest
-// becomes 6, the largest code.  A NaN makes the scale and so all of them NaN;
-// what lies beyond 6 times the largest scale is cut off.
-__device__ __forceinline__ uint2 to_codes(const float (&x)[2][8], float factor, uint32_t* scale) {
+// x / b for a rounding to few bits, from r, the rounded reciprocal of b: the
+// product's remainder corrects it (Markstein's correction).  A quotient that is
+// a midpoint of the few bits comes out exactly: with x = t b the remainder of
+// q = t + d is -d b, exactly, and the correction leaves d r b, 2^-24 of d.  Any
+// other is off by 2^-46 before its rounding.  Where q is past `most`, which the
+// rounding cuts off anyway, it stays, as it may be infinite.
+__device__ __forceinline__ float quotient(float x, float b, float r, float most) {
+  const float q = x * r;
+  const float better = __fmaf_rn(__fmaf_rn(-q, b, x), r, q);
+  return fabsf(q) < most ? better : q;
+}
+
+__device__ __forceinline__ uint2 to_e4m3x8(const float (&x)[8], float scale, float reciprocal) {
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    w[e] = to_e4m3x2(quotient(x[2 * e], scale, reciprocal, 512.f), quotient(x[2 * e + 1], scale, reciprocal, 512.f));
+  return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+}
+
+__device__ __forceinline__ float largest8(const float (&x)[8]) {
   float big = 0.f;
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int e = 0; e < 8; ++e) big = max_nan(big, fabsf(x[e]));
+  return big;
+}
+
+// The scale of a group whose largest magnitude is `big`: that one becomes 6, the
+// largest code.  A NaN makes it, and so all values of the group, NaN; what lies
+// beyond 6 times the largest scale is cut off.
+__device__ __forceinline__ uint32_t scale_of(float big, float factor) {
+  return to_e4m3x2(__fdiv_rn(big, 6.f * factor), 0.f) & 0xffu;
+}
+
+// 8 values as codes; zeros where the scale is 0 or NaN.
+__device__ __forceinline__ uint32_t to_codes(const float (&x)[8], float unit, float reciprocal) {
+  uint32_t word = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) big = max_nan(big, fabsf(x[j][e]));
-  *scale = to_e4m3x2(__fdiv_rn(big, 6.f * factor), 0.f) & 0xffu;
-  const float unit = e4m3_to_float(*scale) * factor;
-  uint32_t word[2] = {0, 0};
-  if (unit > 0.f) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; e += 2)
-        word[j] |= to_e2m1x2(__fdiv_rn(x[j][e], unit), __fdiv_rn(x[j][e + 1], unit)) << (4 * e);
-  }
-  return make_uint2(word[0], word[1]);
+  for (int e = 0; e < 8; e += 2)
+    word |= to_e2m1x2(quotient(x[e], unit, reciprocal, 8.f), quotient(x[e + 1], unit, reciprocal, 8.f)) << (4 * e);
+  return unit > 0.f ? word : 0u;
 }
 
 // ---------------------------------------------------------------------------
@@ -242,128 +300,173 @@ __device__ __forceinline__ TokenPlace place_of(const TokenArgs& a, int64_t token
   return t;
 }
 
-// Cache: the type that keys and values are stored in; In where nothing is.
-template <typename In, typename Cache, int kMode, bool kStores>
-__global__ void __launch_bounds__(32 * kTokenWarps) token_rows_kernel(const __grid_constant__ TokenArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t warp = static_cast<int64_t>(blockIdx.x) * kTokenWarps + (threadIdx.x >> 5);
-  const int64_t token = warp / a.token_warps;
-  const int part = static_cast<int>(warp - token * a.token_warps);
-  if (token >= a.rows) return;
-  const TokenPlace place = place_of<kStores>(a, token);
-  if (!place.live) return;
-  constexpr bool kFour = kStores && Cache::kBytes == 0;
-
-  {
-    // rows of 8 dims per lane: queries, then (unless stored in 4 bits) keys
-    const int lanes = a.dim / 8, rows = 32 / lanes;
-    const int row_of = lane / lanes, d0 = (lane - row_of * lanes) * 8;
-    const int heads = a.q_heads + (kStores && !kFour ? a.kv_heads : 0);
-    if (part * rows < heads) {
-      Turn8<kMode> turn;
-      turn.load(a, place.angles, d0);
-      for (int r = part * rows; r < heads; r += a.token_warps * rows) {
-        const int h = r + row_of;
-        const bool mine = row_of < rows && h < heads;
-        const bool is_query = h < a.q_heads;
-        float x[8];
-        const char* const from = is_query ? a.query + token * a.query_row + h * a.query_head
-                                          : a.key + token * a.key_row + (h - a.q_heads) * a.key_head;
-        if (mine) load_turned<In, kMode>(from, d0, turn, x);
-        __syncwarp();  // a row's place may be its result's
-        if (!mine) continue;
-        if (is_query) {
-          store8<In>(a.query_out + token * a.query_out_row + h * a.query_out_head + d0 * In::kBytes, x);
-        } else if constexpr (kStores && !kFour) {
-          char* const to = a.key_cache + place.block * a.key_cache_block + place.offset * a.key_cache_token +
-                           (h - a.q_heads) * a.key_cache_head + d0 * Cache::kBytes;
-          if constexpr (Cache::kBytes == 1) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = to_e4m3x2(__fdiv_rn(x[2 * e], a.key_scale), __fdiv_rn(x[2 * e + 1], a.key_scale));
-            *reinterpret_cast<uint2*>(to) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
-          } else {
-            store8<Cache>(to, x);
-          }
-        }
-      }
-    }
-    if constexpr (kStores && !kFour) {
-      for (int r = part * rows; r < a.kv_heads; r += a.token_warps * rows) {
-        const int h = r + row_of;
-        if (row_of >= rows || h >= a.kv_heads) continue;
-        const char* const from = a.value + token * a.value_row + h * a.value_head + d0 * In::kBytes;
-        char* const to = a.value_cache + place.block * a.value_cache_block + place.offset * a.value_cache_token +
-                         h * a.value_cache_head + d0 * Cache::kBytes;
-        if constexpr (Cache::kBytes == 1) {
-          float x[8];
-          load8<In>(from, x);
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = to_e4m3x2(__fdiv_rn(x[2 * e], a.value_scale), __fdiv_rn(x[2 * e + 1], a.value_scale));
-          *reinterpret_cast<uint2*>(to) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
-        } else {
-          *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
-        }
-      }
-    }
-  }
-  if constexpr (kFour) {
-    // a group of 16 dims per lane, keys and then values
-    const int lanes = a.dim / 16, rows = 32 / lanes;
-    const int row_of = lane / lanes, group = lane - row_of * lanes;
-    const int64_t codes = static_cast<int64_t>(a.kv_heads) * (a.dim / 2);
-    if (part * rows >= 2 * a.kv_heads) return;
-    Turn8<kMode> turn[2];
-    turn[0].load(a, place.angles, group * 16);
-    turn[1].load(a, place.angles, group * 16 + 8);
-    for (int r = part * rows; r < 2 * a.kv_heads; r += a.token_warps * rows) {
-      int h = r + row_of;
-      if (row_of >= rows || h >= 2 * a.kv_heads) continue;
-      const bool is_key = h < a.kv_heads;
-      float x[2][8];
-      char* to;
-      if (is_key) {
-        const char* const from = a.key + token * a.key_row + h * a.key_head;
-        load_turned<In, kMode>(from, group * 16, turn[0], x[0]);
-        load_turned<In, kMode>(from, group * 16 + 8, turn[1], x[1]);
-        to = a.key_cache + place.block * a.key_cache_block + place.offset * a.key_cache_token;
-      } else {
-        h -= a.kv_heads;
-        const char* const from = a.value + token * a.value_row + h * a.value_head + group * 16 * In::kBytes;
-        load8<In>(from, x[0]);
-        load8<In>(from + 8 * In::kBytes, x[1]);
-        to = a.value_cache + place.block * a.value_cache_block + place.offset * a.value_cache_token;
-      }
-      uint32_t scale;
-      const uint2 word = to_codes(x, is_key ? a.key_scale : a.value_scale, &scale);
-      *reinterpret_cast<uint2*>(to + h * (a.dim / 2) + group * 8) = word;
-      *reinterpret_cast<uint8_t*>(to + codes + h * (a.dim / 16) + group) = static_cast<uint8_t>(scale);
-    }
-  }
-}
-
 struct CacheE2m1Rows {
   static constexpr int kBytes = 0;  // less than one
 };
 
-template <typename In, typename Cache, bool kStores>
-cudaError_t launch_rows(const TokenArgs& a, cudaStream_t stream) {
+// Cache: the type that keys and values are stored in; In where nothing is.
+// kWide: 16 dims to a lane, for the keys and values of a 4-bit cache; its
+// queries then are rows of a warp of their own kind (8 dims to a lane).
+template <typename In, typename Cache, int kMode, bool kStores, bool kWide>
+__device__ __forceinline__ void token_rows(const TokenArgs& a, int64_t token, int part, int parts) {
+  constexpr bool kFour = kStores && Cache::kBytes == 0;
+  using Lane = Lane8<kMode, kWide>;
+  constexpr int kParts = Lane::kParts;
+  const int lane = threadIdx.x & 31;
+  Lane at;
+  at.place(a, lane);
+  const int rows = 32 / at.lanes, row_of = lane / at.lanes;
+  // heads of queries, keys and values in turn
+  const int begin = kWide && kMode != kTurnHalves ? a.q_heads : 0;
+  const int keys = a.q_heads, values = keys + a.kv_heads;
+  const int end = kFour && !kWide && kMode != kTurnHalves ? a.q_heads : kStores ? values + a.kv_heads : a.q_heads;
+  const TokenPlace place = place_of<kStores>(a, token);
+  if (!place.live) return;
+  if (begin + part * rows >= end) return;
+  at.load(a, place.angles);
+  float key_reciprocal = 0.f, value_reciprocal = 0.f;
+  if constexpr (kStores && Cache::kBytes == 1) {
+    key_reciprocal = __frcp_rn(a.key_scale);
+    value_reciprocal = __frcp_rn(a.value_scale);
+  }
+  for (int r = begin + part * rows; r < end; r += parts * rows) {
+    const int h = r + row_of;
+    const bool mine = row_of < rows && h < end;
+    const bool is_query = h < keys, is_value = h >= values;
+    const char* from = nullptr;
+    Raw8<In> raw[kParts];
+    if (mine) {
+      from = is_query ? a.query + token * a.query_row + h * a.query_head
+             : is_value ? a.value + token * a.value_row + (h - values) * a.value_head
+                        : a.key + token * a.key_row + (h - keys) * a.key_head;
+      raw[0].load(from + at.first * In::kBytes);
+      if constexpr (kParts == 2)
+        if (at.second >= 0) raw[1].load(from + at.second * In::kBytes);
+    }
+    float x[kParts][8];
+    if (mine) {
+      if (!is_value) {
+        at.template rotate<In>(a, from, place.angles, raw, x, !is_query && (kFour || (kStores && Cache::kBytes == 1)));
+      } else if constexpr (kStores && Cache::kBytes < 2) {
+#pragma unroll
+        for (int j = 0; j < kParts; ++j) raw[j].get(x[j]);
+      }
+    }
+    if constexpr (kMode == kTurnLoose) __syncwarp();  // another lane's values have been read: their place may be the result's
+    if constexpr (!kStores) {
+      if (!mine) continue;
+      char* const to = a.query_out + token * a.query_out_row + h * a.query_out_head;
+      raw[0].store(to + at.first * In::kBytes);
+      if constexpr (kParts == 2)
+        if (at.second >= 0) raw[1].store(to + at.second * In::kBytes);
+    } else {
+      float big[kParts];
+      if constexpr (kFour && (kMode == kTurnHalves || kWide)) {
+        if constexpr (kMode == kTurnHalves) {
+          // a group is two neighbouring lanes' parts
+#pragma unroll
+          for (int j = 0; j < kParts; ++j) {
+            big[j] = mine && !is_query ? largest8(x[j]) : 0.f;
+            big[j] = max_nan(big[j], __shfl_xor_sync(0xffffffffu, big[j], 1));
+          }
+        } else {
+          big[0] = mine ? max_nan(largest8(x[0]), largest8(x[1])) : 0.f;
+          big[1] = big[0];
+        }
+      }
+      if (!mine) continue;
+      if (is_query) {
+        char* const to = a.query_out + token * a.query_out_row + h * a.query_out_head;
+        raw[0].store(to + at.first * In::kBytes);
+        if constexpr (kParts == 2)
+          if (at.second >= 0) raw[1].store(to + at.second * In::kBytes);
+        continue;
+      }
+      const int head = is_value ? h - values : h - keys;
+      char* const row = is_value
+                            ? a.value_cache + place.block * a.value_cache_block + place.offset * a.value_cache_token
+                            : a.key_cache + place.block * a.key_cache_block + place.offset * a.key_cache_token;
+      const float scale = is_value ? a.value_scale : a.key_scale;
+      if constexpr (kFour) {
+        if constexpr (kMode == kTurnHalves || kWide) {
+          const int64_t codes = static_cast<int64_t>(a.kv_heads) * (a.dim / 2);
+#pragma unroll
+          for (int j = 0; j < kParts; ++j) {
+            const int d = j == 0 ? at.first : at.second;
+            if (d < 0) continue;
+            const uint32_t byte = scale_of(big[j], scale);
+            const float unit = e4m3_to_float(byte) * scale;
+            *reinterpret_cast<uint32_t*>(row + head * (a.dim / 2) + d / 2) = to_codes(x[j], unit, __frcp_rn(unit));
+            if (d % 16 == 0)
+              *reinterpret_cast<uint8_t*>(row + codes + head * (a.dim / 16) + d / 16) = static_cast<uint8_t>(byte);
+          }
+        }
+      } else {
+        char* const to = row + head * (is_value ? a.value_cache_head : a.key_cache_head);
+        if constexpr (Cache::kBytes == 1) {
+          const float reciprocal = is_value ? value_reciprocal : key_reciprocal;
+          *reinterpret_cast<uint2*>(to + at.first) = to_e4m3x8(x[0], scale, reciprocal);
+          if constexpr (kParts == 2)
+            if (at.second >= 0) *reinterpret_cast<uint2*>(to + at.second) = to_e4m3x8(x[1], scale, reciprocal);
+        } else {
+          raw[0].store(to + at.first * In::kBytes);
+          if constexpr (kParts == 2)
+            if (at.second >= 0) raw[1].store(to + at.second * In::kBytes);
+        }
+      }
+    }
+  }
+}
+
+template <typename In, typename Cache, int kMode, bool kStores>
+__global__ void __launch_bounds__(32 * kTokenWarps) token_rows_kernel(const __grid_constant__ TokenArgs a) {
+  const int64_t warp = static_cast<int64_t>(blockIdx.x) * kTokenWarps + (threadIdx.x >> 5);
+  const int64_t token = warp / a.token_warps;
+  const int part = static_cast<int>(warp - token * a.token_warps);
+  if (token >= a.rows) return;
+  if constexpr (kStores && Cache::kBytes == 0 && kMode != kTurnHalves) {
+    if (part < a.query_warps)
+      token_rows<In, Cache, kMode, kStores, false>(a, token, part, a.query_warps);
+    else
+      token_rows<In, Cache, kMode, kStores, true>(a, token, part - a.query_warps, a.token_warps - a.query_warps);
+  } else {
+    token_rows<In, Cache, kMode, kStores, false>(a, token, part, a.token_warps);
+  }
+}
+
+// Warps of a token for so many of its rows, in turns of `rows`: one turn each
+// while that leaves SMs without work, three else (the angles are loaded once).
+int warps_for(int64_t tokens, int heads, int rows, int sms) {
+  const int turns = (heads + rows - 1) / rows;
+  return tokens * turns <= static_cast<int64_t>(sms) * 16 ? turns : (turns + 2) / 3;
+}
+
+template <typename In, typename Cache, int kMode, bool kStores>
+cudaError_t launch_mode(TokenArgs a, int sms, cudaStream_t stream) {
+  constexpr bool kFour = kStores && Cache::kBytes == 0;
+  const int kv = kStores ? 2 * a.kv_heads : 0;
+  if constexpr (kMode == kTurnHalves) {
+    const int lanes = a.rotary / 16 + (a.dim - a.rotary) / 8;
+    a.token_warps = warps_for(a.rows, a.q_heads + kv, 32 / lanes, sms);
+  } else if constexpr (kFour) {
+    a.query_warps = a.q_heads > 0 ? warps_for(a.rows, a.q_heads, 32 / (a.dim / 8), sms) : 0;
+    a.token_warps = a.query_warps + warps_for(a.rows, kv, 32 / (a.dim / 16), sms);
+  } else {
+    a.token_warps = warps_for(a.rows, a.q_heads + kv, 32 / (a.dim / 8), sms);
+  }
   const int64_t warps = a.rows * a.token_warps;
   const dim3 grid(static_cast<unsigned>((warps + kTokenWarps - 1) / kTokenWarps));
-  const int half = a.rotary / 2;
-  if (a.table == nullptr) {
-    if constexpr (kStores) token_rows_kernel<In, Cache, kTurnNone, kStores><<<grid, 32 * kTokenWarps, 0, stream>>>(a);
-  } else if (a.interleaved) {
-    token_rows_kernel<In, Cache, kTurnPairs, kStores><<<grid, 32 * kTokenWarps, 0, stream>>>(a);
-  } else if (half % 8 == 0) {
-    token_rows_kernel<In, Cache, kTurnHalves, kStores><<<grid, 32 * kTokenWarps, 0, stream>>>(a);
-  } else {
-    token_rows_kernel<In, Cache, kTurnHalvesLoose, kStores><<<grid, 32 * kTokenWarps, 0, stream>>>(a);
-  }
+  token_rows_kernel<In, Cache, kMode, kStores><<<grid, 32 * kTokenWarps, 0, stream>>>(a);
   return cudaGetLastError();
+}
+
+template <typename In, typename Cache, bool kStores>
+cudaError_t launch_rows(const TokenArgs& a, int sms, cudaStream_t stream) {
+  const int step = kStores && Cache::kBytes == 0 ? 16 : 8;
+  if (a.table != nullptr && a.interleaved) return launch_mode<In, Cache, kTurnPairs, kStores>(a, sms, stream);
+  if (a.table != nullptr && a.rotary / 2 % step == 0)
+    return launch_mode<In, Cache, kTurnHalves, kStores>(a, sms, stream);
+  return launch_mode<In, Cache, kTurnLoose, kStores>(a, sms, stream);
 }
 
 // ---------------------------------------------------------------------------
@@ -405,7 +508,9 @@ __global__ void __launch_bounds__(256) read_rows_kernel(const __grid_constant__ 
       x[2 * e] = f.x * a.scale, x[2 * e + 1] = f.y * a.scale;
     }
   }
-  store8<Out>(a.out + (token * lanes + at) * 8 * Out::kBytes, x);
+  Raw8<Out> raw;
+  raw.set(x);
+  raw.store(a.out + (token * lanes + at) * 8 * Out::kBytes);
 }
 
 template <typename Out>
@@ -419,41 +524,24 @@ cudaError_t launch_read_to(const ReadArgs& a, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
-// Warps that share a token's heads, each with several rows of them.
-int warps_of(const TokenArgs& a, bool four, bool stores) {
-  const int rows = 32 / (a.dim / 8);
-  const int wide = a.q_heads + (stores && !four ? a.kv_heads : 0);
-  int items = (wide + rows - 1) / rows;
-  if (four) {
-    const int narrow = 32 / (a.dim / 16);
-    const int more = (2 * a.kv_heads + narrow - 1) / narrow;
-    items = items > more ? items : more;
-  }
-  return items;
-}
-
 }  // namespace
 
-cudaError_t launch_append_tokens(const TokenArgs& args, int type, int cache_type, cudaStream_t stream) {
-  TokenArgs a = args;
-  a.token_warps = warps_of(a, cache_type == KVCA_TYPE_E2M1, true);
+cudaError_t launch_append_tokens(const TokenArgs& a, int type, int cache_type, int sms, cudaStream_t stream) {
   if (type == KVCA_TYPE_F16) {
-    if (cache_type == KVCA_TYPE_E4M3) return launch_rows<CacheF16, CacheE4m3, true>(a, stream);
-    if (cache_type == KVCA_TYPE_E2M1) return launch_rows<CacheF16, CacheE2m1Rows, true>(a, stream);
-    return launch_rows<CacheF16, CacheF16, true>(a, stream);
+    if (cache_type == KVCA_TYPE_E4M3) return launch_rows<CacheF16, CacheE4m3, true>(a, sms, stream);
+    if (cache_type == KVCA_TYPE_E2M1) return launch_rows<CacheF16, CacheE2m1Rows, true>(a, sms, stream);
+    return launch_rows<CacheF16, CacheF16, true>(a, sms, stream);
   }
-  if (cache_type == KVCA_TYPE_E4M3) return launch_rows<CacheBf16, CacheE4m3, true>(a, stream);
-  if (cache_type == KVCA_TYPE_E2M1) return launch_rows<CacheBf16, CacheE2m1Rows, true>(a, stream);
-  return launch_rows<CacheBf16, CacheBf16, true>(a, stream);
+  if (cache_type == KVCA_TYPE_E4M3) return launch_rows<CacheBf16, CacheE4m3, true>(a, sms, stream);
+  if (cache_type == KVCA_TYPE_E2M1) return launch_rows<CacheBf16, CacheE2m1Rows, true>(a, sms, stream);
+  return launch_rows<CacheBf16, CacheBf16, true>(a, sms, stream);
 }
 
-cudaError_t launch_rotate_tokens(const TokenArgs& args, int type, cudaStream_t stream) {
-  TokenArgs a = args;
-  a.token_warps = warps_of(a, false, false);
+cudaError_t launch_rotate_tokens(const TokenArgs& a, int type, int sms, cudaStream_t stream) {
   switch (type) {
-    case KVCA_TYPE_F16: return launch_rows<CacheF16, CacheF16, false>(a, stream);
-    case KVCA_TYPE_BF16: return launch_rows<CacheBf16, CacheBf16, false>(a, stream);
-    default: return launch_rows<InF32, InF32, false>(a, stream);
+    case KVCA_TYPE_F16: return launch_rows<CacheF16, CacheF16, false>(a, sms, stream);
+    case KVCA_TYPE_BF16: return launch_rows<CacheBf16, CacheBf16, false>(a, sms, stream);
+    default: return launch_rows<InF32, InF32, false>(a, sms, stream);
   }
 }
 

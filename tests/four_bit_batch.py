@@ -25,14 +25,14 @@ class Batch(attend_oracle.Batch):
             self.rows.append(rows)
             setattr(self, name, token_oracle.values(rows, heads, dim))
 
-    def expect(self, p_eps, *, least=2.0 ** -40, **kw):
-        """As before, with what weights far below the largest may be off.  They are fp16, held times 2^15 of the running
-        maximum (2^7 in chunks, whose maximum lags by up to 2^8): a step of 2^-24 there, half of it rounded away, over a
-        sum of 2^15 (2^7) at least, is 2^-40 (2^-32) of each value that a query sees.  It shows here because 4-bit values
-        are often 0, where a tiny weight of another token is all of a result."""
+    def expect(self, p_eps, **kw):
+        """As before, with what weights far below the largest may be off.  They are fp16, held times 2^7 of a maximum that
+        lags by up to 2^8: a step of 2^-24 there, half of it rounded away, over a sum of 2^7 at least, is 2^-32 of each
+        value that a query sees.  It shows here because 4-bit values are often 0, where a tiny weight of another token is
+        all of a result."""
         rows, (out, lse, bound, lse_bound) = super().expect(p_eps, **kw)
         top = self.value.nan_to_num().abs().max().item() * self.scales.get("value_scale", 1.0)
-        return rows, (out, lse, bound + max(self.lens) * top * least, lse_bound)
+        return rows, (out, lse, bound + max(self.lens) * top * 2.0 ** -32, lse_bound)
 
     def on(self, dev):
         if self.layout == "merged":
