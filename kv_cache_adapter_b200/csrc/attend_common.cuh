@@ -84,13 +84,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// The same for 4 or 8 bytes.
-template <int kSize>
-__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, bool read) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kSize), "r"(read ? kSize : 0)
-               : "memory");
-}
-
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
@@ -160,6 +153,100 @@ __device__ __forceinline__ int power_up(float big) {
 }
 
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+
+// ---------------------------------------------------------------------------
+// Barriers in shared memory
+// ---------------------------------------------------------------------------
+
+constexpr uint32_t kTryTime = 20000;       // ns that a try of a wait may suspend its thread, after the first
+constexpr uint32_t kWaitTries = 1u << 24;  // the second bound of a wait, beside its time
+
+__device__ __forceinline__ void barrier_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+
+// Arrives, and adds bytes to the phase that copies of them are to bring.
+__device__ __forceinline__ void barrier_arrive_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+// `bytes` (a multiple of 16, like both addresses) from global to shared memory,
+// counted at `bar` when they are there.
+__device__ __forceinline__ void copy_bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void barrier_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// Whether a phase is over; suspends the thread for a short while if not (the
+// hardware's choice; `time` nanoseconds or so in the second form).
+__device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+
+__device__ __forceinline__ bool barrier_try_for(uint32_t bar, uint32_t parity, uint32_t time) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done) : "r"(bar), "r"(parity), "r"(time) : "memory");
+  return done != 0;
+}
+
+__device__ __forceinline__ uint64_t now_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  return t;
+}
+
+// Whether a phase is over, without the suspension of a try.
+__device__ __forceinline__ bool barrier_test(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+
+// How long the CTA's waits may take, and whether one of them gave up.
+struct Patience {
+  volatile int* gave_up;
+  int64_t limit;  // ns
+};
+
+// The wait for a phase whose first try was in vain (with the time and the
+// tries bounded here, not in line, drafted tokens took 51.3 us, not 55.5).
+__device__ __noinline__ bool barrier_wait_on(uint32_t bar, uint32_t parity, volatile int* gave_up, int64_t limit) {
+  const uint64_t start = now_ns();
+  for (uint32_t i = 0; i < kWaitTries; ++i) {
+    if (*gave_up) return false;
+    if (static_cast<int64_t>(now_ns() - start) >= limit) break;
+    if (barrier_try_for(bar, parity, kTryTime)) return true;
+  }
+  *gave_up = 1;
+  return false;
+}
+
+// Waits for a phase; gives up, as every other warp of the CTA then does within
+// kTryTime, after the limit or once another warp gave up.
+__device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, const Patience& patience) {
+  return barrier_try(bar, parity) || barrier_wait_on(bar, parity, patience.gave_up, patience.limit);
+}
+
+// The same for a whole warp: every lane waits, and all go on or none.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const Patience& patience) {
+  return __all_sync(0xffffffffu, barrier_wait(bar, parity, patience));
+}
+
+// ---------------------------------------------------------------------------
+// Sequences
+// ---------------------------------------------------------------------------
 
 // The tokens that the query at the end of a sequence of `len` tokens sees,
 // numbered 0 .. count - 1: the first `sinks` ones, then those of the window.

@@ -29,13 +29,13 @@
 #include <stdint.h>
 #include <string.h>
 
-#include "attend_common.cuh"
+#include "attend_step_common.cuh"
 #include "kvca_host.cuh"
 
 namespace kvca {
 namespace {
 
-constexpr int kRows = 16;         // tokens of one m16n8k16
+constexpr int kTile = 16;         // tokens per tile: the rows of one m16n8k16
 constexpr int kScanGroups = 1024; // sequences (or runs of them) in the shared tile counts
 // What a segment costs a warp beside its tiles (queries, the output), in
 // tiles.  It counts when the tiles are dealt out, as tiles before the first.
@@ -51,18 +51,13 @@ __host__ __device__ constexpr int step_warps(int row_bytes, int head_tiles) {
 // DP: head dim padded to 64, 128 or 256; NG: tiles of 8 query heads.
 template <typename Cache, int DP, int NG>
 struct StepShape {
-  static constexpr bool kFour = Cache::kBytes == 0;
-  // Tokens of a tile: two m16n8k16 of 4-bit values, whose pages are looked up at
-  // once, a token per lane.
-  static constexpr int kTile = kFour ? 2 * kRows : kRows;
-  static constexpr int kRowBytes = kFour ? DP / 2 : DP * Cache::kBytes;
+  static constexpr int kRowBytes = DP * Cache::kBytes;
   static constexpr int kChunks = kRowBytes / 16;       // 16-byte chunks of a row
-  static constexpr int kScaleBytes = !kFour ? 0 : Cache::kOdd ? 32 : DP / 16;  // of a row, after those of all rows
-  static constexpr int kStageBytes = 2 * kTile * (kRowBytes + kScaleBytes);
-  static constexpr int kWarps = kFour ? (DP > 128 || (NG > 1 && DP > 64) ? 8 : 16) : step_warps(kRowBytes, NG);
+  static constexpr int kStageBytes = 2 * kTile * kRowBytes;
+  static constexpr int kWarps = step_warps(kRowBytes, NG);
   static constexpr int kThreads = 32 * kWarps;
-  // 192 KiB of rings per SM (4 bits: 216, three stages at head dim 128)
-  static constexpr int kRingBytes = (kFour ? 216 : 192) * 1024 / kWarps;
+  // 192 KiB of rings per SM
+  static constexpr int kRingBytes = 192 * 1024 / kWarps;
   static constexpr int kStages = kRingBytes / kStageBytes < 8 ? kRingBytes / kStageBytes : 8;
   static constexpr int kHeads = 8 * NG;
   static constexpr int kAcc = DP * kHeads;  // floats of a partial output
@@ -73,9 +68,7 @@ struct StepShape {
   // first one were lost); the largest, 2^15, is within fp16's range.  bf16 ones
   // are held 2^16 times smaller, so that sums of 65,536 of the type's largest
   // values do not overflow.
-  // 4-bit ones are held times 2^7: their maximum may lag by up to 2^kGrowth.
-  static constexpr float kShift = kFour ? 7.f : Cache::kBf16 ? -16.f : 15.f;
-  static constexpr float kGrowth = 8.f;
+  static constexpr float kShift = Cache::kBf16 ? -16.f : 15.f;
   // An infinite value at a token that the query sees is the result, however
   // small its weight: a visible token's weight is never 0 (0 x inf is NaN),
   // nor is that of a partial result.  What the least ones add is below a value's
@@ -94,67 +87,6 @@ __device__ __forceinline__ uint32_t chunk_offset(int r, int c) {
     return static_cast<uint32_t>((r * kChunks + (c ^ ((r >> 1) & 3))) * 16);
 }
 
-// The same for rows of 4-bit values, whose lanes read as described at their
-// products: keys a quarter row of token (i / 2) + 4 (i % 2), i = lane / 4;
-// values an eighth of a row of token lane % 4 (+ 4, 8, 12).
-template <int kChunks, bool kValues>
-__device__ __forceinline__ uint32_t chunk_offset_four(int r, int c) {
-  if constexpr (kChunks == 2)  // 32-byte rows: keys with bits 1 and 2 of the row exchanged
-    return static_cast<uint32_t>((kValues ? r : (r & ~6) | (r & 2) << 1 | (r & 4) >> 1) * 32 + c * 16);
-  else if constexpr (kChunks == 4)  // 64-byte rows: keys with bit 2 in front, values with halves exchanged
-    return kValues ? static_cast<uint32_t>(r * 64 + (c ^ (r & 2)) * 16)
-                   : static_cast<uint32_t>(((r & ~7) | (r & 3) << 1 | (r & 4) >> 2) * 64 + c * 16);
-  else
-    return static_cast<uint32_t>(r * 128 + (c ^ (kValues ? (r & 3) << 1 : (r & 4) >> 2)) * 16);
-}
-
-// N = 1, 2 or 4 words of shared memory.
-template <int N>
-__device__ __forceinline__ void load_shared(uint32_t (&w)[N], uint32_t addr) {
-  if constexpr (N == 1)
-    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(addr) : "memory");
-  else if constexpr (N == 2)
-    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
-  else
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
-}
-
-__device__ __forceinline__ uint32_t load_shared16(uint32_t addr) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
-  return v;
-}
-
-__device__ __forceinline__ uint32_t load_shared8(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
-
-// The scales of kGroups groups of a row, each twice in a register: those from
-// `first` on of the row's `groups`, which begin `at` bytes into its place (0
-// unless they are odd); groups beyond have none.
-template <typename Cache, int kGroups>
-__device__ __forceinline__ void read_scales(uint32_t (&unit)[kGroups], uint32_t addr, int first, int at, int groups) {
-  if constexpr (kGroups == 1) {
-    const uint32_t v = load_shared8(addr + at + first);
-    unit[0] = e4m3_to_f16x2(v * 0x101u);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kGroups; j += 2) {
-      const uint32_t v = e4m3_to_f16x2(load_shared16(addr + at + first + j));
-      unit[j] = __byte_perm(v, 0, 0x1010);
-      unit[j + 1] = __byte_perm(v, 0, 0x3232);
-    }
-  }
-  if constexpr (Cache::kOdd) {
-#pragma unroll
-    for (int j = 0; j < kGroups; ++j)
-      if (first + j >= groups) unit[j] = 0;
-  }
-}
-
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -163,24 +95,6 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
-  return r;
-}
-
-template <bool kBf16>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (kBf16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // How a call's work lies on the warps: `span` warps side by side share a run,
@@ -210,100 +124,13 @@ struct StepLayout {
   }
 };
 
-// A segment that several runs share leaves one result per CTA (its first run's
-// place) and one from the run that ends it, unless that is a CTA's first.
-__device__ __forceinline__ int result_count(int first_run, int last_run, int groups) {
-  const int cta = first_run / groups, last_cta = last_run / groups;
-  return last_cta - cta + 1 + (cta == last_cta || last_run != last_cta * groups ? 1 : 0);
-}
-
-__device__ __forceinline__ int result_run(int k, int first_run, int last_run, int groups) {
-  const int cta = first_run / groups, last_cta = last_run / groups;
-  return k == 0 ? first_run : k <= last_cta - cta ? (cta + k) * groups : last_run;
-}
-
-// The workspace: two partial results per warp, slot 0 for a segment that an
-// earlier run began, slot 1 for one that this warp's run began.
-template <int kHeads, int kAcc>
-struct StepWorkspace {
-  float* ml;   // [warp][slot][2][heads]: maxima, then sums
-  float* acc;  // [warp][slot][dim][heads]
-
-  static __host__ __device__ size_t bytes(int64_t warps) {
-    return static_cast<size_t>(warps) * 2 * (2 * kHeads + kAcc) * sizeof(float);
-  }
-  __host__ __device__ StepWorkspace(void* base, int64_t warps) {
-    acc = static_cast<float*>(base);
-    ml = acc + warps * 2 * kAcc;
-  }
-  __device__ __forceinline__ float* ml_of(int64_t warp, int slot) const { return ml + (warp * 2 + slot) * 2 * kHeads; }
-  __device__ __forceinline__ float* acc_of(int64_t warp, int slot) const { return acc + (warp * 2 + slot) * kAcc; }
-};
-
-// A segment to join.
-struct StepJoin {
-  int segment;
-  int first_run, last_run;
-};
-
-__device__ __forceinline__ int64_t run_begin(int64_t tiles, int64_t runs, int64_t r) {
-  return tiles * r / runs;  // below 2^31 tiles x a few thousand runs
-}
-
-__device__ __forceinline__ int run_of(int64_t tiles, int64_t runs, int64_t t) {
-  return static_cast<int>((runs * (t + 1) - 1) / tiles);
-}
-
-// A position in the numbering of tiles: sequence, chunk of head groups, tile.
-template <int kTile>
-struct Cursor {
-  int seq;
-  int chunk;
-  int tile;
-  int tiles;  // of this sequence's visible tokens
-  int left;   // of the run, this tile included; none when <= 0
-  Visible vis;
-
-  __device__ __forceinline__ void load(const AttendArgs& a) {
-    vis = visible_tokens(max(sequence_length(a, seq), 0), a.window, a.sinks);
-    tiles = (vis.count + kTile - 1) / kTile;
-  }
-  __device__ __forceinline__ bool ends() const { return tile + 1 == tiles; }
-  __device__ __forceinline__ bool last() const { return left <= (ends() ? 1 + kSegmentCost : 1); }
-  // To the next tile; only when this one is not the last.
-  __device__ __forceinline__ void advance(const AttendArgs& a, int chunks) {
-    --left;
-    if (++tile < tiles) return;
-    tile = 0;
-    left -= kSegmentCost;
-    if (++chunk < chunks) return;
-    chunk = 0;
-    do {
-      if (++seq >= a.num_seqs) {  // not while the lengths stay as they were counted
-        left = 0;
-        --seq;
-        return;
-      }
-      load(a);
-    } while (tiles == 0);
-  }
-};
-
-// The shares a sequence's segments take of the numbering.
-__device__ __forceinline__ int64_t sequence_share(int tiles, int chunks) {
-  return tiles > 0 ? static_cast<int64_t>(tiles + kSegmentCost) * chunks : 0;
-}
-
 template <typename Cache, int DP, int NG>
 __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
     attend_step_kernel(const __grid_constant__ AttendArgs a, void* workspace, uint32_t* arrived) {
   using Shape = StepShape<Cache, DP, NG>;
   constexpr bool kBf16 = Cache::kBf16;
-  constexpr bool kFour = Shape::kFour;
   constexpr bool kE4m3 = Cache::kBytes == 1;
-  constexpr bool kNarrow = Cache::kBytes < 2;  // widened to fp16
-  constexpr bool kTwoTerms = !kNarrow;         // of a probability
-  constexpr int kTile = Shape::kTile;
+  constexpr bool kTwoTerms = !kE4m3;  // of a probability
   constexpr int kChunks = Shape::kChunks;
   constexpr int kStages = Shape::kStages;
   constexpr int kHeads = Shape::kHeads;
@@ -335,10 +162,10 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
     if (g < groups) {
       const int end = min(a.num_seqs, (g + 1) * per);
       for (int seq = g * per; seq < end; ++seq) {
-        Cursor<Shape::kTile> c;
+        Cursor<kTile, kSegmentCost> c;
         c.seq = seq;
         c.load(a);
-        n += sequence_share(c.tiles, chunks);
+        n += sequence_share<kSegmentCost>(c.tiles, chunks);
       }
     }
     int64_t total;
@@ -373,17 +200,6 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
   // earlier run began (slot 0), and of one that this run began (slot 1)
   StepJoin leaves[2] = {{-1, 0, 0}, {-1, 0, 0}};
 
-  // (4 bits) The token of row lane / 4, and where the head's scales begin in a
-  // row's 32 bytes, if odd.
-  const int my_token = (lane >> 3) + (lane & 4);
-  int scale_at = 0;
-  // The first two values of acc[][t] are of dim first_dim(t), the others of the
-  // one kSecondDim after it.
-  constexpr int kSecondDim = kFour ? 2 : kE4m3 ? 1 : 8;
-  auto first_dim = [lane](int t) {
-    if constexpr (kFour) return (lane >> 2) * (DP / 8) + 4 * (t >> 1) + (t & 1);
-    return t * 16 + (kE4m3 ? 2 * (lane >> 2) : lane >> 2);
-  };
   float acc[NG][kSteps][4];
   float m[NG][2], l[NG][2];  // of the heads 2 * (lane % 4), + 1 of each tile of 8
   // Weight of a token of score s, and of sums whose maximum is `behind` (<= 0) the whole's.
@@ -401,7 +217,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
   if (my_run < runs) {
     const int64_t begin = run_begin(tiles, runs, my_run), finish = run_begin(tiles, runs, my_run + 1);
 
-    Cursor<kTile> at;  // the tile computed next
+    Cursor<kTile, kSegmentCost> at;  // the tile computed next
     {
       int lo = 0, hi = groups;
       while (hi - lo > 1) {
@@ -411,8 +227,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       int64_t rest = begin - prefix[lo];
       at.seq = lo * per;
       at.load(a);
-      while (rest >= sequence_share(at.tiles, chunks) && at.seq + 1 < a.num_seqs) {
-        rest -= sequence_share(at.tiles, chunks);
+      while (rest >= sequence_share<kSegmentCost>(at.tiles, chunks) && at.seq + 1 < a.num_seqs) {
+        rest -= sequence_share<kSegmentCost>(at.tiles, chunks);
         ++at.seq;
         at.load(a);
       }
@@ -427,23 +243,23 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
     }
 
     const uint32_t ring = smem_addr(rings) + warp * (kStages * Shape::kStageBytes);
-    const int row_chunks = kFour ? a.dim / 32 : a.dim * Cache::kBytes / 16;
+    const int row_chunks = a.dim * Cache::kBytes / 16;
     if (row_chunks < kChunks) {  // the padded dims stay zero: no copy writes them
       for (int i = lane; i < kStages * Shape::kStageBytes / 16; i += 32)
         *reinterpret_cast<uint4*>(rings + warp * (kStages * Shape::kStageBytes) + i * 16) = make_uint4(0, 0, 0, 0);
       __syncwarp();
     }
 
-    // Lane i holds K's row of token i % 16, lane 16 + i V's (4 bits: both of token
-    // i).  The page of the next tile is read one iteration before its rows.
-    const int token = kFour ? lane : lane & 15;
+    // Lane i holds K's row of token i % 16, lane 16 + i V's.  The page of the
+    // next tile is read one iteration before its rows.
+    const int token = lane & 15;
     const bool value_side = lane >= 16;
     const char* const plane = value_side ? a.value : a.key;
     const int64_t block_stride = value_side ? a.value_block : a.key_block;
     const int64_t token_stride = value_side ? a.value_token : a.key_token;
     const int64_t head_stride = value_side ? a.value_head : a.key_head;
     constexpr int64_t kHidden = -1ll << 62;  // no token of this tile
-    Cursor<kTile> ahead = at;
+    Cursor<kTile, kSegmentCost> ahead = at;
     bool more = at.left > 0;  // tiles to issue
     int64_t page = kHidden;
     int offset = 0, page_head = 0;
@@ -452,7 +268,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       const int v0 = ahead.tile * kTile, v = v0 + token;
       const int first = ahead.vis.position(v0);
       const int first_offset = a.block_shift >= 0 ? first & (a.block_size - 1) : first % a.block_size;
-      in_page = !kFour && v0 + kTile <= ahead.vis.count && first_offset + kTile <= a.block_size &&
+      in_page = v0 + kTile <= ahead.vis.count && first_offset + kTile <= a.block_size &&
                 ahead.vis.position(v0 + kTile - 1) == first + kTile - 1;
       page = kHidden;
       const int part = ahead.chunk * span + lane_of_heads;
@@ -473,108 +289,38 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       }
     };
     int stage_of = 0;  // ring entry of the next tile issued
-    // The rows of 16 tokens, 16 or 8 bits.
-    auto issue_rows = [&]() {
-      const bool good = page >= 0 && page < a.num_blocks;
-      if (!good && page != kHidden) report(a.status, KVCA_ERR_BAD_INDEX, page);  // its rows read as zeros
-      const unsigned long long row = reinterpret_cast<unsigned long long>(
-          plane + (good ? page : 0) * block_stride + offset * token_stride + page_head * head_stride);
-      const unsigned seen = __ballot_sync(0xffffffffu, good);
-      const uint32_t stage = ring + stage_of * Shape::kStageBytes;
-      constexpr int kPerInstr = 32 / kChunks > 0 ? 32 / kChunks : 1;
-      const int r0 = kChunks >= 32 ? 0 : lane / kChunks;
-      const int c = lane % kChunks;
-      if (in_page && seen == 0xffffffffu) {
-        // one page: rows at a fixed distance
-#pragma unroll
-        for (int side = 0; side < 2; ++side) {
-          const int64_t stride = side == 0 ? a.key_token : a.value_token;
-          const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, side * kTile)) + r0 * stride + c * 16;
-          if (c < row_chunks) {
-#pragma unroll
-            for (int r = 0; r < kTile; r += kPerInstr) {
-              cp_async16(stage + chunk_offset<kChunks>(side * kTile + r + r0, c), src);
-              src += kPerInstr * stride;
-            }
-          }
-        }
-      } else {
-#pragma unroll
-        for (int r = 0; r < 2 * kTile; r += kPerInstr) {
-          const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, r + r0)) + c * 16;
-          if (c < row_chunks) cp_async16(stage + chunk_offset<kChunks>(r + r0, c), src, (seen >> (r + r0)) & 1u);
-        }
-      }
-    };
-    // The rows of 32 tokens, 4 bits, and their scales.
-    auto issue_four = [&]() {
-      const bool good = page >= 0 && page < a.num_blocks;
-      if (!good && page != kHidden) report(a.status, KVCA_ERR_BAD_INDEX, page);  // its rows read as zeros
-      constexpr int kPerInstr = 32 / kChunks;  // rows
-      const int r0 = lane / kChunks, c = lane % kChunks;
-      const uint32_t stage = ring + stage_of * Shape::kStageBytes;
-      const uint32_t values = stage + kTile * Shape::kRowBytes;
-      const int64_t head = page_head * a.key_head;
-      // a lane copies its token's scales; where they do not fill a power of two of
-      // bytes, the 16 bytes that they lie in, or 32
-      const int in_row = a.kv_heads * (a.dim / 2) + page_head * (a.dim / 16);
-      const uint32_t scales = stage + 2 * kTile * Shape::kRowBytes + lane * Shape::kScaleBytes;
-      auto copy_scales = [&](uint32_t to, const char* row) {
-        if constexpr (Cache::kOdd) {
-          const char* const from = row + (in_row & ~15);
-          cp_async16(to, from, good);
-          if ((in_row & 15) + a.dim / 16 > 16) cp_async16(to + 16, from + 16, good);
-        } else if constexpr (Shape::kScaleBytes == 16) {
-          cp_async16(to, row + in_row, good);
-        } else {
-          cp_async_small<Shape::kScaleBytes>(to, row + in_row, good);
-        }
-      };
-      if (a.by_slot) {
-        const int slot = good ? static_cast<int>(page) * a.block_size + offset : -1;
-        const char* const key0 = a.key + head + c * 16;
-        const char* const value0 = a.value + head + c * 16;
-        const int key_token = static_cast<int>(a.key_token), value_token = static_cast<int>(a.value_token);
-#pragma unroll
-        for (int r = 0; r < kTile; r += kPerInstr) {
-          const int from = __shfl_sync(0xffffffffu, slot, r + r0);
-          const int at = max(from, 0);
-          if (c < row_chunks) {
-            cp_async16(stage + chunk_offset_four<kChunks, false>(r + r0, c), key0 + static_cast<int64_t>(at) * key_token, from >= 0);
-            cp_async16(values + chunk_offset_four<kChunks, true>(r + r0, c), value0 + static_cast<int64_t>(at) * value_token,
-                       from >= 0);
-          }
-        }
-        const int at = max(slot, 0);
-        copy_scales(scales, a.key + static_cast<int64_t>(at) * key_token);
-        copy_scales(scales + kTile * Shape::kScaleBytes, a.value + static_cast<int64_t>(at) * value_token);
-      } else {
-        const int64_t block = good ? page : 0;
-        const char* const key_row = a.key + block * a.key_block + offset * a.key_token;
-        const char* const value_row = a.value + block * a.value_block + offset * a.value_token;
-        const unsigned seen = __ballot_sync(0xffffffffu, good);
-#pragma unroll
-        for (int r = 0; r < kTile; r += kPerInstr) {
-          const unsigned long long k_row = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(key_row), r + r0);
-          const unsigned long long v_row =
-              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(value_row), r + r0);
-          const bool read = (seen >> (r + r0)) & 1u;
-          if (c < row_chunks) {
-            cp_async16(stage + chunk_offset_four<kChunks, false>(r + r0, c), reinterpret_cast<const char*>(k_row) + head + c * 16, read);
-            cp_async16(values + chunk_offset_four<kChunks, true>(r + r0, c), reinterpret_cast<const char*>(v_row) + head + c * 16,
-                       read);
-          }
-        }
-        copy_scales(scales, key_row);
-        copy_scales(scales + kTile * Shape::kScaleBytes, value_row);
-      }
-    };
     auto issue = [&]() {
       if (more) {
-        if constexpr (kFour)
-          issue_four();
-        else
-          issue_rows();
+        const bool good = page >= 0 && page < a.num_blocks;
+        if (!good && page != kHidden) report(a.status, KVCA_ERR_BAD_INDEX, page);  // its rows read as zeros
+        const unsigned long long row = reinterpret_cast<unsigned long long>(
+            plane + (good ? page : 0) * block_stride + offset * token_stride + page_head * head_stride);
+        const unsigned seen = __ballot_sync(0xffffffffu, good);
+        const uint32_t stage = ring + stage_of * Shape::kStageBytes;
+        constexpr int kPerInstr = 32 / kChunks > 0 ? 32 / kChunks : 1;
+        const int r0 = kChunks >= 32 ? 0 : lane / kChunks;
+        const int c = lane % kChunks;
+        if (in_page && seen == 0xffffffffu) {
+          // one page: rows at a fixed distance
+#pragma unroll
+          for (int side = 0; side < 2; ++side) {
+            const int64_t stride = side == 0 ? a.key_token : a.value_token;
+            const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, side * kTile)) + r0 * stride + c * 16;
+            if (c < row_chunks) {
+#pragma unroll
+              for (int r = 0; r < kTile; r += kPerInstr) {
+                cp_async16(stage + chunk_offset<kChunks>(side * kTile + r + r0, c), src);
+                src += kPerInstr * stride;
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 2 * kTile; r += kPerInstr) {
+            const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, r + r0)) + c * 16;
+            if (c < row_chunks) cp_async16(stage + chunk_offset<kChunks>(r + r0, c), src, (seen >> (r + r0)) & 1u);
+          }
+        }
         if (++stage_of == kStages) stage_of = 0;
         more = !ahead.last();
         if (more) {
@@ -603,14 +349,13 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
         const int part = at.chunk * span + lane_of_heads;
         const int kv_head = part / head_groups;
         const int first = (part - kv_head * head_groups) * kHeads;
-        if constexpr (kFour && Cache::kOdd) scale_at = (a.kv_heads * (a.dim / 2) + kv_head * (a.dim / 16)) & 15;
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
           const int h = first + n * 8 + (lane >> 2);
           const bool live = h < a.group;
           const uint16_t* row = static_cast<const uint16_t*>(a.query) + static_cast<int64_t>(at.seq) * a.query_row +
                                 static_cast<int64_t>(kv_head * a.group + (live ? h : 0)) * a.query_head;
-          if constexpr (!kNarrow) {
+          if constexpr (!kE4m3) {
 #pragma unroll
             for (int k = 0; k < kSteps; ++k)
 #pragma unroll
@@ -626,7 +371,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
             uint2 raw[kSteps];
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
-              const int d = kFour ? (lane & 3) * (DP / 4) + 4 * k : k * 16 + 4 * (lane & 3);
+              const int d = k * 16 + 4 * (lane & 3);
               raw[k] = live && d < a.dim ? *reinterpret_cast<const uint2*>(row + d) : make_uint2(0, 0);
               const float2 x = bf16 ? unpack2<true>(raw[k].x) : unpack2<false>(raw[k].x);
               const float2 y = bf16 ? unpack2<true>(raw[k].y) : unpack2<false>(raw[k].y);
@@ -663,8 +408,6 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       if (++stage_at == kStages) stage_at = 0;
       issue();  // into the stage that the tile before this one left
 
-      // 16 or 8 bits: the 16 tokens of a tile.
-      auto compute_rows = [&]() {
       // S^T = K Q^T, even and odd steps apart for two shorter chains
       float s[NG][2][4];
 #pragma unroll
@@ -694,7 +437,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       }
 
       // softmax over the tile's tokens (rows lane / 4 and + 8)
-      const int left = at.vis.count - at.tile * kRows;
+      const int left = at.vis.count - at.tile * kTile;
       const bool row0 = (lane >> 2) < left, row1 = (lane >> 2) + 8 < left;
       uint32_t p[NG][2], p_low[NG][2];
       bool grew = false;
@@ -749,7 +492,7 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       }
 
       // O^T += V^T P^T
-      const uint32_t values = keys + kRows * Shape::kRowBytes;
+      const uint32_t values = keys + kTile * Shape::kRowBytes;
 #pragma unroll
       for (int t = 0; t < kSteps; t += kE4m3 ? 2 : 1) {
         uint32_t f[4];
@@ -779,164 +522,6 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
             for (int n = 0; n < NG; ++n) mma16816<false>(acc[n][t + j], w, p[n][0], p[n][1]);
           }
         }
-      }
-      };
-      // 4 bits: 16 of a tile's 32 tokens, from token `sub` on.
-      auto compute_four = [&](int sub) {
-        // S^T = K Q^T.  Lane 4 i + t: dims t DP / 4 and on of the rows' tokens (row i
-        // is token my_token), four dims per step, as the query's are above; a value
-        // times its scale is exact.
-        const uint32_t values = keys + kTile * Shape::kRowBytes;
-        const uint32_t scales = keys + (2 * kTile * Shape::kRowBytes + sub * Shape::kScaleBytes);
-        const int groups = Cache::kOdd ? a.dim / 16 : DP / 16;
-        float s[NG][2][4];
-#pragma unroll
-        for (int n = 0; n < NG; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[n][0][j] = s[n][1][j] = 0.f;
-        {
-          constexpr int kWords = DP / 32, kRead = kWords > 4 ? 4 : kWords;
-          constexpr int kGroups = DP / 64;  // of 16 dims, of a lane
-          uint32_t w[2][kWords], unit16[2][kGroups];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-#pragma unroll
-            for (int part = 0; part < kWords / kRead; ++part) {
-              uint32_t x[kRead];
-              const int byte = (lane & 3) * (DP / 8) + part * 16;
-              load_shared(x, keys + sub * Shape::kRowBytes + 8 * i * Shape::kRowBytes +
-                                 chunk_offset_four<kChunks, false>(my_token, byte / 16) + byte % 16);
-#pragma unroll
-              for (int j = 0; j < kRead; ++j) w[i][part * kRead + j] = x[j];
-            }
-            read_scales<Cache, kGroups>(unit16[i], scales + (my_token + 8 * i) * Shape::kScaleBytes,
-                                        (lane & 3) * kGroups, scale_at, groups);
-          }
-#pragma unroll
-          for (int k = 0; k < kSteps; k += 2) {
-            uint32_t x[4], y[4];
-            e2m1x8_to_f16x2(x, w[0][k / 2]);
-            e2m1x8_to_f16x2(y, w[1][k / 2]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              x[j] = mul_f16x2(x[j], unit16[0][k / 4]);
-              y[j] = mul_f16x2(y[j], unit16[1][k / 4]);
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint32_t f[4] = {x[2 * j], y[2 * j], x[2 * j + 1], y[2 * j + 1]};
-#pragma unroll
-              for (int n = 0; n < NG; ++n) mma16816<false>(s[n][j], f, q[n][k + j][0], q[n][k + j][1]);
-            }
-          }
-        }
-
-        // Softmax.  The maximum is raised only when a score is past it by more than
-        // kGrowth, so that most tiles need no look across the lanes.
-        const int left = at.vis.count - at.tile * kTile - sub;
-        uint32_t p[NG][2];
-        bool grew = false;
-        float x[NG][4];
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[n][j] = (s[n][0][j] + s[n][1][j]) * unit[n][j & 1];
-          if (left < kRows) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (my_token + (j < 2 ? 0 : 8) >= left) x[n][j] = -INFINITY;
-          }
-#pragma unroll
-          for (int j = 0; j < 2; ++j) grew |= fmaxf(x[n][j], x[n][j + 2]) > m[n][j] + Shape::kGrowth;
-        }
-        if (__any_sync(0xffffffffu, grew)) {
-#pragma unroll
-          for (int n = 0; n < NG; ++n) {
-            float decay[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float top = fmaxf(x[n][j], x[n][j + 2]);
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-              const float next = fmaxf(m[n][j], top);
-              decay[j] = exp2_approx(m[n][j] - (next == -INFINITY ? 0.f : next));
-              m[n][j] = next;
-              l[n][j] *= decay[j];
-            }
-#pragma unroll
-            for (int t = 0; t < kSteps; ++t)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[n][t][j] *= decay[j & 1];
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float base = (m[n][j] == -INFINITY ? 0.f : m[n][j]) - Shape::kShift;
-            x[n][j] = exp2_approx(x[n][j] - base);
-            x[n][j + 2] = exp2_approx(x[n][j + 2] - base);
-            l[n][j] += x[n][j] + x[n][j + 2];
-          }
-          // one term, to 2^-11: this cache is bound by instructions, and its values
-          // have 2 bits
-          p[n][0] = transpose8x8(pack2<false>(x[n][0], x[n][1]));
-          p[n][1] = transpose8x8(pack2<false>(x[n][2], x[n][3]));
-        }
-
-        // O^T += V^T P^T.  A lane's byte is two dims of one token, where the operand
-        // wants one dim of two tokens in a register.  So the reduced index goes over
-        // pairs (token, which of the two dims), and the other operand holds the
-        // token's weight beside a 0: two products per step, one for the even dims and
-        // one for the odd ones, on tensor cores that wait anyway, rather than a byte
-        // permutation per register.  Lane 4 i + t: dims i DP / 8 and on of tokens t,
-        // t + 4 and then t + 8, t + 12.
-        constexpr int kWords = DP / 64;  // of a lane's dims of a token
-        constexpr int kGroups = DP > 128 ? 2 : 1;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t w[2][kWords], unit16[2][kGroups];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int tok = (lane & 3) + 4 * i + 8 * half, byte = (lane >> 2) * (DP / 16);
-            load_shared(w[i], values + sub * Shape::kRowBytes + chunk_offset_four<kChunks, true>(tok, byte / 16) + byte % 16);
-            read_scales<Cache, kGroups>(unit16[i], scales + (kTile + tok) * Shape::kScaleBytes,
-                                        DP == 64 ? lane >> 3 : (lane >> 2) * kGroups, scale_at, groups);
-          }
-          uint32_t even[NG][2], odd[NG][2];
-#pragma unroll
-          for (int n = 0; n < NG; ++n) {
-            even[n][0] = p[n][half] & 0xffffu, even[n][1] = p[n][half] >> 16;
-            odd[n][0] = p[n][half] << 16, odd[n][1] = p[n][half] & 0xffff0000u;
-          }
-#pragma unroll
-          for (int r = 0; r < DP / 32; r += 2) {
-            uint32_t x2[4], y2[4];
-            e2m1x8_to_f16x2(x2, w[0][r / 2]);
-            e2m1x8_to_f16x2(y2, w[1][r / 2]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              x2[j] = mul_f16x2(x2[j], unit16[0][r / 4]);
-              y2[j] = mul_f16x2(y2[j], unit16[1][r / 4]);
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint32_t f[4] = {x2[2 * j], x2[2 * j + 1], y2[2 * j], y2[2 * j + 1]};
-#pragma unroll
-              for (int n = 0; n < NG; ++n) {
-                mma16816<false>(acc[n][2 * (r + j)], f, even[n][0], even[n][1]);
-                mma16816<false>(acc[n][2 * (r + j) + 1], f, odd[n][0], odd[n][1]);
-              }
-            }
-          }
-        }
-      };
-      if constexpr (kFour) {
-        compute_four(0);
-        if (at.vis.count - at.tile * kTile > kRows) compute_four(kRows);
-      } else {
-        compute_rows();
       }
 
       const bool ends = at.ends();
@@ -969,7 +554,6 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
           const float r0 = a.value_scale / l[n][0], r1 = a.value_scale / l[n][1];
           const int h = first + n * 8 + (lane >> 2);
           uint16_t* const out = static_cast<uint16_t*>(a.out) + (row + h) * a.dim;
-          uint32_t even_top = 0, even_bottom = 0;  // (4 bits) of the step before
 #pragma unroll
           for (int t = 0; t < kSteps; ++t) {
             uint32_t top, bottom;
@@ -982,23 +566,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
             }
             top = transpose8x8(top);  // now head lane / 4, rows 2 * (lane % 4), + 1
             bottom = transpose8x8(bottom);
-            if constexpr (kFour) {
-              // even dims, then odd ones, of 4 dims in each of two lanes' rows
-              if (t % 2 == 0) {
-                even_top = top, even_bottom = bottom;
-                continue;
-              }
-            }
             if (h >= a.group) continue;
-            if constexpr (kFour) {
-              const int d = (lane & 3) * (DP / 4) + 2 * (t - 1);
-              if (d < a.dim)
-                *reinterpret_cast<uint2*>(out + d) =
-                    make_uint2(__byte_perm(even_top, top, 0x5410), __byte_perm(even_bottom, bottom, 0x5410));
-              if (d + DP / 8 < a.dim)
-                *reinterpret_cast<uint2*>(out + d + DP / 8) =
-                    make_uint2(__byte_perm(even_top, top, 0x7632), __byte_perm(even_bottom, bottom, 0x7632));
-            } else if constexpr (!kE4m3) {
+            if constexpr (!kE4m3) {
               const int d = t * 16 + 2 * (lane & 3);
               if (d < a.dim) *reinterpret_cast<uint32_t*>(out + d) = top;
               if (d + 8 < a.dim) *reinterpret_cast<uint32_t*>(out + d + 8) = bottom;
@@ -1031,7 +600,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
           }
 #pragma unroll
           for (int t = 0; t < kSteps; ++t) {
-            const int d0 = first_dim(t), d1 = d0 + kSecondDim;
+            const int d0 = kE4m3 ? t * 16 + 2 * (lane >> 2) : t * 16 + (lane >> 2);
+            const int d1 = kE4m3 ? d0 + 1 : d0 + 8;
             *reinterpret_cast<float2*>(part + d0 * kHeads + h) = make_float2(acc[n][t][0], acc[n][t][1]);
             *reinterpret_cast<float2*>(part + d1 * kHeads + h) = make_float2(acc[n][t][2], acc[n][t][3]);
           }
@@ -1074,7 +644,8 @@ __global__ void __launch_bounds__(StepShape<Cache, DP, NG>::kThreads, 1)
       }
 #pragma unroll
       for (int t = 0; t < kSteps; ++t) {
-        const int d0 = first_dim(t), d1 = d0 + kSecondDim;
+        const int d0 = kE4m3 ? t * 16 + 2 * (lane >> 2) : t * 16 + (lane >> 2);
+        const int d1 = kE4m3 ? d0 + 1 : d0 + 8;
         *reinterpret_cast<float2*>(mine + d0 * kHeads + h) = make_float2(acc[n][t][0], acc[n][t][1]);
         *reinterpret_cast<float2*>(mine + d1 * kHeads + h) = make_float2(acc[n][t][2], acc[n][t][3]);
       }
@@ -1263,8 +834,7 @@ cudaError_t launch_typed(const AttendArgs& a, void* workspace, uint32_t* arrived
 
 template <typename Cache, int DP>
 size_t workspace_of(int tiles, int sms) {
-  const int64_t warps =
-      static_cast<int64_t>(sms) * (tiles == 1 ? StepShape<Cache, DP, 1>::kWarps : StepShape<Cache, DP, 2>::kWarps);
+  const int64_t warps = static_cast<int64_t>(sms) * step_warps(DP * Cache::kBytes, tiles);
   return tiles == 1 ? StepWorkspace<8, DP * 8>::bytes(warps) : StepWorkspace<16, DP * 16>::bytes(warps);
 }
 
@@ -1275,20 +845,13 @@ int head_tiles(const AttendArgs& a) { return a.group > 8 && a.dim <= 128 ? 2 : 1
 
 }  // namespace
 
-template <typename Cache>
-static size_t workspace_cache(const AttendArgs& a, int sms) {
-  const int n = head_tiles(a);
-  return a.dim <= 64    ? workspace_of<Cache, 64>(n, sms)
-         : a.dim <= 128 ? workspace_of<Cache, 128>(n, sms)
-                        : workspace_of<Cache, 256>(n, sms);
-}
-
 size_t attend_step_workspace(const AttendArgs& a, int sms) {
-  switch (a.cache_type) {
-    case KVCA_TYPE_E4M3: return workspace_cache<CacheE4m3>(a, sms);
-    case KVCA_TYPE_E2M1: return workspace_cache<CacheE2m1<false>>(a, sms);
-    default: return workspace_cache<CacheF16>(a, sms);
-  }
+  const int n = head_tiles(a);
+  if (a.cache_type == KVCA_TYPE_E2M1) return attend_step_four_workspace(a, n, sms);
+  const bool e4m3 = a.cache_type == KVCA_TYPE_E4M3;
+  if (a.dim <= 64) return e4m3 ? workspace_of<CacheE4m3, 64>(n, sms) : workspace_of<CacheF16, 64>(n, sms);
+  if (a.dim <= 128) return e4m3 ? workspace_of<CacheE4m3, 128>(n, sms) : workspace_of<CacheF16, 128>(n, sms);
+  return e4m3 ? workspace_of<CacheE4m3, 256>(n, sms) : workspace_of<CacheF16, 256>(n, sms);
 }
 
 template <typename Cache>
@@ -1309,10 +872,7 @@ cudaError_t launch_attend_step(const AttendArgs& a, void* workspace, uint32_t* a
   switch (a.cache_type) {
     case KVCA_TYPE_F16: return launch_cache<CacheF16>(a, workspace, arrived, sms, stream);
     case KVCA_TYPE_BF16: return launch_cache<CacheBf16>(a, workspace, arrived, sms, stream);
-    case KVCA_TYPE_E2M1:
-      if (a.dim == 64 || a.dim == 128 || a.dim == 256)
-        return launch_cache<CacheE2m1<false>>(a, workspace, arrived, sms, stream);
-      return launch_cache<CacheE2m1<true>>(a, workspace, arrived, sms, stream);
+    case KVCA_TYPE_E2M1: return launch_attend_step_four(a, head_tiles(a), workspace, arrived, sms, stream);
     default: return launch_cache<CacheE4m3>(a, workspace, arrived, sms, stream);
   }
 }

@@ -83,6 +83,8 @@ void to_side(const kvca_chunk_desc* d, kvca::ChunkSide* s) {
 
 bool aligned16(uint64_t x) { return x % 16 == 0; }
 
+std::atomic<int64_t> attend_wait_limit{2000000000};
+
 // The checked arguments of an attention call as the kernels take them.
 int to_attend(const kvca_attend_desc* d, int64_t* d_status, kvca::AttendArgs* a) {
   if (d == nullptr || d->num_seqs < 0 || d->num_blocks < 0 || d->block_size < 1 || d->table_width < 0 ||
@@ -138,14 +140,7 @@ int to_attend(const kvca_attend_desc* d, int64_t* d_status, kvca::AttendArgs* a)
   a->lse = d->lse;
   a->query_type = d->query_type;
   a->cache_type = d->cache_type;
-  if (d->block_size == 1) {  // every offset is 0
-    a->key_token = a->key_block;
-    a->value_token = a->value_block;
-  }
-  const int64_t most = int64_t{1} << 31;
-  a->by_slot = e2m1 && d->block_size < most && d->num_blocks < most / d->block_size && a->key_token < most &&
-               a->value_token < most && a->key_token >= 0 && a->value_token >= 0 &&
-               a->key_block == d->block_size * a->key_token && a->value_block == d->block_size * a->value_token;
+  if (e2m1) a->row_bytes = static_cast<int>((static_cast<int64_t>(d->kv_heads) * d->head_dim * 9 / 16 + 15) / 16 * 16);
   a->status = d_status;
   // without blocks no row is read, but rows that are not read get an address
   if (d->num_blocks == 0) a->key = a->value = static_cast<const char*>(a->query);
@@ -918,6 +913,7 @@ int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t wo
   if (rc != KVCA_OK) return rc;
   if (a.num_seqs == 0) return KVCA_OK;
   if (!attend_pointers_ok(a)) return KVCA_ERR_BAD_ARGUMENT;
+  a.wait_limit = attend_wait_limit.load();
   const int sms = kvca_device_sm_count();
   if (sms < 1) return KVCA_ERR_CUDA;
   if (d_workspace == nullptr || !aligned16(reinterpret_cast<uint64_t>(d_workspace)) || d_counters == nullptr ||
@@ -927,8 +923,6 @@ int kvca_attend_step(const kvca_attend_desc* desc, void* d_workspace, int64_t wo
 }
 
 namespace {
-
-std::atomic<int64_t> attend_wait_limit{2000000000};
 
 int to_chunk(const kvca_attend_desc* desc, int64_t num_rows, int64_t* d_status, kvca::AttendArgs* a) {
   const int rc = to_attend(desc, d_status, a);

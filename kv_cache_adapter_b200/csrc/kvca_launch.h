@@ -143,9 +143,9 @@ struct AttendArgs {
   float* lse;  // (rows, heads), dense, or null
   int query_type;
   int cache_type;
-  // (4 bits) Token rows of both sides at slot * token stride, slots and strides
-  // below 2^31.
-  bool by_slot;
+  // (4 bits) Bytes of a token's row, and ns that a wait of the step's kernel may take.
+  int row_bytes;
+  int64_t wait_limit;
   int64_t* status;
 };
 
@@ -165,6 +165,11 @@ size_t attend_step_workspace(const AttendArgs& args, int sms);
 constexpr int kStepMaxWarps = 16;  // of a CTA: results are counted per warp
 cudaError_t launch_attend_step(const AttendArgs& args, void* workspace, uint32_t* arrived, int sms,
                                cudaStream_t stream);
+
+// The step over 4-bit caches; `tiles`: of 8 query heads that share a pass.
+size_t attend_step_four_workspace(const AttendArgs& args, int tiles, int sms);
+cudaError_t launch_attend_step_four(const AttendArgs& args, int tiles, void* workspace, uint32_t* arrived, int sms,
+                                    cudaStream_t stream);
 
 constexpr int kChunkMaxDim = 128;  // two output tiles fill the tensor memory
 size_t attend_chunk_workspace(const AttendArgs& args, int64_t rows, int sms);
