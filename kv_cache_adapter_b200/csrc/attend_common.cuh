@@ -53,6 +53,13 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// The largest of three.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // The larger of two; NaN when either is.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;

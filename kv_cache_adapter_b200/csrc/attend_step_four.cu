@@ -2,7 +2,7 @@
 // e2m1 codes with an e4m3 scale for each 16 dims.
 //
 // HBM would bound it (144 bytes per token and K/V head of 128 dims, for both
-// sides), were there not 64 conversions, 64 multiplications by scales and 24
+// sides), were there not 64 conversions, 64 multiplications by scales and 16
 // products per 16 tokens and warp to issue in the time that these bytes take.
 // So everything else is kept off the warps that compute:
 //
@@ -144,20 +144,59 @@ __device__ __forceinline__ uint32_t load_shared8(uint32_t addr) {
   return v;
 }
 
+// Both halves of a register alike (the multiplication's operand takes one half
+// twice).
+__device__ __forceinline__ uint32_t low_twice(uint32_t v) {
+  uint32_t r;
+  asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %1;\nmov.b32 %0, {a, a};\n}" : "=r"(r) : "r"(v));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t high_twice(uint32_t v) {
+  uint32_t r;
+  asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %1;\nmov.b32 %0, {b, b};\n}" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// d = a b, with nothing before it.
+__device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // The scales of kGroups groups of a row from group `first` on, at `addr`, each
 // twice in a register; groups from `groups` on, which are padding of odd head
 // dims, have none.
 template <int kGroups, bool kOdd>
 __device__ __forceinline__ void read_scales(uint32_t (&unit)[kGroups], uint32_t addr, int first, int groups) {
   if constexpr (kGroups == 1) {
-    unit[0] = e4m3_to_f16x2(load_shared8(addr) * 0x101u);
+    unit[0] = low_twice(e4m3_to_f16x2(load_shared8(addr)));
   } else {
 #pragma unroll
     for (int j = 0; j < kGroups; j += 2) {
       const uint32_t v = e4m3_to_f16x2(load_shared16(addr + j));
-      unit[j] = __byte_perm(v, 0, 0x1010);
-      unit[j + 1] = __byte_perm(v, 0, 0x3232);
+      unit[j] = low_twice(v);
+      unit[j + 1] = high_twice(v);
     }
+  }
+  if constexpr (kOdd) {
+#pragma unroll
+    for (int j = 0; j < kGroups; ++j)
+      if (first + j >= groups) unit[j] = 0;
+  }
+}
+
+// The same scales of two rows, side by side in a register.
+template <int kGroups, bool kOdd>
+__device__ __forceinline__ void read_scale_pairs(uint32_t (&unit)[kGroups], uint32_t one, uint32_t other, int first,
+                                                 int groups) {
+  if constexpr (kGroups == 1) {
+    unit[0] = e4m3_to_f16x2(__byte_perm(load_shared8(one), load_shared8(other), 0x0040));
+  } else {
+    const uint32_t a = load_shared16(one), b = load_shared16(other);
+    unit[0] = e4m3_to_f16x2(__byte_perm(a, b, 0x0040));
+    unit[1] = e4m3_to_f16x2(__byte_perm(a, b, 0x0051));
   }
   if constexpr (kOdd) {
 #pragma unroll
@@ -247,8 +286,8 @@ __global__ void __launch_bounds__(FourShape<DP, NG>::kThreads, 1)
   StepJoin held_runs{-1, 0, 0};
 
   // Lane 4 i + t has of the heads 2 t and 2 t + 1 of each tile of 8 the maxima, its
-  // share of the sums, and the dims i DP / 8 and on of the outputs: acc[][2 r + p]
-  // are dims 4 r + p of those (both heads), then 4 r + p + 2.
+  // share of the sums, and the dims i DP / 8 and on of the outputs: acc[][b] are dims
+  // 2 b of those (both heads), then 2 b + 1.
   float acc[NG][kSteps][4];
   float m[NG][2], l[NG][2];
 
@@ -265,7 +304,7 @@ __global__ void __launch_bounds__(FourShape<DP, NG>::kThreads, 1)
       uint16_t* const out = static_cast<uint16_t*>(a.out) + (row + h) * a.dim;
 #pragma unroll
       for (int r = 0; r < kSteps / 2; ++r) {
-        uint32_t w[2][2];  // [odd dims][two dims further], heads 2 t and 2 t + 1
+        uint32_t w[2][2];  // dims 4 r + 2 p + j
 #pragma unroll
         for (int p = 0; p < 2; ++p)
 #pragma unroll
@@ -278,10 +317,10 @@ __global__ void __launch_bounds__(FourShape<DP, NG>::kThreads, 1)
         const int d = (lane & 3) * (DP / 4) + 4 * r;
         if (d < a.dim)
           *reinterpret_cast<uint2*>(out + d) =
-              make_uint2(__byte_perm(w[0][0], w[1][0], 0x5410), __byte_perm(w[0][1], w[1][1], 0x5410));
+              make_uint2(__byte_perm(w[0][0], w[0][1], 0x5410), __byte_perm(w[1][0], w[1][1], 0x5410));
         if (d + DP / 8 < a.dim)
           *reinterpret_cast<uint2*>(out + d + DP / 8) =
-              make_uint2(__byte_perm(w[0][0], w[1][0], 0x7632), __byte_perm(w[0][1], w[1][1], 0x7632));
+              make_uint2(__byte_perm(w[0][0], w[0][1], 0x7632), __byte_perm(w[1][0], w[1][1], 0x7632));
       }
       if (a.lse != nullptr && lane < 4) {
 #pragma unroll
@@ -383,7 +422,7 @@ __global__ void __launch_bounds__(FourShape<DP, NG>::kThreads, 1)
     auto look_up = [&](const Position& p) {
       const int v = p.tile * kTile + lane;
       page = kHidden;
-      if (v < p.vis.count) {
+      if (lane < kTile && v < p.vis.count) {
         const int pos = p.vis.position(v);
         const int block = a.block_shift >= 0 ? pos >> a.block_shift : pos / a.block_size;
         offset = pos - block * a.block_size;
@@ -556,10 +595,6 @@ __global__ void __launch_bounds__(FourShape<DP, NG>::kThreads, 1)
         // S^T = K Q^T: row i is token row_token(i), lane 4 i + t has its dims t DP / 4
         // and on, four per step, as the query's are above
         float s[NG][2][4];
-#pragma unroll
-        for (int n = 0; n < NG; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[n][0][j] = s[n][1][j] = 0.f;
         {
           constexpr int kWords = DP / 32, kRead = kWords > 4 ? 4 : kWords;
           constexpr int kGroups = DP / 64;  // of 16 dims, of a lane
@@ -590,7 +625,12 @@ __global__ void __launch_bounds__(FourShape<DP, NG>::kThreads, 1)
             for (int j = 0; j < 2; ++j) {
               const uint32_t f[4] = {x[2 * j], y[2 * j], x[2 * j + 1], y[2 * j + 1]};
 #pragma unroll
-              for (int n = 0; n < NG; ++n) mma16816<false>(s[n][j], f, q[n][k + j][0], q[n][k + j][1]);
+              for (int n = 0; n < NG; ++n) {
+                if (k == 0)
+                  mma16816_first(s[n][j], f, q[n][k + j][0], q[n][k + j][1]);
+                else
+                  mma16816<false>(s[n][j], f, q[n][k + j][0], q[n][k + j][1]);
+              }
             }
           }
         }
@@ -599,16 +639,20 @@ __global__ void __launch_bounds__(FourShape<DP, NG>::kThreads, 1)
         float y[NG][4];
         float most = -INFINITY;
         const bool cut = left < kRows;
-        const bool hidden0 = cut && my_token >= left, hidden1 = cut && my_token + 8 >= left;
+        const bool hidden0 = my_token >= left, hidden1 = my_token + 8 >= left;
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             s[n][0][j] += s[n][1][j];
             y[n][j] = fmaf(s[n][0][j], unit[n][j & 1], kShift - m[n][j & 1]);
-            if (j < 2 ? hidden0 : hidden1) y[n][j] = -INFINITY;  // (whatever the ring held there)
-            most = fmaxf(most, y[n][j]);
           }
+          if (cut) {  // whatever the ring held there
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j < 2 ? hidden0 : hidden1) y[n][j] = -INFINITY;
+          }
+          most = max3(max3(most, y[n][0], y[n][1]), y[n][2], y[n][3]);
         }
         if (__any_sync(0xffffffffu, most > kShift + kGrowth)) {
 #pragma unroll
@@ -648,54 +692,43 @@ __global__ void __launch_bounds__(FourShape<DP, NG>::kThreads, 1)
           p[n][1] = transpose8x8(pack2<false>(y[n][2], y[n][3]));
         }
 
-        // O^T += V^T P^T.  A lane's byte is two dims of one token, where the operand
-        // wants one dim of two tokens in a register.  So the reduced index goes over
-        // pairs (token, which of the two dims), and the other operand holds the
-        // token's weight beside a 0: two products per step, one for the even dims and
-        // one for the odd ones, on tensor cores that wait anyway, rather than a byte
-        // permutation per register.  Lane 4 i + t: dims i DP / 8 and on of the tokens
-        // of rows 2 t, 2 t + 1 and then 2 t + 8, 2 t + 9.
+        // O^T += V^T P^T.  Lane 4 i + t: dims i DP / 8 and on of the tokens of rows 2 t,
+        // 2 t + 1, 2 t + 8 and 2 t + 9.  A converted byte is two dims of one token, the
+        // operand wants one dim of two tokens in a register: a byte permutation each.
+        // (Without it, a product each for the even and the odd dims, tokens' weights
+        // beside zeros: the multiplications by scales wait for the tensor cores, so 7 %
+        // more time for the two sides of a tile in registers and shared memory.)
         constexpr int kWords = DP / 64;  // of a lane's dims of a token
         constexpr int kGroups = DP > 128 ? 2 : 1;
+        uint32_t w[4][kWords], scale[2][kGroups];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t w[2][kWords], scale[2][kGroups];
+        for (int i = 0; i < 4; ++i)
+          load_shared(w[i], own_rows + value_at + 8 * (i / 2) * ring.pitch + (i % 2) * next_row);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t to_row = 8 * half * ring.pitch + i * next_row;
-            load_shared(w[i], own_rows + value_at + to_row);
-            read_scales<kGroups, kOdd>(scale[i], own_rows + value_scale_at + to_row, (lane >> 2) * (DP / 8) / 16,
-                                       a.dim / 16);
-            if (cut && row_token(2 * (lane & 3) + i) + 8 * half >= left) {  // nothing of what the ring held there
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t first_row = own_rows + value_scale_at + 8 * i * ring.pitch;
+          read_scale_pairs<kGroups, kOdd>(scale[i], first_row, first_row + next_row, (lane >> 2) * (DP / 8) / 16,
+                                          a.dim / 16);
+          if (cut) {  // nothing of what the ring held there
+            const uint32_t keep = (row_token(2 * (lane & 3)) + 8 * i < left ? 0xffffu : 0u) |
+                                  (row_token(2 * (lane & 3) + 1) + 8 * i < left ? 0xffff0000u : 0u);
 #pragma unroll
-              for (int j = 0; j < kGroups; ++j) scale[i][j] = 0;
-            }
+            for (int j = 0; j < kGroups; ++j) scale[i][j] &= keep;
           }
-          uint32_t even[NG][2], odd[NG][2];
+        }
 #pragma unroll
-          for (int n = 0; n < NG; ++n) {
-            even[n][0] = p[n][half] & 0xffffu, even[n][1] = p[n][half] >> 16;
-            odd[n][0] = p[n][half] << 16, odd[n][1] = p[n][half] & 0xffff0000u;
-          }
+        for (int r = 0; r < kWords; ++r) {
+          uint32_t x[4][4];
 #pragma unroll
-          for (int r = 0; r < DP / 32; r += 2) {
-            uint32_t x[4], z[4];
-            e2m1x8_to_f16x2(x, w[0][r / 2]);
-            e2m1x8_to_f16x2(z, w[1][r / 2]);
+          for (int i = 0; i < 4; ++i) e2m1x8_to_f16x2(x[i], w[i][r]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              x[j] = mul_f16x2(x[j], scale[0][r / 4]);
-              z[j] = mul_f16x2(z[j], scale[1][r / 4]);
-            }
+          for (int b = 0; b < 4; ++b) {
+            const uint32_t f[4] = {mul_f16x2(__byte_perm(x[0][b], x[1][b], 0x5410), scale[0][r / 2]),
+                                   mul_f16x2(__byte_perm(x[0][b], x[1][b], 0x7632), scale[0][r / 2]),
+                                   mul_f16x2(__byte_perm(x[2][b], x[3][b], 0x5410), scale[1][r / 2]),
+                                   mul_f16x2(__byte_perm(x[2][b], x[3][b], 0x7632), scale[1][r / 2])};
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint32_t f[4] = {x[2 * j], x[2 * j + 1], z[2 * j], z[2 * j + 1]};
-#pragma unroll
-              for (int n = 0; n < NG; ++n) {
-                mma16816<false>(acc[n][2 * (r + j)], f, even[n][0], even[n][1]);
-                mma16816<false>(acc[n][2 * (r + j) + 1], f, odd[n][0], odd[n][1]);
-              }
-            }
+            for (int n = 0; n < NG; ++n) mma16816<false>(acc[n][4 * r + b], f, p[n][0], p[n][1]);
           }
         }
       }
