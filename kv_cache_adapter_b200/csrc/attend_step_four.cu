@@ -109,7 +109,7 @@ struct RunRing {
 };
 
 // What a warp keeps in shared memory of the tiles that it has to fetch.
-struct Fetch {
+struct alignas(16) Fetch {
   Position at;         // the next one
   int stage, round;    // of the ring, for it
   uint32_t mine, parity;  // stages that this warp has filled, and the phase that its copies end
@@ -583,7 +583,6 @@ __global__ void __launch_bounds__(FourShape<DP, NG>::kThreads, 1)
         fresh = false;
       }
 
-      if (done + ring.ahead >= due) fetch();
       ok = warp_wait(ring_bars + 16 * stage, phase, patience) && ok;
       const uint32_t rows = ring_base + stage * ring.stage_bytes;
       const int count = at.vis.count - at.tile * kTile;
@@ -731,6 +730,9 @@ __global__ void __launch_bounds__(FourShape<DP, NG>::kThreads, 1)
             for (int n = 0; n < NG; ++n) mma16816<false>(acc[n][4 * r + b], f, p[n][0], p[n][1]);
           }
         }
+        // in the middle of a tile, when the other warps have long left the stage of
+        // the tile before it
+        if (sub == 0 && done + ring.ahead >= due) fetch();
       }
       __syncwarp();
       if (lane == 0) barrier_arrive(ring_bars + 16 * stage + 8);
