@@ -1135,7 +1135,9 @@ int kvca_read_tokens(const kvca_read_desc* d, int64_t* d_status, kvca_stream_t s
   a.scale = d->scale;
   a.out = reinterpret_cast<char*>(d->out);
   a.status = d_status;
-  return status_of(kvca::launch_read_tokens(a, d->type, stream));
+  const int sms = kvca_device_sm_count();
+  if (sms < 1) return KVCA_ERR_CUDA;
+  return status_of(kvca::launch_read_tokens(a, d->type, sms, stream));
 }
 
 int kvca_copy_paged(const kvca_paged_desc* src, const kvca_paged_desc* dst, int64_t num_planes,

@@ -224,7 +224,7 @@ struct ReadArgs {
   int64_t* status;
 };
 
-cudaError_t launch_read_tokens(const ReadArgs& args, int type, cudaStream_t stream);
+cudaError_t launch_read_tokens(const ReadArgs& args, int type, int sms, cudaStream_t stream);
 
 // The slot pool and the page tables of the operators on sequences' pages.
 struct PagePool {

@@ -307,7 +307,7 @@ struct CacheE2m1Rows {
 // Cache: the type that keys and values are stored in; In where nothing is.
 // kWide: 16 dims to a lane, for the keys and values of a 4-bit cache; its
 // queries then are rows of a warp of their own kind (8 dims to a lane).
-template <typename In, typename Cache, int kMode, bool kStores, bool kWide>
+template <typename In, typename Cache, int kMode, bool kStores, bool kWide, int kBatch>
 __device__ __forceinline__ void token_rows(const TokenArgs& a, int64_t token, int part, int parts) {
   constexpr bool kFour = kStores && Cache::kBytes == 0;
   using Lane = Lane8<kMode, kWide>;
@@ -320,105 +320,120 @@ __device__ __forceinline__ void token_rows(const TokenArgs& a, int64_t token, in
   const int begin = kWide && kMode != kTurnHalves ? a.q_heads : 0;
   const int keys = a.q_heads, values = keys + a.kv_heads;
   const int end = kFour && !kWide && kMode != kTurnHalves ? a.q_heads : kStores ? values + a.kv_heads : a.q_heads;
-  const TokenPlace place = place_of<kStores>(a, token);
-  if (!place.live) return;
   if (begin + part * rows >= end) return;
-  at.load(a, place.angles);
+  TokenPlace place;
   float key_reciprocal = 0.f, value_reciprocal = 0.f;
   if constexpr (kStores && Cache::kBytes == 1) {
     key_reciprocal = __frcp_rn(a.key_scale);
     value_reciprocal = __frcp_rn(a.value_scale);
   }
-  for (int r = begin + part * rows; r < end; r += parts * rows) {
-    const int h = r + row_of;
-    const bool mine = row_of < rows && h < end;
-    const bool is_query = h < keys, is_value = h >= values;
-    const char* from = nullptr;
-    Raw8<In> raw[kParts];
-    if (mine) {
-      from = is_query ? a.query + token * a.query_row + h * a.query_head
-             : is_value ? a.value + token * a.value_row + (h - values) * a.value_head
-                        : a.key + token * a.key_row + (h - keys) * a.key_head;
-      raw[0].load(from + at.first * In::kBytes);
-      if constexpr (kParts == 2)
-        if (at.second >= 0) raw[1].load(from + at.second * In::kBytes);
-    }
-    float x[kParts][8];
-    if (mine) {
-      if (!is_value) {
-        at.template rotate<In>(a, from, place.angles, raw, x, !is_query && (kFour || (kStores && Cache::kBytes == 1)));
-      } else if constexpr (kStores && Cache::kBytes < 2) {
+  // The rows of kBatch turns are on their way together, the first ones before the
+  // token's slot and position are known.
+  const int step = parts * rows;
+#pragma unroll 1
+  for (int r0 = begin + part * rows; r0 < end; r0 += kBatch * step) {
+    Raw8<In> batch[kBatch][kParts];
+    const char* from[kBatch];
 #pragma unroll
-        for (int j = 0; j < kParts; ++j) raw[j].get(x[j]);
-      }
-    }
-    if constexpr (kMode == kTurnLoose) __syncwarp();  // another lane's values have been read: their place may be the result's
-    if constexpr (!kStores) {
-      if (!mine) continue;
-      char* const to = a.query_out + token * a.query_out_row + h * a.query_out_head;
-      raw[0].store(to + at.first * In::kBytes);
+    for (int b = 0; b < kBatch; ++b) {
+      const int h = r0 + b * step + row_of;
+      if (row_of >= rows || h >= end) continue;
+      from[b] = h < keys     ? a.query + token * a.query_row + h * a.query_head
+                : h >= values ? a.value + token * a.value_row + (h - values) * a.value_head
+                              : a.key + token * a.key_row + (h - keys) * a.key_head;
+      batch[b][0].load(from[b] + at.first * In::kBytes);
       if constexpr (kParts == 2)
-        if (at.second >= 0) raw[1].store(to + at.second * In::kBytes);
-    } else {
-      float big[kParts];
-      if constexpr (kFour && (kMode == kTurnHalves || kWide)) {
-        if constexpr (kMode == kTurnHalves) {
-          // a group is two neighbouring lanes' parts
+        if (at.second >= 0) batch[b][1].load(from[b] + at.second * In::kBytes);
+    }
+    if (r0 == begin + part * rows) {
+      place = place_of<kStores>(a, token);
+      if (!place.live) return;
+      at.load(a, place.angles);
+    }
 #pragma unroll
-          for (int j = 0; j < kParts; ++j) {
-            big[j] = mine && !is_query ? largest8(x[j]) : 0.f;
-            big[j] = max_nan(big[j], __shfl_xor_sync(0xffffffffu, big[j], 1));
-          }
-        } else {
-          big[0] = mine ? max_nan(largest8(x[0]), largest8(x[1])) : 0.f;
-          big[1] = big[0];
+    for (int b = 0; b < kBatch; ++b) {
+      if (r0 + b * step >= end) break;
+      const int h = r0 + b * step + row_of;
+      const bool mine = row_of < rows && h < end;
+      const bool is_query = h < keys, is_value = h >= values;
+      Raw8<In>(&raw)[kParts] = batch[b];
+      float x[kParts][8];
+      if (mine) {
+        if (!is_value) {
+          at.template rotate<In>(a, from[b], place.angles, raw, x, !is_query && (kFour || (kStores && Cache::kBytes == 1)));
+        } else if constexpr (kStores && Cache::kBytes < 2) {
+#pragma unroll
+          for (int j = 0; j < kParts; ++j) raw[j].get(x[j]);
         }
       }
-      if (!mine) continue;
-      if (is_query) {
+      if constexpr (kMode == kTurnLoose) __syncwarp();  // another lane's values have been read: their place may be the result's
+      if constexpr (!kStores) {
+        if (!mine) continue;
         char* const to = a.query_out + token * a.query_out_row + h * a.query_out_head;
         raw[0].store(to + at.first * In::kBytes);
         if constexpr (kParts == 2)
           if (at.second >= 0) raw[1].store(to + at.second * In::kBytes);
-        continue;
-      }
-      const int head = is_value ? h - values : h - keys;
-      char* const row = is_value
-                            ? a.value_cache + place.block * a.value_cache_block + place.offset * a.value_cache_token
-                            : a.key_cache + place.block * a.key_cache_block + place.offset * a.key_cache_token;
-      const float scale = is_value ? a.value_scale : a.key_scale;
-      if constexpr (kFour) {
-        if constexpr (kMode == kTurnHalves || kWide) {
-          const int64_t codes = static_cast<int64_t>(a.kv_heads) * (a.dim / 2);
-#pragma unroll
-          for (int j = 0; j < kParts; ++j) {
-            const int d = j == 0 ? at.first : at.second;
-            if (d < 0) continue;
-            const uint32_t byte = scale_of(big[j], scale);
-            const float unit = e4m3_to_float(byte) * scale;
-            *reinterpret_cast<uint32_t*>(row + head * (a.dim / 2) + d / 2) = to_codes(x[j], unit, __frcp_rn(unit));
-            if (d % 16 == 0)
-              *reinterpret_cast<uint8_t*>(row + codes + head * (a.dim / 16) + d / 16) = static_cast<uint8_t>(byte);
+      } else {
+        float big[kParts];
+        if constexpr (kFour && (kMode == kTurnHalves || kWide)) {
+          if constexpr (kMode == kTurnHalves) {
+            // a group is two neighbouring lanes' parts
+  #pragma unroll
+            for (int j = 0; j < kParts; ++j) {
+              big[j] = mine && !is_query ? largest8(x[j]) : 0.f;
+              big[j] = max_nan(big[j], __shfl_xor_sync(0xffffffffu, big[j], 1));
+            }
+          } else {
+            big[0] = mine ? max_nan(largest8(x[0]), largest8(x[1])) : 0.f;
+            big[1] = big[0];
           }
         }
-      } else {
-        char* const to = row + head * (is_value ? a.value_cache_head : a.key_cache_head);
-        if constexpr (Cache::kBytes == 1) {
-          const float reciprocal = is_value ? value_reciprocal : key_reciprocal;
-          *reinterpret_cast<uint2*>(to + at.first) = to_e4m3x8(x[0], scale, reciprocal);
-          if constexpr (kParts == 2)
-            if (at.second >= 0) *reinterpret_cast<uint2*>(to + at.second) = to_e4m3x8(x[1], scale, reciprocal);
-        } else {
+        if (!mine) continue;
+        if (is_query) {
+          char* const to = a.query_out + token * a.query_out_row + h * a.query_out_head;
           raw[0].store(to + at.first * In::kBytes);
           if constexpr (kParts == 2)
             if (at.second >= 0) raw[1].store(to + at.second * In::kBytes);
+          continue;
+        }
+        const int head = is_value ? h - values : h - keys;
+        char* const row = is_value
+                              ? a.value_cache + place.block * a.value_cache_block + place.offset * a.value_cache_token
+                              : a.key_cache + place.block * a.key_cache_block + place.offset * a.key_cache_token;
+        const float scale = is_value ? a.value_scale : a.key_scale;
+        if constexpr (kFour) {
+          if constexpr (kMode == kTurnHalves || kWide) {
+            const int64_t codes = static_cast<int64_t>(a.kv_heads) * (a.dim / 2);
+  #pragma unroll
+            for (int j = 0; j < kParts; ++j) {
+              const int d = j == 0 ? at.first : at.second;
+              if (d < 0) continue;
+              const uint32_t byte = scale_of(big[j], scale);
+              const float unit = e4m3_to_float(byte) * scale;
+              *reinterpret_cast<uint32_t*>(row + head * (a.dim / 2) + d / 2) = to_codes(x[j], unit, __frcp_rn(unit));
+              if (d % 16 == 0)
+                *reinterpret_cast<uint8_t*>(row + codes + head * (a.dim / 16) + d / 16) = static_cast<uint8_t>(byte);
+            }
+          }
+        } else {
+          char* const to = row + head * (is_value ? a.value_cache_head : a.key_cache_head);
+          if constexpr (Cache::kBytes == 1) {
+            const float reciprocal = is_value ? value_reciprocal : key_reciprocal;
+            *reinterpret_cast<uint2*>(to + at.first) = to_e4m3x8(x[0], scale, reciprocal);
+            if constexpr (kParts == 2)
+              if (at.second >= 0) *reinterpret_cast<uint2*>(to + at.second) = to_e4m3x8(x[1], scale, reciprocal);
+          } else {
+            raw[0].store(to + at.first * In::kBytes);
+            if constexpr (kParts == 2)
+              if (at.second >= 0) raw[1].store(to + at.second * In::kBytes);
+          }
         }
       }
     }
   }
 }
 
-template <typename In, typename Cache, int kMode, bool kStores>
+template <typename In, typename Cache, int kMode, bool kStores, int kBatch>
 __global__ void __launch_bounds__(32 * kTokenWarps) token_rows_kernel(const __grid_constant__ TokenArgs a) {
   const int64_t warp = static_cast<int64_t>(blockIdx.x) * kTokenWarps + (threadIdx.x >> 5);
   const int64_t token = warp / a.token_warps;
@@ -426,37 +441,44 @@ __global__ void __launch_bounds__(32 * kTokenWarps) token_rows_kernel(const __gr
   if (token >= a.rows) return;
   if constexpr (kStores && Cache::kBytes == 0 && kMode != kTurnHalves) {
     if (part < a.query_warps)
-      token_rows<In, Cache, kMode, kStores, false>(a, token, part, a.query_warps);
+      token_rows<In, Cache, kMode, kStores, false, kBatch>(a, token, part, a.query_warps);
     else
-      token_rows<In, Cache, kMode, kStores, true>(a, token, part - a.query_warps, a.token_warps - a.query_warps);
+      token_rows<In, Cache, kMode, kStores, true, kBatch>(a, token, part - a.query_warps, a.token_warps - a.query_warps);
   } else {
-    token_rows<In, Cache, kMode, kStores, false>(a, token, part, a.token_warps);
+    token_rows<In, Cache, kMode, kStores, false, kBatch>(a, token, part, a.token_warps);
   }
 }
 
-// Warps of a token for so many of its rows, in turns of `rows`: one turn each
-// while that leaves SMs without work, three else (the angles are loaded once).
-int warps_for(int64_t tokens, int heads, int rows, int sms) {
-  const int turns = (heads + rows - 1) / rows;
-  return tokens * turns <= static_cast<int64_t>(sms) * 16 ? turns : (turns + 2) / 3;
-}
+constexpr int kTurns = 3;  // of a warp, where there are tokens enough
 
 template <typename In, typename Cache, int kMode, bool kStores>
 cudaError_t launch_mode(TokenArgs a, int sms, cudaStream_t stream) {
   constexpr bool kFour = kStores && Cache::kBytes == 0;
   const int kv = kStores ? 2 * a.kv_heads : 0;
+  // Turns of a token's heads, `rows` at a time; of queries by themselves, and of
+  // what is stored in 4 bits (16 dims to a lane).
+  const auto turns_of = [](int heads, int rows) { return (heads + rows - 1) / rows; };
+  int turns = 0, query_turns = 0;
   if constexpr (kMode == kTurnHalves) {
-    const int lanes = a.rotary / 16 + (a.dim - a.rotary) / 8;
-    a.token_warps = warps_for(a.rows, a.q_heads + kv, 32 / lanes, sms);
+    turns = turns_of(a.q_heads + kv, 32 / (a.rotary / 16 + (a.dim - a.rotary) / 8));
   } else if constexpr (kFour) {
-    a.query_warps = a.q_heads > 0 ? warps_for(a.rows, a.q_heads, 32 / (a.dim / 8), sms) : 0;
-    a.token_warps = a.query_warps + warps_for(a.rows, kv, 32 / (a.dim / 16), sms);
+    query_turns = turns_of(a.q_heads, 32 / (a.dim / 8));
+    turns = turns_of(kv, 32 / (a.dim / 16));
   } else {
-    a.token_warps = warps_for(a.rows, a.q_heads + kv, 32 / (a.dim / 8), sms);
+    turns = turns_of(a.q_heads + kv, 32 / (a.dim / 8));
   }
+  // A turn per warp while that leaves SMs without work, kTurns else (the angles are
+  // loaded once for them, the rows together).
+  const bool few = a.rows * (turns + query_turns) <= static_cast<int64_t>(sms) * 16;
+  const int each = few ? 1 : kTurns;
+  a.query_warps = (query_turns + each - 1) / each;
+  a.token_warps = a.query_warps + (turns + each - 1) / each;
   const int64_t warps = a.rows * a.token_warps;
   const dim3 grid(static_cast<unsigned>((warps + kTokenWarps - 1) / kTokenWarps));
-  token_rows_kernel<In, Cache, kMode, kStores><<<grid, 32 * kTokenWarps, 0, stream>>>(a);
+  if (few)
+    token_rows_kernel<In, Cache, kMode, kStores, 1><<<grid, 32 * kTokenWarps, 0, stream>>>(a);
+  else
+    token_rows_kernel<In, Cache, kMode, kStores, kTurns><<<grid, 32 * kTokenWarps, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
@@ -473,54 +495,87 @@ cudaError_t launch_rows(const TokenArgs& a, int sms, cudaStream_t stream) {
 // Back from 8 or 4 bits
 // ---------------------------------------------------------------------------
 
+constexpr int kReadThreads = 256;
+constexpr int kReadUnits = 4;  // of 8 values, of a thread
+
+// A block reads `tokens` rows, a thread 8 values of one at a time.  Bound by HBM.
 template <typename Out, bool kFour>
-__global__ void __launch_bounds__(256) read_rows_kernel(const __grid_constant__ ReadArgs a) {
-  const int lanes = a.heads * (a.dim / 8);  // of 8 values each, per token
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t token = i / lanes;
-  if (token >= a.rows) return;
-  const int at = static_cast<int>(i - token * lanes);
-  const int64_t slot = __ldg(a.slots + token);
-  if (slot < 0) return;
-  if (slot >= a.num_slots) {
-    report(a.status, KVCA_ERR_BAD_INDEX, slot);
-    return;
-  }
-  const int64_t block = a.block_shift >= 0 ? slot >> a.block_shift : slot / a.block_size;
-  const char* const row = a.cache + block * a.cache_block + (slot - block * a.block_size) * a.cache_token;
-  const int h = at / (a.dim / 8), d0 = (at - h * (a.dim / 8)) * 8;
-  float x[8];
-  if constexpr (kFour) {
-    const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(row) + at);
-    const float unit =
-        e4m3_to_float(__ldg(reinterpret_cast<const uint8_t*>(row) + a.heads * (a.dim / 2) + at / 2)) * a.scale;
+__global__ void __launch_bounds__(kReadThreads) read_rows_kernel(const __grid_constant__ ReadArgs a, int tokens,
+                                                                uint32_t reciprocal) {
+  const uint32_t lanes = a.heads * (a.dim / 8);  // units of a token
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * tokens;
+  const uint32_t units = static_cast<uint32_t>(min(static_cast<int64_t>(tokens), a.rows - first)) * lanes;
+#pragma unroll 1
+  for (uint32_t base = threadIdx.x; base < units; base += kReadThreads * kReadUnits) {
+    uint2 raw[kReadUnits];
+    uint32_t scale[kReadUnits];
+    bool live[kReadUnits];
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const float2 f = unpack2<false>(e2m1_to_f16x2(word >> (4 * e)));
-      x[e] = f.x * unit, x[e + 1] = f.y * unit;
+    for (int u = 0; u < kReadUnits; ++u) {
+      const uint32_t i = base + u * kReadThreads;
+      live[u] = false;
+      if (i >= units) continue;
+      const uint32_t token = __umulhi(i, reciprocal);  // i / lanes
+      const uint32_t at = i - token * lanes;
+      const int64_t slot = __ldg(a.slots + first + token);
+      if (slot < 0) continue;
+      if (slot >= a.num_slots) {
+        report(a.status, KVCA_ERR_BAD_INDEX, slot);
+        continue;
+      }
+      live[u] = true;
+      const int64_t block = a.block_shift >= 0 ? slot >> a.block_shift : slot / a.block_size;
+      const char* const row = a.cache + block * a.cache_block + (slot - block * a.block_size) * a.cache_token;
+      if constexpr (kFour) {
+        raw[u].x = __ldg(reinterpret_cast<const uint32_t*>(row) + at);
+        scale[u] = __ldg(reinterpret_cast<const uint8_t*>(row) + a.heads * (a.dim / 2) + at / 2);
+      } else {
+        const uint32_t h = at / (a.dim / 8);
+        raw[u] = __ldg(reinterpret_cast<const uint2*>(row + h * a.cache_head + (at - h * (a.dim / 8)) * 8));
+      }
     }
-  } else {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(row + h * a.cache_head + d0));
-    const uint32_t w[4] = {v.x, v.x >> 16, v.y, v.y >> 16};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = unpack2<false>(e4m3_to_f16x2(w[e]));
-      x[2 * e] = f.x * a.scale, x[2 * e + 1] = f.y * a.scale;
+    for (int u = 0; u < kReadUnits; ++u) {
+      if (!live[u]) continue;
+      float x[8];
+      if constexpr (kFour) {
+        const float unit = e4m3_to_float(scale[u]) * a.scale;
+        uint32_t w[4];
+        e2m1x8_to_f16x2(w, raw[u].x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack2<false>(w[e]);
+          x[2 * e] = f.x * unit, x[2 * e + 1] = f.y * unit;
+        }
+      } else {
+        const uint32_t w[4] = {raw[u].x, raw[u].x >> 16, raw[u].y, raw[u].y >> 16};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack2<false>(e4m3_to_f16x2(w[e]));
+          x[2 * e] = f.x * a.scale, x[2 * e + 1] = f.y * a.scale;
+        }
+      }
+      Raw8<Out> wide;
+      wide.set(x);
+      wide.store(a.out + (first * lanes + base + u * kReadThreads) * 8 * Out::kBytes);
     }
   }
-  Raw8<Out> raw;
-  raw.set(x);
-  raw.store(a.out + (token * lanes + at) * 8 * Out::kBytes);
 }
 
 template <typename Out>
-cudaError_t launch_read_to(const ReadArgs& a, cudaStream_t stream) {
-  const int64_t threads = a.rows * a.heads * (a.dim / 8);
-  const dim3 grid(static_cast<unsigned>((threads + 255) / 256));
+cudaError_t launch_read_to(const ReadArgs& a, int sms, cudaStream_t stream) {
+  const int64_t lanes = static_cast<int64_t>(a.heads) * (a.dim / 8);  // 32,768 at most
+  // kReadUnits rounds of a block where there are rows enough for all SMs
+  int64_t tokens = kReadThreads * kReadUnits / lanes;
+  while (tokens > 1 && (a.rows + tokens - 1) / tokens < 4 * sms) tokens /= 2;
+  if (tokens < 1) tokens = 1;
+  const dim3 grid(static_cast<unsigned>((a.rows + tokens - 1) / tokens));
+  // exact for i below 2^16 or a token's own 2^15: i * lanes < 2^32
+  const uint32_t reciprocal = static_cast<uint32_t>(((int64_t{1} << 32) + lanes - 1) / lanes);
   if (a.cache_type == KVCA_TYPE_E2M1)
-    read_rows_kernel<Out, true><<<grid, 256, 0, stream>>>(a);
+    read_rows_kernel<Out, true><<<grid, kReadThreads, 0, stream>>>(a, static_cast<int>(tokens), reciprocal);
   else
-    read_rows_kernel<Out, false><<<grid, 256, 0, stream>>>(a);
+    read_rows_kernel<Out, false><<<grid, kReadThreads, 0, stream>>>(a, static_cast<int>(tokens), reciprocal);
   return cudaGetLastError();
 }
 
@@ -545,11 +600,11 @@ cudaError_t launch_rotate_tokens(const TokenArgs& a, int type, int sms, cudaStre
   }
 }
 
-cudaError_t launch_read_tokens(const ReadArgs& a, int type, cudaStream_t stream) {
+cudaError_t launch_read_tokens(const ReadArgs& a, int type, int sms, cudaStream_t stream) {
   switch (type) {
-    case KVCA_TYPE_F16: return launch_read_to<CacheF16>(a, stream);
-    case KVCA_TYPE_BF16: return launch_read_to<CacheBf16>(a, stream);
-    default: return launch_read_to<InF32>(a, stream);
+    case KVCA_TYPE_F16: return launch_read_to<CacheF16>(a, sms, stream);
+    case KVCA_TYPE_BF16: return launch_read_to<CacheBf16>(a, sms, stream);
+    default: return launch_read_to<InF32>(a, sms, stream);
   }
 }
 

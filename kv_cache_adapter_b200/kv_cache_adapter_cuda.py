@@ -1753,67 +1753,85 @@ def _e2m1_heads(cache: torch.Tensor, dim: int, name: str) -> int:
     return heads
 
 
-def _span(t: torch.Tensor) -> tuple[int, int]:
-    """First and last address (past it) of a tensor's elements."""
-    at = t.data_ptr()
-    return at, at + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else at
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    return a0 < b1 and b0 < a1
-
-
-def _distinct(t: torch.Tensor, name: str) -> None:
-    """No two elements of a tensor that is written share a place."""
-    if t.is_contiguous():
-        return
-    end = 1
-    for stride, size in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
-        if stride < end:
-            raise ValueError(f"{name}: elements must not share memory")
-        end = stride * (size - 1) + end
-
-
-def _token_rows(t: torch.Tensor, dev: torch.device, name: str) -> None:
+def _token_rows(t: torch.Tensor, index: int, dtype: torch.dtype | None, size: int,
+                name: str) -> tuple[int, int, int, int]:
+    """The checked address of rows (rows, heads, head_dim), their strides in bytes
+    (0 for a dim of size 1) and where their memory ends."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be torch.Tensor")
-    if t.device != dev:
-        raise ValueError(f"{name} must be on {dev}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be on cuda:{index}")
     if t.dim() != 3:
         raise ValueError(f"{name} must be (rows, heads, head_dim)")
+    if dtype is not None and t.dtype is not dtype:
+        raise TypeError(f"{name} has incorrect dtype {t.dtype}")
+    rows, heads, dim = t.shape
+    row, head, last = t.stride()
+    row = row * size if rows > 1 else 0
+    head = head * size if heads > 1 else 0
+    at = t.data_ptr()
+    if (at | row | head) & 15 or (last != 1 and rows):
+        raise ValueError(f"{name}: rows of head_dim must be contiguous and 16-byte aligned")
+    return at, row, head, at + (rows - 1) * row + (heads - 1) * head + dim * size if rows else at
 
 
-def _rotation(table: torch.Tensor, positions: torch.Tensor, rows: int, dim: int, dev: torch.device) -> None:
+def _distinct(sizes, strides, unit: int, name: str) -> None:
+    """No two elements of a tensor that is written share a place: rows of `unit`
+    bytes, in dims of these sizes and strides in bytes."""
+    end = unit
+    for stride, size in sorted(zip(strides, sizes)):
+        if size > 1:
+            if stride < end:
+                raise ValueError(f"{name}: elements must not share memory")
+            end += stride * (size - 1)
+
+
+def _index_rows(t: torch.Tensor, index: int, rows: int, name: str) -> int:
+    """The address of an int64 entry per row."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.int64 and t.dim() == 1 and t.get_device() == index
+            and t.is_contiguous()):
+        _require_index(t, torch.device("cuda", index), name)
+    if t.shape[0] != rows:
+        raise ValueError(f"{name} needs one entry per row")
+    return t.data_ptr()
+
+
+def _rotation(table: torch.Tensor, index: int, dim: int) -> tuple[int, int, int]:
+    """Address, positions and rotary_dim of a rotation's table."""
     if not isinstance(table, torch.Tensor):
         raise TypeError("table must be torch.Tensor")
     if table.dtype is not torch.float32:
         raise TypeError(f"table has incorrect dtype {table.dtype}")
-    if table.device != dev or table.dim() != 2 or not table.is_contiguous() or table.data_ptr() % 16:
-        raise ValueError(f"table must be a contiguous, 16-byte aligned (positions, rotary_dim) tensor on {dev}")
-    positions_held, rotary = table.shape
-    if positions_held < 1:
+    at = table.data_ptr()
+    if table.get_device() != index or table.dim() != 2 or not table.is_contiguous() or at & 15:
+        raise ValueError(f"table must be a contiguous, 16-byte aligned (positions, rotary_dim) tensor on cuda:{index}")
+    held, rotary = table.shape
+    if held < 1:
         raise ValueError("table holds no positions")
     if rotary < 2 or rotary % 2 or rotary > dim:
         raise ValueError(f"the table's rotary_dim must be even and at most head_dim {dim}, got {rotary}")
-    _ids(positions, dev, "positions")
-    if positions.shape[0] != rows:
-        raise ValueError("positions needs one entry per row")
+    return at, held, rotary
 
 
-def _result_rows(out: torch.Tensor | None, x: torch.Tensor, name: str) -> torch.Tensor:
-    """The result of rows x: x itself, or a tensor that nothing of x lies in."""
+def _result_rows(out: torch.Tensor | None, x: torch.Tensor, at: tuple[int, int, int, int], index: int, size: int,
+                 name: str) -> tuple[torch.Tensor, tuple[int, int, int, int]]:
+    """The result of the rows x (`at`: _token_rows): x itself, or a tensor that
+    nothing of x lies in, and its _token_rows."""
     if out is None:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if out is not x:
-        _token_rows(out, x.device, name)
-    _distinct(out, name)
-    if out.shape != x.shape or out.dtype is not x.dtype:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    to = at if out is x else _token_rows(out, index, x.dtype, size, name)
+    if out.shape != x.shape:
         raise ValueError(f"{name} must be {tuple(x.shape)} {x.dtype}")
-    same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
-    if not same and _overlap(out, x):
+    rows, heads, dim = x.shape
+    _distinct((rows, heads), to[1:3], dim * size, name)
+    if to[0] < at[3] and at[0] < to[3] and to != at:
         raise ValueError(f"{name} must not overlap what it is computed from (unless it is the same rows)")
-    return out
+    return out, to
+
+
+_pack_rotate = _lib.packer(_lib.RotateDesc)
+_pack_append = _lib.packer(_lib.AppendDesc)
+_pack_read = _lib.packer(_lib.ReadDesc)
 
 
 def rotate_tokens(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, *, interleaved: bool = False,
@@ -1828,37 +1846,50 @@ def rotate_tokens(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor,
     itself; rows of negative position are left as they were in it."""
     if not isinstance(x, torch.Tensor):
         raise TypeError("x must be torch.Tensor")
-    if not x.is_cuda:
+    index = x.get_device()
+    if index < 0:
         raise ValueError("x must be a CUDA tensor")
-    if x.dtype not in _ROW_TYPES:
-        raise TypeError(f"x has incorrect dtype {x.dtype}")
-    dev = x.device
-    _token_rows(x, dev, "x")
+    dtype = x.dtype
+    kind = _ROW_TYPES.get(dtype)
+    if kind is None:
+        raise TypeError(f"x has incorrect dtype {dtype}")
+    size = 4 if dtype is torch.float32 else 2
+    at = _token_rows(x, index, None, size, "x")
     rows, heads, dim = x.shape
     if heads < 1 or dim < 8 or dim > 256 or dim % 8:
         raise ValueError(f"x must have heads, and a head_dim in multiples of 8 up to 256, got {heads} and {dim}")
-    _rotation(table, positions, rows, dim, dev)
-    strides = _attend_rows(x, x.shape, "x")
-    out = _result_rows(out, x, "out")
-    if _overlap(out, table) or _overlap(out, positions):
+    angles, held, rotary = _rotation(table, index, dim)
+    at_positions = _index_rows(positions, index, rows, "positions")
+    out, to = _result_rows(out, x, at, index, size, "out")
+    if (to[0] < angles + 4 * held * rotary and angles < to[3]
+            or to[0] < at_positions + 8 * rows and at_positions < to[3]):
         raise ValueError("out must not overlap table or positions")
     if rows == 0:
         return out
-    desc = _lib.RotateDesc(rows, x.data_ptr(), *strides, out.data_ptr(), *_attend_rows(out, out.shape, "out"),
-                           positions.data_ptr(), table.data_ptr() or None, table.shape[0], heads, dim, table.shape[1],
-                           _ROW_TYPES[x.dtype], bool(interleaved), bool(transpose))
+    dev = x.device
+    desc = _pack_rotate(rows, at[0], at[1], at[2], to[0], to[1], to[2], at_positions, angles, held, heads, dim, rotary,
+                        kind, bool(interleaved), bool(transpose))
     with _on(dev):
-        rc = _lib_handle.kvca_rotate_tokens(ctypes.byref(desc), _status(dev).data_ptr(), _stream(dev))
+        rc = _lib_handle.kvca_rotate_tokens(desc, _status(dev).data_ptr(), _stream(dev))
     _host_rc(rc, "rotate_tokens")
     _maybe_check(dev, check, "rotate_tokens")
     return out
 
 
-def _cache_side(cache: torch.Tensor, heads: int, dim: int, name: str) -> list[int]:
-    """Strides in bytes of a cache plane's blocks, tokens and heads."""
-    if cache.dtype is not torch.uint8:
-        return _attend_rows(cache, cache.shape, name)
-    return [*_attend_rows(cache, cache.shape, name), dim // 2]
+def _cache_rows(cache: torch.Tensor, size: int, head: int, name: str) -> tuple[int, int, int, int, int]:
+    """The checked address of a cache plane (rows of `size` bytes per element; `head`:
+    bytes between heads where rows hold all of them), its strides in bytes, and
+    where it ends."""
+    shape, stride = cache.shape, cache.stride()
+    at = cache.data_ptr()
+    steps = [x * size if n > 1 else 0 for n, x in zip(shape[:-1], stride)]
+    bits, end = at, at + shape[-1] * size
+    for n, x in zip(shape, steps):
+        bits |= x
+        end += (n - 1) * x
+    if bits & 15 or (stride[-1] != 1 and cache.numel()):
+        raise ValueError(f"{name}: rows of head_dim must be contiguous and 16-byte aligned")
+    return at, steps[0], steps[1], steps[2] if len(steps) == 3 else head, end if cache.numel() else at
 
 
 def append_tokens(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -1880,81 +1911,84 @@ def append_tokens(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tenso
     without them keys are stored as they are.  Returns ``query_out`` (the query
     itself if given as such), None without a query."""
     tensor = torch.Tensor
-    for t, name in ((key, "key"), (value, "value"), (key_cache, "key_cache"), (value_cache, "value_cache"),
-                    (slot_mapping, "slot_mapping")):
-        if not isinstance(t, tensor):
-            raise TypeError(f"{name} must be torch.Tensor")
-    if not key.is_cuda:
+    if not (isinstance(key, tensor) and isinstance(value, tensor) and isinstance(key_cache, tensor)
+            and isinstance(value_cache, tensor)):
+        for t, name in ((key, "key"), (value, "value"), (key_cache, "key_cache"), (value_cache, "value_cache")):
+            if not isinstance(t, tensor):
+                raise TypeError(f"{name} must be torch.Tensor")
+    index, dtype, ctype = key.get_device(), key.dtype, key_cache.dtype
+    if index < 0:
         raise ValueError("key must be a CUDA tensor")
-    dev, dtype, ctype = key.device, key.dtype, key_cache.dtype
     if dtype is not torch.float16 and dtype is not torch.bfloat16:
         raise TypeError(f"key has incorrect dtype {dtype}")
-    _token_rows(key, dev, "key")
-    _token_rows(value, dev, "value")
+    k = _token_rows(key, index, None, 2, "key")
+    v = _token_rows(value, index, dtype, 2, "value")
     rows, heads, dim = key.shape
-    if value.shape != key.shape or value.dtype is not dtype:
+    if value.shape != key.shape:
         raise ValueError("key and value must share shape and dtype")
-    four = ctype is torch.uint8
-    if not four and ctype is not torch.float8_e4m3fn and ctype is not dtype:
+    four, same = ctype is torch.uint8, ctype is dtype
+    if not four and not same and ctype is not torch.float8_e4m3fn:
         raise TypeError(f"key_cache has incorrect dtype {ctype}")
-    if value_cache.dtype is not ctype or value_cache.shape != key_cache.shape:
+    cshape = key_cache.shape
+    if value_cache.dtype is not ctype or value_cache.shape != cshape:
         raise ValueError("key_cache and value_cache must share shape and dtype")
-    if key_cache.device != dev or value_cache.device != dev:
-        raise ValueError(f"key_cache and value_cache must be on {dev}")
-    if heads < 1 or dim < 8 or dim > 256 or dim % (32 if four else 16 if ctype is not dtype else 8):
+    if key_cache.get_device() != index or value_cache.get_device() != index:
+        raise ValueError(f"key_cache and value_cache must be on cuda:{index}")
+    if heads < 1 or dim < 8 or dim > 256 or dim % (32 if four else 8 if same else 16):
         raise ValueError(f"heads or head_dim out of range: {heads} and {dim}")
     if four:
         if _e2m1_heads(key_cache, dim, "key_cache") != heads:
             raise ValueError(f"the caches do not hold {heads} heads of {dim}")
-    elif key_cache.dim() != 4 or key_cache.shape[2:] != (heads, dim):
+    elif len(cshape) != 4 or cshape[2] != heads or cshape[3] != dim:
         raise ValueError(f"the caches must be (num_blocks, block_size, {heads}, {dim})")
-    num_blocks, block_size = key_cache.shape[:2]
-    if block_size < 1:
+    if cshape[1] < 1:
         raise ValueError("block_size must be positive")
-    if ctype is dtype and (key_scale != 1.0 or value_scale != 1.0):
+    if same and (key_scale != 1.0 or value_scale != 1.0):
         raise ValueError("key_scale and value_scale belong to a cache of 8 or 4 bits")
     if not (2.0 ** -60 <= key_scale <= 2.0 ** 60 and 2.0 ** -60 <= value_scale <= 2.0 ** 60):
         raise ValueError("key_scale and value_scale must be positive (2^-60 to 2^60)")
-    _ids(slot_mapping, dev, "slot_mapping")
-    if slot_mapping.shape[0] != rows:
-        raise ValueError("slot_mapping needs one entry per row")
+    size = 2 if same else 1
+    kc = _cache_rows(key_cache, size, dim // 2, "key_cache")
+    vc = _cache_rows(value_cache, size, dim // 2, "value_cache")
+    if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+        for c, name in ((kc, "key_cache"), (vc, "value_cache")):
+            _distinct(cshape[:-1], c[1:len(cshape)], cshape[-1] * size, name)
+    at_slots = _index_rows(slot_mapping, index, rows, "slot_mapping")
     if (positions is None) != (table is None):
         raise ValueError("positions and table go together")
+    at_positions = angles = held = rotary = 0
     if table is not None:
-        _rotation(table, positions, rows, dim, dev)
-    q = (0, 0, 0, 0, 0, 0)
+        angles, held, rotary = _rotation(table, index, dim)
+        at_positions = _index_rows(positions, index, rows, "positions")
+    q = q_out = (0, 0, 0, 0)
     q_heads = 0
     if query is not None:
-        _token_rows(query, dev, "query")
+        q = _token_rows(query, index, dtype, 2, "query")
         if table is None:
             raise ValueError("query needs positions and table")
         q_heads = query.shape[1]
-        if query.shape[0] != rows or query.shape[2] != dim or query.dtype is not dtype or q_heads < 1:
+        if query.shape[0] != rows or query.shape[2] != dim or q_heads < 1:
             raise ValueError(f"query must be ({rows}, heads, {dim}) {dtype}")
-        query_out = _result_rows(query_out, query, "query_out")
-        if query_out.data_ptr() != query.data_ptr() and (_overlap(query_out, key) or _overlap(query_out, value)):
+        query_out, q_out = _result_rows(query_out, query, q, index, 2, "query_out")
+        if q_out != q and (q_out[0] < k[3] and k[0] < q_out[3] or q_out[0] < v[3] and v[0] < q_out[3]):
             raise ValueError("query_out must not overlap key or value")
-        q = (query.data_ptr(), *_attend_rows(query, query.shape, "query"), query_out.data_ptr(),
-             *_attend_rows(query_out, query_out.shape, "query_out"))
     elif query_out is not None:
         raise ValueError("query_out needs a query")
-    for cache in (key_cache, value_cache):
-        _distinct(cache, "caches")
-        if any(t is not None and _overlap(cache, t) for t in (key, value, query, query_out)):
+    for c in (kc, vc):
+        begin, end = c[0], c[4]
+        if (begin < k[3] and k[0] < end or begin < v[3] and v[0] < end or begin < q[3] and q[0] < end
+                or begin < q_out[3] and q_out[0] < end):
             raise ValueError("the caches must not overlap the rows")
-    if key_cache.data_ptr() == value_cache.data_ptr() and key_cache.numel():
+    if kc[0] == vc[0] and kc[4] > kc[0]:
         raise ValueError("key_cache and value_cache must be two caches")
-    desc = _lib.AppendDesc(
-        rows, *q, key.data_ptr(), *_attend_rows(key, key.shape, "key"), value.data_ptr(),
-        *_attend_rows(value, value.shape, "value"), key_cache.data_ptr(), *_cache_side(key_cache, heads, dim, "key_cache"),
-        value_cache.data_ptr(), *_cache_side(value_cache, heads, dim, "value_cache"), num_blocks, block_size,
-        slot_mapping.data_ptr() or None, None if positions is None else positions.data_ptr() or None,
-        None if table is None else table.data_ptr() or None, 0 if table is None else table.shape[0], q_heads, heads, dim,
-        0 if table is None else table.shape[1], _ROW_TYPES[dtype],
-        _lib.KVCA_TYPE_E2M1 if four else _ATTEND_TYPES[ctype], bool(interleaved), key_scale, value_scale)
     if rows:
+        dev = key.device
+        desc = _pack_append(
+            rows, q[0], q[1], q[2], q_out[0], q_out[1], q_out[2], k[0], k[1], k[2], v[0], v[1], v[2], kc[0], kc[1], kc[2],
+            kc[3], vc[0], vc[1], vc[2], vc[3], cshape[0], cshape[1], at_slots, at_positions, angles, held, q_heads, heads,
+            dim, rotary, _ROW_TYPES[dtype], _ATTEND_TYPES[ctype], bool(interleaved), key_scale, value_scale)
         with _on(dev):
-            rc = _lib_handle.kvca_append_tokens(ctypes.byref(desc), _status(dev).data_ptr(), _stream(dev))
+            rc = _lib_handle.kvca_append_tokens(desc, _status(dev).data_ptr(), _stream(dev))
         _host_rc(rc, "append_tokens")
         _maybe_check(dev, check, "append_tokens")
     return query_out
@@ -1971,14 +2005,16 @@ def read_tokens(cache: torch.Tensor, slot_mapping: torch.Tensor, *, head_dim: in
     negative slot are left as they were in ``out``."""
     if not isinstance(cache, torch.Tensor):
         raise TypeError("cache must be torch.Tensor")
-    if not cache.is_cuda:
+    index = cache.get_device()
+    if index < 0:
         raise ValueError("cache must be a CUDA tensor")
     dev = cache.device
     four = cache.dtype is torch.uint8
     if four:
         if head_dim is None:
             raise ValueError("a 4-bit cache needs head_dim")
-        heads, dim = _e2m1_heads(cache, int(head_dim), "cache"), int(head_dim)
+        dim = int(head_dim)
+        heads = _e2m1_heads(cache, dim, "cache")
     elif cache.dtype is torch.float8_e4m3fn:
         if cache.dim() != 4:
             raise ValueError("cache must be (num_blocks, block_size, kv_heads, head_dim)")
@@ -1989,29 +2025,30 @@ def read_tokens(cache: torch.Tensor, slot_mapping: torch.Tensor, *, head_dim: in
             raise ValueError(f"heads or head_dim out of range: {heads} and {dim}")
     else:
         raise TypeError(f"cache has incorrect dtype {cache.dtype}")
-    if cache.shape[1] < 1:
+    num_blocks, block_size = cache.shape[:2]
+    if block_size < 1:
         raise ValueError("block_size must be positive")
-    _ids(slot_mapping, dev, "slot_mapping")
-    rows = slot_mapping.shape[0]
+    c = _cache_rows(cache, 1, dim // 2, "cache")
+    if not isinstance(slot_mapping, torch.Tensor):
+        raise TypeError("slot_mapping must be torch.Tensor")
+    rows = slot_mapping.numel()
+    at_slots = _index_rows(slot_mapping, index, rows, "slot_mapping")
+    kind = _ROW_TYPES.get(dtype if out is None else out.dtype if isinstance(out, torch.Tensor) else None)
+    if kind is None:
+        raise TypeError(f"incorrect dtype {dtype}" if out is None else "out has incorrect dtype")
     if out is None:
-        if dtype not in _ROW_TYPES:
-            raise TypeError(f"incorrect dtype {dtype}")
         out = torch.empty((rows, heads, dim), dtype=dtype, device=dev)
-    else:
-        _token_rows(out, dev, "out")
-        if out.dtype not in _ROW_TYPES:
-            raise TypeError(f"out has incorrect dtype {out.dtype}")
-        if out.shape != (rows, heads, dim) or not out.is_contiguous() or out.data_ptr() % 16:
-            raise ValueError(f"out must be a contiguous, 16-byte aligned ({rows}, {heads}, {dim}) tensor on {dev}")
-        if _overlap(out, cache) or _overlap(out, slot_mapping):
-            raise ValueError("out must not overlap cache or slot_mapping")
-    strides = _cache_side(cache, heads, dim, "cache")
+    at = out.data_ptr()
+    if out.shape != (rows, heads, dim) or out.get_device() != index or not out.is_contiguous() or at & 15:
+        raise ValueError(f"out must be a contiguous, 16-byte aligned ({rows}, {heads}, {dim}) tensor on cuda:{index}")
+    end = at + rows * heads * dim * (4 if kind == _lib.KVCA_TYPE_F32 else 2)
+    if at < c[4] and c[0] < end or at < at_slots + 8 * rows and at_slots < end:
+        raise ValueError("out must not overlap cache or slot_mapping")
     if rows:
-        desc = _lib.ReadDesc(cache.data_ptr(), *strides, cache.shape[0], cache.shape[1], slot_mapping.data_ptr(), rows,
-                             heads, dim, _lib.KVCA_TYPE_E2M1 if four else _lib.KVCA_TYPE_E4M3, _ROW_TYPES[out.dtype],
-                             scale, 0, out.data_ptr())
+        desc = _pack_read(c[0], c[1], c[2], c[3], num_blocks, block_size, at_slots, rows, heads, dim,
+                          _lib.KVCA_TYPE_E2M1 if four else _lib.KVCA_TYPE_E4M3, kind, scale, 0, at)
         with _on(dev):
-            rc = _lib_handle.kvca_read_tokens(ctypes.byref(desc), _status(dev).data_ptr(), _stream(dev))
+            rc = _lib_handle.kvca_read_tokens(desc, _status(dev).data_ptr(), _stream(dev))
         _host_rc(rc, "read_tokens")
         _maybe_check(dev, check, "read_tokens")
     return out

@@ -120,13 +120,18 @@ def test_python_refuses_cpu_tensors():
 
 
 def test_elements_of_results_share_no_memory():
-    base = torch.zeros(100)
-    ops._distinct(base.view(10, 10).t(), "x")
-    ops._distinct(base.as_strided((3, 2, 4), (20, 4, 1)), "x")
-    ops._distinct(base.as_strided((1, 2, 4), (0, 4, 1)), "x")
-    for shape, stride in (((2, 3, 4), (0, 4, 1)), ((2, 3, 4), (8, 4, 1)), ((5, 1, 4), (3, 1, 1))):
+    ops._distinct((10, 10), (4, 40), 4, "x")
+    ops._distinct((3, 2), (80, 16), 16, "x")
+    ops._distinct((1, 2), (0, 16), 16, "x")
+    for sizes, strides in (((2, 3), (0, 16)), ((2, 3), (32, 16)), ((5, 1), (8, 0))):
         with pytest.raises(ValueError, match="share"):
-            ops._distinct(base.as_strided(shape, stride), "x")
+            ops._distinct(sizes, strides, 16, "x")
+
+
+def test_packed_descriptors():
+    for desc in (_lib.RotateDesc, _lib.AppendDesc, _lib.ReadDesc):
+        values = [n + 1 for n in range(len(desc._fields_))]
+        assert _lib.packer(desc)(*values) == bytes(desc(*values))
 
 
 def test_table():
