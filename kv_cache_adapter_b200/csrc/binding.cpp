@@ -967,7 +967,8 @@ int64_t kvca_e2m1_row_bytes(int64_t kv_heads, int64_t head_dim) {
 
 namespace {
 
-constexpr int64_t kMostTokenRows = int64_t{1} << 24;  // x at most 65,536 heads: a grid's blocks
+// Rows of a call, and rows of its heads: the warps of a grid are counted in 32 bits.
+constexpr int64_t kMostTokenRows = int64_t{1} << 24, kMostHeadRows = int64_t{1} << 31;
 
 int log2_or_minus(int64_t x) {
   for (int b = 0; b < 31; ++b)
@@ -1005,7 +1006,8 @@ int kvca_rotate_tokens(const kvca_rotate_desc* d, int64_t* d_status, kvca_stream
                             static_cast<uint64_t>(d->out_row_stride), static_cast<uint64_t>(d->out_head_stride),
                             reinterpret_cast<uint64_t>(d->table)};
   if (!all_aligned16(words)) return KVCA_ERR_BAD_ARGUMENT;
-  if (d->num_rows > kMostTokenRows || d->heads > 65536) return KVCA_ERR_SIZE_LIMIT;
+  if (d->num_rows > kMostTokenRows || d->heads > 65536 || d->num_rows * d->heads > kMostHeadRows)
+    return KVCA_ERR_SIZE_LIMIT;
   if (d->num_rows == 0) return KVCA_OK;
   if (d->x == 0 || d->out == 0 || d->positions == nullptr || d->table == nullptr) return KVCA_ERR_BAD_ARGUMENT;
   kvca::TokenArgs a;
@@ -1060,6 +1062,7 @@ int kvca_append_tokens(const kvca_append_desc* d, int64_t* d_status, kvca_stream
   kvca::TokenArgs a;
   memset(&a, 0, sizeof(a));
   if (d->num_rows > kMostTokenRows || d->q_heads > 65536 || d->kv_heads > 65536 ||
+      d->num_rows * (d->q_heads + 2 * static_cast<int64_t>(d->kv_heads)) > kMostHeadRows ||
       !cache_slots(d->num_blocks, d->block_size, &a.num_slots, &a.block_size, &a.block_shift))
     return KVCA_ERR_SIZE_LIMIT;
   if (d->num_rows == 0) return KVCA_OK;

@@ -433,10 +433,17 @@ __device__ __forceinline__ void token_rows(const TokenArgs& a, int64_t token, in
   }
 }
 
+// Blocks per SM that the registers leave room for: bound by how many rows are on
+// their way, so 28 warps with two turns each at 72 registers beat 20 with three at
+// 96 (prompt of 16,384 tokens, 48 heads: 74 us and 77).  The other modes take what
+// they need.
+template <int kMode>
+constexpr int kTokenBlocks = kMode == kTurnHalves ? 7 : 1;
+
 template <typename In, typename Cache, int kMode, bool kStores, int kBatch>
-__global__ void __launch_bounds__(32 * kTokenWarps) token_rows_kernel(const __grid_constant__ TokenArgs a) {
-  const int64_t warp = static_cast<int64_t>(blockIdx.x) * kTokenWarps + (threadIdx.x >> 5);
-  const int64_t token = warp / a.token_warps;
+__global__ void __launch_bounds__(32 * kTokenWarps, kTokenBlocks<kMode>) token_rows_kernel(const __grid_constant__ TokenArgs a) {
+  const uint32_t warp = blockIdx.x * kTokenWarps + (threadIdx.x >> 5);  // below 2^32
+  const uint32_t token = warp / a.token_warps;
   const int part = static_cast<int>(warp - token * a.token_warps);
   if (token >= a.rows) return;
   if constexpr (kStores && Cache::kBytes == 0 && kMode != kTurnHalves) {
@@ -449,7 +456,10 @@ __global__ void __launch_bounds__(32 * kTokenWarps) token_rows_kernel(const __gr
   }
 }
 
-constexpr int kTurns = 3;  // of a warp, where there are tokens enough
+// Turns of a warp at most, for which the token's angles are loaded once and its
+// slot and position looked up (the prompt of 16,384 tokens, 12 turns to a token:
+// one turn to a warp 150 us, 3 88, 12 74).
+constexpr int kTurns = 12;
 
 template <typename In, typename Cache, int kMode, bool kStores>
 cudaError_t launch_mode(TokenArgs a, int sms, cudaStream_t stream) {
@@ -467,18 +477,17 @@ cudaError_t launch_mode(TokenArgs a, int sms, cudaStream_t stream) {
   } else {
     turns = turns_of(a.q_heads + kv, 32 / (a.dim / 8));
   }
-  // A turn per warp while that leaves SMs without work, kTurns else (the angles are
-  // loaded once for them, the rows together).
-  const bool few = a.rows * (turns + query_turns) <= static_cast<int64_t>(sms) * 16;
-  const int each = few ? 1 : kTurns;
+  // Fewer turns while that leaves SMs with fewer than 16 warps.
+  const int64_t share = a.rows * (turns + query_turns) / (static_cast<int64_t>(sms) * 16);
+  const int each = static_cast<int>(share < 1 ? 1 : share < kTurns ? share : kTurns);
   a.query_warps = (query_turns + each - 1) / each;
   a.token_warps = a.query_warps + (turns + each - 1) / each;
   const int64_t warps = a.rows * a.token_warps;
   const dim3 grid(static_cast<unsigned>((warps + kTokenWarps - 1) / kTokenWarps));
-  if (few)
+  if (each == 1)
     token_rows_kernel<In, Cache, kMode, kStores, 1><<<grid, 32 * kTokenWarps, 0, stream>>>(a);
   else
-    token_rows_kernel<In, Cache, kMode, kStores, kTurns><<<grid, 32 * kTokenWarps, 0, stream>>>(a);
+    token_rows_kernel<In, Cache, kMode, kStores, 2><<<grid, 32 * kTokenWarps, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
