@@ -64,6 +64,7 @@ constexpr int kJoinThreads = 256;
 constexpr int kJoinRows = 16;   // rows per block of the join
 constexpr int kSlots = 4;       // segments announced ahead
 constexpr int kReaders = 15;    // warps that read them
+constexpr uint32_t kAhead = 2;  // tiles (of keys or values) in flight behind the one being issued
 static_assert(kSlots == 4, "marks of tiles in flight hold a slot in two bits");
 // What a segment costs beside its tiles, in tiles: queries, first loads, the
 // output.  It counts when the tiles are dealt out, as tiles before the first.
@@ -85,6 +86,10 @@ struct ChunkShape {
   static constexpr int kStages = 128 * 1024 / kTileBytes;
   static constexpr int kQueries = DP == 64 ? 2 : 1;        // segments whose queries are there at once
   static constexpr int kSmem = 1024 + (2 * kQueries + kStages) * kTileBytes;
+  // 4 bits: rows as they lie in memory, of kAhead + 1 sides (keys or values) per
+  // loading warp: 32 rows of values, then of up to 8 bytes with their scales.
+  static constexpr int kFourSide = 32 * (DP / 2 + 8);
+  static constexpr int kFourBytes = 4 * (kAhead + 1) * kFourSide;
 };
 
 // ---------------------------------------------------------------------------
@@ -187,9 +192,65 @@ __device__ __noinline__ int64_t block_incl_max(int64_t x, int64_t* sm) {
   return x;
 }
 
+// bf16 queries for the products with 4-bit keys: fp16 times a power of two per
+// row (power_up), whose inverse goes into its score factor, with the sign or the
+// zeros of the scores' factor; by all warps of blocks 1 and on, a row on dim / 8
+// lanes.  (By the two warps that fetch queries, as with e4m3 keys, it held up every
+// segment: prompts 691 us, not 420.)
+__device__ __forceinline__ void lift_queries(const AttendArgs& a, const ChunkArgs& c) {
+  const int lanes = a.dim / 8, per_warp = 32 / lanes;
+  const int lane = threadIdx.x & 31, row_of = lane / lanes, chunk = lane - row_of * lanes;
+  const int heads = a.kv_heads * a.group;
+  const int64_t total = c.rows * heads, warps = static_cast<int64_t>(gridDim.x - 1) * (kPlanThreads / 32);
+  const int64_t warp = static_cast<int64_t>(blockIdx.x - 1) * (kPlanThreads / 32) + (threadIdx.x >> 5);
+  constexpr int kBatch = 4;
+#pragma unroll 1
+  for (int64_t first = warp * per_warp; first < total; first += warps * per_warp * kBatch) {
+    uint4 x[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int64_t at = first + b * warps * per_warp + row_of;
+      x[b] = make_uint4(0, 0, 0, 0);
+      if (row_of >= per_warp || at >= total) continue;
+      const int64_t row = at / heads;
+      x[b] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.query) + row * a.query_row +
+                                                  (at - row * heads) * a.query_head) + chunk);
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int64_t at = first + b * warps * per_warp + row_of;
+      uint32_t word[4] = {x[b].x, x[b].y, x[b].z, x[b].w};
+      float2 f[4];
+      float big = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[j] = unpack2<true>(word[j]);
+        big = fmaxf(big, fmaxf(fabsf(f[j].x), fabsf(f[j].y)));
+      }
+      float all = big;  // of the row's lanes, wherever they begin
+#pragma unroll 1
+      for (int o = 1; o < lanes; ++o) {
+        const int from = row_of * lanes + (chunk + o >= lanes ? chunk + o - lanes : chunk + o);
+        all = fmaxf(all, __shfl_sync(0xffffffffu, big, from & 31));
+      }
+      const int e = power_up(all);
+      const float up = power_of_two(e);
+      if (row_of >= per_warp || at >= total) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) word[j] = (pack2<false>(f[j].x * up, f[j].y * up) & c.query_and) ^ c.query_xor;
+      reinterpret_cast<uint4*>(c.queries + at * a.dim)[chunk] = make_uint4(word[0], word[1], word[2], word[3]);
+      if (chunk == 0) c.units[at] = power_of_two(-e);
+    }
+  }
+}
+
 __global__ void __launch_bounds__(kPlanThreads) attend_chunk_plan_kernel(const __grid_constant__ AttendArgs a,
                                                                         const __grid_constant__ ChunkArgs c,
                                                                         void* workspace, int dp, int64_t ctas) {
+  if (blockIdx.x > 0) {
+    lift_queries(a, c);
+    return;
+  }
   __shared__ int64_t scan[33];
   __shared__ int64_t highest[kPlanThreads];
   ChunkWorkspace ws(workspace, dp, ctas, c.max_blocks);
@@ -626,8 +687,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     attend_chunk_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ ChunkArgs c, void* workspace) {
   using Shape = ChunkShape<DP>;
   constexpr bool kBf16 = Cache::kBf16;
+  constexpr bool kE4m3 = Cache::kBytes == 1;
   constexpr bool kFour = Cache::kBytes == 0;
-  constexpr bool kNarrow = Cache::kBytes < 2;  // widened to fp16
+  constexpr bool kNarrow = Cache::kBytes < 2;  // widened on the way
   constexpr int kStages = Shape::kStages;
   constexpr int kTileBytes = Shape::kTileBytes;
   constexpr int kQueries = Shape::kQueries;
@@ -837,7 +899,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         const Share& s = shares[segment % kSlots];
         if (s.end == s.tile) break;
-        // Queries.  With e4m3 and e2m1 they go through registers, times a power of two
+        // Queries.  With e4m3 they go through registers, times a power of two
         // per row (power_up); so they do when the sign of a negative
         // scale or the zeros of a zero one go into them.
         if (segment >= kQueries)
@@ -845,17 +907,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         const uint32_t tile = (2 * (segment % kQueries) + w) * kTileBytes;  // of this warp's 128 rows
         float* const unit_of = row_unit[segment % kQueries] + w * 128;
-        const bool as_is = !kNarrow && c.query_and == 0xffffffffu && c.query_xor == 0u;
+        const bool as_is = Cache::kLifted || (!kE4m3 && c.query_and == 0xffffffffu && c.query_xor == 0u);
 #pragma unroll 1
         for (int r0 = 0; r0 < 128 && w < s.row_tiles(); r0 += 32) {  // a lane finds one of 32 rows
           const int r = w * 128 + r0 + lane;
           const int row = s.view.row + r, token = row / a.group;
-          const uint16_t* own = static_cast<const uint16_t*>(a.query) + (s.out_row + token) * a.query_row +
-                                static_cast<int64_t>(s.head * a.group + row - token * a.group) * a.query_head;
+          const int q_head = s.head * a.group + row - token * a.group;
+          const int64_t lifted = (s.out_row + token) * (static_cast<int64_t>(a.kv_heads) * a.group) + q_head;
+          const uint16_t* own = Cache::kLifted ? c.queries + lifted * a.dim
+                                               : static_cast<const uint16_t*>(a.query) +
+                                                     (s.out_row + token) * a.query_row +
+                                                     static_cast<int64_t>(q_head) * a.query_head;
           const bool live = r < s.view.rows;
           const unsigned lives = __ballot_sync(0xffffffffu, live);
-          const unsigned long long row_at = reinterpret_cast<unsigned long long>(live ? own : a.query);
-          if (!kNarrow) unit_of[r0 + lane] = c.scale_log2;
+          const unsigned long long row_at =
+              reinterpret_cast<unsigned long long>(live ? static_cast<const void*>(own) : a.query);
+          if (Cache::kLifted)
+            unit_of[r0 + lane] = live ? c.scale_log2 * __ldg(c.units + lifted) : 1.f;
+          else if (!kE4m3)
+            unit_of[r0 + lane] = c.scale_log2;
           if (as_is) {
             const char* src[32 / kPerInstr];
 #pragma unroll
@@ -870,7 +940,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             continue;
           }
 #pragma unroll 1
-          for (int r1 = 0; r1 < 32; r1 += kBatch * kPerInstr) {
+          for (int r1 = 0; r1 < (Cache::kLifted ? 0 : 32); r1 += kBatch * kPerInstr) {
             uint4 x[kBatch];
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
@@ -883,7 +953,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int at = r0 + r1 + i * kPerInstr + sub;
               uint32_t word[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
               float unit = c.scale_log2;
-              if constexpr (kNarrow) {
+              if constexpr (kE4m3) {
                 const bool bf16 = a.query_type == KVCA_TYPE_BF16;
                 float2 f[4];
                 float big = 0.f;
@@ -900,7 +970,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int j = 0; j < 4; ++j) word[j] = pack2<false>(f[j].x * up, f[j].y * up);
                 unit *= power_of_two(-e);
               }
-              if (kNarrow && chunk == 0) unit_of[at] = unit;
+              if (kE4m3 && chunk == 0) unit_of[at] = unit;
 #pragma unroll
               for (int j = 0; j < 4; ++j) word[j] = (word[j] & c.query_and) ^ c.query_xor;
               if (chunk < row_chunks)
@@ -919,13 +989,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---------------------------------------------------------------- loads
     if (working) {
       const int w = warp - 8;
+      [[maybe_unused]] const uint32_t four_smem =
+          kv_smem + kStages * kTileBytes + w * ((kAhead + 1) * Shape::kFourSide);
       constexpr int kRowChunks = DP / 8;             // of a row in shared memory
       constexpr int kPerInstr = 32 / kRowChunks;     // rows per instruction (16-bit rows)
       const int chunk = lane % kRowChunks, sub = lane / kRowChunks;
       bool ok = true;
       uint32_t issued = 0, arrived = 0;
       uint32_t segment = 0;
-      constexpr uint32_t kAhead = 2;  // tiles in flight behind the one being issued
       // Of each tile in flight four bits: values of a cut tile, and the
       // segment's slot (nobody reuses it before its softmax, thus these, is done).
       uint32_t marks = 0;
@@ -943,13 +1014,68 @@ __global__ void __launch_bounds__(kThreads, 1)
         barrier_arrive(full + 8 * (arrived % kStages));
         ++arrived;
       };
+      // The same with 4-bit rows: widens them into the next tile.  A lane has 32 values
+      // with their two scales of one row at a time; the lanes of a quarter warp, two
+      // pieces of four rows, read and write distinct banks.
+      [[maybe_unused]] auto complete_four = [&]() {
+        constexpr int kPieces = DP / 32;
+        const uint32_t src = four_smem + (arrived % (kAhead + 1)) * Shape::kFourSide;
+        const uint32_t mark = marks >> (4 * (arrived & 7u));
+        __syncwarp();
+        if (arrived >= kStages)
+          ok = warp_wait(empty + 8 * (arrived % kStages), ((arrived / kStages) - 1) & 1, patience) && ok;
+        if (!ok) return;
+        unsigned char* const dst = smem_ptr + 2 * kQueries * kTileBytes + (arrived % kStages) * kTileBytes;
+        uint32_t found = 0;
+        auto part_of = [lane](int i) { return kPieces > 2 ? (lane & 1) + 2 * (i & 1) : lane & 1; };
+        auto row_of = [lane](int i) { return (lane >> 1) + 16 * (kPieces > 2 ? i >> 1 : i); };
+        uint4 raw[kPieces];
+        uint16_t bytes[kPieces];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {  // all of them before the first store
+          const int part = part_of(i), r = row_of(i);
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(raw[i].x), "=r"(raw[i].y), "=r"(raw[i].z), "=r"(raw[i].w)
+                       : "r"(src + r * (DP / 2) + ((part ^ (kPieces > 2 ? r & 2 : 0)) * 16)) : "memory");
+          asm volatile("ld.shared.u16 %0, [%1];"
+                       : "=h"(bytes[i]) : "r"(src + 32 * (DP / 2) + r * 8 + ((mark >> 2) & 2u) + 2 * part) : "memory");
+        }
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const int part = part_of(i), r = row_of(i);
+          if (part * 32 >= a.dim) continue;
+          const uint4 x = raw[i];
+          uint32_t scales = bytes[i];
+          if (mark & 1u) scales = drop_nan4(scales, &found);
+          const uint32_t both = e4m3_to_f16x2(scales);
+          const uint32_t factor[2] = {__byte_perm(both, 0, 0x1010), __byte_perm(both, 0, 0x3232)};
+          const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t wide[4];
+            e2m1x8_to_f16x2(wide, in[j]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) wide[e] = mul_f16x2(wide[e], factor[j / 2]);
+            *reinterpret_cast<uint4*>(dst + place(w * 32 + r, 4 * part + j)) =
+                make_uint4(wide[0], wide[1], wide[2], wide[3]);
+          }
+        }
+        if (found != 0) *const_cast<volatile int*>(&dropped[(mark >> 1) & 3u]) = 1;
+        __syncwarp();  // the place may be filled again
+        fence_async_proxy();
+        barrier_arrive(full + 8 * (arrived % kStages));
+        ++arrived;
+      };
       auto drain = [&]() {
-        while (arrived < issued) {
+        while (arrived < issued && (!kFour || ok)) {
           if (issued - arrived == kAhead)
             cp_async_wait<kAhead - 1>();
           else
             cp_async_wait<0>();
-          complete();
+          if constexpr (kFour)
+            complete_four();
+          else
+            complete();
         }
       };
       // The ring entry of the next tile.  Before it waits for one, a warp
@@ -963,7 +1089,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       constexpr int64_t kHidden = -1ll << 62;
       for (; ok; ++segment) {
-        if constexpr (!kNarrow) {
+        if constexpr (!kNarrow || kFour) {
           // nothing in flight is held back while the next segment is awaited
           if (arrived < issued &&
               !__all_sync(0xffffffffu, barrier_test(announced + 8 * (segment % kSlots), (segment / kSlots) & 1)))
@@ -1023,47 +1149,35 @@ __global__ void __launch_bounds__(kThreads, 1)
                 complete();
               }
             } else if constexpr (kFour) {
-              // 32 e2m1 values per load, with two scales, become four chunks
-              constexpr int kLoads = kRowChunks / 4;       // per row
-              constexpr int kRowsPer = 32 / kLoads;
-              const int part = lane % kLoads, which = lane / kLoads;
-              const int scales = scales_after(a, s.head) + 2 * part;
-              uint4 x[32 / kRowsPer];
-              uint32_t unit[32 / kRowsPer];
+              // to the warp's own place, in 16-byte pieces of 32 values (pieces of rows
+              // 2 and 3 of 4 with halves exchanged: see complete_four); a lane copies its
+              // row's scales, at most two 4-byte words
+              constexpr int kPieces = DP / 32, kRowsPer = 32 / kPieces;
+              const int part = lane % kPieces, which = lane / kPieces;
+              const uint32_t dst = four_smem + (issued % (kAhead + 1)) * Shape::kFourSide;
 #pragma unroll
-              for (int i = 0; i < 32 / kRowsPer; ++i) {
+              for (int i = 0; i < kPieces; ++i) {
                 const int r = i * kRowsPer + which;
-                const char* const from = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, r));
-                const bool read = ((seen >> r) & 1u) && part * 32 < a.dim;
-                x[i] = read ? __ldg(reinterpret_cast<const uint4*>(from) + part) : make_uint4(0, 0, 0, 0);
-                unit[i] = read ? __ldg(reinterpret_cast<const uint16_t*>(from + scales)) : 0;
+                const char* const from = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, row, r)) + part * 16;
+                if (part * 32 < a.dim)
+                  cp_async16(dst + r * (DP / 2) + ((part ^ (kPieces > 2 ? r & 2 : 0)) * 16), from, (seen >> r) & 1u);
               }
-              if (side == 1 && cut) {
-                uint32_t found = 0;
-#pragma unroll
-                for (int i = 0; i < 32 / kRowsPer; ++i) unit[i] = drop_nan4(unit[i], &found);
-                if (found != 0) *const_cast<volatile int*>(&dropped[segment % kSlots]) = 1;
-                __syncwarp();
-              }
-              claim();
-              if (!ok) break;
-              unsigned char* const dst = smem_ptr + 2 * kQueries * kTileBytes + (issued % kStages) * kTileBytes;
-#pragma unroll
-              for (int i = 0; i < 32 / kRowsPer; ++i) {
-                const int r = w * 32 + i * kRowsPer + which;
-                const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-                const uint32_t both = e4m3_to_f16x2(unit[i]);
-                const uint32_t factor[2] = {__byte_perm(both, 0, 0x1010), __byte_perm(both, 0, 0x3232)};
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  *reinterpret_cast<uint4*>(dst + place(r, 4 * part + j)) =
-                      make_uint4(mul_f16x2(e2m1_to_f16x2(in[j]), factor[j / 2]),
-                                 mul_f16x2(e2m1_to_f16x2(in[j] >> 8), factor[j / 2]),
-                                 mul_f16x2(e2m1_to_f16x2(in[j] >> 16), factor[j / 2]),
-                                 mul_f16x2(e2m1_to_f16x2(in[j] >> 24), factor[j / 2]));
-              }
+              const int scales = scales_after(a, s.head);
+              const int off = scales & 2;  // rows and their values are multiples of 16
+              const char* const from = reinterpret_cast<const char*>(row) + (scales - off);
+              const uint32_t to = dst + 32 * (DP / 2) + lane * 8;
+              const bool read = (seen >> lane) & 1u;
+              cp_async4(to, from, read);
+              if (off + a.dim / 16 > 4) cp_async4(to + 4, from + 4, read);
+              cp_async_commit();
+              const uint32_t mark = (side == 1 && cut ? 1u : 0u) | (segment % kSlots) << 1 | static_cast<uint32_t>(off) << 2;
+              marks = (marks & ~(15u << (4 * (issued & 7u)))) | mark << (4 * (issued & 7u));
               ++issued;
-              complete();
+              if (issued - arrived > kAhead) {
+                cp_async_wait<kAhead>();
+                complete_four();
+                if (!ok) break;
+              }
             } else {
               // 16 e4m3 values per load become two chunks
               constexpr int kLoads = kRowChunks / 2;       // per row
@@ -1109,7 +1223,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         release_segment(segment);
       }
-      if constexpr (!kNarrow) drain();
+      if constexpr (!kNarrow || kFour) drain();
       cp_async_wait<0>();
     }
   } else {
@@ -1400,19 +1514,23 @@ __global__ void __launch_bounds__(kJoinThreads) attend_chunk_join_kernel(const _
 template <typename Cache, int DP>
 cudaError_t launch_typed(const AttendArgs& a, const ChunkArgs& c, void* workspace, int sms, cudaStream_t stream) {
   auto kernel = attend_chunk_kernel<Cache, DP>;
+  constexpr int kSmem = ChunkShape<DP>::kSmem + (Cache::kBytes == 0 ? ChunkShape<DP>::kFourBytes : 0);
   static DeviceFlags configured;
   int dev = -1;
   if (needs_setup(configured, &dev)) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkShape<DP>::kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
     mark_setup(configured, dev);
   }
   const int64_t ctas = sms;
-  attend_chunk_plan_kernel<<<1, kPlanThreads, 0, stream>>>(a, c, workspace, DP, ctas);
+  // a block to plan, and with queries to lift as many as their rows keep busy
+  int64_t lifting = 0;
+  if (Cache::kLifted) lifting = (c.rows * a.kv_heads * a.group + 4 * kPlanThreads / 32 - 1) / (4 * kPlanThreads / 32);
+  attend_chunk_plan_kernel<<<1 + static_cast<int>(lifting < 2 * sms ? lifting : 2 * sms), kPlanThreads, 0, stream>>>(
+      a, c, workspace, DP, ctas);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  e = launch_dependent(kernel, dim3(sms), kThreads, ChunkShape<DP>::kSmem, stream, a, c, workspace);
+  e = launch_dependent(kernel, dim3(sms), kThreads, kSmem, stream, a, c, workspace);
   if (e != cudaSuccess) return e;
   return launch_dependent(attend_chunk_join_kernel<DP>, dim3(sms, kRows / kJoinRows), kJoinThreads, 0, stream, a, c,
                           workspace, ctas);
@@ -1430,8 +1548,18 @@ int64_t attend_chunk_max_blocks(const AttendArgs& a, int64_t rows) {
   return rows * a.group / kRows + a.num_seqs;  // each sequence's last block may be short
 }
 
+// Bytes of the workspace before the lifted queries.
+static size_t chunk_workspace_plan(const AttendArgs& a, int64_t rows, int sms) {
+  return (ChunkWorkspace::bytes(a.dim <= 64 ? 64 : 128, sms, attend_chunk_max_blocks(a, rows)) + 15) / 16 * 16;
+}
+
+static bool lifts_queries(const AttendArgs& a) {
+  return a.cache_type == KVCA_TYPE_E2M1 && a.query_type == KVCA_TYPE_BF16;
+}
+
 size_t attend_chunk_workspace(const AttendArgs& a, int64_t rows, int sms) {
-  return ChunkWorkspace::bytes(a.dim <= 64 ? 64 : 128, sms, attend_chunk_max_blocks(a, rows));
+  const size_t query_rows = lifts_queries(a) ? static_cast<size_t>(rows) * a.kv_heads * a.group : 0;
+  return chunk_workspace_plan(a, rows, sms) + query_rows * (a.dim * sizeof(uint16_t) + sizeof(float));
 }
 
 cudaError_t launch_attend_chunk(const AttendArgs& args, const int64_t* offsets, int64_t rows, int64_t wait_limit,
@@ -1446,11 +1574,19 @@ cudaError_t launch_attend_chunk(const AttendArgs& args, const int64_t* offsets, 
   c.scale_log2 = a.scale_log2 == 0.f ? 1.f : fabsf(a.scale_log2);
   c.query_and = a.scale_log2 == 0.f ? 0u : 0xffffffffu;
   c.query_xor = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+  c.queries = nullptr;
+  c.units = nullptr;
+  if (lifts_queries(a)) {
+    c.queries = reinterpret_cast<uint16_t*>(static_cast<char*>(workspace) + chunk_workspace_plan(a, rows, sms));
+    c.units = reinterpret_cast<float*>(c.queries + rows * a.kv_heads * a.group * a.dim);
+  }
   c.shift = a.cache_type == KVCA_TYPE_BF16 ? kShift<CacheBf16> : kShift<CacheF16>;
   switch (a.cache_type) {
     case KVCA_TYPE_F16: return launch_cache<CacheF16>(a, c, workspace, sms, stream);
     case KVCA_TYPE_BF16: return launch_cache<CacheBf16>(a, c, workspace, sms, stream);
-    case KVCA_TYPE_E2M1: return launch_cache<CacheE2m1<false>>(a, c, workspace, sms, stream);
+    case KVCA_TYPE_E2M1:
+      return a.query_type == KVCA_TYPE_BF16 ? launch_cache<CacheE2m1<true>>(a, c, workspace, sms, stream)
+                                            : launch_cache<CacheE2m1<false>>(a, c, workspace, sms, stream);
     default: return launch_cache<CacheE4m3>(a, c, workspace, sms, stream);
   }
 }

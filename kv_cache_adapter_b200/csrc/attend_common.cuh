@@ -22,29 +22,29 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Storage types of the cache, and what its matrix products run in: e4m3
-// widens to fp16, which holds every e4m3 value, and e2m1 times its scale, which
-// fp16 holds too (2 bits times 4, from 2^-10 to 2,688).
+// widens to fp16, which holds every e4m3 value, and so does e2m1 times its scale,
+// which fp16 holds too (2 bits times 4, from 2^-10 to 2,688).
 struct CacheF16 {
   static constexpr int kBytes = 2;
   static constexpr bool kBf16 = false;
-  static constexpr bool kOdd = false;
+  static constexpr bool kLifted = false;
 };
 struct CacheBf16 {
   static constexpr int kBytes = 2;
   static constexpr bool kBf16 = true;
-  static constexpr bool kOdd = false;
+  static constexpr bool kLifted = false;
 };
 struct CacheE4m3 {
   static constexpr int kBytes = 1;
   static constexpr bool kBf16 = false;
-  static constexpr bool kOdd = false;
+  static constexpr bool kLifted = false;
 };
-// Odd: a head's scales do not fill 4, 8 or 16 bytes of their own.
-template <bool Odd>
+// Lifted: queries that were bf16 lie in the workspace of a chunk call as fp16.
+template <bool Lifted>
 struct CacheE2m1 {
   static constexpr int kBytes = 0;  // half of one
   static constexpr bool kBf16 = false;
-  static constexpr bool kOdd = Odd;
+  static constexpr bool kLifted = Lifted;
 };
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -89,6 +89,11 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool r
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// The same for 4 bytes.
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool read) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(read ? 4 : 0) : "memory");
 }
 
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }

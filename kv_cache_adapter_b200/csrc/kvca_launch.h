@@ -159,6 +159,8 @@ struct ChunkArgs {
   uint32_t query_and, query_xor;
   float shift;  // log2 of the factor in partial sums
   int64_t wait_limit;  // ns that a wait of the kernel may take
+  uint16_t* queries;   // (4 bits, bf16 queries) (rows, heads, dim) as fp16 times a
+  float* units;        // power of two per row, and its inverse, in the workspace
 };
 
 size_t attend_step_workspace(const AttendArgs& args, int sms);
