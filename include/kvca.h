@@ -813,7 +813,7 @@ int kvca_attend_chunk(const kvca_attend_desc* desc, const int64_t* d_query_offse
 
 /*
  * Sets how long a wait within the kernels of later kvca_attend_chunk calls of
- * this process may take, in nanoseconds (2 s at first; 0: a wait whose event
+ * this process, and of kvca_attend_step calls over 4-bit caches, may take, in nanoseconds (2 s at first; 0: a wait whose event
  * has not come yet gives up), and returns the limit before; only returns it
  * when negative.  A graph keeps the limit of its capture.
  */

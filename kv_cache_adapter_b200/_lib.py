@@ -384,13 +384,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [ctypes.POINTER(PagePool), ctypes.POINTER(PagedDesc), c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_ptr],
     ),
-    "kvca_attend_step_workspace_bytes": (c_i64, [ctypes.POINTER(AttendDesc)]),
+    "kvca_attend_step_workspace_bytes": (c_i64, [c_ptr]),
     "kvca_stream_id": (ctypes.c_uint64, [c_ptr]),
     "kvca_attend_step_counters": (c_i64, []),
-    "kvca_attend_step": (c_int, [ctypes.POINTER(AttendDesc), c_ptr, c_i64, c_ptr, c_ptr, c_ptr]),
-    "kvca_attend_chunk_workspace_bytes": (c_i64, [ctypes.POINTER(AttendDesc), c_i64]),
+    "kvca_attend_step": (c_int, [c_ptr, c_ptr, c_i64, c_ptr, c_ptr, c_ptr]),
+    "kvca_attend_chunk_workspace_bytes": (c_i64, [c_ptr, c_i64]),
     "kvca_attend_wait_limit": (c_i64, [c_i64]),
-    "kvca_attend_chunk": (c_int, [ctypes.POINTER(AttendDesc), c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr]),
+    "kvca_attend_chunk": (c_int, [c_ptr, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr]),
     "kvca_rotate_tokens": (c_int, [c_ptr, c_ptr, c_ptr]),
     "kvca_e2m1_row_bytes": (c_i64, [c_i64, c_i64]),
     "kvca_append_tokens": (c_int, [c_ptr, c_ptr, c_ptr]),

@@ -939,43 +939,45 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             continue;
           }
+          if constexpr (!Cache::kLifted) {
 #pragma unroll 1
-          for (int r1 = 0; r1 < (Cache::kLifted ? 0 : 32); r1 += kBatch * kPerInstr) {
-            uint4 x[kBatch];
+            for (int r1 = 0; r1 < 32; r1 += kBatch * kPerInstr) {
+              uint4 x[kBatch];
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-              const int from = r1 + i * kPerInstr + sub;
-              const uint4* src = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, row_at, from)) + chunk;
-              x[i] = ((lives >> from) & 1u) && chunk < row_chunks ? __ldg(src) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-              const int at = r0 + r1 + i * kPerInstr + sub;
-              uint32_t word[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-              float unit = c.scale_log2;
-              if constexpr (kE4m3) {
-                const bool bf16 = a.query_type == KVCA_TYPE_BF16;
-                float2 f[4];
-                float big = 0.f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  f[j] = bf16 ? unpack2<true>(word[j]) : unpack2<false>(word[j]);
-                  big = fmaxf(big, fmaxf(fabsf(f[j].x), fabsf(f[j].y)));
-                }
-#pragma unroll
-                for (int o = kRowChunks / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-                const int e = power_up(big);
-                const float up = power_of_two(e);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) word[j] = pack2<false>(f[j].x * up, f[j].y * up);
-                unit *= power_of_two(-e);
+              for (int i = 0; i < kBatch; ++i) {
+                const int from = r1 + i * kPerInstr + sub;
+                const uint4* src = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, row_at, from)) + chunk;
+                x[i] = ((lives >> from) & 1u) && chunk < row_chunks ? __ldg(src) : make_uint4(0, 0, 0, 0);
               }
-              if (kE4m3 && chunk == 0) unit_of[at] = unit;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) word[j] = (word[j] & c.query_and) ^ c.query_xor;
-              if (chunk < row_chunks)
-                *reinterpret_cast<uint4*>(smem_ptr + tile + place(at, chunk)) =
-                    make_uint4(word[0], word[1], word[2], word[3]);
+              for (int i = 0; i < kBatch; ++i) {
+                const int at = r0 + r1 + i * kPerInstr + sub;
+                uint32_t word[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                float unit = c.scale_log2;
+                if constexpr (kE4m3) {
+                  const bool bf16 = a.query_type == KVCA_TYPE_BF16;
+                  float2 f[4];
+                  float big = 0.f;
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    f[j] = bf16 ? unpack2<true>(word[j]) : unpack2<false>(word[j]);
+                    big = fmaxf(big, fmaxf(fabsf(f[j].x), fabsf(f[j].y)));
+                  }
+#pragma unroll
+                  for (int o = kRowChunks / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+                  const int e = power_up(big);
+                  const float up = power_of_two(e);
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) word[j] = pack2<false>(f[j].x * up, f[j].y * up);
+                  unit *= power_of_two(-e);
+                }
+                if (kE4m3 && chunk == 0) unit_of[at] = unit;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) word[j] = (word[j] & c.query_and) ^ c.query_xor;
+                if (chunk < row_chunks)
+                  *reinterpret_cast<uint4*>(smem_ptr + tile + place(at, chunk)) =
+                      make_uint4(word[0], word[1], word[2], word[3]);
+              }
             }
           }
         }

@@ -387,6 +387,15 @@ __global__ void __launch_bounds__(FourShape<DP, NG>::kThreads, 1)
     const uint32_t ring_base = smem_addr(rings) + warp / span * RunRing::ring_bytes(layout);
     const uint32_t ring_bars = smem_addr(bars) + warp / span * (16 * kMaxStages);
     bool ok = true;  // no wait has given up
+    // With a limit of 0, whether the phase is over now.
+    auto await = [&](uint32_t bar, uint32_t parity) {
+      if (a.wait_limit > 0) {
+        ok = warp_wait(bar, parity, patience) && ok;
+      } else if (!__all_sync(0xffffffffu, barrier_test(bar, parity))) {
+        *patience.gave_up = 1;
+        ok = false;
+      }
+    };
 
     Position at;  // the tile computed next
     {
@@ -460,7 +469,7 @@ __global__ void __launch_bounds__(FourShape<DP, NG>::kThreads, 1)
       const bool good = page >= 0 && page < a.num_blocks;
       if (!good && page != kHidden) report(a.status, KVCA_ERR_BAD_INDEX, page);
       const uint32_t full = ring_bars + 16 * f.stage;
-      if (f.round > 0) ok = warp_wait(full + 8, static_cast<uint32_t>(f.round - 1) & 1u, patience) && ok;
+      if (f.round > 0) await(full + 8, static_cast<uint32_t>(f.round - 1) & 1u);
       if (ok) {
         const unsigned seen = __ballot_sync(0xffffffffu, good);
         // K/V heads of which the run has parts, and the pieces of their scales
@@ -583,7 +592,7 @@ __global__ void __launch_bounds__(FourShape<DP, NG>::kThreads, 1)
         fresh = false;
       }
 
-      ok = warp_wait(ring_bars + 16 * stage, phase, patience) && ok;
+      await(ring_bars + 16 * stage, phase);
       const uint32_t rows = ring_base + stage * ring.stage_bytes;
       const int count = at.vis.count - at.tile * kTile;
 

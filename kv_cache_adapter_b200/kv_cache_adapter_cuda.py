@@ -1493,19 +1493,24 @@ def _attend_rows(t: torch.Tensor, shape, name: str) -> list[int]:
     return out
 
 
+_pack_attend = _lib.packer(_lib.AttendDesc)
+
+
 def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
                  block_tables: torch.Tensor, seq_lens: torch.Tensor, scale, window, sinks, key_scale, value_scale,
-                 out, lse) -> tuple[_lib.AttendDesc, torch.Tensor]:
-    """The checked arguments of an attention call and its output tensor."""
+                 out, lse) -> tuple[bytes, torch.Tensor, tuple[int, int, int]]:
+    """The checked arguments of an attention call, its output tensor, and what its
+    workspace goes by (query heads of a K/V head, head_dim, cache type)."""
     tensor = torch.Tensor
     if not (isinstance(query, tensor) and isinstance(key_cache, tensor) and isinstance(value_cache, tensor)
             and isinstance(block_tables, tensor) and isinstance(seq_lens, tensor)):
         raise TypeError("query, key_cache, value_cache, block_tables and seq_lens must be torch.Tensor")
     dev = query.device
-    if dev.type != "cuda":
+    index = query.get_device()
+    if index < 0:
         raise ValueError("query must be a CUDA tensor")
-    if (key_cache.device != dev or value_cache.device != dev or block_tables.device != dev
-            or seq_lens.device != dev):
+    if (key_cache.get_device() != index or value_cache.get_device() != index or block_tables.get_device() != index
+            or seq_lens.get_device() != index):
         raise ValueError(f"key_cache, value_cache, block_tables and seq_lens must be on {dev}")
     qtype, ctype = query.dtype, key_cache.dtype
     if qtype is not torch.float16 and qtype is not torch.bfloat16:
@@ -1567,28 +1572,28 @@ def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torc
         raise TypeError("out must be torch.Tensor")
     else:
         out_ptr = out.data_ptr()
-        if (out.shape != qshape or out.dtype is not qtype or out.device != dev or not out.is_contiguous()
+        if (out.shape != qshape or out.dtype is not qtype or out.get_device() != index or not out.is_contiguous()
                 or out_ptr % 16):
             raise ValueError(f"out must be a contiguous, 16-byte aligned {tuple(qshape)} {qtype} tensor on {dev}")
         if out_ptr < q_end and q_ptr < out_ptr + size and not (out_ptr == q_ptr and query.is_contiguous()):
             raise ValueError("out must not overlap query (unless it is the query)")
     if lse is None:
-        lse_ptr = None
+        lse_ptr = 0
     elif not isinstance(lse, tensor):
         raise TypeError("lse must be torch.Tensor")
-    elif lse.shape != qshape[:2] or lse.dtype is not torch.float32 or lse.device != dev or not lse.is_contiguous():
+    elif lse.shape != qshape[:2] or lse.dtype is not torch.float32 or lse.get_device() != index or not lse.is_contiguous():
         raise ValueError(f"lse must be a contiguous {tuple(qshape[:2])} float32 tensor on {dev}")
     else:
         lse_ptr = lse.data_ptr()
         lse_end = lse_ptr + 4 * rows * heads
         if lse_ptr < q_end and q_ptr < lse_end or lse_ptr < out_ptr + size and out_ptr < lse_end:
             raise ValueError("lse must not overlap query or out")
-    desc = _lib.AttendDesc(
-        key_cache.data_ptr(), value_cache.data_ptr(), *ks, *vs, num_blocks, block_size,
-        block_tables.data_ptr() or None, tstride[0], tshape[1], seq_lens.data_ptr() or None, seqs, heads, kv_heads, dim,
-        _ATTEND_TYPES[qtype], _ATTEND_TYPES[ctype], dim ** -0.5 if scale is None else scale, key_scale, value_scale,
-        window, sinks, q_ptr, *qs, out_ptr, lse_ptr)
-    return desc, out
+    kind = _ATTEND_TYPES[ctype]
+    desc = _pack_attend(
+        key_cache.data_ptr(), value_cache.data_ptr(), *ks, *vs, num_blocks, block_size, block_tables.data_ptr(),
+        tstride[0], tshape[1], seq_lens.data_ptr(), seqs, heads, kv_heads, dim, _ATTEND_TYPES[qtype], kind,
+        dim ** -0.5 if scale is None else scale, key_scale, value_scale, window, sinks, q_ptr, *qs, out_ptr, lse_ptr)
+    return desc, out, (heads // kv_heads, dim, kind)
 
 
 def attend_step(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -1610,8 +1615,8 @@ def attend_step(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
     softmax's sum.  A sequence of length 0 gives zeros (``lse`` -inf); rows of
     negative length are left as they were.  No gradients: the cache holds no
     graph."""
-    desc, out = _attend_desc(query, key_cache, value_cache, block_tables, seq_lens, scale, window, sinks, key_scale,
-                             value_scale, out, lse)
+    desc, out, sizes = _attend_desc(query, key_cache, value_cache, block_tables, seq_lens, scale, window, sinks,
+                                    key_scale, value_scale, out, lse)
     if query.shape[0] != seq_lens.shape[0]:
         raise ValueError("query needs one row per sequence")
     if query.shape[0] == 0:
@@ -1619,15 +1624,15 @@ def attend_step(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
     dev = query.device
     with _on(dev):
         stream = _scratch_stream(dev)
-        shape = ("step", _index(dev), desc.q_heads // desc.kv_heads, desc.head_dim, desc.cache_type)
+        shape = ("step", _index(dev), *sizes)
         need = _attend_workspace_bytes.get(shape)
         if need is None:
-            need = _lib_handle.kvca_attend_step_workspace_bytes(ctypes.byref(desc))
+            need = _lib_handle.kvca_attend_step_workspace_bytes(desc)
             if need < 0:
                 _raise_for(_lib.KVCA_ERR_BAD_ARGUMENT, 0, "attend_step")
             _attend_workspace_bytes[shape] = need
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        rc = _lib_handle.kvca_attend_step(ctypes.byref(desc), workspace.data_ptr(), need,
+        rc = _lib_handle.kvca_attend_step(desc, workspace.data_ptr(), need,
                                           _step_counters(dev, stream).data_ptr(), _status(dev).data_ptr(), stream)
     _host_rc(rc, "attend_step")
     _maybe_check(dev, check, "attend_step")
@@ -1649,8 +1654,8 @@ def attend_chunk(query: torch.Tensor, query_offsets: torch.Tensor, key_cache: to
     sequence.  The other arguments and ``lse`` are ``attend_step``'s.  Rows
     outside the offsets, and those of a sequence of negative length, are left
     as they were."""
-    desc, out = _attend_desc(query, key_cache, value_cache, block_tables, seq_lens, scale, window, sinks, key_scale,
-                             value_scale, out, lse)
+    desc, out, _ = _attend_desc(query, key_cache, value_cache, block_tables, seq_lens, scale, window, sinks, key_scale,
+                                value_scale, out, lse)
     if query.shape[2] > 128:
         raise ValueError(f"head_dim must be at most 128, got {query.shape[2]}")
     dev = query.device
@@ -1662,11 +1667,11 @@ def attend_chunk(query: torch.Tensor, query_offsets: torch.Tensor, key_cache: to
         return out
     with _on(dev):
         stream = _scratch_stream(dev)
-        need = _lib_handle.kvca_attend_chunk_workspace_bytes(ctypes.byref(desc), rows)
+        need = _lib_handle.kvca_attend_chunk_workspace_bytes(desc, rows)
         if need < 0:
             _raise_for(_lib.KVCA_ERR_BAD_ARGUMENT, 0, "attend_chunk")
         workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        rc = _lib_handle.kvca_attend_chunk(ctypes.byref(desc), query_offsets.data_ptr(), rows, workspace.data_ptr(),
+        rc = _lib_handle.kvca_attend_chunk(desc, query_offsets.data_ptr(), rows, workspace.data_ptr(),
                                            need, _ptr(_status(dev)), stream)
     _host_rc(rc, "attend_chunk")
     _maybe_check(dev, check, "attend_chunk")

@@ -430,6 +430,25 @@ def test_read_e2m1(ops, dev, heads, dim):
     oracle.check_rows(out.cpu()[live], want[live], want[live].abs() * 2.0 ** -22, F32)
 
 
+@pytest.mark.parametrize("heads,dim,kind", [(1, 16, E4M3), (2, 16, E4M3), (1, 32, "e2m1"), (13, 256, "e2m1"),
+                                            (13, 256, E4M3)])
+def test_read_of_many_rows(ops, dev, heads, dim, kind):
+    g = torch.Generator(device=dev).manual_seed(dim)
+    mapping = torch.randperm(40 * 160, generator=g, device=dev)[:6001]
+    if kind == E4M3:
+        plane = torch.randn((160, 40, heads, dim), generator=g, device=dev).to(E4M3)
+        want = plane.float().flatten(0, 1)[mapping]
+    else:
+        plane = torch.randint(0, 256, (160, 40, ops.e2m1_row_bytes(heads, dim)), generator=g, device=dev,
+                              dtype=torch.uint8)
+        plane[:, :, heads * dim // 2:] &= 0x3f  # scales from 0 to 1.9
+        want = oracle.values(plane.flatten(0, 1)[mapping].cpu(), heads, dim).float().to(dev)
+    for offset in (0, 8):  # places in steps of 32 bytes, and of 16
+        out = torch.empty(want.numel() + 8, dtype=F16, device=dev)[offset:offset + want.numel()].view(want.shape)
+        ops.read_tokens(plane, mapping, head_dim=dim, out=out, check=True)
+        assert torch.equal(out, want.half())
+
+
 @pytest.mark.parametrize("four", [False, True])
 def test_read_reports_a_bad_slot_and_goes_on(ops, dev, four):
     plane = torch.zeros((2, 4, 80), dtype=torch.uint8, device=dev) if four else \
