@@ -718,7 +718,11 @@ int kvca_compact_pages(const kvca_page_pool* pool, const kvca_paged_desc* cache,
  * are multiples of 16 bytes, head_dim a multiple of 8 (of 16 with e4m3), at
  * most 256.  q_heads is a multiple of kv_heads: query head h reads K/V head
  * h / (q_heads / kv_heads).  An e4m3 value stands for itself times key_scale
- * (value_scale); both are 1 otherwise.
+ * (value_scale).  With KVCA_TYPE_E2M1 a token's row is the one that
+ * kvca_append_tokens describes, at block and token strides of its own (the head
+ * strides are not looked at), and head_dim a multiple of 32; a value is its code
+ * times its scale times key_scale (value_scale); a NaN scale makes its 16 values
+ * NaN.  Both factors are 1 with caches of 16 bits.
  *
  * A query at position p of its sequence sees the tokens
  *   j <= p  with  window == 0, or j > p - window, or j < sinks,
@@ -753,7 +757,7 @@ typedef struct kvca_attend_desc {
   int32_t kv_heads;
   int32_t head_dim;
   int32_t query_type;
-  int32_t cache_type; /* the query's, or KVCA_TYPE_E4M3 */
+  int32_t cache_type; /* the query's, KVCA_TYPE_E4M3 or KVCA_TYPE_E2M1 */
   float scale;
   float key_scale;
   float value_scale;
@@ -773,7 +777,10 @@ typedef struct kvca_attend_desc {
  * -inf).  One launch, no host synchronisation; the work is split evenly over
  * the SMs whatever the lengths.  workspace:
  * kvca_attend_step_workspace_bytes(desc) bytes (lengths and values do not
- * matter) of device memory, 16-byte aligned, any contents.  d_counters:
+ * matter) of device memory, 16-byte aligned, any contents.  Over a 4-bit cache a
+ * wait within the kernel that takes longer than the limit (kvca_attend_wait_limit)
+ * gives KVCA_ERR_DEVICE_TIMEOUT; the outputs then hold no defined values, the
+ * counters are as they should be.  d_counters:
  * kvca_attend_step_counters() words, zero on entry and zero again on exit
  * (unless seq_lens changed while the call ran: zero them then).  Calls that
  * may overlap on the GPU (other streams, graphs replayed side by side) need

@@ -7,8 +7,10 @@ adapter.py:316-330, :397-415, :437-454, :477-491, :557-593, :615-645).  The
 row movers replace the torch indexing the reference uses to move KV bytes
 (adapter.py:543, :653-656, :779-787) and its slot_mapping transfer
 (adapter.py:1200-1243, :1275-1285).  Beyond the reference: attention over the
-paged cache (``attend_step``, ``attend_chunk``) and the pages of sequences
-(``fork_sequences``, ``free_sequences``, ``compact_pages``).
+paged cache (``attend_step``, ``attend_chunk``), the pages of sequences
+(``fork_sequences``, ``free_sequences``, ``compact_pages``) and the rows of new
+tokens (``append_tokens``, ``rotate_tokens``, ``read_tokens``: rotary positions,
+caches of 16, 8 and 4 bits).
 
 Every op launches on the current CUDA stream of its tensors' device.  Errors
 found on the device land in a per-device status word.  ``pop_reusable_slots``
@@ -1610,6 +1612,9 @@ def attend_step(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch
     ``seq_lens`` int64, the new token included.  The token at the end of a
     sequence sees all of it, or with ``window`` its last ``window`` tokens and
     the first ``sinks`` ones.  ``scale`` defaults to ``head_dim ** -0.5``.
+    Caches of 4 bits are uint8 ``(num_blocks, block_size, e2m1_row_bytes(kv_heads,
+    head_dim))``, as ``append_tokens`` writes them (head_dim a multiple of 32;
+    ``key_scale`` / ``value_scale`` too).
     Returns ``out`` ``(num_seqs, heads, head_dim)``, which may be the query
     itself; ``lse`` (float32 ``(num_seqs, heads)``) also gets the log of each
     softmax's sum.  A sequence of length 0 gives zeros (``lse`` -inf); rows of
@@ -1977,6 +1982,10 @@ def append_tokens(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tenso
         query_out, q_out = _result_rows(query_out, query, q, index, 2, "query_out")
         if q_out != q and (q_out[0] < k[3] and k[0] < q_out[3] or q_out[0] < v[3] and v[0] < q_out[3]):
             raise ValueError("query_out must not overlap key or value")
+        if (q_out[0] < angles + 4 * held * rotary and angles < q_out[3]
+                or q_out[0] < at_positions + 8 * rows and at_positions < q_out[3]
+                or q_out[0] < at_slots + 8 * rows and at_slots < q_out[3]):
+            raise ValueError("query_out must not overlap table, positions or slot_mapping")
     elif query_out is not None:
         raise ValueError("query_out needs a query")
     for c in (kc, vc):
@@ -1984,8 +1993,11 @@ def append_tokens(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tenso
         if (begin < k[3] and k[0] < end or begin < v[3] and v[0] < end or begin < q[3] and q[0] < end
                 or begin < q_out[3] and q_out[0] < end):
             raise ValueError("the caches must not overlap the rows")
-    if kc[0] == vc[0] and kc[4] > kc[0]:
-        raise ValueError("key_cache and value_cache must be two caches")
+    if kc[0] < vc[4] and vc[0] < kc[4]:  # planes of one merged cache lie side by side in its strides
+        if kc[1:4] != vc[1:4]:
+            raise ValueError("key_cache and value_cache must not overlap")
+        _distinct((*cshape[:-1], 2), (*kc[1:len(cshape)], abs(vc[0] - kc[0])), cshape[-1] * size,
+                  "key_cache and value_cache")
     if rows:
         dev = key.device
         desc = _pack_append(

@@ -540,3 +540,54 @@ def test_nothing_to_do(ops, dev):
     ops.append_tokens(one, one, empty, empty.clone(), torch.tensor([-1], device=dev), check=True)
     with pytest.raises(IndexError):
         ops.append_tokens(one, one, empty, empty.clone(), torch.tensor([0], device=dev), check=True)
+
+
+def test_refusals(ops, dev):
+    k, at = torch.zeros((4, 2, 64), dtype=F16, device=dev), torch.zeros(4, dtype=torch.int64, device=dev)
+    table = ops.rotary_table(8, 64).to(dev)
+    kc, vc = cache_of(F16, 4, 16, 2, 64, dev)
+    four = cache_of("e2m1", 4, 16, 2, 64, dev)
+    good = dict(positions=at, table=table, query=k, query_out=torch.empty_like(k))
+    ops.append_tokens(k, k, kc, vc, torch.arange(4, device=dev), check=True, **good)
+    merged = torch.zeros((4, 16, 2, 2, 64), dtype=F16, device=dev)
+    ops.append_tokens(k, k, merged[:, :, 1], merged[:, :, 0], at + 63, check=True)
+    for args, kw, match in (
+            ((k, k[:3], kc, vc, at), {}, "share shape"),
+            ((k, k, kc, four[1], at), {}, "share shape"),
+            ((k, k, kc.float(), vc.float(), at), {}, "incorrect dtype"),
+            ((k, k, kc[:, :, :1], vc[:, :, :1], at), {}, "must be"),
+            ((k, k, four[0][:, :, :64], four[1][:, :, :64], at), {}, "no heads"),
+            ((k[..., :48].contiguous(), k[..., :48].contiguous(), *four, at), {}, "out of range"),
+            ((k, k, kc, vc, at[:3]), {}, "one entry"),
+            ((k, k, kc, vc, at.int()), {}, "incorrect dtype"),
+            ((k, k, kc, vc, at), dict(positions=at), "go together"),
+            ((k, k, kc, vc, at), dict(query=k), "needs positions"),
+            ((k, k, kc, vc, at), dict(query_out=k), "needs a query"),
+            ((k, k, kc, vc, at), dict(key_scale=2.0), "belong to"),
+            ((k, k, *four, at), dict(key_scale=0.0), "positive"),
+            ((k, k, *four, at), dict(value_scale=math.nan), "positive"),
+            ((k, k, kc, kc, at), {}, "share memory"),
+            ((k, k, kc[:2], kc[1:3], at), {}, "share memory"),
+            ((k, k, kc.expand(2, 4, 16, 2, 64)[:, 0], vc[:2], at), {}, "share memory"),
+            ((kc[0][:4], k, kc, vc, at), {}, "overlap the rows"),
+            ((k, k, kc, vc, at), dict(good, table=table[:, :3]), "contiguous"),
+            ((k, k, kc, vc, at), dict(good, table=table.half()), "incorrect dtype"),
+            ((k, k, kc, vc, at), dict(good, table=ops.rotary_table(8, 66).to(dev)), "at most head_dim"),
+            ((k, k, kc, vc, at), dict(good, query_out=torch.empty((4, 2, 64), device=dev)), "incorrect dtype"),
+            ((k, k, kc, vc, at), dict(good, query=k.expand(4, 2, 64)[:, :1].expand(4, 3, 64), query_out=k[:, :1].expand(4, 3, 64)),
+             "share memory")):
+        with pytest.raises((ValueError, TypeError), match=match):
+            ops.append_tokens(*args, **kw)
+    x = torch.zeros((6, 2, 64), dtype=F16, device=dev)
+    for args, kw, match in (((x.double(), at, table), {}, "incorrect dtype"), ((x[0], at, table), {}, "must be"),
+                            ((x, at, table), {}, "one entry"), ((x[:4], at, table), dict(out=x[1:5]), "overlap"),
+                            ((x[:4, :, ::2], at, table), {}, "contiguous"), ((x[:4, :, :12], at, table), {}, "multiples"),
+                            ((x[:4], at, table.cpu()), {}, "on cuda")):
+        with pytest.raises((ValueError, TypeError), match=match):
+            ops.rotate_tokens(*args, **kw)
+    for args, kw, match in (((four[0], at), {}, "needs head_dim"), ((kc, at), {}, "incorrect dtype"),
+                            ((four[0], at), dict(head_dim=96), "no heads"),
+                            ((four[0], at), dict(head_dim=64, dtype=torch.int8), "incorrect dtype"),
+                            ((four[0], at), dict(head_dim=64, out=k[:3]), "must be a contiguous")):
+        with pytest.raises((ValueError, TypeError), match=match):
+            ops.read_tokens(*args, **kw)

@@ -88,6 +88,20 @@ def test_c_abi_nothing_to_do_and_size_limits(call, desc):
         assert fn(ctypes.byref(desc(num_blocks=1 << 60, block_size=1 << 20)), None, None) == _lib.KVCA_ERR_SIZE_LIMIT
 
 
+@pytest.mark.parametrize("bad", [dict(head_dim=48), dict(head_dim=80), dict(key=8), dict(value_token_stride=24),
+                                 dict(query_type=_lib.KVCA_TYPE_E2M1), dict(query_type=_lib.KVCA_TYPE_F32)],
+                         ids=lambda b: ",".join(b))
+def test_attention_over_four_bits_refuses(bad):
+    import test_attend_refusals
+
+    d = test_attend_refusals.desc(**{"cache_type": _lib.KVCA_TYPE_E2M1, "head_dim": 64, **bad})
+    lib = _lib.load()
+    assert lib.kvca_attend_step(ctypes.byref(d), 4096, 1 << 40, 4096, None, None) == BAD
+    assert lib.kvca_attend_step_workspace_bytes(ctypes.byref(d)) == -1
+    assert lib.kvca_attend_chunk(ctypes.byref(d), 4096, 4, 4096, 1 << 40, None, None) == BAD
+    assert lib.kvca_attend_chunk_workspace_bytes(ctypes.byref(d), 4) == -1
+
+
 def test_rows_of_four_bit_caches():
     assert ops.e2m1_row_bytes(8, 128) == 8 * (64 + 8)
     assert ops.e2m1_row_bytes(1, 128) == 80 and ops.e2m1_row_bytes(1, 32) == 32 and ops.e2m1_row_bytes(3, 256) == 432
