@@ -701,11 +701,11 @@ __global__ void __launch_bounds__(FourShape<DP, NG>::kThreads, 1)
         }
 
         // O^T += V^T P^T.  Lane 4 i + t: dims i DP / 8 and on of the tokens of rows 2 t,
-        // 2 t + 1, 2 t + 8 and 2 t + 9.  A converted byte is two dims of one token, the
-        // operand wants one dim of two tokens in a register: a byte permutation each.
-        // (Without it, a product each for the even and the odd dims, tokens' weights
-        // beside zeros: the multiplications by scales wait for the tensor cores, so 7 %
-        // more time for the two sides of a tile in registers and shared memory.)
+        // 2 t + 1, 2 t + 8 and 2 t + 9.  A byte is two dims of one token, the operand wants
+        // one dim of two tokens in a register: the codes of two tokens are paired before
+        // they are converted, 16 operations for 32 registers.  (With a product each for
+        // the even and the odd dims instead, tokens' weights beside zeros, the
+        // multiplications by scales wait for the tensor cores: 203 us for 187.)
         constexpr int kWords = DP / 64;  // of a lane's dims of a token
         constexpr int kGroups = DP > 128 ? 2 : 1;
         uint32_t w[4][kWords], scale[2][kGroups];
@@ -726,15 +726,17 @@ __global__ void __launch_bounds__(FourShape<DP, NG>::kThreads, 1)
         }
 #pragma unroll
         for (int r = 0; r < kWords; ++r) {
-          uint32_t x[4][4];
+          uint32_t x[4][4];  // even dims of the first two tokens, odd ones, and of the others
 #pragma unroll
-          for (int i = 0; i < 4; ++i) e2m1x8_to_f16x2(x[i], w[i][r]);
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t one = w[2 * i][r], other = w[2 * i + 1][r];
+            e2m1x8_to_f16x2(x[2 * i], (one & 0x0f0f0f0fu) | (other << 4 & 0xf0f0f0f0u));
+            e2m1x8_to_f16x2(x[2 * i + 1], (one >> 4 & 0x0f0f0f0fu) | (other & 0xf0f0f0f0u));
+          }
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
-            const uint32_t f[4] = {mul_f16x2(__byte_perm(x[0][b], x[1][b], 0x5410), scale[0][r / 2]),
-                                   mul_f16x2(__byte_perm(x[0][b], x[1][b], 0x7632), scale[0][r / 2]),
-                                   mul_f16x2(__byte_perm(x[2][b], x[3][b], 0x5410), scale[1][r / 2]),
-                                   mul_f16x2(__byte_perm(x[2][b], x[3][b], 0x7632), scale[1][r / 2])};
+            const uint32_t f[4] = {mul_f16x2(x[0][b], scale[0][r / 2]), mul_f16x2(x[1][b], scale[0][r / 2]),
+                                   mul_f16x2(x[2][b], scale[1][r / 2]), mul_f16x2(x[3][b], scale[1][r / 2])};
 #pragma unroll
             for (int n = 0; n < NG; ++n) mma16816<false>(acc[n][4 * r + b], f, p[n][0], p[n][1]);
           }
