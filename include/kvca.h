@@ -841,7 +841,8 @@ int64_t kvca_attend_wait_limit(int64_t nanoseconds);
  * dims stay as they are.
  *
  * kvca_rotate_tokens: (num_rows, heads, head_dim) of fp16, bf16 or fp32 into
- * out, which may be x itself (the same strides) and otherwise overlaps nothing.
+ * out, which may be x itself (the same strides) and otherwise overlaps nothing
+ * (KVCA_ERR_BAD_ARGUMENT); no stride is negative.
  * Row r turns by positions[r]; a row of negative position is left as it was,
  * one outside the table too (KVCA_ERR_BAD_INDEX).  Addresses and strides are
  * multiples of 16 bytes, head_dim a multiple of 8, at most 256.  One launch.
@@ -888,8 +889,9 @@ int kvca_rotate_tokens(const kvca_rotate_desc* desc, int64_t* d_status, kvca_str
  *     heads have no stride.  A NaN makes its 16 values NaN, an infinity becomes
  *     the largest value.
  * Ties go to even.  Addresses and strides are multiples of 16 bytes, head_dim a
- * multiple of 8 (16 with e4m3), at most 256.  query_out may be the query (the
- * same strides); nothing else overlaps.  One launch, no host synchronisation.
+ * multiple of 8 (16 with e4m3), at most 256; no stride is negative.  query_out
+ * may be the query (the same strides); nothing else that is written overlaps
+ * anything (KVCA_ERR_BAD_ARGUMENT).  One launch, no host synchronisation.
  */
 typedef struct kvca_append_desc {
   int64_t num_rows;

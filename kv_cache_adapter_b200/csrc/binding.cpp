@@ -991,6 +991,65 @@ bool all_aligned16(std::initializer_list<uint64_t> words) {
   return aligned16(bits);
 }
 
+// Memory of some dims (sizes, strides in bytes) of rows of `unit` bytes.
+struct Dim {
+  int64_t size, stride;
+};
+
+struct Extent {
+  unsigned __int128 begin, end;  // equal without rows
+};
+
+Extent extent_of(uint64_t address, std::initializer_list<Dim> dims, int64_t unit) {
+  Extent e{address, address};
+  unsigned __int128 last = 0;
+  for (const Dim& d : dims) {
+    if (d.size <= 0) return e;
+    last += static_cast<unsigned __int128>(d.size - 1) * static_cast<uint64_t>(d.stride);
+  }
+  e.end += last + static_cast<uint64_t>(unit);
+  return e;
+}
+
+bool meet(const Extent& a, const Extent& b) {
+  return a.begin < b.end && b.begin < a.end && a.begin < a.end && b.begin < b.end;
+}
+
+// No two rows share a place (strides are not negative).
+bool distinct(std::initializer_list<Dim> dims, int64_t unit) {
+  Dim sorted[5];
+  int n = 0;
+  for (const Dim& d : dims) {
+    if (d.stride < 0) return false;
+    if (d.size <= 1) continue;
+    int at = n++;
+    for (; at > 0 && sorted[at - 1].stride > d.stride; --at) sorted[at] = sorted[at - 1];
+    sorted[at] = d;
+  }
+  unsigned __int128 end = static_cast<uint64_t>(unit);
+  for (int i = 0; i < n; ++i) {
+    if (static_cast<uint64_t>(sorted[i].stride) < end) return false;
+    end += static_cast<unsigned __int128>(sorted[i].size - 1) * static_cast<uint64_t>(sorted[i].stride);
+  }
+  return true;
+}
+
+Extent table_extent(const float* table, int64_t rows, int32_t rotary) {
+  const int64_t row = 4 * static_cast<int64_t>(rotary);
+  return extent_of(reinterpret_cast<uint64_t>(table), {{rows, row}}, row);
+}
+
+bool any_negative(std::initializer_list<int64_t> strides) {
+  for (const int64_t s : strides)
+    if (s < 0) return true;
+  return false;
+}
+
+// Rows of `to` are those of `from`, or lie apart from them.
+bool same_or_apart(const Extent& from, int64_t row, int64_t head, const Extent& to, int64_t to_row, int64_t to_head) {
+  return !meet(from, to) || (from.begin == to.begin && row == to_row && head == to_head);
+}
+
 bool rotation_ok(int32_t rotary_dim, int32_t head_dim, int64_t table_rows) {
   return rotary_dim >= 2 && rotary_dim % 2 == 0 && rotary_dim <= head_dim && table_rows >= 0;
 }
@@ -1009,7 +1068,18 @@ int kvca_rotate_tokens(const kvca_rotate_desc* d, int64_t* d_status, kvca_stream
   if (d->num_rows > kMostTokenRows || d->heads > 65536 || d->num_rows * d->heads > kMostHeadRows)
     return KVCA_ERR_SIZE_LIMIT;
   if (d->num_rows == 0) return KVCA_OK;
-  if (d->x == 0 || d->out == 0 || d->positions == nullptr || d->table == nullptr) return KVCA_ERR_BAD_ARGUMENT;
+  if (d->x == 0 || d->out == 0 || d->positions == nullptr || d->table == nullptr ||
+      any_negative({d->row_stride, d->head_stride, d->out_row_stride, d->out_head_stride}))
+    return KVCA_ERR_BAD_ARGUMENT;
+  const int64_t unit = static_cast<int64_t>(d->head_dim) * (d->type == KVCA_TYPE_F32 ? 4 : 2);
+  const Dim out_rows{d->num_rows, d->out_row_stride}, out_heads{d->heads, d->out_head_stride};
+  const Extent x = extent_of(d->x, {{d->num_rows, d->row_stride}, {d->heads, d->head_stride}}, unit);
+  const Extent out = extent_of(d->out, {out_rows, out_heads}, unit);
+  if (!distinct({out_rows, out_heads}, unit) ||
+      !same_or_apart(x, d->row_stride, d->head_stride, out, d->out_row_stride, d->out_head_stride) ||
+      meet(out, table_extent(d->table, d->table_rows, d->rotary_dim)) ||
+      meet(out, extent_of(reinterpret_cast<uint64_t>(d->positions), {{d->num_rows, 8}}, 8)))
+    return KVCA_ERR_BAD_ARGUMENT;
   kvca::TokenArgs a;
   memset(&a, 0, sizeof(a));
   a.rows = d->num_rows;
@@ -1068,8 +1138,47 @@ int kvca_append_tokens(const kvca_append_desc* d, int64_t* d_status, kvca_stream
   if (d->num_rows == 0) return KVCA_OK;
   if (d->key == 0 || d->value == 0 || d->slot_mapping == nullptr || (turns && (d->table == nullptr || d->positions == nullptr)) ||
       (d->q_heads > 0 && (d->query == 0 || d->query_out == 0)) ||
-      (a.num_slots > 0 && (d->key_cache == 0 || d->value_cache == 0)))
+      (a.num_slots > 0 && (d->key_cache == 0 || d->value_cache == 0)) ||
+      any_negative({d->query_row_stride, d->query_head_stride, d->query_out_row_stride, d->query_out_head_stride,
+                    d->key_row_stride, d->key_head_stride, d->value_row_stride, d->value_head_stride,
+                    d->key_block_stride, d->key_token_stride, d->value_block_stride, d->value_token_stride}) ||
+      (!e2m1 && any_negative({d->key_cache_head_stride, d->value_cache_head_stride})))
     return KVCA_ERR_BAD_ARGUMENT;
+  const int64_t n = d->num_rows, unit = 2 * static_cast<int64_t>(d->head_dim);
+  const int64_t held = e2m1 ? kvca_e2m1_row_bytes(d->kv_heads, d->head_dim) : d->head_dim * (e4m3 ? int64_t{1} : 2);
+  const Dim key_dims[] = {{d->num_blocks, d->key_block_stride}, {d->block_size, d->key_token_stride},
+                          {e2m1 ? 1 : d->kv_heads, d->key_cache_head_stride}};
+  const Dim value_dims[] = {{d->num_blocks, d->value_block_stride}, {d->block_size, d->value_token_stride},
+                            {e2m1 ? 1 : d->kv_heads, d->value_cache_head_stride}};
+  const Extent k = extent_of(d->key, {{n, d->key_row_stride}, {d->kv_heads, d->key_head_stride}}, unit);
+  const Extent v = extent_of(d->value, {{n, d->value_row_stride}, {d->kv_heads, d->value_head_stride}}, unit);
+  const Extent q = extent_of(d->query, {{n, d->query_row_stride}, {d->q_heads, d->query_head_stride}}, unit);
+  const Extent q_out = extent_of(d->query_out, {{n, d->query_out_row_stride}, {d->q_heads, d->query_out_head_stride}}, unit);
+  const Extent kc = extent_of(d->key_cache, {key_dims[0], key_dims[1], key_dims[2]}, held);
+  const Extent vc = extent_of(d->value_cache, {value_dims[0], value_dims[1], value_dims[2]}, held);
+  if (d->q_heads > 0) {
+    const bool in_place = q.begin == q_out.begin;  // (with the same strides)
+    if (!distinct({{n, d->query_out_row_stride}, {d->q_heads, d->query_out_head_stride}}, unit) ||
+        !same_or_apart(q, d->query_row_stride, d->query_head_stride, q_out, d->query_out_row_stride,
+                       d->query_out_head_stride) ||
+        // (slices of one projection, rotated in place, interleave with the keys and values beside them)
+        (in_place ? q.begin == k.begin || q.begin == v.begin : meet(q_out, k) || meet(q_out, v)) ||
+        meet(q_out, table_extent(d->table, d->table_rows, d->rotary_dim)) ||
+        meet(q_out, extent_of(reinterpret_cast<uint64_t>(d->positions), {{n, 8}}, 8)) ||
+        meet(q_out, extent_of(reinterpret_cast<uint64_t>(d->slot_mapping), {{n, 8}}, 8)))
+      return KVCA_ERR_BAD_ARGUMENT;
+  }
+  if (!distinct({key_dims[0], key_dims[1], key_dims[2]}, held) ||
+      !distinct({value_dims[0], value_dims[1], value_dims[2]}, held))
+    return KVCA_ERR_BAD_ARGUMENT;
+  if (meet(kc, vc)) {  // planes of one merged cache lie side by side in its strides
+    const int64_t apart = static_cast<int64_t>(kc.begin > vc.begin ? kc.begin - vc.begin : vc.begin - kc.begin);
+    for (int i = 0; i < 3; ++i)
+      if (key_dims[i].size > 1 && key_dims[i].stride != value_dims[i].stride) return KVCA_ERR_BAD_ARGUMENT;
+    if (!distinct({key_dims[0], key_dims[1], key_dims[2], {2, apart}}, held)) return KVCA_ERR_BAD_ARGUMENT;
+  }
+  for (const Extent& c : {kc, vc})
+    if (meet(c, k) || meet(c, v) || meet(c, q) || meet(c, q_out)) return KVCA_ERR_BAD_ARGUMENT;
   a.rows = d->num_rows;
   a.query = reinterpret_cast<const char*>(d->query);
   a.query_row = d->query_row_stride;
@@ -1125,7 +1234,16 @@ int kvca_read_tokens(const kvca_read_desc* d, int64_t* d_status, kvca_stream_t s
       !cache_slots(d->num_blocks, d->block_size, &a.num_slots, &a.block_size, &a.block_shift))
     return KVCA_ERR_SIZE_LIMIT;
   if (d->num_rows == 0) return KVCA_OK;
-  if (d->slot_mapping == nullptr || d->out == 0 || (a.num_slots > 0 && d->cache == 0)) return KVCA_ERR_BAD_ARGUMENT;
+  if (d->slot_mapping == nullptr || d->out == 0 || (a.num_slots > 0 && d->cache == 0) ||
+      any_negative({d->block_stride, d->token_stride, e2m1 ? 0 : d->head_stride}))
+    return KVCA_ERR_BAD_ARGUMENT;
+  const int64_t wide = static_cast<int64_t>(d->head_dim) * d->kv_heads * (d->type == KVCA_TYPE_F32 ? 4 : 2);
+  const int64_t held = e2m1 ? kvca_e2m1_row_bytes(d->kv_heads, d->head_dim) : d->head_dim;
+  const Extent out = extent_of(d->out, {{d->num_rows, wide}}, wide);
+  if (meet(out, extent_of(d->cache, {{d->num_blocks, d->block_stride}, {d->block_size, d->token_stride},
+                                     {e2m1 ? 1 : d->kv_heads, d->head_stride}}, held)) ||
+      meet(out, extent_of(reinterpret_cast<uint64_t>(d->slot_mapping), {{d->num_rows, 8}}, 8)))
+    return KVCA_ERR_BAD_ARGUMENT;
   a.cache = reinterpret_cast<const char*>(d->cache);
   a.cache_block = d->block_stride;
   a.cache_token = d->token_stride;

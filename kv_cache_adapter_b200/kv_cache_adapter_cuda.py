@@ -1823,12 +1823,10 @@ def _rotation(table: torch.Tensor, index: int, dim: int) -> tuple[int, int, int]
     return at, held, rotary
 
 
-def _result_rows(out: torch.Tensor | None, x: torch.Tensor, at: tuple[int, int, int, int], index: int, size: int,
-                 name: str) -> tuple[torch.Tensor, tuple[int, int, int, int]]:
-    """The result of the rows x (`at`: _token_rows): x itself, or a tensor that
-    nothing of x lies in, and its _token_rows."""
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+def _result_rows(out: torch.Tensor, x: torch.Tensor, at: tuple[int, int, int, int], index: int, size: int,
+                 name: str) -> tuple[int, int, int, int]:
+    """_token_rows of the result of the rows x (`at`: theirs): x itself, or a tensor
+    that nothing of x lies in."""
     to = at if out is x else _token_rows(out, index, x.dtype, size, name)
     if out.shape != x.shape:
         raise ValueError(f"{name} must be {tuple(x.shape)} {x.dtype}")
@@ -1836,7 +1834,7 @@ def _result_rows(out: torch.Tensor | None, x: torch.Tensor, at: tuple[int, int, 
     _distinct((rows, heads), to[1:3], dim * size, name)
     if to[0] < at[3] and at[0] < to[3] and to != at:
         raise ValueError(f"{name} must not overlap what it is computed from (unless it is the same rows)")
-    return out, to
+    return to
 
 
 _pack_rotate = _lib.packer(_lib.RotateDesc)
@@ -1844,16 +1842,8 @@ _pack_append = _lib.packer(_lib.AppendDesc)
 _pack_read = _lib.packer(_lib.ReadDesc)
 
 
-def rotate_tokens(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, *, interleaved: bool = False,
-                  transpose: bool = False, out: torch.Tensor | None = None,
-                  check: bool | None = None) -> torch.Tensor:
-    """Rotary positions (kvca_rotate_tokens): ``x`` ``(rows, heads, head_dim)``
-    fp16, bf16 or fp32, row r turned by ``positions[r]`` (int64), the angles from
-    ``table`` (``rotary_table``), whose width says how many dims of a head turn:
-    pairs ``(i, i + rotary_dim / 2)``, or ``(2 i, 2 i + 1)`` with ``interleaved``.
-    ``transpose`` multiplies by the transposed rotation: the gradient of the
-    former, and the way back to position 0.  Returns ``out``, which may be ``x``
-    itself; rows of negative position are left as they were in it."""
+def _refuse_rotate(x, positions, table, out) -> None:
+    """Raises what is wrong with a call of rotate_tokens."""
     if not isinstance(x, torch.Tensor):
         raise TypeError("x must be torch.Tensor")
     index = x.get_device()
@@ -1870,19 +1860,57 @@ def rotate_tokens(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor,
         raise ValueError(f"x must have heads, and a head_dim in multiples of 8 up to 256, got {heads} and {dim}")
     angles, held, rotary = _rotation(table, index, dim)
     at_positions = _index_rows(positions, index, rows, "positions")
-    out, to = _result_rows(out, x, at, index, size, "out")
+    to = at if out is None else _result_rows(out, x, at, index, size, "out")
+    if out is None:
+        return
     if (to[0] < angles + 4 * held * rotary and angles < to[3]
             or to[0] < at_positions + 8 * rows and at_positions < to[3]):
         raise ValueError("out must not overlap table or positions")
-    if rows == 0:
-        return out
+    raise ValueError("rotate_tokens: invalid arguments")
+
+
+def rotate_tokens(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, *, interleaved: bool = False,
+                  transpose: bool = False, out: torch.Tensor | None = None,
+                  check: bool | None = None) -> torch.Tensor:
+    """Rotary positions (kvca_rotate_tokens): ``x`` ``(rows, heads, head_dim)``
+    fp16, bf16 or fp32, row r turned by ``positions[r]`` (int64), the angles from
+    ``table`` (``rotary_table``), whose width says how many dims of a head turn:
+    pairs ``(i, i + rotary_dim / 2)``, or ``(2 i, 2 i + 1)`` with ``interleaved``.
+    ``transpose`` multiplies by the transposed rotation: the gradient of the
+    former, and the way back to position 0.  Returns ``out``, which may be ``x``
+    itself; rows of negative position are left as they were in it."""
+    tensor = torch.Tensor
+    index = x.get_device() if isinstance(x, tensor) else -1
+    if index < 0 or not (isinstance(positions, tensor) and isinstance(table, tensor)):
+        _refuse_rotate(x, positions, table, None)
+    dtype, shape = x.dtype, x.shape
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=x.device)
+    kind, rotary, rows = _ROW_TYPES.get(dtype), table.shape, positions.shape
+    if not (kind is not None and len(shape) == 3 and len(rotary) == 2 and rows == shape[:1] and isinstance(out, tensor)
+            and out.shape == shape and out.dtype is dtype and out.get_device() == index
+            and positions.get_device() == index and positions.dtype is torch.int64 and positions.is_contiguous()
+            and table.get_device() == index and table.dtype is torch.float32 and table.is_contiguous()):
+        _refuse_rotate(x, positions, table, out)
+    rows, heads, dim = shape
+    held, rotary = rotary
+    row, head, last = x.stride()
+    to_row, to_head, to_last = out.stride()
+    if held == 0 or (rows and (last != 1 or to_last != 1)):
+        _refuse_rotate(x, positions, table, out)
+    size = 4 if kind == _lib.KVCA_TYPE_F32 else 2
+    several, wide = (size, size if heads > 1 else 0) if rows > 1 else (0, size if heads > 1 else 0)
+    desc = _pack_rotate(rows, x.data_ptr(), row * several, head * wide, out.data_ptr(), to_row * several,
+                        to_head * wide, positions.data_ptr(), table.data_ptr(), held, heads, dim,
+                        rotary, kind, bool(interleaved), bool(transpose))
     dev = x.device
-    desc = _pack_rotate(rows, at[0], at[1], at[2], to[0], to[1], to[2], at_positions, angles, held, heads, dim, rotary,
-                        kind, bool(interleaved), bool(transpose))
     with _on(dev):
         rc = _lib_handle.kvca_rotate_tokens(desc, _status(dev).data_ptr(), _stream(dev))
+    if rc == _lib.KVCA_ERR_BAD_ARGUMENT:
+        _refuse_rotate(x, positions, table, out)
     _host_rc(rc, "rotate_tokens")
-    _maybe_check(dev, check, "rotate_tokens")
+    if rows:
+        _maybe_check(dev, check, "rotate_tokens")
     return out
 
 
@@ -1902,24 +1930,9 @@ def _cache_rows(cache: torch.Tensor, size: int, head: int, name: str) -> tuple[i
     return at, steps[0], steps[1], steps[2] if len(steps) == 3 else head, end if cache.numel() else at
 
 
-def append_tokens(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
-                  slot_mapping: torch.Tensor, *, positions: torch.Tensor | None = None,
-                  table: torch.Tensor | None = None, interleaved: bool = False, query: torch.Tensor | None = None,
-                  query_out: torch.Tensor | None = None, key_scale: float = 1.0, value_scale: float = 1.0,
-                  check: bool | None = None) -> torch.Tensor | None:
-    """Keys and values of new tokens into the paged cache, keys rotated on the
-    way, and the tokens' queries rotated (kvca_append_tokens): the step before
-    ``attend_step`` or ``attend_chunk``, in one launch.  ``key`` and ``value``
-    ``(rows, kv_heads, head_dim)`` and ``query`` ``(rows, heads, head_dim)`` are
-    fp16 or bf16, in any order of rows and heads (slices of one projection too).
-    Row r goes to slot ``slot_mapping[r]`` (int64, block * block_size + offset,
-    distinct); rows of negative slot are padding: nothing of them is written.
-    The caches are those of ``attend_step``: of the rows' dtype, e4m3 (which
-    holds ``x / key_scale``, ``x / value_scale``), or uint8 rows of 4-bit values
-    (``e2m1_row_bytes``; scales chosen per 16 dims, times ``key_scale``,
-    ``value_scale``).  ``positions`` and ``table`` are ``rotate_tokens``'s;
-    without them keys are stored as they are.  Returns ``query_out`` (the query
-    itself if given as such), None without a query."""
+def _refuse_append(key, value, key_cache, value_cache, slot_mapping, positions, table, query, query_out, key_scale,
+                   value_scale) -> None:
+    """Raises what is wrong with a call of append_tokens."""
     tensor = torch.Tensor
     if not (isinstance(key, tensor) and isinstance(value, tensor) and isinstance(key_cache, tensor)
             and isinstance(value_cache, tensor)):
@@ -1979,13 +1992,15 @@ def append_tokens(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tenso
         q_heads = query.shape[1]
         if query.shape[0] != rows or query.shape[2] != dim or q_heads < 1:
             raise ValueError(f"query must be ({rows}, heads, {dim}) {dtype}")
-        query_out, q_out = _result_rows(query_out, query, q, index, 2, "query_out")
-        if q_out != q and (q_out[0] < k[3] and k[0] < q_out[3] or q_out[0] < v[3] and v[0] < q_out[3]):
-            raise ValueError("query_out must not overlap key or value")
-        if (q_out[0] < angles + 4 * held * rotary and angles < q_out[3]
-                or q_out[0] < at_positions + 8 * rows and at_positions < q_out[3]
-                or q_out[0] < at_slots + 8 * rows and at_slots < q_out[3]):
-            raise ValueError("query_out must not overlap table, positions or slot_mapping")
+        if query_out is not None:
+            q_out = _result_rows(query_out, query, q, index, 2, "query_out")
+            if (q[0] in (k[0], v[0]) if q_out == q else
+                    q_out[0] < k[3] and k[0] < q_out[3] or q_out[0] < v[3] and v[0] < q_out[3]):
+                raise ValueError("query_out must not overlap key or value")
+            if (q_out[0] < angles + 4 * held * rotary and angles < q_out[3]
+                    or q_out[0] < at_positions + 8 * rows and at_positions < q_out[3]
+                    or q_out[0] < at_slots + 8 * rows and at_slots < q_out[3]):
+                raise ValueError("query_out must not overlap table, positions or slot_mapping")
     elif query_out is not None:
         raise ValueError("query_out needs a query")
     for c in (kc, vc):
@@ -1998,34 +2013,118 @@ def append_tokens(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tenso
             raise ValueError("key_cache and value_cache must not overlap")
         _distinct((*cshape[:-1], 2), (*kc[1:len(cshape)], abs(vc[0] - kc[0])), cshape[-1] * size,
                   "key_cache and value_cache")
+    raise ValueError("append_tokens: invalid arguments")
+
+
+def append_tokens(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                  slot_mapping: torch.Tensor, *, positions: torch.Tensor | None = None,
+                  table: torch.Tensor | None = None, interleaved: bool = False, query: torch.Tensor | None = None,
+                  query_out: torch.Tensor | None = None, key_scale: float = 1.0, value_scale: float = 1.0,
+                  check: bool | None = None) -> torch.Tensor | None:
+    """Keys and values of new tokens into the paged cache, keys rotated on the
+    way, and the tokens' queries rotated (kvca_append_tokens): the step before
+    ``attend_step`` or ``attend_chunk``, in one launch.  ``key`` and ``value``
+    ``(rows, kv_heads, head_dim)`` and ``query`` ``(rows, heads, head_dim)`` are
+    fp16 or bf16, in any order of rows and heads (slices of one projection too).
+    Row r goes to slot ``slot_mapping[r]`` (int64, block * block_size + offset,
+    distinct); rows of negative slot are padding: nothing of them is written.
+    The caches are those of ``attend_step``: of the rows' dtype, e4m3 (which
+    holds ``x / key_scale``, ``x / value_scale``), or uint8 rows of 4-bit values
+    (``e2m1_row_bytes``; scales chosen per 16 dims, times ``key_scale``,
+    ``value_scale``).  ``positions`` and ``table`` are ``rotate_tokens``'s;
+    without them keys are stored as they are.  Returns ``query_out`` (the query
+    itself if given as such), None without a query."""
+    tensor, args = torch.Tensor, (key, value, key_cache, value_cache, slot_mapping, positions, table, query, query_out,
+                                  key_scale, value_scale)
+    if not (isinstance(key, tensor) and isinstance(value, tensor) and isinstance(key_cache, tensor)
+            and isinstance(value_cache, tensor) and isinstance(slot_mapping, tensor)):
+        _refuse_append(*args)
+    index, dtype, ctype, shape, cshape = key.get_device(), key.dtype, key_cache.dtype, key.shape, key_cache.shape
+    kind, cache_kind = _ROW_TYPES.get(dtype), _ATTEND_TYPES.get(ctype)
+    if not (index >= 0 and kind is not None and cache_kind is not None and len(shape) == 3 and value.shape == shape
+            and value.dtype is dtype and value.get_device() == index and value_cache.shape == cshape
+            and value_cache.dtype is ctype and key_cache.get_device() == index and value_cache.get_device() == index
+            and slot_mapping.shape == shape[:1] and slot_mapping.dtype is torch.int64
+            and slot_mapping.get_device() == index and slot_mapping.is_contiguous()):
+        _refuse_append(*args)
+    rows, heads, dim = shape
+    several, wide = 2 if rows > 1 else 0, 2 if heads > 1 else 0
+    key_row, key_head, key_last = key.stride()
+    value_row, value_head, value_last = value.stride()
+    good = key_last == value_last == 1 or rows == 0
+    if ctype is torch.uint8:
+        good = good and len(cshape) == 3 and cshape[2] == _lib_handle.kvca_e2m1_row_bytes(heads, dim)
+    else:
+        good = good and len(cshape) == 4 and cshape[2] == heads and cshape[3] == dim
+    if not good:
+        _refuse_append(*args)
+    size = 2 if ctype is dtype else 1
+    k, v = key_cache.stride(), value_cache.stride()
+    blocks, block_size = cshape[:2]
+    many, deep = size if blocks > 1 else 0, size if block_size > 1 else 0
+    if len(cshape) == 4:
+        across = size if heads > 1 else 0
+        key_across, value_across, good = k[2] * across, v[2] * across, k[3] == v[3] == 1
+    else:
+        key_across, value_across, good = 0, 0, k[2] == v[2] == 1
+    at_positions = angles = held = rotary = 0
+    if table is not None:
+        good = good and (isinstance(positions, tensor) and isinstance(table, tensor) and positions.shape == shape[:1]
+                         and positions.dtype is torch.int64 and positions.get_device() == index
+                         and positions.is_contiguous() and table.dtype is torch.float32 and table.dim() == 2
+                         and table.get_device() == index and table.is_contiguous())
+        if good:
+            held, rotary = table.shape
+            at_positions, angles = positions.data_ptr(), table.data_ptr()
+    elif positions is not None:
+        good = False
+    q_at = q_row = q_head = to = to_row = to_head = q_heads = 0
+    if query is not None:
+        good = good and held > 0 and isinstance(query, tensor) and query.dtype is dtype and query.get_device() == index
+        if not good:
+            _refuse_append(*args)
+        if query_out is None:
+            query_out = torch.empty(query.shape, dtype=dtype, device=key.device)
+        qshape = query.shape
+        good = (len(qshape) == 3 and qshape[0] == rows and qshape[2] == dim and qshape[1] > 0
+                and isinstance(query_out, tensor) and query_out.shape == qshape and query_out.dtype is dtype
+                and query_out.get_device() == index)
+        if good:
+            q_heads = qshape[1]
+            across = 2 if q_heads > 1 else 0
+            q_row, q_head, q_last = query.stride()
+            to_row, to_head, to_last = query_out.stride()
+            q_at, q_row, q_head = query.data_ptr(), q_row * several, q_head * across
+            to, to_row, to_head = query_out.data_ptr(), to_row * several, to_head * across
+            good = q_last == to_last == 1 or rows == 0
+    elif query_out is not None:
+        good = False
+    if not (good and 0 < key_scale < 2.0 ** 61 and 0 < value_scale < 2.0 ** 61):
+        _refuse_append(*args)
+    dev = key.device
+    desc = _pack_append(
+        rows, q_at, q_row, q_head, to, to_row, to_head, key.data_ptr(), key_row * several, key_head * wide,
+        value.data_ptr(), value_row * several, value_head * wide, key_cache.data_ptr(), k[0] * many, k[1] * deep,
+        key_across, value_cache.data_ptr(), v[0] * many, v[1] * deep, value_across, blocks, block_size,
+        slot_mapping.data_ptr(), at_positions, angles, held, q_heads, heads, dim, rotary, kind, cache_kind,
+        bool(interleaved), key_scale, value_scale)
+    with _on(dev):
+        rc = _lib_handle.kvca_append_tokens(desc, _status(dev).data_ptr(), _stream(dev))
+    if rc == _lib.KVCA_ERR_BAD_ARGUMENT:
+        _refuse_append(*args)
+    _host_rc(rc, "append_tokens")
     if rows:
-        dev = key.device
-        desc = _pack_append(
-            rows, q[0], q[1], q[2], q_out[0], q_out[1], q_out[2], k[0], k[1], k[2], v[0], v[1], v[2], kc[0], kc[1], kc[2],
-            kc[3], vc[0], vc[1], vc[2], vc[3], cshape[0], cshape[1], at_slots, at_positions, angles, held, q_heads, heads,
-            dim, rotary, _ROW_TYPES[dtype], _ATTEND_TYPES[ctype], bool(interleaved), key_scale, value_scale)
-        with _on(dev):
-            rc = _lib_handle.kvca_append_tokens(desc, _status(dev).data_ptr(), _stream(dev))
-        _host_rc(rc, "append_tokens")
         _maybe_check(dev, check, "append_tokens")
     return query_out
 
 
-def read_tokens(cache: torch.Tensor, slot_mapping: torch.Tensor, *, head_dim: int | None = None, scale: float = 1.0,
-                dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
-                check: bool | None = None) -> torch.Tensor:
-    """Token rows of an 8- or 4-bit cache plane as wider values
-    (kvca_read_tokens): row ``slot_mapping[r]`` of ``cache`` (e4m3 ``(num_blocks,
-    block_size, kv_heads, head_dim)`` or uint8 rows of 4-bit values, whose
-    ``head_dim`` has to be given) times ``scale`` in ``out`` ``(rows, kv_heads,
-    head_dim)`` fp16, bf16 or fp32 (``dtype`` where it is not given).  Rows of
-    negative slot are left as they were in ``out``."""
+def _refuse_read(cache, slot_mapping, head_dim, dtype, out) -> None:
+    """Raises what is wrong with a call of read_tokens."""
     if not isinstance(cache, torch.Tensor):
         raise TypeError("cache must be torch.Tensor")
     index = cache.get_device()
     if index < 0:
         raise ValueError("cache must be a CUDA tensor")
-    dev = cache.device
     four = cache.dtype is torch.uint8
     if four:
         if head_dim is None:
@@ -2054,19 +2153,61 @@ def read_tokens(cache: torch.Tensor, slot_mapping: torch.Tensor, *, head_dim: in
     if kind is None:
         raise TypeError(f"incorrect dtype {dtype}" if out is None else "out has incorrect dtype")
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=dtype, device=dev)
+        raise ValueError("read_tokens: invalid arguments")
     at = out.data_ptr()
     if out.shape != (rows, heads, dim) or out.get_device() != index or not out.is_contiguous() or at & 15:
         raise ValueError(f"out must be a contiguous, 16-byte aligned ({rows}, {heads}, {dim}) tensor on cuda:{index}")
     end = at + rows * heads * dim * (4 if kind == _lib.KVCA_TYPE_F32 else 2)
     if at < c[4] and c[0] < end or at < at_slots + 8 * rows and at_slots < end:
         raise ValueError("out must not overlap cache or slot_mapping")
+    raise ValueError("read_tokens: invalid arguments")
+
+
+def read_tokens(cache: torch.Tensor, slot_mapping: torch.Tensor, *, head_dim: int | None = None, scale: float = 1.0,
+                dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
+                check: bool | None = None) -> torch.Tensor:
+    """Token rows of an 8- or 4-bit cache plane as wider values
+    (kvca_read_tokens): row ``slot_mapping[r]`` of ``cache`` (e4m3 ``(num_blocks,
+    block_size, kv_heads, head_dim)`` or uint8 rows of 4-bit values, whose
+    ``head_dim`` has to be given) times ``scale`` in ``out`` ``(rows, kv_heads,
+    head_dim)`` fp16, bf16 or fp32 (``dtype`` where it is not given).  Rows of
+    negative slot are left as they were in ``out``."""
+    tensor, given = torch.Tensor, out
+    if not (isinstance(cache, tensor) and isinstance(slot_mapping, tensor)
+            and (out is None or isinstance(out, tensor))):
+        _refuse_read(cache, slot_mapping, head_dim, dtype, given)
+    index, ctype, shape, rows = cache.get_device(), cache.dtype, cache.shape, slot_mapping.numel()
+    kind = _ROW_TYPES.get(dtype if out is None else out.dtype)
+    good = (index >= 0 and kind is not None and slot_mapping.dtype is torch.int64 and slot_mapping.dim() == 1
+            and slot_mapping.get_device() == index and slot_mapping.is_contiguous())
+    heads = dim = across = 0
+    if ctype is torch.uint8:
+        if good and head_dim is not None:
+            dim = int(head_dim)
+            heads = _e2m1_heads(cache, dim, "cache")
+    elif ctype is torch.float8_e4m3fn and len(shape) == 4:
+        heads, dim = shape[2:]
+        good = good and (head_dim is None or head_dim == dim)
+    if not (good and heads > 0 and dim > 0):
+        _refuse_read(cache, slot_mapping, head_dim, dtype, given)
+    dev, stride = cache.device, cache.stride()
+    if out is None:
+        out = torch.empty((rows, heads, dim), dtype=dtype, device=dev)
+    if not (stride[-1] == 1 and (given is None or out.shape == (rows, heads, dim) and out.get_device() == index
+                                 and out.is_contiguous())):
+        _refuse_read(cache, slot_mapping, head_dim, dtype, given)
+    blocks, block_size = shape[:2]
+    if len(shape) == 4 and heads > 1:
+        across = stride[2]
+    desc = _pack_read(cache.data_ptr(), stride[0] if blocks > 1 else 0, stride[1] if block_size > 1 else 0, across,
+                      blocks, block_size, slot_mapping.data_ptr(), rows, heads, dim, _ATTEND_TYPES[ctype], kind, scale,
+                      0, out.data_ptr())
+    with _on(dev):
+        rc = _lib_handle.kvca_read_tokens(desc, _status(dev).data_ptr(), _stream(dev))
+    if rc == _lib.KVCA_ERR_BAD_ARGUMENT:
+        _refuse_read(cache, slot_mapping, head_dim, dtype, given)
+    _host_rc(rc, "read_tokens")
     if rows:
-        desc = _pack_read(c[0], c[1], c[2], c[3], num_blocks, block_size, at_slots, rows, heads, dim,
-                          _lib.KVCA_TYPE_E2M1 if four else _lib.KVCA_TYPE_E4M3, kind, scale, 0, at)
-        with _on(dev):
-            rc = _lib_handle.kvca_read_tokens(desc, _status(dev).data_ptr(), _stream(dev))
-        _host_rc(rc, "read_tokens")
         _maybe_check(dev, check, "read_tokens")
     return out
 

@@ -76,6 +76,37 @@ def test_c_abi_refuses(call, desc, bad):
     assert getattr(_lib.load(), call)(ctypes.byref(desc(**bad)), None, None) == BAD
 
 
+# what is written meets itself, or something that is read (byte ranges of the descriptors above)
+FUSED = dict(key=(1 << 20) + 2048, value=(1 << 20) + 2560, query_row_stride=1 << 12, key_row_stride=1 << 12,
+             value_row_stride=1 << 12)
+MERGED = dict(value_cache=(1 << 24) + 512, key_token_stride=1024, value_token_stride=1024, key_block_stride=16384,
+              value_block_stride=16384)
+ROTATE_MEETS = [dict(out=(1 << 20) + 256), dict(out=1 << 20, out_row_stride=4096), dict(out_head_stride=128),
+                dict(out_row_stride=1024), dict(out_head_stride=0), dict(out=8192), dict(out=4096), dict(out=4112),
+                dict(row_stride=-2048), dict(out_head_stride=-256)]
+APPEND_MEETS = [dict(query_out=(1 << 20) + 256), dict(query_out=1 << 20, query_out_row_stride=4096),
+                dict(query_out_head_stride=0), dict(query_out_row_stride=1024), dict(query_out=8192),
+                dict(query_out=4096), dict(query_out=1 << 22), dict(query_out=(1 << 23) + 512),
+                dict(query_out=(1 << 20) + 2048, query_out_row_stride=1 << 12, **FUSED),
+                dict(query_out=1 << 20, query=1 << 20, key=1 << 20), dict(key_cache=1 << 20), dict(key_cache=1 << 21),
+                dict(value_cache=1 << 22), dict(value_cache=(1 << 23) + 1536), dict(value_cache=1 << 24),
+                dict(value_cache=(1 << 24) + 256), dict(key_token_stride=256), dict(key_block_stride=4096),
+                dict(value_block_stride=0), dict(value_cache_head_stride=0), dict(key_row_stride=-512),
+                dict(value_block_stride=-8192), dict(value_cache_head_stride=-256),
+                {**MERGED, "value_token_stride": 512}, {**MERGED, "value_cache": (1 << 24) + 256},
+                dict(cache_type=_lib.KVCA_TYPE_E2M1, value_cache=(1 << 24) + 64)]
+READ_MEETS = [dict(out=1 << 20), dict(out=(1 << 20) + 16), dict(out=(1 << 20) - 1024), dict(out=4096),
+              dict(token_stride=-256), dict(cache_type=_lib.KVCA_TYPE_E2M1, out=(1 << 20) + 7 * 4096)]
+
+
+@pytest.mark.parametrize("call,desc,bad", [("kvca_rotate_tokens", rotate_desc, b) for b in ROTATE_MEETS]
+                         + [("kvca_append_tokens", append_desc, b) for b in APPEND_MEETS]
+                         + [("kvca_read_tokens", read_desc, b) for b in READ_MEETS],
+                         ids=lambda v: ",".join(v) if isinstance(v, dict) else None)
+def test_c_abi_refuses_overlaps(call, desc, bad):
+    assert getattr(_lib.load(), call)(ctypes.byref(desc(**bad)), None, None) == BAD
+
+
 @pytest.mark.parametrize("call,desc", [("kvca_rotate_tokens", rotate_desc), ("kvca_append_tokens", append_desc),
                                        ("kvca_read_tokens", read_desc)])
 def test_c_abi_nothing_to_do_and_size_limits(call, desc):
