@@ -2,9 +2,10 @@
 
     python -m kv_cache_adapter_b200.build [--force] [--ptxas-verbose]
 
-Compiles csrc/kv_adapter_cuda.cu (kernels), csrc/row_ceiling.cu (the
-random-row roofline reference) and csrc/binding.cpp (the C ABI of
-include/kvca.h) with nvcc into a shared library next to this file, with
+Compiles csrc/kv_adapter_cuda.cu (movers and metadata), csrc/attend_*.cu
+(attention over the pages), csrc/page_ops.cu (pages of sequences),
+csrc/token_ops.cu (rows of new tokens), csrc/row_ceiling.cu (the random-row
+roofline reference) and csrc/binding.cpp (the C ABI of include/kvca.h) with nvcc into a shared library next to this file, with
 the CUDA runtime linked statically so the library has no runtime dependency
 beyond the driver.
 """
@@ -21,11 +22,11 @@ PKG = pathlib.Path(__file__).resolve().parent
 REPO = PKG.parent
 CSRC = PKG / "csrc"
 INCLUDE = REPO / "include"
-SOURCES = [CSRC / "kv_adapter_cuda.cu", CSRC / "attend_step.cu", CSRC / "attend_step_four.cu", CSRC / "attend_chunk.cu", CSRC / "page_ops.cu",
-           CSRC / "token_ops.cu", CSRC / "row_ceiling.cu", CSRC / "binding.cpp"]
+SOURCES = [CSRC / "kv_adapter_cuda.cu", CSRC / "attend_step.cu", CSRC / "attend_step_four.cu",
+           CSRC / "attend_chunk.cu", CSRC / "page_ops.cu", CSRC / "token_ops.cu", CSRC / "row_ceiling.cu",
+           CSRC / "binding.cpp"]
 HEADERS = [CSRC / "kvca_launch.h", CSRC / "kvca_device.cuh", CSRC / "kvca_host.cuh", CSRC / "attend_common.cuh",
-           CSRC / "attend_step_common.cuh",
-           INCLUDE / "kvca.h"]
+           CSRC / "attend_step_common.cuh", INCLUDE / "kvca.h"]
 TARGET = PKG / "libkvca_b200.so"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

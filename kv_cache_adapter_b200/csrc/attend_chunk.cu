@@ -32,6 +32,13 @@
 // 64, e4m3, 275-279 us: 19, 41 and 46 %.  24 sequences with 1-8 tokens over
 // 27,000 keys 51-53 us (2.1 TB/s): at most 32 rows of a block's 256.
 //
+// 4-bit rows are bytes to shared memory first (kAhead tiles in flight), from
+// where the same four warps widen a tile once it has arrived: code times scale,
+// exact in fp16.  bf16 queries are lifted to fp16 (with a power of two per row)
+// by blocks of the planning kernel, to be copied like fp16 ones: converted by
+// warps 14 and 15 they held up each segment (691 us for 6,465 prompt tokens, now
+// 433-440; the same ones over a 16-bit cache take 370, the rest is the widening).
+//
 // Probabilities go into the second product as the 16-bit type that the tensor
 // cores multiply values in, rounded to half a step: 2^-11 of each as fp16 (fp16
 // and e4m3 caches), 2^-8 as bf16, as much as the result's own rounding and

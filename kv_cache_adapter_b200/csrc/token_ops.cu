@@ -14,6 +14,15 @@
 // sides of 8 of them, so each value is loaded once and its place may be its
 // result's; neighbouring pairs (and pairs at odd distances) lie 8 dims to a lane,
 // 16 where they are stored in 4 bits: a group with its scale.
+//
+// Bytes bound the large calls: each row is read and written once, so a turn of 8
+// dims costs 32 bytes and some 20 instructions.  A warp takes up to 12 turns, two
+// loaded at a time.  16,384 tokens (32 query and 2 x 8 K/V heads of 128, bf16):
+// 67 us, 64 of bytes at the copy's rate (91 us with three turns to a warp, all loaded at once);
+// the gradient of 8,192 x 32 fp32 heads, neighbouring pairs: 47 us, 43 of bytes.
+// To 4 bits, 8,191 such tokens and their way back: 53 us, 33 of bytes; there the
+// warps issue on 62 % of the cycles (maxima over lanes, two divisions to the
+// nearest, codes).  Few tokens: the host's 8-12 us, in a replayed graph 4.
 
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -534,7 +543,7 @@ __device__ __forceinline__ void store16(char* p, const float (&x)[16], bool wide
 
 // A block reads `tokens` rows, a thread 16 values of one at a time (4 bits: a group
 // with its scale).  Bound by HBM, once enough rows are on their way: 65,536 tokens
-// of 8 heads of 128 from 4 bits to bf16 (172 MB) 35 us; with 8 values to a unit 48.
+// of 8 heads of 128 from 4 bits to bf16 (172 MB) 31 us; with 8 values to a unit a fifth more.
 template <typename Out, bool kFour>
 __global__ void __launch_bounds__(kReadThreads) read_rows_kernel(const __grid_constant__ ReadArgs a, int tokens,
                                                                 uint32_t reciprocal) {
