@@ -1878,11 +1878,16 @@ def rotate_tokens(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor,
     pairs ``(i, i + rotary_dim / 2)``, or ``(2 i, 2 i + 1)`` with ``interleaved``.
     ``transpose`` multiplies by the transposed rotation: the gradient of the
     former, and the way back to position 0.  Returns ``out``, which may be ``x``
-    itself; rows of negative position are left as they were in it."""
+    itself; rows of negative position are left as they were in it.  Nothing is
+    recorded for autograd, so an ``x`` that wants a gradient is refused where
+    gradients are on: call this from an autograd function's two sides."""
     tensor = torch.Tensor
     index = x.get_device() if isinstance(x, tensor) else -1
     if index < 0 or not (isinstance(positions, tensor) and isinstance(table, tensor)):
         _refuse_rotate(x, positions, table, None)
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("rotate_tokens records no gradient: call it without (torch.no_grad, or an autograd "
+                           "function whose backward has transpose=True)")
     dtype, shape = x.dtype, x.shape
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=x.device)
@@ -2033,7 +2038,8 @@ def append_tokens(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tenso
     (``e2m1_row_bytes``; scales chosen per 16 dims, times ``key_scale``,
     ``value_scale``).  ``positions`` and ``table`` are ``rotate_tokens``'s;
     without them keys are stored as they are.  Returns ``query_out`` (the query
-    itself if given as such), None without a query."""
+    itself if given as such), None without a query.  No gradients: the cache
+    holds no graph."""
     tensor, args = torch.Tensor, (key, value, key_cache, value_cache, slot_mapping, positions, table, query, query_out,
                                   key_scale, value_scale)
     if not (isinstance(key, tensor) and isinstance(value, tensor) and isinstance(key_cache, tensor)

@@ -591,3 +591,48 @@ def test_refusals(ops, dev):
                             ((four[0], at), dict(head_dim=64, out=k[:3]), "must be a contiguous")):
         with pytest.raises((ValueError, TypeError), match=match):
             ops.read_tokens(*args, **kw)
+
+
+class Rotated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ops, x, positions, table, interleaved):
+        ctx.save_for_backward(positions, table)
+        ctx.ops, ctx.interleaved = ops, interleaved
+        return ops.rotate_tokens(x, positions, table, interleaved=interleaved, check=True)
+
+    @staticmethod
+    def backward(ctx, grad):
+        return (None, ctx.ops.rotate_tokens(grad.contiguous(), *ctx.saved_tensors, interleaved=ctx.interleaved,
+                                            transpose=True, check=True), None, None, None)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_gradients_through_an_autograd_function_and_refused_without(ops, dev, interleaved):
+    """The loss <w, y> + |y|^2 / 2 of y = R x changes over a step d by exactly
+    <gradient, d> + |d|^2 / 2.  In fp32 a value of y is off by at most 4 half steps of
+    |x1| + |x2| (two products, a sum, the table), which count |w| + |y| times in the
+    loss, and so does the gradient: over a head, whose sums hold every pair's, and for
+    two losses, the gradient and lengths that the table keeps but for its rounding, 4
+    times that.  The rest is in 64 bits."""
+    x, step, w = (rows_of((33, 5, 64), F32, seed).to(dev) for seed in (1, 2, 3))
+    at = places(33, 500, 4).to(dev)
+    table = ops.rotary_table(500, 64, device=dev)
+    x.requires_grad_()
+    for out in (None, x.detach().clone()):
+        with pytest.raises(RuntimeError, match="records no gradient"):
+            ops.rotate_tokens(x, at, table, interleaved=interleaved, out=out)
+    with torch.no_grad():
+        assert not ops.rotate_tokens(x, at, table, interleaved=interleaved).requires_grad
+
+    def loss(v):
+        y = Rotated.apply(ops, v, at, table, interleaved).double()
+        return (y * w.double()).sum() + (y ** 2).sum() / 2
+
+    (grad,) = torch.autograd.grad(loss(x), x)
+    with torch.no_grad():
+        there = x + step
+        moved = there.double() - x.double()
+        want = (grad.double() * moved).sum() + (moved ** 2).sum() / 2
+        size = (x.abs() + there.abs()).double()
+        bound = 4 * 4 * 2.0 ** -24 * (size.sum(-1) * (w.abs().double() + size).sum(-1)).sum()
+        assert abs(loss(there) - loss(x) - want) <= bound
