@@ -37,7 +37,7 @@
 // exact in fp16.  bf16 queries are lifted to fp16 (with a power of two per row)
 // by blocks of the planning kernel, to be copied like fp16 ones: converted by
 // warps 14 and 15 they held up each segment (691 us for 6,465 prompt tokens, now
-// 433-440; the same ones over a 16-bit cache take 370, the rest is the widening).
+// 433-441; the same ones over a 16-bit cache take 370, the rest is the widening).
 //
 // Probabilities go into the second product as the 16-bit type that the tensor
 // cores multiply values in, rounded to half a step: 2^-11 of each as fp16 (fp16

@@ -21,8 +21,8 @@
 // 67 us, 64 of bytes at the copy's rate (91 us with three turns to a warp, all loaded at once);
 // the gradient of 8,192 x 32 fp32 heads, neighbouring pairs: 47 us, 43 of bytes.
 // To 4 bits, 8,191 such tokens and their way back: 53 us, 33 of bytes; there the
-// warps issue on 62 % of the cycles (maxima over lanes, two divisions to the
-// nearest, codes).  Few tokens: the host's 8-12 us, in a replayed graph 4.
+// registers bound the rows in flight (6 blocks per SM 59 us, 8 with spills 57;
+// fewer instructions per group the same).  Few tokens: the host's 8-12 us, in a replayed graph 4.
 
 #include <cuda_runtime.h>
 #include <stdint.h>
