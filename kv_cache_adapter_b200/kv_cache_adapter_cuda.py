@@ -1485,16 +1485,22 @@ def _step_counters(dev: torch.device, stream: int) -> torch.Tensor:
 def _attend_rows(t: torch.Tensor, shape, name: str) -> list[int]:
     """Strides in bytes of the leading dims of rows of head_dim (0 for a dim of size 1)."""
     size = t.element_size()
-    stride = t.stride()
-    out = [x * size if n > 1 else 0 for n, x in zip(shape[:-1], stride)]
-    bits = t.data_ptr()
-    for x in out:
-        bits |= x
-    if bits & 15 or (stride[-1] != 1 and t.numel()):
+    if len(shape) == 3:
+        a, b, _ = shape
+        one, two, last = t.stride()
+        out = [one * size if a > 1 else 0, two * size if b > 1 else 0]
+        bits = t.data_ptr() | out[0] | out[1]
+    else:
+        a, b, c, _ = shape
+        one, two, three, last = t.stride()
+        out = [one * size if a > 1 else 0, two * size if b > 1 else 0, three * size if c > 1 else 0]
+        bits = t.data_ptr() | out[0] | out[1] | out[2]
+    if bits & 15 or (last != 1 and t.numel()):
         raise ValueError(f"{name}: rows of head_dim must be contiguous and 16-byte aligned")
     return out
 
 
+_DENSE = torch.contiguous_format  # (empty_like reads a shape in half the time that torch.empty takes)
 _pack_attend = _lib.packer(_lib.AttendDesc)
 
 
@@ -1568,7 +1574,7 @@ def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torc
     q_end = q_ptr + (rows - 1) * qs[0] + (heads - 1) * qs[1] + 2 * dim  # (without rows nothing is written)
     size = 2 * rows * heads * dim
     if out is None:
-        out = torch.empty(qshape, dtype=qtype, device=dev)
+        out = torch.empty_like(query, memory_format=_DENSE)
         out_ptr = out.data_ptr()
     elif not isinstance(out, tensor):
         raise TypeError("out must be torch.Tensor")
@@ -1890,7 +1896,7 @@ def rotate_tokens(x: torch.Tensor, positions: torch.Tensor, table: torch.Tensor,
                            "function whose backward has transpose=True)")
     dtype, shape = x.dtype, x.shape
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=_DENSE)
     kind, rotary, rows = _ROW_TYPES.get(dtype), table.shape, positions.shape
     if not (kind is not None and len(shape) == 3 and len(rotary) == 2 and rows == shape[:1] and isinstance(out, tensor)
             and out.shape == shape and out.dtype is dtype and out.get_device() == index
@@ -2090,7 +2096,7 @@ def append_tokens(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tenso
         if not good:
             _refuse_append(*args)
         if query_out is None:
-            query_out = torch.empty(query.shape, dtype=dtype, device=key.device)
+            query_out = torch.empty_like(query, memory_format=_DENSE)
         qshape = query.shape
         good = (len(qshape) == 3 and qshape[0] == rows and qshape[2] == dim and qshape[1] > 0
                 and isinstance(query_out, tensor) and query_out.shape == qshape and query_out.dtype is dtype
