@@ -1050,6 +1050,56 @@ bool same_or_apart(const Extent& from, int64_t row, int64_t head, const Extent& 
   return !meet(from, to) || (from.begin == to.begin && row == to_row && head == to_head);
 }
 
+// (num_rows, heads) rows of a tensor, strides in bytes.
+struct HeadRows {
+  uint64_t address;
+  int64_t row;
+  int64_t heads, head;
+};
+
+constexpr int64_t kMostHeadPairs = int64_t{1} << 16;
+
+// Whether rows of two tensors, `unit` bytes each, meet; strides are not negative.
+// Exact where both have the same row stride and the same head stride, or heads side
+// by side, or few of them: for two heads, rows of the one lie multiples of the row
+// stride from those of the other.  Others that interleave count as meeting.
+bool rows_meet(int64_t num_rows, HeadRows a, HeadRows b, int64_t unit) {
+  using wide = __int128;
+  if (!meet(extent_of(a.address, {{num_rows, a.row}, {a.heads, a.head}}, unit),
+            extent_of(b.address, {{num_rows, b.row}, {b.heads, b.head}}, unit)))
+    return false;
+  if (num_rows == 1) a.row = b.row = 0;
+  if (a.row != b.row) return true;
+  int64_t a_unit = unit, b_unit = unit;
+  const auto join = [unit](HeadRows* t, int64_t* whole) {  // heads that lie side by side
+    if (t->head > unit && t->heads > 1) return;
+    *whole = (t->heads - 1) * t->head + unit;
+    t->heads = 1;
+  };
+  join(&a, &a_unit);
+  join(&b, &b_unit);
+  const bool alike = a.heads > 1 && b.heads > 1 && a.head == b.head;  // only differences of heads count
+  if (!alike && a.heads * b.heads > kMostHeadPairs) return true;
+  const int64_t pairs = alike ? a.heads + b.heads - 1 : a.heads * b.heads;
+  for (int64_t p = 0; p < pairs; ++p) {
+    wide d = static_cast<wide>(b.address) - static_cast<wide>(a.address);
+    if (alike)
+      d += static_cast<wide>(p - (a.heads - 1)) * a.head;
+    else
+      d += static_cast<wide>(p % b.heads) * b.head - static_cast<wide>(p / b.heads) * a.head;
+    // the first of b's rows, from the first that any of a's may have beside it, to end behind a's begin
+    if (a.row > 0) {
+      const wide least = 1 - b_unit - d, most = num_rows - 1;
+      wide rows = least / a.row + (least > 0 && least % a.row != 0 ? 1 : 0);
+      if (rows < -most) rows = -most;
+      if (rows > most) continue;
+      d += rows * a.row;
+    }
+    if (d < a_unit && d + b_unit > 0) return true;
+  }
+  return false;
+}
+
 bool rotation_ok(int32_t rotary_dim, int32_t head_dim, int64_t table_rows) {
   return rotary_dim >= 2 && rotary_dim % 2 == 0 && rotary_dim <= head_dim && table_rows >= 0;
 }
@@ -1158,11 +1208,14 @@ int kvca_append_tokens(const kvca_append_desc* d, int64_t* d_status, kvca_stream
   const Extent vc = extent_of(d->value_cache, {value_dims[0], value_dims[1], value_dims[2]}, held);
   if (d->q_heads > 0) {
     const bool in_place = q.begin == q_out.begin;  // (with the same strides)
+    const HeadRows queries{d->query, d->query_row_stride, d->q_heads, d->query_head_stride};
     if (!distinct({{n, d->query_out_row_stride}, {d->q_heads, d->query_out_head_stride}}, unit) ||
         !same_or_apart(q, d->query_row_stride, d->query_head_stride, q_out, d->query_out_row_stride,
                        d->query_out_head_stride) ||
         // (slices of one projection, rotated in place, interleave with the keys and values beside them)
-        (in_place ? q.begin == k.begin || q.begin == v.begin : meet(q_out, k) || meet(q_out, v)) ||
+        (in_place ? rows_meet(n, queries, {d->key, d->key_row_stride, d->kv_heads, d->key_head_stride}, unit) ||
+                        rows_meet(n, queries, {d->value, d->value_row_stride, d->kv_heads, d->value_head_stride}, unit)
+                  : meet(q_out, k) || meet(q_out, v)) ||
         meet(q_out, table_extent(d->table, d->table_rows, d->rotary_dim)) ||
         meet(q_out, extent_of(reinterpret_cast<uint64_t>(d->positions), {{n, 8}}, 8)) ||
         meet(q_out, extent_of(reinterpret_cast<uint64_t>(d->slot_mapping), {{n, 8}}, 8)))

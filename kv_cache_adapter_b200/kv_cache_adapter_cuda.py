@@ -1843,6 +1843,41 @@ def _result_rows(out: torch.Tensor, x: torch.Tensor, at: tuple[int, int, int, in
     return to
 
 
+def _rows_meet(rows: int, a: tuple[int, int, int, int], b: tuple[int, int, int, int], unit: int) -> bool:
+    """Whether rows of two tensors (address, row stride, heads, head stride), `unit`
+    bytes each, meet, as the C interface finds it: exact where the strides are the
+    same, or heads lie side by side."""
+    if not rows:
+        return False
+    ends = [t[0] + (rows - 1) * t[1] + (t[2] - 1) * t[3] + unit for t in (a, b)]
+    if a[0] >= ends[1] or b[0] >= ends[0]:
+        return False
+    row = a[1] if rows > 1 else 0
+    if rows > 1 and b[1] != row:
+        return True
+    spans = []
+    for address, _, heads, head in (a, b):  # heads that lie side by side are one
+        joined = head <= unit or heads == 1
+        spans.append((address, 1 if joined else heads, head, (heads - 1) * head + unit if joined else unit))
+    (at, heads, head, size), (other, other_heads, other_head, other_size) = spans
+    if heads > 1 and other_heads > 1 and head == other_head:  # only differences of heads count
+        shifts = [h * head for h in range(1 - heads, other_heads)]
+    elif heads * other_heads > 1 << 16:
+        return True
+    else:
+        shifts = [h * other_head - g * head for g in range(heads) for h in range(other_heads)]
+    for shift in shifts:
+        d = other - at + shift
+        if row:  # the first of b's rows that ends behind a's begin
+            n = max(-((other_size - 1 + d) // row), 1 - rows)
+            if n >= rows:
+                continue
+            d += n * row
+        if -other_size < d < size:
+            return True
+    return False
+
+
 _pack_rotate = _lib.packer(_lib.RotateDesc)
 _pack_append = _lib.packer(_lib.AppendDesc)
 _pack_read = _lib.packer(_lib.ReadDesc)
@@ -2005,8 +2040,11 @@ def _refuse_append(key, value, key_cache, value_cache, slot_mapping, positions, 
             raise ValueError(f"query must be ({rows}, heads, {dim}) {dtype}")
         if query_out is not None:
             q_out = _result_rows(query_out, query, q, index, 2, "query_out")
-            if (q[0] in (k[0], v[0]) if q_out == q else
-                    q_out[0] < k[3] and k[0] < q_out[3] or q_out[0] < v[3] and v[0] < q_out[3]):
+            if q_out == q:
+                met = any(_rows_meet(rows, (*q[:2], q_heads, q[2]), (*t[:2], heads, t[2]), 2 * dim) for t in (k, v))
+            else:
+                met = q_out[0] < k[3] and k[0] < q_out[3] or q_out[0] < v[3] and v[0] < q_out[3]
+            if met:
                 raise ValueError("query_out must not overlap key or value")
             if (q_out[0] < angles + 4 * held * rotary and angles < q_out[3]
                     or q_out[0] < at_positions + 8 * rows and at_positions < q_out[3]
