@@ -1230,8 +1230,14 @@ int kvca_append_tokens(const kvca_append_desc* d, int64_t* d_status, kvca_stream
       if (key_dims[i].size > 1 && key_dims[i].stride != value_dims[i].stride) return KVCA_ERR_BAD_ARGUMENT;
     if (!distinct({key_dims[0], key_dims[1], key_dims[2], {2, apart}}, held)) return KVCA_ERR_BAD_ARGUMENT;
   }
+  // (without a table neither it nor positions are looked at)
+  const Extent slots = extent_of(reinterpret_cast<uint64_t>(d->slot_mapping), {{n, 8}}, 8);
+  const Extent positions = extent_of(reinterpret_cast<uint64_t>(d->positions), {{turns ? n : 0, 8}}, 8);
+  const Extent table = table_extent(d->table, turns ? d->table_rows : 0, d->rotary_dim);
   for (const Extent& c : {kc, vc})
-    if (meet(c, k) || meet(c, v) || meet(c, q) || meet(c, q_out)) return KVCA_ERR_BAD_ARGUMENT;
+    if (meet(c, k) || meet(c, v) || meet(c, q) || meet(c, q_out) || meet(c, slots) || meet(c, positions) ||
+        meet(c, table))
+      return KVCA_ERR_BAD_ARGUMENT;
   a.rows = d->num_rows;
   a.query = reinterpret_cast<const char*>(d->query);
   a.query_row = d->query_row_stride;

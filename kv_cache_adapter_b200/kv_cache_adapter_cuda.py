@@ -2057,6 +2057,9 @@ def _refuse_append(key, value, key_cache, value_cache, slot_mapping, positions, 
         if (begin < k[3] and k[0] < end or begin < v[3] and v[0] < end or begin < q[3] and q[0] < end
                 or begin < q_out[3] and q_out[0] < end):
             raise ValueError("the caches must not overlap the rows")
+        if (begin < at_slots + 8 * rows and at_slots < end or begin < at_positions + 8 * rows and at_positions < end
+                or begin < angles + 4 * held * rotary and angles < end):
+            raise ValueError("the caches must not overlap slot_mapping, positions or table")
     if kc[0] < vc[4] and vc[0] < kc[4]:  # planes of one merged cache lie side by side in its strides
         if kc[1:4] != vc[1:4]:
             raise ValueError("key_cache and value_cache must not overlap")

@@ -57,3 +57,19 @@ def test_rows_that_meet():
             assert got == truth, (rows, unit, a, b)
             met, apart = met + truth, apart + (not truth)
     assert met > 300 and apart > 300
+
+
+# The descriptor's slot_mapping and positions (32 bytes each) lie at 4096, its table (51,200 bytes) at 8192; with the
+# strides as they are a cache holds 64 KB.
+APART = dict(slot_mapping=1 << 26, positions=1 << 27, table=1 << 28)
+CACHE_MEETS = [dict(key_cache=4096), dict(value_cache=4096), {**APART, "slot_mapping": (1 << 24) + 65536 - 8},
+               {**APART, "slot_mapping": (1 << 25) - 24}, {**APART, "positions": (1 << 24) + 512},
+               {**APART, "positions": (1 << 25) + 65536 - 8}, {**APART, "table": (1 << 24) + 65536 - 16},
+               {**APART, "table": (1 << 25) - 51200 + 16},
+               {**APART, "table": (1 << 25) - 51200 + 16, "cache_type": _lib.KVCA_TYPE_E2M1},
+               {**APART, "slot_mapping": (1 << 24) + 7 * 8192 + 15 * 512, "cache_type": _lib.KVCA_TYPE_E4M3}]
+
+
+@pytest.mark.parametrize("bad", CACHE_MEETS, ids=lambda v: ",".join(v))
+def test_caches_over_what_a_call_reads_of_its_tokens(bad):
+    assert _lib.load().kvca_append_tokens(ctypes.byref(append_desc(**bad)), None, None) == BAD
