@@ -96,10 +96,11 @@ int to_attend(const kvca_attend_desc* d, int64_t* d_status, kvca::AttendArgs* a)
   if (!e4m3 && !e2m1 && d->cache_type != d->query_type) return KVCA_ERR_BAD_ARGUMENT;
   if (d->head_dim % (e2m1 ? 32 : e4m3 ? 16 : 8) != 0) return KVCA_ERR_BAD_ARGUMENT;
   const uint64_t strides[] = {d->key, d->value, static_cast<uint64_t>(d->key_block_stride),
-                              static_cast<uint64_t>(d->key_token_stride), static_cast<uint64_t>(d->key_head_stride),
+                              static_cast<uint64_t>(d->key_token_stride),
+                              e2m1 ? 0 : static_cast<uint64_t>(d->key_head_stride),
                               static_cast<uint64_t>(d->value_block_stride),
                               static_cast<uint64_t>(d->value_token_stride),
-                              static_cast<uint64_t>(d->value_head_stride), d->query,
+                              e2m1 ? 0 : static_cast<uint64_t>(d->value_head_stride), d->query,
                               static_cast<uint64_t>(d->query_row_stride),
                               static_cast<uint64_t>(d->query_head_stride), d->out};
   for (uint64_t x : strides)
