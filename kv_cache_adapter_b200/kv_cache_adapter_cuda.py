@@ -2085,8 +2085,12 @@ def append_tokens(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tenso
     (``e2m1_row_bytes``; scales chosen per 16 dims, times ``key_scale``,
     ``value_scale``).  ``positions`` and ``table`` are ``rotate_tokens``'s;
     without them keys are stored as they are.  Returns ``query_out`` (the query
-    itself if given as such), None without a query.  No gradients: the cache
-    holds no graph."""
+    itself if given as such), None without a query.  No gradients: what the cache
+    holds has no graph, and a ``query`` that wants one is refused where gradients
+    are on (``rotate_tokens`` in an autograd function records its rotation)."""
+    if isinstance(query, torch.Tensor) and query.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("append_tokens records no gradient: call it without (torch.no_grad), or rotate the query by "
+                           "rotate_tokens in an autograd function")
     tensor, args = torch.Tensor, (key, value, key_cache, value_cache, slot_mapping, positions, table, query, query_out,
                                   key_scale, value_scale)
     if not (isinstance(key, tensor) and isinstance(value, tensor) and isinstance(key_cache, tensor)
