@@ -820,9 +820,10 @@ int kvca_attend_chunk(const kvca_attend_desc* desc, const int64_t* d_query_offse
 
 /*
  * Sets how long a wait within the kernels of later kvca_attend_chunk calls of
- * this process, and of kvca_attend_step calls over 4-bit caches, may take, in nanoseconds (2 s at first; 0: a wait whose event
- * has not come yet gives up), and returns the limit before; only returns it
- * when negative.  A graph keeps the limit of its capture.
+ * this process, and of kvca_attend_step calls over 4-bit caches, may take, in
+ * nanoseconds (2 s at first; 0: a wait whose event has not come yet gives up),
+ * and returns the limit before; only returns it when negative.  A graph keeps
+ * the limit of its capture.
  */
 int64_t kvca_attend_wait_limit(int64_t nanoseconds);
 
@@ -845,7 +846,8 @@ int64_t kvca_attend_wait_limit(int64_t nanoseconds);
  * (KVCA_ERR_BAD_ARGUMENT); no stride is negative.
  * Row r turns by positions[r]; a row of negative position is left as it was,
  * one outside the table too (KVCA_ERR_BAD_INDEX).  Addresses and strides are
- * multiples of 16 bytes, head_dim a multiple of 8, at most 256.  One launch.
+ * multiples of 16 bytes, head_dim a multiple of 8, at most 256.  At most 2^24
+ * rows, 65,536 heads and 2^31 rows of heads (KVCA_ERR_SIZE_LIMIT).  One launch.
  * No reference counterpart.
  */
 typedef struct kvca_rotate_desc {
@@ -890,8 +892,11 @@ int kvca_rotate_tokens(const kvca_rotate_desc* desc, int64_t* d_status, kvca_str
  *     the largest value.
  * Ties go to even.  Addresses and strides are multiples of 16 bytes, head_dim a
  * multiple of 8 (16 with e4m3), at most 256; no stride is negative.  query_out
- * may be the query (the same strides); nothing else that is written overlaps
- * anything (KVCA_ERR_BAD_ARGUMENT).  One launch, no host synchronisation.
+ * may be the query (the same strides), whose rows may lie between those of the
+ * keys and values (one projection's, at one row stride); nothing else that is
+ * written overlaps anything (KVCA_ERR_BAD_ARGUMENT).  At most 2^24 rows, 65,536
+ * heads of queries or of keys and 2^31 rows of heads in all
+ * (KVCA_ERR_SIZE_LIMIT).  One launch, no host synchronisation.
  */
 typedef struct kvca_append_desc {
   int64_t num_rows;
@@ -939,7 +944,8 @@ int kvca_append_tokens(const kvca_append_desc* desc, int64_t* d_status, kvca_str
  * Token rows slot_mapping[r] of a cache of 8 or 4 bits as fp16, bf16 or fp32
  * values times scale: out (num_rows, kv_heads, head_dim), dense, 16-byte
  * aligned.  Rows of negative slot are left as they were, those of a slot
- * outside the cache too (KVCA_ERR_BAD_INDEX).  One launch.
+ * outside the cache too (KVCA_ERR_BAD_INDEX).  At most 2^24 rows and 1,024 heads
+ * (KVCA_ERR_SIZE_LIMIT).  One launch.
  */
 typedef struct kvca_read_desc {
   uint64_t cache;

@@ -5,9 +5,9 @@
 Compiles csrc/kv_adapter_cuda.cu (movers and metadata), csrc/attend_*.cu
 (attention over the pages), csrc/page_ops.cu (pages of sequences),
 csrc/token_ops.cu (rows of new tokens), csrc/row_ceiling.cu (the random-row
-roofline reference) and csrc/binding.cpp (the C ABI of include/kvca.h) with nvcc into a shared library next to this file, with
-the CUDA runtime linked statically so the library has no runtime dependency
-beyond the driver.
+roofline reference) and csrc/binding.cpp (the C ABI of include/kvca.h) with
+nvcc into a shared library next to this file, with the CUDA runtime linked
+statically so the library has no runtime dependency beyond the driver.
 """
 from __future__ import annotations
 

@@ -203,7 +203,7 @@ __device__ __noinline__ int64_t block_incl_max(int64_t x, int64_t* sm) {
 // row (power_up), whose inverse goes into its score factor, with the sign or the
 // zeros of the scores' factor; by all warps of blocks 1 and on, a row on dim / 8
 // lanes.  (By the two warps that fetch queries, as with e4m3 keys, it held up every
-// segment: prompts 691 us, not 420.)
+// segment: prompts 691 us, not 433-441.)
 __device__ __forceinline__ void lift_queries(const AttendArgs& a, const ChunkArgs& c) {
   const int lanes = a.dim / 8, per_warp = 32 / lanes;
   const int lane = threadIdx.x & 31, row_of = lane / lanes, chunk = lane - row_of * lanes;
@@ -1179,7 +1179,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               cp_async4(to, from, read);
               if (off + a.dim / 16 > 4) cp_async4(to + 4, from + 4, read);
               cp_async_commit();
-              const uint32_t mark = (side == 1 && cut ? 1u : 0u) | (segment % kSlots) << 1 | static_cast<uint32_t>(off) << 2;
+              const uint32_t mark =
+                  (side == 1 && cut ? 1u : 0u) | (segment % kSlots) << 1 | static_cast<uint32_t>(off) << 2;
               marks = (marks & ~(15u << (4 * (issued & 7u)))) | mark << (4 * (issued & 7u));
               ++issued;
               if (issued - arrived > kAhead) {

@@ -28,6 +28,11 @@
 // 128): 183-188 us, of which some 27 are fixed (lengths, queries, joins; the last
 // run's wait), the rest 2.1 us per tile of 16 warps: 5.0 TB/s, issue slots 60 %,
 // ALU 51 %.  (121 us of bytes at the copy's rate; e4m3, twice the bytes, 277.)
+//
+// Where a run has a part of the heads only, a token's row takes four copies of that
+// part's codes and scales.  For the bytes of 94 us at the copy's rate (128 sequences,
+// head dim 128): 8 K/V heads 141 us, 16 149; 17 (runs of one head) 560, 32 (of 16)
+// 372, 40 (of 10) 302, where e4m3 takes 196-230 for its 167.
 
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -64,8 +69,12 @@ struct FourShape {
 };
 
 // How a call's work lies on the warps: `span` warps side by side share a run,
-// each for a head group of its own.  As many of them as there are warps for:
-// with 3 or 5 K/V heads one warp of 16 is left out.
+// each for a head group of its own: the largest divisor of the head groups that
+// there are warps for.  Warps that make no whole run are left out: of 16, one with 3
+// or 5 head groups, 4 with 6, 7 with 9, 6 with 10, 5 with 11, 4 with 12; of 8, two
+// with 3 and 3 with 5.  Whole rows make up for it (bytes of 94 us: 6 K/V heads 148 us,
+// 11 155, 12 144, against 141 with 8), at 9 (185) and 10 (166) not quite; a prime
+// above the warps gives runs of one head.
 struct FourLayout {
   int parts;   // head groups of a sequence: K/V heads x tiles of query heads
   int span;    // of them in a run
@@ -165,7 +174,8 @@ __device__ __forceinline__ uint32_t high_twice(uint32_t v) {
 
 // d = a b, with nothing before it.
 __device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+               "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }

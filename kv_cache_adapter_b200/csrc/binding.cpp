@@ -1112,7 +1112,8 @@ int kvca_rotate_tokens(const kvca_rotate_desc* d, int64_t* d_status, kvca_stream
       !rotation_ok(d->rotary_dim, d->head_dim, d->table_rows) ||
       (d->type != KVCA_TYPE_F16 && d->type != KVCA_TYPE_BF16 && d->type != KVCA_TYPE_F32))
     return KVCA_ERR_BAD_ARGUMENT;
-  const std::initializer_list<uint64_t> words = {d->x, d->out, static_cast<uint64_t>(d->row_stride), static_cast<uint64_t>(d->head_stride),
+  const std::initializer_list<uint64_t> words = {d->x, d->out, static_cast<uint64_t>(d->row_stride),
+                            static_cast<uint64_t>(d->head_stride),
                             static_cast<uint64_t>(d->out_row_stride), static_cast<uint64_t>(d->out_head_stride),
                             reinterpret_cast<uint64_t>(d->table)};
   if (!all_aligned16(words)) return KVCA_ERR_BAD_ARGUMENT;
@@ -1187,7 +1188,8 @@ int kvca_append_tokens(const kvca_append_desc* d, int64_t* d_status, kvca_stream
       !cache_slots(d->num_blocks, d->block_size, &a.num_slots, &a.block_size, &a.block_shift))
     return KVCA_ERR_SIZE_LIMIT;
   if (d->num_rows == 0) return KVCA_OK;
-  if (d->key == 0 || d->value == 0 || d->slot_mapping == nullptr || (turns && (d->table == nullptr || d->positions == nullptr)) ||
+  if (d->key == 0 || d->value == 0 || d->slot_mapping == nullptr ||
+      (turns && (d->table == nullptr || d->positions == nullptr)) ||
       (d->q_heads > 0 && (d->query == 0 || d->query_out == 0)) ||
       (a.num_slots > 0 && (d->key_cache == 0 || d->value_cache == 0)) ||
       any_negative({d->query_row_stride, d->query_head_stride, d->query_out_row_stride, d->query_out_head_stride,
@@ -1204,7 +1206,8 @@ int kvca_append_tokens(const kvca_append_desc* d, int64_t* d_status, kvca_stream
   const Extent k = extent_of(d->key, {{n, d->key_row_stride}, {d->kv_heads, d->key_head_stride}}, unit);
   const Extent v = extent_of(d->value, {{n, d->value_row_stride}, {d->kv_heads, d->value_head_stride}}, unit);
   const Extent q = extent_of(d->query, {{n, d->query_row_stride}, {d->q_heads, d->query_head_stride}}, unit);
-  const Extent q_out = extent_of(d->query_out, {{n, d->query_out_row_stride}, {d->q_heads, d->query_out_head_stride}}, unit);
+  const Extent q_out =
+      extent_of(d->query_out, {{n, d->query_out_row_stride}, {d->q_heads, d->query_out_head_stride}}, unit);
   const Extent kc = extent_of(d->key_cache, {key_dims[0], key_dims[1], key_dims[2]}, held);
   const Extent vc = extent_of(d->value_cache, {value_dims[0], value_dims[1], value_dims[2]}, held);
   if (d->q_heads > 0) {
@@ -1285,7 +1288,8 @@ int kvca_read_tokens(const kvca_read_desc* d, int64_t* d_status, kvca_stream_t s
     return KVCA_ERR_BAD_ARGUMENT;
   const bool e2m1 = d->cache_type == KVCA_TYPE_E2M1;
   if (d->head_dim % (e2m1 ? 32 : 16) != 0) return KVCA_ERR_BAD_ARGUMENT;
-  const std::initializer_list<uint64_t> words = {d->cache, static_cast<uint64_t>(d->block_stride), static_cast<uint64_t>(d->token_stride),
+  const std::initializer_list<uint64_t> words = {d->cache, static_cast<uint64_t>(d->block_stride),
+                            static_cast<uint64_t>(d->token_stride),
                             e2m1 ? 0 : static_cast<uint64_t>(d->head_stride), d->out};
   if (!all_aligned16(words)) return KVCA_ERR_BAD_ARGUMENT;
   kvca::ReadArgs a;

@@ -15,14 +15,23 @@
 // result's; neighbouring pairs (and pairs at odd distances) lie 8 dims to a lane,
 // 16 where they are stored in 4 bits: a group with its scale.
 //
-// Bytes bound the large calls: each row is read and written once, so a turn of 8
-// dims costs 32 bytes and some 20 instructions.  A warp takes up to 12 turns, two
-// loaded at a time.  16,384 tokens (32 query and 2 x 8 K/V heads of 128, bf16):
-// 67 us, 64 of bytes at the copy's rate (91 us with three turns to a warp, all loaded at once);
-// the gradient of 8,192 x 32 fp32 heads, neighbouring pairs: 47 us, 43 of bytes.
-// To 4 bits, 8,191 such tokens and their way back: 53 us, 33 of bytes; there the
-// registers bound the rows in flight (6 blocks per SM 59 us, 8 with spills 57;
-// fewer instructions per group the same).  Few tokens: the host's 8-12 us, in a replayed graph 4.
+// Bytes bound the large calls with pairs at distances of a multiple of 8 dims, and of
+// neighbouring pairs to 16 bits: each row is read and written once, so a turn of 8 dims
+// costs 32 bytes and some 20 instructions.  A warp takes up to 12 turns, two loaded at a
+// time.  16,384 tokens (32 query and 2 x 8 K/V heads of 128, bf16): 67 us, 64 of bytes
+// at the copy's rate (91 us with three turns to a warp, all loaded at once), 65 to e4m3
+// (58 of bytes); the gradient of 8,192 x 32 fp32 heads, neighbouring pairs: 47 us, 43 of
+// bytes.  To 4 bits, 8,191 such tokens and their way back: 53 us, 33 of bytes; there the
+// registers that rows in flight lie in bound it (7 blocks per SM, with 16 bytes spilled;
+// 6 blocks 59 us, 8 with more spills 57; fewer instructions per group the same).
+//
+// The other forms are far from their bytes, for their registers (90-138 neighbouring
+// pairs, 142-255 the loose mode: 8-20 warps per SM) and, in the loose mode, three loads
+// of single values per rotated one, for each head again.  us, and of bytes, for 16,384
+// tokens (to 4 bits 8,191): neighbouring pairs to e4m3 102 (58), to 4 bits 74 (28; pairs
+// of halves 40); no table, 2 x 8 heads of 128: to 16 bits 49 (21), to e4m3 74 (16), to 4
+// bits 30 (7); 84 of 112 dims, 32 heads, rotated: 121 (37); 72 of 96 dims to 4 bits: 133
+// (21).  Few tokens: the host's 8-12 us, in a replayed graph 4.
 
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -92,7 +101,7 @@ __device__ __forceinline__ float load1(const char* p) {
 
 enum TurnMode {
   kTurnHalves,  // pairs (i, i + rotary / 2) with rotary / 2 a multiple of 8 (4 bits: of 16): a lane has both sides
-  kTurnLoose,   // the same at any distance, or no rotation
+  kTurnLoose,   // the same at any distance, or no rotation (far from its bytes: above)
   kTurnPairs,   // pairs (2 i, 2 i + 1)
 };
 
@@ -200,7 +209,8 @@ struct Lane8 {
           const bool back = d >= half;
           const float sine = __ldg(angles + (back ? d : d + half));
           x[j][e] = turned(x[j][e], __ldg(angles + (back ? d - half : d)),
-                           load1<In>(p + (back ? d - half : d + half) * In::kBytes), back != a.transpose ? sine : -sine);
+                           load1<In>(p + (back ? d - half : d + half) * In::kBytes),
+                           back != a.transpose ? sine : -sine);
         }
         if (!keep_floats) raw[j].set(x[j]);
       }
@@ -369,13 +379,15 @@ __device__ __forceinline__ void token_rows(const TokenArgs& a, int64_t token, in
       float x[kParts][8];
       if (mine) {
         if (!is_value) {
-          at.template rotate<In>(a, from[b], place.angles, raw, x, !is_query && (kFour || (kStores && Cache::kBytes == 1)));
+          at.template rotate<In>(a, from[b], place.angles, raw, x,
+                                 !is_query && (kFour || (kStores && Cache::kBytes == 1)));
         } else if constexpr (kStores && Cache::kBytes < 2) {
 #pragma unroll
           for (int j = 0; j < kParts; ++j) raw[j].get(x[j]);
         }
       }
-      if constexpr (kMode == kTurnLoose) __syncwarp();  // another lane's values have been read: their place may be the result's
+      // another lane's values have been read: their place may be the result's
+      if constexpr (kMode == kTurnLoose) __syncwarp();
       if constexpr (!kStores) {
         if (!mine) continue;
         char* const to = a.query_out + token * a.query_out_row + h * a.query_out_head;
@@ -444,13 +456,14 @@ __device__ __forceinline__ void token_rows(const TokenArgs& a, int64_t token, in
 
 // Blocks per SM that the registers leave room for: bound by how many rows are on
 // their way, so 28 warps with two turns each at 72 registers beat 20 with three at
-// 96 (prompt of 16,384 tokens, 48 heads: 74 us and 77).  The other modes take what
-// they need.
+// 96 (prompt of 16,384 tokens, 48 heads: 74 us and 77, before what brought it to 67).
+// The other modes take what they need.
 template <int kMode>
 constexpr int kTokenBlocks = kMode == kTurnHalves ? 7 : 1;
 
 template <typename In, typename Cache, int kMode, bool kStores, int kBatch>
-__global__ void __launch_bounds__(32 * kTokenWarps, kTokenBlocks<kMode>) token_rows_kernel(const __grid_constant__ TokenArgs a) {
+__global__ void __launch_bounds__(32 * kTokenWarps, kTokenBlocks<kMode>)
+    token_rows_kernel(const __grid_constant__ TokenArgs a) {
   const uint32_t warp = blockIdx.x * kTokenWarps + (threadIdx.x >> 5);  // below 2^32
   const uint32_t token = warp / a.token_warps;
   const int part = static_cast<int>(warp - token * a.token_warps);
@@ -459,7 +472,8 @@ __global__ void __launch_bounds__(32 * kTokenWarps, kTokenBlocks<kMode>) token_r
     if (part < a.query_warps)
       token_rows<In, Cache, kMode, kStores, false, kBatch>(a, token, part, a.query_warps);
     else
-      token_rows<In, Cache, kMode, kStores, true, kBatch>(a, token, part - a.query_warps, a.token_warps - a.query_warps);
+      token_rows<In, Cache, kMode, kStores, true, kBatch>(a, token, part - a.query_warps,
+                                                          a.token_warps - a.query_warps);
   } else {
     token_rows<In, Cache, kMode, kStores, false, kBatch>(a, token, part, a.token_warps);
   }
@@ -467,7 +481,7 @@ __global__ void __launch_bounds__(32 * kTokenWarps, kTokenBlocks<kMode>) token_r
 
 // Turns of a warp at most, for which the token's angles are loaded once and its
 // slot and position looked up (the prompt of 16,384 tokens, 12 turns to a token:
-// one turn to a warp 150 us, 3 88, 12 74).
+// one turn to a warp 150 us, 3 88, 12 74, before what brought it to 67).
 constexpr int kTurns = 12;
 
 template <typename In, typename Cache, int kMode, bool kStores>

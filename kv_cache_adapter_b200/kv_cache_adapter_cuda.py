@@ -1589,7 +1589,8 @@ def _attend_desc(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torc
         lse_ptr = 0
     elif not isinstance(lse, tensor):
         raise TypeError("lse must be torch.Tensor")
-    elif lse.shape != qshape[:2] or lse.dtype is not torch.float32 or lse.get_device() != index or not lse.is_contiguous():
+    elif (lse.shape != qshape[:2] or lse.dtype is not torch.float32 or lse.get_device() != index
+          or not lse.is_contiguous()):
         raise ValueError(f"lse must be a contiguous {tuple(qshape[:2])} float32 tensor on {dev}")
     else:
         lse_ptr = lse.data_ptr()
@@ -2077,7 +2078,8 @@ def append_tokens(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tenso
     way, and the tokens' queries rotated (kvca_append_tokens): the step before
     ``attend_step`` or ``attend_chunk``, in one launch.  ``key`` and ``value``
     ``(rows, kv_heads, head_dim)`` and ``query`` ``(rows, heads, head_dim)`` are
-    fp16 or bf16, in any order of rows and heads (slices of one projection too).
+    fp16 or bf16, in any order of rows and heads (slices of one projection too);
+    ``query_out`` may be the query, then beside such slices but not over them.
     Row r goes to slot ``slot_mapping[r]`` (int64, block * block_size + offset,
     distinct); rows of negative slot are padding: nothing of them is written.
     The caches are those of ``attend_step``: of the rows' dtype, e4m3 (which
