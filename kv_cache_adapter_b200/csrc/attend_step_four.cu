@@ -25,7 +25,7 @@
 // runs and places of partial results this one's agree.
 //
 // 256 sequences of 500-16,384 tokens, window 4,096 (64 query heads on 8, head dim
-// 128): 183-188 us, of which some 27 are fixed (lengths, queries, joins; the last
+// 128): 174-188 us, of which some 27 are fixed (lengths, queries, joins; the last
 // run's wait), the rest 2.1 us per tile of 16 warps: 5.0 TB/s, issue slots 60 %,
 // ALU 51 %.  (121 us of bytes at the copy's rate; e4m3, twice the bytes, 277.)
 //

@@ -1058,19 +1058,21 @@ struct HeadRows {
   int64_t heads, head;
 };
 
-constexpr int64_t kMostHeadPairs = int64_t{1} << 16;
+constexpr int64_t kMostPairs = int64_t{1} << 16;
 
 // Whether rows of two tensors, `unit` bytes each, meet; strides are not negative.
-// Exact where both have the same row stride and the same head stride, or heads side
-// by side, or few of them: for two heads, rows of the one lie multiples of the row
-// stride from those of the other.  Others that interleave count as meeting.
+// At one row stride only the difference of two rows counts, at one head stride that
+// of two heads, and heads side by side are one.  What is left is looked at pair by
+// pair; above kMostPairs tensors that interleave count as meeting.
 bool rows_meet(int64_t num_rows, HeadRows a, HeadRows b, int64_t unit) {
   using wide = __int128;
   if (!meet(extent_of(a.address, {{num_rows, a.row}, {a.heads, a.head}}, unit),
             extent_of(b.address, {{num_rows, b.row}, {b.heads, b.head}}, unit)))
     return false;
   if (num_rows == 1) a.row = b.row = 0;
-  if (a.row != b.row) return true;
+  // rows of b to look at, and the least and most rows from each to one of a
+  const int64_t b_rows = a.row == b.row || b.row == 0 ? 1 : num_rows;
+  const wide least_rows = 1 - num_rows, most_rows = a.row == b.row ? num_rows - 1 : 0;
   int64_t a_unit = unit, b_unit = unit;
   const auto join = [unit](HeadRows* t, int64_t* whole) {  // heads that lie side by side
     if (t->head > unit && t->heads > 1) return;
@@ -1080,20 +1082,22 @@ bool rows_meet(int64_t num_rows, HeadRows a, HeadRows b, int64_t unit) {
   join(&a, &a_unit);
   join(&b, &b_unit);
   const bool alike = a.heads > 1 && b.heads > 1 && a.head == b.head;  // only differences of heads count
-  if (!alike && a.heads * b.heads > kMostHeadPairs) return true;
   const int64_t pairs = alike ? a.heads + b.heads - 1 : a.heads * b.heads;
-  for (int64_t p = 0; p < pairs; ++p) {
+  if (pairs > kMostPairs / b_rows) return true;
+  for (int64_t i = 0; i < pairs * b_rows; ++i) {
+    const int64_t p = i / b_rows;
     wide d = static_cast<wide>(b.address) - static_cast<wide>(a.address);
     if (alike)
       d += static_cast<wide>(p - (a.heads - 1)) * a.head;
     else
       d += static_cast<wide>(p % b.heads) * b.head - static_cast<wide>(p / b.heads) * a.head;
-    // the first of b's rows, from the first that any of a's may have beside it, to end behind a's begin
+    d += static_cast<wide>(i % b_rows) * b.row;
+    // the nearest of a's rows that begins before b's ends
     if (a.row > 0) {
-      const wide least = 1 - b_unit - d, most = num_rows - 1;
+      const wide least = 1 - b_unit - d;
       wide rows = least / a.row + (least > 0 && least % a.row != 0 ? 1 : 0);
-      if (rows < -most) rows = -most;
-      if (rows > most) continue;
+      if (rows < least_rows) rows = least_rows;
+      if (rows > most_rows) continue;
       d += rows * a.row;
     }
     if (d < a_unit && d + b_unit > 0) return true;

@@ -1846,36 +1846,39 @@ def _result_rows(out: torch.Tensor, x: torch.Tensor, at: tuple[int, int, int, in
 
 def _rows_meet(rows: int, a: tuple[int, int, int, int], b: tuple[int, int, int, int], unit: int) -> bool:
     """Whether rows of two tensors (address, row stride, heads, head stride), `unit`
-    bytes each, meet, as the C interface finds it: exact where the strides are the
-    same, or heads lie side by side."""
+    bytes each, meet, as the C interface finds it: where more than 2^16 pairs of
+    heads and rows would have to be looked at, they do if their ranges do."""
     if not rows:
         return False
     ends = [t[0] + (rows - 1) * t[1] + (t[2] - 1) * t[3] + unit for t in (a, b)]
     if a[0] >= ends[1] or b[0] >= ends[0]:
         return False
-    row = a[1] if rows > 1 else 0
-    if rows > 1 and b[1] != row:
-        return True
+    row, other_row = (a[1], b[1]) if rows > 1 else (0, 0)
+    # rows of b to look at, and the most rows from each to one of a
+    other_rows = 1 if row == other_row or other_row == 0 else rows
+    most = rows - 1 if row == other_row else 0
     spans = []
     for address, _, heads, head in (a, b):  # heads that lie side by side are one
         joined = head <= unit or heads == 1
         spans.append((address, 1 if joined else heads, head, (heads - 1) * head + unit if joined else unit))
     (at, heads, head, size), (other, other_heads, other_head, other_size) = spans
-    if heads > 1 and other_heads > 1 and head == other_head:  # only differences of heads count
-        shifts = [h * head for h in range(1 - heads, other_heads)]
-    elif heads * other_heads > 1 << 16:
+    alike = heads > 1 and other_heads > 1 and head == other_head  # only differences of heads count
+    if (heads + other_heads - 1 if alike else heads * other_heads) > (1 << 16) // other_rows:
         return True
+    if alike:
+        shifts = [h * head for h in range(1 - heads, other_heads)]
     else:
         shifts = [h * other_head - g * head for g in range(heads) for h in range(other_heads)]
     for shift in shifts:
-        d = other - at + shift
-        if row:  # the first of b's rows that ends behind a's begin
-            n = max(-((other_size - 1 + d) // row), 1 - rows)
-            if n >= rows:
-                continue
-            d += n * row
-        if -other_size < d < size:
-            return True
+        for r in range(other_rows):
+            d = other - at + shift + r * other_row
+            if row:  # the nearest of a's rows that begins before b's ends
+                n = max(-((other_size - 1 + d) // row), 1 - rows)
+                if n > most:
+                    continue
+                d += n * row
+            if -other_size < d < size:
+                return True
     return False
 
 

@@ -67,3 +67,19 @@ def test_what_meets_is_named(ops, dev):
         with pytest.raises(ValueError, match="caches must not overlap slot_mapping"):
             ops.append_tokens(rows, rows, kc, vc, slots, positions=positions, table=turns)
     assert not kc.any() and not vc.any()
+
+
+def test_keys_of_one_row_for_all(ops, dev):
+    x = rows_of((9, 12, 64), BF16, 8)
+    live = x.to(dev)
+    kc, vc = (torch.zeros((4, 16, 2, 64), dtype=BF16, device=dev) for _ in range(2))
+    at, table = places(9, 60, 9), ops.rotary_table(60, 64)
+    key = live[3:4, 8:10].expand(9, 2, 64)
+    ops.append_tokens(key, live[:, 10:], kc, vc, torch.arange(9, device=dev), positions=at.to(dev),
+                      table=table.to(dev), query=live[:, :8], query_out=live[:, :8], check=True)
+    for have, rotated in ((live[:, :8], x[:, :8]), (kc.flatten(0, 1)[:9], x[3:4, 8:10].expand(9, 2, 64))):
+        want, bound = oracle.rotate(rotated, at, table)
+        oracle.check_rows(have.cpu(), want, bound, BF16)
+    with pytest.raises(ValueError, match="query_out must not overlap key or value"):
+        ops.append_tokens(live[3:4, 7:9].expand(9, 2, 64), live[:, 10:], kc, vc, torch.arange(9, device=dev),
+                          positions=at.to(dev), table=table.to(dev), query=live[:, :8], query_out=live[:, :8])
